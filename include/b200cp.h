@@ -3,7 +3,7 @@
  * Plain C: pointers, sizes, an opaque stream handle.  Every pointer named
  * "device" must be device memory of the current CUDA device; the *_host entry
  * points take ordinary host memory and do the transfers themselves.  All
- * tensors are fp32, row-major, last index fastest:
+ * tensors are fp32 (where no type is named), row-major, last index fastest:
  *
  *   X  [N, C, H, W]   U, dU [N, T, H, W]
  *   K0 [T, R]  K1 [C, R]  KH [Y, R]  KW [X, R]      (the reference's FT, FC, FY, FX)
@@ -365,6 +365,43 @@ int b200cp_cp4_step_allreduce_pipelined(void* p2p_ctx, const b200cp_tensor_shape
                                         float* dX, float* dK_scratch, float* dK_prev, void* workspace,
                                         size_t workspace_bytes, void* stream, int flags);
 int b200cp_p2p_flush(void* ctx, float* dK_last, void* stream);
+
+/* Types of the operators below that take more than fp32. */
+enum { B200CP_FLOAT32 = 0, B200CP_BFLOAT16 = 1, B200CP_FLOAT16 = 2 };
+
+/* ---- AdamW step ------------------------------------------------------------ */
+
+/* One tensor of a step, n values (0: skipped).  The moments are float[n], or codes of 8 bits (exp_avg int8, exp_avg_sq uint8) with a
+ * float per block of 256 values in scale_avg / scale_sq: m = s (c / 127)^2 with c's sign (-128: not finite), v = s (c / 254)^4
+ * (255: not finite).  All zero is the state of a first step.  master: the fp32 copy of a 16-bit parameter, or NULL. */
+typedef struct b200cp_adamw_tensor {
+  void* param;
+  const void* grad;
+  void *exp_avg, *exp_avg_sq;
+  float *scale_avg, *scale_sq;
+  float* master;
+  unsigned long long n;
+} b200cp_adamw_tensor;
+
+/* step counts from one.  device_step (or NULL): the step as an int64 in device memory, read by the launch, instead of `step`;
+ * device_lr (or NULL): lr as a float in device memory.  A captured step takes both from there at each replay. */
+typedef struct b200cp_adamw {
+  double lr, beta1, beta2, eps, weight_decay;
+  long long step;
+  const long long* device_step;
+  const float* device_lr;
+} b200cp_adamw;
+
+/* m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p - lr wd p - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps) for all tensors
+ * (one launch per 448), in place, in fp32 arithmetic.  param_type: of param; grad_type: that type, or float.  moment_bits: 32 or 8.
+ * No two entries may overlap.  Replaces the optimiser step after the reference's gradients, which its layers leave to
+ * TensorFlow (test/layers.py has no optimiser of its own). */
+int b200cp_adamw_step(const b200cp_adamw_tensor* tensors, int count, int param_type, int grad_type, int moment_bits,
+                      const b200cp_adamw* hyper, void* stream);
+
+/* The values that 8-bit moments stand for, as out_type. */
+int b200cp_adamw_moments(unsigned long long n, const void* exp_avg, const void* exp_avg_sq, const float* scale_avg,
+                         const float* scale_sq, int out_type, void* m, void* v, void* stream);
 
 /* ---- misc --------------------------------------------------------------- */
 

@@ -21,6 +21,10 @@ class TensorShape(C.Structure):
     _fields_ = [(k, C.c_uint) for k in ("N", "H", "W", "pad", "T", "C", "Y", "X", "Rank")]
 
 
+# types of the operators that take more than float32 (include/b200cp.h)
+FLOAT32, BFLOAT16, FLOAT16 = 0, 1, 2
+
+
 class B200CPError(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(f"b200cp status {status}: {msg}")
@@ -97,6 +101,8 @@ def _load():
         "b200cp_dense_matmul": (i, [i, i, i, fp, fp, fp, vp, sz, vp]),
         "b200cp_dense_bwd_workspace_bytes": (sz, [i, i, ip, ip, i, i]),
         "b200cp_dense_bwd": (i, [i, i, ip, ip, i, fp, fp, pp, fp, pp, vp, sz, vp, i]),
+        "b200cp_adamw_step": (i, [vp, i, i, i, i, vp, vp]),
+        "b200cp_adamw_moments": (i, [C.c_ulonglong, vp, vp, fp, fp, i, vp, vp, vp]),
         "b200cp_device_status": (i, []),
         "b200cp_last_error_string": (C.c_char_p, []),
         "b200cp_status_string": (C.c_char_p, [i]),

@@ -83,8 +83,7 @@ def build(force=False, verbose=False):
 
 def _build_binding(force):
     src = os.path.join(CSRC, "torch_binding.cpp")
-    hdr = os.path.join(ROOT, "include", "b200cp.h")
-    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) > max(os.path.getmtime(src), os.path.getmtime(hdr)):
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) > _newest_source(src):
         return
     import sysconfig
 

@@ -1,0 +1,380 @@
+// AdamW over many tensors in one launch, moments in 32 or in 8 bits.
+//
+//   m <- b1 m + (1 - b1) g      v <- b2 v + (1 - b2) g^2      p <- p - lr wd p - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+//
+// A tensor is cut into pieces of kPiece values, a CTA takes one piece of one tensor; the table of tensors is a kernel parameter (so that a
+// captured launch carries it, and nothing is copied), and a CTA finds its tensor by bisection over the pieces' sums.
+//
+// Moments in 8 bits: blocks of 256 values, which are those of a warp, with the largest magnitude s of each.  |m| = s (c / 127)^2 and
+// v = s (c / 254)^4: the codes' steps are relative ones over most of the range, v reaches down to 2.4e-10 s and m to 6e-5 s, which is its
+// square root and four times more.  So where a value's v is rounded to nothing, its m has been; a v above zero has a code of one at least all
+// the same, and no m is ever divided by eps alone.  A value that is not finite keeps a code of its own (-128; 255) and reads as NaN, so it costs
+// the other 255 nothing.  The parameter is updated with the moments before they are rounded.  All arithmetic is fp32, the roundings of the
+// moments those of separate products and sums; to fewer bits are rounded the codes (half a step: 0.8 % of the largest values) and a 16-bit
+// parameter, whose fp32 copy (master) is what is updated where there is one.
+//
+// Bound by HBM: 28 bytes a value (p, m, v read and written, g read), 16.06 with 8-bit moments.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+
+namespace b200cp {
+namespace {
+
+constexpr int kThreads = 256, kPiece = 2048, kBlock = 256;   // a warp has 256 values: two groups of four per lane
+constexpr int kFew = 48, kMany = 448;                        // tensors of a launch: tables of 3.5 and 31 KB (32 764 bytes are the most)
+
+struct Entry {
+  void* p;
+  const void* g;
+  void *m, *v;
+  float *ms, *vs, *w;
+  long long n;
+};
+struct Rates {
+  float b1, b2, c1, c2;        // c = 1 - b
+  float decay, eps;            // lr wd
+  float step, root;            // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  const long long* t;          // on the device: step and root are formed by the kernel
+  const float* lr;
+  double lr_, wd, b1_, b2_;    // then from these
+};
+template <int CAP>
+struct Table {
+  Rates r;
+  int count;
+  int first[CAP + 1];          // pieces before each tensor
+  Entry e[CAP];
+};
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) { return (float)v; }
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, long long i, long long n, bool vec, float (&x)[4]) {
+  if (vec && i + 4 <= n) {
+    const Four<T> q = *reinterpret_cast<const Four<T>*>(p + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = (float)q.v[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = i + k < n ? (float)p[i + k] : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, long long i, long long n, bool vec, const float (&x)[4]) {
+  if (vec && i + 4 <= n) {
+    Four<T> q;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q.v[k] = (T)x[k];
+    *reinterpret_cast<Four<T>*>(p + i) = q;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < n) p[i + k] = (T)x[k];
+  }
+}
+template <typename T>
+__device__ __forceinline__ bool aligned4(const T* p) { return !(reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)); }
+
+// Within 2^-22 of the root and of the quotient: enough for a step, and for a code that is not next to a border.
+__device__ __forceinline__ float fast_sqrt(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_sqrt_ftz(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_div(float x, float y) {
+  float q;
+  asm("div.approx.f32 %0, %1, %2;" : "=f"(q) : "f"(x), "f"(y));
+  return q;
+}
+__device__ __forceinline__ float of_m(float c, float s) {
+  const float q = c * (1.f / 127);
+  return c == -128.f ? __int_as_float(0x7fffffff) : q * fabsf(q) * s;
+}
+__device__ __forceinline__ float of_v(float c, float s) {
+  const float q = c * (1.f / 254), r = q * q;
+  return c == 255.f ? __int_as_float(0x7fffffff) : r * r * s;
+}
+// The code is that of 127 sqrt(|x| / s) with every operation rounded to nearest: found by the fast operations, and again by the exact
+// ones where those end within 2e-4 of a border (their error is below 5e-5 of a step), one value in 2500.  Exact codes do not depend
+// on how an operation is approximated: two implementations that round alike hold the same state.
+__device__ __noinline__ float exact_code(float x, float s, float steps) {
+  const float q = sqrtf(__fdiv_rn(fabsf(x), s));
+  return rintf(steps * (steps > 200.f ? sqrtf(q) : q));
+}
+__device__ __forceinline__ float code_m(float x, float s, float inverse) {
+  if (!(fabsf(x) < __int_as_float(0x7f800000))) return -128.f;
+  const float t = 127.f * fast_sqrt_ftz(fabsf(x) * inverse);
+  float c = rintf(t);
+  if (fabsf(t - c) > 0.4998f || inverse == 0.f) c = s > 0.f ? exact_code(x, s, 127.f) : 0.f;
+  return copysignf(c, x);
+}
+__device__ __forceinline__ float code_v(float x, float s, float inverse) {
+  if (!(x < __int_as_float(0x7f800000))) return 255.f;
+  const float t = 254.f * fast_sqrt_ftz(fast_sqrt_ftz(x * inverse));
+  float c = rintf(t);
+  if (fabsf(t - c) > 0.4998f || inverse == 0.f) c = s > 0.f ? exact_code(x, s, 254.f) : 0.f;
+  return x > 0.f ? fmaxf(c, 1.f) : 0.f;
+}
+__device__ __forceinline__ float finite_magnitude(float x) { return fabsf(x) < __int_as_float(0x7f800000) ? fabsf(x) : 0.f; }
+__device__ __forceinline__ float warp_max(float x) {   // of magnitudes
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x)));
+}
+// 1 / s, or 0 where s or that is no normal number (then every code of the block is found by the exact operations)
+__device__ __forceinline__ float inverse_of(float s) { return s > 1e-37f && s < 1e37f ? 1.f / s : 0.f; }
+
+template <typename P, typename G, bool SMALL, int CAP>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<CAP> t) {
+  int a = 0, b = t.count;   // the tensor whose pieces hold this CTA's
+  while (b - a > 1) {
+    const int c = (a + b) / 2;
+    if (t.first[c] <= (int)blockIdx.x) a = c; else b = c;
+  }
+  const Entry& e = t.e[a];
+  const long long n = e.n, base = (long long)((int)blockIdx.x - t.first[a]) * kPiece + (threadIdx.x >> 5) * kBlock;
+  float step = t.r.step, root = t.r.root, decay = t.r.decay;
+  if (t.r.t || t.r.lr) {
+    __shared__ float rates[3];
+    if (threadIdx.x == 0) {
+      const double lr = t.r.lr ? (double)*t.r.lr : t.r.lr_;
+      double s = t.r.step, q = t.r.root;   // (of lr = 1, where lr is on the device)
+      if (t.r.t) {
+        const double at = (double)*t.r.t;
+        s = 1.0 / (1.0 - pow(t.r.b1_, at));
+        q = 1.0 / sqrt(1.0 - pow(t.r.b2_, at));
+      }
+      rates[0] = (float)(lr * s);
+      rates[1] = (float)q;
+      rates[2] = (float)(lr * t.r.wd);
+    }
+    __syncthreads();
+    step = rates[0];
+    root = rates[1];
+    decay = rates[2];
+  }
+  if (base >= n) return;
+  const int lane = threadIdx.x & 31;
+  P* p = static_cast<P*>(e.p);
+  const G* g = static_cast<const G*>(e.g);
+  float *w = e.w, ms = 0.f, vs = 0.f;
+  const long long block = base / kBlock;
+  const bool vp = aligned4(p), vg = aligned4(g), vw = aligned4(w);
+  float x[2][4], d[2][4], m[2][4], v[2][4];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const long long i = base + j * 128 + lane * 4;
+    if (w) load4(w, i, n, vw, x[j]); else load4(p, i, n, vp, x[j]);
+    load4(g, i, n, vg, d[j]);
+  }
+  if constexpr (SMALL) {
+    const int8_t* cm = static_cast<const int8_t*>(e.m);
+    const uint8_t* cv = static_cast<const uint8_t*>(e.v);
+    const bool vm = aligned4(cm), vv = aligned4(cv);
+    ms = e.ms[block];
+    vs = e.vs[block];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const long long i = base + j * 128 + lane * 4;
+      load4(cm, i, n, vm, m[j]);
+      load4(cv, i, n, vv, v[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        m[j][k] = of_m(m[j][k], ms);
+        v[j][k] = of_v(v[j][k], vs);
+      }
+    }
+  } else {
+    const float *fm = static_cast<const float*>(e.m), *fv = static_cast<const float*>(e.v);
+    const bool vm = aligned4(fm), vv = aligned4(fv);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const long long i = base + j * 128 + lane * 4;
+      load4(fm, i, n, vm, m[j]);
+      load4(fv, i, n, vv, v[j]);
+    }
+  }
+  float mm = 0.f, mv = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      m[j][k] = fmaf(t.r.c1, d[j][k], __fmul_rn(t.r.b1, m[j][k]));
+      v[j][k] = fmaf(t.r.c2, __fmul_rn(d[j][k], d[j][k]), __fmul_rn(t.r.b2, v[j][k]));
+      x[j][k] = fmaf(-step, fast_div(m[j][k], fmaf(fast_sqrt(v[j][k]), root, t.r.eps)), fmaf(-decay, x[j][k], x[j][k]));
+      if (SMALL) {   // (values past the end are zero: they change no maximum)
+        mm = fmaxf(mm, finite_magnitude(m[j][k]));
+        mv = fmaxf(mv, finite_magnitude(v[j][k]));
+      }
+    }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const long long i = base + j * 128 + lane * 4;
+    if (w) store4(w, i, n, vw, x[j]);
+    store4(p, i, n, vp, x[j]);
+  }
+  if constexpr (SMALL) {
+    int8_t* cm = static_cast<int8_t*>(e.m);
+    uint8_t* cv = static_cast<uint8_t*>(e.v);
+    mm = warp_max(mm);
+    mv = warp_max(mv);
+    const float im = inverse_of(mm), iv = inverse_of(mv);
+    if (lane == 0) {
+      e.ms[block] = mm;
+      e.vs[block] = mv;
+    }
+    const bool vm = aligned4(cm), vv = aligned4(cv);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const long long i = base + j * 128 + lane * 4;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        m[j][k] = code_m(m[j][k], mm, im);
+        v[j][k] = code_v(v[j][k], mv, iv);
+      }
+      store4(cm, i, n, vm, m[j]);
+      store4(cv, i, n, vv, v[j]);
+    }
+  } else {
+    float *fm = static_cast<float*>(e.m), *fv = static_cast<float*>(e.v);
+    const bool vm = aligned4(fm), vv = aligned4(fv);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const long long i = base + j * 128 + lane * 4;
+      store4(fm, i, n, vm, m[j]);
+      store4(fv, i, n, vv, v[j]);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) moments_kernel(long long n, const int8_t* cm, const uint8_t* cv, const float* ms, const float* vs,
+                                                           T* m, T* v) {
+  const long long i = ((long long)blockIdx.x * kThreads + threadIdx.x) * 4;
+  if (i >= n) return;
+  const float a = ms[i / kBlock], b = vs[i / kBlock];
+  float x[4], y[4];
+  load4(cm, i, n, aligned4(cm), x);
+  load4(cv, i, n, aligned4(cv), y);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[k] = of_m(x[k], a);
+    y[k] = of_v(y[k], b);
+  }
+  store4(m, i, n, aligned4(m), x);
+  store4(v, i, n, aligned4(v), y);
+}
+
+template <typename P, typename G, bool SMALL, int CAP>
+int launch_some(const b200cp_adamw_tensor* ts, int count, const Rates& r, cudaStream_t st) {
+  Table<CAP> t;
+  t.r = r;
+  int at = 0;
+  while (at < count) {   // tables of up to CAP tensors and 2^30 pieces
+    long long pieces = 0;
+    t.count = 0;
+    for (; at < count && t.count < CAP; ++at) {
+      const b200cp_adamw_tensor& s = ts[at];
+      if (s.n == 0) continue;
+      const long long mine = (long long)((s.n + kPiece - 1) / kPiece);
+      if (pieces + mine > 0x3fffffff) {
+        if (t.count == 0) return fail(B200CP_ERR_UNSUPPORTED, "b200cp_adamw_step: a tensor of %llu values", s.n);
+        break;
+      }
+      t.first[t.count] = (int)pieces;
+      t.e[t.count++] = Entry{s.param, s.grad, s.exp_avg, s.exp_avg_sq, s.scale_avg, s.scale_sq, s.master, (long long)s.n};
+      pieces += mine;
+    }
+    if (t.count == 0) break;
+    t.first[t.count] = (int)pieces;
+    adamw_kernel<P, G, SMALL, CAP><<<(unsigned)pieces, kThreads, 0, st>>>(t);
+    B200CP_LAUNCH_OK("adamw_kernel");
+  }
+  return B200CP_OK;
+}
+template <typename P, typename G, bool SMALL>
+int launch_all(const b200cp_adamw_tensor* ts, int count, const Rates& r, cudaStream_t st) {
+  return count <= kFew ? launch_some<P, G, SMALL, kFew>(ts, count, r, st) : launch_some<P, G, SMALL, kMany>(ts, count, r, st);
+}
+template <typename P, typename G>
+int launch_bits(const b200cp_adamw_tensor* ts, int count, int bits, const Rates& r, cudaStream_t st) {
+  return bits == 8 ? launch_all<P, G, true>(ts, count, r, st) : launch_all<P, G, false>(ts, count, r, st);
+}
+
+}  // namespace
+}  // namespace b200cp
+
+using namespace b200cp;
+
+extern "C" {
+
+int b200cp_adamw_step(const b200cp_adamw_tensor* tensors, int count, int param_type, int grad_type, int moment_bits,
+                      const b200cp_adamw* h, void* stream) {
+  if (count < 0 || (count && !tensors) || !h) return fail(B200CP_ERR_INVALID_ARG, "b200cp_adamw_step: null argument or negative count");
+  if (moment_bits != 8 && moment_bits != 32) return fail(B200CP_ERR_INVALID_ARG, "b200cp_adamw_step: moments of %d bits", moment_bits);
+  if (!(h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1 && h->eps >= 0))
+    return fail(B200CP_ERR_INVALID_ARG, "b200cp_adamw_step: betas %g, %g or eps %g out of range", h->beta1, h->beta2, h->eps);
+  if (!h->device_step && h->step < 1) return fail(B200CP_ERR_INVALID_ARG, "b200cp_adamw_step: step %lld (they count from one)", h->step);
+  for (int i = 0; i < count; ++i) {
+    const b200cp_adamw_tensor& s = tensors[i];
+    if (s.n && (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || (moment_bits == 8 && (!s.scale_avg || !s.scale_sq))))
+      return fail(B200CP_ERR_INVALID_ARG, "b200cp_adamw_step: null pointer in tensor %d", i);
+    if (s.n && s.master && param_type == B200CP_FLOAT32)
+      return fail(B200CP_ERR_INVALID_ARG, "b200cp_adamw_step: a float32 parameter has no float32 copy (tensor %d)", i);
+  }
+  Rates r{};
+  r.b1 = (float)h->beta1; r.b2 = (float)h->beta2; r.c1 = (float)(1 - h->beta1); r.c2 = (float)(1 - h->beta2);
+  r.eps = (float)h->eps;
+  r.decay = (float)(h->lr * h->weight_decay);
+  r.t = h->device_step; r.lr = h->device_lr;
+  r.lr_ = h->lr; r.wd = h->weight_decay; r.b1_ = h->beta1; r.b2_ = h->beta2;
+  if (!h->device_step) {
+    r.step = (float)((h->device_lr ? 1.0 : h->lr) / (1 - std::pow(h->beta1, (double)h->step)));
+    r.root = (float)(1 / std::sqrt(1 - std::pow(h->beta2, (double)h->step)));
+  }
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define TYPES(P, G) return launch_bits<P, G>(tensors, count, moment_bits, r, st)
+  if (param_type == B200CP_FLOAT32 && grad_type == B200CP_FLOAT32) TYPES(float, float);
+  if (param_type == B200CP_BFLOAT16 && grad_type == B200CP_BFLOAT16) TYPES(__nv_bfloat16, __nv_bfloat16);
+  if (param_type == B200CP_FLOAT16 && grad_type == B200CP_FLOAT16) TYPES(__half, __half);
+  if (param_type == B200CP_BFLOAT16 && grad_type == B200CP_FLOAT32) TYPES(__nv_bfloat16, float);
+  if (param_type == B200CP_FLOAT16 && grad_type == B200CP_FLOAT32) TYPES(__half, float);
+#undef TYPES
+  return fail(B200CP_ERR_UNSUPPORTED, "b200cp_adamw_step: parameters of type %d with gradients of type %d", param_type, grad_type);
+}
+
+int b200cp_adamw_moments(unsigned long long n, const void* exp_avg, const void* exp_avg_sq, const float* scale_avg, const float* scale_sq,
+                         int out_type, void* m, void* v, void* stream) {
+  if (n == 0) return B200CP_OK;
+  if (!exp_avg || !exp_avg_sq || !scale_avg || !scale_sq || !m || !v)
+    return fail(B200CP_ERR_INVALID_ARG, "b200cp_adamw_moments: null pointer");
+  const unsigned long long ctas = (n + 4 * kThreads - 1) / (4 * kThreads);
+  if (ctas > 0x7fffffffull) return fail(B200CP_ERR_UNSUPPORTED, "b200cp_adamw_moments: %llu values", n);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const auto go = [&](auto* out_m, auto* out_v) {
+    moments_kernel<<<(unsigned)ctas, kThreads, 0, st>>>((long long)n, static_cast<const int8_t*>(exp_avg), static_cast<const uint8_t*>(exp_avg_sq),
+                                                        scale_avg, scale_sq, out_m, out_v);
+    B200CP_LAUNCH_OK("moments_kernel");
+    return (int)B200CP_OK;
+  };
+  switch (out_type) {
+    case B200CP_FLOAT32: return go(static_cast<float*>(m), static_cast<float*>(v));
+    case B200CP_BFLOAT16: return go(static_cast<__nv_bfloat16*>(m), static_cast<__nv_bfloat16*>(v));
+    case B200CP_FLOAT16: return go(static_cast<__half*>(m), static_cast<__half*>(v));
+  }
+  return fail(B200CP_ERR_INVALID_ARG, "b200cp_adamw_moments: type %d", out_type);
+}
+
+}  // extern "C"

@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <array>
 #include <string>
 #include <vector>
@@ -830,12 +831,15 @@ PyObject* py_set_error_class(PyObject*, PyObject* cls) {
   Py_RETURN_NONE;
 }
 
+#include "torch_operators.hpp"   // the operators beside the factored layers, which take more types than float32
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FAST(cp4_forward), FAST(cp4_forward_save), FAST(cp4_backward_data), FAST(cp4_backward_data_save),
                            FAST(cp4_forward_backward_data), FAST(cp4_backward_filter), FAST(cp4_backward_filter_saved),
                            FAST(cp4_step), FAST(cp3_forward), FAST(cp3_backward_data), FAST(cp3_backward_filter),
                            FAST(rcp_forward), FAST(rcp_backward), FAST(dense_forward), FAST(dense_backward),
                            FAST(cp4_apply), FAST(cp3_apply), FAST(rcp_apply), FAST(dense_apply),
+                           FAST(adamw_step), FAST(adamw_moments),
                            {"set_error_class", py_set_error_class, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_C", "native operator bindings", -1, g_methods, nullptr, nullptr, nullptr,

@@ -393,6 +393,26 @@ def dense_cp_rebuild(U, *kernels):
     return dense_matmul(U, dense_cp_recompose(*kernels))
 
 
+# ---- AdamW step -----------------------------------------------------------------
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, master=None, scales=None):
+    """One AdamW step over all tensors of the lists, in place and in one launch (``b200cp_adamw_step``):
+    ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g**2``, ``p -= lr wd p + lr (m / (1 - b1**t)) / (sqrt(v / (1 - b2**t)) + eps)``.
+
+    ``params``: contiguous tensors of one type on one device; ``grads`` of that type or float32.  Moments: float32 of the parameters'
+    sizes, or, with ``scales = (list, list)``, int8 and uint8 codes with a float32 scale per 256 values (all zero before the first step).
+    ``master``: the float32 copies of 16-bit parameters; then they are what is updated, and the parameters are their roundings.
+    ``step`` counts from one; it may be one int64 in a CUDA tensor, and ``lr`` one float32 in one, which a captured step reads at each replay."""
+    ms, vs = scales if scales is not None else (None, None)
+    _C.adamw_step(params, grads, exp_avg, exp_avg_sq, ms, vs, master, step, lr, betas[0], betas[1], eps, weight_decay)
+
+
+def adamw_moments(exp_avg, exp_avg_sq, scales, dtype=torch.bfloat16):
+    """The two moments that the 8-bit codes of a tensor stand for, as ``dtype``."""
+    m, v = torch.empty_like(exp_avg, dtype=dtype), torch.empty_like(exp_avg_sq, dtype=dtype)
+    _C.adamw_moments(exp_avg, exp_avg_sq, scales[0], scales[1], m, v)
+    return m, v
+
+
 # ---- autograd wrappers ----------------------------------------------------------
 # The nodes are native (csrc/torch_binding.cpp); each class keeps the ``apply`` its layer calls.
 class CP4Conv2dFunction:
