@@ -403,6 +403,30 @@ int b200cp_adamw_step(const b200cp_adamw_tensor* tensors, int count, int param_t
 int b200cp_adamw_moments(unsigned long long n, const void* exp_avg, const void* exp_avg_sq, const float* scale_avg,
                          const float* scale_sq, int out_type, void* m, void* v, void* stream);
 
+/* ---- low-rank adapters of many requests beside a shared projection ------------------------------------------- */
+
+/* Rows in the order of their adapters, made once for a batch and used by every layer that the batch meets.  adapters[rows] (device):
+ * the adapter of each row, 0 .. count - 1; any other number: none.  plan: b200cp_adapter_plan_bytes() of device memory, 16-byte
+ * aligned; it depends on rows, count and adapters only.  count is at most 16384. */
+size_t b200cp_adapter_plan_bytes(int rows, int count);
+int b200cp_adapter_plan(int rows, int count, const int* adapters, void* plan, size_t plan_bytes, void* stream);
+
+/* out[s] = Y[s] + scale[a] (X[s] A[a]) B[a] with a the adapter of row s; rows without one: out[s] = Y[s].
+ * X [rows, I], Y, out [rows, O], A [count, I, R], B [count, R, O] of one type (B200CP_FLOAT32, _BFLOAT16, _FLOAT16), R at most 128;
+ * scale [count] floats, or NULL for ones.  out may be Y.  V (or NULL): [rows, R] of the same type, receives scale X A for the backward
+ * (rows without an adapter are left as they are).  Stands beside b200cp_dense_fwd, whose Y it takes (a serving batch of
+ * test/test_dense_cp.py:41 with one correction per request); the reference has no adapters. */
+int b200cp_dense_adapters(int rows, int I, int O, int R, int count, int type, const void* Y, const void* X, const void* A, const void* B,
+                          const float* scale, const void* plan, void* out, void* V, void* stream);
+
+/* Gradients: dX[s] = scale (dY[s] B^T) A^T (zero for rows without an adapter), dA[a] = sum_s X[s]^T scale (dY[s] B^T),
+ * dB[a] = sum_s V[s]^T dY[s] (zero for adapters without rows); dY itself is Y's gradient.  dX, dA and dB may each be NULL.  The sums have a
+ * fixed order.  The workspace is 16-byte aligned. */
+size_t b200cp_dense_adapters_bwd_workspace_bytes(int rows, int I, int O, int R, int count, int type);
+int b200cp_dense_adapters_bwd(int rows, int I, int O, int R, int count, int type, const void* dY, const void* X, const void* V,
+                              const void* A, const void* B, const float* scale, const void* plan, void* dX, void* dA, void* dB,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- misc --------------------------------------------------------------- */
 
 /* Synchronises the device and reports whether any tensor-path kernel gave up a bounded wait since

@@ -101,6 +101,11 @@ def _load():
         "b200cp_dense_matmul": (i, [i, i, i, fp, fp, fp, vp, sz, vp]),
         "b200cp_dense_bwd_workspace_bytes": (sz, [i, i, ip, ip, i, i]),
         "b200cp_dense_bwd": (i, [i, i, ip, ip, i, fp, fp, pp, fp, pp, vp, sz, vp, i]),
+        "b200cp_adapter_plan_bytes": (sz, [i, i]),
+        "b200cp_adapter_plan": (i, [i, i, vp, vp, sz, vp]),
+        "b200cp_dense_adapters": (i, [i, i, i, i, i, i, vp, vp, vp, vp, fp, vp, vp, vp, vp]),
+        "b200cp_dense_adapters_bwd_workspace_bytes": (sz, [i, i, i, i, i, i]),
+        "b200cp_dense_adapters_bwd": (i, [i, i, i, i, i, i, vp, vp, vp, vp, vp, fp, vp, vp, vp, vp, vp, sz, vp]),
         "b200cp_adamw_step": (i, [vp, i, i, i, i, vp, vp]),
         "b200cp_adamw_moments": (i, [C.c_ulonglong, vp, vp, fp, fp, i, vp, vp, vp]),
         "b200cp_device_status": (i, []),

@@ -52,8 +52,6 @@ struct Table {
 };
 
 template <typename T>
-__device__ __forceinline__ float to_float(T v) { return (float)v; }
-template <typename T>
 struct alignas(4 * sizeof(T)) Four {
   T v[4];
 };
@@ -95,10 +93,43 @@ __device__ __forceinline__ float fast_sqrt_ftz(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float fast_div(float x, float y) {
-  float q;
-  asm("div.approx.f32 %0, %1, %2;" : "=f"(q) : "f"(x), "f"(y));
-  return q;
+__device__ __forceinline__ float fast_inverse(float x) {   // (of a denominator, which is no subnormal number: its square root is not)
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Codes to numbers and back by the integer bits of a float around 2^23 and 1.5 2^23 (nearest, ties to even): the conversion instructions share the pipe
+// of the roots, sixteen lanes a cycle, and were half of its work.
+constexpr float kWhole = 12582912.f;
+__device__ __forceinline__ float code_at(uint32_t four, int k) { return __uint_as_float(__byte_perm(four, 0x4b000000u, 0x7440 + k)) - 8388608.f; }
+__device__ __forceinline__ void codes_of_m(uint32_t four, float (&x)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] = code_at(four ^ 0x80808080u, k) - 128.f;
+}
+__device__ __forceinline__ void codes_of_v(uint32_t four, float (&x)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] = code_at(four, k);
+}
+__device__ __forceinline__ uint32_t to_codes(const float (&x)[4]) {   // of whole numbers
+  const auto bits = [](float c) { return __float_as_uint(c + kWhole); };
+  return __byte_perm(__byte_perm(bits(x[0]), bits(x[1]), 0x0040), __byte_perm(bits(x[2]), bits(x[3]), 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, long long i, long long n, bool vec) {
+  if (vec && i + 4 <= n) return *reinterpret_cast<const uint32_t*>(p + i);
+  uint32_t c = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (i + k < n) c |= (uint32_t)p[i + k] << (8 * k);
+  return c;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, long long i, long long n, bool vec, uint32_t c) {
+  if (vec && i + 4 <= n) {
+    *reinterpret_cast<uint32_t*>(p + i) = c;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (i + k < n) p[i + k] = (uint8_t)(c >> (8 * k));
 }
 __device__ __forceinline__ float of_m(float c, float s) {
   const float q = c * (1.f / 127);
@@ -109,24 +140,26 @@ __device__ __forceinline__ float of_v(float c, float s) {
   return c == 255.f ? __int_as_float(0x7fffffff) : r * r * s;
 }
 // The code is that of 127 sqrt(|x| / s) with every operation rounded to nearest: found by the fast operations, and again by the exact
-// ones where those end within 2e-4 of a border (their error is below 5e-5 of a step), one value in 2500.  Exact codes do not depend
-// on how an operation is approximated: two implementations that round alike hold the same state.
+// ones where those end within 1e-4 (v: 2e-4) of a border (the two are within 5e-5, 1.1e-4 of a step of one another), one value in 3000.  Exact codes do not
+// depend on how an operation is approximated: two implementations that round alike hold the same state.
 __device__ __noinline__ float exact_code(float x, float s, float steps) {
   const float q = sqrtf(__fdiv_rn(fabsf(x), s));
   return rintf(steps * (steps > 200.f ? sqrtf(q) : q));
 }
 __device__ __forceinline__ float code_m(float x, float s, float inverse) {
-  if (!(fabsf(x) < __int_as_float(0x7f800000))) return -128.f;
   const float t = 127.f * fast_sqrt_ftz(fabsf(x) * inverse);
-  float c = rintf(t);
-  if (fabsf(t - c) > 0.4998f || inverse == 0.f) c = s > 0.f ? exact_code(x, s, 127.f) : 0.f;
-  return copysignf(c, x);
+  float c = (t + kWhole) - kWhole;
+  if (!(fabsf(t - c) <= 0.4999f) || inverse == 0.f)   // (what is not finite ends here too)
+    c = !(fabsf(x) < __int_as_float(0x7f800000)) ? 128.f : s > 0.f ? exact_code(x, s, 127.f) : 0.f;
+  return c == 128.f ? -128.f : copysignf(c, x);
 }
 __device__ __forceinline__ float code_v(float x, float s, float inverse) {
-  if (!(x < __int_as_float(0x7f800000))) return 255.f;
   const float t = 254.f * fast_sqrt_ftz(fast_sqrt_ftz(x * inverse));
-  float c = rintf(t);
-  if (fabsf(t - c) > 0.4998f || inverse == 0.f) c = s > 0.f ? exact_code(x, s, 254.f) : 0.f;
+  float c = (t + kWhole) - kWhole;
+  if (!(fabsf(t - c) <= 0.4998f) || inverse == 0.f) {
+    if (!(x < __int_as_float(0x7f800000))) return 255.f;
+    c = s > 0.f ? exact_code(x, s, 254.f) : 0.f;
+  }
   return x > 0.f ? fmaxf(c, 1.f) : 0.f;
 }
 __device__ __forceinline__ float finite_magnitude(float x) { return fabsf(x) < __int_as_float(0x7f800000) ? fabsf(x) : 0.f; }
@@ -180,16 +213,15 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     load4(g, i, n, vg, d[j]);
   }
   if constexpr (SMALL) {
-    const int8_t* cm = static_cast<const int8_t*>(e.m);
-    const uint8_t* cv = static_cast<const uint8_t*>(e.v);
+    const uint8_t *cm = static_cast<const uint8_t*>(e.m), *cv = static_cast<const uint8_t*>(e.v);
     const bool vm = aligned4(cm), vv = aligned4(cv);
     ms = e.ms[block];
     vs = e.vs[block];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const long long i = base + j * 128 + lane * 4;
-      load4(cm, i, n, vm, m[j]);
-      load4(cv, i, n, vv, v[j]);
+      codes_of_m(load_codes(cm, i, n, vm), m[j]);
+      codes_of_v(load_codes(cv, i, n, vv), v[j]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         m[j][k] = of_m(m[j][k], ms);
@@ -213,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     for (int k = 0; k < 4; ++k) {
       m[j][k] = fmaf(t.r.c1, d[j][k], __fmul_rn(t.r.b1, m[j][k]));
       v[j][k] = fmaf(t.r.c2, __fmul_rn(d[j][k], d[j][k]), __fmul_rn(t.r.b2, v[j][k]));
-      x[j][k] = fmaf(-step, fast_div(m[j][k], fmaf(fast_sqrt(v[j][k]), root, t.r.eps)), fmaf(-decay, x[j][k], x[j][k]));
+      x[j][k] = fmaf(-step, m[j][k] * fast_inverse(fmaf(fast_sqrt(v[j][k]), root, t.r.eps)), fmaf(-decay, x[j][k], x[j][k]));
       if (SMALL) {   // (values past the end are zero: they change no maximum)
         mm = fmaxf(mm, finite_magnitude(m[j][k]));
         mv = fmaxf(mv, finite_magnitude(v[j][k]));
@@ -226,8 +258,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     store4(p, i, n, vp, x[j]);
   }
   if constexpr (SMALL) {
-    int8_t* cm = static_cast<int8_t*>(e.m);
-    uint8_t* cv = static_cast<uint8_t*>(e.v);
+    uint8_t *cm = static_cast<uint8_t*>(e.m), *cv = static_cast<uint8_t*>(e.v);
     mm = warp_max(mm);
     mv = warp_max(mv);
     const float im = inverse_of(mm), iv = inverse_of(mv);
@@ -244,8 +275,8 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         m[j][k] = code_m(m[j][k], mm, im);
         v[j][k] = code_v(v[j][k], mv, iv);
       }
-      store4(cm, i, n, vm, m[j]);
-      store4(cv, i, n, vv, v[j]);
+      store_codes(cm, i, n, vm, to_codes(m[j]));
+      store_codes(cv, i, n, vv, to_codes(v[j]));
     }
   } else {
     float *fm = static_cast<float*>(e.m), *fv = static_cast<float*>(e.v);
@@ -259,22 +290,39 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
   }
 }
 
+// Four groups of four values per thread, so that enough bytes are in flight (with one group 111 us of 58.7 M values).
+constexpr int kMomentGroups = 4;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) moments_kernel(long long n, const int8_t* cm, const uint8_t* cv, const float* ms, const float* vs,
+__global__ void __launch_bounds__(kThreads) moments_kernel(long long n, const uint8_t* cm, const uint8_t* cv, const float* ms, const float* vs,
                                                            T* m, T* v) {
-  const long long i = ((long long)blockIdx.x * kThreads + threadIdx.x) * 4;
-  if (i >= n) return;
-  const float a = ms[i / kBlock], b = vs[i / kBlock];
-  float x[4], y[4];
-  load4(cm, i, n, aligned4(cm), x);
-  load4(cv, i, n, aligned4(cv), y);
+  const long long i0 = (long long)blockIdx.x * (kThreads * 4 * kMomentGroups) + threadIdx.x * 4;
+  const bool a = aligned4(cm), b = aligned4(cv), c = aligned4(m), d = aligned4(v);
+  uint32_t p[kMomentGroups], q[kMomentGroups];
+  float s[kMomentGroups], r[kMomentGroups];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    x[k] = of_m(x[k], a);
-    y[k] = of_v(y[k], b);
+  for (int j = 0; j < kMomentGroups; ++j) {
+    const long long i = i0 + j * (kThreads * 4);
+    if (i >= n) break;
+    p[j] = load_codes(cm, i, n, a);
+    q[j] = load_codes(cv, i, n, b);
+    s[j] = ms[i / kBlock];
+    r[j] = vs[i / kBlock];
   }
-  store4(m, i, n, aligned4(m), x);
-  store4(v, i, n, aligned4(v), y);
+#pragma unroll
+  for (int j = 0; j < kMomentGroups; ++j) {
+    const long long i = i0 + j * (kThreads * 4);
+    if (i >= n) break;
+    float x[4], y[4];
+    codes_of_m(p[j], x);
+    codes_of_v(q[j], y);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[k] = of_m(x[k], s[j]);
+      y[k] = of_v(y[k], r[j]);
+    }
+    store4(m, i, n, c, x);
+    store4(v, i, n, d, y);
+  }
 }
 
 template <typename P, typename G, bool SMALL, int CAP>
@@ -360,11 +408,12 @@ int b200cp_adamw_moments(unsigned long long n, const void* exp_avg, const void* 
   if (n == 0) return B200CP_OK;
   if (!exp_avg || !exp_avg_sq || !scale_avg || !scale_sq || !m || !v)
     return fail(B200CP_ERR_INVALID_ARG, "b200cp_adamw_moments: null pointer");
-  const unsigned long long ctas = (n + 4 * kThreads - 1) / (4 * kThreads);
+  constexpr unsigned long long per = 4 * kThreads * kMomentGroups;
+  const unsigned long long ctas = (n + per - 1) / per;
   if (ctas > 0x7fffffffull) return fail(B200CP_ERR_UNSUPPORTED, "b200cp_adamw_moments: %llu values", n);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const auto go = [&](auto* out_m, auto* out_v) {
-    moments_kernel<<<(unsigned)ctas, kThreads, 0, st>>>((long long)n, static_cast<const int8_t*>(exp_avg), static_cast<const uint8_t*>(exp_avg_sq),
+    moments_kernel<<<(unsigned)ctas, kThreads, 0, st>>>((long long)n, static_cast<const uint8_t*>(exp_avg), static_cast<const uint8_t*>(exp_avg_sq),
                                                         scale_avg, scale_sq, out_m, out_v);
     B200CP_LAUNCH_OK("moments_kernel");
     return (int)B200CP_OK;

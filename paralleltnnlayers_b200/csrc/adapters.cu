@@ -1,0 +1,899 @@
+// Low-rank adapters of many requests beside a shared projection, forward and gradients.
+//
+//   V[s] = c[a] X[s] A[a],  out[s] = Y[s] + V[s] B[a]            a: the adapter of row s
+//   W[s] = c[a] dY[s] B[a]^T,  dX[s] = W[s] A[a]^T,  dA[a] = sum_s X[s]^T W[s],  dB[a] = sum_s V[s]^T dY[s]
+//
+// Forward and dX are one kernel (the second with the factors transposed): a tile of 16 or 64 rows of one adapter, whose sum over the features runs
+// over the CTAs of a cluster and is joined through their shared memory, so that X is read once, V stays on the chip between the two
+// products and a few rows still fill the machine.  What bounds it is HBM: X and Y in, out once; the products take 2 R (I + O) operations a row, on
+// mma.sync for 16-bit types (R columns are too few to feed anything wider) and FFMA for fp32, whose sums are then those of fp32.
+// Rows of a tile are gathered by the plan's order, so requests may lie anywhere in the batch; a row's result depends on its own row and
+// adapter only, and values that are not finite stay with theirs.  V and W are rounded once to the 16-bit type: they are operands of products.
+//
+// dA and dB are one kernel over the rows in the plan's order, cut into ranges of equal length: a CTA has 128 (fp32: 64) features of a range and adds
+// row after row in registers until the adapter changes.  Adapters inside a range are written at once, those that reach into another range as
+// partial sums that a second launch joins in order: no atomics, the same bits each time.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace b200cp {
+namespace {
+
+constexpr int kThreads = 256, kWarps = 8, kMostRank = 128, kMostAdapters = 16384;
+
+// ---- plan -------------------------------------------------------------------------------------------------------------------
+// ints: [0] tiles, [1] rows with an adapter, [2..3] free | start[count + 2] | tile_adapter[tiles] | tile_first[tiles] | order[rows].
+// Rows without an adapter are those of "adapter" count, behind the others.
+struct Plan {
+  int tm, tiles;   // rows of a tile; the most tiles there can be
+  size_t start, adapter, first, order, ints;
+};
+Plan plan_of(int rows, int count) {
+  Plan p;
+  const int groups = std::min(rows, count);
+  // Tiles of 64 rows read an adapter once per 64 rows, tiles of 16 waste less of themselves on adapters of a few rows.
+  p.tm = groups > 0 && rows / groups >= 48 ? 64 : 16;
+  p.tiles = rows / p.tm + std::min(rows, count + 1);
+  p.start = 4;
+  p.adapter = p.start + count + 2;
+  p.first = p.adapter + p.tiles;
+  p.order = p.first + p.tiles;
+  p.ints = align_up(p.order + rows, 4);
+  return p;
+}
+
+// exclusive sums of the values of all 1024 threads; `total` gets the sum of all
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int s = warp_sums[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += y;
+    }
+    warp_sums[lane] = s;
+  }
+  __syncthreads();
+  const int before = warp ? warp_sums[warp - 1] : 0;
+  *total = warp_sums[31];
+  __syncthreads();
+  return before + x - v;
+}
+
+// A stable counting sort by one CTA: the first `sorters` warps count the rows of a range each, every (adapter, warp) gets its place, and the warps put
+// their rows there in order.  shared: counts[(count + 1) * sorters] | tiles before each adapter [count + 2]
+__global__ void __launch_bounds__(1024) plan_kernel(int rows, int count, int tm, int sorters, const int* adapters, int* plan, size_t at_adapter,
+                                                    size_t at_first, size_t at_order) {
+  extern __shared__ int counts[];
+  __shared__ int warp_sums[32];
+  const int keys = count + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int* tiles_before = counts + keys * sorters;
+  for (int i = tid; i < keys * sorters; i += 1024) counts[i] = 0;
+  __syncthreads();
+  const int per = ((rows + sorters - 1) / sorters + 31) / 32 * 32, r0 = min(rows, warp * per), r1 = min(rows, r0 + per);
+  const auto key_of = [&](int r) {
+    const int a = adapters[r];
+    return a >= 0 && a < count ? a : count;
+  };
+  if (warp < sorters)
+    for (int b = r0; b < r1; b += 32) {
+      const bool in = b + lane < r1;
+      const int key = in ? key_of(b + lane) : -1;
+      const unsigned same = __match_any_sync(0xffffffffu, key);
+      if (in && (same & ((1u << lane) - 1)) == 0) counts[key * sorters + warp] += __popc(same);
+      __syncwarp();
+    }
+  __syncthreads();
+  {   // places: sums over (adapter, warp)
+    const int n = keys * sorters, each = (n + 1023) / 1024, b = min(n, tid * each), e = min(n, b + each);
+    int sum = 0, total;
+    for (int i = b; i < e; ++i) sum += counts[i];
+    int at = block_scan(sum, warp_sums, &total);
+    for (int i = b; i < e; ++i) {
+      const int c = counts[i];
+      counts[i] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  int* start = plan + 4;
+  int tiles;
+  {
+    const int each = (keys + 1023) / 1024, b = min(keys, tid * each), e = min(keys, b + each);
+    int sum = 0;
+    const auto rows_of = [&](int k) { return (k + 1 < keys ? counts[(k + 1) * sorters] : rows) - counts[k * sorters]; };
+    for (int k = b; k < e; ++k) sum += (rows_of(k) + tm - 1) / tm;
+    int at = block_scan(sum, warp_sums, &tiles);
+    for (int k = b; k < e; ++k) {
+      tiles_before[k] = at;
+      at += (rows_of(k) + tm - 1) / tm;
+      start[k] = counts[k * sorters];
+    }
+  }
+  if (tid == 0) {
+    start[keys] = rows;
+    plan[0] = tiles;
+    plan[1] = counts[count * sorters];
+  }
+  __syncthreads();
+  for (int t = tid; t < tiles; t += 1024) {
+    int a = 0, b = keys;   // the last adapter with no more than t tiles before it (the ones after it with as many have none)
+    while (b - a > 1) {
+      const int c = (a + b) / 2;
+      if (tiles_before[c] <= t) a = c; else b = c;
+    }
+    plan[at_adapter + t] = a;
+    plan[at_first + t] = counts[a * sorters] + (t - tiles_before[a]) * tm;
+  }
+  __syncthreads();
+  if (warp < sorters)
+    for (int b = r0; b < r1; b += 32) {
+      const bool in = b + lane < r1;
+      const int key = in ? key_of(b + lane) : -1;
+      const unsigned same = __match_any_sync(0xffffffffu, key), before = same & ((1u << lane) - 1);
+      const int at = in ? counts[key * sorters + warp] + __popc(before) : 0;
+      __syncwarp();
+      if (in) {
+        plan[at_order + at] = b + lane;
+        if (before == 0) counts[key * sorters + warp] += __popc(same);
+      }
+      __syncwarp();
+    }
+}
+
+// ---- loads ------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(void* dst, const void* src, int bytes) {   // the rest of the 16 is zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_at(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Rows of `pieces` x 16 bytes into shared memory: row r from row(r) (null: zeros), from column c0 on, zero past `cols`.  `vec`: the rows start on
+// 16-byte boundaries (then the copies are asynchronous).
+template <typename T, typename Row>
+__device__ __forceinline__ void load_rows(char* dst, int stride, int rows, int pieces, const void* any, Row row, int c0, int cols, bool vec) {
+  constexpr int E = 16 / sizeof(T);
+  for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
+    const int r = i / pieces, q = i - r * pieces, c = c0 + q * E;
+    const T* src = row(r);
+    const int left = src ? min(E, max(0, cols - c)) : 0;
+    char* to = dst + r * stride + q * 16;
+    if (vec) {
+      copy16(to, left > 0 ? (const void*)(src + c) : any, left * (int)sizeof(T));
+    } else {
+      alignas(16) T v[E];
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] = k < left ? src[c + k] : (T)0.f;
+      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(v);
+    }
+  }
+}
+
+// ---- products ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(shared_at(p))
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(shared_at(p))
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The 16 x 16 block at p of rows `stride` bytes apart, as mma's A (16 rows of 16 k), and as its B for two groups of eight columns (r[0], r[1] and r[2],
+// r[3]): `kmajor` where a row holds the k of one column, else a row holds the columns of one k.  For A with a row per k: a_of_k.
+__device__ __forceinline__ void a_block(uint32_t (&r)[4], const char* p, int stride) {
+  const int l = threadIdx.x & 31;
+  ldsm4(r, p + (l & 15) * stride + (l >> 4) * 16);
+}
+__device__ __forceinline__ void a_of_k(uint32_t (&r)[4], const char* p, int stride) {
+  const int l = threadIdx.x & 31;
+  ldsm4t(r, p + ((l & 7) + (l >> 4) * 8) * stride + ((l >> 3) & 1) * 16);
+}
+template <bool KMAJOR>
+__device__ __forceinline__ void b_block(uint32_t (&r)[4], const char* p, int stride) {
+  const int l = threadIdx.x & 31;
+  if (KMAJOR)
+    ldsm4(r, p + ((l & 7) + (l >> 4) * 8) * stride + ((l >> 3) & 1) * 16);
+  else
+    ldsm4t(r, p + ((l & 7) + ((l >> 3) & 1) * 8) * stride + (l >> 4) * 16);
+}
+
+// ---- forward and dX ---------------------------------------------------------------------------------------------------------
+struct Args {
+  int rows, K, N, R, count;   // the first product sums over K, the second gives N columns
+  const void *X, *Y;          // [rows][K]; [rows][N], or null: nothing is added
+  const void *F1, *F2;        // forward: A [K][R], B [R][N] of an adapter; BACK: B [R][K], A [N][R]
+  const float* scale;
+  const int *start, *tile_adapter, *tile_first, *order, *head;
+  void *out, *V;              // [rows][N]; [rows][R] or null
+  int vx, vy, v1, v2;         // rows of X, of Y and out, of the factors start on 16-byte boundaries
+};
+
+template <typename T, int TM, int RP>
+struct Shape {
+  static constexpr int E = 16 / sizeof(T), KC = 256 / sizeof(T);        // a chunk is 256 bytes of each row
+  static constexpr int xs = 256 + 16;                                   // bytes from row to row: ldmatrix and 16-byte reads without conflicts
+  static constexpr int ls = RP * (int)sizeof(T) + 16;                   // of a factor with the rank innermost
+  static constexpr int factor = KC * ls > RP * xs ? KC * ls : RP * xs;
+  static constexpr int stage = TM * xs + factor;
+  static constexpr int stages = RP <= 32 ? 4 : 3;
+  static constexpr int CG = sizeof(T) == 4 && RP > 32 ? RP / 32 : 1;    // fp32: groups of 32 ranks over warps
+  static constexpr int MG = sizeof(T) == 4 ? 1 : TM / 16;               // 16-bit: groups of 16 rows over warps
+  static constexpr int KG = kWarps / (MG * CG);                         // parts of a chunk's sum over warps
+  static constexpr int red = KG * TM * RP * 4;
+  static constexpr int ring = stages * stage > red ? stages * stage : red;
+  static constexpr int part = TM * RP * 4, vs = TM * ls;
+  static constexpr int smem = ring + part + vs + TM * 4;
+};
+
+template <typename T, int TM, int RP, bool BACK>
+__global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constant__ Args g) {
+  using S = Shape<T, TM, RP>;
+  constexpr int KC = S::KC, E = S::E;
+  extern __shared__ __align__(16) char sm[];
+  float* part = reinterpret_cast<float*>(sm + S::ring);
+  char* vs = sm + S::ring + S::part;
+  int* rowat = reinterpret_cast<int*>(vs + S::vs);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t crank, csize;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
+  grid_dependency_wait();   // the plan
+  const int tile = (int)(blockIdx.x / csize);
+  if (tile >= g.head[0]) return;   // (all CTAs of the cluster)
+  const int a = g.tile_adapter[tile], first = g.tile_first[tile], len = min(TM, g.start[a + 1] - first);
+  const T *X = static_cast<const T*>(g.X), *Y = static_cast<const T*>(g.Y);
+  T* out = static_cast<T*>(g.out);
+  const int K = g.K, N = g.N, R = g.R;
+  if (tid < TM) rowat[tid] = tid < len ? g.order[first + tid] : 0;
+  __syncthreads();
+  const int nn = (N + KC - 1) / KC, nper = (nn + (int)csize - 1) / (int)csize, n0 = min(nn, (int)crank * nper), n1 = min(nn, n0 + nper);
+  const auto store_chunk = [&](const char* src, int c0) {   // [len][KC] in shared memory -> out
+    for (int i = tid; i < len * 16; i += kThreads) {
+      const int r = i >> 4, q = i & 15, c = c0 + q * E;
+      if (c >= N) continue;
+      T* to = out + (size_t)rowat[r] * N + c;
+      const uint4 v = *reinterpret_cast<const uint4*>(src + r * S::xs + q * 16);
+      if (g.vy && c + E <= N) {
+        *reinterpret_cast<uint4*>(to) = v;
+      } else {
+        alignas(16) T e[E];
+        *reinterpret_cast<uint4*>(e) = v;
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+          if (c + k < N) to[k] = e[k];
+      }
+    }
+  };
+  if (a == g.count) {   // rows without an adapter
+    if (out == Y) return;
+    for (int n = n0; n < n1; ++n) {
+      const auto row = [&](int r) { return Y && r < len ? Y + (size_t)rowat[r] * N : nullptr; };
+      load_rows<T>(sm, S::xs, TM, 16, g.out, row, n * KC, N, g.vy);
+      copies_end_group();
+      copies_wait<0>();
+      __syncthreads();
+      store_chunk(sm, n * KC);
+      __syncthreads();
+    }
+    return;
+  }
+  const T *F1 = static_cast<const T*>(g.F1) + (size_t)a * R * K, *F2 = static_cast<const T*>(g.F2) + (size_t)a * R * N;
+  // a factor's chunk: KC features by the ranks, as it lies in memory
+  const auto load_factor = [&](char* dst, const T* F, int n, bool long_rows, int c0, bool vec) {
+    if (long_rows)
+      load_rows<T>(dst, S::xs, RP, 16, F, [&](int r) { return r < R ? F + (size_t)r * n : nullptr; }, c0, n, vec);
+    else
+      load_rows<T>(dst, S::ls, KC, RP / E, F, [&](int r) { return c0 + r < n ? F + (size_t)(c0 + r) * R : nullptr; }, 0, R, vec);
+  };
+
+  // ---- V: this CTA's part of the sum over K ----
+  const int nk = (K + KC - 1) / KC, kper = (nk + (int)csize - 1) / (int)csize, k0 = min(nk, (int)crank * kper), k1 = min(nk, k0 + kper);
+  const auto load_k = [&](int k) {
+    if (k < k1) {
+      char* st = sm + (k - k0) % S::stages * S::stage;
+      load_rows<T>(st, S::xs, TM, 16, X, [&](int r) { return r < len ? X + (size_t)rowat[r] * K : nullptr; }, k * KC, K, g.vx);
+      load_factor(st + TM * S::xs, F1, K, BACK, k * KC, g.v1);
+    }
+    copies_end_group();
+  };
+  // fp32: a lane has rows lr + 8 i, and ranks lc + 4 j (BACK) or 8 lc + j of its warp's group
+  constexpr int RC = RP < 32 ? RP : 32, LC = RC / 4, LR = TM / 8;
+  constexpr bool F32 = sizeof(T) == 4;
+  float acc[F32 ? LR : RP / 8][F32 ? LC : 4] = {};
+  const int mg = warp % S::MG, kg = F32 ? warp / S::CG : warp / S::MG, cg = F32 ? warp % S::CG : 0, lr = lane >> 2, lc = lane & 3;
+#pragma unroll
+  for (int s = 0; s < S::stages - 1; ++s) load_k(k0 + s);
+  for (int k = k0; k < k1; ++k) {
+    copies_wait<S::stages - 2>();
+    __syncthreads();
+    load_k(k + S::stages - 1);
+    const char *xt = sm + (k - k0) % S::stages * S::stage, *ft = xt + TM * S::xs;
+    if constexpr (F32) {
+      constexpr int KW = KC / S::KG;   // 8, or with groups of ranks 16, 32
+#pragma unroll 2
+      for (int q = kg * KW; q < (kg + 1) * KW; q += 4) {
+        float x[LR][4];
+#pragma unroll
+        for (int i = 0; i < LR; ++i) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(xt + (lr + 8 * i) * S::xs + q * 4);
+        if (BACK) {
+#pragma unroll
+          for (int j = 0; j < LC; ++j) {
+            const float4 f = *reinterpret_cast<const float4*>(ft + (cg * 32 + lc + 4 * j) * S::xs + q * 4);
+#pragma unroll
+            for (int i = 0; i < LR; ++i) acc[i][j] = fmaf(x[i][0], f.x, fmaf(x[i][1], f.y, fmaf(x[i][2], f.z, fmaf(x[i][3], f.w, acc[i][j]))));
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < LC; j += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(ft + (q + u) * S::ls + (cg * 32 + lc * LC + j) * 4);
+#pragma unroll
+              for (int i = 0; i < LR; ++i) {
+                acc[i][j] = fmaf(x[i][u], f.x, acc[i][j]);
+                acc[i][j + 1] = fmaf(x[i][u], f.y, acc[i][j + 1]);
+                acc[i][j + 2] = fmaf(x[i][u], f.z, acc[i][j + 2]);
+                acc[i][j + 3] = fmaf(x[i][u], f.w, acc[i][j + 3]);
+              }
+            }
+        }
+      }
+    } else {
+      constexpr int KW = KC / S::KG;   // 64 or 16
+#pragma unroll
+      for (int q = kg * KW; q < (kg + 1) * KW; q += 16) {
+        uint32_t x[4];
+        a_block(x, xt + mg * 16 * S::xs + q * 2, S::xs);
+#pragma unroll
+        for (int j = 0; j < RP; j += 16) {
+          uint32_t f[4];
+          if (BACK)
+            b_block<true>(f, ft + j * S::xs + q * 2, S::xs);
+          else
+            b_block<false>(f, ft + q * S::ls + j * 2, S::ls);
+          mma16<T>(acc[j / 8], x, f[0], f[1]);
+          mma16<T>(acc[j / 8 + 1], x, f[2], f[3]);
+        }
+      }
+    }
+  }
+  copies_wait<0>();
+  __syncthreads();
+  // the warps' parts, then the cluster's
+  float* red = reinterpret_cast<float*>(sm) + kg * TM * RP;
+  if constexpr (F32) {
+#pragma unroll
+    for (int i = 0; i < LR; ++i)
+#pragma unroll
+      for (int j = 0; j < LC; ++j) red[(lr + 8 * i) * RP + cg * 32 + (BACK ? lc + 4 * j : lc * LC + j)] = acc[i][j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float2*>(&red[(mg * 16 + lr + 8 * h) * RP + j * 8 + lc * 2]) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+  }
+  __syncthreads();
+  for (int i = tid; i < TM * RP; i += kThreads) {
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < S::KG; ++q) v += reinterpret_cast<const float*>(sm)[q * TM * RP + i];
+    part[i] = v;
+  }
+  __syncthreads();
+  const auto load_n = [&](int n) {
+    if (n < n1) {
+      char* st = sm + (n - n0) % S::stages * S::stage;
+      if (Y) load_rows<T>(st, S::xs, TM, 16, Y, [&](int r) { return r < len ? Y + (size_t)rowat[r] * N : nullptr; }, n * KC, N, g.vy);
+      load_factor(st + TM * S::xs, F2, N, !BACK, n * KC, g.v2);
+    }
+    copies_end_group();
+  };
+#pragma unroll
+  for (int s = 0; s < S::stages - 1; ++s) load_n(n0 + s);   // while the cluster's parts are joined
+  const float c = g.scale ? g.scale[a] : 1.f;
+  if (csize > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  for (int i = tid * 2; i < TM * RP; i += kThreads * 2) {
+    float2 v = make_float2(0.f, 0.f);
+    if (csize == 1) {
+      v = *reinterpret_cast<const float2*>(part + i);
+    } else {
+      float2 from[8];
+#pragma unroll
+      for (uint32_t p = 0; p < 8; ++p) {
+        from[p] = make_float2(0.f, 0.f);
+        if (p < csize) {
+          uint32_t at;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_at(part + i)), "r"(p));
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(from[p].x), "=f"(from[p].y) : "r"(at) : "memory");
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        v.x += from[p].x;
+        v.y += from[p].y;
+      }
+    }
+    const int r = i / RP, j = i - r * RP;
+    T* to = reinterpret_cast<T*>(vs + r * S::ls) + j;
+    to[0] = (T)(v.x * c);
+    to[1] = (T)(v.y * c);
+    if (g.V && crank == 0 && r < len) {
+      T* w = static_cast<T*>(g.V) + (size_t)rowat[r] * R + j;
+      if (j < R) w[0] = to[0];
+      if (j + 1 < R) w[1] = to[1];
+    }
+  }
+  __syncthreads();
+  if (csize > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this CTA reads no other's part any more
+
+  // ---- out = Y + V F2 ----
+  constexpr int NG = kWarps / (TM / 16);
+  uint32_t va[F32 ? 1 : RP / 16][4];
+  if constexpr (!F32) {
+#pragma unroll
+    for (int j = 0; j < RP / 16; ++j) a_block(va[j], vs + mg * 16 * S::ls + j * 32, S::ls);
+  }
+  for (int n = n0; n < n1; ++n) {
+    copies_wait<S::stages - 2>();
+    __syncthreads();
+    load_n(n + S::stages - 1);
+    char* yt = sm + (n - n0) % S::stages * S::stage;
+    const char* ft = yt + TM * S::xs;
+    if constexpr (F32) {
+      constexpr int RW = TM / kWarps;   // rows of a warp; a lane has two columns
+      float o[RW][2] = {};
+#pragma unroll 4
+      for (int j = 0; j < RP; j += 4) {
+        float v[RW][4];
+#pragma unroll
+        for (int i = 0; i < RW; ++i) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(vs + (warp * RW + i) * S::ls + j * 4);
+        float f[2][4];
+        if (BACK) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(f[h]) = *reinterpret_cast<const float4*>(ft + (lane + 32 * h) * S::ls + j * 4);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            f[0][u] = *reinterpret_cast<const float*>(ft + (j + u) * S::xs + lane * 4);
+            f[1][u] = *reinterpret_cast<const float*>(ft + (j + u) * S::xs + (lane + 32) * 4);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < RW; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[i][h] = fmaf(v[i][u], f[h][u], o[i][h]);
+      }
+#pragma unroll
+      for (int i = 0; i < RW; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float* p = reinterpret_cast<float*>(yt + (warp * RW + i) * S::xs) + lane + 32 * h;
+          *p = Y ? *p + o[i][h] : o[i][h];
+        }
+    } else {
+      constexpr int NW = KC / NG;   // columns of a warp: 64 or 16
+      const int nc = (warp / S::MG) * NW;
+#pragma unroll
+      for (int q = 0; q < NW; q += 16) {
+        float o[2][4] = {};
+#pragma unroll
+        for (int j = 0; j < RP; j += 16) {
+          uint32_t f[4];
+          if (BACK)
+            b_block<true>(f, ft + (nc + q) * S::ls + j * 2, S::ls);
+          else
+            b_block<false>(f, ft + j * S::xs + (nc + q) * 2, S::xs);
+          mma16<T>(o[0], va[j / 16], f[0], f[1]);
+          mma16<T>(o[1], va[j / 16], f[2], f[3]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            T* p = reinterpret_cast<T*>(yt + (mg * 16 + lr + 8 * e) * S::xs) + nc + q + h * 8 + lc * 2;
+            const float y0 = Y ? (float)p[0] : 0.f, y1 = Y ? (float)p[1] : 0.f;
+            p[0] = (T)(y0 + o[h][2 * e]);
+            p[1] = (T)(y1 + o[h][2 * e + 1]);
+          }
+      }
+    }
+    __syncthreads();
+    store_chunk(yt, n * KC);
+  }
+  copies_wait<0>();
+  if (csize > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ---- dA and dB --------------------------------------------------------------------------------------------------------------
+struct GradArgs {
+  int rows, I, O, R, count, tiles_i, ranges;
+  const void *X, *W, *V, *dY;   // [rows][I], [rows][R], [rows][R], [rows][O]
+  const int *start, *order, *head;
+  void *dA, *dB;
+  float* partial;               // [range][2][I + O][RP]
+  int vx, vy, vr;
+};
+template <typename T, int RP>
+struct GradShape {
+  static constexpr int E = 16 / sizeof(T), LT = 256 / sizeof(T), KT = sizeof(T) == 4 ? 32 : 64;   // features and rows of a step
+  static constexpr int zs = 256 + 16, ws = RP * (int)sizeof(T) + 16;
+  static constexpr int stage = KT * (zs + ws), stages = RP <= 64 ? 4 : 3;
+  static constexpr int smem = stages * stage;
+};
+__device__ __forceinline__ int range_rows(const GradArgs& g, int kt) {   // of a range: a multiple of a step
+  const int each = (g.head[1] + g.ranges - 1) / g.ranges;
+  return max(kt, (each + kt - 1) / kt * kt);
+}
+__device__ __forceinline__ int adapter_at(const int* start, int count, int pos) {   // the adapter that has row `pos` of the order
+  int a = 0, b = count + 1;
+  while (b - a > 1) {
+    const int c = (a + b) / 2;
+    if (start[c] <= pos) a = c; else b = c;
+  }
+  return a;
+}
+// The steps of a range: up to KT rows of one adapter each.
+struct Steps {
+  const int* start;
+  int count, end, pos, a, stop;   // stop: where the adapter's rows (of the range) end
+  __device__ Steps(const GradArgs& g, int b, int e) : start(g.start), count(g.count), end(e), pos(b), a(0), stop(b) { find(); }
+  __device__ void find() {
+    if (pos >= end) return;
+    a = adapter_at(start, count, pos);
+    stop = min(end, start[a + 1]);
+  }
+  __device__ bool done() const { return pos >= end; }
+  __device__ void next(int kt) {
+    pos = min(pos + kt, stop);
+    if (pos == stop) find();
+  }
+};
+
+template <typename T, int RP>
+__global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_constant__ GradArgs g) {
+  using S = GradShape<T, RP>;
+  constexpr int KT = S::KT, LT = S::LT, E = S::E;
+  constexpr bool F32 = sizeof(T) == 4;
+  extern __shared__ __align__(16) char sm[];
+  grid_dependency_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool second = (int)blockIdx.x >= g.tiles_i;   // dB
+  const int L = second ? g.O : g.I, l0 = ((int)blockIdx.x - (second ? g.tiles_i : 0)) * LT, R = g.R;
+  const T *Z = static_cast<const T*>(second ? g.dY : g.X), *W = static_cast<const T*>(second ? g.V : g.W);
+  T* out = static_cast<T*>(second ? g.dB : g.dA);
+  const bool vz = second ? g.vy : g.vx;
+  const int per = range_rows(g, KT), b = min(g.head[1], (int)blockIdx.y * per), e = min(g.head[1], b + per);
+  Steps load(g, b, e), at = load;
+  int loaded = 0;
+  const auto load_step = [&] {
+    if (!load.done()) {
+      char* st = sm + loaded % S::stages * S::stage;
+      const int n = min(KT, load.stop - load.pos), p = load.pos;
+      load_rows<T>(st, S::zs, KT, 16, Z, [&](int r) { return r < n ? Z + (size_t)g.order[p + r] * L : nullptr; }, l0, L, vz);
+      load_rows<T>(st + KT * S::zs, S::ws, KT, RP / E, W, [&](int r) { return r < n ? W + (size_t)g.order[p + r] * R : nullptr; }, 0, R, g.vr);
+      load.next(KT);
+      ++loaded;
+    }
+    copies_end_group();
+  };
+#pragma unroll
+  for (int s = 0; s < S::stages - 1; ++s) load_step();
+  // fp32: a warp has eight features, a lane LR of them and LC ranks; 16 bits: a warp has sixteen features and all ranks
+  constexpr int LC = RP == 16 ? 2 : 4, CGN = RP / LC, LR = CGN / 4;   // 8 / (32 / CGN)
+  float acc[F32 ? LR : RP / 8][F32 ? LC : 4] = {};
+  const int lr = F32 ? lane / CGN : lane >> 2, lc = F32 ? lane % CGN : lane & 3;
+  for (int k = 0; !at.done(); ++k) {
+    copies_wait<S::stages - 2>();
+    __syncthreads();
+    load_step();
+    const char *zt = sm + k % S::stages * S::stage, *wt = zt + KT * S::zs;
+    if constexpr (F32) {
+#pragma unroll 4
+      for (int t = 0; t < KT; ++t) {
+        const float *z = reinterpret_cast<const float*>(zt + t * S::zs) + warp * 8 + lr * LR, *w = reinterpret_cast<const float*>(wt + t * S::ws) + lc * LC;
+        float x[LR], y[LC];
+#pragma unroll
+        for (int i = 0; i < LR; ++i) x[i] = z[i];
+#pragma unroll
+        for (int j = 0; j < LC; ++j) y[j] = w[j];
+#pragma unroll
+        for (int i = 0; i < LR; ++i)
+#pragma unroll
+          for (int j = 0; j < LC; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < KT; t += 16) {
+        uint32_t z[4];
+        a_of_k(z, zt + t * S::zs + warp * 32, S::zs);
+#pragma unroll
+        for (int j = 0; j < RP; j += 16) {
+          uint32_t w[4];
+          b_block<false>(w, wt + t * S::ws + j * 2, S::ws);
+          mma16<T>(acc[j / 8], z, w[0], w[1]);
+          mma16<T>(acc[j / 8 + 1], z, w[2], w[3]);
+        }
+      }
+    }
+    const int a = at.a;
+    const bool last = at.pos + KT >= at.stop;
+    at.next(KT);
+    if (!last) continue;
+    // the adapter's rows of this range end here
+    const int ab = g.start[a], ae = g.start[a + 1];
+    const bool whole = ab >= b && ae <= e;
+    float* p = g.partial + ((size_t)(blockIdx.y * 2 + (ab >= b ? 1 : 0)) * (g.I + g.O) + (second ? g.I : 0)) * RP;
+    const auto put = [&](int l, int r, float v) {
+      l += l0;
+      if (l >= L) return;
+      if (!whole)
+        p[(size_t)l * RP + r] = v;
+      else if (r < R)
+        out[second ? ((size_t)a * R + r) * L + l : ((size_t)a * L + l) * R + r] = (T)v;
+    };
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < LR; ++i)
+#pragma unroll
+        for (int j = 0; j < LC; ++j) {
+          put(warp * 8 + lr * LR + i, lc * LC + j, acc[i][j]);
+          acc[i][j] = 0.f;
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          put(warp * 16 + lr + (v >> 1) * 8, j * 8 + lc * 2 + (v & 1), acc[j][v]);
+          acc[j][v] = 0.f;
+        }
+    }
+  }
+  copies_wait<0>();
+}
+
+// Adapters that lie in several ranges: the sum of their parts in the order of the ranges.  Adapters without rows: zero.
+template <typename T, int RP>
+__global__ void __launch_bounds__(kThreads) join_grads_kernel(const __grid_constant__ GradArgs g) {
+  constexpr int KT = GradShape<T, RP>::KT;
+  grid_dependency_wait();
+  const int a = blockIdx.x, ab = g.start[a], ae = g.start[a + 1], per = range_rows(g, KT);
+  const int r0 = ab / per, r1 = ae > ab ? (ae - 1) / per : r0;
+  if (ae > ab && r0 == r1) return;
+  const long na = g.dA ? (long)g.I * g.R : 0, n = na + (g.dB ? (long)g.O * g.R : 0);
+  for (long i = (long)blockIdx.y * kThreads + threadIdx.x; i < n; i += (long)gridDim.y * kThreads) {
+    const bool second = i >= na;
+    const long q = second ? i - na : i;
+    const int l = second ? (int)(q % g.O) : (int)(q / g.R), r = second ? (int)(q / g.O) : (int)(q % g.R);
+    float v = 0.f;
+    if (ae > ab) {
+      const float* p = g.partial + ((size_t)(second ? g.I : 0) + l) * RP + r;
+      const size_t step = (size_t)(g.I + g.O) * RP;
+      v = p[(size_t)(2 * r0 + 1) * step];
+      for (int k = r0 + 1; k <= r1; ++k) v += p[(size_t)(2 * k) * step];
+    }
+    static_cast<T*>(second ? g.dB : g.dA)[(size_t)a * (second ? g.O : g.I) * g.R + q] = (T)v;
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+int sms() {
+  DeviceInfo di;
+  return device_info(&di) ? 148 : di.sm_count;
+}
+bool rows16(const void* p, size_t row_bytes) { return !(reinterpret_cast<uintptr_t>(p) & 15) && row_bytes % 16 == 0; }
+
+template <typename T, int TM, int RP, bool BACK>
+int launch_tiles(const Args& g, int tiles, cudaStream_t st) {
+  using S = Shape<T, TM, RP>;
+  const auto kern = adapters_kernel<T, TM, RP, BACK>;
+  static std::atomic<int> set[64];
+  B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, S::smem));
+  // CTAs of a tile: as many as fill the machine twice over, with a chunk of the longer product for each
+  int c = 1;
+  const int chunks = std::max(ceil_div(g.K, S::KC), ceil_div(g.N, S::KC));
+  while (c < 8 && tiles * c < 2 * sms() && 2 * c <= chunks) c *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)tiles * c);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = c;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  B200CP_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, g));
+  B200CP_LAUNCH_OK("adapters_kernel");
+  return B200CP_OK;
+}
+template <typename T, bool BACK>
+int launch_rank(const Args& g, const Plan& p, cudaStream_t st) {
+#define RANK(RP) return p.tm == 64 ? launch_tiles<T, 64, RP, BACK>(g, p.tiles, st) : launch_tiles<T, 16, RP, BACK>(g, p.tiles, st)
+  if (g.R <= 16) RANK(16);
+  if (g.R <= 32) RANK(32);
+  if (g.R <= 64) RANK(64);
+  RANK(128);
+#undef RANK
+}
+int padded(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
+int ranges_of(int rows, int I, int O, int type) {
+  const int lt = type == B200CP_FLOAT32 ? 64 : 128, kt = type == B200CP_FLOAT32 ? 32 : 64;
+  const int tiles = ceil_div(I, lt) + ceil_div(O, lt);
+  return std::max(1, std::min(ceil_div(4 * 148, tiles), ceil_div(rows, kt)));
+}
+template <typename T, int RP>
+int launch_grads(const GradArgs& g, cudaStream_t st) {
+  using S = GradShape<T, RP>;
+  static std::atomic<int> set[64];
+  const int tiles = g.tiles_i + (g.dB ? ceil_div(g.O, S::LT) : 0);
+  if (g.rows) {
+    const auto kern = adapter_grads_kernel<T, RP>;
+    B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, S::smem));
+    B200CP_CUDA_OK(launch_kernel(kern, dim3(tiles, g.ranges), dim3(kThreads), S::smem, st, true, g));
+    B200CP_LAUNCH_OK("adapter_grads_kernel");
+  }
+  const long n = (long)g.R * ((g.dA ? g.I : 0) + (g.dB ? g.O : 0));
+  const int per = (int)std::min<long>(65535, std::min<long>((n + 4 * kThreads - 1) / (4 * kThreads), std::max(1, 16 * 148 / g.count)));
+  B200CP_CUDA_OK(launch_kernel(join_grads_kernel<T, RP>, dim3(g.count, per), dim3(kThreads), 0, st, true, g));
+  B200CP_LAUNCH_OK("join_grads_kernel");
+  return B200CP_OK;
+}
+template <typename T>
+int launch_grads_rank(const GradArgs& g, cudaStream_t st) {
+  switch (padded(g.R)) {
+    case 16: return launch_grads<T, 16>(g, st);
+    case 32: return launch_grads<T, 32>(g, st);
+    case 64: return launch_grads<T, 64>(g, st);
+    default: return launch_grads<T, 128>(g, st);
+  }
+}
+int check_sizes(const char* who, int rows, int I, int O, int R, int count, int type) {
+  if (rows < 0 || I < 1 || O < 1 || R < 1 || count < 1)
+    return fail(B200CP_ERR_INVALID_ARG, "%s: rows=%d I=%d O=%d R=%d count=%d", who, rows, I, O, R, count);
+  if (type != B200CP_FLOAT32 && type != B200CP_BFLOAT16 && type != B200CP_FLOAT16)
+    return fail(B200CP_ERR_INVALID_ARG, "%s: type %d", who, type);
+  if (R > kMostRank || count > kMostAdapters || rows > (1 << 28) || I > (1 << 28) || O > (1 << 28))
+    return fail(B200CP_ERR_UNSUPPORTED, "%s: rank %d (at most %d), %d adapters (at most %d), %d rows, %d and %d features (at most 2^28)", who, R,
+                kMostRank, count, kMostAdapters, rows, I, O);
+  return B200CP_OK;
+}
+void plan_into(const int* plan, const Plan& p, const int** head, const int** start, const int** order) {
+  *head = plan;
+  *start = plan + p.start;
+  *order = plan + p.order;
+}
+template <bool BACK>
+int run_tiles(int type, Args& g, const Plan& p, const int* plan, cudaStream_t st) {
+  const size_t size = type == B200CP_FLOAT32 ? 4 : 2;
+  plan_into(plan, p, &g.head, &g.start, &g.order);
+  g.tile_adapter = plan + p.adapter;
+  g.tile_first = plan + p.first;
+  g.vx = rows16(g.X, g.K * size);
+  g.vy = rows16(g.out, g.N * size) && (!g.Y || rows16(g.Y, g.N * size));
+  g.v1 = rows16(g.F1, (BACK ? g.K : g.R) * size) && (size_t)g.K * g.R * size % 16 == 0;
+  g.v2 = rows16(g.F2, (BACK ? g.R : g.N) * size) && (size_t)g.N * g.R * size % 16 == 0;
+  if (type == B200CP_FLOAT32) return launch_rank<float, BACK>(g, p, st);
+  if (type == B200CP_BFLOAT16) return launch_rank<__nv_bfloat16, BACK>(g, p, st);
+  return launch_rank<__half, BACK>(g, p, st);
+}
+size_t w_bytes(int rows, int R, int type) { return align_up((size_t)rows * R * (type == B200CP_FLOAT32 ? 4 : 2), 256); }
+
+}  // namespace
+}  // namespace b200cp
+
+using namespace b200cp;
+
+extern "C" {
+
+size_t b200cp_adapter_plan_bytes(int rows, int count) {
+  if (rows < 0 || count < 1 || count > kMostAdapters || rows > (1 << 28)) return 0;
+  return plan_of(rows, count).ints * sizeof(int);
+}
+
+int b200cp_adapter_plan(int rows, int count, const int* adapters, void* plan, size_t plan_bytes, void* stream) {
+  const size_t need = b200cp_adapter_plan_bytes(rows, count);
+  if (!need) return fail(B200CP_ERR_INVALID_ARG, "b200cp_adapter_plan: %d rows, %d adapters (1 to %d)", rows, count, kMostAdapters);
+  if ((rows && !adapters) || !plan) return fail(B200CP_ERR_INVALID_ARG, "b200cp_adapter_plan: null pointer");
+  if (plan_bytes < need || (reinterpret_cast<uintptr_t>(plan) & 15))
+    return fail(B200CP_ERR_WORKSPACE, "b200cp_adapter_plan: a 16-byte aligned plan of %zu bytes is needed, %zu given", need, plan_bytes);
+  const Plan p = plan_of(rows, count);
+  const int keys = count + 1;
+  const int sorters = std::max(1, std::min({32, ceil_div(std::max(rows, 1), 32), 40000 / keys - 1}));   // counts: at most 156 KB
+  const size_t smem = ((size_t)keys * sorters + keys + 1) * sizeof(int);
+  static std::atomic<int> set[64];
+  B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(plan_kernel), set, (int)smem));
+  plan_kernel<<<1, 1024, smem, static_cast<cudaStream_t>(stream)>>>(rows, count, p.tm, sorters, adapters, static_cast<int*>(plan), p.adapter, p.first,
+                                                                    p.order);
+  B200CP_LAUNCH_OK("plan_kernel");
+  return B200CP_OK;
+}
+
+int b200cp_dense_adapters(int rows, int I, int O, int R, int count, int type, const void* Y, const void* X, const void* A, const void* B,
+                          const float* scale, const void* plan, void* out, void* V, void* stream) {
+  if (int rc = check_sizes("b200cp_dense_adapters", rows, I, O, R, count, type)) return rc;
+  if (rows == 0) return B200CP_OK;
+  if (!Y || !X || !A || !B || !plan || !out) return fail(B200CP_ERR_INVALID_ARG, "b200cp_dense_adapters: null pointer");
+  Args g{};
+  g.rows = rows; g.K = I; g.N = O; g.R = R; g.count = count;
+  g.X = X; g.Y = Y; g.F1 = A; g.F2 = B; g.scale = scale; g.out = out; g.V = V;
+  return run_tiles<false>(type, g, plan_of(rows, count), static_cast<const int*>(plan), static_cast<cudaStream_t>(stream));
+}
+
+size_t b200cp_dense_adapters_bwd_workspace_bytes(int rows, int I, int O, int R, int count, int type) {
+  if (check_sizes("b200cp_dense_adapters_bwd_workspace_bytes", rows, I, O, R, count, type)) return 0;
+  return w_bytes(rows, R, type) + (size_t)ranges_of(rows, I, O, type) * 2 * ((size_t)I + O) * padded(R) * sizeof(float);
+}
+
+int b200cp_dense_adapters_bwd(int rows, int I, int O, int R, int count, int type, const void* dY, const void* X, const void* V,
+                              const void* A, const void* B, const float* scale, const void* plan, void* dX, void* dA, void* dB,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "b200cp_dense_adapters_bwd";
+  if (int rc = check_sizes(who, rows, I, O, R, count, type)) return rc;
+  if (!plan || (rows && (!dY || ((dX || dA) && (!A || !B)) || (dA && !X) || (dB && !V)))) return fail(B200CP_ERR_INVALID_ARG, "%s: null pointer", who);
+  const size_t need = b200cp_dense_adapters_bwd_workspace_bytes(rows, I, O, R, count, type);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(B200CP_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, %zu given", who, need, workspace_bytes);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const Plan p = plan_of(rows, count);
+  const size_t size = type == B200CP_FLOAT32 ? 4 : 2;
+  void* W = workspace;
+  if (rows && (dX || dA)) {
+    Args g{};
+    g.rows = rows; g.K = O; g.N = dX ? I : 0; g.R = R; g.count = count;
+    g.X = dY; g.F1 = B; g.F2 = A; g.scale = scale; g.out = dX; g.V = W;
+    if (int rc = run_tiles<true>(type, g, p, static_cast<const int*>(plan), st)) return rc;
+  }
+  if (!dA && !dB) return B200CP_OK;
+  GradArgs g{};
+  g.rows = rows; g.I = I; g.O = O; g.R = R; g.count = count; g.ranges = ranges_of(rows, I, O, type);
+  g.tiles_i = dA ? ceil_div(I, type == B200CP_FLOAT32 ? 64 : 128) : 0;
+  g.X = X; g.W = W; g.V = V; g.dY = dY; g.dA = dA; g.dB = dB;
+  plan_into(static_cast<const int*>(plan), p, &g.head, &g.start, &g.order);
+  g.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + w_bytes(rows, R, type));
+  g.vx = rows16(X, I * size);
+  g.vy = rows16(dY, O * size);
+  g.vr = rows16(V, R * size) && R * size % 16 == 0;
+  if (type == B200CP_FLOAT32) return launch_grads_rank<float>(g, st);
+  if (type == B200CP_BFLOAT16) return launch_grads_rank<__nv_bfloat16>(g, st);
+  return launch_grads_rank<__half>(g, st);
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-// Bindings of the operators that stand beside the factored layers: the AdamW step.
+// Bindings of the operators that stand beside the factored layers: low-rank adapters and the AdamW step.
 // Part of torch_binding.cpp's namespace, whose helpers it uses.
 
 // ---- types ------------------------------------------------------------------------------------------------------------
@@ -24,6 +24,204 @@ double float_arg(PyObject* o) {
 // an operand that is written in place, as autograd has to know it
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+inline Tensor empty_as(at::IntArrayRef size, const Tensor& like) {
+  return at::detail::empty_cuda(size, like.scalar_type(), like.device(), std::nullopt);
+}
+Tensor contiguous(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+Tensor bytes_on(size_t n, const Tensor& like) {
+  return at::detail::empty_cuda({(int64_t)std::max<size_t>(n, 16)}, at::kByte, like.device(), std::nullopt);
+}
+int size_arg(int64_t n, const char* name) {
+  TORCH_CHECK_VALUE(n <= 0x7fffffff, name, " is ", n, ", at most 2**31 - 1 is possible");
+  return (int)n;
+}
+
+// ---- low-rank adapters ------------------------------------------------------------------------------------------------
+// The plan of a batch: bytes on the device that depend on the rows' adapters and on the number of adapters
+Tensor adapter_plan(const Tensor& which_, int64_t count) {
+  TORCH_CHECK_TYPE(which_.scalar_type() == at::kInt || which_.scalar_type() == at::kLong, "adapters must be an int32 or int64 CUDA tensor");
+  const int rows = size_arg(which_.numel(), "the number of rows"), n = size_arg(count, "the number of adapters");
+  const size_t need = b200cp_adapter_plan_bytes(rows, n);
+  TORCH_CHECK_VALUE(need, "adapter_plan: ", rows, " rows and ", n, " adapters (1 to 16384 of them)");
+  const c10::cuda::OptionalCUDAGuard guard(which_.device());
+  const Tensor which = contiguous(which_.scalar_type() == at::kInt ? which_ : which_.clamp(-1, count).to(at::kInt));
+  Tensor plan = bytes_on(need, which);
+  ok(b200cp_adapter_plan(rows, n, static_cast<const int*>(which.const_data_ptr()), plan.data_ptr(), need, stream(which)));
+  return plan;
+}
+struct Adapters {   // operands, checked and contiguous
+  Tensor x, A, B, scale;
+  int rows, I, O, R, count, type;
+  Adapters(const Tensor& x_, const Tensor& A_, const Tensor& B_, const Tensor& scale_) {
+    type = type_of(x_, "X");
+    TORCH_CHECK_VALUE(x_.dim() >= 1 && A_.dim() == 3 && B_.dim() == 3, "expected X [..., I], A [count, I, R] and B [count, R, O]");
+    TORCH_CHECK_VALUE(A_.size(1) == x_.size(-1) && B_.size(0) == A_.size(0) && B_.size(1) == A_.size(2), "A ", A_.sizes(), " and B ", B_.sizes(),
+                      " do not go with X ", x_.sizes());
+    for (const Tensor* t : {&A_, &B_}) same(*t, x_, t == &A_ ? "A" : "B");
+    I = size_arg(A_.size(1), "I");
+    R = size_arg(A_.size(2), "the rank");
+    O = size_arg(B_.size(2), "O");
+    count = size_arg(A_.size(0), "the number of adapters");
+    TORCH_CHECK_VALUE(I > 0 && O > 0 && R > 0 && count > 0, "A and B may not be empty");
+    rows = size_arg(x_.numel() / I, "the number of rows");
+    if (scale_.defined()) {
+      TORCH_CHECK_TYPE(scale_.is_cuda() && scale_.scalar_type() == at::kFloat, "scale must be a float32 CUDA tensor");
+      TORCH_CHECK_VALUE(scale_.device() == x_.device() && scale_.numel() == count, "scale has to have a value per adapter, on X's device");
+      scale = contiguous(scale_);
+    }
+    x = contiguous(x_);
+    A = contiguous(A_);
+    B = contiguous(B_);
+  }
+  static void same(const Tensor& t, const Tensor& like, const char* name) {
+    TORCH_CHECK_TYPE(t.is_cuda() && t.scalar_type() == like.scalar_type(), name, " must be a CUDA tensor of X's type, ", like.scalar_type());
+    TORCH_CHECK_VALUE(t.device() == like.device(), name, " is on ", t.device(), ", X on ", like.device());
+  }
+  void fits(const Tensor& y, const char* name) const {
+    same(y, x, name);
+    TORCH_CHECK_VALUE(y.dim() == x.dim() && y.size(-1) == O && y.sizes().slice(0, y.dim() - 1) == x.sizes().slice(0, x.dim() - 1), name, " is ",
+                      y.sizes(), " where X is ", x.sizes(), " and B has ", O, " columns");
+  }
+  // `which`: the adapter of every row, or (planned) the bytes of a plan
+  Tensor plan(const Tensor& which, bool planned) const {
+    TORCH_CHECK_VALUE(which.device() == x.device(), "the adapters' numbers are on ", which.device(), ", X on ", x.device());
+    if (!planned) {
+      TORCH_CHECK_VALUE(which.sizes() == x.sizes().slice(0, x.dim() - 1), "there are numbers of adapters for ", which.sizes(), ", X is ", x.sizes());
+      return adapter_plan(which, count);
+    }
+    TORCH_CHECK_VALUE(which.scalar_type() == at::kByte && which.is_contiguous() &&
+                          (size_t)which.numel() == std::max<size_t>(16, b200cp_adapter_plan_bytes(rows, count)),
+                      "the plan is not one of ", rows, " rows and ", count, " adapters");
+    return which;
+  }
+  void takes(const Tensor& out, const Tensor& y) const {   // as the place of the result
+    fits(out, "out");
+    TORCH_CHECK_VALUE(out.is_contiguous(), "out has to be contiguous");
+    for (const Tensor* t : {&x, &A, &B}) TORCH_CHECK_VALUE(!t->is_alias_of(out), "out may share memory with Y alone");
+    TORCH_CHECK_VALUE(!y.is_alias_of(out) || (y.is_contiguous() && y.const_data_ptr() == out.const_data_ptr()),
+                      "out may be Y, but not another part or order of its memory");
+  }
+  const float* scales() const { return scale.defined() ? cp(scale) : nullptr; }
+};
+Tensor dense_adapters(const Adapters& a, const Tensor& y_, const Tensor& plan, Tensor out, Tensor* V) {
+  a.fits(y_, "Y");
+  const Tensor y = contiguous(y_);
+  if (!out.defined()) out = empty_as(y.sizes(), y);
+  const c10::cuda::OptionalCUDAGuard guard(a.x.device());
+  if (V) *V = empty_as({a.rows, a.R}, a.x);
+  ok(b200cp_dense_adapters(a.rows, a.I, a.O, a.R, a.count, a.type, y.const_data_ptr(), a.x.const_data_ptr(), a.A.const_data_ptr(), a.B.const_data_ptr(),
+                           a.scales(), plan.const_data_ptr(), out.data_ptr(), V ? V->data_ptr() : nullptr, stream(a.x)));
+  return out;
+}
+std::array<Tensor, 3> dense_adapters_backward(const Adapters& a, const Tensor& dy_, const Tensor& V, const Tensor& plan, bool need_x, bool need_a,
+                                              bool need_b) {
+  std::array<Tensor, 3> g;
+  a.fits(dy_, "dY");
+  const Tensor dy = contiguous(dy_);
+  const c10::cuda::OptionalCUDAGuard guard(a.x.device());
+  if (need_x) g[0] = empty_as(a.x.sizes(), a.x);
+  if (need_a) g[1] = empty_as(a.A.sizes(), a.x);
+  if (need_b) g[2] = empty_as(a.B.sizes(), a.x);
+  const Tensor ws = bytes_on(b200cp_dense_adapters_bwd_workspace_bytes(a.rows, a.I, a.O, a.R, a.count, a.type), a.x);
+  const auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  ok(b200cp_dense_adapters_bwd(a.rows, a.I, a.O, a.R, a.count, a.type, dy.const_data_ptr(), a.x.const_data_ptr(), V.const_data_ptr(),
+                               a.A.const_data_ptr(), a.B.const_data_ptr(), a.scales(), plan.const_data_ptr(), at(g[0]), at(g[1]), at(g[2]),
+                               ws.data_ptr(), (size_t)ws.numel(), stream(a.x)));
+  return g;
+}
+struct AdaptersNode : torch::autograd::Function<AdaptersNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& x, const Tensor& A, const Tensor& B, const Tensor& plan,
+                        const std::optional<Tensor>& scale_) {
+    const Tensor scale = scale_.value_or(Tensor());
+    const Adapters a(x, A, B, scale);
+    Tensor V;
+    Tensor out = dense_adapters(a, y, plan, Tensor(), &V);
+    ctx->save_for_backward({x, A, B, plan, scale, V});
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list v = ctx->get_saved_variables();
+    variable_list out(6);
+    if (ctx->needs_input_grad(0)) out[0] = grads[0];
+    const bool need_x = ctx->needs_input_grad(1), need_a = ctx->needs_input_grad(2), need_b = ctx->needs_input_grad(3);
+    if (need_x || need_a || need_b) {
+      const Adapters a(v[0], v[1], v[2], v[4]);
+      const std::array<Tensor, 3> g = dense_adapters_backward(a, grads[0], v[5], v[3], need_x, need_a, need_b);
+      for (int i = 0; i < 3; ++i) out[1 + i] = g[i];
+    }
+    return out;
+  }
+};
+
+Tensor optional_tensor(PyObject* o, const char* name) { return o == Py_None ? Tensor() : any_tensor(o, name); }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
+  return v != 0;
+}
+PYFN(py_adapter_plan) {
+  HANDLE_TH_ERRORS
+  count_args(n, 2);
+  const Tensor& which = any_tensor(a[0], "adapters");
+  const int64_t count = int_arg(a[1]);
+  return wrap(unlocked([&] { return adapter_plan(which, count); }));
+  END_HANDLE_TH_ERRORS
+}
+// (Y, X, A, B, which, planned, scale or None, out or None)
+PYFN(py_dense_adapters) {
+  HANDLE_TH_ERRORS
+  count_args(n, 8);
+  const Tensor &y = any_tensor(a[0], "Y"), &x = any_tensor(a[1], "X"), &A = any_tensor(a[2], "A"), &B = any_tensor(a[3], "B"),
+               &which = any_tensor(a[4], "adapters");
+  const bool planned = truth(a[5]);
+  const Tensor scale = optional_tensor(a[6], "scale"), to = optional_tensor(a[7], "out");
+  Tensor out = unlocked([&] {
+    const Adapters op(x, A, B, scale);
+    op.fits(y, "Y");
+    if (to.defined()) op.takes(to, y);
+    return dense_adapters(op, y, op.plan(which, planned), to, nullptr);
+  });
+  if (to.defined()) written(to);
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+// (dY, X, V, A, B, plan, scale or None, need_dx, need_da, need_db)
+PYFN(py_dense_adapters_backward) {
+  HANDLE_TH_ERRORS
+  count_args(n, 10);
+  const Tensor &dy = any_tensor(a[0], "dY"), &x = any_tensor(a[1], "X"), &V_ = any_tensor(a[2], "V"), &A = any_tensor(a[3], "A"),
+               &B = any_tensor(a[4], "B"), &plan = any_tensor(a[5], "plan");
+  const Tensor scale = optional_tensor(a[6], "scale");
+  const bool nx = truth(a[7]), na = truth(a[8]), nb = truth(a[9]);
+  return wrap_tuple(unlocked([&] {
+    const Adapters op(x, A, B, scale);
+    Adapters::same(V_, x, "V");
+    TORCH_CHECK_VALUE(V_.numel() == (int64_t)op.rows * op.R, "V has ", V_.numel(), " values, ", op.rows, " rows of rank ", op.R, " are needed");
+    return dense_adapters_backward(op, dy, contiguous(V_), op.plan(plan, true), nx, na, nb);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+// (y, x, A, B, which, planned, scale or None)
+PYFN(py_adapters_apply) {
+  HANDLE_TH_ERRORS
+  count_args(n, 7);
+  const Tensor &y = any_tensor(a[0], "Y"), &x = any_tensor(a[1], "X"), &A = any_tensor(a[2], "A"), &B = any_tensor(a[3], "B"),
+               &which = any_tensor(a[4], "adapters");
+  const bool planned = truth(a[5]);
+  const Tensor scale = optional_tensor(a[6], "scale");
+  return wrap(unlocked([&] {
+    Tensor plan;
+    {
+      at::NoGradGuard none;
+      const Adapters op(x, A, B, scale);
+      op.fits(y, "Y");
+      plan = op.plan(which, planned);
+    }
+    return AdaptersNode::apply(y, x, A, B, plan, scale.defined() ? std::optional<Tensor>(scale) : std::nullopt);
+  }));
+  END_HANDLE_TH_ERRORS
 }
 
 // ---- AdamW step -----------------------------------------------------------------------------------------------------------

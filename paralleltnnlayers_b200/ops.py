@@ -393,6 +393,51 @@ def dense_cp_rebuild(U, *kernels):
     return dense_matmul(U, dense_cp_recompose(*kernels))
 
 
+# ---- low-rank adapters of many requests beside a shared projection ---------------
+class AdapterPlan:
+    """The rows of a batch in the order of their adapters, made once and used by every layer that the batch meets.
+
+    ``adapters``: int32 (or int64) CUDA tensor with the adapter of each row, ``0 .. count - 1``; any other number: none.  Its values are
+    taken over at this call; what they become later does not change the plan."""
+
+    def __init__(self, adapters, count):
+        self.data, self.shape, self.count = _C.adapter_plan(adapters, count), tuple(adapters.shape), count
+
+
+def adapter_plan(adapters, count):
+    """``AdapterPlan(adapters, count)``."""
+    return AdapterPlan(adapters, count)
+
+
+def _which(adapters, X):
+    """The operand for the binding, and whether it is a plan."""
+    if not isinstance(adapters, AdapterPlan):
+        return adapters, False
+    if adapters.shape != tuple(X.shape[:-1]):
+        raise ValueError(f"the plan is of rows {adapters.shape}, the input of {tuple(X.shape[:-1])}")
+    return adapters.data, True
+
+
+def dense_adapters(Y, X, A, B, adapters, scale=None, out=None):
+    """``out[s] = Y[s] + scale[a] (X[s] A[a]) B[a]``, ``a`` the adapter of row ``s``: what a shared projection gave for a batch of many requests,
+    corrected for each by its own low-rank adapter (``b200cp_dense_adapters``).  Rows without an adapter come out as ``Y``.
+
+    ``X [..., I]``, ``Y [..., O]``, ``A [count, I, R]``, ``B [count, R, O]`` of one type: float32, bfloat16 or float16 (sums in float32; ``X A`` is
+    rounded to the type before the second product); ``R`` at most 128.  ``adapters``: an int32 or int64 tensor of ``X``'s leading shape, or
+    the ``AdapterPlan`` of one.  ``scale``: float32 per adapter.  ``out`` may be ``Y``."""
+    which, planned = _which(adapters, X)
+    return _C.dense_adapters(Y, X, A, B, which, planned, scale, out)
+
+
+def dense_adapters_backward(dY, X, V, A, B, plan, scale=None, need_dx=True, need_da=True, need_db=True):
+    """Gradients of ``dense_adapters``: (dX, dA, dB), None where not needed; ``dY`` itself is that of ``Y``.  ``V``: ``scale (X A)`` of each
+    row, rounded to the type of ``X`` (rows without an adapter: any finite or other values, they are not read)."""
+    which, planned = _which(plan, X)
+    if not planned:
+        raise TypeError("dense_adapters_backward takes the AdapterPlan of the forward")
+    return _C.dense_adapters_backward(dY, X, V, A, B, which, scale, need_dx, need_da, need_db)
+
+
 # ---- AdamW step -----------------------------------------------------------------
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, master=None, scales=None):
     """One AdamW step over all tensors of the lists, in place and in one launch (``b200cp_adamw_step``):
@@ -433,3 +478,12 @@ class RCPConv2dFunction:
 class CPDenseFunction:
     """y = CP dense(x; F...): ``apply(x, K0, K1, ...)``."""
     apply = staticmethod(_C.dense_apply)
+
+
+class DenseAdaptersFunction:
+    """``dense_adapters`` with its gradients: ``apply(y, x, A, B, adapters, scale=None)``; ``scale`` has none."""
+
+    @staticmethod
+    def apply(y, x, A, B, adapters, scale=None):
+        which, planned = _which(adapters, x)
+        return _C.adapters_apply(y, x, A, B, which, planned, scale)

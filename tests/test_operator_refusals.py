@@ -64,3 +64,58 @@ def test_adamw_refuses_rates_out_of_range(lib_built):
     for bad in (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(bits=4), dict(eps=-1.0), dict(weight_decay=-1.0)):
         with pytest.raises(ValueError):
             AdamW(p, **bad)
+
+
+ADAPTERS = {
+    "x type": (TypeError, lambda c: (c(2, 4), c(2, 8, dtype=torch.float64), c(3, 8, 2), c(3, 2, 4), c(2, dtype=torch.int32))),
+    "y type": (TypeError, lambda c: (c(2, 4), c(2, 8, dtype=torch.float16), c(3, 8, 2, dtype=torch.float16), c(3, 2, 4, dtype=torch.float16), c(2, dtype=torch.int32))),
+    "A type": (TypeError, lambda c: (c(2, 4), c(2, 8), c(3, 8, 2, dtype=torch.bfloat16), c(3, 2, 4), c(2, dtype=torch.int32))),
+    "A features": (ValueError, lambda c: (c(2, 4), c(2, 8), c(3, 7, 2), c(3, 2, 4), c(2, dtype=torch.int32))),
+    "rank": (ValueError, lambda c: (c(2, 4), c(2, 8), c(3, 8, 2), c(3, 3, 4), c(2, dtype=torch.int32))),
+    "count": (ValueError, lambda c: (c(2, 4), c(2, 8), c(3, 8, 2), c(4, 2, 4), c(2, dtype=torch.int32))),
+    "y features": (ValueError, lambda c: (c(2, 5), c(2, 8), c(3, 8, 2), c(3, 2, 4), c(2, dtype=torch.int32))),
+    "y rows": (ValueError, lambda c: (c(3, 4), c(2, 8), c(3, 8, 2), c(3, 2, 4), c(2, dtype=torch.int32))),
+    "numbers": (ValueError, lambda c: (c(2, 4), c(2, 8), c(3, 8, 2), c(3, 2, 4), c(3, dtype=torch.int32))),
+    "numbers type": (TypeError, lambda c: (c(2, 4), c(2, 8), c(3, 8, 2), c(3, 2, 4), c(2))),
+    "numbers device": (ValueError, lambda c: (c(2, 4), c(2, 8), c(3, 8, 2), c(3, 2, 4), c(2, dtype=torch.int32, dev=1))),
+    "B device": (ValueError, lambda c: (c(2, 4), c(2, 8), c(3, 8, 2), c(3, 2, 4, dev=1), c(2, dtype=torch.int32))),
+    "scale size": (ValueError, lambda c: (c(2, 4), c(2, 8), c(3, 8, 2), c(3, 2, 4), c(2, dtype=torch.int32), c(2))),
+    "scale type": (TypeError, lambda c: (c(2, 4), c(2, 8), c(3, 8, 2), c(3, 2, 4), c(2, dtype=torch.int32), c(3, dtype=torch.float16))),
+    "empty": (ValueError, lambda c: (c(2, 4), c(2, 8), c(0, 8, 2), c(0, 2, 4), c(2, dtype=torch.int32))),
+    "not a tensor": (TypeError, lambda c: (c(2, 4), None, c(3, 8, 2), c(3, 2, 4), c(2, dtype=torch.int32))),
+}
+
+
+@pytest.mark.parametrize("what", ADAPTERS)
+def test_adapters_refuse(fake, what):
+    import paralleltnnlayers_b200 as P
+    error, args = ADAPTERS[what]
+    with pytest.raises(error):
+        P.dense_adapters(*args(fake))
+    with pytest.raises(error):
+        P.DenseAdaptersFunction.apply(*args(fake))
+
+
+def test_adapters_refuse_an_out_that_does_not_fit(fake):
+    import paralleltnnlayers_b200 as P
+    args = (fake(2, 4), fake(2, 4), fake(3, 4, 2), fake(3, 2, 4), fake(2, dtype=torch.int32))
+    for out in (fake(3, 4), fake(2, 4, dtype=torch.float16), fake(2, 4, dev=1)):
+        with pytest.raises((TypeError, ValueError)):
+            P.dense_adapters(*args, out=out)
+
+
+def test_adapter_sizes_the_library_refuses(lib_built):
+    from paralleltnnlayers_b200 import _lib
+    lib = _lib.lib
+    assert lib.b200cp_adapter_plan_bytes(4, 0) == 0 and lib.b200cp_adapter_plan_bytes(4, 16385) == 0 and lib.b200cp_adapter_plan_bytes(-1, 3) == 0
+    assert lib.b200cp_adapter_plan_bytes(0, 1) > 0
+    assert lib.b200cp_adapter_plan(4, 3, None, None, 0, None) == -1
+    assert lib.b200cp_adapter_plan(4, 3, 16, 16, 8, None) == -3        # too small a plan
+    assert lib.b200cp_adapter_plan(4, 3, 16, 24, 1 << 20, None) == -3  # not on sixteen bytes
+    fwd = lambda *a: lib.b200cp_dense_adapters(*a, *[16] * 4, None, 16, 16, None, None)  # noqa: E731
+    assert fwd(0, 4, 4, 4, 1, 0) == 0
+    assert fwd(4, 4, 4, 129, 1, 0) == -2 and fwd(4, 4, 4, 4, 16385, 0) == -2
+    assert fwd(4, 0, 4, 4, 1, 0) == -1 and fwd(4, 4, 4, 4, 1, 3) == -1 and fwd(-1, 4, 4, 4, 1, 0) == -1
+    assert lib.b200cp_dense_adapters(4, 4, 4, 4, 1, 0, *[None] * 9) == -1
+    assert lib.b200cp_dense_adapters_bwd(4, 4, 4, 4, 1, 0, *[16] * 5, None, 16, 16, 16, 16, 16, 4, None) == -3
+    assert lib.b200cp_dense_adapters_bwd(4, 4, 4, 4, 1, 0, *[None] * 5, None, 16, 16, 16, 16, 16, 1 << 20, None) == -1
