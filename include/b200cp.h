@@ -427,6 +427,24 @@ int b200cp_dense_adapters_bwd(int rows, int I, int O, int R, int count, int type
                               const void* A, const void* B, const float* scale, const void* plan, void* dX, void* dA, void* dB,
                               void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- gated feed-forward block ------------------------------------------------------------------------------ */
+
+enum { B200CP_SILU = 0, B200CP_GELU = 1, B200CP_GELU_TANH = 2 };
+
+/* H = act(X Wg) * (X Wu), elementwise product, both projections in one kernel.  X [rows, I], Wg, Wu [I, F], H [rows, F] of one 16-bit
+ * type (B200CP_BFLOAT16 or _FLOAT16); sums are fp32.  G, U (both or neither): [rows, F] floats, receive X Wg and X Wu for the
+ * backward.  The workspace is 256-byte aligned (and may be NULL where the size is 0).  Beside b200cp_dense_matmul; no counterpart in the reference. */
+size_t b200cp_dense_gated_workspace_bytes(int rows, int I, int F, int type);
+int b200cp_dense_gated(int rows, int I, int F, int type, int activation, const void* X, const void* Wg, const void* Wu, void* H, float* G,
+                       float* U, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dG = dH * U * act'(G), dU = dH * act(G) (rounded to the 16-bit type as operands), dX = dG Wg^T + dU Wu^T, dWg = X^T dG, dWu = X^T dU.
+ * dX may be NULL, and so may dWg and dWu together. */
+size_t b200cp_dense_gated_bwd_workspace_bytes(int rows, int I, int F, int type);
+int b200cp_dense_gated_bwd(int rows, int I, int F, int type, int activation, const void* X, const void* Wg, const void* Wu, const float* G,
+                           const float* U, const void* dH, void* dX, void* dWg, void* dWu, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 /* ---- misc --------------------------------------------------------------- */
 
 /* Synchronises the device and reports whether any tensor-path kernel gave up a bounded wait since

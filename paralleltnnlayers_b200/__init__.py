@@ -20,7 +20,8 @@ _OPS_NAMES = ("allclose", "CP3Conv2dFunction", "conv2d_cp_fused_nchw", "cp3_conv
               "conv2d_dense_forward", "cp4_conv2d_forward_backward_data", "cp4_conv2d_backward_filter_saved",
               "cp4_conv2d_forward_save", "cp4_conv2d_backward_data_save", "cp4_conv2d_rebuild_forward", "rcp_recompose", "conv2d_rcp_rebuild_nchw",
               "dense_cp_recompose", "dense_matmul", "dense_cp_rebuild", "adamw_step", "adamw_moments",
-              "AdapterPlan", "adapter_plan", "dense_adapters", "dense_adapters_backward", "DenseAdaptersFunction")
+              "AdapterPlan", "adapter_plan", "dense_adapters", "dense_adapters_backward", "DenseAdaptersFunction",
+              "dense_gated", "dense_gated_save", "dense_gated_backward", "DenseGatedFunction")
 __all__ = list(_LIB_NAMES + _OPS_NAMES)
 
 

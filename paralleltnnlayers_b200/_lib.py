@@ -106,6 +106,10 @@ def _load():
         "b200cp_dense_adapters": (i, [i, i, i, i, i, i, vp, vp, vp, vp, fp, vp, vp, vp, vp]),
         "b200cp_dense_adapters_bwd_workspace_bytes": (sz, [i, i, i, i, i, i]),
         "b200cp_dense_adapters_bwd": (i, [i, i, i, i, i, i, vp, vp, vp, vp, vp, fp, vp, vp, vp, vp, vp, sz, vp]),
+        "b200cp_dense_gated_workspace_bytes": (sz, [i, i, i, i]),
+        "b200cp_dense_gated": (i, [i, i, i, i, i, vp, vp, vp, vp, fp, fp, vp, sz, vp]),
+        "b200cp_dense_gated_bwd_workspace_bytes": (sz, [i, i, i, i]),
+        "b200cp_dense_gated_bwd": (i, [i, i, i, i, i, vp, vp, vp, fp, fp, vp, vp, vp, vp, vp, sz, vp]),
         "b200cp_adamw_step": (i, [vp, i, i, i, i, vp, vp]),
         "b200cp_adamw_moments": (i, [C.c_ulonglong, vp, vp, fp, fp, i, vp, vp, vp]),
         "b200cp_device_status": (i, []),

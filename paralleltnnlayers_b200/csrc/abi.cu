@@ -1290,6 +1290,8 @@ int b200cp_device_status(void) {
   if (v) return fail(B200CP_ERR_TIMEOUT, "weight as operand planes: a bounded wait ran out in block %d", v & 0xffff);
   if (int rc = halves_device_status(&v)) return rc;
   if (v) return fail(B200CP_ERR_TIMEOUT, "factor contraction: a bounded wait ran out in block %d", v & 0xffff);
+  if (int rc = gated_device_status(&v)) return rc;
+  if (v) return fail(B200CP_ERR_TIMEOUT, "gated feed-forward block: a bounded wait ran out in block %d", v & 0xffff);
   return B200CP_OK;
 }
 

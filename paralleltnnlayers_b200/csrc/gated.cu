@@ -1,0 +1,541 @@
+// Gated feed-forward block: H = act(X Wg) * (X Wu) and its gradients, 16-bit operands, fp32 sums, on the tcgen05 tensor cores.
+//
+//   G = X Wg, U = X Wu, H = act(G) U;  dG = dH U act'(G), dU = dH act(G);  dX = dG Wg^T + dU Wu^T;  dWg = X^T dG, dWu = X^T dU
+//
+// One kernel in three forms.  A pair of CTAs (cta_group::2) forms 256 x 256 sums, 128 rows in each CTA's tensor memory, from a ring of 64-deep
+// steps that TMA fills; one thread issues the products, the other warps move finished sums out while the next tile's products run.
+//   forward   128 columns of G and the same 128 of U are one tile: the first CTA loads the columns of Wg, the second those of Wu, and both
+//             halves of a sum lie side by side in tensor memory, so that act(G) U is formed there and neither G nor U need leave the chip.
+//   data      dG Wg^T and dU Wu^T are one sum, twice as long.
+//   weights   X^T dG and X^T dU are two results of one launch.
+// Weights lie as [inputs][outputs] and activations as [rows][features]; tcgen05 takes either order of either operand, so nothing is transposed.
+// For the backward the forward keeps G and U in fp32 (8 bytes a value, where the 16-bit tensors that autograd would keep take 6): with 16-bit
+// copies dG and dU would carry two roundings more.  They are rounded once, as operands.
+// Rows of odd length are copied to rows of a multiple of eight values first (TMA's strides are multiples of 16 bytes).
+// Every wait is bounded: one that runs out sets a status word and the CTA leaves through its normal exit.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "tc_common.cuh"
+#include "tc_pair.cuh"
+
+namespace b200cp {
+
+__device__ int g_gated_status = 0;   // 0 ok; otherwise (code << 16) | (linear block index & 0xffff)
+
+namespace {
+
+using namespace tc;
+
+enum Form { kForward, kData, kWeights };
+constexpr int kTile = 256, kStep = 64, kHalf = 128 * kStep * 2, kStage = 2 * kHalf, kStages = 6;   // bytes: of an operand's half, of a step
+constexpr int kBox = 64 * kStep * 2;              // a box of 64 columns by 64 k
+constexpr int kReaders = 8, kThreads = 64 + 32 * kReaders;
+constexpr size_t kSmem = (size_t)kStages * kStage + 1024 + 256;
+
+struct Gemm {
+  int M, N;                      // of a result
+  int tiles_m, tiles_n, units;   // units: tiles of all results
+  int steps, first;              // of a sum; steps of its first product
+  int act;
+  void* out[2];
+  int vec;                       // rows of out start on 16-byte boundaries
+  float *G, *U;                  // forward: where the sums are kept, or null
+  int vecg;
+};
+
+__device__ __forceinline__ void tma_load_pair_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+template <typename T>
+__host__ __device__ constexpr uint32_t instruction(uint32_t m, uint32_t n, uint32_t a_mn, uint32_t b_mn) {
+  constexpr uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (bf << 7) | (bf << 10) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// ---- the activation -----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }   // (exp(-x) = inf: 0)
+constexpr float kRootHalf = 0.70710678118654752f, kRootPi = 0.79788456080286536f;   // sqrt(1/2), sqrt(2/pi)
+// act(g) = g * share; *slope = act'(g)
+template <bool SLOPE>
+__device__ __forceinline__ float gate_share(int act, float g, float* slope) {
+  if (act == B200CP_SILU) {
+    const float s = sigmoid(g);
+    if (SLOPE) *slope = s * fmaf(g, 1.f - s, 1.f);
+    return s;
+  }
+  if (act == B200CP_GELU) {
+    const float s = 0.5f * erfcf(-kRootHalf * g);   // (1 + erf would lose the left tail)
+    if (SLOPE) *slope = fmaf(g * (0.5f * kRootPi), __expf(-0.5f * g * g), s);
+    return s;
+  }
+  const float q = kRootPi * fmaf(0.044715f * g, g * g, g), s = sigmoid(2.f * q);   // (1 + tanh q) / 2
+  if (SLOPE) *slope = s * fmaf(2.f * (1.f - s) * g, kRootPi * fmaf(3.f * 0.044715f * g, g, 1.f), 1.f);
+  return s;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+// 16 values of a row from column n on (of N)
+template <typename T>
+__device__ __forceinline__ void put16(T* row, int n, int N, bool vec, const float (&v)[16]) {
+  if (vec && n + 16 <= N) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 8)
+      *reinterpret_cast<uint4*>(row + n + j) = make_uint4(pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]), pack2<T>(v[j + 4], v[j + 5]),
+                                                          pack2<T>(v[j + 6], v[j + 7]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (n + j < N) row[n + j] = (T)v[j];
+  }
+}
+__device__ __forceinline__ void put16(float* row, int n, int N, bool vec, const float (&v)[16]) {
+  if (vec && n + 16 <= N) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(row + n + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (n + j < N) row[n + j] = v[j];
+  }
+}
+
+// ---- the kernel ---------------------------------------------------------------------------------------------------------------
+struct UnitAt {
+  int m0, n0, result;
+};
+// Groups of kGroup tiles along M share the columns: their rows of A stay in L2 while the columns of B pass by once.
+constexpr int kGroup = 16;
+template <Form FORM>
+__device__ __forceinline__ UnitAt unit_at(const Gemm& g, int unit) {
+  const int per = g.tiles_m * g.tiles_n, r = unit / per, t = unit - r * per, band = t / (kGroup * g.tiles_n);
+  const int m1 = band * kGroup, height = min(kGroup, g.tiles_m - m1), q = t - m1 * g.tiles_n;
+  return UnitAt{(m1 + q % height) * kTile, (q / height) * (FORM == kForward ? kTile / 2 : kTile), r};
+}
+
+template <Form FORM, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapA1,
+             const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kStages * kStage);
+  uint64_t* full = bars;                 // [kStages] the leader's: the step of both CTAs has landed  (tx bytes)
+  uint64_t* empty = full + kStages;      // [kStages] the products that read the step are done         (commit, both CTAs)
+  uint64_t* accfull = empty + kStages;   // [2] the sums of a tile are complete                        (commit, both CTAs)
+  uint64_t* accfree = accfull + 2;       // [2] the leader's: read out by the warps of both CTAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accfree + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&accfull[i], 1);
+      mbar_init(&accfree[i], 2 * kReaders);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&mapA0);
+    tma_prefetch_desc(&mapB0);
+    if (FORM != kWeights) tma_prefetch_desc(FORM == kData ? &mapA1 : &mapB1);
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot, ring = smem_u32(sm);
+  const uint32_t fullb = smem_u32(full), emptyb = smem_u32(empty), accfullb = smem_u32(accfull), accfreeb = smem_u32(accfree),
+                 abortb = smem_u32(const_cast<int*>(abort_flag));
+  grid_dependency_wait();
+
+  if (warp == 0) {
+    // ================= TMA: this CTA's rows of A and its half of the columns of B ===========================================
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int unit = pair; unit < g.units && ok; unit += npairs) {
+        const UnitAt t = unit_at<FORM>(g, unit);
+        for (int k = 0; k < g.steps; ++k, ++it) {
+          const int slot = it % kStages;
+          if (it >= kStages && !(ok = wait_or_abort(emptyb + slot * 8, ((it / kStages) - 1) & 1, abortb))) break;
+          if (rank == 0) mbar_expect_tx(&full[slot], 2 * kStage);
+          const uint32_t bar = leader_addr(fullb + slot * 8), a = ring + slot * kStage, b = a + kHalf;
+          if (FORM == kForward) {
+            const CUtensorMap* w = rank == 0 ? &mapB0 : &mapB1;
+            tma_load_pair_2d(a, &mapA0, bar, k * kStep, t.m0 + rank * 128);
+            tma_load_pair_2d(b, w, bar, t.n0, k * kStep);
+            tma_load_pair_2d(b + kBox, w, bar, t.n0 + 64, k * kStep);
+          } else if (FORM == kData) {
+            const bool second = k >= g.first;
+            const int x = (k - (second ? g.first : 0)) * kStep;
+            tma_load_pair_2d(a, second ? &mapA1 : &mapA0, bar, x, t.m0 + rank * 128);
+            tma_load_pair_2d(b, second ? &mapB1 : &mapB0, bar, x, t.n0 + rank * 128);
+          } else {
+            const CUtensorMap* w = t.result ? &mapB1 : &mapB0;
+            tma_load_pair_2d(a, &mapA0, bar, t.m0 + rank * 128, k * kStep);
+            tma_load_pair_2d(a + kBox, &mapA0, bar, t.m0 + rank * 128 + 64, k * kStep);
+            tma_load_pair_2d(b, w, bar, t.n0 + rank * 128, k * kStep);
+            tma_load_pair_2d(b + kBox, w, bar, t.n0 + rank * 128 + 64, k * kStep);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ================= products: one thread of the pair ======================================================================
+    if (rank == 0 && elect_one()) {
+      constexpr bool a_mn = FORM == kWeights, b_mn = FORM != kData;
+      constexpr uint32_t idesc = instruction<T>(256, 256, a_mn, b_mn);
+      // K-major: rows of 128 bytes, eight rows per swizzle atom (1024 bytes); 16 k = 32 bytes on.
+      // MN-major: 64 columns (128 bytes) per k, eight k per atom, the next 64 columns a box on; 16 k = 2048 bytes on.
+      const uint64_t da = make_smem_desc(0, a_mn ? kBox : 16, 1024, kSwizzle128B), db = make_smem_desc(0, b_mn ? kBox : 16, 1024, kSwizzle128B);
+      constexpr uint64_t sa = (a_mn ? 2048 : 32) >> 4, sb = (b_mn ? 2048 : 32) >> 4;
+      int it = 0, done = 0;
+      bool ok = true;
+      for (int unit = pair; unit < g.units && ok; unit += npairs, ++done) {
+        const int buf = done & 1;
+        if (done >= 2 && !(ok = wait_or_abort(accfreeb + buf * 8, (done / 2 - 1) & 1, abortb))) break;
+        tc_fence_after_sync();
+        const uint32_t d = tmem_base + buf * 256;
+        for (int k = 0; k < g.steps; ++k, ++it) {
+          const int slot = it % kStages;
+          if (!(ok = wait_or_abort(fullb + slot * 8, (it / kStages) & 1, abortb))) break;
+          tc_fence_after_sync();
+          const uint32_t a = ring + slot * kStage;
+          const uint64_t ad = da + (a >> 4), bd = db + ((a + kHalf) >> 4);
+#pragma unroll
+          for (int i = 0; i < kStep / 16; ++i) mma_f16_pair(d, ad + i * sa, bd + i * sb, idesc, k > 0 || i > 0);
+          commit_pair(emptyb + slot * 8);
+        }
+        if (ok) commit_pair(accfullb + buf * 8);
+      }
+    }
+  } else {
+    // ================= read-out ===============================================================================================
+    const int qd = warp & 3, half = (warp - 2) >> 2;   // the lane quarter that this warp may read, and its half of the columns
+    int done = 0;
+    for (int unit = pair; unit < g.units; unit += npairs, ++done) {
+      const UnitAt t = unit_at<FORM>(g, unit);
+      const int buf = done & 1;
+      if (!__all_sync(0xffffffffu, wait_or_abort(accfullb + buf * 8, (done / 2) & 1, abortb))) break;
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + ((uint32_t)(qd * 32) << 16) + buf * 256;
+      const int m = t.m0 + rank * 128 + qd * 32 + lane;
+      const bool in = m < g.M;
+      if (FORM == kForward) {
+        const size_t row = (size_t)m * g.N;
+#pragma unroll 1
+        for (int j = half * 64; j < half * 64 + 64 && t.n0 + j < g.N; j += 16) {
+          float a[16], u[16];
+          tmem_ld16(taddr + j, a);
+          tmem_ld16(taddr + 128 + j, u);
+          if (in && g.G) {
+            put16(g.G + row, t.n0 + j, g.N, g.vecg, a);
+            put16(g.U + row, t.n0 + j, g.N, g.vecg, u);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) a[i] = a[i] * gate_share<false>(g.act, a[i], nullptr) * u[i];
+          if (in) put16(static_cast<T*>(g.out[0]) + row, t.n0 + j, g.N, g.vec, a);
+        }
+      } else {
+        T* row = static_cast<T*>(g.out[t.result]) + (size_t)m * g.N;
+#pragma unroll 1
+        for (int j = half * 128; j < half * 128 + 128 && t.n0 + j < g.N; j += 16) {
+          float a[16];
+          tmem_ld16(taddr + j, a);
+          if (in) put16(row, t.n0 + j, g.N, g.vec, a);
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) {
+    atomicCAS(&g_gated_status, 0, (1 << 16) | (blockIdx.x & 0xffff));
+    const long long t0 = clock64();   // copies in flight land before the shared memory is given back
+    while (clock64() - t0 < 40000000ll) {
+    }
+  }
+  cluster_sync();   // the peer's products read this CTA's shared memory, and its commits arrive on its barriers
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ---- elementwise -----------------------------------------------------------------------------------------------------------------
+// dG = dH U act'(G), dU = dH act(G): rows of N values to rows of ld, eight per thread.  Bound by HBM: 14 bytes a value.
+template <typename T>
+__global__ void __launch_bounds__(256) slopes_kernel(int M, int N, int ld, int act, int vec, const float* G, const float* U, const T* dH, T* dG, T* dU) {
+  const int groups = (N + 7) / 8;
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (size_t)M * groups) return;
+  const size_t m = i / groups;
+  const int n = (int)(i - m * groups) * 8, left = min(8, N - n);
+  const size_t src = m * N + n, dst = m * ld + n;
+  float a[8], u[8], d[8];
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      *reinterpret_cast<float4*>(a + j) = *reinterpret_cast<const float4*>(G + src + j);
+      *reinterpret_cast<float4*>(u + j) = *reinterpret_cast<const float4*>(U + src + j);
+    }
+    alignas(16) T h[8];
+    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(dH + src);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] = (float)h[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      a[j] = j < left ? G[src + j] : 0.f;
+      u[j] = j < left ? U[src + j] : 0.f;
+      d[j] = j < left ? (float)dH[src + j] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float slope;
+    const float share = gate_share<true>(act, a[j], &slope);
+    const float up = d[j] * a[j] * share;
+    a[j] = d[j] * u[j] * slope;
+    u[j] = up;
+  }
+  *reinterpret_cast<uint4*>(dG + dst) = make_uint4(pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3]), pack2<T>(a[4], a[5]), pack2<T>(a[6], a[7]));
+  *reinterpret_cast<uint4*>(dU + dst) = make_uint4(pack2<T>(u[0], u[1]), pack2<T>(u[2], u[3]), pack2<T>(u[4], u[5]), pack2<T>(u[6], u[7]));
+}
+
+// Rows of `cols` 16-bit values to rows of ld (a multiple of eight), up to three matrices in one launch.
+struct PadJob {
+  const uint16_t* src;
+  uint16_t* dst;
+  int rows, cols, ld;
+  unsigned first;   // CTA
+};
+struct PadJobs {
+  PadJob job[3];
+  int count;
+};
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ PadJobs p) {
+  int k = 0;
+  while (k + 1 < p.count && blockIdx.x >= p.job[k + 1].first) ++k;
+  const PadJob& q = p.job[k];
+  const int groups = q.ld / 8;
+  const size_t i = (size_t)(blockIdx.x - q.first) * 256 + threadIdx.x;
+  if (i >= (size_t)q.rows * groups) return;
+  const size_t r = i / groups;
+  const int c = (int)(i - r * groups) * 8;
+  const uint16_t* s = q.src + r * q.cols + c;
+  alignas(16) uint16_t v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = c + j < q.cols ? s[j] : (uint16_t)0;
+  *reinterpret_cast<uint4*>(q.dst + r * q.ld + c) = *reinterpret_cast<const uint4*>(v);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+int ld8(int n) { return (n + 7) / 8 * 8; }
+size_t plane(size_t rows, int cols) { return align_up(rows * ld8(cols) * 2, 256); }
+bool odd(int cols) { return cols % 8 != 0; }
+
+struct Matrix {   // as the kernel reads it
+  const void* p;
+  int rows, cols, ld;
+};
+template <typename T>
+int encode(CUtensorMap* map, const Matrix& m, unsigned box_rows) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (!enc) return fail(B200CP_ERR_NO_DEVICE, "cuTensorMapEncodeTiled entry point not available");
+  const cuuint64_t dim[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, stride[1] = {(cuuint64_t)m.ld * 2};
+  const cuuint32_t box[2] = {64, box_rows}, estr[2] = {1, 1};
+  const CUresult cr = enc(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                          const_cast<void*>(m.p), dim, stride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (cr != CUDA_SUCCESS) return fail(B200CP_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)cr);
+  return B200CP_OK;
+}
+// Copies the matrices whose rows are of odd length to the workspace, which is moved on.
+int pad(Matrix** ms, int count, char*& ws, cudaStream_t st) {
+  PadJobs jobs{};
+  unsigned ctas = 0;
+  for (int i = 0; i < count; ++i) {
+    Matrix& m = *ms[i];
+    m.ld = ld8(m.cols);
+    if (!odd(m.cols)) continue;
+    const size_t n = ((size_t)m.rows * (m.ld / 8) + 255) / 256;
+    jobs.job[jobs.count++] = PadJob{static_cast<const uint16_t*>(m.p), reinterpret_cast<uint16_t*>(ws), m.rows, m.cols, m.ld, ctas};
+    ctas += (unsigned)n;
+    m.p = ws;
+    ws += plane(m.rows, m.cols);
+  }
+  if (!ctas) return B200CP_OK;
+  pad_rows_kernel<<<ctas, 256, 0, st>>>(jobs);
+  B200CP_LAUNCH_OK("pad_rows_kernel");
+  return B200CP_OK;
+}
+size_t pad_bytes(int rows, int I, int F) { return (odd(I) ? plane(rows, I) : 0) + (odd(F) ? 2 * plane(I, F) : 0); }
+bool rows16(const void* p, size_t row_bytes) { return !(reinterpret_cast<uintptr_t>(p) & 15) && row_bytes % 16 == 0; }
+
+template <Form FORM, typename T>
+int launch(Gemm g, int results, const Matrix& a0, const Matrix& a1, const Matrix& b0, const Matrix& b1, cudaStream_t st) {
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  CUtensorMap ma0, ma1, mb0, mb1;
+  constexpr unsigned ra = FORM == kWeights ? kStep : 128, rb = FORM == kData ? 128 : kStep;
+  if (int rc = encode<T>(&ma0, a0, ra)) return rc;
+  if (int rc = encode<T>(&ma1, a1, ra)) return rc;
+  if (int rc = encode<T>(&mb0, b0, rb)) return rc;
+  if (int rc = encode<T>(&mb1, b1, rb)) return rc;
+  g.tiles_m = ceil_div(g.M, kTile);
+  g.tiles_n = ceil_div(g.N, FORM == kForward ? kTile / 2 : kTile);
+  const long units = (long)g.tiles_m * g.tiles_n * results;
+  if (units > 0x3fffffff) return fail(B200CP_ERR_UNSUPPORTED, "gated feed-forward block: %d x %d is too large", g.M, g.N);
+  g.units = (int)units;
+  g.vec = rows16(g.out[0], (size_t)g.N * 2) && rows16(g.out[results - 1], (size_t)g.N * 2);
+  g.vecg = rows16(g.G, (size_t)g.N * 4) && rows16(g.U, (size_t)g.N * 4);
+  const auto kern = gated_kernel<FORM, T>;
+  static std::atomic<int> set[64];
+  B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, (int)kSmem));
+  const int pairs = std::min(g.units, di.sm_count / 2);
+  B200CP_CUDA_OK(launch_kernel(kern, dim3(2 * pairs), dim3(kThreads), kSmem, st, true, g, ma0, ma1, mb0, mb1));
+  B200CP_LAUNCH_OK("gated_kernel");
+  return B200CP_OK;
+}
+
+template <typename T>
+int forward(int rows, int I, int F, int act, const void* X, const void* Wg, const void* Wu, void* H, float* G, float* U, char* ws, cudaStream_t st) {
+  Matrix x{X, rows, I, 0}, g{Wg, I, F, 0}, u{Wu, I, F, 0}, *ms[3] = {&x, &g, &u};
+  if (int rc = pad(ms, 3, ws, st)) return rc;
+  Gemm p{};
+  p.M = rows; p.N = F; p.steps = p.first = ceil_div(I, kStep); p.act = act;
+  p.out[0] = p.out[1] = H; p.G = G; p.U = U;
+  return launch<kForward, T>(p, 1, x, x, g, u, st);
+}
+
+template <typename T>
+int backward(int rows, int I, int F, int act, const void* X, const void* Wg, const void* Wu, const float* G, const float* U, const void* dH, void* dX,
+             void* dWg, void* dWu, char* ws, cudaStream_t st) {
+  const int ld = ld8(F);
+  T *dG = reinterpret_cast<T*>(ws), *dU = reinterpret_cast<T*>(ws + plane(rows, F));
+  ws += 2 * plane(rows, F);
+  Matrix x{X, rows, I, 0}, g{Wg, I, F, 0}, u{Wu, I, F, 0}, *ms[3];
+  int count = 0;
+  if (dWg) ms[count++] = &x;
+  if (dX) {
+    ms[count++] = &g;
+    ms[count++] = &u;
+  }
+  if (int rc = pad(ms, count, ws, st)) return rc;
+  const size_t n = ((size_t)rows * (ld / 8) + 255) / 256;
+  if (n > 0x7fffffffull) return fail(B200CP_ERR_UNSUPPORTED, "gated feed-forward block: %d x %d is too large", rows, F);
+  const int vec = rows16(G, (size_t)F * 4) && rows16(U, (size_t)F * 4) && rows16(dH, (size_t)F * 2);
+  slopes_kernel<T><<<(unsigned)n, 256, 0, st>>>(rows, F, ld, act, vec, G, U, static_cast<const T*>(dH), dG, dU);
+  B200CP_LAUNCH_OK("slopes_kernel");
+  const Matrix a{dG, rows, F, ld}, b{dU, rows, F, ld};
+  Gemm p{};
+  if (dX) {
+    p.M = rows; p.N = I; p.first = ceil_div(F, kStep); p.steps = 2 * p.first;
+    p.out[0] = p.out[1] = dX;
+    if (int rc = launch<kData, T>(p, 1, a, b, g, u, st)) return rc;
+  }
+  if (dWg) {
+    p.M = I; p.N = F; p.steps = p.first = ceil_div(rows, kStep);
+    p.out[0] = dWg; p.out[1] = dWu;
+    if (int rc = launch<kWeights, T>(p, 2, x, x, a, b, st)) return rc;
+  }
+  return B200CP_OK;
+}
+
+int check_gated(const char* who, int rows, int I, int F, int type, int act) {
+  if (rows < 0 || I < 1 || F < 1 || act < B200CP_SILU || act > B200CP_GELU_TANH)
+    return fail(B200CP_ERR_INVALID_ARG, "%s: rows=%d I=%d F=%d activation=%d", who, rows, I, F, act);
+  if (type != B200CP_BFLOAT16 && type != B200CP_FLOAT16) return fail(B200CP_ERR_UNSUPPORTED, "%s: type %d (16-bit types only)", who, type);
+  if (rows > (1 << 28) || I > (1 << 28) || F > (1 << 28)) return fail(B200CP_ERR_UNSUPPORTED, "%s: sizes above 2^28", who);
+  return B200CP_OK;
+}
+
+}  // namespace
+
+int gated_device_status(int* out) {
+  int v = 0, zero = 0;
+  B200CP_CUDA_OK(cudaMemcpyFromSymbol(&v, g_gated_status, sizeof(int)));
+  if (v) B200CP_CUDA_OK(cudaMemcpyToSymbol(g_gated_status, &zero, sizeof(int)));
+  *out = v;
+  return B200CP_OK;
+}
+
+}  // namespace b200cp
+
+using namespace b200cp;
+
+extern "C" {
+
+size_t b200cp_dense_gated_workspace_bytes(int rows, int I, int F, int type) {
+  if (check_gated("b200cp_dense_gated_workspace_bytes", rows, I, F, type, 0)) return 0;
+  return pad_bytes(rows, I, F);
+}
+
+int b200cp_dense_gated(int rows, int I, int F, int type, int activation, const void* X, const void* Wg, const void* Wu, void* H, float* G,
+                       float* U, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "b200cp_dense_gated";
+  if (int rc = check_gated(who, rows, I, F, type, activation)) return rc;
+  if (rows == 0) return B200CP_OK;
+  if (!X || !Wg || !Wu || !H || !G != !U) return fail(B200CP_ERR_INVALID_ARG, "%s: null pointer", who);
+  for (const void* p : {X, Wg, Wu})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(B200CP_ERR_INVALID_ARG, "%s: X, Wg and Wu have to start on 16-byte boundaries", who);
+  const size_t need = b200cp_dense_gated_workspace_bytes(rows, I, F, type);
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return fail(B200CP_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, %zu given", who, need, workspace_bytes);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  return type == B200CP_BFLOAT16 ? forward<__nv_bfloat16>(rows, I, F, activation, X, Wg, Wu, H, G, U, ws, st)
+                                 : forward<__half>(rows, I, F, activation, X, Wg, Wu, H, G, U, ws, st);
+}
+
+size_t b200cp_dense_gated_bwd_workspace_bytes(int rows, int I, int F, int type) {
+  if (check_gated("b200cp_dense_gated_bwd_workspace_bytes", rows, I, F, type, 0)) return 0;
+  return 2 * plane(rows, F) + pad_bytes(rows, I, F);
+}
+
+int b200cp_dense_gated_bwd(int rows, int I, int F, int type, int activation, const void* X, const void* Wg, const void* Wu, const float* G,
+                           const float* U, const void* dH, void* dX, void* dWg, void* dWu, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  const char* who = "b200cp_dense_gated_bwd";
+  if (int rc = check_gated(who, rows, I, F, type, activation)) return rc;
+  if (!dWg != !dWu) return fail(B200CP_ERR_INVALID_ARG, "%s: one of dWg and dWu is null", who);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    for (void* p : {dWg, dWu})
+      if (p) B200CP_CUDA_OK(cudaMemsetAsync(p, 0, (size_t)I * F * 2, st));
+    return B200CP_OK;
+  }
+  if (!G || !U || !dH || (dWg && !X) || (dX && (!Wg || !Wu))) return fail(B200CP_ERR_INVALID_ARG, "%s: null pointer", who);
+  for (const void* p : {X, Wg, Wu})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(B200CP_ERR_INVALID_ARG, "%s: X, Wg and Wu have to start on 16-byte boundaries", who);
+  const size_t need = b200cp_dense_gated_bwd_workspace_bytes(rows, I, F, type);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return fail(B200CP_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, %zu given", who, need, workspace_bytes);
+  char* ws = static_cast<char*>(workspace);
+  return type == B200CP_BFLOAT16 ? backward<__nv_bfloat16>(rows, I, F, activation, X, Wg, Wu, G, U, dH, dX, dWg, dWu, ws, st)
+                                 : backward<__half>(rows, I, F, activation, X, Wg, Wu, G, U, dH, dX, dWg, dWu, ws, st);
+}
+
+}  // extern "C"

@@ -35,6 +35,7 @@
 
 #include "common.cuh"
 #include "tc_common.cuh"
+#include "tc_pair.cuh"
 
 namespace b200cp {
 
@@ -87,54 +88,6 @@ struct SplitGemm {
   const int* dropped;
 };
 
-// ---- PTX of a CTA pair --------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// the same shared variable in the leader CTA of the pair
-__device__ __forceinline__ uint32_t leader_addr(uint32_t p) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(0));
-  return r;
-}
-__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// into this CTA's shared memory, counted on a barrier of either CTA of the pair (no multicast)
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
-      "[%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(0)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(ncols) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
-      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-// one arrival on the barrier of both CTAs when the products issued so far have completed
-__device__ __forceinline__ void commit_pair(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"((uint16_t)3)
-      : "memory");
-}
 // registers -> TMEM: 16 columns of the warp's lane quarter
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
   asm volatile(
@@ -148,35 +101,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
 // MN-major operands are bf16.
 __host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t n, uint32_t mn) {
   return (1u << 4) | (mn << 7) | (mn << 10) | (mn << 15) | (mn << 16) | ((n >> 3) << 17) | ((256u >> 4) << 24);
-}
-
-// Bounded wait shared by the roles: gives up after about a second, or as soon as another role of the CTA has given up.
-// (Shared-memory addresses in 32 bits: the read-out warps have no register to spare.)
-__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, uint32_t abort_flag) {
-  long long t0 = 0;
-  for (int it = 0;; ++it) {
-    uint32_t done;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if ((it & 31) == 31) {
-      uint32_t given_up;
-      asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(given_up) : "r"(abort_flag) : "memory");
-      if (given_up) return false;
-      if (t0 == 0) t0 = clock64();
-      if (clock64() - t0 > 1500000000ll) {
-        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_flag), "r"(1) : "memory");
-        return false;
-      }
-    }
-  }
 }
 
 __device__ __forceinline__ int tap_shift(const SplitGemm& g, int tap);

@@ -840,6 +840,7 @@ PyMethodDef g_methods[] = {FAST(cp4_forward), FAST(cp4_forward_save), FAST(cp4_b
                            FAST(rcp_forward), FAST(rcp_backward), FAST(dense_forward), FAST(dense_backward),
                            FAST(cp4_apply), FAST(cp3_apply), FAST(rcp_apply), FAST(dense_apply),
                            FAST(adapter_plan), FAST(dense_adapters), FAST(dense_adapters_backward), FAST(adapters_apply),
+                           FAST(dense_gated), FAST(dense_gated_save), FAST(dense_gated_backward), FAST(gated_apply),
                            FAST(adamw_step), FAST(adamw_moments),
                            {"set_error_class", py_set_error_class, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};

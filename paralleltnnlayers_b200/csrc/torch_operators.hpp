@@ -1,4 +1,4 @@
-// Bindings of the operators that stand beside the factored layers: low-rank adapters and the AdamW step.
+// Bindings of the operators that stand beside the factored layers: low-rank adapters, the gated feed-forward block and the AdamW step.
 // Part of torch_binding.cpp's namespace, whose helpers it uses.
 
 // ---- types ------------------------------------------------------------------------------------------------------------
@@ -155,6 +155,86 @@ struct AdaptersNode : torch::autograd::Function<AdaptersNode> {
   }
 };
 
+// ---- gated feed-forward block ------------------------------------------------------------------------------------------
+struct Gated {   // operands, checked, contiguous and on 16-byte boundaries
+  Tensor x, Wg, Wu;
+  int rows, I, F, type, act;
+  Gated(const Tensor& x_, const Tensor& Wg_, const Tensor& Wu_, int64_t act_) : act((int)act_) {
+    type = type_of(x_, "X");
+    TORCH_CHECK_TYPE(type != B200CP_FLOAT32, "X must be a bfloat16 or float16 CUDA tensor (float32: dense_matmul)");
+    TORCH_CHECK_VALUE(x_.dim() >= 1 && Wg_.dim() == 2 && Wg_.sizes() == Wu_.sizes(), "expected X [..., I], Wg and Wu [I, F]");
+    TORCH_CHECK_VALUE(x_.size(-1) == Wg_.size(0), "X ", x_.sizes(), " does not go with weights ", Wg_.sizes());
+    Adapters::same(Wg_, x_, "Wg");
+    Adapters::same(Wu_, x_, "Wu");
+    I = size_arg(Wg_.size(0), "I");
+    F = size_arg(Wg_.size(1), "F");
+    TORCH_CHECK_VALUE(I > 0 && F > 0, "the weights may not be empty");
+    rows = size_arg(x_.numel() / I, "the number of rows");
+    x = whole(x_);
+    Wg = whole(Wg_);
+    Wu = whole(Wu_);
+  }
+  static Tensor whole(const Tensor& t) {
+    const Tensor c = contiguous(t);
+    return (reinterpret_cast<uintptr_t>(c.const_data_ptr()) & 15) == 0 ? c : c.clone();
+  }
+  std::vector<int64_t> size(int64_t last) const {
+    std::vector<int64_t> s = x.sizes().vec();
+    s.back() = last;
+    return s;
+  }
+};
+Tensor dense_gated(const Gated& g, Tensor* G, Tensor* U) {
+  const c10::cuda::OptionalCUDAGuard guard(g.x.device());
+  Tensor H = empty_as(g.size(g.F), g.x);
+  if (G) {
+    *G = empty({g.rows, g.F}, g.x);
+    *U = empty({g.rows, g.F}, g.x);
+  }
+  const Scratch ws(b200cp_dense_gated_workspace_bytes(g.rows, g.I, g.F, g.type), g.x);
+  ok(b200cp_dense_gated(g.rows, g.I, g.F, g.type, g.act, g.x.const_data_ptr(), g.Wg.const_data_ptr(), g.Wu.const_data_ptr(), H.data_ptr(),
+                        G ? mp(*G) : nullptr, U ? mp(*U) : nullptr, ws.ptr, ws.bytes, stream(g.x)));
+  return H;
+}
+std::array<Tensor, 3> dense_gated_backward(const Gated& g, const Tensor& G_, const Tensor& U_, const Tensor& dH_, bool need_x, bool need_w) {
+  Adapters::same(dH_, g.x, "dH");
+  TORCH_CHECK_VALUE(dH_.sizes() == at::IntArrayRef(g.size(g.F)), "dH is ", dH_.sizes(), ", ", at::IntArrayRef(g.size(g.F)), " is needed");
+  const Tensor G = dev(G_, "G", g.x), U = dev(U_, "U", g.x), dH = contiguous(dH_);
+  check_size(G, "G", {g.rows, g.F});
+  check_size(U, "U", {g.rows, g.F});
+  const c10::cuda::OptionalCUDAGuard guard(g.x.device());
+  std::array<Tensor, 3> d;
+  if (need_x) d[0] = empty_as(g.x.sizes(), g.x);
+  if (need_w) {
+    d[1] = empty_as(g.Wg.sizes(), g.x);
+    d[2] = empty_as(g.Wg.sizes(), g.x);
+  }
+  if (!need_x && !need_w) return d;
+  const auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  const Scratch ws(b200cp_dense_gated_bwd_workspace_bytes(g.rows, g.I, g.F, g.type), g.x);
+  ok(b200cp_dense_gated_bwd(g.rows, g.I, g.F, g.type, g.act, g.x.const_data_ptr(), g.Wg.const_data_ptr(), g.Wu.const_data_ptr(), cp(G), cp(U),
+                            dH.const_data_ptr(), at(d[0]), at(d[1]), at(d[2]), ws.ptr, ws.bytes, stream(g.x)));
+  return d;
+}
+struct GatedNode : torch::autograd::Function<GatedNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& Wg, const Tensor& Wu, int64_t act, bool grad) {
+    const Gated g(x, Wg, Wu, act);
+    ctx->saved_data["act"] = act;
+    if (!grad) return dense_gated(g, nullptr, nullptr);
+    Tensor G, U;
+    Tensor H = dense_gated(g, &G, &U);
+    ctx->save_for_backward({x, Wg, Wu, G, U});
+    return H;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list v = ctx->get_saved_variables();
+    const Gated g(v[0], v[1], v[2], ctx->saved_data["act"].toInt());
+    const std::array<Tensor, 3> d =
+        dense_gated_backward(g, v[3], v[4], grads[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
+    return {d[0], d[1], d[2], Tensor(), Tensor()};
+  }
+};
+
 Tensor optional_tensor(PyObject* o, const char* name) { return o == Py_None ? Tensor() : any_tensor(o, name); }
 bool truth(PyObject* o) {
   const int v = PyObject_IsTrue(o);
@@ -221,6 +301,46 @@ PYFN(py_adapters_apply) {
     }
     return AdaptersNode::apply(y, x, A, B, plan, scale.defined() ? std::optional<Tensor>(scale) : std::nullopt);
   }));
+  END_HANDLE_TH_ERRORS
+}
+
+// (X, Wg, Wu, activation)
+PYFN(py_dense_gated) {
+  HANDLE_TH_ERRORS
+  count_args(n, 4);
+  const Tensor &x = any_tensor(a[0], "X"), &g = any_tensor(a[1], "Wg"), &u = any_tensor(a[2], "Wu");
+  const int64_t act = int_arg(a[3]);
+  return wrap(unlocked([&] { return dense_gated(Gated(x, g, u, act), nullptr, nullptr); }));
+  END_HANDLE_TH_ERRORS
+}
+PYFN(py_dense_gated_save) {
+  HANDLE_TH_ERRORS
+  count_args(n, 4);
+  const Tensor &x = any_tensor(a[0], "X"), &g = any_tensor(a[1], "Wg"), &u = any_tensor(a[2], "Wu");
+  const int64_t act = int_arg(a[3]);
+  std::array<Tensor, 3> r;
+  unlocked([&] { r[0] = dense_gated(Gated(x, g, u, act), &r[1], &r[2]); });
+  return wrap_tuple(r);
+  END_HANDLE_TH_ERRORS
+}
+// (dH, X, Wg, Wu, G, U, activation, need_dx, need_dw)
+PYFN(py_dense_gated_backward) {
+  HANDLE_TH_ERRORS
+  count_args(n, 9);
+  const Tensor &dh = any_tensor(a[0], "dH"), &x = any_tensor(a[1], "X"), &wg = any_tensor(a[2], "Wg"), &wu = any_tensor(a[3], "Wu"),
+               &g = any_tensor(a[4], "G"), &u = any_tensor(a[5], "U");
+  const int64_t act = int_arg(a[6]);
+  const bool nx = truth(a[7]), nw = truth(a[8]);
+  return wrap_tuple(unlocked([&] { return dense_gated_backward(Gated(x, wg, wu, act), g, u, dh, nx, nw); }));
+  END_HANDLE_TH_ERRORS
+}
+PYFN(py_gated_apply) {
+  HANDLE_TH_ERRORS
+  count_args(n, 4);
+  const Tensor &x = any_tensor(a[0], "X"), &g = any_tensor(a[1], "Wg"), &u = any_tensor(a[2], "Wu");
+  const int64_t act = int_arg(a[3]);
+  const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || g.requires_grad() || u.requires_grad());
+  return wrap(unlocked([&] { return GatedNode::apply(x, g, u, act, grad); }));
   END_HANDLE_TH_ERRORS
 }
 

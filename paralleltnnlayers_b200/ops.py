@@ -438,6 +438,32 @@ def dense_adapters_backward(dY, X, V, A, B, plan, scale=None, need_dx=True, need
     return _C.dense_adapters_backward(dY, X, V, A, B, which, scale, need_dx, need_da, need_db)
 
 
+# ---- gated feed-forward block -----------------------------------------------------
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+
+
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise ValueError(f"activation {name!r}: one of {', '.join(ACTIVATIONS)} is possible")
+    return ACTIVATIONS[name]
+
+
+def dense_gated(X, Wg, Wu, activation="silu"):
+    """``act(X Wg) * (X Wu)``, both projections and the product in one kernel (``b200cp_dense_gated``): ``X [..., I]``, ``Wg`` and ``Wu [I, F]`` of one type,
+    bfloat16 or float16 (sums in float32); ``activation``: silu, gelu (with the error function) or gelu_tanh."""
+    return _C.dense_gated(X, Wg, Wu, _activation(activation))
+
+
+def dense_gated_save(X, Wg, Wu, activation="silu"):
+    """The same, with ``G = X Wg`` and ``U = X Wu`` in float32 (``[rows, F]``) for ``dense_gated_backward``: (H, G, U)."""
+    return _C.dense_gated_save(X, Wg, Wu, _activation(activation))
+
+
+def dense_gated_backward(dH, X, Wg, Wu, G, U, activation="silu", need_dx=True, need_dw=True):
+    """Gradients of ``dense_gated``: (dX, dWg, dWu), None where not needed."""
+    return _C.dense_gated_backward(dH, X, Wg, Wu, G, U, _activation(activation), need_dx, need_dw)
+
+
 # ---- AdamW step -----------------------------------------------------------------
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, master=None, scales=None):
     """One AdamW step over all tensors of the lists, in place and in one launch (``b200cp_adamw_step``):
@@ -487,3 +513,11 @@ class DenseAdaptersFunction:
     def apply(y, x, A, B, adapters, scale=None):
         which, planned = _which(adapters, x)
         return _C.adapters_apply(y, x, A, B, which, planned, scale)
+
+
+class DenseGatedFunction:
+    """``dense_gated`` with its gradients: ``apply(x, Wg, Wu, activation="silu")``."""
+
+    @staticmethod
+    def apply(x, Wg, Wu, activation="silu"):
+        return _C.gated_apply(x, Wg, Wu, _activation(activation))

@@ -119,3 +119,54 @@ def test_adapter_sizes_the_library_refuses(lib_built):
     assert lib.b200cp_dense_adapters(4, 4, 4, 4, 1, 0, *[None] * 9) == -1
     assert lib.b200cp_dense_adapters_bwd(4, 4, 4, 4, 1, 0, *[16] * 5, None, 16, 16, 16, 16, 16, 4, None) == -3
     assert lib.b200cp_dense_adapters_bwd(4, 4, 4, 4, 1, 0, *[None] * 5, None, 16, 16, 16, 16, 16, 1 << 20, None) == -1
+
+
+B16 = torch.bfloat16
+GATED = {
+    "x type": (TypeError, lambda c: (c(2, 8), c(8, 4), c(8, 4))),
+    "Wg type": (TypeError, lambda c: (c(2, 8, dtype=B16), c(8, 4, dtype=torch.float16), c(8, 4, dtype=B16))),
+    "Wu type": (TypeError, lambda c: (c(2, 8, dtype=B16), c(8, 4, dtype=B16), c(8, 4))),
+    "Wu size": (ValueError, lambda c: (c(2, 8, dtype=B16), c(8, 4, dtype=B16), c(8, 5, dtype=B16))),
+    "features": (ValueError, lambda c: (c(2, 7, dtype=B16), c(8, 4, dtype=B16), c(8, 4, dtype=B16))),
+    "device": (ValueError, lambda c: (c(2, 8, dtype=B16), c(8, 4, dtype=B16), c(8, 4, dtype=B16, dev=1))),
+    "dimensions": (ValueError, lambda c: (c(2, 8, dtype=B16), c(1, 8, 4, dtype=B16), c(1, 8, 4, dtype=B16))),
+    "empty": (ValueError, lambda c: (c(2, 8, dtype=B16), c(8, 0, dtype=B16), c(8, 0, dtype=B16))),
+    "not a tensor": (TypeError, lambda c: (c(2, 8, dtype=B16), None, c(8, 4, dtype=B16))),
+    "activation": (ValueError, lambda c: (c(2, 8, dtype=B16), c(8, 4, dtype=B16), c(8, 4, dtype=B16), "relu")),
+}
+
+
+@pytest.mark.parametrize("what", GATED)
+def test_gated_refuses(fake, what):
+    import paralleltnnlayers_b200 as P
+    error, args = GATED[what]
+    for call in (P.dense_gated, P.dense_gated_save, P.DenseGatedFunction.apply):
+        with pytest.raises(error):
+            call(*args(fake))
+
+
+def test_gated_backward_refuses_what_does_not_fit(fake):
+    import paralleltnnlayers_b200 as P
+    c = fake
+    good = dict(dH=c(2, 4, dtype=B16), X=c(2, 8, dtype=B16), Wg=c(8, 4, dtype=B16), Wu=c(8, 4, dtype=B16), G=c(2, 4), U=c(2, 4))
+    for name, bad, error in (("dH", c(2, 5, dtype=B16), ValueError), ("dH", c(2, 4), TypeError), ("G", c(2, 5), ValueError), ("U", c(2, 4, dtype=B16), TypeError),
+                             ("U", c(2, 4, dev=1), ValueError)):
+        with pytest.raises(error):
+            P.dense_gated_backward(**{**good, name: bad})
+
+
+def test_gated_sizes_the_library_refuses(lib_built):
+    from paralleltnnlayers_b200 import _lib
+    lib = _lib.lib
+    assert lib.b200cp_dense_gated_workspace_bytes(4, 8, 8, 1) == 0 and lib.b200cp_dense_gated_workspace_bytes(4, 8, 9, 1) > 0
+    assert lib.b200cp_dense_gated_workspace_bytes(4, 8, 9, 0) == 0
+    fwd = lambda *a: lib.b200cp_dense_gated(*a, None, 0, None)  # noqa: E731
+    assert fwd(0, 8, 8, 1, 0, None, None, None, None, None, None) == 0
+    assert fwd(4, 8, 8, 0, 0, 16, 16, 16, 16, None, None) == -2      # fp32
+    assert fwd(4, 8, 8, 1, 3, 16, 16, 16, 16, None, None) == -1      # no such activation
+    assert fwd(4, 8, 8, 1, 0, 16, 16, 16, 16, 16, None) == -1        # G without U
+    assert fwd(4, 8, 8, 1, 0, 16, 24, 16, 16, None, None) == -1      # not on sixteen bytes
+    assert fwd(4, 8, 9, 1, 0, 16, 16, 16, 16, None, None) == -3      # no workspace
+    bwd = lambda *a: lib.b200cp_dense_gated_bwd(*a, None, 0, None)  # noqa: E731
+    assert bwd(4, 8, 8, 1, 0, 16, 16, 16, 16, 16, 16, 16, 16, None) == -1
+    assert bwd(4, 8, 8, 1, 0, 16, 16, 16, 16, 16, 16, 16, 16, 16) == -3
