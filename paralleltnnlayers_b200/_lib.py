@@ -103,7 +103,7 @@ def _load():
         "b200cp_dense_bwd": (i, [i, i, ip, ip, i, fp, fp, pp, fp, pp, vp, sz, vp, i]),
         "b200cp_adapter_plan_bytes": (sz, [i, i]),
         "b200cp_adapter_plan": (i, [i, i, vp, vp, sz, vp]),
-        "b200cp_dense_adapters": (i, [i, i, i, i, i, i, vp, vp, vp, vp, fp, vp, vp, vp, vp]),
+        "b200cp_dense_adapters": (i, [i, i, i, i, i, i, vp, vp, vp, vp, fp, vp, vp, vp, vp, vp]),
         "b200cp_dense_adapters_bwd_workspace_bytes": (sz, [i, i, i, i, i, i]),
         "b200cp_dense_adapters_bwd": (i, [i, i, i, i, i, i, vp, vp, vp, vp, vp, fp, vp, vp, vp, vp, vp, sz, vp]),
         "b200cp_dense_gated_workspace_bytes": (sz, [i, i, i, i]),

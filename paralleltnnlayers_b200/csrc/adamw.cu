@@ -131,36 +131,62 @@ __device__ __forceinline__ void store_codes(uint8_t* p, long long i, long long n
   for (int k = 0; k < 4; ++k)
     if (i + k < n) p[i + k] = (uint8_t)(c >> (8 * k));
 }
-__device__ __forceinline__ float of_m(float c, float s) {
-  const float q = c * (1.f / 127);
-  return c == -128.f ? __int_as_float(0x7fffffff) : q * fabsf(q) * s;
+// Whether one of four bytes is zero (of the codes xor that of NaN): a value in none but a broken state.
+__device__ __forceinline__ bool has_zero(uint32_t x) { return ((x - 0x01010101u) & ~x & 0x80808080u) != 0; }
+__device__ __forceinline__ void values_of_m(uint32_t four, float s, float (&x)[4]) {
+  codes_of_m(four, x);
+  const bool broken = has_zero(four ^ 0x80808080u);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float q = x[k] * (1.f / 127), v = q * fabsf(q) * s;
+    x[k] = broken && x[k] == -128.f ? __int_as_float(0x7fffffff) : v;
+  }
 }
-__device__ __forceinline__ float of_v(float c, float s) {
-  const float q = c * (1.f / 254), r = q * q;
-  return c == 255.f ? __int_as_float(0x7fffffff) : r * r * s;
+__device__ __forceinline__ void values_of_v(uint32_t four, float s, float (&x)[4]) {
+  codes_of_v(four, x);
+  const bool broken = has_zero(~four);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float q = x[k] * (1.f / 254), r = q * q, v = r * r * s;
+    x[k] = broken && x[k] == 255.f ? __int_as_float(0x7fffffff) : v;
+  }
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 // The code is that of 127 sqrt(|x| / s) with every operation rounded to nearest: found by the fast operations, and again by the exact
-// ones where those end within 1e-4 (v: 2e-4) of a border (the two are within 5e-5, 1.1e-4 of a step of one another), one value in 3000.  Exact codes do not
+// ones where one of a thread's eight ends within 2e-4 of a border (the two are within 1.1e-4 of a step of one another).  Exact codes do not
 // depend on how an operation is approximated: two implementations that round alike hold the same state.
-__device__ __noinline__ float exact_code(float x, float s, float steps) {
-  const float q = sqrtf(__fdiv_rn(fabsf(x), s));
-  return rintf(steps * (steps > 200.f ? sqrtf(q) : q));
+__device__ __noinline__ float exact_m(float x, float s) {
+  if (!(fabsf(x) < __int_as_float(0x7f800000))) return -128.f;
+  return s > 0.f ? copysignf(rintf(127.f * sqrtf(__fdiv_rn(fabsf(x), s))), x) : 0.f;
 }
-__device__ __forceinline__ float code_m(float x, float s, float inverse) {
-  const float t = 127.f * fast_sqrt_ftz(fabsf(x) * inverse);
-  float c = (t + kWhole) - kWhole;
-  if (!(fabsf(t - c) <= 0.4999f) || inverse == 0.f)   // (what is not finite ends here too)
-    c = !(fabsf(x) < __int_as_float(0x7f800000)) ? 128.f : s > 0.f ? exact_code(x, s, 127.f) : 0.f;
-  return c == 128.f ? -128.f : copysignf(c, x);
+__device__ __noinline__ float exact_v(float x, float s) {
+  if (!(x < __int_as_float(0x7f800000))) return 255.f;
+  return x > 0.f && s > 0.f ? fmaxf(rintf(254.f * sqrtf(sqrtf(__fdiv_rn(x, s)))), 1.f) : 0.f;
 }
-__device__ __forceinline__ float code_v(float x, float s, float inverse) {
-  const float t = 254.f * fast_sqrt_ftz(fast_sqrt_ftz(x * inverse));
-  float c = (t + kWhole) - kWhole;
-  if (!(fabsf(t - c) <= 0.4998f) || inverse == 0.f) {
-    if (!(x < __int_as_float(0x7f800000))) return 255.f;
-    c = s > 0.f ? exact_code(x, s, 254.f) : 0.f;
+__device__ __forceinline__ void codes_from(const float (&m)[4], const float (&v)[4], float sm, float sv, float im, float iv, uint32_t& cm, uint32_t& cv) {
+  float a[4], b[4], off = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float t = 127.f * fast_sqrt_ftz(fabsf(m[k]) * im), u = 254.f * fast_sqrt_ftz(fast_sqrt_ftz(v[k] * iv));
+    a[k] = (t + kWhole) - kWhole;
+    b[k] = (u + kWhole) - kWhole;
+    off = max_nan(max_nan(off, fabsf(t - a[k])), fabsf(u - b[k]));
+    a[k] = copysignf(a[k], m[k]);
+    b[k] = fmaxf(b[k], v[k] > 0.f ? 1.f : 0.f);
   }
-  return x > 0.f ? fmaxf(c, 1.f) : 0.f;
+  if (!(off <= 0.4998f) || im == 0.f || iv == 0.f) {   // (what is not finite ends here too)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      a[k] = exact_m(m[k], sm);
+      b[k] = exact_v(v[k], sv);
+    }
+  }
+  cm = to_codes(a);
+  cv = to_codes(b);
 }
 __device__ __forceinline__ float finite_magnitude(float x) { return fabsf(x) < __int_as_float(0x7f800000) ? fabsf(x) : 0.f; }
 __device__ __forceinline__ float warp_max(float x) {   // of magnitudes
@@ -220,13 +246,8 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const long long i = base + j * 128 + lane * 4;
-      codes_of_m(load_codes(cm, i, n, vm), m[j]);
-      codes_of_v(load_codes(cv, i, n, vv), v[j]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        m[j][k] = of_m(m[j][k], ms);
-        v[j][k] = of_v(v[j][k], vs);
-      }
+      values_of_m(load_codes(cm, i, n, vm), ms, m[j]);
+      values_of_v(load_codes(cv, i, n, vv), vs, v[j]);
     }
   } else {
     const float *fm = static_cast<const float*>(e.m), *fv = static_cast<const float*>(e.v);
@@ -239,16 +260,17 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     }
   }
   float mm = 0.f, mv = 0.f;
+  const bool tiny_eps = t.r.eps < 1e-12f;   // then the square root of a subnormal v counts beside it
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       m[j][k] = fmaf(t.r.c1, d[j][k], __fmul_rn(t.r.b1, m[j][k]));
       v[j][k] = fmaf(t.r.c2, __fmul_rn(d[j][k], d[j][k]), __fmul_rn(t.r.b2, v[j][k]));
-      x[j][k] = fmaf(-step, m[j][k] * fast_inverse(fmaf(fast_sqrt(v[j][k]), root, t.r.eps)), fmaf(-decay, x[j][k], x[j][k]));
-      if (SMALL) {   // (values past the end are zero: they change no maximum)
-        mm = fmaxf(mm, finite_magnitude(m[j][k]));
-        mv = fmaxf(mv, finite_magnitude(v[j][k]));
+      x[j][k] = fmaf(-step, m[j][k] * fast_inverse(fmaf(tiny_eps ? fast_sqrt(v[j][k]) : fast_sqrt_ftz(v[j][k]), root, t.r.eps)), fmaf(-decay, x[j][k], x[j][k]));
+      if (SMALL) {   // (values past the end are zero, and a NaN is never the larger: neither changes a maximum)
+        mm = fmaxf(mm, fabsf(m[j][k]));
+        mv = fmaxf(mv, v[j][k]);
       }
     }
 #pragma unroll
@@ -261,6 +283,18 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     uint8_t *cm = static_cast<uint8_t*>(e.m), *cv = static_cast<uint8_t*>(e.v);
     mm = warp_max(mm);
     mv = warp_max(mv);
+    if (fmaxf(mm, mv) > 3.4028235e38f) {   // an infinity: the largest of the finite ones
+      mm = mv = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          mm = fmaxf(mm, finite_magnitude(m[j][k]));
+          mv = fmaxf(mv, finite_magnitude(v[j][k]));
+        }
+      mm = warp_max(mm);
+      mv = warp_max(mv);
+    }
     const float im = inverse_of(mm), iv = inverse_of(mv);
     if (lane == 0) {
       e.ms[block] = mm;
@@ -270,13 +304,10 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const long long i = base + j * 128 + lane * 4;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        m[j][k] = code_m(m[j][k], mm, im);
-        v[j][k] = code_v(v[j][k], mv, iv);
-      }
-      store_codes(cm, i, n, vm, to_codes(m[j]));
-      store_codes(cv, i, n, vv, to_codes(v[j]));
+      uint32_t p4, q4;
+      codes_from(m[j], v[j], mm, mv, im, iv, p4, q4);
+      store_codes(cm, i, n, vm, p4);
+      store_codes(cv, i, n, vv, q4);
     }
   } else {
     float *fm = static_cast<float*>(e.m), *fv = static_cast<float*>(e.v);
@@ -313,13 +344,8 @@ __global__ void __launch_bounds__(kThreads) moments_kernel(long long n, const ui
     const long long i = i0 + j * (kThreads * 4);
     if (i >= n) break;
     float x[4], y[4];
-    codes_of_m(p[j], x);
-    codes_of_v(q[j], y);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[k] = of_m(x[k], s[j]);
-      y[k] = of_v(y[k], r[j]);
-    }
+    values_of_m(p[j], s[j], x);
+    values_of_v(q[j], r[j], y);
     store4(m, i, n, c, x);
     store4(v, i, n, d, y);
   }

@@ -25,6 +25,7 @@ namespace b200cp {
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8, kMostRank = 128, kMostAdapters = 16384;
+static_assert(B200CP_ADAPTERS_WITHOUT_PLAN <= kThreads, "a thread has a row");
 
 // ---- plan -------------------------------------------------------------------------------------------------------------------
 // ints: [0] tiles, [1] rows with an adapter, [2..3] free | start[count + 2] | tile_adapter[tiles] | tile_first[tiles] | order[rows].
@@ -89,13 +90,19 @@ __global__ void __launch_bounds__(1024) plan_kernel(int rows, int count, int tm,
     const int a = adapters[r];
     return a >= 0 && a < count ? a : count;
   };
+  constexpr int Q = 8;   // turns of a warp whose loads are in flight together
   if (warp < sorters)
-    for (int b = r0; b < r1; b += 32) {
-      const bool in = b + lane < r1;
-      const int key = in ? key_of(b + lane) : -1;
-      const unsigned same = __match_any_sync(0xffffffffu, key);
-      if (in && (same & ((1u << lane) - 1)) == 0) counts[key * sorters + warp] += __popc(same);
-      __syncwarp();
+    for (int b = r0; b < r1; b += 32 * Q) {
+      int key[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) key[q] = b + q * 32 + lane < r1 ? key_of(b + q * 32 + lane) : -1;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        if (b + q * 32 >= r1) break;
+        const unsigned same = __match_any_sync(0xffffffffu, key[q]);
+        if (key[q] >= 0 && (same & ((1u << lane) - 1)) == 0) counts[key[q] * sorters + warp] += __popc(same);
+        __syncwarp();
+      }
     }
   __syncthreads();
   {   // places: sums over (adapter, warp)
@@ -141,29 +148,38 @@ __global__ void __launch_bounds__(1024) plan_kernel(int rows, int count, int tm,
   }
   __syncthreads();
   if (warp < sorters)
-    for (int b = r0; b < r1; b += 32) {
-      const bool in = b + lane < r1;
-      const int key = in ? key_of(b + lane) : -1;
-      const unsigned same = __match_any_sync(0xffffffffu, key), before = same & ((1u << lane) - 1);
-      const int at = in ? counts[key * sorters + warp] + __popc(before) : 0;
-      __syncwarp();
-      if (in) {
-        plan[at_order + at] = b + lane;
-        if (before == 0) counts[key * sorters + warp] += __popc(same);
+    for (int b = r0; b < r1; b += 32 * Q) {
+      int key[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) key[q] = b + q * 32 + lane < r1 ? key_of(b + q * 32 + lane) : -1;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        if (b + q * 32 >= r1) break;
+        const unsigned same = __match_any_sync(0xffffffffu, key[q]), before = same & ((1u << lane) - 1);
+        const bool in = key[q] >= 0;
+        const int at = in ? counts[key[q] * sorters + warp] + __popc(before) : 0;
+        __syncwarp();
+        if (in) {
+          plan[at_order + at] = b + q * 32 + lane;
+          if (before == 0) counts[key[q] * sorters + warp] += __popc(same);
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
 }
 
 // ---- loads ------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(void* dst, const void* src, int bytes) {   // the rest of the 16 is zero
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_at(dst)), "l"(src), "r"(bytes) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(shared_at(dst)), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+__device__ __forceinline__ void prefetch(const void* p, size_t bytes) {   // into L2; both multiples of 16
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((uint32_t)bytes) : "memory");
+}
 // Rows of `pieces` x 16 bytes into shared memory: row r from row(r) (null: zeros), from column c0 on, zero past `cols`.  `vec`: the rows start on
 // 16-byte boundaries (then the copies are asynchronous).
 template <typename T, typename Row>
@@ -234,15 +250,18 @@ struct Args {
   const void *X, *Y;          // [rows][K]; [rows][N], or null: nothing is added
   const void *F1, *F2;        // forward: A [K][R], B [R][N] of an adapter; BACK: B [R][K], A [N][R]
   const float* scale;
-  const int *start, *tile_adapter, *tile_first, *order, *head;
+  const int *start, *tile_adapter, *tile_first, *order, *head;   // of the plan; or
+  const int* adapters;        // of each row, at most kThreads of them: every CTA finds its tile itself
   void *out, *V;              // [rows][N]; [rows][R] or null
   int vx, vy, v1, v2;         // rows of X, of Y and out, of the factors start on 16-byte boundaries
 };
 
 template <typename T, int TM, int RP>
 struct Shape {
-  static constexpr int E = 16 / sizeof(T), KC = 256 / sizeof(T);        // a chunk is 256 bytes of each row
-  static constexpr int xs = 256 + 16;                                   // bytes from row to row: ldmatrix and 16-byte reads without conflicts
+  // A chunk is 128 bytes of each of 64 rows, so that three or four CTAs share an SM (with 256 bytes two; 4096 rows 4096 -> 4096 at rank 16
+  // 39 us), or 256 bytes of 16.
+  static constexpr int CB = TM == 64 ? 128 : 256, E = 16 / sizeof(T), KC = CB / sizeof(T), pieces = CB / 16;
+  static constexpr int xs = CB + 16;                                    // bytes from row to row: ldmatrix and 16-byte reads without conflicts
   static constexpr int ls = RP * (int)sizeof(T) + 16;                   // of a factor with the rank innermost
   static constexpr int factor = KC * ls > RP * xs ? KC * ls : RP * xs;
   static constexpr int stage = TM * xs + factor;
@@ -270,17 +289,58 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
   grid_dependency_wait();   // the plan
   const int tile = (int)(blockIdx.x / csize);
-  if (tile >= g.head[0]) return;   // (all CTAs of the cluster)
-  const int a = g.tile_adapter[tile], first = g.tile_first[tile], len = min(TM, g.start[a + 1] - first);
+  int a, len;
+  if (g.adapters) {
+    // A row whose rank among its adapter's rows is a multiple of TM leads a tile; the tiles are in the order of their leaders.
+    int *keys = reinterpret_cast<int*>(sm), *tiles = keys + kThreads, *mine = tiles + kWarps;   // (where the ring will be)
+    int key = -1;
+    if (tid < g.rows) {
+      key = g.adapters[tid];
+      if (key < 0 || key > g.count) key = g.count;
+    }
+    keys[tid] = key;
+    __syncthreads();
+    int rank = 0;
+    for (int j = 0; j < g.rows; j += 4) {
+      const int4 k = *reinterpret_cast<const int4*>(keys + j);
+      rank += (k.x == key && j < tid) + (k.y == key && j + 1 < tid) + (k.z == key && j + 2 < tid) + (k.w == key && j + 3 < tid);
+    }
+    const bool leads = tid < g.rows && rank % TM == 0;
+    const unsigned leaders = __ballot_sync(0xffffffffu, leads);
+    if (lane == 0) tiles[warp] = __popc(leaders);
+    __syncthreads();
+    int before = __popc(leaders & ((1u << lane) - 1)), total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      before += w < warp ? tiles[w] : 0;
+      total += tiles[w];
+    }
+    if (tile >= total) return;   // (all CTAs of the cluster)
+    if (leads && before == tile) {
+      mine[0] = key;
+      mine[1] = rank;
+    }
+    __syncthreads();
+    a = mine[0];
+    const int place = rank - mine[1];
+    const bool in = key == a && place >= 0 && place < TM;
+    if (in) rowat[place] = tid;
+    len = __syncthreads_count(in);
+  } else {
+    if (tile >= g.head[0]) return;   // (all CTAs of the cluster)
+    a = g.tile_adapter[tile];
+    const int first = g.tile_first[tile];
+    len = min(TM, g.start[a + 1] - first);
+    if (tid < len) rowat[tid] = g.order[first + tid];
+    __syncthreads();
+  }
   const T *X = static_cast<const T*>(g.X), *Y = static_cast<const T*>(g.Y);
   T* out = static_cast<T*>(g.out);
   const int K = g.K, N = g.N, R = g.R;
-  if (tid < TM) rowat[tid] = tid < len ? g.order[first + tid] : 0;
-  __syncthreads();
   const int nn = (N + KC - 1) / KC, nper = (nn + (int)csize - 1) / (int)csize, n0 = min(nn, (int)crank * nper), n1 = min(nn, n0 + nper);
   const auto store_chunk = [&](const char* src, int c0) {   // [len][KC] in shared memory -> out
-    for (int i = tid; i < len * 16; i += kThreads) {
-      const int r = i >> 4, q = i & 15, c = c0 + q * E;
+    for (int i = tid; i < len * S::pieces; i += kThreads) {
+      const int r = i / S::pieces, q = i % S::pieces, c = c0 + q * E;
       if (c >= N) continue;
       T* to = out + (size_t)rowat[r] * N + c;
       const uint4 v = *reinterpret_cast<const uint4*>(src + r * S::xs + q * 16);
@@ -299,7 +359,7 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
     if (out == Y) return;
     for (int n = n0; n < n1; ++n) {
       const auto row = [&](int r) { return Y && r < len ? Y + (size_t)rowat[r] * N : nullptr; };
-      load_rows<T>(sm, S::xs, TM, 16, g.out, row, n * KC, N, g.vy);
+      load_rows<T>(sm, S::xs, TM, S::pieces, g.out, row, n * KC, N, g.vy);
       copies_end_group();
       copies_wait<0>();
       __syncthreads();
@@ -312,17 +372,30 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
   // a factor's chunk: KC features by the ranks, as it lies in memory
   const auto load_factor = [&](char* dst, const T* F, int n, bool long_rows, int c0, bool vec) {
     if (long_rows)
-      load_rows<T>(dst, S::xs, RP, 16, F, [&](int r) { return r < R ? F + (size_t)r * n : nullptr; }, c0, n, vec);
+      load_rows<T>(dst, S::xs, RP, S::pieces, F, [&](int r) { return r < R ? F + (size_t)r * n : nullptr; }, c0, n, vec);
     else
       load_rows<T>(dst, S::ls, KC, RP / E, F, [&](int r) { return c0 + r < n ? F + (size_t)(c0 + r) * R : nullptr; }, 0, R, vec);
   };
+
+  // what the second product reads is on its way to L2 meanwhile
+  if (n1 > n0) {
+    const int c0 = n0 * KC, cols = min(N, n1 * KC) - c0;
+    if (Y && g.vy && tid < len) prefetch(Y + (size_t)rowat[tid] * N + c0, cols * sizeof(T));
+    if (g.v2) {
+      if (BACK) {
+        if (tid == 128 && cols < 4096) prefetch(F2 + (size_t)c0 * R, (size_t)cols * R * sizeof(T));
+      } else if (tid >= 128 && tid - 128 < R) {
+        prefetch(F2 + (size_t)(tid - 128) * N + c0, cols * sizeof(T));
+      }
+    }
+  }
 
   // ---- V: this CTA's part of the sum over K ----
   const int nk = (K + KC - 1) / KC, kper = (nk + (int)csize - 1) / (int)csize, k0 = min(nk, (int)crank * kper), k1 = min(nk, k0 + kper);
   const auto load_k = [&](int k) {
     if (k < k1) {
       char* st = sm + (k - k0) % S::stages * S::stage;
-      load_rows<T>(st, S::xs, TM, 16, X, [&](int r) { return r < len ? X + (size_t)rowat[r] * K : nullptr; }, k * KC, K, g.vx);
+      load_rows<T>(st, S::xs, TM, S::pieces, X, [&](int r) { return r < len ? X + (size_t)rowat[r] * K : nullptr; }, k * KC, K, g.vx);
       load_factor(st + TM * S::xs, F1, K, BACK, k * KC, g.v1);
     }
     copies_end_group();
@@ -340,7 +413,7 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
     load_k(k + S::stages - 1);
     const char *xt = sm + (k - k0) % S::stages * S::stage, *ft = xt + TM * S::xs;
     if constexpr (F32) {
-      constexpr int KW = KC / S::KG;   // 8, or with groups of ranks 16, 32
+      constexpr int KW = KC / S::KG;   // 4 or 8, with groups of ranks more
 #pragma unroll 2
       for (int q = kg * KW; q < (kg + 1) * KW; q += 4) {
         float x[LR][4];
@@ -370,7 +443,7 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
         }
       }
     } else {
-      constexpr int KW = KC / S::KG;   // 64 or 16
+      constexpr int KW = KC / S::KG;   // 32 or 16
 #pragma unroll
       for (int q = kg * KW; q < (kg + 1) * KW; q += 16) {
         uint32_t x[4];
@@ -415,7 +488,7 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
   const auto load_n = [&](int n) {
     if (n < n1) {
       char* st = sm + (n - n0) % S::stages * S::stage;
-      if (Y) load_rows<T>(st, S::xs, TM, 16, Y, [&](int r) { return r < len ? Y + (size_t)rowat[r] * N : nullptr; }, n * KC, N, g.vy);
+      if (Y) load_rows<T>(st, S::xs, TM, S::pieces, Y, [&](int r) { return r < len ? Y + (size_t)rowat[r] * N : nullptr; }, n * KC, N, g.vy);
       load_factor(st + TM * S::xs, F2, N, !BACK, n * KC, g.v2);
     }
     copies_end_group();
@@ -472,40 +545,39 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
     char* yt = sm + (n - n0) % S::stages * S::stage;
     const char* ft = yt + TM * S::xs;
     if constexpr (F32) {
-      constexpr int RW = TM / kWarps;   // rows of a warp; a lane has two columns
-      float o[RW][2] = {};
+      constexpr int RW = TM / kWarps, CL = KC / 32;   // rows of a warp, columns of a lane
+      float o[RW][CL] = {};
 #pragma unroll 4
       for (int j = 0; j < RP; j += 4) {
         float v[RW][4];
 #pragma unroll
         for (int i = 0; i < RW; ++i) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(vs + (warp * RW + i) * S::ls + j * 4);
-        float f[2][4];
+        float f[CL][4];
         if (BACK) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(f[h]) = *reinterpret_cast<const float4*>(ft + (lane + 32 * h) * S::ls + j * 4);
+          for (int h = 0; h < CL; ++h) *reinterpret_cast<float4*>(f[h]) = *reinterpret_cast<const float4*>(ft + (lane + 32 * h) * S::ls + j * 4);
         } else {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            f[0][u] = *reinterpret_cast<const float*>(ft + (j + u) * S::xs + lane * 4);
-            f[1][u] = *reinterpret_cast<const float*>(ft + (j + u) * S::xs + (lane + 32) * 4);
-          }
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int h = 0; h < CL; ++h) f[h][u] = *reinterpret_cast<const float*>(ft + (j + u) * S::xs + (lane + 32 * h) * 4);
         }
 #pragma unroll
         for (int i = 0; i < RW; ++i)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < CL; ++h)
 #pragma unroll
             for (int u = 0; u < 4; ++u) o[i][h] = fmaf(v[i][u], f[h][u], o[i][h]);
       }
 #pragma unroll
       for (int i = 0; i < RW; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < CL; ++h) {
           float* p = reinterpret_cast<float*>(yt + (warp * RW + i) * S::xs) + lane + 32 * h;
           *p = Y ? *p + o[i][h] : o[i][h];
         }
     } else {
-      constexpr int NW = KC / NG;   // columns of a warp: 64 or 16
+      constexpr int NW = KC / NG;   // columns of a warp: 32 or 16
       const int nc = (warp / S::MG) * NW;
 #pragma unroll
       for (int q = 0; q < NW; q += 16) {
@@ -551,8 +623,10 @@ template <typename T, int RP>
 struct GradShape {
   static constexpr int E = 16 / sizeof(T), LT = 256 / sizeof(T), KT = sizeof(T) == 4 ? 32 : 64;   // features and rows of a step
   static constexpr int zs = 256 + 16, ws = RP * (int)sizeof(T) + 16;
-  static constexpr int stage = KT * (zs + ws), stages = RP <= 64 ? 4 : 3;
-  static constexpr int smem = stages * stage;
+  static constexpr int stage = KT * (zs + ws), stages = 3;
+  static constexpr int index = 2 * KT * 4, table = 1024;   // rows of two steps; adapters whose starts fit beside them
+  static constexpr int smem = stages * stage + index + table * 4;
+  static constexpr int ctas() { return 227 * 1024 / (smem + 1024); }   // of an SM
 };
 __device__ __forceinline__ int range_rows(const GradArgs& g, int kt) {   // of a range: a multiple of a step
   const int each = (g.head[1] + g.ranges - 1) / g.ranges;
@@ -570,7 +644,7 @@ __device__ __forceinline__ int adapter_at(const int* start, int count, int pos) 
 struct Steps {
   const int* start;
   int count, end, pos, a, stop;   // stop: where the adapter's rows (of the range) end
-  __device__ Steps(const GradArgs& g, int b, int e) : start(g.start), count(g.count), end(e), pos(b), a(0), stop(b) { find(); }
+  __device__ Steps(const int* start_, int count_, int b, int e) : start(start_), count(count_), end(e), pos(b), a(0), stop(b) { find(); }
   __device__ void find() {
     if (pos >= end) return;
     a = adapter_at(start, count, pos);
@@ -597,21 +671,43 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
   T* out = static_cast<T*>(second ? g.dB : g.dA);
   const bool vz = second ? g.vy : g.vx;
   const int per = range_rows(g, KT), b = min(g.head[1], (int)blockIdx.y * per), e = min(g.head[1], b + per);
-  Steps load(g, b, e), at = load;
+  // Where the adapters' rows start, beside the ring where they fit: a step that begins an adapter searches them.
+  int *index = reinterpret_cast<int*>(sm + S::stages * S::stage), *table = index + 2 * KT;
+  const bool fits = g.count + 2 <= S::table;
+  if (fits)
+    for (int i = tid; i < g.count + 2; i += kThreads) table[i] = g.start[i];
+  __syncthreads();
+  const int* start = fits ? table : g.start;
+  Steps load(start, g.count, b, e), at = load;
   int loaded = 0;
+  // The rows of a step come from the order: read one step ahead into a register, and into shared memory before the barrier that the copies wait for.
+  int ahead = tid < KT && load.pos + tid < e ? g.order[load.pos + tid] : 0;
+  const auto next_rows = [&] {
+    if (tid < KT) index[loaded % 2 * KT + tid] = ahead;
+    if (load.done()) return;
+    Steps then = load;
+    then.next(KT);
+    ahead = tid < KT && then.pos + tid < e ? g.order[then.pos + tid] : 0;
+  };
   const auto load_step = [&] {
     if (!load.done()) {
       char* st = sm + loaded % S::stages * S::stage;
-      const int n = min(KT, load.stop - load.pos), p = load.pos;
-      load_rows<T>(st, S::zs, KT, 16, Z, [&](int r) { return r < n ? Z + (size_t)g.order[p + r] * L : nullptr; }, l0, L, vz);
-      load_rows<T>(st + KT * S::zs, S::ws, KT, RP / E, W, [&](int r) { return r < n ? W + (size_t)g.order[p + r] * R : nullptr; }, 0, R, g.vr);
+      const int n = min(KT, load.stop - load.pos);
+      const int* rows = index + loaded % 2 * KT;
+      load_rows<T>(st, S::zs, KT, 16, Z, [&](int r) { return r < n ? Z + (size_t)rows[r] * L : nullptr; }, l0, L, vz);
+      load_rows<T>(st + KT * S::zs, S::ws, KT, RP / E, W, [&](int r) { return r < n ? W + (size_t)rows[r] * R : nullptr; }, 0, R, g.vr);
       load.next(KT);
       ++loaded;
     }
     copies_end_group();
   };
+  next_rows();
 #pragma unroll
-  for (int s = 0; s < S::stages - 1; ++s) load_step();
+  for (int s = 0; s < S::stages - 1; ++s) {
+    __syncthreads();
+    load_step();
+    next_rows();
+  }
   // fp32: a warp has eight features, a lane LR of them and LC ranks; 16 bits: a warp has sixteen features and all ranks
   constexpr int LC = RP == 16 ? 2 : 4, CGN = RP / LC, LR = CGN / 4;   // 8 / (32 / CGN)
   float acc[F32 ? LR : RP / 8][F32 ? LC : 4] = {};
@@ -620,6 +716,7 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
     copies_wait<S::stages - 2>();
     __syncthreads();
     load_step();
+    next_rows();
     const char *zt = sm + k % S::stages * S::stage, *wt = zt + KT * S::zs;
     if constexpr (F32) {
 #pragma unroll 4
@@ -654,7 +751,7 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
     at.next(KT);
     if (!last) continue;
     // the adapter's rows of this range end here
-    const int ab = g.start[a], ae = g.start[a + 1];
+    const int ab = start[a], ae = start[a + 1];
     const bool whole = ab >= b && ae <= e;
     float* p = g.partial + ((size_t)(blockIdx.y * 2 + (ab >= b ? 1 : 0)) * (g.I + g.O) + (second ? g.I : 0)) * RP;
     const auto put = [&](int l, int r, float v) {
@@ -694,19 +791,31 @@ __global__ void __launch_bounds__(kThreads) join_grads_kernel(const __grid_const
   const int a = blockIdx.x, ab = g.start[a], ae = g.start[a + 1], per = range_rows(g, KT);
   const int r0 = ab / per, r1 = ae > ab ? (ae - 1) / per : r0;
   if (ae > ab && r0 == r1) return;
-  const long na = g.dA ? (long)g.I * g.R : 0, n = na + (g.dB ? (long)g.O * g.R : 0);
-  for (long i = (long)blockIdx.y * kThreads + threadIdx.x; i < n; i += (long)gridDim.y * kThreads) {
-    const bool second = i >= na;
-    const long q = second ? i - na : i;
-    const int l = second ? (int)(q % g.O) : (int)(q / g.R), r = second ? (int)(q / g.O) : (int)(q % g.R);
-    float v = 0.f;
+  // A thread has a feature and four ranks; neighbours have neighbouring features.
+  constexpr int Q = RP / 4;
+  const int la = g.dA ? g.I : 0, n = la + (g.dB ? g.O : 0), quads = (g.R + 3) / 4;
+  for (int i = blockIdx.y * kThreads + threadIdx.x; i < n * quads; i += gridDim.y * kThreads) {
+    const int q = i / n, x = i - q * n;
+    const bool second = x >= la;
+    const int l = second ? x - la : x, L = second ? g.O : g.I;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (ae > ab) {
-      const float* p = g.partial + ((size_t)(second ? g.I : 0) + l) * RP + r;
-      const size_t step = (size_t)(g.I + g.O) * RP;
+      const float4* p = reinterpret_cast<const float4*>(g.partial) + ((size_t)(second ? g.I : 0) + l) * Q + q;
+      const size_t step = (size_t)(g.I + g.O) * Q;
       v = p[(size_t)(2 * r0 + 1) * step];
-      for (int k = r0 + 1; k <= r1; ++k) v += p[(size_t)(2 * k) * step];
+#pragma unroll 4
+      for (int k = r0 + 1; k <= r1; ++k) {
+        const float4 w = p[(size_t)(2 * k) * step];
+        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+      }
     }
-    static_cast<T*>(second ? g.dB : g.dA)[(size_t)a * (second ? g.O : g.I) * g.R + q] = (T)v;
+    const float e[4] = {v.x, v.y, v.z, v.w};
+    T* out = static_cast<T*>(second ? g.dB : g.dA) + (size_t)a * L * g.R;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = q * 4 + j;
+      if (r < g.R) out[second ? (size_t)r * L + l : (size_t)l * g.R + r] = (T)e[j];
+    }
   }
 }
 
@@ -723,10 +832,16 @@ int launch_tiles(const Args& g, int tiles, cudaStream_t st) {
   const auto kern = adapters_kernel<T, TM, RP, BACK>;
   static std::atomic<int> set[64];
   B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, S::smem));
-  // CTAs of a tile: as many as fill the machine twice over, with a chunk of the longer product for each
+  // CTAs of a tile: as many as the machine holds at once, with a chunk of the longer product for each
+  static std::atomic<int> resident{0};
+  int per = resident.load(std::memory_order_relaxed);
+  if (!per) {
+    B200CP_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, kThreads, S::smem));
+    resident.store(per = std::max(per, 1), std::memory_order_relaxed);
+  }
   int c = 1;
   const int chunks = std::max(ceil_div(g.K, S::KC), ceil_div(g.N, S::KC));
-  while (c < 8 && tiles * c < 2 * sms() && 2 * c <= chunks) c *= 2;
+  while (c < 8 && (long)tiles * c * 2 <= (long)sms() * per && 2 * c <= chunks) c *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)tiles * c);
   cfg.blockDim = dim3(kThreads);
@@ -754,10 +869,20 @@ int launch_rank(const Args& g, const Plan& p, cudaStream_t st) {
 #undef RANK
 }
 int padded(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
-int ranges_of(int rows, int I, int O, int type) {
-  const int lt = type == B200CP_FLOAT32 ? 64 : 128, kt = type == B200CP_FLOAT32 ? 32 : 64;
-  const int tiles = ceil_div(I, lt) + ceil_div(O, lt);
-  return std::max(1, std::min(ceil_div(4 * 148, tiles), ceil_div(rows, kt)));
+template <typename T, int RP>
+int ranges_for(int rows, int I, int O) {   // as many as the machine holds at once with all tiles of features
+  using S = GradShape<T, RP>;
+  const int tiles = ceil_div(I, S::LT) + ceil_div(O, S::LT);
+  return std::max(1, std::min({148 * S::ctas() / tiles, ceil_div(rows, S::KT), 65535}));
+}
+int ranges_of(int rows, int I, int O, int R, int type) {
+  const bool f32 = type == B200CP_FLOAT32;
+  switch (padded(R)) {
+    case 16: return f32 ? ranges_for<float, 16>(rows, I, O) : ranges_for<__half, 16>(rows, I, O);
+    case 32: return f32 ? ranges_for<float, 32>(rows, I, O) : ranges_for<__half, 32>(rows, I, O);
+    case 64: return f32 ? ranges_for<float, 64>(rows, I, O) : ranges_for<__half, 64>(rows, I, O);
+    default: return f32 ? ranges_for<float, 128>(rows, I, O) : ranges_for<__half, 128>(rows, I, O);
+  }
 }
 template <typename T, int RP>
 int launch_grads(const GradArgs& g, cudaStream_t st) {
@@ -770,8 +895,8 @@ int launch_grads(const GradArgs& g, cudaStream_t st) {
     B200CP_CUDA_OK(launch_kernel(kern, dim3(tiles, g.ranges), dim3(kThreads), S::smem, st, true, g));
     B200CP_LAUNCH_OK("adapter_grads_kernel");
   }
-  const long n = (long)g.R * ((g.dA ? g.I : 0) + (g.dB ? g.O : 0));
-  const int per = (int)std::min<long>(65535, std::min<long>((n + 4 * kThreads - 1) / (4 * kThreads), std::max(1, 16 * 148 / g.count)));
+  const long n = (long)ceil_div(g.R, 4) * ((g.dA ? g.I : 0) + (g.dB ? g.O : 0));
+  const int per = (int)std::min<long>((n + kThreads - 1) / kThreads, std::max(1, 16 * 148 / g.count));
   B200CP_CUDA_OK(launch_kernel(join_grads_kernel<T, RP>, dim3(g.count, per), dim3(kThreads), 0, st, true, g));
   B200CP_LAUNCH_OK("join_grads_kernel");
   return B200CP_OK;
@@ -790,8 +915,8 @@ int check_sizes(const char* who, int rows, int I, int O, int R, int count, int t
     return fail(B200CP_ERR_INVALID_ARG, "%s: rows=%d I=%d O=%d R=%d count=%d", who, rows, I, O, R, count);
   if (type != B200CP_FLOAT32 && type != B200CP_BFLOAT16 && type != B200CP_FLOAT16)
     return fail(B200CP_ERR_INVALID_ARG, "%s: type %d", who, type);
-  if (R > kMostRank || count > kMostAdapters || rows > (1 << 28) || I > (1 << 28) || O > (1 << 28))
-    return fail(B200CP_ERR_UNSUPPORTED, "%s: rank %d (at most %d), %d adapters (at most %d), %d rows, %d and %d features (at most 2^28)", who, R,
+  if (R > kMostRank || count > kMostAdapters || rows > (1 << 28) || I > (1 << 24) || O > (1 << 24))
+    return fail(B200CP_ERR_UNSUPPORTED, "%s: rank %d (at most %d), %d adapters (at most %d), %d rows (2^28), %d and %d features (2^24)", who, R,
                 kMostRank, count, kMostAdapters, rows, I, O);
   return B200CP_OK;
 }
@@ -803,9 +928,11 @@ void plan_into(const int* plan, const Plan& p, const int** head, const int** sta
 template <bool BACK>
 int run_tiles(int type, Args& g, const Plan& p, const int* plan, cudaStream_t st) {
   const size_t size = type == B200CP_FLOAT32 ? 4 : 2;
-  plan_into(plan, p, &g.head, &g.start, &g.order);
-  g.tile_adapter = plan + p.adapter;
-  g.tile_first = plan + p.first;
+  if (plan) {
+    plan_into(plan, p, &g.head, &g.start, &g.order);
+    g.tile_adapter = plan + p.adapter;
+    g.tile_first = plan + p.first;
+  }
   g.vx = rows16(g.X, g.K * size);
   g.vy = rows16(g.out, g.N * size) && (!g.Y || rows16(g.Y, g.N * size));
   g.v1 = rows16(g.F1, (BACK ? g.K : g.R) * size) && (size_t)g.K * g.R * size % 16 == 0;
@@ -847,19 +974,22 @@ int b200cp_adapter_plan(int rows, int count, const int* adapters, void* plan, si
 }
 
 int b200cp_dense_adapters(int rows, int I, int O, int R, int count, int type, const void* Y, const void* X, const void* A, const void* B,
-                          const float* scale, const void* plan, void* out, void* V, void* stream) {
+                          const float* scale, const int* adapters, const void* plan, void* out, void* V, void* stream) {
   if (int rc = check_sizes("b200cp_dense_adapters", rows, I, O, R, count, type)) return rc;
   if (rows == 0) return B200CP_OK;
-  if (!Y || !X || !A || !B || !plan || !out) return fail(B200CP_ERR_INVALID_ARG, "b200cp_dense_adapters: null pointer");
+  if (!Y || !X || !A || !B || (!plan && !adapters) || !out) return fail(B200CP_ERR_INVALID_ARG, "b200cp_dense_adapters: null pointer");
+  if (!plan && rows > B200CP_ADAPTERS_WITHOUT_PLAN)
+    return fail(B200CP_ERR_UNSUPPORTED, "b200cp_dense_adapters: %d rows without a plan (at most %d)", rows, B200CP_ADAPTERS_WITHOUT_PLAN);
   Args g{};
   g.rows = rows; g.K = I; g.N = O; g.R = R; g.count = count;
   g.X = X; g.Y = Y; g.F1 = A; g.F2 = B; g.scale = scale; g.out = out; g.V = V;
+  g.adapters = plan ? nullptr : adapters;
   return run_tiles<false>(type, g, plan_of(rows, count), static_cast<const int*>(plan), static_cast<cudaStream_t>(stream));
 }
 
 size_t b200cp_dense_adapters_bwd_workspace_bytes(int rows, int I, int O, int R, int count, int type) {
   if (check_sizes("b200cp_dense_adapters_bwd_workspace_bytes", rows, I, O, R, count, type)) return 0;
-  return w_bytes(rows, R, type) + (size_t)ranges_of(rows, I, O, type) * 2 * ((size_t)I + O) * padded(R) * sizeof(float);
+  return w_bytes(rows, R, type) + (size_t)ranges_of(rows, I, O, R, type) * 2 * ((size_t)I + O) * padded(R) * sizeof(float);
 }
 
 int b200cp_dense_adapters_bwd(int rows, int I, int O, int R, int count, int type, const void* dY, const void* X, const void* V,
@@ -883,7 +1013,7 @@ int b200cp_dense_adapters_bwd(int rows, int I, int O, int R, int count, int type
   }
   if (!dA && !dB) return B200CP_OK;
   GradArgs g{};
-  g.rows = rows; g.I = I; g.O = O; g.R = R; g.count = count; g.ranges = ranges_of(rows, I, O, type);
+  g.rows = rows; g.I = I; g.O = O; g.R = R; g.count = count; g.ranges = ranges_of(rows, I, O, R, type);
   g.tiles_i = dA ? ceil_div(I, type == B200CP_FLOAT32 ? 64 : 128) : 0;
   g.X = X; g.W = W; g.V = V; g.dY = dY; g.dA = dA; g.dB = dB;
   plan_into(static_cast<const int*>(plan), p, &g.head, &g.start, &g.order);

@@ -39,14 +39,18 @@ int size_arg(int64_t n, const char* name) {
 }
 
 // ---- low-rank adapters ------------------------------------------------------------------------------------------------
+// The adapters' numbers as the library takes them
+Tensor adapter_numbers(const Tensor& which, int64_t count) {
+  TORCH_CHECK_TYPE(which.scalar_type() == at::kInt || which.scalar_type() == at::kLong, "adapters must be an int32 or int64 CUDA tensor");
+  return contiguous(which.scalar_type() == at::kInt ? which : which.clamp(-1, count).to(at::kInt));
+}
 // The plan of a batch: bytes on the device that depend on the rows' adapters and on the number of adapters
 Tensor adapter_plan(const Tensor& which_, int64_t count) {
-  TORCH_CHECK_TYPE(which_.scalar_type() == at::kInt || which_.scalar_type() == at::kLong, "adapters must be an int32 or int64 CUDA tensor");
   const int rows = size_arg(which_.numel(), "the number of rows"), n = size_arg(count, "the number of adapters");
   const size_t need = b200cp_adapter_plan_bytes(rows, n);
   TORCH_CHECK_VALUE(need, "adapter_plan: ", rows, " rows and ", n, " adapters (1 to 16384 of them)");
   const c10::cuda::OptionalCUDAGuard guard(which_.device());
-  const Tensor which = contiguous(which_.scalar_type() == at::kInt ? which_ : which_.clamp(-1, count).to(at::kInt));
+  const Tensor which = adapter_numbers(which_, count);
   Tensor plan = bytes_on(need, which);
   ok(b200cp_adapter_plan(rows, n, static_cast<const int*>(which.const_data_ptr()), plan.data_ptr(), need, stream(which)));
   return plan;
@@ -86,15 +90,27 @@ struct Adapters {   // operands, checked and contiguous
   }
   // `which`: the adapter of every row, or (planned) the bytes of a plan
   Tensor plan(const Tensor& which, bool planned) const {
+    check_numbers(which, planned);
+    return planned ? which : adapter_plan(which, count);
+  }
+  // the numbers themselves where a batch is small enough to go without a plan, or else a plan (*planned)
+  Tensor numbers(const Tensor& which, bool* planned) const {
+    check_numbers(which, *planned);
+    if (*planned) return which;
+    *planned = rows > B200CP_ADAPTERS_WITHOUT_PLAN;
+    return *planned ? adapter_plan(which, count) : adapter_numbers(which, count);
+  }
+  void check_numbers(const Tensor& which, bool planned) const {
     TORCH_CHECK_VALUE(which.device() == x.device(), "the adapters' numbers are on ", which.device(), ", X on ", x.device());
     if (!planned) {
+      TORCH_CHECK_TYPE(which.scalar_type() == at::kInt || which.scalar_type() == at::kLong, "adapters must be an int32 or int64 CUDA tensor");
       TORCH_CHECK_VALUE(which.sizes() == x.sizes().slice(0, x.dim() - 1), "there are numbers of adapters for ", which.sizes(), ", X is ", x.sizes());
-      return adapter_plan(which, count);
+      TORCH_CHECK_VALUE(b200cp_adapter_plan_bytes(rows, count), rows, " rows and ", count, " adapters (1 to 16384 of them)");
+      return;
     }
     TORCH_CHECK_VALUE(which.scalar_type() == at::kByte && which.is_contiguous() &&
                           (size_t)which.numel() == std::max<size_t>(16, b200cp_adapter_plan_bytes(rows, count)),
                       "the plan is not one of ", rows, " rows and ", count, " adapters");
-    return which;
   }
   void takes(const Tensor& out, const Tensor& y) const {   // as the place of the result
     fits(out, "out");
@@ -105,14 +121,16 @@ struct Adapters {   // operands, checked and contiguous
   }
   const float* scales() const { return scale.defined() ? cp(scale) : nullptr; }
 };
-Tensor dense_adapters(const Adapters& a, const Tensor& y_, const Tensor& plan, Tensor out, Tensor* V) {
+Tensor dense_adapters(const Adapters& a, const Tensor& y_, const Tensor& which, bool planned, Tensor out, Tensor* V) {
   a.fits(y_, "Y");
   const Tensor y = contiguous(y_);
   if (!out.defined()) out = empty_as(y.sizes(), y);
   const c10::cuda::OptionalCUDAGuard guard(a.x.device());
   if (V) *V = empty_as({a.rows, a.R}, a.x);
+  const void* by = which.const_data_ptr();
   ok(b200cp_dense_adapters(a.rows, a.I, a.O, a.R, a.count, a.type, y.const_data_ptr(), a.x.const_data_ptr(), a.A.const_data_ptr(), a.B.const_data_ptr(),
-                           a.scales(), plan.const_data_ptr(), out.data_ptr(), V ? V->data_ptr() : nullptr, stream(a.x)));
+                           a.scales(), planned ? nullptr : static_cast<const int*>(by), planned ? by : nullptr, out.data_ptr(),
+                           V ? V->data_ptr() : nullptr, stream(a.x)));
   return out;
 }
 std::array<Tensor, 3> dense_adapters_backward(const Adapters& a, const Tensor& dy_, const Tensor& V, const Tensor& plan, bool need_x, bool need_a,
@@ -137,7 +155,7 @@ struct AdaptersNode : torch::autograd::Function<AdaptersNode> {
     const Tensor scale = scale_.value_or(Tensor());
     const Adapters a(x, A, B, scale);
     Tensor V;
-    Tensor out = dense_adapters(a, y, plan, Tensor(), &V);
+    Tensor out = dense_adapters(a, y, plan, true, Tensor(), &V);
     ctx->save_for_backward({x, A, B, plan, scale, V});
     return out;
   }
@@ -255,13 +273,14 @@ PYFN(py_dense_adapters) {
   count_args(n, 8);
   const Tensor &y = any_tensor(a[0], "Y"), &x = any_tensor(a[1], "X"), &A = any_tensor(a[2], "A"), &B = any_tensor(a[3], "B"),
                &which = any_tensor(a[4], "adapters");
-  const bool planned = truth(a[5]);
+  bool planned = truth(a[5]);
   const Tensor scale = optional_tensor(a[6], "scale"), to = optional_tensor(a[7], "out");
   Tensor out = unlocked([&] {
     const Adapters op(x, A, B, scale);
     op.fits(y, "Y");
     if (to.defined()) op.takes(to, y);
-    return dense_adapters(op, y, op.plan(which, planned), to, nullptr);
+    const Tensor by = op.numbers(which, &planned);
+    return dense_adapters(op, y, by, planned, to, nullptr);
   });
   if (to.defined()) written(to);
   return wrap(out);

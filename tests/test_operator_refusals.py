@@ -112,11 +112,12 @@ def test_adapter_sizes_the_library_refuses(lib_built):
     assert lib.b200cp_adapter_plan(4, 3, None, None, 0, None) == -1
     assert lib.b200cp_adapter_plan(4, 3, 16, 16, 8, None) == -3        # too small a plan
     assert lib.b200cp_adapter_plan(4, 3, 16, 24, 1 << 20, None) == -3  # not on sixteen bytes
-    fwd = lambda *a: lib.b200cp_dense_adapters(*a, *[16] * 4, None, 16, 16, None, None)  # noqa: E731
+    fwd = lambda *a, by=(16, None): lib.b200cp_dense_adapters(*a, *[16] * 4, None, *by, 16, None, None)  # noqa: E731
     assert fwd(0, 4, 4, 4, 1, 0) == 0
     assert fwd(4, 4, 4, 129, 1, 0) == -2 and fwd(4, 4, 4, 4, 16385, 0) == -2
     assert fwd(4, 0, 4, 4, 1, 0) == -1 and fwd(4, 4, 4, 4, 1, 3) == -1 and fwd(-1, 4, 4, 4, 1, 0) == -1
-    assert lib.b200cp_dense_adapters(4, 4, 4, 4, 1, 0, *[None] * 9) == -1
+    assert fwd(257, 4, 4, 4, 1, 0) == -2 and fwd(4, 4, 4, 4, 1, 0, by=(None, None)) == -1   # too many rows without a plan; neither
+    assert lib.b200cp_dense_adapters(4, 4, 4, 4, 1, 0, *[None] * 10) == -1
     assert lib.b200cp_dense_adapters_bwd(4, 4, 4, 4, 1, 0, *[16] * 5, None, 16, 16, 16, 16, 16, 4, None) == -3
     assert lib.b200cp_dense_adapters_bwd(4, 4, 4, 4, 1, 0, *[None] * 5, None, 16, 16, 16, 16, 16, 1 << 20, None) == -1
 
