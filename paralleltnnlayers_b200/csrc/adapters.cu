@@ -180,22 +180,45 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 __device__ __forceinline__ void prefetch(const void* p, size_t bytes) {   // into L2; both multiples of 16
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((uint32_t)bytes) : "memory");
 }
-// Rows of `pieces` x 16 bytes into shared memory: row r from row(r) (null: zeros), from column c0 on, zero past `cols`.  `vec`: the rows start on
-// 16-byte boundaries (then the copies are asynchronous).
-template <typename T, typename Row>
-__device__ __forceinline__ void load_rows(char* dst, int stride, int rows, int pieces, const void* any, Row row, int c0, int cols, bool vec) {
-  constexpr int E = 16 / sizeof(T);
-  for (int i = threadIdx.x; i < rows * pieces; i += kThreads) {
-    const int r = i / pieces, q = i - r * pieces, c = c0 + q * E;
+// ROWS rows of PIECES x 16 bytes into shared memory, a thread the same place of every row that it has: row r from row(r) (null: zeros), from column c0
+// on, zero past `cols`.  `vec`: the rows start on 16-byte boundaries (then the copies are asynchronous).  Else fp32 comes in asynchronous
+// words, and 16-bit values in words that a shift puts in place (a word that reaches past the row's ends is not read).
+template <typename T, int ROWS, int PIECES, typename Row>
+__device__ __forceinline__ void load_rows(char* dst, int stride, Row row, int c0, int cols, bool vec, const void* any) {
+  constexpr int E = 16 / sizeof(T), STEP = kThreads / PIECES, N = (ROWS + STEP - 1) / STEP;
+  const int q = threadIdx.x % PIECES, r0 = threadIdx.x / PIECES, c = c0 + q * E, left = min(E, max(0, cols - c));
+  dst += r0 * stride + q * 16;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int r = r0 + i * STEP;
+    if (ROWS % STEP != 0 && r >= ROWS) break;
     const T* src = row(r);
-    const int left = src ? min(E, max(0, cols - c)) : 0;
-    char* to = dst + r * stride + q * 16;
+    char* to = dst + i * STEP * stride;
     if (vec) {
-      copy16(to, left > 0 ? (const void*)(src + c) : any, left * (int)sizeof(T));
+      copy16(to, src && left ? (const void*)(src + c) : any, src ? left * (int)sizeof(T) : 0);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const bool in = src && k < left;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_at(to + 4 * k)), "l"(in ? (const void*)(src + c + k) : any), "r"(in ? 4 : 0)
+                     : "memory");
+      }
+    } else if (src && c > 0 && c + E < cols) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(src + c);
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+      uint32_t x[E / 2 + 1];
+#pragma unroll
+      for (int k = 0; k < E / 2; ++k) x[k] = w[k];
+      if (at & 2) {
+        x[E / 2] = w[E / 2];
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) x[k] = __funnelshift_r(x[k], x[k + 1], 16);
+      }
+      *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
     } else {
       alignas(16) T v[E];
 #pragma unroll
-      for (int k = 0; k < E; ++k) v[k] = k < left ? src[c + k] : (T)0.f;
+      for (int k = 0; k < E; ++k) v[k] = src && k < left ? src[c + k] : (T)0.f;
       *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(v);
     }
   }
@@ -242,6 +265,22 @@ __device__ __forceinline__ void b_block(uint32_t (&r)[4], const char* p, int str
     ldsm4(r, p + ((l & 7) + (l >> 4) * 8) * stride + ((l >> 3) & 1) * 16);
   else
     ldsm4t(r, p + ((l & 7) + ((l >> 3) & 1) * 8) * stride + (l >> 4) * 16);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
 // ---- forward and dX ---------------------------------------------------------------------------------------------------------
@@ -339,27 +378,26 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
   const int K = g.K, N = g.N, R = g.R;
   const int nn = (N + KC - 1) / KC, nper = (nn + (int)csize - 1) / (int)csize, n0 = min(nn, (int)crank * nper), n1 = min(nn, n0 + nper);
   const auto store_chunk = [&](const char* src, int c0) {   // [len][KC] in shared memory -> out
-    for (int i = tid; i < len * S::pieces; i += kThreads) {
-      const int r = i / S::pieces, q = i % S::pieces, c = c0 + q * E;
-      if (c >= N) continue;
-      T* to = out + (size_t)rowat[r] * N + c;
-      const uint4 v = *reinterpret_cast<const uint4*>(src + r * S::xs + q * 16);
-      if (g.vy && c + E <= N) {
-        *reinterpret_cast<uint4*>(to) = v;
-      } else {
-        alignas(16) T e[E];
-        *reinterpret_cast<uint4*>(e) = v;
+    if (g.vy) {
+      const int q = tid % S::pieces, c = c0 + q * E;
+      if (c >= N) return;   // (rows of whole pieces)
 #pragma unroll
-        for (int k = 0; k < E; ++k)
-          if (c + k < N) to[k] = e[k];
+      for (int i = 0; i < TM * S::pieces / kThreads; ++i) {
+        const int r = tid / S::pieces + i * (kThreads / S::pieces);
+        if (r < len) *reinterpret_cast<uint4*>(out + (size_t)rowat[r] * N + c) = *reinterpret_cast<const uint4*>(src + r * S::xs + q * 16);
       }
+    } else {
+      const int q = tid % KC, c = c0 + q;
+      if (c >= N) return;
+#pragma unroll 4
+      for (int r = tid / KC; r < len; r += kThreads / KC) out[(size_t)rowat[r] * N + c] = reinterpret_cast<const T*>(src + r * S::xs)[q];
     }
   };
   if (a == g.count) {   // rows without an adapter
     if (out == Y) return;
     for (int n = n0; n < n1; ++n) {
       const auto row = [&](int r) { return Y && r < len ? Y + (size_t)rowat[r] * N : nullptr; };
-      load_rows<T>(sm, S::xs, TM, S::pieces, g.out, row, n * KC, N, g.vy);
+      load_rows<T, TM, S::pieces>(sm, S::xs, row, n * KC, N, g.vy, g.out);
       copies_end_group();
       copies_wait<0>();
       __syncthreads();
@@ -372,9 +410,9 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
   // a factor's chunk: KC features by the ranks, as it lies in memory
   const auto load_factor = [&](char* dst, const T* F, int n, bool long_rows, int c0, bool vec) {
     if (long_rows)
-      load_rows<T>(dst, S::xs, RP, S::pieces, F, [&](int r) { return r < R ? F + (size_t)r * n : nullptr; }, c0, n, vec);
+      load_rows<T, RP, S::pieces>(dst, S::xs, [&](int r) { return r < R ? F + (size_t)r * n : nullptr; }, c0, n, vec, F);
     else
-      load_rows<T>(dst, S::ls, KC, RP / E, F, [&](int r) { return c0 + r < n ? F + (size_t)(c0 + r) * R : nullptr; }, 0, R, vec);
+      load_rows<T, KC, RP / E>(dst, S::ls, [&](int r) { return c0 + r < n ? F + (size_t)(c0 + r) * R : nullptr; }, 0, R, vec, F);
   };
 
   // what the second product reads is on its way to L2 meanwhile
@@ -395,7 +433,7 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
   const auto load_k = [&](int k) {
     if (k < k1) {
       char* st = sm + (k - k0) % S::stages * S::stage;
-      load_rows<T>(st, S::xs, TM, S::pieces, X, [&](int r) { return r < len ? X + (size_t)rowat[r] * K : nullptr; }, k * KC, K, g.vx);
+      load_rows<T, TM, S::pieces>(st, S::xs, [&](int r) { return r < len ? X + (size_t)rowat[r] * K : nullptr; }, k * KC, K, g.vx, X);
       load_factor(st + TM * S::xs, F1, K, BACK, k * KC, g.v1);
     }
     copies_end_group();
@@ -488,7 +526,7 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
   const auto load_n = [&](int n) {
     if (n < n1) {
       char* st = sm + (n - n0) % S::stages * S::stage;
-      if (Y) load_rows<T>(st, S::xs, TM, S::pieces, Y, [&](int r) { return r < len ? Y + (size_t)rowat[r] * N : nullptr; }, n * KC, N, g.vy);
+      if (Y) load_rows<T, TM, S::pieces>(st, S::xs, [&](int r) { return r < len ? Y + (size_t)rowat[r] * N : nullptr; }, n * KC, N, g.vy, Y);
       load_factor(st + TM * S::xs, F2, N, !BACK, n * KC, g.v2);
     }
     copies_end_group();
@@ -546,7 +584,11 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
     const char* ft = yt + TM * S::xs;
     if constexpr (F32) {
       constexpr int RW = TM / kWarps, CL = KC / 32;   // rows of a warp, columns of a lane
-      float o[RW][CL] = {};
+      float o[RW][CL];
+#pragma unroll
+      for (int i = 0; i < RW; ++i)
+#pragma unroll
+        for (int h = 0; h < CL; ++h) o[i][h] = Y ? reinterpret_cast<const float*>(yt + (warp * RW + i) * S::xs)[lane + 32 * h] : 0.f;
 #pragma unroll 4
       for (int j = 0; j < RP; j += 4) {
         float v[RW][4];
@@ -573,15 +615,25 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
       for (int i = 0; i < RW; ++i)
 #pragma unroll
         for (int h = 0; h < CL; ++h) {
-          float* p = reinterpret_cast<float*>(yt + (warp * RW + i) * S::xs) + lane + 32 * h;
-          *p = Y ? *p + o[i][h] : o[i][h];
+          reinterpret_cast<float*>(yt + (warp * RW + i) * S::xs)[lane + 32 * h] = o[i][h];
         }
     } else {
       constexpr int NW = KC / NG;   // columns of a warp: 32 or 16
       const int nc = (warp / S::MG) * NW;
 #pragma unroll
       for (int q = 0; q < NW; q += 16) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(yt + (mg * 16 + lr) * S::xs + (nc + q + lc * 2) * 2);   // two columns; of the other half 4 words on, of eight rows more
         float o[2][4] = {};
+        if (Y) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 y = unpack2<T>(at[h * 4 + e * 8 * (S::xs / 4)]);
+              o[h][2 * e] = y.x;
+              o[h][2 * e + 1] = y.y;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < RP; j += 16) {
           uint32_t f[4];
@@ -595,12 +647,7 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            T* p = reinterpret_cast<T*>(yt + (mg * 16 + lr + 8 * e) * S::xs) + nc + q + h * 8 + lc * 2;
-            const float y0 = Y ? (float)p[0] : 0.f, y1 = Y ? (float)p[1] : 0.f;
-            p[0] = (T)(y0 + o[h][2 * e]);
-            p[1] = (T)(y1 + o[h][2 * e + 1]);
-          }
+          for (int e = 0; e < 2; ++e) at[h * 4 + e * 8 * (S::xs / 4)] = pack2<T>(o[h][2 * e], o[h][2 * e + 1]);
       }
     }
     __syncthreads();
@@ -694,8 +741,8 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
       char* st = sm + loaded % S::stages * S::stage;
       const int n = min(KT, load.stop - load.pos);
       const int* rows = index + loaded % 2 * KT;
-      load_rows<T>(st, S::zs, KT, 16, Z, [&](int r) { return r < n ? Z + (size_t)rows[r] * L : nullptr; }, l0, L, vz);
-      load_rows<T>(st + KT * S::zs, S::ws, KT, RP / E, W, [&](int r) { return r < n ? W + (size_t)rows[r] * R : nullptr; }, 0, R, g.vr);
+      load_rows<T, KT, 16>(st, S::zs, [&](int r) { return r < n ? Z + (size_t)rows[r] * L : nullptr; }, l0, L, vz, Z);
+      load_rows<T, KT, RP / E>(st + KT * S::zs, S::ws, [&](int r) { return r < n ? W + (size_t)rows[r] * R : nullptr; }, 0, R, g.vr, W);
       load.next(KT);
       ++loaded;
     }
