@@ -434,8 +434,9 @@ int b200cp_dense_adapters_bwd(int rows, int I, int O, int R, int count, int type
 enum { B200CP_SILU = 0, B200CP_GELU = 1, B200CP_GELU_TANH = 2 };
 
 /* H = act(X Wg) * (X Wu), elementwise product, both projections in one kernel.  X [rows, I], Wg, Wu [I, F], H [rows, F] of one 16-bit
- * type (B200CP_BFLOAT16 or _FLOAT16); sums are fp32.  G, U (both or neither): [rows, F] floats, receive X Wg and X Wu for the
- * backward.  The workspace is 256-byte aligned (and may be NULL where the size is 0).  Beside b200cp_dense_matmul; no counterpart in the reference. */
+ * type (B200CP_BFLOAT16 or _FLOAT16); sums are fp32.  G, U (both or neither): [rows][F rounded up to a multiple of 8] floats, receive
+ * X Wg and X Wu for the backward.  X, Wg, Wu, G and U start on 16-byte boundaries, the workspace on a 256-byte one (it may be NULL
+ * where the size is 0).  Beside b200cp_dense_matmul; no counterpart in the reference. */
 size_t b200cp_dense_gated_workspace_bytes(int rows, int I, int F, int type);
 int b200cp_dense_gated(int rows, int I, int F, int type, int activation, const void* X, const void* Wg, const void* Wu, void* H, float* G,
                        float* U, void* workspace, size_t workspace_bytes, void* stream);

@@ -195,8 +195,9 @@ __device__ __forceinline__ float warp_max(float x) {   // of magnitudes
 // 1 / s, or 0 where s or that is no normal number (then every code of the block is found by the exact operations)
 __device__ __forceinline__ float inverse_of(float s) { return s > 1e-37f && s < 1e37f ? 1.f / s : 0.f; }
 
+// (Six CTAs on an SM: 59 M values with 8-bit moments 228 -> 204 us, five 216.)
 template <typename P, typename G, bool SMALL, int CAP>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<CAP> t) {
+__global__ void __launch_bounds__(kThreads, 6) adamw_kernel(const __grid_constant__ Table<CAP> t) {
   int a = 0, b = t.count;   // the tensor whose pieces hold this CTA's
   while (b - a > 1) {
     const int c = (a + b) / 2;

@@ -32,7 +32,8 @@ enum Form { kForward, kData, kWeights };
 constexpr int kTile = 256, kStep = 64, kHalf = 128 * kStep * 2, kStage = 2 * kHalf, kStages = 6;   // bytes: of an operand's half, of a step
 constexpr int kBox = 64 * kStep * 2;              // a box of 64 columns by 64 k
 constexpr int kReaders = 8, kThreads = 64 + 32 * kReaders;
-constexpr size_t kSmem = (size_t)kStages * kStage + 1024 + 256;
+constexpr int kPitch = 80, kPatch = 32 * kPitch;   // bytes of a row and of a warp's 32 x 32 block on its way out
+constexpr size_t kSmem = (size_t)kStages * kStage + kReaders * kPatch + 1024 + 256;
 
 struct Gemm {
   int M, N;                      // of a result
@@ -40,9 +41,9 @@ struct Gemm {
   int steps, first;              // of a sum; steps of its first product
   int act;
   void* out[2];
-  int vec;                       // rows of out start on 16-byte boundaries
+  int vec;                       // values that a store takes: 8, 2 or 1, by how the rows of out are aligned
   float *G, *U;                  // forward: where the sums are kept, or null
-  int vecg;
+  int ldg;                       // of their rows, a multiple of eight
 };
 
 __device__ __forceinline__ void tma_load_pair_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
@@ -88,29 +89,57 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
-// 16 values of a row from column n on (of N)
+// A warp's 32 rows of 32 values (a lane has a row) go through shared memory, so that neighbouring lanes store neighbouring columns: stores of a row
+// per lane write 32 sectors each, which in rows of odd length (one value per store) took ten times as long as the products.
 template <typename T>
-__device__ __forceinline__ void put16(T* row, int n, int N, bool vec, const float (&v)[16]) {
-  if (vec && n + 16 <= N) {
+__device__ __forceinline__ void put_block(uint8_t* patch, T* out, int vec, int m0, int M, int n, int N, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+  uint4* mine = reinterpret_cast<uint4*>(patch + lane * kPitch);
 #pragma unroll
-    for (int j = 0; j < 16; j += 8)
-      *reinterpret_cast<uint4*>(row + n + j) = make_uint4(pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]), pack2<T>(v[j + 4], v[j + 5]),
-                                                          pack2<T>(v[j + 6], v[j + 7]));
+  for (int j = 0; j < 4; ++j)
+    mine[j] = make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]), pack2<T>(v[8 * j + 4], v[8 * j + 5]),
+                         pack2<T>(v[8 * j + 6], v[8 * j + 7]));
+  __syncwarp();
+  const int rows = min(32, M - m0), cols = min(32, N - n);
+  if (vec == 8) {
+    const int q = lane & 3;
+    if (q * 8 < cols)
+#pragma unroll
+      for (int r = lane >> 2; r < 32; r += 8)
+        if (r < rows) *reinterpret_cast<uint4*>(out + (size_t)(m0 + r) * N + n + q * 8) = *reinterpret_cast<const uint4*>(patch + r * kPitch + q * 16);
+  } else if (vec == 2) {
+    const int q = lane & 15;
+    if (q * 2 < cols)
+#pragma unroll 4
+      for (int r = lane >> 4; r < rows; r += 2)
+        *reinterpret_cast<uint32_t*>(out + (size_t)(m0 + r) * N + n + q * 2) = *reinterpret_cast<const uint32_t*>(patch + r * kPitch + q * 4);
   } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (n + j < N) row[n + j] = (T)v[j];
+    if (lane < cols)
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r) out[(size_t)(m0 + r) * N + n + lane] = reinterpret_cast<const T*>(patch + r * kPitch)[lane];
   }
+  __syncwarp();
 }
-__device__ __forceinline__ void put16(float* row, int n, int N, bool vec, const float (&v)[16]) {
-  if (vec && n + 16 <= N) {
+// 32 values of a kept row; columns past the end are those of the row's padding, or of nothing
+__device__ __forceinline__ void keep_row(float* row, int n, int ld, const float (&v)[32]) {
 #pragma unroll
-    for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(row + n + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-  } else {
+  for (int j = 0; j < 32; j += 4)
+    if (n + j < ld) *reinterpret_cast<float4*>(row + n + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+}
+// 32 columns of the warp's lane quarter
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+      "%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (n + j < N) row[n + j] = v[j];
-  }
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // ---- the kernel ---------------------------------------------------------------------------------------------------------------
@@ -132,7 +161,8 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
              const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kStages * kStage);
+  uint8_t* patches = sm + kStages * kStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(patches + kReaders * kPatch);
   uint64_t* full = bars;                 // [kStages] the leader's: the step of both CTAs has landed  (tx bytes)
   uint64_t* empty = full + kStages;      // [kStages] the products that read the step are done         (commit, both CTAs)
   uint64_t* accfull = empty + kStages;   // [2] the sums of a tile are complete                        (commit, both CTAs)
@@ -237,32 +267,27 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
       if (!__all_sync(0xffffffffu, wait_or_abort(accfullb + buf * 8, (done / 2) & 1, abortb))) break;
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + ((uint32_t)(qd * 32) << 16) + buf * 256;
-      const int m = t.m0 + rank * 128 + qd * 32 + lane;
-      const bool in = m < g.M;
-      if (FORM == kForward) {
-        const size_t row = (size_t)m * g.N;
+      const int m0 = t.m0 + rank * 128 + qd * 32;
+      uint8_t* patch = patches + (warp - 2) * kPatch;
+      T* out = static_cast<T*>(g.out[FORM == kWeights ? t.result : 0]);
+      constexpr int cols = FORM == kForward ? 64 : 128;
+      if (m0 < g.M)
 #pragma unroll 1
-        for (int j = half * 64; j < half * 64 + 64 && t.n0 + j < g.N; j += 16) {
-          float a[16], u[16];
-          tmem_ld16(taddr + j, a);
-          tmem_ld16(taddr + 128 + j, u);
-          if (in && g.G) {
-            put16(g.G + row, t.n0 + j, g.N, g.vecg, a);
-            put16(g.U + row, t.n0 + j, g.N, g.vecg, u);
-          }
+        for (int j = half * cols; j < half * cols + cols && t.n0 + j < g.N; j += 32) {
+          float a[32];
+          tmem_ld32(taddr + j, a);
+          if constexpr (FORM == kForward) {
+            float u[32];
+            tmem_ld32(taddr + 128 + j, u);
+            if (g.G && m0 + lane < g.M) {
+              keep_row(g.G + (size_t)(m0 + lane) * g.ldg, t.n0 + j, g.ldg, a);
+              keep_row(g.U + (size_t)(m0 + lane) * g.ldg, t.n0 + j, g.ldg, u);
+            }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) a[i] = a[i] * gate_share<false>(g.act, a[i], nullptr) * u[i];
-          if (in) put16(static_cast<T*>(g.out[0]) + row, t.n0 + j, g.N, g.vec, a);
+            for (int i = 0; i < 32; ++i) a[i] = a[i] * gate_share<false>(g.act, a[i], nullptr) * u[i];
+          }
+          put_block(patch, out, g.vec, m0, g.M, t.n0 + j, g.N, a);
         }
-      } else {
-        T* row = static_cast<T*>(g.out[t.result]) + (size_t)m * g.N;
-#pragma unroll 1
-        for (int j = half * 128; j < half * 128 + 128 && t.n0 + j < g.N; j += 16) {
-          float a[16];
-          tmem_ld16(taddr + j, a);
-          if (in) put16(row, t.n0 + j, g.N, g.vec, a);
-        }
-      }
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
@@ -283,8 +308,165 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
   }
 }
 
+// ---- few rows -------------------------------------------------------------------------------------------------------------------
+// G^T = Wg^T X^T and U^T: the weights are the 128 rows of the products and X's rows their NT columns, so that nothing of a product is wasted on rows that
+// are not there, and every weight is read once.  Bound by HBM (the weights); a cluster shares the sum over the inputs, so that 128
+// columns of the weights are not one CTA's alone, and each of its CTAs adds the parts of its share of the columns, in their order.
+template <int NT>
+struct Few {
+  static constexpr int weights = 128 * kStep * 2, stage = 2 * weights + NT * kStep * 2;   // bytes: of a tile of a weight, of a step
+  static constexpr int stages = NT <= 32 ? 3 : NT == 64 ? 5 : 4;                          // 102 to 107 KB, two CTAs on an SM, or 200 and 192
+  static constexpr int tmem = 2 * NT < 32 ? 32 : 2 * NT;
+  static constexpr int parts = 2 * NT * 128 * 4;                                          // sums, in place of the ring
+  static constexpr size_t smem = (size_t)stages * stage + 1024 + 128;
+  static_assert(parts <= stages * stage, "");
+};
+struct FewArgs {
+  int M, N, steps, act;   // steps: of K, all CTAs of a cluster together
+  void* H;
+  float *G, *U;
+  int ldg;
+};
+constexpr int kFewThreads = 192;
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar),
+      "r"(x), "r"(y)
+      : "memory");
+}
+template <int NT, typename T>
+__global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_constant__ FewArgs g, const __grid_constant__ CUtensorMap mapX,
+                                                                const __grid_constant__ CUtensorMap mapG, const __grid_constant__ CUtensorMap mapU) {
+  using F = Few<NT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + F::stages * F::stage);
+  uint64_t *empty = full + F::stages, *ready = empty + F::stages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ready + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t csize;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
+  const int rank = (int)cluster_rank(), f0 = (int)(blockIdx.x / csize) * 128;
+  if (tid == 0) {
+    for (int i = 0; i < F::stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(ready, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&mapX);
+    tma_prefetch_desc(&mapG);
+    tma_prefetch_desc(&mapU);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, F::tmem);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot, ring = smem_u32(sm), abortb = smem_u32(const_cast<int*>(abort_flag));
+  grid_dependency_wait();
+  // this CTA's steps of K
+  const int per = (g.steps + (int)csize - 1) / (int)csize, k0 = min(g.steps, rank * per), n = min(g.steps, k0 + per) - k0;
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < n; ++i) {
+        const int slot = i % F::stages, k = (k0 + i) * kStep;
+        if (i >= F::stages && !wait_or_abort(smem_u32(&empty[slot]), (i / F::stages - 1) & 1, abortb)) break;
+        mbar_expect_tx(&full[slot], F::stage);
+        const uint32_t bar = smem_u32(&full[slot]), a = ring + slot * F::stage;
+        tma_load_2d(a, &mapG, bar, f0, k);
+        tma_load_2d(a + kBox, &mapG, bar, f0 + 64, k);
+        tma_load_2d(a + F::weights, &mapU, bar, f0, k);
+        tma_load_2d(a + F::weights + kBox, &mapU, bar, f0 + 64, k);
+        tma_load_2d(a + 2 * F::weights, &mapX, bar, k, 0);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = instruction<T>(128, NT, 1, 0);
+      const uint64_t da = make_smem_desc(0, kBox, 1024, kSwizzle128B), db = make_smem_desc(0, 16, 1024, kSwizzle128B);
+      bool ok = true;
+      for (int i = 0; i < n && ok; ++i) {
+        const int slot = i % F::stages;
+        if (!(ok = wait_or_abort(smem_u32(&full[slot]), (i / F::stages) & 1, abortb))) break;
+        tc_fence_after_sync();
+        const uint32_t a = ring + slot * F::stage;
+        // (a shared address of a CTA other than the cluster's first has bits above those of the descriptor's field)
+        const auto at = [](uint32_t p) { return (uint64_t)((p >> 4) & 0x3fff); };
+        const uint64_t ag = da + at(a), au = da + at(a + F::weights), b = db + at(a + 2 * F::weights);
+#pragma unroll
+        for (int j = 0; j < kStep / 16; ++j) mma_f16_ss(tmem_base, ag + j * (2048 >> 4), b + j * (32 >> 4), idesc, i > 0 || j > 0);
+#pragma unroll
+        for (int j = 0; j < kStep / 16; ++j) mma_f16_ss(tmem_base + NT, au + j * (2048 >> 4), b + j * (32 >> 4), idesc, i > 0 || j > 0);
+        mma_commit(&empty[slot]);
+      }
+      if (ok) mma_commit(ready);
+    }
+  } else {
+    // sums -> shared memory, [G, U][row of X][column of the weights]: the ring is free once the last product is done
+    const bool ok = __all_sync(0xffffffffu, wait_or_abort(smem_u32(ready), 0, abortb));
+    tc_fence_after_sync();
+    if (ok) {
+      const int qd = warp & 3;
+      float* part = reinterpret_cast<float*>(sm) + qd * 32 + lane;
+      const uint32_t taddr = tmem_base + ((uint32_t)(qd * 32) << 16);
+#pragma unroll 1
+      for (int j = 0; j < 2 * NT; j += 16) {
+        float v[16];
+        if (n > 0) tmem_ld16(taddr + j, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[(j + i) * 128] = n > 0 ? v[i] : 0.f;
+      }
+    }
+    tc_fence_before_sync();
+  }
+  __syncthreads();
+  cluster_sync();
+  // the cluster's parts of a share of the columns
+  const int share = 128 / (int)csize, c0 = rank * share, rows = min(NT, g.M);
+  for (int i = tid; i < share * rows; i += kFewThreads) {
+    const int m = i / share, c = c0 + (i - m * share), f = f0 + c;
+    if (f >= g.N) continue;
+    float v[2][8];
+    const uint32_t at = ring + (m * 128 + c) * 4;
+#pragma unroll
+    for (uint32_t p = 0; p < 8; ++p)
+      if (p < csize) {
+        uint32_t from;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(p));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[0][p]) : "r"(from) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[1][p]) : "r"(from + NT * 128 * 4) : "memory");
+      }
+    float a = 0.f, u = 0.f;
+#pragma unroll
+    for (uint32_t p = 0; p < 8; ++p)
+      if (p < csize) {
+        a += v[0][p];
+        u += v[1][p];
+      }
+    if (g.G) {
+      g.G[(size_t)m * g.ldg + f] = a;
+      g.U[(size_t)m * g.ldg + f] = u;
+    }
+    static_cast<T*>(g.H)[(size_t)m * g.N + f] = (T)(a * gate_share<false>(g.act, a, nullptr) * u);
+  }
+  __syncthreads();
+  if (tid == 0 && *abort_flag) {
+    atomicCAS(&g_gated_status, 0, (2 << 16) | (blockIdx.x & 0xffff));
+    const long long t0 = clock64();   // copies in flight land before the shared memory is given back
+    while (clock64() - t0 < 40000000ll) {
+    }
+  }
+  cluster_sync();   // nobody reads this CTA's parts any more
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, F::tmem);
+  }
+}
+
 // ---- elementwise -----------------------------------------------------------------------------------------------------------------
-// dG = dH U act'(G), dU = dH act(G): rows of N values to rows of ld, eight per thread.  Bound by HBM: 14 bytes a value.
+// dG = dH U act'(G), dU = dH act(G): dH has rows of N values, the others of ld, eight per thread (the padding is written, and read by nothing).  Bound by HBM: 14 bytes a value.
 template <typename T>
 __global__ void __launch_bounds__(256) slopes_kernel(int M, int N, int ld, int act, int vec, const float* G, const float* U, const T* dH, T* dG, T* dU) {
   const int groups = (N + 7) / 8;
@@ -294,23 +476,19 @@ __global__ void __launch_bounds__(256) slopes_kernel(int M, int N, int ld, int a
   const int n = (int)(i - m * groups) * 8, left = min(8, N - n);
   const size_t src = m * N + n, dst = m * ld + n;
   float a[8], u[8], d[8];
-  if (vec) {
 #pragma unroll
-    for (int j = 0; j < 8; j += 4) {
-      *reinterpret_cast<float4*>(a + j) = *reinterpret_cast<const float4*>(G + src + j);
-      *reinterpret_cast<float4*>(u + j) = *reinterpret_cast<const float4*>(U + src + j);
-    }
+  for (int j = 0; j < 8; j += 4) {
+    *reinterpret_cast<float4*>(a + j) = *reinterpret_cast<const float4*>(G + dst + j);
+    *reinterpret_cast<float4*>(u + j) = *reinterpret_cast<const float4*>(U + dst + j);
+  }
+  if (vec) {
     alignas(16) T h[8];
     *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(dH + src);
 #pragma unroll
     for (int j = 0; j < 8; ++j) d[j] = (float)h[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      a[j] = j < left ? G[src + j] : 0.f;
-      u[j] = j < left ? U[src + j] : 0.f;
-      d[j] = j < left ? (float)dH[src + j] : 0.f;
-    }
+    for (int j = 0; j < 8; ++j) d[j] = j < left ? (float)dH[src + j] : 0.f;
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -409,8 +587,9 @@ int launch(Gemm g, int results, const Matrix& a0, const Matrix& a1, const Matrix
   const long units = (long)g.tiles_m * g.tiles_n * results;
   if (units > 0x3fffffff) return fail(B200CP_ERR_UNSUPPORTED, "gated feed-forward block: %d x %d is too large", g.M, g.N);
   g.units = (int)units;
-  g.vec = rows16(g.out[0], (size_t)g.N * 2) && rows16(g.out[results - 1], (size_t)g.N * 2);
-  g.vecg = rows16(g.G, (size_t)g.N * 4) && rows16(g.U, (size_t)g.N * 4);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(g.out[0]) | reinterpret_cast<uintptr_t>(g.out[results - 1]) | (uintptr_t)g.N * 2;
+  g.vec = at % 16 == 0 ? 8 : at % 4 == 0 ? 2 : 1;
+  g.ldg = ld8(g.N);
   const auto kern = gated_kernel<FORM, T>;
   static std::atomic<int> set[64];
   B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, (int)kSmem));
@@ -420,10 +599,53 @@ int launch(Gemm g, int results, const Matrix& a0, const Matrix& a1, const Matrix
   return B200CP_OK;
 }
 
+// Batches of up to this many rows.
+constexpr int kFewRows = 128;
+template <int NT, typename T>
+int launch_few(FewArgs g, const Matrix& x, const Matrix& wg, const Matrix& wu, cudaStream_t st) {
+  using F = Few<NT>;
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  CUtensorMap mx, mg, mu;
+  if (int rc = encode<T>(&mx, x, NT)) return rc;
+  if (int rc = encode<T>(&mg, wg, kStep)) return rc;
+  if (int rc = encode<T>(&mu, wu, kStep)) return rc;
+  const auto kern = gated_few_kernel<NT, T>;
+  static std::atomic<int> set[64];
+  B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, (int)F::smem));
+  // as many CTAs for a tile of columns as the machine holds at once, with two steps each
+  const int tiles = ceil_div(g.N, 128), slots = di.sm_count * (NT <= 32 ? 2 : 1);
+  int c = 1;
+  while (c < 8 && tiles * c * 2 <= slots && g.steps >= 4 * c) c *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)tiles * c);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = F::smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = c;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  B200CP_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, g, mx, mg, mu));
+  B200CP_LAUNCH_OK("gated_few_kernel");
+  return B200CP_OK;
+}
+
 template <typename T>
 int forward(int rows, int I, int F, int act, const void* X, const void* Wg, const void* Wu, void* H, float* G, float* U, char* ws, cudaStream_t st) {
   Matrix x{X, rows, I, 0}, g{Wg, I, F, 0}, u{Wu, I, F, 0}, *ms[3] = {&x, &g, &u};
   if (int rc = pad(ms, 3, ws, st)) return rc;
+  if (rows <= kFewRows) {
+    const FewArgs f{rows, F, ceil_div(I, kStep), act, H, G, U, ld8(F)};
+    if (rows <= 16) return launch_few<16, T>(f, x, g, u, st);
+    if (rows <= 32) return launch_few<32, T>(f, x, g, u, st);
+    if (rows <= 64) return launch_few<64, T>(f, x, g, u, st);
+    return launch_few<128, T>(f, x, g, u, st);
+  }
   Gemm p{};
   p.M = rows; p.N = F; p.steps = p.first = ceil_div(I, kStep); p.act = act;
   p.out[0] = p.out[1] = H; p.G = G; p.U = U;
@@ -446,7 +668,7 @@ int backward(int rows, int I, int F, int act, const void* X, const void* Wg, con
   if (int rc = pad(ms, count, ws, st)) return rc;
   const size_t n = ((size_t)rows * (ld / 8) + 255) / 256;
   if (n > 0x7fffffffull) return fail(B200CP_ERR_UNSUPPORTED, "gated feed-forward block: %d x %d is too large", rows, F);
-  const int vec = rows16(G, (size_t)F * 4) && rows16(U, (size_t)F * 4) && rows16(dH, (size_t)F * 2);
+  const int vec = rows16(dH, (size_t)F * 2);
   slopes_kernel<T><<<(unsigned)n, 256, 0, st>>>(rows, F, ld, act, vec, G, U, static_cast<const T*>(dH), dG, dU);
   B200CP_LAUNCH_OK("slopes_kernel");
   const Matrix a{dG, rows, F, ld}, b{dU, rows, F, ld};
@@ -499,8 +721,8 @@ int b200cp_dense_gated(int rows, int I, int F, int type, int activation, const v
   if (int rc = check_gated(who, rows, I, F, type, activation)) return rc;
   if (rows == 0) return B200CP_OK;
   if (!X || !Wg || !Wu || !H || !G != !U) return fail(B200CP_ERR_INVALID_ARG, "%s: null pointer", who);
-  for (const void* p : {X, Wg, Wu})
-    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(B200CP_ERR_INVALID_ARG, "%s: X, Wg and Wu have to start on 16-byte boundaries", who);
+  for (const void* p : {X, Wg, Wu, (const void*)G, (const void*)U})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(B200CP_ERR_INVALID_ARG, "%s: X, Wg, Wu, G and U have to start on 16-byte boundaries", who);
   const size_t need = b200cp_dense_gated_workspace_bytes(rows, I, F, type);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return fail(B200CP_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, %zu given", who, need, workspace_bytes);
@@ -528,8 +750,8 @@ int b200cp_dense_gated_bwd(int rows, int I, int F, int type, int activation, con
     return B200CP_OK;
   }
   if (!G || !U || !dH || (dWg && !X) || (dX && (!Wg || !Wu))) return fail(B200CP_ERR_INVALID_ARG, "%s: null pointer", who);
-  for (const void* p : {X, Wg, Wu})
-    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(B200CP_ERR_INVALID_ARG, "%s: X, Wg and Wu have to start on 16-byte boundaries", who);
+  for (const void* p : {X, Wg, Wu, (const void*)G, (const void*)U})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(B200CP_ERR_INVALID_ARG, "%s: X, Wg, Wu, G and U have to start on 16-byte boundaries", who);
   const size_t need = b200cp_dense_gated_bwd_workspace_bytes(rows, I, F, type);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(B200CP_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, %zu given", who, need, workspace_bytes);

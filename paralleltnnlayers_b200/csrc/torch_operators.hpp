@@ -192,6 +192,7 @@ struct Gated {   // operands, checked, contiguous and on 16-byte boundaries
     Wg = whole(Wg_);
     Wu = whole(Wu_);
   }
+  int64_t kept() const { return ((int64_t)F + 7) / 8 * 8; }   // floats of a row of G and U
   static Tensor whole(const Tensor& t) {
     const Tensor c = contiguous(t);
     return (reinterpret_cast<uintptr_t>(c.const_data_ptr()) & 15) == 0 ? c : c.clone();
@@ -206,8 +207,8 @@ Tensor dense_gated(const Gated& g, Tensor* G, Tensor* U) {
   const c10::cuda::OptionalCUDAGuard guard(g.x.device());
   Tensor H = empty_as(g.size(g.F), g.x);
   if (G) {
-    *G = empty({g.rows, g.F}, g.x);
-    *U = empty({g.rows, g.F}, g.x);
+    *G = empty({g.rows, g.kept()}, g.x);
+    *U = empty({g.rows, g.kept()}, g.x);
   }
   const Scratch ws(b200cp_dense_gated_workspace_bytes(g.rows, g.I, g.F, g.type), g.x);
   ok(b200cp_dense_gated(g.rows, g.I, g.F, g.type, g.act, g.x.const_data_ptr(), g.Wg.const_data_ptr(), g.Wu.const_data_ptr(), H.data_ptr(),
@@ -217,10 +218,25 @@ Tensor dense_gated(const Gated& g, Tensor* G, Tensor* U) {
 std::array<Tensor, 3> dense_gated_backward(const Gated& g, const Tensor& G_, const Tensor& U_, const Tensor& dH_, bool need_x, bool need_w) {
   Adapters::same(dH_, g.x, "dH");
   TORCH_CHECK_VALUE(dH_.sizes() == at::IntArrayRef(g.size(g.F)), "dH is ", dH_.sizes(), ", ", at::IntArrayRef(g.size(g.F)), " is needed");
-  const Tensor G = dev(G_, "G", g.x), U = dev(U_, "U", g.x), dH = contiguous(dH_);
-  check_size(G, "G", {g.rows, g.F});
-  check_size(U, "U", {g.rows, g.F});
+  // G and U as the forward left them (padded rows, or the columns of those), or any others of the right size
+  const auto check = [&](const Tensor& t, const char* name) {
+    TORCH_CHECK_TYPE(t.is_cuda() && t.scalar_type() == at::kFloat, name, " must be a float32 CUDA tensor");
+    TORCH_CHECK_VALUE(t.device() == g.x.device(), name, " is on ", t.device(), ", X on ", g.x.device());
+    TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == g.rows && (t.size(1) == g.F || t.size(1) == g.kept()), name, " is ", t.sizes(), " where [", g.rows,
+                      ", ", g.F, "] is needed");
+  };
+  check(G_, "G");
+  check(U_, "U");
+  const auto kept = [&](const Tensor& t) {
+    const bool as_left = t.stride(1) == 1 && (t.stride(0) == g.kept() || g.rows <= 1) &&
+                         (int64_t)(t.storage().nbytes() / sizeof(float)) - t.storage_offset() >= g.rows * g.kept();
+    if (as_left && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0) return t;
+    Tensor c = empty({g.rows, g.kept()}, g.x);
+    c.narrow(1, 0, t.size(1)).copy_(t);
+    return c;
+  };
   const c10::cuda::OptionalCUDAGuard guard(g.x.device());
+  const Tensor G = kept(G_), U = kept(U_), dH = contiguous(dH_);
   std::array<Tensor, 3> d;
   if (need_x) d[0] = empty_as(g.x.sizes(), g.x);
   if (need_w) {
@@ -338,7 +354,11 @@ PYFN(py_dense_gated_save) {
   const Tensor &x = any_tensor(a[0], "X"), &g = any_tensor(a[1], "Wg"), &u = any_tensor(a[2], "Wu");
   const int64_t act = int_arg(a[3]);
   std::array<Tensor, 3> r;
-  unlocked([&] { r[0] = dense_gated(Gated(x, g, u, act), &r[1], &r[2]); });
+  unlocked([&] {
+    const Gated op(x, g, u, act);
+    r[0] = dense_gated(op, &r[1], &r[2]);
+    for (int i = 1; i < 3; ++i) r[i] = r[i].narrow(1, 0, op.F);
+  });
   return wrap_tuple(r);
   END_HANDLE_TH_ERRORS
 }
