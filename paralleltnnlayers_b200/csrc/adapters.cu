@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "cluster_util.cuh"
 #include "common.cuh"
 
 namespace b200cp {
@@ -867,10 +868,6 @@ __global__ void __launch_bounds__(kThreads) join_grads_kernel(const __grid_const
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
-int sms() {
-  DeviceInfo di;
-  return device_info(&di) ? 148 : di.sm_count;
-}
 bool rows16(const void* p, size_t row_bytes) { return !(reinterpret_cast<uintptr_t>(p) & 15) && row_bytes % 16 == 0; }
 
 template <typename T, int TM, int RP, bool BACK>
@@ -880,29 +877,15 @@ int launch_tiles(const Args& g, int tiles, cudaStream_t st) {
   static std::atomic<int> set[64];
   B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, S::smem));
   // CTAs of a tile: as many as the machine holds at once, with a chunk of the longer product for each
-  static std::atomic<int> resident{0};
-  int per = resident.load(std::memory_order_relaxed);
-  if (!per) {
-    B200CP_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, kThreads, S::smem));
-    resident.store(per = std::max(per, 1), std::memory_order_relaxed);
-  }
+  static std::atomic<int> cache[9];
   int c = 1;
   const int chunks = std::max(ceil_div(g.K, S::KC), ceil_div(g.N, S::KC));
-  while (c < 8 && (long)tiles * c * 2 <= (long)sms() * per && 2 * c <= chunks) c *= 2;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)tiles * c);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = S::smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = c;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  B200CP_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, g));
+  for (int q = 2; q <= 8 && q <= chunks; q *= 2) {
+    int n = 0;
+    B200CP_CUDA_OK(resident_clusters(kern, kThreads, S::smem, q, cache, &n));
+    if (tiles <= n) c = q;
+  }
+  B200CP_CUDA_OK(launch_clusters(kern, tiles, c, kThreads, S::smem, st, g));
   B200CP_LAUNCH_OK("adapters_kernel");
   return B200CP_OK;
 }

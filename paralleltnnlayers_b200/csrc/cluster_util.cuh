@@ -110,4 +110,47 @@ inline int pick_cluster(long tiles, int units, int least, int sm_count) {
   return s;
 }
 
+// ---- launch of clusters along x ------------------------------------------------------------------------------------------
+// How many clusters of c CTAs of a kernel the device holds at once, asked once per kernel and size (`cache`: nine zeros): those of seven, say,
+// are fewer than a seventh of the CTAs, since a cluster lies within one group of SMs.
+template <typename Kern>
+cudaError_t resident_clusters(Kern kern, int threads, size_t smem, int c, std::atomic<int>* cache, int* out) {
+  int n = cache[c].load(std::memory_order_relaxed);
+  cudaError_t e = cudaSuccess;
+  if (!n) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)c);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)c;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+    if (e == cudaSuccess) cache[c].store(n > 0 ? n : (n = 1), std::memory_order_relaxed);
+  }
+  *out = n;
+  return e;
+}
+// A programmatic dependent launch of `clusters` clusters of c CTAs.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_clusters(void (*kern)(KArgs...), int clusters, int c, int threads, size_t smem, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)clusters * (unsigned)c);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)c;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
 }  // namespace b200cp

@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "cluster_util.cuh"
 #include "common.cuh"
 #include "tc_common.cuh"
 #include "tc_pair.cuh"
@@ -94,20 +95,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <typename T>
 __device__ __forceinline__ void put_block(uint8_t* patch, T* out, int vec, int m0, int M, int n, int N, const float (&v)[32]) {
   const int lane = threadIdx.x & 31;
-  uint4* mine = reinterpret_cast<uint4*>(patch + lane * kPitch);
+  // (rows on 16-byte boundaries straight from the registers: 64 bytes of each, 3 % of a large product less)
+  uint4* mine = vec == 8 ? reinterpret_cast<uint4*>(out + (size_t)(m0 + lane) * N + n) : reinterpret_cast<uint4*>(patch + lane * kPitch);
+  const int pieces = vec == 8 ? (m0 + lane < M ? min(4, (N - n) / 8) : 0) : 4;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    mine[j] = make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]), pack2<T>(v[8 * j + 4], v[8 * j + 5]),
+    if (j < pieces) mine[j] = make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]), pack2<T>(v[8 * j + 4], v[8 * j + 5]),
                          pack2<T>(v[8 * j + 6], v[8 * j + 7]));
+  if (vec == 8) return;
   __syncwarp();
   const int rows = min(32, M - m0), cols = min(32, N - n);
-  if (vec == 8) {
-    const int q = lane & 3;
-    if (q * 8 < cols)
-#pragma unroll
-      for (int r = lane >> 2; r < 32; r += 8)
-        if (r < rows) *reinterpret_cast<uint4*>(out + (size_t)(m0 + r) * N + n + q * 8) = *reinterpret_cast<const uint4*>(patch + r * kPitch + q * 16);
-  } else if (vec == 2) {
+  if (vec == 2) {
     const int q = lane & 15;
     if (q * 2 < cols)
 #pragma unroll 4
@@ -310,20 +308,23 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------------
 // G^T = Wg^T X^T and U^T: the weights are the 128 rows of the products and X's rows their NT columns, so that nothing of a product is wasted on rows that
-// are not there, and every weight is read once.  Bound by HBM (the weights); a cluster shares the sum over the inputs, so that 128
-// columns of the weights are not one CTA's alone, and each of its CTAs adds the parts of its share of the columns, in their order.
-template <int NT>
+// are not there, and every weight is read once.  Bound by HBM (the weights).  An SM holds one CTA that uses tensor memory and reads some
+// 54 bytes per nanosecond, so what counts is how many SMs have one: a CTA has W x 128 columns, a cluster of up to eight shares the sum over
+// the inputs (each adds the parts of its share of the columns, in their order), and W and the cluster are those that give the most CTAs
+// (48 rows 4096 -> 10240: 80 CTAs of 128 columns 39 us, 40 clusters of three with 256 columns 34; 64 rows 8192 -> 8192 47, 5.7 TB/s).
+template <int NT, int W>
 struct Few {
-  static constexpr int weights = 128 * kStep * 2, stage = 2 * weights + NT * kStep * 2;   // bytes: of a tile of a weight, of a step
-  static constexpr int stages = NT <= 32 ? 3 : NT == 64 ? 5 : 4;                          // 102 to 107 KB, two CTAs on an SM, or 200 and 192
-  static constexpr int tmem = 2 * NT < 32 ? 32 : 2 * NT;
-  static constexpr int parts = 2 * NT * 128 * 4;                                          // sums, in place of the ring
+  static constexpr int weights = 128 * kStep * 2, stage = 2 * W * weights + NT * kStep * 2;   // bytes: of a tile of a weight, of a step
+  static constexpr int stages = W == 2 ? 3 : NT <= 32 ? 6 : NT == 64 ? 5 : 4;                 // 192 to 216 KB
+  static constexpr int tmem = 2 * W * NT < 32 ? 32 : 2 * W * NT, cols = 128 * W;
+  static constexpr int parts = 2 * NT * cols * 4;                                             // sums, in place of the ring
   static constexpr size_t smem = (size_t)stages * stage + 1024 + 128;
-  static_assert(parts <= stages * stage, "");
+  static_assert(parts <= stages * stage && smem <= 227 * 1024 && (tmem & (tmem - 1)) == 0, "");
 };
 struct FewArgs {
   int M, N, steps, act;   // steps: of K, all CTAs of a cluster together
   void* H;
+  int vec;                // four columns of H start on 8-byte boundaries
   float *G, *U;
   int ldg;
 };
@@ -334,10 +335,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       "r"(x), "r"(y)
       : "memory");
 }
-template <int NT, typename T>
+template <int NT, int W, typename T>
 __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_constant__ FewArgs g, const __grid_constant__ CUtensorMap mapX,
                                                                 const __grid_constant__ CUtensorMap mapG, const __grid_constant__ CUtensorMap mapU) {
-  using F = Few<NT>;
+  using F = Few<NT, W>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + F::stages * F::stage);
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t csize;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
-  const int rank = (int)cluster_rank(), f0 = (int)(blockIdx.x / csize) * 128;
+  const int rank = (int)cluster_rank(), f0 = (int)(blockIdx.x / csize) * F::cols;
   if (tid == 0) {
     for (int i = 0; i < F::stages; ++i) {
       mbar_init(&full[i], 1);
@@ -375,11 +376,12 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
         if (i >= F::stages && !wait_or_abort(smem_u32(&empty[slot]), (i / F::stages - 1) & 1, abortb)) break;
         mbar_expect_tx(&full[slot], F::stage);
         const uint32_t bar = smem_u32(&full[slot]), a = ring + slot * F::stage;
-        tma_load_2d(a, &mapG, bar, f0, k);
-        tma_load_2d(a + kBox, &mapG, bar, f0 + 64, k);
-        tma_load_2d(a + F::weights, &mapU, bar, f0, k);
-        tma_load_2d(a + F::weights + kBox, &mapU, bar, f0 + 64, k);
-        tma_load_2d(a + 2 * F::weights, &mapX, bar, k, 0);
+#pragma unroll
+        for (int w = 0; w < 2 * W; ++w) {
+          tma_load_2d(a + w * kBox, &mapG, bar, f0 + w * 64, k);
+          tma_load_2d(a + W * F::weights + w * kBox, &mapU, bar, f0 + w * 64, k);
+        }
+        tma_load_2d(a + 2 * W * F::weights, &mapX, bar, k, 0);
       }
     }
   } else if (warp == 1) {
@@ -394,11 +396,13 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
         const uint32_t a = ring + slot * F::stage;
         // (a shared address of a CTA other than the cluster's first has bits above those of the descriptor's field)
         const auto at = [](uint32_t p) { return (uint64_t)((p >> 4) & 0x3fff); };
-        const uint64_t ag = da + at(a), au = da + at(a + F::weights), b = db + at(a + 2 * F::weights);
+        const uint64_t b = db + at(a + 2 * W * F::weights);
 #pragma unroll
-        for (int j = 0; j < kStep / 16; ++j) mma_f16_ss(tmem_base, ag + j * (2048 >> 4), b + j * (32 >> 4), idesc, i > 0 || j > 0);
+        for (int w = 0; w < 2 * W; ++w) {   // tiles of Wg, then of Wu
+          const uint64_t p = da + at(a + w * F::weights);
 #pragma unroll
-        for (int j = 0; j < kStep / 16; ++j) mma_f16_ss(tmem_base + NT, au + j * (2048 >> 4), b + j * (32 >> 4), idesc, i > 0 || j > 0);
+          for (int j = 0; j < kStep / 16; ++j) mma_f16_ss(tmem_base + w * NT, p + j * (2048 >> 4), b + j * (32 >> 4), idesc, i > 0 || j > 0);
+        }
         mma_commit(&empty[slot]);
       }
       if (ok) mma_commit(ready);
@@ -412,44 +416,60 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
       float* part = reinterpret_cast<float*>(sm) + qd * 32 + lane;
       const uint32_t taddr = tmem_base + ((uint32_t)(qd * 32) << 16);
 #pragma unroll 1
-      for (int j = 0; j < 2 * NT; j += 16) {
+      for (int j = 0; j < 2 * W * NT; j += 16) {
+        const int w = j / NT, m = j % NT;   // the tile, and the row of X
+        float* to = part + ((w / W) * NT + m) * F::cols + (w % W) * 128;
         float v[16];
         if (n > 0) tmem_ld16(taddr + j, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part[(j + i) * 128] = n > 0 ? v[i] : 0.f;
+        for (int i = 0; i < 16; ++i) to[i * F::cols] = n > 0 ? v[i] : 0.f;
       }
     }
     tc_fence_before_sync();
   }
   __syncthreads();
   cluster_sync();
-  // the cluster's parts of a share of the columns
-  const int share = 128 / (int)csize, c0 = rank * share, rows = min(NT, g.M);
-  for (int i = tid; i < share * rows; i += kFewThreads) {
-    const int m = i / share, c = c0 + (i - m * share), f = f0 + c;
-    if (f >= g.N) continue;
-    float v[2][8];
-    const uint32_t at = ring + (m * 128 + c) * 4;
+  // The cluster's parts of a share of the columns, four at a time (a read of another CTA's memory takes half a microsecond).
+  const int quads = (32 * W + (int)csize - 1) / (int)csize, q0 = rank * quads, rows = min(NT, g.M);
+#pragma unroll 2
+  for (int i = tid; i < quads * rows; i += kFewThreads) {
+    const int m = i / quads, q = q0 + (i - m * quads), f = f0 + 4 * q;
+    if (q >= 32 * W || f >= g.N) continue;
+    float4 v[2][8];
+    const uint32_t at = ring + (m * F::cols + 4 * q) * 4;
 #pragma unroll
     for (uint32_t p = 0; p < 8; ++p)
       if (p < csize) {
         uint32_t from;
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(p));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[0][p]) : "r"(from) : "memory");
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[1][p]) : "r"(from + NT * 128 * 4) : "memory");
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[k][p].x), "=f"(v[k][p].y), "=f"(v[k][p].z), "=f"(v[k][p].w)
+                       : "r"(from + k * NT * F::cols * 4)
+                       : "memory");
       }
-    float a = 0.f, u = 0.f;
+    float a[4] = {}, u[4] = {};
 #pragma unroll
     for (uint32_t p = 0; p < 8; ++p)
       if (p < csize) {
-        a += v[0][p];
-        u += v[1][p];
+        a[0] += v[0][p].x; a[1] += v[0][p].y; a[2] += v[0][p].z; a[3] += v[0][p].w;
+        u[0] += v[1][p].x; u[1] += v[1][p].y; u[2] += v[1][p].z; u[3] += v[1][p].w;
       }
-    if (g.G) {
-      g.G[(size_t)m * g.ldg + f] = a;
-      g.U[(size_t)m * g.ldg + f] = u;
+    if (g.G) {   // (columns past the end are those of the row's padding)
+      *reinterpret_cast<float4*>(g.G + (size_t)m * g.ldg + f) = make_float4(a[0], a[1], a[2], a[3]);
+      *reinterpret_cast<float4*>(g.U + (size_t)m * g.ldg + f) = make_float4(u[0], u[1], u[2], u[3]);
     }
-    static_cast<T*>(g.H)[(size_t)m * g.N + f] = (T)(a * gate_share<false>(g.act, a, nullptr) * u);
+    T* h = static_cast<T*>(g.H) + (size_t)m * g.N + f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a[k] = a[k] * gate_share<false>(g.act, a[k], nullptr) * u[k];
+    if (g.vec) {
+      *reinterpret_cast<uint2*>(h) = make_uint2(pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (f + k < g.N) h[k] = (T)a[k];
+    }
   }
   __syncthreads();
   if (tid == 0 && *abort_flag) {
@@ -599,40 +619,49 @@ int launch(Gemm g, int results, const Matrix& a0, const Matrix& a1, const Matrix
   return B200CP_OK;
 }
 
-// Batches of up to this many rows.
-constexpr int kFewRows = 128;
+constexpr int kFewRows = 128;   // batches of up to this many rows
+// CTAs that a shape of the kernel gives: the largest cluster (and two steps for each of its CTAs) of which the device holds all tiles at once
+template <int NT, int W, typename T>
+int few_ctas(const FewArgs& g, int* cluster, int* ctas) {
+  using F = Few<NT, W>;
+  const auto kern = gated_few_kernel<NT, W, T>;
+  static std::atomic<int> set[64], cache[9];
+  B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, (int)F::smem));
+  const int tiles = ceil_div(g.N, F::cols);
+  *cluster = 1;
+  for (int q = 2; q <= 8 && g.steps >= 2 * q; ++q) {
+    int n = 0;
+    B200CP_CUDA_OK(resident_clusters(kern, kFewThreads, F::smem, q, cache, &n));
+    if (tiles <= n) *cluster = q;
+  }
+  *ctas = tiles * *cluster;
+  return B200CP_OK;
+}
+template <int NT, int W, typename T>
+int launch_few(const FewArgs& g, int cluster, const CUtensorMap& x, const CUtensorMap& wg, const CUtensorMap& wu, cudaStream_t st) {
+  using F = Few<NT, W>;
+  B200CP_CUDA_OK(launch_clusters(gated_few_kernel<NT, W, T>, ceil_div(g.N, F::cols), cluster, kFewThreads, F::smem, st, g, x, wg, wu));
+  B200CP_LAUNCH_OK("gated_few_kernel");
+  return B200CP_OK;
+}
 template <int NT, typename T>
-int launch_few(FewArgs g, const Matrix& x, const Matrix& wg, const Matrix& wu, cudaStream_t st) {
-  using F = Few<NT>;
+int run_few(const FewArgs& g, const Matrix& x, const Matrix& wg, const Matrix& wu, cudaStream_t st) {
   DeviceInfo di;
   if (int rc = device_info(&di)) return rc;
   CUtensorMap mx, mg, mu;
   if (int rc = encode<T>(&mx, x, NT)) return rc;
   if (int rc = encode<T>(&mg, wg, kStep)) return rc;
   if (int rc = encode<T>(&mu, wu, kStep)) return rc;
-  const auto kern = gated_few_kernel<NT, T>;
-  static std::atomic<int> set[64];
-  B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, (int)F::smem));
-  // as many CTAs for a tile of columns as the machine holds at once, with two steps each
-  const int tiles = ceil_div(g.N, 128), slots = di.sm_count * (NT <= 32 ? 2 : 1);
-  int c = 1;
-  while (c < 8 && tiles * c * 2 <= slots && g.steps >= 4 * c) c *= 2;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)tiles * c);
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = F::smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = c;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  B200CP_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, g, mx, mg, mu));
-  B200CP_LAUNCH_OK("gated_few_kernel");
-  return B200CP_OK;
+  int c1 = 1, n1 = 0;
+  if (int rc = few_ctas<NT, 1, T>(g, &c1, &n1)) return rc;
+  if constexpr (NT <= 64) {
+    int c2 = 1, n2 = 0;
+    if (n1 < di.sm_count) {
+      if (int rc = few_ctas<NT, 2, T>(g, &c2, &n2)) return rc;
+      if (n2 > n1) return launch_few<NT, 2, T>(g, c2, mx, mg, mu, st);
+    }
+  }
+  return launch_few<NT, 1, T>(g, c1, mx, mg, mu, st);
 }
 
 template <typename T>
@@ -640,11 +669,11 @@ int forward(int rows, int I, int F, int act, const void* X, const void* Wg, cons
   Matrix x{X, rows, I, 0}, g{Wg, I, F, 0}, u{Wu, I, F, 0}, *ms[3] = {&x, &g, &u};
   if (int rc = pad(ms, 3, ws, st)) return rc;
   if (rows <= kFewRows) {
-    const FewArgs f{rows, F, ceil_div(I, kStep), act, H, G, U, ld8(F)};
-    if (rows <= 16) return launch_few<16, T>(f, x, g, u, st);
-    if (rows <= 32) return launch_few<32, T>(f, x, g, u, st);
-    if (rows <= 64) return launch_few<64, T>(f, x, g, u, st);
-    return launch_few<128, T>(f, x, g, u, st);
+    const FewArgs f{rows, F, ceil_div(I, kStep), act, H, F % 4 == 0 && reinterpret_cast<uintptr_t>(H) % 8 == 0, G, U, ld8(F)};
+    if (rows <= 16) return run_few<16, T>(f, x, g, u, st);
+    if (rows <= 32) return run_few<32, T>(f, x, g, u, st);
+    if (rows <= 64) return run_few<64, T>(f, x, g, u, st);
+    return run_few<128, T>(f, x, g, u, st);
   }
   Gemm p{};
   p.M = rows; p.N = F; p.steps = p.first = ceil_div(I, kStep); p.act = act;
