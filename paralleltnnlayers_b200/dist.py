@@ -170,9 +170,22 @@ class P2PAllreduce:
             self._ctx = None
 
 
-def cp4_data_parallel_step(X, dU, FT, FC, FY, FX, pad=1, flags=0, group=None):
-    """forward, backward-data and backward-filter on this rank's shard, then the gradient allreduce.
-    Returns (U, dX, (dFT, dFC, dFY, dFX)) with the gradients summed over every rank's shard."""
+def _update(optimizer, params, grads):
+    """The summed gradients handed to ``optimizer`` (an ``optim.AdamW`` over the factors, or any optimiser with torch's interface) and one
+    step of it: every rank takes the same step."""
+    if optimizer is None:
+        return
+    known = {id(p) for g in optimizer.param_groups for p in g["params"]}
+    if not all(id(p) in known for p in params):
+        raise ValueError("the optimizer has to be over the factors of this step")
+    for p, g in zip(params, grads):
+        p.grad = g
+    optimizer.step()
+
+
+def cp4_data_parallel_step(X, dU, FT, FC, FY, FX, pad=1, flags=0, group=None, optimizer=None):
+    """forward, backward-data and backward-filter on this rank's shard, then the gradient allreduce and, with ``optimizer`` (over the four
+    factors), its step.  Returns (U, dX, (dFT, dFC, dFY, dFX)) with the gradients summed over every rank's shard."""
     from . import ops
     U = ops.cp4_conv2d_forward(X, FT, FC, FY, FX, pad, flags)
     dX = ops.cp4_conv2d_backward_data(dU, FT, FC, FY, FX, pad, flags)
@@ -182,6 +195,7 @@ def cp4_data_parallel_step(X, dU, FT, FC, FY, FX, pad=1, flags=0, group=None):
     sizes = [FT.shape[0] * R, FC.shape[0] * R, FY.shape[0] * R, FX.shape[0] * R]
     parts = torch.split(packed, sizes)
     grads = tuple(p.view(-1, R) for p in parts)
+    _update(optimizer, (FT, FC, FY, FX), grads)
     return U, dX, grads
 
 
@@ -197,10 +211,10 @@ def _unpack(packed, like):
     return out
 
 
-def rcp_data_parallel_step(X, dV, A, S, allreduce=None, group=None):
+def rcp_data_parallel_step(X, dV, A, S, allreduce=None, group=None, optimizer=None):
     """Reshaped-CP conv on this rank's batch shard: forward, data gradient and factor gradients, then ONE allreduce of
     the packed factor gradients ``[dA_1 | ... | dA_m | dS]`` (sum_k c_k t_k R + FH FW R floats).  ``allreduce`` is a
-    callable on the packed buffer (e.g. a ``P2PAllreduce``); default: ``allreduce_factor_grads``.
+    callable on the packed buffer (e.g. a ``P2PAllreduce``); default: ``allreduce_factor_grads``.  ``optimizer`` (over the factors): takes its step.
     Returns (V, dX, [dA_k], dS) with the gradients summed over all ranks."""
     from . import ops
     V = ops.conv2d_rcp_fused_nchw(X, *A, S)
@@ -208,16 +222,19 @@ def rcp_data_parallel_step(X, dV, A, S, allreduce=None, group=None):
     packed = _pack(list(dA) + [dS])
     (allreduce or (lambda t: allreduce_factor_grads(t, group)))(packed)
     *dA, dS = _unpack(packed, list(dA) + [dS])
+    _update(optimizer, [*A, S], [*dA, dS])
     return V, dX, dA, dS
 
 
-def dense_data_parallel_step(X, dY, F, allreduce=None, group=None):
+def dense_data_parallel_step(X, dY, F, allreduce=None, group=None, optimizer=None):
     """CP dense layer on this rank's batch shard: forward, data gradient and factor gradients, then ONE allreduce of
-    the packed factor gradients (sum_k i_k o_k R floats: 8 192 at 8^4 -> 8^4, R = 32).
+    the packed factor gradients (sum_k i_k o_k R floats: 8 192 at 8^4 -> 8^4, R = 32).  ``optimizer`` (over the factors): takes its step.
     Returns (Y, dX, [dF_k]) with the gradients summed over all ranks."""
     from . import ops
     Y = ops.dense_cp(X, *F)
     dX, dF = ops.dense_cp_backward(X, dY, *F)
     packed = _pack(dF)
     (allreduce or (lambda t: allreduce_factor_grads(t, group)))(packed)
-    return Y, dX, _unpack(packed, dF)
+    dF = _unpack(packed, dF)
+    _update(optimizer, F, dF)
+    return Y, dX, dF

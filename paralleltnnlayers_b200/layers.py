@@ -4,7 +4,8 @@ The reference builds its layers with ``conv2d_tensor`` / ``dense_tensor`` (test/
 compression ``rate`` is turned into a CP rank by ``generate_params_*`` (pure integer arithmetic, restated here),
 factor variables are created, and the layer is the sequential or the fused op.  These modules keep that
 interface for the three CP layer families of the hot path; weights live in the layout the C ABI takes
-(``[dim, R]`` factors for CP4, ``[c_k, t_k, R]`` for rCP, ``[i_k, o_k, R]`` for the dense layer).
+(``[dim, R]`` factors for CP4, ``[c_k, t_k, R]`` for rCP, ``[i_k, o_k, R]`` for the dense layer).  Beside them stand
+``AdaptedDense`` (a shared projection with low-rank adapters per request) and ``GatedDense`` (the gated half of a feed-forward block).
 """
 from __future__ import annotations
 
@@ -191,3 +192,57 @@ class CPDense(nn.Module):
         else:
             y = _ops().CPDenseFunction.apply(x.reshape(-1, x.shape[-1]).contiguous(), *self.factors).reshape(*x.shape[:-1], -1)
         return y if self.bias is None else y + self.bias
+
+
+class AdaptedDense(nn.Module):
+    """A shared projection with one low-rank adapter per request: ``shared(x) + scale[a] (x A[a]) B[a]`` for rows of adapter ``a``.
+
+    ``shared``: a ``CPDense`` or any module ``[..., in_features] -> [..., out_features]``; its parameters are frozen unless ``freeze=False``.  ``count``
+    adapters of rank ``rank`` start at zero (``B`` is zero), in the type of ``dtype`` (the shared layer's).  ``forward(x, adapters)``: ``adapters``
+    holds the adapter of each row (any number outside ``0 .. count - 1``: none), or is an ``ops.AdapterPlan`` that all layers of a batch share."""
+
+    def __init__(self, shared, count, rank, in_features=None, out_features=None, scale=1.0, freeze=True, dtype=None):
+        super().__init__()
+        if isinstance(shared, CPDense):
+            in_features, out_features = math.prod(shared.input_shape), math.prod(shared.output_shape)
+        in_features = in_features or getattr(shared, "in_features", None)
+        out_features = out_features or getattr(shared, "out_features", None)
+        if not in_features or not out_features:
+            raise ValueError("in_features and out_features of the shared projection are needed")
+        if count < 1 or not 1 <= rank <= 128:
+            raise ValueError("at least one adapter, of a rank of 1 to 128")
+        self.shared = shared
+        if freeze:
+            for p in shared.parameters():
+                p.requires_grad_(False)
+        if dtype is None:
+            dtype = next((p.dtype for p in shared.parameters()), torch.float32)
+        self.A = nn.Parameter((torch.randn(count, in_features, rank) * in_features ** -0.5).to(dtype))
+        self.B = nn.Parameter(torch.zeros(count, rank, out_features, dtype=dtype))
+        self.register_buffer("scale", torch.full((count,), float(scale), dtype=torch.float32))
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self.scale = self.scale.float()   # a type given to the module is that of the adapters; the scales stay float32
+        return self
+
+    def forward(self, x, adapters):
+        return _ops().DenseAdaptersFunction.apply(self.shared(x), x, self.A, self.B, adapters, self.scale)
+
+
+class GatedDense(nn.Module):
+    """The gated half of a feed-forward block, ``act(x Wg) * (x Wu)`` as one kernel; bfloat16 or float16.  What follows it is any dense layer
+    (``CPDense`` in float32, or a product of its own type)."""
+
+    def __init__(self, in_features, hidden_features, activation="silu", dtype=torch.bfloat16):
+        super().__init__()
+        if activation not in ("silu", "gelu", "gelu_tanh"):
+            raise ValueError("activation is silu, gelu or gelu_tanh")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("dtype is bfloat16 or float16")
+        self.activation = activation
+        make = lambda: nn.Parameter((torch.randn(in_features, hidden_features) * in_features ** -0.5).to(dtype))  # noqa: E731
+        self.Wg, self.Wu = make(), make()
+
+    def forward(self, x):
+        return _ops().DenseGatedFunction.apply(x, self.Wg, self.Wu, self.activation)

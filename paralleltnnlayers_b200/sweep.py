@@ -1,6 +1,6 @@
 """Kernel timings of every layer family at the sizes of the benchmark configurations.
 
-    python -m paralleltnnlayers_b200.sweep [cp4] [rcp] [dense] [--reps 12] [--json]
+    python -m paralleltnnlayers_b200.sweep [cp4] [rcp] [dense] [adapters] [gated] [adamw] [--reps 12] [--json]
     python -m paralleltnnlayers_b200.sweep --shapes FILE [--ranks 1,2,4,8,16] [--reps 47] [--out results.csv] [--mem]
 
 The second form reads a shape list in the reference's format (``N C H W pad T Y X`` per line, ``#`` comments;
@@ -132,6 +132,60 @@ def sweep_dense(P, reps, rows):
                  "hbm_floor_us": 2 * X.numel() * 4 / 6.45e12 * 1e6})
 
 
+ADAPTERS = [(64, 32, 16), (4096, 8, 16), (4096, 8, 64)]   # rows, adapters, rank; 4096 -> 4096
+GATED = [1, 64, 4096]                                     # rows; 4096 -> 10240
+
+
+def sweep_adapters(P, reps, rows):
+    for (S, n, R) in ADAPTERS:
+        for dtype in (torch.bfloat16, torch.float32):
+            gen = torch.Generator(device="cuda").manual_seed(40)
+            mk = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dtype)  # noqa: E731,B023
+            I = O = 4096
+            A, B = mk(n, I, R) * I ** -0.5, mk(n, R, O) * R ** -0.5
+            Xs, Ys = _sets(mk(S, I), most=8), _sets(mk(S, O), most=8)
+            k = len(Xs)
+            which = torch.randint(n, (S,), generator=gen, device="cuda", dtype=torch.int32)
+            plan = P.adapter_plan(which, n)
+            V = mk(S, R)
+            size = torch.finfo(dtype).bits // 8
+            rows.append({"layer": "adapters", "rows": S, "adapters": n, "R": R, "dtype": str(dtype)[6:],
+                         "fwd": timeit(lambda i: P.dense_adapters(Ys[i % k], Xs[i % k], A, B, which), reps),
+                         "fwd_planned": timeit(lambda i: P.dense_adapters(Ys[i % k], Xs[i % k], A, B, plan), reps),
+                         "bwd": timeit(lambda i: P.dense_adapters_backward(Ys[i % k], Xs[i % k], V, A, B, plan), reps),
+                         "hbm_floor_us": size * (S * (I + 2 * O) + min(n, S) * R * (I + O)) / 6.45e12 * 1e6})
+            del Xs, Ys
+            torch.cuda.empty_cache()
+
+
+def sweep_gated(P, reps, rows):
+    I, F = 4096, 10240
+    for S in GATED:
+        gen = torch.Generator(device="cuda").manual_seed(50)
+        mk = lambda *s: torch.randn(*s, generator=gen, device="cuda").bfloat16()  # noqa: E731,B023
+        W = [(mk(I, F) * I ** -0.5, mk(I, F) * I ** -0.5) for _ in range(2 if S < 512 else 1)]   # weights of two layers are more than the L2 holds
+        x, dh = mk(S, I), mk(S, F)
+        row = {"layer": "gated", "rows": S, "I": I, "F": F, "fwd": timeit(lambda i: P.dense_gated(x, *W[i % len(W)]), reps)}
+        _, G, U = P.dense_gated_save(x, *W[0])
+        row["bwd"] = timeit(lambda i: P.dense_gated_backward(dh, x, *W[i % len(W)], G, U), max(2, reps // 3))
+        row["hbm_floor_us"] = 2 * (S * (I + F) + 2 * I * F) / 6.45e12 * 1e6
+        rows.append(row)
+        torch.cuda.empty_cache()
+    P.device_status()
+
+
+def sweep_adamw(P, reps, rows):
+    for name, sizes in (("factors", [1024] * 6 + [4096] * 8 + [8192] * 16 + [48] * 60), ("weights", [4096 * 4096] * 2)):
+        for bits in (32, 8):
+            z = lambda n, t: torch.zeros(n, dtype=t, device="cuda")  # noqa: E731
+            p, g = ([torch.randn(n, device="cuda") for n in sizes] for _ in range(2))
+            m, v = ([z(n, t) for n in sizes] for t in ((torch.int8, torch.uint8) if bits == 8 else (torch.float32,) * 2))
+            scales = tuple([z((n + 255) // 256, torch.float32) for n in sizes] for _ in range(2)) if bits == 8 else None
+            rows.append({"layer": "adamw", "tensors": name, "values": sum(sizes), "bits": bits,
+                         "step": timeit(lambda i: P.adamw_step(p, g, m, v, 10, 1e-3, scales=scales), reps),
+                         "hbm_floor_us": sum(sizes) * (28 if bits == 32 else 16.0625) / 6.45e12 * 1e6})
+
+
 def read_shapes(path):
     """Unique shapes of a reference-format list, in the order ``tensor_shape::operator<`` gives them
     (Cuda_kernels/Tensor.cuh:10-25: lexicographic over N, C, H, W, pad, T, Y, X)."""
@@ -191,9 +245,12 @@ def bench_shapes(P, path, ranks, reps, out):
         sys.stdout.write(text)
 
 
+SWEEPS = {"cp4": sweep_cp4, "rcp": sweep_rcp, "dense": sweep_dense, "adapters": sweep_adapters, "gated": sweep_gated, "adamw": sweep_adamw}
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
-    ap.add_argument("which", nargs="*", help="any of cp4, rcp, dense (default: all)")
+    ap.add_argument("which", nargs="*", help="any of cp4, rcp, dense (default: these three), adapters, gated, adamw")
     ap.add_argument("--reps", type=int, default=12)
     ap.add_argument("--json", action="store_true", help="one JSON object per line instead of text")
     ap.add_argument("--shapes", help="shape list in the reference's format: time the CP4 forward per shape and rank")
@@ -212,13 +269,13 @@ def main(argv=None):
         return 0
     args.which = args.which or ["cp4", "rcp", "dense"]
     for w in args.which:
-        if w not in ("cp4", "rcp", "dense"):
+        if w not in SWEEPS:
             ap.error(f"unknown layer family {w!r}")
     import paralleltnnlayers_b200 as P   # raises if libb200cp.so is missing
     assert torch.cuda.is_available(), "the sweep needs a CUDA device"
     rows = []
     for w in args.which:
-        {"cp4": sweep_cp4, "rcp": sweep_rcp, "dense": sweep_dense}[w](P, args.reps, rows)
+        SWEEPS[w](P, args.reps, rows)
     for r in rows:
         if args.json:
             print(json.dumps(r))
