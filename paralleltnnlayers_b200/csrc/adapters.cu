@@ -225,6 +225,40 @@ __device__ __forceinline__ void load_rows(char* dst, int stride, Row row, int c0
   }
 }
 
+// The same for rows that start on 16-byte boundaries, chunk after chunk of PIECES x 16 bytes (or, STEP given, of STEP bytes in memory): where a thread's pieces
+// come from is worked out once, so that a chunk takes a few instructions of it (worked out anew for each: 4096 rows 36 us).
+template <typename T, int ROWS, int PIECES>
+struct Rows {
+  static constexpr int E = 16 / sizeof(T), EACH = kThreads / PIECES, N = (ROWS + EACH - 1) / EACH;
+  const char* from[N];
+  bool in[N];
+  template <typename Row>
+  __device__ __forceinline__ void set(Row row, const void* any) {
+    const int q = threadIdx.x % PIECES, r0 = threadIdx.x / PIECES;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = r0 + i * EACH;
+      const T* p = ROWS % EACH == 0 || r < ROWS ? row(r) : nullptr;
+      in[i] = p != nullptr;
+      from[i] = p ? reinterpret_cast<const char*>(p + q * E) : static_cast<const char*>(any);
+    }
+  }
+  // `at` bytes on from the first chunk; bytes: of this thread's piece of a row that are inside (16, or less in the last chunk)
+  __device__ __forceinline__ void load(char* dst, int stride, size_t at, int bytes) const {
+    dst += threadIdx.x / PIECES * stride + threadIdx.x % PIECES * 16;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (ROWS % EACH == 0 || threadIdx.x / PIECES + i * EACH < ROWS)
+        copy16(dst + i * EACH * stride, bytes > 0 ? from[i] + at : from[i], in[i] ? bytes : 0);
+  }
+};
+// of a thread's piece of a chunk from column c0 on
+template <typename T, int PIECES>
+__device__ __forceinline__ int piece_bytes(int c0, int cols) {
+  constexpr int E = 16 / sizeof(T);
+  return c0 + PIECES * E <= cols ? 16 : min(16, max(0, (cols - c0 - (int)(threadIdx.x % PIECES) * E) * (int)sizeof(T)));
+}
+
 // ---- products ---------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -305,7 +339,7 @@ struct Shape {
   static constexpr int ls = RP * (int)sizeof(T) + 16;                   // of a factor with the rank innermost
   static constexpr int factor = KC * ls > RP * xs ? KC * ls : RP * xs;
   static constexpr int stage = TM * xs + factor;
-  static constexpr int stages = RP <= 32 ? 4 : 3;
+  static constexpr int stages = 4;
   static constexpr int CG = sizeof(T) == 4 && RP > 32 ? RP / 32 : 1;    // fp32: groups of 32 ranks over warps
   static constexpr int MG = sizeof(T) == 4 ? 1 : TM / 16;               // 16-bit: groups of 16 rows over warps
   static constexpr int KG = kWarps / (MG * CG);                         // parts of a chunk's sum over warps
@@ -313,10 +347,11 @@ struct Shape {
   static constexpr int ring = stages * stage > red ? stages * stage : red;
   static constexpr int part = TM * RP * 4, vs = TM * ls;
   static constexpr int smem = ring + part + vs + TM * 4;
+  static constexpr int fit = 227 * 1024 / (smem + 1024), ctas = fit > 4 ? 4 : fit < 1 ? 1 : fit;   // of an SM, which the registers have to allow too
 };
 
 template <typename T, int TM, int RP, bool BACK>
-__global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constant__ Args g) {
+__global__ void __launch_bounds__(kThreads, (Shape<T, TM, RP>::ctas)) adapters_kernel(const __grid_constant__ Args g) {
   using S = Shape<T, TM, RP>;
   constexpr int KC = S::KC, E = S::E;
   extern __shared__ __align__(16) char sm[];
@@ -378,21 +413,11 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
   T* out = static_cast<T*>(g.out);
   const int K = g.K, N = g.N, R = g.R;
   const int nn = (N + KC - 1) / KC, nper = (nn + (int)csize - 1) / (int)csize, n0 = min(nn, (int)crank * nper), n1 = min(nn, n0 + nper);
-  const auto store_chunk = [&](const char* src, int c0) {   // [len][KC] in shared memory -> out
-    if (g.vy) {
-      const int q = tid % S::pieces, c = c0 + q * E;
-      if (c >= N) return;   // (rows of whole pieces)
-#pragma unroll
-      for (int i = 0; i < TM * S::pieces / kThreads; ++i) {
-        const int r = tid / S::pieces + i * (kThreads / S::pieces);
-        if (r < len) *reinterpret_cast<uint4*>(out + (size_t)rowat[r] * N + c) = *reinterpret_cast<const uint4*>(src + r * S::xs + q * 16);
-      }
-    } else {
-      const int q = tid % KC, c = c0 + q;
-      if (c >= N) return;
+  const auto store_values = [&](const char* src, int c0) {   // [len][KC] in shared memory -> out, value by value
+    const int q = tid % KC, c = c0 + q;
+    if (c >= N) return;
 #pragma unroll 4
-      for (int r = tid / KC; r < len; r += kThreads / KC) out[(size_t)rowat[r] * N + c] = reinterpret_cast<const T*>(src + r * S::xs)[q];
-    }
+    for (int r = tid / KC; r < len; r += kThreads / KC) out[(size_t)rowat[r] * N + c] = reinterpret_cast<const T*>(src + r * S::xs)[q];
   };
   if (a == g.count) {   // rows without an adapter
     if (out == Y) return;
@@ -402,19 +427,37 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
       copies_end_group();
       copies_wait<0>();
       __syncthreads();
-      store_chunk(sm, n * KC);
+      store_values(sm, n * KC);
       __syncthreads();
     }
     return;
   }
   const T *F1 = static_cast<const T*>(g.F1) + (size_t)a * R * K, *F2 = static_cast<const T*>(g.F2) + (size_t)a * R * N;
   // a factor's chunk: KC features by the ranks, as it lies in memory
-  const auto load_factor = [&](char* dst, const T* F, int n, bool long_rows, int c0, bool vec) {
+  const auto load_factor = [&](char* dst, const T* F, int n, bool long_rows, int c0) {
     if (long_rows)
-      load_rows<T, RP, S::pieces>(dst, S::xs, [&](int r) { return r < R ? F + (size_t)r * n : nullptr; }, c0, n, vec, F);
+      load_rows<T, RP, S::pieces>(dst, S::xs, [&](int r) { return r < R ? F + (size_t)r * n : nullptr; }, c0, n, false, F);
     else
-      load_rows<T, KC, RP / E>(dst, S::ls, [&](int r) { return c0 + r < n ? F + (size_t)(c0 + r) * R : nullptr; }, 0, R, vec, F);
+      load_rows<T, KC, RP / E>(dst, S::ls, [&](int r) { return c0 + r < n ? F + (size_t)(c0 + r) * R : nullptr; }, 0, R, false, F);
   };
+  // LONG: rows of n features, a row per rank; else rows of R ranks, of which a chunk has KC and the last one fewer
+  Rows<T, BACK ? RP : KC, BACK ? S::pieces : RP / E> f1;
+  const int rank_bytes = min(16, max(0, (R - (int)(tid % (RP / E)) * E) * (int)sizeof(T)));
+  f1.set([&](int r) { return BACK ? (r < R ? F1 + (size_t)r * K : nullptr) : F1 + (size_t)r * R; }, F1);
+  // (a chunk's rows past the last feature: a thread has one, since a chunk's KC rows are at most as many as its threads' places)
+  const auto load_ranks = [&](const auto& f, char* dst, int c0, int n) {
+    constexpr int EACH = kThreads / (RP / E);
+    dst += tid / (RP / E) * S::ls + tid % (RP / E) * 16;
+#pragma unroll
+    for (int i = 0; i < (KC + EACH - 1) / EACH; ++i) {
+      const int r = tid / (RP / E) + i * EACH;
+      if (KC % EACH != 0 && r >= KC) break;
+      const int bytes = c0 + r < n ? rank_bytes : 0;
+      copy16(dst + i * EACH * S::ls, bytes ? f.from[i] + (size_t)c0 * R * sizeof(T) : f.from[0], bytes);
+    }
+  };
+  Rows<T, TM, S::pieces> xr;
+  xr.set([&](int r) { return r < len ? X + (size_t)rowat[r] * K : nullptr; }, X);
 
   // what the second product reads is on its way to L2 meanwhile
   if (n1 > n0) {
@@ -434,8 +477,19 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
   const auto load_k = [&](int k) {
     if (k < k1) {
       char* st = sm + (k - k0) % S::stages * S::stage;
-      load_rows<T, TM, S::pieces>(st, S::xs, [&](int r) { return r < len ? X + (size_t)rowat[r] * K : nullptr; }, k * KC, K, g.vx, X);
-      load_factor(st + TM * S::xs, F1, K, BACK, k * KC, g.v1);
+      const int c0 = k * KC, bytes = piece_bytes<T, S::pieces>(c0, K);
+      if (g.vx)
+        xr.load(st, S::xs, (size_t)c0 * sizeof(T), bytes);
+      else
+        load_rows<T, TM, S::pieces>(st, S::xs, [&](int r) { return r < len ? X + (size_t)rowat[r] * K : nullptr; }, c0, K, false, X);
+      st += TM * S::xs;
+      if (!g.v1) {
+        load_factor(st, F1, K, BACK, c0);
+      } else if constexpr (BACK) {
+        f1.load(st, S::xs, (size_t)c0 * sizeof(T), bytes);
+      } else {
+        load_ranks(f1, st, c0, K);
+      }
     }
     copies_end_group();
   };
@@ -524,11 +578,43 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(const __grid_constan
     part[i] = v;
   }
   __syncthreads();
+  // (set here, and not before: what the second product needs takes no registers of the first)
+  Rows<T, BACK ? KC : RP, BACK ? RP / E : S::pieces> f2;
+  f2.set([&](int r) { return BACK ? F2 + (size_t)r * R : (r < R ? F2 + (size_t)r * N : nullptr); }, F2);
+  Rows<T, TM, S::pieces> yr;
+  if (Y) yr.set([&](int r) { return r < len ? Y + (size_t)rowat[r] * N : nullptr; }, Y);
+  constexpr int STORES = TM * S::pieces / kThreads;
+  T* outat[STORES];   // where a thread's pieces of a chunk go, in the first one
+#pragma unroll
+  for (int i = 0; i < STORES; ++i) {
+    const int r = tid / S::pieces + i * (kThreads / S::pieces);
+    outat[i] = out + (size_t)(r < len ? rowat[r] : 0) * N + tid % S::pieces * E;
+  }
+  const auto store_chunk = [&](const char* src, int c0) {
+    if (!g.vy) return store_values(src, c0);
+    const int q = tid % S::pieces;
+    if (c0 + q * E >= N) return;   // (rows of whole pieces)
+#pragma unroll
+    for (int i = 0; i < STORES; ++i)
+      if (tid / S::pieces + i * (kThreads / S::pieces) < len)
+        *reinterpret_cast<uint4*>(outat[i] + c0) = *reinterpret_cast<const uint4*>(src + (tid / S::pieces + i * (kThreads / S::pieces)) * S::xs + q * 16);
+  };
   const auto load_n = [&](int n) {
     if (n < n1) {
       char* st = sm + (n - n0) % S::stages * S::stage;
-      if (Y) load_rows<T, TM, S::pieces>(st, S::xs, [&](int r) { return r < len ? Y + (size_t)rowat[r] * N : nullptr; }, n * KC, N, g.vy, Y);
-      load_factor(st + TM * S::xs, F2, N, !BACK, n * KC, g.v2);
+      const int c0 = n * KC, bytes = piece_bytes<T, S::pieces>(c0, N);
+      if (Y && g.vy)
+        yr.load(st, S::xs, (size_t)c0 * sizeof(T), bytes);
+      else if (Y)
+        load_rows<T, TM, S::pieces>(st, S::xs, [&](int r) { return r < len ? Y + (size_t)rowat[r] * N : nullptr; }, c0, N, false, Y);
+      st += TM * S::xs;
+      if (!g.v2) {
+        load_factor(st, F2, N, !BACK, c0);
+      } else if constexpr (BACK) {
+        load_ranks(f2, st, c0, N);
+      } else {
+        f2.load(st, S::xs, (size_t)c0 * sizeof(T), bytes);
+      }
     }
     copies_end_group();
   };
@@ -676,9 +762,9 @@ struct GradShape {
   static constexpr int smem = stages * stage + index + table * 4;
   static constexpr int ctas() { return 227 * 1024 / (smem + 1024); }   // of an SM
 };
-__device__ __forceinline__ int range_rows(const GradArgs& g, int kt) {   // of a range: a multiple of a step
+__device__ __forceinline__ int range_rows(const GradArgs& g) {   // of a range: a multiple of 16
   const int each = (g.head[1] + g.ranges - 1) / g.ranges;
-  return max(kt, (each + kt - 1) / kt * kt);
+  return max(16, (each + 15) / 16 * 16);
 }
 __device__ __forceinline__ int adapter_at(const int* start, int count, int pos) {   // the adapter that has row `pos` of the order
   int a = 0, b = count + 1;
@@ -718,7 +804,7 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
   const T *Z = static_cast<const T*>(second ? g.dY : g.X), *W = static_cast<const T*>(second ? g.V : g.W);
   T* out = static_cast<T*>(second ? g.dB : g.dA);
   const bool vz = second ? g.vy : g.vx;
-  const int per = range_rows(g, KT), b = min(g.head[1], (int)blockIdx.y * per), e = min(g.head[1], b + per);
+  const int per = range_rows(g), b = min(g.head[1], (int)blockIdx.y * per), e = min(g.head[1], b + per);
   // Where the adapters' rows start, beside the ring where they fit: a step that begins an adapter searches them.
   int *index = reinterpret_cast<int*>(sm + S::stages * S::stage), *table = index + 2 * KT;
   const bool fits = g.count + 2 <= S::table;
@@ -834,9 +920,8 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
 // Adapters that lie in several ranges: the sum of their parts in the order of the ranges.  Adapters without rows: zero.
 template <typename T, int RP>
 __global__ void __launch_bounds__(kThreads) join_grads_kernel(const __grid_constant__ GradArgs g) {
-  constexpr int KT = GradShape<T, RP>::KT;
   grid_dependency_wait();
-  const int a = blockIdx.x, ab = g.start[a], ae = g.start[a + 1], per = range_rows(g, KT);
+  const int a = blockIdx.x, ab = g.start[a], ae = g.start[a + 1], per = range_rows(g);
   const int r0 = ab / per, r1 = ae > ab ? (ae - 1) / per : r0;
   if (ae > ab && r0 == r1) return;
   // A thread has a feature and four ranks; neighbours have neighbouring features.
@@ -903,7 +988,7 @@ template <typename T, int RP>
 int ranges_for(int rows, int I, int O) {   // as many as the machine holds at once with all tiles of features
   using S = GradShape<T, RP>;
   const int tiles = ceil_div(I, S::LT) + ceil_div(O, S::LT);
-  return std::max(1, std::min({148 * S::ctas() / tiles, ceil_div(rows, S::KT), 65535}));
+  return std::max(1, std::min({148 * S::ctas() / tiles, ceil_div(rows, 16), 65535}));
 }
 int ranges_of(int rows, int I, int O, int R, int type) {
   const bool f32 = type == B200CP_FLOAT32;
