@@ -55,9 +55,10 @@ template <typename T>
 struct alignas(4 * sizeof(T)) Four {
   T v[4];
 };
+// (`vec`: all four of every thread are inside and on a boundary of four)
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, long long i, long long n, bool vec, float (&x)[4]) {
-  if (vec && i + 4 <= n) {
+  if (vec) {
     const Four<T> q = *reinterpret_cast<const Four<T>*>(p + i);
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = (float)q.v[k];
@@ -68,7 +69,7 @@ __device__ __forceinline__ void load4(const T* p, long long i, long long n, bool
 }
 template <typename T>
 __device__ __forceinline__ void store4(T* p, long long i, long long n, bool vec, const float (&x)[4]) {
-  if (vec && i + 4 <= n) {
+  if (vec) {
     Four<T> q;
 #pragma unroll
     for (int k = 0; k < 4; ++k) q.v[k] = (T)x[k];
@@ -115,7 +116,7 @@ __device__ __forceinline__ uint32_t to_codes(const float (&x)[4]) {   // of whol
   return __byte_perm(__byte_perm(bits(x[0]), bits(x[1]), 0x0040), __byte_perm(bits(x[2]), bits(x[3]), 0x0040), 0x5410);
 }
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, long long i, long long n, bool vec) {
-  if (vec && i + 4 <= n) return *reinterpret_cast<const uint32_t*>(p + i);
+  if (vec) return *reinterpret_cast<const uint32_t*>(p + i);
   uint32_t c = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -123,7 +124,7 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, long long i, lo
   return c;
 }
 __device__ __forceinline__ void store_codes(uint8_t* p, long long i, long long n, bool vec, uint32_t c) {
-  if (vec && i + 4 <= n) {
+  if (vec) {
     *reinterpret_cast<uint32_t*>(p + i) = c;
     return;
   }
@@ -195,80 +196,48 @@ __device__ __forceinline__ float warp_max(float x) {   // of magnitudes
 // 1 / s, or 0 where s or that is no normal number (then every code of the block is found by the exact operations)
 __device__ __forceinline__ float inverse_of(float s) { return s > 1e-37f && s < 1e37f ? 1.f / s : 0.f; }
 
-// (Six CTAs on an SM: 59 M values with 8-bit moments 228 -> 204 us, five 216.)
-template <typename P, typename G, bool SMALL, int CAP>
-__global__ void __launch_bounds__(kThreads, 6) adamw_kernel(const __grid_constant__ Table<CAP> t) {
-  int a = 0, b = t.count;   // the tensor whose pieces hold this CTA's
-  while (b - a > 1) {
-    const int c = (a + b) / 2;
-    if (t.first[c] <= (int)blockIdx.x) a = c; else b = c;
-  }
-  const Entry& e = t.e[a];
-  const long long n = e.n, base = (long long)((int)blockIdx.x - t.first[a]) * kPiece + (threadIdx.x >> 5) * kBlock;
-  float step = t.r.step, root = t.r.root, decay = t.r.decay;
-  if (t.r.t || t.r.lr) {
-    __shared__ float rates[3];
-    if (threadIdx.x == 0) {
-      const double lr = t.r.lr ? (double)*t.r.lr : t.r.lr_;
-      double s = t.r.step, q = t.r.root;   // (of lr = 1, where lr is on the device)
-      if (t.r.t) {
-        const double at = (double)*t.r.t;
-        s = 1.0 / (1.0 - pow(t.r.b1_, at));
-        q = 1.0 / sqrt(1.0 - pow(t.r.b2_, at));
-      }
-      rates[0] = (float)(lr * s);
-      rates[1] = (float)q;
-      rates[2] = (float)(lr * t.r.wd);
-    }
-    __syncthreads();
-    step = rates[0];
-    root = rates[1];
-    decay = rates[2];
-  }
-  if (base >= n) return;
+// A warp's 256 values of a tensor, from `base` on.  WHOLE: all are there and every array is on a boundary of four (without a check per access, which were a
+// tenth of the instructions of 8-bit moments).
+template <typename P, typename G, bool SMALL, bool WHOLE>
+__device__ __forceinline__ void update(const Entry& e, const Rates& r, float step, float root, float decay, long long base) {
   const int lane = threadIdx.x & 31;
+  const long long n = e.n, block = base / kBlock;
   P* p = static_cast<P*>(e.p);
   const G* g = static_cast<const G*>(e.g);
-  float *w = e.w, ms = 0.f, vs = 0.f;
-  const long long block = base / kBlock;
-  const bool vp = aligned4(p), vg = aligned4(g), vw = aligned4(w);
+  float* w = e.w;
   float x[2][4], d[2][4], m[2][4], v[2][4];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const long long i = base + j * 128 + lane * 4;
-    if (w) load4(w, i, n, vw, x[j]); else load4(p, i, n, vp, x[j]);
-    load4(g, i, n, vg, d[j]);
+    if (w) load4(w, i, n, WHOLE, x[j]); else load4(p, i, n, WHOLE, x[j]);
+    load4(g, i, n, WHOLE, d[j]);
   }
   if constexpr (SMALL) {
     const uint8_t *cm = static_cast<const uint8_t*>(e.m), *cv = static_cast<const uint8_t*>(e.v);
-    const bool vm = aligned4(cm), vv = aligned4(cv);
-    ms = e.ms[block];
-    vs = e.vs[block];
+    const float ms = e.ms[block], vs = e.vs[block];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const long long i = base + j * 128 + lane * 4;
-      values_of_m(load_codes(cm, i, n, vm), ms, m[j]);
-      values_of_v(load_codes(cv, i, n, vv), vs, v[j]);
+      values_of_m(load_codes(cm, i, n, WHOLE), ms, m[j]);
+      values_of_v(load_codes(cv, i, n, WHOLE), vs, v[j]);
     }
   } else {
-    const float *fm = static_cast<const float*>(e.m), *fv = static_cast<const float*>(e.v);
-    const bool vm = aligned4(fm), vv = aligned4(fv);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const long long i = base + j * 128 + lane * 4;
-      load4(fm, i, n, vm, m[j]);
-      load4(fv, i, n, vv, v[j]);
+      load4(static_cast<const float*>(e.m), i, n, WHOLE, m[j]);
+      load4(static_cast<const float*>(e.v), i, n, WHOLE, v[j]);
     }
   }
   float mm = 0.f, mv = 0.f;
-  const bool tiny_eps = t.r.eps < 1e-12f;   // then the square root of a subnormal v counts beside it
+  const bool tiny_eps = r.eps < 1e-12f;   // then the square root of a subnormal v counts beside it
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      m[j][k] = fmaf(t.r.c1, d[j][k], __fmul_rn(t.r.b1, m[j][k]));
-      v[j][k] = fmaf(t.r.c2, __fmul_rn(d[j][k], d[j][k]), __fmul_rn(t.r.b2, v[j][k]));
-      x[j][k] = fmaf(-step, m[j][k] * fast_inverse(fmaf(tiny_eps ? fast_sqrt(v[j][k]) : fast_sqrt_ftz(v[j][k]), root, t.r.eps)), fmaf(-decay, x[j][k], x[j][k]));
+      m[j][k] = fmaf(r.c1, d[j][k], __fmul_rn(r.b1, m[j][k]));
+      v[j][k] = fmaf(r.c2, __fmul_rn(d[j][k], d[j][k]), __fmul_rn(r.b2, v[j][k]));
+      x[j][k] = fmaf(-step, m[j][k] * fast_inverse(fmaf(tiny_eps ? fast_sqrt(v[j][k]) : fast_sqrt_ftz(v[j][k]), root, r.eps)), fmaf(-decay, x[j][k], x[j][k]));
       if (SMALL) {   // (values past the end are zero, and a NaN is never the larger: neither changes a maximum)
         mm = fmaxf(mm, fabsf(m[j][k]));
         mv = fmaxf(mv, v[j][k]);
@@ -277,8 +246,8 @@ __global__ void __launch_bounds__(kThreads, 6) adamw_kernel(const __grid_constan
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const long long i = base + j * 128 + lane * 4;
-    if (w) store4(w, i, n, vw, x[j]);
-    store4(p, i, n, vp, x[j]);
+    if (w) store4(w, i, n, WHOLE, x[j]);
+    store4(p, i, n, WHOLE, x[j]);
   }
   if constexpr (SMALL) {
     uint8_t *cm = static_cast<uint8_t*>(e.m), *cv = static_cast<uint8_t*>(e.v);
@@ -301,25 +270,61 @@ __global__ void __launch_bounds__(kThreads, 6) adamw_kernel(const __grid_constan
       e.ms[block] = mm;
       e.vs[block] = mv;
     }
-    const bool vm = aligned4(cm), vv = aligned4(cv);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const long long i = base + j * 128 + lane * 4;
       uint32_t p4, q4;
       codes_from(m[j], v[j], mm, mv, im, iv, p4, q4);
-      store_codes(cm, i, n, vm, p4);
-      store_codes(cv, i, n, vv, q4);
+      store_codes(cm, i, n, WHOLE, p4);
+      store_codes(cv, i, n, WHOLE, q4);
     }
   } else {
-    float *fm = static_cast<float*>(e.m), *fv = static_cast<float*>(e.v);
-    const bool vm = aligned4(fm), vv = aligned4(fv);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const long long i = base + j * 128 + lane * 4;
-      store4(fm, i, n, vm, m[j]);
-      store4(fv, i, n, vv, v[j]);
+      store4(static_cast<float*>(e.m), i, n, WHOLE, m[j]);
+      store4(static_cast<float*>(e.v), i, n, WHOLE, v[j]);
     }
   }
+}
+
+// (Six CTAs on an SM: 59 M values with 8-bit moments 228 -> 204 us, five 216.)
+template <typename P, typename G, bool SMALL, int CAP>
+__global__ void __launch_bounds__(kThreads, 6) adamw_kernel(const __grid_constant__ Table<CAP> t) {
+  int a = 0, b = t.count;   // the tensor whose pieces hold this CTA's
+  while (b - a > 1) {
+    const int c = (a + b) / 2;
+    if (t.first[c] <= (int)blockIdx.x) a = c; else b = c;
+  }
+  const Entry& e = t.e[a];
+  const long long base = (long long)((int)blockIdx.x - t.first[a]) * kPiece + (threadIdx.x >> 5) * kBlock;
+  float step = t.r.step, root = t.r.root, decay = t.r.decay;
+  if (t.r.t || t.r.lr) {
+    __shared__ float rates[3];
+    if (threadIdx.x == 0) {
+      const double lr = t.r.lr ? (double)*t.r.lr : t.r.lr_;
+      double s = t.r.step, q = t.r.root;   // (of lr = 1, where lr is on the device)
+      if (t.r.t) {
+        const double at = (double)*t.r.t;
+        s = 1.0 / (1.0 - pow(t.r.b1_, at));
+        q = 1.0 / sqrt(1.0 - pow(t.r.b2_, at));
+      }
+      rates[0] = (float)(lr * s);
+      rates[1] = (float)q;
+      rates[2] = (float)(lr * t.r.wd);
+    }
+    __syncthreads();
+    step = rates[0];
+    root = rates[1];
+    decay = rates[2];
+  }
+  if (base >= e.n) return;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(e.p) % (4 * sizeof(P)) | reinterpret_cast<uintptr_t>(e.g) % (4 * sizeof(G)) |
+                       reinterpret_cast<uintptr_t>(e.w) % 16 | (reinterpret_cast<uintptr_t>(e.m) | reinterpret_cast<uintptr_t>(e.v)) % (SMALL ? 4 : 16);
+  if (base + kBlock <= e.n && at == 0)
+    update<P, G, SMALL, true>(e, t.r, step, root, decay, base);
+  else
+    update<P, G, SMALL, false>(e, t.r, step, root, decay, base);
 }
 
 // Four groups of four values per thread, so that enough bytes are in flight (with one group 111 us of 58.7 M values).
@@ -328,7 +333,8 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) moments_kernel(long long n, const uint8_t* cm, const uint8_t* cv, const float* ms, const float* vs,
                                                            T* m, T* v) {
   const long long i0 = (long long)blockIdx.x * (kThreads * 4 * kMomentGroups) + threadIdx.x * 4;
-  const bool a = aligned4(cm), b = aligned4(cv), c = aligned4(m), d = aligned4(v);
+  const bool whole = i0 + (kMomentGroups - 1) * (kThreads * 4) + 4 <= n, a = whole && aligned4(cm), b = whole && aligned4(cv), c = whole && aligned4(m),
+             d = whole && aligned4(v);
   uint32_t p[kMomentGroups], q[kMomentGroups];
   float s[kMomentGroups], r[kMomentGroups];
 #pragma unroll

@@ -7,6 +7,8 @@
 // over the CTAs of a cluster and is joined through their shared memory, so that X is read once, V stays on the chip between the two
 // products and a few rows still fill the machine.  What bounds it is HBM: X and Y in, out once; the products take 2 R (I + O) operations a row, on
 // mma.sync for 16-bit types (R columns are too few to feed anything wider) and FFMA for fp32, whose sums are then those of fp32.
+// (Of what was tried to bring rows in sooner, prefetches of their parts into L2 cost 10 % more and copies of whole parts (cp.async.bulk, a thread per row)
+// 40 %: such a request takes an SM some 30 cycles, and there are thousands.)
 // Rows of a tile are gathered by the plan's order, so requests may lie anywhere in the batch; a row's result depends on its own row and
 // adapter only, and values that are not finite stay with theirs.  V and W are rounded once to the 16-bit type: they are operands of products.
 //
@@ -178,9 +180,6 @@ __device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.comm
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ void prefetch(const void* p, size_t bytes) {   // into L2; both multiples of 16
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((uint32_t)bytes) : "memory");
-}
 // ROWS rows of PIECES x 16 bytes into shared memory, a thread the same place of every row that it has: row r from row(r) (null: zeros), from column c0
 // on, zero past `cols`.  `vec`: the rows start on 16-byte boundaries (then the copies are asynchronous).  Else fp32 comes in asynchronous
 // words, and 16-bit values in words that a shift puts in place (a word that reaches past the row's ends is not read).
@@ -332,14 +331,15 @@ struct Args {
 
 template <typename T, int TM, int RP>
 struct Shape {
-  // A chunk is 128 bytes of each of 64 rows, so that three or four CTAs share an SM (with 256 bytes two; 4096 rows 4096 -> 4096 at rank 16
-  // 39 us), or 256 bytes of 16.
-  static constexpr int CB = TM == 64 ? 128 : 256, E = 16 / sizeof(T), KC = CB / sizeof(T), pieces = CB / 16;
+  // Bytes of a row in a chunk.  Of 64 rows 128, so that three or four CTAs share an SM, or 256 where two are all that fit anyway (rank 64) or what is done
+  // with a chunk is long (fp32 at rank 16: 93 us with 128, 76 with 256); of 16 rows 512 (64 requests 10.5 us with 256, 9.8 with 512).
+  static constexpr int CB = TM == 16 ? (RP <= 32 ? 512 : 256) : RP == 64 || (RP == 16 && sizeof(T) == 4) ? 256 : 128;
+  static constexpr int E = 16 / sizeof(T), KC = CB / sizeof(T), pieces = CB / 16;   // values of 16 bytes, values and pieces of a chunk
   static constexpr int xs = CB + 16;                                    // bytes from row to row: ldmatrix and 16-byte reads without conflicts
   static constexpr int ls = RP * (int)sizeof(T) + 16;                   // of a factor with the rank innermost
   static constexpr int factor = KC * ls > RP * xs ? KC * ls : RP * xs;
   static constexpr int stage = TM * xs + factor;
-  static constexpr int stages = 4;
+  static constexpr int stages = 3;
   static constexpr int CG = sizeof(T) == 4 && RP > 32 ? RP / 32 : 1;    // fp32: groups of 32 ranks over warps
   static constexpr int MG = sizeof(T) == 4 ? 1 : TM / 16;               // 16-bit: groups of 16 rows over warps
   static constexpr int KG = kWarps / (MG * CG);                         // parts of a chunk's sum over warps
@@ -348,6 +348,7 @@ struct Shape {
   static constexpr int part = TM * RP * 4, vs = TM * ls;
   static constexpr int smem = ring + part + vs + TM * 4;
   static constexpr int fit = 227 * 1024 / (smem + 1024), ctas = fit > 4 ? 4 : fit < 1 ? 1 : fit;   // of an SM, which the registers have to allow too
+  static_assert(smem <= 227 * 1024, "");
 };
 
 template <typename T, int TM, int RP, bool BACK>
@@ -458,19 +459,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, TM, RP>::ctas)) adapters_k
   };
   Rows<T, TM, S::pieces> xr;
   xr.set([&](int r) { return r < len ? X + (size_t)rowat[r] * K : nullptr; }, X);
-
-  // what the second product reads is on its way to L2 meanwhile
-  if (n1 > n0) {
-    const int c0 = n0 * KC, cols = min(N, n1 * KC) - c0;
-    if (Y && g.vy && tid < len) prefetch(Y + (size_t)rowat[tid] * N + c0, cols * sizeof(T));
-    if (g.v2) {
-      if (BACK) {
-        if (tid == 128 && cols < 4096) prefetch(F2 + (size_t)c0 * R, (size_t)cols * R * sizeof(T));
-      } else if (tid >= 128 && tid - 128 < R) {
-        prefetch(F2 + (size_t)(tid - 128) * N + c0, cols * sizeof(T));
-      }
-    }
-  }
 
   // ---- V: this CTA's part of the sum over K ----
   const int nk = (K + KC - 1) / KC, kper = (nk + (int)csize - 1) / (int)csize, k0 = min(nk, (int)crank * kper), k1 = min(nk, k0 + kper);
