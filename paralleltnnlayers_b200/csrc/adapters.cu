@@ -12,7 +12,7 @@
 // Rows of a tile are gathered by the plan's order, so requests may lie anywhere in the batch; a row's result depends on its own row and
 // adapter only, and values that are not finite stay with theirs.  V and W are rounded once to the 16-bit type: they are operands of products.
 //
-// dA and dB are one kernel over the rows in the plan's order, cut into ranges of equal length: a CTA has 128 (fp32: 64) features of a range and adds
+// dA and dB are one kernel over the rows in the plan's order, cut into ranges of equal length: a CTA has 128 features of a range and adds
 // row after row in registers until the adapter changes.  Adapters inside a range are written at once, those that reach into another range as
 // partial sums that a second launch joins in order: no atomics, the same bits each time.
 #include <cuda_bf16.h>
@@ -741,10 +741,11 @@ struct GradArgs {
   float* partial;               // [range][2][I + O][RP]
   int vx, vy, vr;
 };
+constexpr int kFeatures = 128;   // of a CTA of the gradients
 template <typename T, int RP>
 struct GradShape {
-  static constexpr int E = 16 / sizeof(T), LT = 256 / sizeof(T), KT = sizeof(T) == 4 ? 32 : 64;   // features and rows of a step
-  static constexpr int zs = 256 + 16, ws = RP * (int)sizeof(T) + 16;
+  static constexpr int E = 16 / sizeof(T), LT = kFeatures, KT = sizeof(T) == 4 ? 32 : 64;   // features and rows of a step
+  static constexpr int pieces = LT / E, zs = LT * (int)sizeof(T) + 16, ws = RP * (int)sizeof(T) + 16;
   static constexpr int stage = KT * (zs + ws), stages = 3;
   static constexpr int index = 2 * KT * 4, table = 1024;   // rows of two steps; adapters whose starts fit beside them
   static constexpr int smem = stages * stage + index + table * 4;
@@ -816,7 +817,7 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
       char* st = sm + loaded % S::stages * S::stage;
       const int n = min(KT, load.stop - load.pos);
       const int* rows = index + loaded % 2 * KT;
-      load_rows<T, KT, 16>(st, S::zs, [&](int r) { return r < n ? Z + (size_t)rows[r] * L : nullptr; }, l0, L, vz, Z);
+      load_rows<T, KT, S::pieces>(st, S::zs, [&](int r) { return r < n ? Z + (size_t)rows[r] * L : nullptr; }, l0, L, vz, Z);
       load_rows<T, KT, RP / E>(st + KT * S::zs, S::ws, [&](int r) { return r < n ? W + (size_t)rows[r] * R : nullptr; }, 0, R, g.vr, W);
       load.next(KT);
       ++loaded;
@@ -830,8 +831,8 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
     load_step();
     next_rows();
   }
-  // fp32: a warp has eight features, a lane LR of them and LC ranks; 16 bits: a warp has sixteen features and all ranks
-  constexpr int LC = RP == 16 ? 2 : 4, CGN = RP / LC, LR = CGN / 4;   // 8 / (32 / CGN)
+  // A warp has sixteen features and all ranks; fp32: a lane LR of them and LC ranks
+  constexpr int LC = RP == 16 ? 2 : 4, CGN = RP / LC, LR = CGN / 2;   // 16 / (32 / CGN)
   float acc[F32 ? LR : RP / 8][F32 ? LC : 4] = {};
   const int lr = F32 ? lane / CGN : lane >> 2, lc = F32 ? lane % CGN : lane & 3;
   for (int k = 0; !at.done(); ++k) {
@@ -843,12 +844,12 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
     if constexpr (F32) {
 #pragma unroll 4
       for (int t = 0; t < KT; ++t) {
-        const float *z = reinterpret_cast<const float*>(zt + t * S::zs) + warp * 8 + lr * LR, *w = reinterpret_cast<const float*>(wt + t * S::ws) + lc * LC;
+        const float *z = reinterpret_cast<const float*>(zt + t * S::zs) + warp * 16 + lr * LR, *w = reinterpret_cast<const float*>(wt + t * S::ws) + lc * LC;
         float x[LR], y[LC];
 #pragma unroll
-        for (int i = 0; i < LR; ++i) x[i] = z[i];
-#pragma unroll
-        for (int j = 0; j < LC; ++j) y[j] = w[j];
+        for (int i = 0; i < LR; i += 4) *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(z + i);
+        if constexpr (LC == 2) *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(w);
+        else *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(w);
 #pragma unroll
         for (int i = 0; i < LR; ++i)
 #pragma unroll
@@ -889,7 +890,7 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
       for (int i = 0; i < LR; ++i)
 #pragma unroll
         for (int j = 0; j < LC; ++j) {
-          put(warp * 8 + lr * LR + i, lc * LC + j, acc[i][j]);
+          put(warp * 16 + lr * LR + i, lc * LC + j, acc[i][j]);
           acc[i][j] = 0.f;
         }
     } else {
@@ -912,17 +913,17 @@ __global__ void __launch_bounds__(kThreads) join_grads_kernel(const __grid_const
   const int a = blockIdx.x, ab = g.start[a], ae = g.start[a + 1], per = range_rows(g);
   const int r0 = ab / per, r1 = ae > ab ? (ae - 1) / per : r0;
   if (ae > ab && r0 == r1) return;
-  // A thread has a feature and four ranks; neighbours have neighbouring features.
+  // A thread has a feature and four ranks: neighbours have neighbouring ranks of dA, and neighbouring features of dB, as they lie there.
   constexpr int Q = RP / 4;
-  const int la = g.dA ? g.I : 0, n = la + (g.dB ? g.O : 0), quads = (g.R + 3) / 4;
-  for (int i = blockIdx.y * kThreads + threadIdx.x; i < n * quads; i += gridDim.y * kThreads) {
-    const int q = i / n, x = i - q * n;
-    const bool second = x >= la;
-    const int l = second ? x - la : x, L = second ? g.O : g.I;
+  const int quads = (g.R + 3) / 4, na = g.dA ? g.I * quads : 0, n = na + (g.dB ? g.O * quads : 0);
+  const size_t step = (size_t)(g.I + g.O) * Q;
+  const bool vec = g.R % 4 == 0 && reinterpret_cast<uintptr_t>(g.dA) % (4 * sizeof(T)) == 0;
+  for (int i = blockIdx.y * kThreads + threadIdx.x; i < n; i += gridDim.y * kThreads) {
+    const bool second = i >= na;
+    const int x = second ? i - na : i, q = second ? x / g.O : x % quads, l = second ? x - q * g.O : x / quads;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (ae > ab) {
       const float4* p = reinterpret_cast<const float4*>(g.partial) + ((size_t)(second ? g.I : 0) + l) * Q + q;
-      const size_t step = (size_t)(g.I + g.O) * Q;
       v = p[(size_t)(2 * r0 + 1) * step];
 #pragma unroll 4
       for (int k = r0 + 1; k <= r1; ++k) {
@@ -931,11 +932,21 @@ __global__ void __launch_bounds__(kThreads) join_grads_kernel(const __grid_const
       }
     }
     const float e[4] = {v.x, v.y, v.z, v.w};
-    T* out = static_cast<T*>(second ? g.dB : g.dA) + (size_t)a * L * g.R;
+    if (!second) {
+      T* out = static_cast<T*>(g.dA) + ((size_t)a * g.I + l) * g.R + q * 4;
+      if (vec) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = v;
+        else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+      } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = q * 4 + j;
-      if (r < g.R) out[second ? (size_t)r * L + l : (size_t)l * g.R + r] = (T)e[j];
+        for (int j = 0; j < 4; ++j)
+          if (q * 4 + j < g.R) out[j] = (T)e[j];
+      }
+    } else {
+      T* out = static_cast<T*>(g.dB) + ((size_t)a * g.R + q * 4) * g.O + l;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (q * 4 + j < g.R) out[(size_t)j * g.O] = (T)e[j];
     }
   }
 }
@@ -1117,7 +1128,7 @@ int b200cp_dense_adapters_bwd(int rows, int I, int O, int R, int count, int type
   if (!dA && !dB) return B200CP_OK;
   GradArgs g{};
   g.rows = rows; g.I = I; g.O = O; g.R = R; g.count = count; g.ranges = ranges_of(rows, I, O, R, type);
-  g.tiles_i = dA ? ceil_div(I, type == B200CP_FLOAT32 ? 64 : 128) : 0;
+  g.tiles_i = dA ? ceil_div(I, kFeatures) : 0;
   g.X = X; g.W = W; g.V = V; g.dY = dY; g.dA = dA; g.dB = dB;
   plan_into(static_cast<const int*>(plan), p, &g.head, &g.start, &g.order);
   g.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + w_bytes(rows, R, type));
