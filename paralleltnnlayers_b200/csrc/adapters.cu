@@ -10,7 +10,9 @@
 // (Of what was tried to bring rows in sooner, prefetches of their parts into L2 cost 10 % more and copies of whole parts (cp.async.bulk, a thread per row)
 // 40 %: such a request takes an SM some 30 cycles, and there are thousands.)
 // Rows of a tile are gathered by the plan's order, so requests may lie anywhere in the batch; a row's result depends on its own row and
-// adapter only, and values that are not finite stay with theirs.  V and W are rounded once to the 16-bit type: they are operands of products.
+// adapter only, and values that are not finite stay with theirs.  As operands of the second
+// product V and W are two parts of the 16-bit type (rounded once, out of a token and an adapter would be as far off as by its own rounding, and at a
+// small rank up to twice that); they are rounded once where they are kept for dA and dB.
 //
 // dA and dB are one kernel over the rows in the plan's order, cut into ranges of equal length: a CTA has 128 features of a range and adds
 // row after row in registers until the adapter changes.  Adapters inside a range are written at once, those that reach into another range as
@@ -345,7 +347,7 @@ struct Shape {
   static constexpr int KG = kWarps / (MG * CG);                         // parts of a chunk's sum over warps
   static constexpr int red = KG * TM * RP * 4;
   static constexpr int ring = stages * stage > red ? stages * stage : red;
-  static constexpr int part = TM * RP * 4, vs = TM * ls;
+  static constexpr int part = TM * RP * 4, vs = TM * ls * (sizeof(T) == 2 ? 2 : 1);   // (V as two parts of a 16-bit type)
   static constexpr int smem = ring + part + vs + TM * 4;
   static constexpr int fit = 227 * 1024 / (smem + 1024), ctas = fit > 4 ? 4 : fit < 1 ? 1 : fit;   // of an SM, which the registers have to allow too
   static_assert(smem <= 227 * 1024, "");
@@ -635,6 +637,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, TM, RP>::ctas)) adapters_k
     T* to = reinterpret_cast<T*>(vs + r * S::ls) + j;
     to[0] = (T)(v.x * c);
     to[1] = (T)(v.y * c);
+    if constexpr (sizeof(T) == 2) {   // what the rounding left (of an infinity nothing)
+      T* rest = reinterpret_cast<T*>(vs + (TM + r) * S::ls) + j;
+      const float a0 = (float)to[0], a1 = (float)to[1];
+      rest[0] = fabsf(a0) < __int_as_float(0x7f800000) ? (T)(v.x * c - a0) : (T)0.f;
+      rest[1] = fabsf(a1) < __int_as_float(0x7f800000) ? (T)(v.y * c - a1) : (T)0.f;
+    }
     if (g.V && crank == 0 && r < len) {
       T* w = static_cast<T*>(g.V) + (size_t)rowat[r] * R + j;
       if (j < R) w[0] = to[0];
@@ -646,10 +654,13 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, TM, RP>::ctas)) adapters_k
 
   // ---- out = Y + V F2 ----
   constexpr int NG = kWarps / (TM / 16);
-  uint32_t va[F32 ? 1 : RP / 16][4];
+  uint32_t va[F32 ? 1 : RP / 16][4], vr[F32 ? 1 : RP / 16][4];
   if constexpr (!F32) {
 #pragma unroll
-    for (int j = 0; j < RP / 16; ++j) a_block(va[j], vs + mg * 16 * S::ls + j * 32, S::ls);
+    for (int j = 0; j < RP / 16; ++j) {
+      a_block(va[j], vs + mg * 16 * S::ls + j * 32, S::ls);
+      a_block(vr[j], vs + (TM + mg * 16) * S::ls + j * 32, S::ls);
+    }
   }
   for (int n = n0; n < n1; ++n) {
     copies_wait<S::stages - 2>();
@@ -718,6 +729,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, TM, RP>::ctas)) adapters_k
             b_block<false>(f, ft + j * S::xs + (nc + q) * 2, S::xs);
           mma16<T>(o[0], va[j / 16], f[0], f[1]);
           mma16<T>(o[1], va[j / 16], f[2], f[3]);
+          mma16<T>(o[0], vr[j / 16], f[0], f[1]);
+          mma16<T>(o[1], vr[j / 16], f[2], f[3]);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)

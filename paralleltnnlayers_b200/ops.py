@@ -422,8 +422,8 @@ def dense_adapters(Y, X, A, B, adapters, scale=None, out=None):
     """``out[s] = Y[s] + scale[a] (X[s] A[a]) B[a]``, ``a`` the adapter of row ``s``: what a shared projection gave for a batch of many requests,
     corrected for each by its own low-rank adapter (``b200cp_dense_adapters``).  Rows without an adapter come out as ``Y``.
 
-    ``X [..., I]``, ``Y [..., O]``, ``A [count, I, R]``, ``B [count, R, O]`` of one type: float32, bfloat16 or float16 (sums in float32; ``X A`` is
-    rounded to the type before the second product); ``R`` at most 128.  ``adapters``: an int32 or int64 tensor of ``X``'s leading shape, or
+    ``X [..., I]``, ``Y [..., O]``, ``A [count, I, R]``, ``B [count, R, O]`` of one type: float32, bfloat16 or float16 (sums in float32; ``scale (X A)``
+    has to be in the type's range); ``R`` at most 128.  ``adapters``: an int32 or int64 tensor of ``X``'s leading shape, or
     the ``AdapterPlan`` of one.  ``scale``: float32 per adapter.  ``out`` may be ``Y``."""
     which, planned = _which(adapters, X)
     return _C.dense_adapters(Y, X, A, B, which, planned, scale, out)

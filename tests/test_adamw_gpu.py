@@ -229,6 +229,19 @@ def test_optimiser_and_its_saved_state(bits, dtype):
     assert torch.equal(a[0].detach(), before) and one.state[a[0]]["step"] == 4 and one.state[a[1]]["step"] == 5
 
 
+def test_offsets_past_32_bits():
+    P = _p()
+    n = 2 ** 31 + 300
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    m, v = torch.zeros(n, dtype=torch.int8, device="cuda"), torch.zeros(n, dtype=torch.uint8, device="cuda")
+    s = [torch.zeros((n + 255) // 256, device="cuda") for _ in range(2)]
+    at = torch.tensor([0, 2 ** 31 - 1, 2 ** 31, n - 300, n - 1], device="cuda")
+    g[at] = torch.tensor([1.0, -2.0, 3.0, -4.0, 5.0], dtype=torch.bfloat16, device="cuda")
+    P.adamw_step([p], [g], [m], [v], 1, 0.5, weight_decay=0.0, scales=([s[0]], [s[1]]))
+    assert torch.equal(p[at], -0.5 * g[at].sign())   # a first step is lr times the gradient's sign
+    assert int(torch.count_nonzero(p)) == 4 + (1 if n - 300 != 2 ** 31 else 0) and int(torch.count_nonzero(m)) == len(set(at.tolist()))
+
+
 def test_a_tensor_twice_is_refused():
     P = _p()
     c = lambda: torch.ones(8, device="cuda")  # noqa: E731
