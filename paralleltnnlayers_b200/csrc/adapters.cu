@@ -36,7 +36,7 @@ static_assert(B200CP_ADAPTERS_WITHOUT_PLAN <= kThreads, "a thread has a row");
 // ints: [0] tiles, [1] rows with an adapter, [2..3] free | start[count + 2] | tile_adapter[tiles] | tile_first[tiles] | order[rows].
 // Rows without an adapter are those of "adapter" count, behind the others.
 struct Plan {
-  int tm, tiles;   // rows of a tile; the most tiles there can be
+  int tm, tiles, likely;   // rows of a tile; the most tiles there can be; as many as adapters whose last tile is half full give
   size_t start, adapter, first, order, ints;
 };
 Plan plan_of(int rows, int count) {
@@ -45,6 +45,7 @@ Plan plan_of(int rows, int count) {
   // Tiles of 64 rows read an adapter once per 64 rows, tiles of 16 waste less of themselves on adapters of a few rows.
   p.tm = groups > 0 && rows / groups >= 48 ? 64 : 16;
   p.tiles = rows / p.tm + std::min(rows, count + 1);
+  p.likely = rows / p.tm + (std::min(rows, count + 1) + 1) / 2;
   p.start = 4;
   p.adapter = p.start + count + 2;
   p.first = p.adapter + p.tiles;
@@ -86,6 +87,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(int rows, int count, int tm,
                                                     size_t at_first, size_t at_order) {
   extern __shared__ int counts[];
   __shared__ int warp_sums[32];
+  grid_launch_dependents();   // the kernel that reads the plan takes its place on the other SMs, and waits for this one there
   const int keys = count + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int* tiles_before = counts + keys * sorters;
   for (int i = tid; i < keys * sorters; i += 1024) counts[i] = 0;
@@ -95,10 +97,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(int rows, int count, int tm,
     const int a = adapters[r];
     return a >= 0 && a < count ? a : count;
   };
-  constexpr int Q = 8;   // turns of a warp whose loads are in flight together
+  constexpr int Q = 8;   // turns of a warp whose loads are in flight together (of a range of one such load they are kept for the second pass)
+  int key[Q];
   if (warp < sorters)
     for (int b = r0; b < r1; b += 32 * Q) {
-      int key[Q];
 #pragma unroll
       for (int q = 0; q < Q; ++q) key[q] = b + q * 32 + lane < r1 ? key_of(b + q * 32 + lane) : -1;
 #pragma unroll
@@ -154,9 +156,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(int rows, int count, int tm,
   __syncthreads();
   if (warp < sorters)
     for (int b = r0; b < r1; b += 32 * Q) {
-      int key[Q];
+      if (r1 - r0 > 32 * Q) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) key[q] = b + q * 32 + lane < r1 ? key_of(b + q * 32 + lane) : -1;
+        for (int q = 0; q < Q; ++q) key[q] = b + q * 32 + lane < r1 ? key_of(b + q * 32 + lane) : -1;
+      }
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         if (b + q * 32 >= r1) break;
@@ -333,9 +336,9 @@ struct Args {
 
 template <typename T, int TM, int RP>
 struct Shape {
-  // Bytes of a row in a chunk.  Of 64 rows 128, so that three or four CTAs share an SM, or 256 where two are all that fit anyway (rank 64) or what is done
-  // with a chunk is long (fp32 at rank 16: 93 us with 128, 76 with 256); of 16 rows 512 (64 requests 10.5 us with 256, 9.8 with 512).
-  static constexpr int CB = TM == 16 ? (RP <= 32 ? 512 : 256) : RP == 64 || (RP == 16 && sizeof(T) == 4) ? 256 : 128;
+  // Bytes of a row in a chunk.  Of 64 rows 128, so that two to four CTAs share an SM (at rank 64 43 us with 128, 51 with 256), in fp32 at rank 16, where a
+  // chunk's sums take long, 256 (67 us, and 89 with 128); of 16 rows 512 (64 requests 10.5 us with 256, 9.5 with 512).
+  static constexpr int CB = TM == 16 ? (RP <= 32 ? 512 : 256) : RP == 16 && sizeof(T) == 4 ? 256 : 128;
   static constexpr int E = 16 / sizeof(T), KC = CB / sizeof(T), pieces = CB / 16;   // values of 16 bytes, values and pieces of a chunk
   static constexpr int xs = CB + 16;                                    // bytes from row to row: ldmatrix and 16-byte reads without conflicts
   static constexpr int ls = RP * (int)sizeof(T) + 16;                   // of a factor with the rank innermost
@@ -669,40 +672,39 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, TM, RP>::ctas)) adapters_k
     char* yt = sm + (n - n0) % S::stages * S::stage;
     const char* ft = yt + TM * S::xs;
     if constexpr (F32) {
-      constexpr int RW = TM / kWarps, CL = KC / 32;   // rows of a warp, columns of a lane
-      float o[RW][CL];
+      // a warp has 16 columns of some rows, a lane four of them (BACK: every fourth, whose ranks lie on other banks) and every eighth row
+      constexpr int WC = KC / 16, RW = TM / (kWarps / WC), OR = RW / 8;
+      const int wr = warp / WC * RW + lr, wc = warp % WC * 16 + (BACK ? lc : lc * 4);
+      float o[OR][4];
 #pragma unroll
-      for (int i = 0; i < RW; ++i)
-#pragma unroll
-        for (int h = 0; h < CL; ++h) o[i][h] = Y ? reinterpret_cast<const float*>(yt + (warp * RW + i) * S::xs)[lane + 32 * h] : 0.f;
-#pragma unroll 4
+      for (int i = 0; i < OR; ++i)
+        *reinterpret_cast<float4*>(o[i]) = !BACK && Y ? *reinterpret_cast<const float4*>(yt + (wr + 8 * i) * S::xs + wc * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
       for (int j = 0; j < RP; j += 4) {
-        float v[RW][4];
+        float v[OR][4], f[4][4];   // f: [rank][column], BACK: [column][rank]
 #pragma unroll
-        for (int i = 0; i < RW; ++i) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(vs + (warp * RW + i) * S::ls + j * 4);
-        float f[CL][4];
-        if (BACK) {
+        for (int i = 0; i < OR; ++i) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(vs + (wr + 8 * i) * S::ls + j * 4);
 #pragma unroll
-          for (int h = 0; h < CL; ++h) *reinterpret_cast<float4*>(f[h]) = *reinterpret_cast<const float4*>(ft + (lane + 32 * h) * S::ls + j * 4);
-        } else {
+        for (int u = 0; u < 4; ++u)
+          *reinterpret_cast<float4*>(f[u]) = BACK ? *reinterpret_cast<const float4*>(ft + (wc + 4 * u) * S::ls + j * 4)
+                                                  : *reinterpret_cast<const float4*>(ft + (j + u) * S::xs + wc * 4);
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
+        for (int i = 0; i < OR; ++i)
 #pragma unroll
-            for (int h = 0; h < CL; ++h) f[h][u] = *reinterpret_cast<const float*>(ft + (j + u) * S::xs + (lane + 32 * h) * 4);
-        }
+          for (int h = 0; h < 4; ++h)
 #pragma unroll
-        for (int i = 0; i < RW; ++i)
-#pragma unroll
-          for (int h = 0; h < CL; ++h)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) o[i][h] = fmaf(v[i][u], f[h][u], o[i][h]);
+            for (int u = 0; u < 4; ++u) o[i][h] = fmaf(v[i][u], BACK ? f[h][u] : f[u][h], o[i][h]);
       }
 #pragma unroll
-      for (int i = 0; i < RW; ++i)
+      for (int i = 0; i < OR; ++i) {
+        float* to = reinterpret_cast<float*>(yt + (wr + 8 * i) * S::xs) + wc;
+        if (BACK) {
 #pragma unroll
-        for (int h = 0; h < CL; ++h) {
-          reinterpret_cast<float*>(yt + (warp * RW + i) * S::xs)[lane + 32 * h] = o[i][h];
+          for (int h = 0; h < 4; ++h) to[4 * h] = o[i][h];
+        } else {
+          *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(o[i]);
         }
+      }
     } else {
       constexpr int NW = KC / NG;   // columns of a warp: 32 or 16
       const int nc = (warp / S::MG) * NW;
@@ -968,27 +970,27 @@ __global__ void __launch_bounds__(kThreads) join_grads_kernel(const __grid_const
 bool rows16(const void* p, size_t row_bytes) { return !(reinterpret_cast<uintptr_t>(p) & 15) && row_bytes % 16 == 0; }
 
 template <typename T, int TM, int RP, bool BACK>
-int launch_tiles(const Args& g, int tiles, cudaStream_t st) {
+int launch_tiles(const Args& g, const Plan& p, cudaStream_t st) {
   using S = Shape<T, TM, RP>;
   const auto kern = adapters_kernel<T, TM, RP, BACK>;
   static std::atomic<int> set[64];
   B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, S::smem));
-  // CTAs of a tile: as many as the machine holds at once, with a chunk of the longer product for each
+  // CTAs of a tile: as many as the machine is likely to hold at once, with a chunk of the longer product for each
   static std::atomic<int> cache[9];
   int c = 1;
   const int chunks = std::max(ceil_div(g.K, S::KC), ceil_div(g.N, S::KC));
   for (int q = 2; q <= 8 && q <= chunks; q *= 2) {
     int n = 0;
     B200CP_CUDA_OK(resident_clusters(kern, kThreads, S::smem, q, cache, &n));
-    if (tiles <= n) c = q;
+    if (p.likely <= n) c = q;
   }
-  B200CP_CUDA_OK(launch_clusters(kern, tiles, c, kThreads, S::smem, st, g));
+  B200CP_CUDA_OK(launch_clusters(kern, p.tiles, c, kThreads, S::smem, st, g));
   B200CP_LAUNCH_OK("adapters_kernel");
   return B200CP_OK;
 }
 template <typename T, bool BACK>
 int launch_rank(const Args& g, const Plan& p, cudaStream_t st) {
-#define RANK(RP) return p.tm == 64 ? launch_tiles<T, 64, RP, BACK>(g, p.tiles, st) : launch_tiles<T, 16, RP, BACK>(g, p.tiles, st)
+#define RANK(RP) return p.tm == 64 ? launch_tiles<T, 64, RP, BACK>(g, p, st) : launch_tiles<T, 16, RP, BACK>(g, p, st)
   if (g.R <= 16) RANK(16);
   if (g.R <= 32) RANK(32);
   if (g.R <= 64) RANK(64);
