@@ -94,7 +94,7 @@ __device__ __forceinline__ float fast_sqrt_ftz(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float fast_inverse(float x) {   // (of a denominator, which is no subnormal number: its square root is not)
+__device__ __forceinline__ float fast_inverse(float x) {   // (of normal numbers)
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
@@ -230,14 +230,15 @@ __device__ __forceinline__ void update(const Entry& e, const Rates& r, float ste
     }
   }
   float mm = 0.f, mv = 0.f;
-  const bool tiny_eps = r.eps < 1e-12f;   // then the square root of a subnormal v counts beside it
+  const bool tiny_eps = r.eps < 1e-12f;   // then the square root of a subnormal v counts beside it, and their sum may be subnormal itself
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       m[j][k] = fmaf(r.c1, d[j][k], __fmul_rn(r.b1, m[j][k]));
       v[j][k] = fmaf(r.c2, __fmul_rn(d[j][k], d[j][k]), __fmul_rn(r.b2, v[j][k]));
-      x[j][k] = fmaf(-step, m[j][k] * fast_inverse(fmaf(tiny_eps ? fast_sqrt(v[j][k]) : fast_sqrt_ftz(v[j][k]), root, r.eps)), fmaf(-decay, x[j][k], x[j][k]));
+      const float by = fmaf(tiny_eps ? fast_sqrt(v[j][k]) : fast_sqrt_ftz(v[j][k]), root, r.eps);
+      x[j][k] = fmaf(-step, tiny_eps ? __fdiv_rn(m[j][k], by) : m[j][k] * fast_inverse(by), fmaf(-decay, x[j][k], x[j][k]));
       if (SMALL) {   // (values past the end are zero, and a NaN is never the larger: neither changes a maximum)
         mm = fmaxf(mm, fabsf(m[j][k]));
         mv = fmaxf(mv, v[j][k]);

@@ -115,8 +115,15 @@ struct Adapters {   // operands, checked and contiguous
   void takes(const Tensor& out, const Tensor& y) const {   // as the place of the result
     fits(out, "out");
     TORCH_CHECK_VALUE(out.is_contiguous(), "out has to be contiguous");
-    for (const Tensor* t : {&x, &A, &B}) TORCH_CHECK_VALUE(!t->is_alias_of(out), "out may share memory with Y alone");
-    TORCH_CHECK_VALUE(!y.is_alias_of(out) || (y.is_contiguous() && y.const_data_ptr() == out.const_data_ptr()),
+    const auto meets = [&](const Tensor& t) {   // (from the first to behind the last value that a tensor holds)
+      if (!t.numel() || !out.numel()) return false;
+      int64_t last = 0;
+      for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+      const auto a = reinterpret_cast<uintptr_t>(t.const_data_ptr()), b = reinterpret_cast<uintptr_t>(out.const_data_ptr());
+      return a < b + out.nbytes() && b < a + (size_t)(last + 1) * t.element_size();
+    };
+    for (const Tensor* t : {&x, &A, &B}) TORCH_CHECK_VALUE(!meets(*t), "out may share memory with Y alone");
+    TORCH_CHECK_VALUE(!meets(y) || (y.is_contiguous() && y.const_data_ptr() == out.const_data_ptr()),
                       "out may be Y, but not another part or order of its memory");
   }
   const float* scales() const { return scale.defined() ? cp(scale) : nullptr; }
@@ -384,21 +391,20 @@ PYFN(py_gated_apply) {
 }
 
 // ---- AdamW step -----------------------------------------------------------------------------------------------------------
-// A list of tensors by address: what bounds a step over many small tensors is the host, and a copy of a tensor counts its references
+// The tensors of a list by address: what bounds a step over many small tensors is the host, and a copy of a tensor counts its references.  (`hold` is a tuple of
+// its own: the list may be changed by others while the interpreter is given up.)
 struct TensorList {
   pybind11::object hold;
   std::vector<const Tensor*> t;
   TensorList() = default;
   TensorList(PyObject* o, const char* name) {
-    PyObject* seq = PySequence_Fast(o, name);
-    if (!seq) {
-      PyErr_Format(PyExc_TypeError, "%s must be a list of CUDA tensors", name);
-      throw python_error();
-    }
+    TORCH_CHECK_TYPE(PySequence_Check(o) && !THPVariable_Check(o), name, " must be a list of CUDA tensors");
+    PyObject* seq = PySequence_Tuple(o);
+    if (!seq) throw python_error();
     hold = pybind11::reinterpret_steal<pybind11::object>(seq);
-    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+    const Py_ssize_t n = PyTuple_GET_SIZE(seq);
     t.reserve((size_t)n);
-    for (Py_ssize_t i = 0; i < n; ++i) t.push_back(&any_tensor(PySequence_Fast_GET_ITEM(seq, i), name));
+    for (Py_ssize_t i = 0; i < n; ++i) t.push_back(&any_tensor(PyTuple_GET_ITEM(seq, i), name));
   }
   size_t size() const { return t.size(); }
   const Tensor& operator[](size_t i) const { return *t[i]; }

@@ -88,6 +88,16 @@ class AdamW(torch.optim.Optimizer):
                                ([s["scale_avg"] for s in ss], [s["scale_sq"] for s in ss]) if group["bits"] == 8 else None)
         return loss
 
+    def __setstate__(self, state):
+        """A copied or unpickled optimiser: the parameters of a group share its count again."""
+        super().__setstate__(state)
+        self._counts = {}
+        for at, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                s = self.state.get(p)
+                if group["capturable"] and s and torch.is_tensor(s.get("step")):
+                    s["step"] = self._counts.setdefault((at, p.device), s["step"])
+
     def load_state_dict(self, state_dict):
         """As the base class, but the state keeps its own types (codes, float32 moments of 16-bit parameters)."""
         super().load_state_dict(state_dict)

@@ -251,6 +251,35 @@ def test_a_tensor_twice_is_refused():
             P.adamw_step(ps, [c(), c()], ms, [c(), c()], 1, LR)
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-30])
+def test_an_eps_of_next_to_nothing(eps):
+    """Gradients whose squares are subnormal: the steps are still lr times their signs (v is within 2**-149 of its value: of 1e-40, 1e-5)."""
+    P = _p()
+    g = torch.tensor([1e-19, -1e-20, 1.0, -3e-3] * 64, device="cuda")
+    p, m, v = torch.zeros(256, device="cuda"), torch.zeros(256, device="cuda"), torch.zeros(256, device="cuda")
+    P.adamw_step([p], [g], [m], [v], 1, LR, betas=(B1, B2), eps=eps, weight_decay=0.0)
+    want = -LR * (g.double() / (g.double().abs() + (eps if eps > 1e-45 else 0)))
+    near(p, want, 0.05 * LR * torch.ones_like(want) * (g.double().abs() < 1e-18) + 1e-5 * LR)
+
+
+def test_a_copied_optimiser_counts_on():
+    import copy
+    import pickle
+
+    from paralleltnnlayers_b200.optim import AdamW
+    p = [torch.nn.Parameter(torch.ones(5, device="cuda")), torch.nn.Parameter(torch.ones(7, device="cuda"))]
+    opt = AdamW(p, capturable=True)
+    for q in p:
+        q.grad = torch.ones_like(q)
+    opt.step()
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        ps = other.param_groups[0]["params"]
+        for q in ps:
+            q.grad = torch.ones_like(q)
+        other.step()
+        assert [int(other.state[q]["step"]) for q in ps] == [2, 2] and int(opt.state[p[0]]["step"]) == 1
+
+
 def test_autograd_sees_the_update():
     P = _p()
     p = torch.ones(4, device="cuda", requires_grad=True)

@@ -145,6 +145,16 @@ def test_shapes_strides_and_out():
     P.dense_adapters(t["y"], x, t["A"], t["B"], t["which"], t["scale"], out=out)
     near(out, want, "off sixteen bytes")
     assert bool((buf[:3] == 7).all()) and bool((buf[3 + 48 * 40:] == 7).all())
+    # operands and output as parts of one buffer
+    one = torch.zeros(48, 72 + 40, dtype=BF16, device="cuda").view(-1)
+    xs, os_ = one[:48 * 72].view(48, 72), one[48 * 72:].view(48, 40)
+    xs.copy_(t["x"])
+    near(P.dense_adapters(t["y"], xs, t["A"], t["B"], t["which"], t["scale"], out=os_), want, "parts of one buffer")
+    for bad in (one[48 * 40:48 * 80].view(48, 40), one[:48 * 40].view(48, 40)):
+        with pytest.raises(ValueError, match="share memory"):
+            P.dense_adapters(t["y"], xs, t["A"], t["B"], t["which"], out=bad)
+    with pytest.raises(ValueError, match="out may be Y"):
+        P.dense_adapters(one[8:8 + 48 * 40].view(48, 40), t["x"], t["A"], t["B"], t["which"], out=one[:48 * 40].view(48, 40))
     none = P.dense_adapters(t["y"][:0], t["x"][:0], t["A"], t["B"], t["which"][:0])
     assert none.shape == (0, 40)
 
