@@ -102,17 +102,17 @@ __device__ __forceinline__ float fast_inverse(float x) {   // (of normal numbers
 // Codes to numbers and back by the integer bits of a float around 2^23 and 1.5 2^23 (nearest, ties to even): the conversion instructions share the pipe
 // of the roots, sixteen lanes a cycle, and were half of its work.
 constexpr float kWhole = 12582912.f;
-__device__ __forceinline__ float code_at(uint32_t four, int k) { return __uint_as_float(__byte_perm(four, 0x4b000000u, 0x7440 + k)) - 8388608.f; }
+__device__ __forceinline__ float code_at(uint32_t four, int k, float zero) { return __uint_as_float(__byte_perm(four, 0x4b000000u, 0x7440 + k)) - zero; }
 __device__ __forceinline__ void codes_of_m(uint32_t four, float (&x)[4]) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) x[k] = code_at(four ^ 0x80808080u, k) - 128.f;
+  for (int k = 0; k < 4; ++k) x[k] = code_at(four ^ 0x80808080u, k, 8388608.f + 128.f);
 }
 __device__ __forceinline__ void codes_of_v(uint32_t four, float (&x)[4]) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) x[k] = code_at(four, k);
+  for (int k = 0; k < 4; ++k) x[k] = code_at(four, k, 8388608.f);
 }
-__device__ __forceinline__ uint32_t to_codes(const float (&x)[4]) {   // of whole numbers
-  const auto bits = [](float c) { return __float_as_uint(c + kWhole); };
+__device__ __forceinline__ uint32_t to_codes(const float (&x)[4]) {   // of whole numbers with kWhole added
+  const auto bits = [](float c) { return __float_as_uint(c); };
   return __byte_perm(__byte_perm(bits(x[0]), bits(x[1]), 0x0040), __byte_perm(bits(x[2]), bits(x[3]), 0x0040), 0x5410);
 }
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, long long i, long long n, bool vec) {
@@ -136,20 +136,28 @@ __device__ __forceinline__ void store_codes(uint8_t* p, long long i, long long n
 __device__ __forceinline__ bool has_zero(uint32_t x) { return ((x - 0x01010101u) & ~x & 0x80808080u) != 0; }
 __device__ __forceinline__ void values_of_m(uint32_t four, float s, float (&x)[4]) {
   codes_of_m(four, x);
-  const bool broken = has_zero(four ^ 0x80808080u);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const float q = x[k] * (1.f / 127), v = q * fabsf(q) * s;
-    x[k] = broken && x[k] == -128.f ? __int_as_float(0x7fffffff) : v;
+    const float q = x[k] * (1.f / 127);
+    x[k] = q * fabsf(q) * s;
+  }
+  if (has_zero(four ^ 0x80808080u)) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if ((four >> (8 * k) & 255) == 128) x[k] = __int_as_float(0x7fffffff);
   }
 }
 __device__ __forceinline__ void values_of_v(uint32_t four, float s, float (&x)[4]) {
   codes_of_v(four, x);
-  const bool broken = has_zero(~four);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const float q = x[k] * (1.f / 254), r = q * q, v = r * r * s;
-    x[k] = broken && x[k] == 255.f ? __int_as_float(0x7fffffff) : v;
+    const float q = x[k] * (1.f / 254), r = q * q;
+    x[k] = r * r * s;
+  }
+  if (has_zero(~four)) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if ((four >> (8 * k) & 255) == 255) x[k] = __int_as_float(0x7fffffff);
   }
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -172,18 +180,17 @@ __device__ __forceinline__ void codes_from(const float (&m)[4], const float (&v)
   float a[4], b[4], off = 0.f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const float t = 127.f * fast_sqrt_ftz(fabsf(m[k]) * im), u = 254.f * fast_sqrt_ftz(fast_sqrt_ftz(v[k] * iv));
-    a[k] = (t + kWhole) - kWhole;
-    b[k] = (u + kWhole) - kWhole;
-    off = max_nan(max_nan(off, fabsf(t - a[k])), fabsf(u - b[k]));
-    a[k] = copysignf(a[k], m[k]);
-    b[k] = fmaxf(b[k], v[k] > 0.f ? 1.f : 0.f);
+    const float t = copysignf(127.f * fast_sqrt_ftz(fabsf(m[k]) * im), m[k]), u = 254.f * fast_sqrt_ftz(fast_sqrt_ftz(v[k] * iv));
+    a[k] = t + kWhole;
+    b[k] = u + kWhole;
+    off = max_nan(max_nan(off, fabsf(t - (a[k] - kWhole))), fabsf(u - (b[k] - kWhole)));
+    b[k] = fmaxf(b[k], v[k] > 0.f ? kWhole + 1.f : kWhole);
   }
   if (!(off <= 0.4998f) || im == 0.f || iv == 0.f) {   // (what is not finite ends here too)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      a[k] = exact_m(m[k], sm);
-      b[k] = exact_v(v[k], sv);
+      a[k] = exact_m(m[k], sm) + kWhole;
+      b[k] = exact_v(v[k], sv) + kWhole;
     }
   }
   cm = to_codes(a);
@@ -215,11 +222,17 @@ __device__ __forceinline__ void update(const Entry& e, const Rates& r, float ste
   if constexpr (SMALL) {
     const uint8_t *cm = static_cast<const uint8_t*>(e.m), *cv = static_cast<const uint8_t*>(e.v);
     const float ms = e.ms[block], vs = e.vs[block];
+    uint32_t pm[2], pv[2];   // (all loads before the first code is looked at)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const long long i = base + j * 128 + lane * 4;
-      values_of_m(load_codes(cm, i, n, WHOLE), ms, m[j]);
-      values_of_v(load_codes(cv, i, n, WHOLE), vs, v[j]);
+      pm[j] = load_codes(cm, i, n, WHOLE);
+      pv[j] = load_codes(cv, i, n, WHOLE);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      values_of_m(pm[j], ms, m[j]);
+      values_of_v(pv[j], vs, v[j]);
     }
   } else {
 #pragma unroll
@@ -230,20 +243,30 @@ __device__ __forceinline__ void update(const Entry& e, const Rates& r, float ste
     }
   }
   float mm = 0.f, mv = 0.f;
-  const bool tiny_eps = r.eps < 1e-12f;   // then the square root of a subnormal v counts beside it, and their sum may be subnormal itself
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       m[j][k] = fmaf(r.c1, d[j][k], __fmul_rn(r.b1, m[j][k]));
       v[j][k] = fmaf(r.c2, __fmul_rn(d[j][k], d[j][k]), __fmul_rn(r.b2, v[j][k]));
-      const float by = fmaf(tiny_eps ? fast_sqrt(v[j][k]) : fast_sqrt_ftz(v[j][k]), root, r.eps);
-      x[j][k] = fmaf(-step, tiny_eps ? __fdiv_rn(m[j][k], by) : m[j][k] * fast_inverse(by), fmaf(-decay, x[j][k], x[j][k]));
       if (SMALL) {   // (values past the end are zero, and a NaN is never the larger: neither changes a maximum)
         mm = fmaxf(mm, fabsf(m[j][k]));
         mv = fmaxf(mv, v[j][k]);
       }
     }
+  if (r.eps >= 1e-12f) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        x[j][k] = fmaf(-step, m[j][k] * fast_inverse(fmaf(fast_sqrt_ftz(v[j][k]), root, r.eps)), fmaf(-decay, x[j][k], x[j][k]));
+  } else {   // the square root of a subnormal v counts beside such an eps, and their sum may be subnormal itself
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        x[j][k] = fmaf(-step, __fdiv_rn(m[j][k], fmaf(fast_sqrt(v[j][k]), root, r.eps)), fmaf(-decay, x[j][k], x[j][k]));
+  }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const long long i = base + j * 128 + lane * 4;
@@ -289,9 +312,9 @@ __device__ __forceinline__ void update(const Entry& e, const Rates& r, float ste
   }
 }
 
-// (Five CTAs on an SM: 59 M values with 8-bit moments 180 us with four, 166, 170 with six; 42 M in bfloat16 with copies 167, 167, 176.)
+// (CTAs of an SM, 59 M values with 8-bit moments: 188 us with four, 172 with five, 165 with six; 42 M in bfloat16 with copies 169, 169, 171.)
 template <typename P, typename G, bool SMALL, int CAP>
-__global__ void __launch_bounds__(kThreads, 5) adamw_kernel(const __grid_constant__ Table<CAP> t) {
+__global__ void __launch_bounds__(kThreads, SMALL ? 6 : 5) adamw_kernel(const __grid_constant__ Table<CAP> t) {
   int a = 0, b = t.count;   // the tensor whose pieces hold this CTA's
   while (b - a > 1) {
     const int c = (a + b) / 2;
