@@ -26,7 +26,7 @@ namespace b200cp {
 namespace {
 
 constexpr int kThreads = 256, kPiece = 2048, kBlock = 256;   // a warp has 256 values: two groups of four per lane
-constexpr int kFew = 48, kMany = 448;                        // tensors of a launch: tables of 3.5 and 31 KB (32 764 bytes are the most)
+constexpr int kFew = 48, kSome = 128, kMany = 448;           // tensors of a launch: tables of 3.5, 9 and 31 KB (32 764 bytes are the most)
 
 struct Entry {
   void* p;
@@ -411,7 +411,8 @@ int launch_some(const b200cp_adamw_tensor* ts, int count, const Rates& r, cudaSt
 }
 template <typename P, typename G, bool SMALL>
 int launch_all(const b200cp_adamw_tensor* ts, int count, const Rates& r, cudaStream_t st) {
-  return count <= kFew ? launch_some<P, G, SMALL, kFew>(ts, count, r, st) : launch_some<P, G, SMALL, kMany>(ts, count, r, st);
+  if (count <= kFew) return launch_some<P, G, SMALL, kFew>(ts, count, r, st);
+  return count <= kSome ? launch_some<P, G, SMALL, kSome>(ts, count, r, st) : launch_some<P, G, SMALL, kMany>(ts, count, r, st);
 }
 template <typename P, typename G>
 int launch_bits(const b200cp_adamw_tensor* ts, int count, int bits, const Rates& r, cudaStream_t st) {
