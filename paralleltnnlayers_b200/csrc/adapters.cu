@@ -229,8 +229,8 @@ __device__ __forceinline__ void load_rows(char* dst, int stride, Row row, int c0
   }
 }
 
-// The same for rows that start on 16-byte boundaries, chunk after chunk of PIECES x 16 bytes (or, STEP given, of STEP bytes in memory): where a thread's pieces
-// come from is worked out once, so that a chunk takes a few instructions of it (worked out anew for each: 4096 rows 36 us).
+// The same for rows that start on 16-byte boundaries, chunk after chunk: where a thread's pieces come from is worked out once, so that a chunk takes a few
+// instructions of it (worked out anew for each chunk: 4096 rows 36 us, and 32).
 template <typename T, int ROWS, int PIECES>
 struct Rows {
   static constexpr int E = 16 / sizeof(T), EACH = kThreads / PIECES, N = (ROWS + EACH - 1) / EACH;
@@ -446,11 +446,10 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, TM, RP>::ctas)) adapters_k
     else
       load_rows<T, KC, RP / E>(dst, S::ls, [&](int r) { return c0 + r < n ? F + (size_t)(c0 + r) * R : nullptr; }, 0, R, false, F);
   };
-  // LONG: rows of n features, a row per rank; else rows of R ranks, of which a chunk has KC and the last one fewer
   Rows<T, BACK ? RP : KC, BACK ? S::pieces : RP / E> f1;
   const int rank_bytes = min(16, max(0, (R - (int)(tid % (RP / E)) * E) * (int)sizeof(T)));
   f1.set([&](int r) { return BACK ? (r < R ? F1 + (size_t)r * K : nullptr) : F1 + (size_t)r * R; }, F1);
-  // (a chunk's rows past the last feature: a thread has one, since a chunk's KC rows are at most as many as its threads' places)
+  // a chunk of a factor whose rows are features: KC rows of R ranks, in the last chunk fewer
   const auto load_ranks = [&](const auto& f, char* dst, int c0, int n) {
     constexpr int EACH = kThreads / (RP / E);
     dst += tid / (RP / E) * S::ls + tid % (RP / E) * 16;

@@ -30,11 +30,18 @@ namespace {
 using namespace tc;
 
 enum Form { kForward, kData, kWeights };
-constexpr int kTile = 256, kStep = 64, kHalf = 128 * kStep * 2, kStage = 2 * kHalf, kStages = 6;   // bytes: of an operand's half, of a step
+constexpr int kTile = 256, kStep = 64, kHalf = 128 * kStep * 2, kStage = 2 * kHalf;   // bytes: of an operand's half, of a step
 constexpr int kBox = 64 * kStep * 2;              // a box of 64 columns by 64 k
 constexpr int kReaders = 8, kThreads = 64 + 32 * kReaders;
 constexpr int kPitch = 80, kPatch = 32 * kPitch;   // bytes of a row and of a warp's 32 x 32 block on its way out
-constexpr size_t kSmem = (size_t)kStages * kStage + kReaders * kPatch + 1024 + 256;
+constexpr int kKept = 32 * 32 * 4;                               // bytes of a warp's 32 x 32 block of G or U
+// The forward of a training step: five steps in flight and two blocks per read-out warp, else six and a patch.
+template <bool KEEP>
+struct Ring {
+  static constexpr int stages = KEEP ? 5 : 6, out = KEEP ? 2 * kKept : kPatch;
+  static constexpr size_t smem = (size_t)stages * kStage + kReaders * out + 1024 + 256;
+  static_assert(smem <= 227 * 1024 && out >= kPatch, "");
+};
 
 struct Gemm {
   int M, N;                      // of a result
@@ -118,23 +125,20 @@ __device__ __forceinline__ void put_block(uint8_t* patch, T* out, int vec, int m
   }
   __syncwarp();
 }
-// The warp's 32 kept rows of 32 floats, 16 columns at a time by the same way: 64 bytes of eight rows per store.  (Columns past the end are those of the rows'
-// padding, or of nothing.)
-__device__ __forceinline__ void keep_block(uint8_t* patch, float* out, int m0, int M, int n, int ld, const float (&v)[32]) {
-  const int lane = threadIdx.x & 31, q = lane & 3;
+// The warp's 32 kept rows of 32 floats as the box of a tensor store (128-byte rows, swizzled: neighbouring lanes on other banks).  G and U are 8 of the 10 bytes
+// that a value of the forward writes; stored by the lanes themselves, 16 bytes of a row each or 64 bytes of eight rows through shared memory, they were
+// what a tile of few inputs waited for (8192 x 1024 -> 2816: 132 us).
+__device__ __forceinline__ void keep_block(uint8_t* block, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int h = 0; h < 32; h += 16) {
-    float4* mine = reinterpret_cast<float4*>(patch + lane * kPitch);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) mine[j] = make_float4(v[h + 4 * j], v[h + 4 * j + 1], v[h + 4 * j + 2], v[h + 4 * j + 3]);
-    __syncwarp();
-    if (n + h + 4 * q < ld)
-#pragma unroll
-      for (int r = lane >> 2; r < 32; r += 8)
-        if (m0 + r < M) *reinterpret_cast<float4*>(out + (size_t)(m0 + r) * ld + n + h + 4 * q) = *reinterpret_cast<const float4*>(patch + r * kPitch + q * 16);
-    __syncwarp();
-  }
+  for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(block + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
 }
+// A box from shared memory; what lies outside the tensor is not written.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void stores_end_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void stores_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 // 32 columns of the warp's lane quarter
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
@@ -164,14 +168,16 @@ __device__ __forceinline__ UnitAt unit_at(const Gemm& g, int unit) {
   return UnitAt{(m1 + q % height) * kTile, (q / height) * (FORM == kForward ? kTile / 2 : kTile), r};
 }
 
-template <Form FORM, typename T>
+// KEEP (forward): G and U are kept, through mapA1 and mapK.
+template <Form FORM, bool KEEP, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapA1,
-             const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1) {
+             const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1, const __grid_constant__ CUtensorMap mapK) {
+  constexpr int kStages = Ring<KEEP>::stages, kOut = Ring<KEEP>::out;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* patches = sm + kStages * kStage;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(patches + kReaders * kPatch);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(patches + kReaders * kOut);
   uint64_t* full = bars;                 // [kStages] the leader's: the step of both CTAs has landed  (tx bytes)
   uint64_t* empty = full + kStages;      // [kStages] the products that read the step are done         (commit, both CTAs)
   uint64_t* accfull = empty + kStages;   // [2] the sums of a tile are complete                        (commit, both CTAs)
@@ -194,6 +200,10 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
     tma_prefetch_desc(&mapA0);
     tma_prefetch_desc(&mapB0);
     if (FORM != kWeights) tma_prefetch_desc(FORM == kData ? &mapA1 : &mapB1);
+    if (KEEP) {
+      tma_prefetch_desc(&mapA1);
+      tma_prefetch_desc(&mapK);
+    }
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before_sync();
@@ -277,7 +287,7 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + ((uint32_t)(qd * 32) << 16) + buf * 256;
       const int m0 = t.m0 + rank * 128 + qd * 32;
-      uint8_t* patch = patches + (warp - 2) * kPatch;
+      uint8_t* patch = patches + (warp - 2) * kOut;
       T* out = static_cast<T*>(g.out[FORM == kWeights ? t.result : 0]);
       constexpr int cols = FORM == kForward ? 64 : 128;
       if (m0 < g.M)
@@ -288,12 +298,26 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
           if constexpr (FORM == kForward) {
             float u[32];
             tmem_ld32(taddr + 128 + j, u);
-            if (g.G) {
-              keep_block(patch, g.G, m0, g.M, t.n0 + j, g.ldg, a);
-              keep_block(patch, g.U, m0, g.M, t.n0 + j, g.ldg, u);
+            if constexpr (KEEP) {
+              // (nobody reads the blocks any more, nor is the patch in them in use)
+              if (lane == 0) stores_wait_read();
+              __syncwarp();
+              keep_block(patch, a);
+              keep_block(patch + kKept, u);
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&mapA1, patch, t.n0 + j, m0);
+                tma_store_2d(&mapK, patch + kKept, t.n0 + j, m0);
+                stores_end_group();
+              }
             }
 #pragma unroll
             for (int i = 0; i < 32; ++i) a[i] = a[i] * gate_share<false>(g.act, a[i], nullptr) * u[i];
+          }
+          if (KEEP && g.vec != 8) {   // the patch lies in a block that is on its way out
+            if (lane == 0) stores_wait_read();
+            __syncwarp();
           }
           put_block(patch, out, g.vec, m0, g.M, t.n0 + j, g.N, a);
         }
@@ -301,6 +325,7 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
       __syncwarp();
       if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
     }
+    if (KEEP && lane == 0) stores_wait_read();
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -603,14 +628,31 @@ int pad(Matrix** ms, int count, char*& ws, cudaStream_t st) {
 size_t pad_bytes(int rows, int I, int F) { return (odd(I) ? plane(rows, I) : 0) + (odd(F) ? 2 * plane(I, F) : 0); }
 bool rows16(const void* p, size_t row_bytes) { return !(reinterpret_cast<uintptr_t>(p) & 15) && row_bytes % 16 == 0; }
 
-template <Form FORM, typename T>
+// rows of floats for boxes of 32 x 32
+int encode_kept(CUtensorMap* map, const float* p, int rows, int ld) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  const cuuint64_t dim[2] = {(cuuint64_t)ld, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)ld * 4};
+  const cuuint32_t box[2] = {32, 32}, estr[2] = {1, 1};
+  const CUresult cr = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(p), dim, stride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (cr != CUDA_SUCCESS) return fail(B200CP_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)cr);
+  return B200CP_OK;
+}
+template <Form FORM, bool KEEP, typename T>
 int launch(Gemm g, int results, const Matrix& a0, const Matrix& a1, const Matrix& b0, const Matrix& b1, cudaStream_t st) {
   DeviceInfo di;
   if (int rc = device_info(&di)) return rc;
-  CUtensorMap ma0, ma1, mb0, mb1;
+  CUtensorMap ma0, ma1, mb0, mb1, mk;
   constexpr unsigned ra = FORM == kWeights ? kStep : 128, rb = FORM == kData ? 128 : kStep;
   if (int rc = encode<T>(&ma0, a0, ra)) return rc;
-  if (int rc = encode<T>(&ma1, a1, ra)) return rc;
+  g.ldg = ld8(g.N);
+  if constexpr (KEEP) {
+    if (int rc = encode_kept(&ma1, g.G, g.M, g.ldg)) return rc;
+    if (int rc = encode_kept(&mk, g.U, g.M, g.ldg)) return rc;
+  } else {
+    if (int rc = encode<T>(&ma1, a1, ra)) return rc;
+    mk = ma1;
+  }
   if (int rc = encode<T>(&mb0, b0, rb)) return rc;
   if (int rc = encode<T>(&mb1, b1, rb)) return rc;
   g.tiles_m = ceil_div(g.M, kTile);
@@ -620,12 +662,12 @@ int launch(Gemm g, int results, const Matrix& a0, const Matrix& a1, const Matrix
   g.units = (int)units;
   const uintptr_t at = reinterpret_cast<uintptr_t>(g.out[0]) | reinterpret_cast<uintptr_t>(g.out[results - 1]) | (uintptr_t)g.N * 2;
   g.vec = at % 16 == 0 ? 8 : at % 4 == 0 ? 2 : 1;
-  g.ldg = ld8(g.N);
-  const auto kern = gated_kernel<FORM, T>;
+  constexpr size_t kSmem = Ring<KEEP>::smem;
+  const auto kern = gated_kernel<FORM, KEEP, T>;
   static std::atomic<int> set[64];
   B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, (int)kSmem));
   const int pairs = std::min(g.units, di.sm_count / 2);
-  B200CP_CUDA_OK(launch_kernel(kern, dim3(2 * pairs), dim3(kThreads), kSmem, st, true, g, ma0, ma1, mb0, mb1));
+  B200CP_CUDA_OK(launch_kernel(kern, dim3(2 * pairs), dim3(kThreads), kSmem, st, true, g, ma0, ma1, mb0, mb1, mk));
   B200CP_LAUNCH_OK("gated_kernel");
   return B200CP_OK;
 }
@@ -689,7 +731,7 @@ int forward(int rows, int I, int F, int act, const void* X, const void* Wg, cons
   Gemm p{};
   p.M = rows; p.N = F; p.steps = p.first = ceil_div(I, kStep); p.act = act;
   p.out[0] = p.out[1] = H; p.G = G; p.U = U;
-  return launch<kForward, T>(p, 1, x, x, g, u, st);
+  return G ? launch<kForward, true, T>(p, 1, x, x, g, u, st) : launch<kForward, false, T>(p, 1, x, x, g, u, st);
 }
 
 template <typename T>
@@ -716,12 +758,12 @@ int backward(int rows, int I, int F, int act, const void* X, const void* Wg, con
   if (dX) {
     p.M = rows; p.N = I; p.first = ceil_div(F, kStep); p.steps = 2 * p.first;
     p.out[0] = p.out[1] = dX;
-    if (int rc = launch<kData, T>(p, 1, a, b, g, u, st)) return rc;
+    if (int rc = launch<kData, false, T>(p, 1, a, b, g, u, st)) return rc;
   }
   if (dWg) {
     p.M = I; p.N = F; p.steps = p.first = ceil_div(rows, kStep);
     p.out[0] = dWg; p.out[1] = dWu;
-    if (int rc = launch<kWeights, T>(p, 2, x, x, a, b, st)) return rc;
+    if (int rc = launch<kWeights, false, T>(p, 2, x, x, a, b, st)) return rc;
   }
   return B200CP_OK;
 }
