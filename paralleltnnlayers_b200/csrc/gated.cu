@@ -34,13 +34,13 @@ constexpr int kTile = 256, kStep = 64, kHalf = 128 * kStep * 2, kStage = 2 * kHa
 constexpr int kBox = 64 * kStep * 2;              // a box of 64 columns by 64 k
 constexpr int kReaders = 8, kThreads = 64 + 32 * kReaders;
 constexpr int kPitch = 80, kPatch = 32 * kPitch;   // bytes of a row and of a warp's 32 x 32 block on its way out
-constexpr int kKept = 32 * 32 * 4;                               // bytes of a warp's 32 x 32 block of G or U
-// The forward of a training step: five steps in flight and two blocks per read-out warp, else six and a patch.
+constexpr int kKept = 32 * 32 * 4;                 // bytes of a warp's 32 x 32 block of G or U
+constexpr int kStages = 6;                         // 192 KB in flight
 template <bool KEEP>
 struct Ring {
-  static constexpr int stages = KEEP ? 5 : 6, out = KEEP ? 2 * kKept : kPatch;
-  static constexpr size_t smem = (size_t)stages * kStage + kReaders * out + 1024 + 256;
-  static_assert(smem <= 227 * 1024 && out >= kPatch, "");
+  static constexpr int out = KEEP ? kKept : kPatch;   // a read-out warp's block
+  static constexpr size_t smem = (size_t)kStages * kStage + kReaders * out + 1024 + 256;
+  static_assert(smem <= 227 * 1024 && out >= kPatch && kPatch % 16 == 0 && (kStages * kStage) % 1024 == 0 && kKept % 1024 == 0, "");
 };
 
 struct Gemm {
@@ -125,9 +125,10 @@ __device__ __forceinline__ void put_block(uint8_t* patch, T* out, int vec, int m
   }
   __syncwarp();
 }
-// The warp's 32 kept rows of 32 floats as the box of a tensor store (128-byte rows, swizzled: neighbouring lanes on other banks).  G and U are 8 of the 10 bytes
-// that a value of the forward writes; stored by the lanes themselves, 16 bytes of a row each or 64 bytes of eight rows through shared memory, they were
-// what a tile of few inputs waited for (8192 x 1024 -> 2816: 132 us).
+// The warp's 32 kept rows of 32 floats as the box of a tensor store (128-byte rows, swizzled: neighbouring lanes on other banks).  G and U are 8
+// of the 10 bytes that a value of the forward writes, and what a tile of few inputs waits for: 8192 x 1024 -> 2816 takes 132 us, 2048 x 2048 ->
+// 5120 95, and 167 and 110 where the lanes store them, 64 bytes of a row at a time through the patch.  One block for both, not two: two leave room
+// for five steps of the ring, which saves nothing there (125 and 100 us).
 __device__ __forceinline__ void keep_block(uint8_t* block, const float (&v)[32]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -173,7 +174,7 @@ template <Form FORM, bool KEEP, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapA1,
              const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1, const __grid_constant__ CUtensorMap mapK) {
-  constexpr int kStages = Ring<KEEP>::stages, kOut = Ring<KEEP>::out;
+  constexpr int kOut = Ring<KEEP>::out;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* patches = sm + kStages * kStage;
@@ -303,12 +304,19 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
               if (lane == 0) stores_wait_read();
               __syncwarp();
               keep_block(patch, a);
-              keep_block(patch + kKept, u);
               fence_proxy_async();
               __syncwarp();
               if (lane == 0) {
                 tma_store_2d(&mapA1, patch, t.n0 + j, m0);
-                tma_store_2d(&mapK, patch + kKept, t.n0 + j, m0);
+                stores_end_group();
+                stores_wait_read();
+              }
+              __syncwarp();
+              keep_block(patch, u);
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&mapK, patch, t.n0 + j, m0);
                 stores_end_group();
               }
             }
