@@ -333,7 +333,7 @@ gated_kernel(const __grid_constant__ Gemm g, const __grid_constant__ CUtensorMap
       __syncwarp();
       if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
     }
-    if (KEEP && lane == 0) stores_wait_read();
+    if (KEEP && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // (written, not only read)
   }
   tc_fence_before_sync();
   __syncthreads();
