@@ -407,7 +407,8 @@ int b200cp_adamw_moments(unsigned long long n, const void* exp_avg, const void* 
 
 /* Rows in the order of their adapters, made once for a batch and used by every layer that the batch meets.  adapters[rows] (device):
  * the adapter of each row, 0 .. count - 1; any other number: none.  plan: b200cp_adapter_plan_bytes() of device memory, 16-byte
- * aligned; it depends on rows, count and adapters only.  count is at most 16384. */
+ * aligned; it depends on rows, count and adapters only.  count is at most 16384.  A call that is given the plan of other rows or of another
+ * count computes nothing; b200cp_device_status() reports it (B200CP_ERR_INVALID_ARG). */
 size_t b200cp_adapter_plan_bytes(int rows, int count);
 int b200cp_adapter_plan(int rows, int count, const int* adapters, void* plan, size_t plan_bytes, void* stream);
 

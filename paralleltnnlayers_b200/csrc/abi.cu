@@ -1292,6 +1292,8 @@ int b200cp_device_status(void) {
   if (v) return fail(B200CP_ERR_TIMEOUT, "factor contraction: a bounded wait ran out in block %d", v & 0xffff);
   if (int rc = gated_device_status(&v)) return rc;
   if (v) return fail(B200CP_ERR_TIMEOUT, "gated feed-forward block: a bounded wait ran out in block %d", v & 0xffff);
+  if (int rc = adapters_device_status(&v)) return rc;
+  if (v) return fail(B200CP_ERR_INVALID_ARG, "low-rank adapters: a plan of other rows or of another number of adapters (nothing was computed)");
   return B200CP_OK;
 }
 

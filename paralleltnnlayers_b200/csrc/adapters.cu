@@ -27,14 +27,18 @@
 #include "common.cuh"
 
 namespace b200cp {
+
+__device__ int g_adapters_status = 0;   // 1: a plan of other rows or another number of adapters
+
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8, kMostRank = 128, kMostAdapters = 16384;
 static_assert(B200CP_ADAPTERS_WITHOUT_PLAN <= kThreads, "a thread has a row");
 
 // ---- plan -------------------------------------------------------------------------------------------------------------------
-// ints: [0] tiles, [1] rows with an adapter, [2..3] free | start[count + 2] | tile_adapter[tiles] | tile_first[tiles] | order[rows].
-// Rows without an adapter are those of "adapter" count, behind the others.
+// ints: [0] tiles, [1] rows with an adapter, [2] rows, [3] count | start[count + 2] | tile_adapter[tiles] | tile_first[tiles] | order[rows].
+// Rows without an adapter are those of "adapter" count, behind the others.  Where the arrays lie depends on rows and count: a kernel that is
+// handed the plan of others leaves it alone, records that and returns (plans of neighbouring counts often have the same size).
 struct Plan {
   int tm, tiles, likely;   // rows of a tile; the most tiles there can be; as many as adapters whose last tile is half full give
   size_t start, adapter, first, order, ints;
@@ -142,6 +146,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(int rows, int count, int tm,
     start[keys] = rows;
     plan[0] = tiles;
     plan[1] = counts[count * sorters];
+    plan[2] = rows;
+    plan[3] = count;
   }
   __syncthreads();
   for (int t = tid; t < tiles; t += 1024) {
@@ -174,6 +180,13 @@ __global__ void __launch_bounds__(1024) plan_kernel(int rows, int count, int tm,
         __syncwarp();
       }
     }
+}
+
+// Whether a plan is one of these rows and adapters: the same answer for all threads of a launch, which reads nothing else of a plan that is not.
+__device__ __forceinline__ bool plan_is_of(const int4& head, int rows, int count) {
+  if (head.z == rows && head.w == count) return true;
+  if (threadIdx.x == 0) atomicCAS(&g_adapters_status, 0, 1);
+  return false;
 }
 
 // ---- loads ------------------------------------------------------------------------------------------------------------------
@@ -408,7 +421,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, TM, RP>::ctas)) adapters_k
     if (in) rowat[place] = tid;
     len = __syncthreads_count(in);
   } else {
-    if (tile >= g.head[0]) return;   // (all CTAs of the cluster)
+    const int4 head = *reinterpret_cast<const int4*>(g.head);
+    if (!plan_is_of(head, g.rows, g.count) || tile >= head.x) return;   // (all CTAs of the cluster)
     a = g.tile_adapter[tile];
     const int first = g.tile_first[tile];
     len = min(TM, g.start[a + 1] - first);
@@ -801,6 +815,7 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
   constexpr bool F32 = sizeof(T) == 4;
   extern __shared__ __align__(16) char sm[];
   grid_dependency_wait();
+  if (!plan_is_of(*reinterpret_cast<const int4*>(g.head), g.rows, g.count)) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool second = (int)blockIdx.x >= g.tiles_i;   // dB
   const int L = second ? g.O : g.I, l0 = ((int)blockIdx.x - (second ? g.tiles_i : 0)) * LT, R = g.R;
@@ -924,6 +939,7 @@ __global__ void __launch_bounds__(kThreads) adapter_grads_kernel(const __grid_co
 template <typename T, int RP>
 __global__ void __launch_bounds__(kThreads) join_grads_kernel(const __grid_constant__ GradArgs g) {
   grid_dependency_wait();
+  if (!plan_is_of(*reinterpret_cast<const int4*>(g.head), g.rows, g.count)) return;
   const int a = blockIdx.x, ab = g.start[a], ae = g.start[a + 1], per = range_rows(g);
   const int r0 = ab / per, r1 = ae > ab ? (ae - 1) / per : r0;
   if (ae > ab && r0 == r1) return;
@@ -1072,6 +1088,15 @@ int run_tiles(int type, Args& g, const Plan& p, const int* plan, cudaStream_t st
 size_t w_bytes(int rows, int R, int type) { return align_up((size_t)rows * R * (type == B200CP_FLOAT32 ? 4 : 2), 256); }
 
 }  // namespace
+
+int adapters_device_status(int* out) {
+  int v = 0, zero = 0;
+  B200CP_CUDA_OK(cudaMemcpyFromSymbol(&v, g_adapters_status, sizeof(int)));
+  if (v) B200CP_CUDA_OK(cudaMemcpyToSymbol(g_adapters_status, &zero, sizeof(int)));
+  *out = v;
+  return B200CP_OK;
+}
+
 }  // namespace b200cp
 
 using namespace b200cp;
@@ -1106,6 +1131,7 @@ int b200cp_dense_adapters(int rows, int I, int O, int R, int count, int type, co
   if (int rc = check_sizes("b200cp_dense_adapters", rows, I, O, R, count, type)) return rc;
   if (rows == 0) return B200CP_OK;
   if (!Y || !X || !A || !B || (!plan && !adapters) || !out) return fail(B200CP_ERR_INVALID_ARG, "b200cp_dense_adapters: null pointer");
+  if (reinterpret_cast<uintptr_t>(plan) & 15) return fail(B200CP_ERR_INVALID_ARG, "b200cp_dense_adapters: the plan is not on a 16-byte boundary");
   if (!plan && rows > B200CP_ADAPTERS_WITHOUT_PLAN)
     return fail(B200CP_ERR_UNSUPPORTED, "b200cp_dense_adapters: %d rows without a plan (at most %d)", rows, B200CP_ADAPTERS_WITHOUT_PLAN);
   Args g{};
@@ -1126,6 +1152,7 @@ int b200cp_dense_adapters_bwd(int rows, int I, int O, int R, int count, int type
   const char* who = "b200cp_dense_adapters_bwd";
   if (int rc = check_sizes(who, rows, I, O, R, count, type)) return rc;
   if (!plan || (rows && (!dY || ((dX || dA) && (!A || !B)) || (dA && !X) || (dB && !V)))) return fail(B200CP_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (reinterpret_cast<uintptr_t>(plan) & 15) return fail(B200CP_ERR_INVALID_ARG, "%s: the plan is not on a 16-byte boundary", who);
   const size_t need = b200cp_dense_adapters_bwd_workspace_bytes(rows, I, O, R, count, type);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return fail(B200CP_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, %zu given", who, need, workspace_bytes);

@@ -88,19 +88,19 @@ struct Adapters {   // operands, checked and contiguous
     TORCH_CHECK_VALUE(y.dim() == x.dim() && y.size(-1) == O && y.sizes().slice(0, y.dim() - 1) == x.sizes().slice(0, x.dim() - 1), name, " is ",
                       y.sizes(), " where X is ", x.sizes(), " and B has ", O, " columns");
   }
-  // `which`: the adapter of every row, or (planned) the bytes of a plan
-  Tensor plan(const Tensor& which, bool planned) const {
+  // `which`: the adapter of every row, or the bytes of a plan for `planned` adapters (0: no plan)
+  Tensor plan(const Tensor& which, int64_t planned) const {
     check_numbers(which, planned);
     return planned ? which : adapter_plan(which, count);
   }
   // the numbers themselves where a batch is small enough to go without a plan, or else a plan (*planned)
-  Tensor numbers(const Tensor& which, bool* planned) const {
+  Tensor numbers(const Tensor& which, int64_t* planned) const {
     check_numbers(which, *planned);
     if (*planned) return which;
-    *planned = rows > B200CP_ADAPTERS_WITHOUT_PLAN;
+    if (rows > B200CP_ADAPTERS_WITHOUT_PLAN) *planned = count;
     return *planned ? adapter_plan(which, count) : adapter_numbers(which, count);
   }
-  void check_numbers(const Tensor& which, bool planned) const {
+  void check_numbers(const Tensor& which, int64_t planned) const {
     TORCH_CHECK_VALUE(which.device() == x.device(), "the adapters' numbers are on ", which.device(), ", X on ", x.device());
     if (!planned) {
       TORCH_CHECK_TYPE(which.scalar_type() == at::kInt || which.scalar_type() == at::kLong, "adapters must be an int32 or int64 CUDA tensor");
@@ -108,6 +108,8 @@ struct Adapters {   // operands, checked and contiguous
       TORCH_CHECK_VALUE(b200cp_adapter_plan_bytes(rows, count), rows, " rows and ", count, " adapters (1 to 16384 of them)");
       return;
     }
+    // (the sizes of two plans may be the same where their counts are not)
+    TORCH_CHECK_VALUE(planned == count, "the plan is one of ", planned, " adapters, A and B are of ", count);
     TORCH_CHECK_VALUE(which.scalar_type() == at::kByte && which.is_contiguous() &&
                           (size_t)which.numel() == std::max<size_t>(16, b200cp_adapter_plan_bytes(rows, count)),
                       "the plan is not one of ", rows, " rows and ", count, " adapters");
@@ -290,13 +292,13 @@ PYFN(py_adapter_plan) {
   return wrap(unlocked([&] { return adapter_plan(which, count); }));
   END_HANDLE_TH_ERRORS
 }
-// (Y, X, A, B, which, planned, scale or None, out or None)
+// (Y, X, A, B, which, the count of the plan or 0, scale or None, out or None)
 PYFN(py_dense_adapters) {
   HANDLE_TH_ERRORS
   count_args(n, 8);
   const Tensor &y = any_tensor(a[0], "Y"), &x = any_tensor(a[1], "X"), &A = any_tensor(a[2], "A"), &B = any_tensor(a[3], "B"),
                &which = any_tensor(a[4], "adapters");
-  bool planned = truth(a[5]);
+  int64_t planned = int_arg(a[5]);
   const Tensor scale = optional_tensor(a[6], "scale"), to = optional_tensor(a[7], "out");
   Tensor out = unlocked([&] {
     const Adapters op(x, A, B, scale);
@@ -309,29 +311,30 @@ PYFN(py_dense_adapters) {
   return wrap(out);
   END_HANDLE_TH_ERRORS
 }
-// (dY, X, V, A, B, plan, scale or None, need_dx, need_da, need_db)
+// (dY, X, V, A, B, plan, its count, scale or None, need_dx, need_da, need_db)
 PYFN(py_dense_adapters_backward) {
   HANDLE_TH_ERRORS
-  count_args(n, 10);
+  count_args(n, 11);
   const Tensor &dy = any_tensor(a[0], "dY"), &x = any_tensor(a[1], "X"), &V_ = any_tensor(a[2], "V"), &A = any_tensor(a[3], "A"),
                &B = any_tensor(a[4], "B"), &plan = any_tensor(a[5], "plan");
-  const Tensor scale = optional_tensor(a[6], "scale");
-  const bool nx = truth(a[7]), na = truth(a[8]), nb = truth(a[9]);
+  const int64_t planned = int_arg(a[6]);
+  const Tensor scale = optional_tensor(a[7], "scale");
+  const bool nx = truth(a[8]), na = truth(a[9]), nb = truth(a[10]);
   return wrap_tuple(unlocked([&] {
     const Adapters op(x, A, B, scale);
     Adapters::same(V_, x, "V");
     TORCH_CHECK_VALUE(V_.numel() == (int64_t)op.rows * op.R, "V has ", V_.numel(), " values, ", op.rows, " rows of rank ", op.R, " are needed");
-    return dense_adapters_backward(op, dy, contiguous(V_), op.plan(plan, true), nx, na, nb);
+    return dense_adapters_backward(op, dy, contiguous(V_), op.plan(plan, planned), nx, na, nb);
   }));
   END_HANDLE_TH_ERRORS
 }
-// (y, x, A, B, which, planned, scale or None)
+// (y, x, A, B, which, the count of the plan or 0, scale or None)
 PYFN(py_adapters_apply) {
   HANDLE_TH_ERRORS
   count_args(n, 7);
   const Tensor &y = any_tensor(a[0], "Y"), &x = any_tensor(a[1], "X"), &A = any_tensor(a[2], "A"), &B = any_tensor(a[3], "B"),
                &which = any_tensor(a[4], "adapters");
-  const bool planned = truth(a[5]);
+  const int64_t planned = int_arg(a[5]);
   const Tensor scale = optional_tensor(a[6], "scale");
   return wrap(unlocked([&] {
     Tensor plan;

@@ -410,12 +410,12 @@ def adapter_plan(adapters, count):
 
 
 def _which(adapters, X):
-    """The operand for the binding, and whether it is a plan."""
+    """The operand for the binding, and the number of adapters of a plan (0: it is none)."""
     if not isinstance(adapters, AdapterPlan):
-        return adapters, False
+        return adapters, 0
     if adapters.shape != tuple(X.shape[:-1]):
         raise ValueError(f"the plan is of rows {adapters.shape}, the input of {tuple(X.shape[:-1])}")
-    return adapters.data, True
+    return adapters.data, adapters.count
 
 
 def dense_adapters(Y, X, A, B, adapters, scale=None, out=None):
@@ -435,7 +435,7 @@ def dense_adapters_backward(dY, X, V, A, B, plan, scale=None, need_dx=True, need
     which, planned = _which(plan, X)
     if not planned:
         raise TypeError("dense_adapters_backward takes the AdapterPlan of the forward")
-    return _C.dense_adapters_backward(dY, X, V, A, B, which, scale, need_dx, need_da, need_db)
+    return _C.dense_adapters_backward(dY, X, V, A, B, which, planned, scale, need_dx, need_da, need_db)
 
 
 # ---- gated feed-forward block -----------------------------------------------------
