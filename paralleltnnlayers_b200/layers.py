@@ -222,8 +222,10 @@ class AdaptedDense(nn.Module):
         self.register_buffer("scale", torch.full((count,), float(scale), dtype=torch.float32))
 
     def _apply(self, fn, recurse=True):
+        scale = self.scale
         super()._apply(fn, recurse)
-        self.scale = self.scale.float()   # a type given to the module is that of the adapters; the scales stay float32
+        if self.scale.dtype != torch.float32:   # a type given to the module is that of the adapters; the scales stay as they are, in float32
+            self.scale = scale.to(self.scale.device)
         return self
 
     def forward(self, x, adapters):
