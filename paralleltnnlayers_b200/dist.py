@@ -172,20 +172,30 @@ class P2PAllreduce:
 
 def _update(optimizer, params, grads):
     """The summed gradients handed to ``optimizer`` (an ``optim.AdamW`` over the factors, or any optimiser with torch's interface) and one
-    step of it: every rank takes the same step."""
+    step of it: every rank takes the same step.  What else the optimiser holds stays as it is: its gradients (another layer's, from that
+    layer's own step) are set aside meanwhile."""
     if optimizer is None:
         return
-    known = {id(p) for g in optimizer.param_groups for p in g["params"]}
-    if not all(id(p) in known for p in params):
+    held = {id(p): p for g in optimizer.param_groups for p in g["params"]}
+    if not all(id(p) in held for p in params):
         raise ValueError("the optimizer has to be over the factors of this step")
+    for p in params:
+        held.pop(id(p), None)
+    aside = [(p, p.grad) for p in held.values() if p.grad is not None]
     for p, g in zip(params, grads):
         p.grad = g
-    optimizer.step()
+    try:
+        for p, _ in aside:
+            p.grad = None
+        optimizer.step()
+    finally:
+        for p, g in aside:
+            p.grad = g
 
 
 def cp4_data_parallel_step(X, dU, FT, FC, FY, FX, pad=1, flags=0, group=None, optimizer=None):
     """forward, backward-data and backward-filter on this rank's shard, then the gradient allreduce and, with ``optimizer`` (over the four
-    factors), its step.  Returns (U, dX, (dFT, dFC, dFY, dFX)) with the gradients summed over every rank's shard."""
+    factors, and others that this step leaves alone), its step.  Returns (U, dX, (dFT, dFC, dFY, dFX)) with the gradients summed over every rank's shard."""
     from . import ops
     U = ops.cp4_conv2d_forward(X, FT, FC, FY, FX, pad, flags)
     dX = ops.cp4_conv2d_backward_data(dU, FT, FC, FY, FX, pad, flags)
@@ -214,7 +224,7 @@ def _unpack(packed, like):
 def rcp_data_parallel_step(X, dV, A, S, allreduce=None, group=None, optimizer=None):
     """Reshaped-CP conv on this rank's batch shard: forward, data gradient and factor gradients, then ONE allreduce of
     the packed factor gradients ``[dA_1 | ... | dA_m | dS]`` (sum_k c_k t_k R + FH FW R floats).  ``allreduce`` is a
-    callable on the packed buffer (e.g. a ``P2PAllreduce``); default: ``allreduce_factor_grads``.  ``optimizer`` (over the factors): takes its step.
+    callable on the packed buffer (e.g. a ``P2PAllreduce``); default: ``allreduce_factor_grads``.  ``optimizer`` (over the factors, and others that it leaves alone): takes its step.
     Returns (V, dX, [dA_k], dS) with the gradients summed over all ranks."""
     from . import ops
     V = ops.conv2d_rcp_fused_nchw(X, *A, S)
@@ -228,7 +238,7 @@ def rcp_data_parallel_step(X, dV, A, S, allreduce=None, group=None, optimizer=No
 
 def dense_data_parallel_step(X, dY, F, allreduce=None, group=None, optimizer=None):
     """CP dense layer on this rank's batch shard: forward, data gradient and factor gradients, then ONE allreduce of
-    the packed factor gradients (sum_k i_k o_k R floats: 8 192 at 8^4 -> 8^4, R = 32).  ``optimizer`` (over the factors): takes its step.
+    the packed factor gradients (sum_k i_k o_k R floats: 8 192 at 8^4 -> 8^4, R = 32).  ``optimizer`` (over the factors, and others that it leaves alone): takes its step.
     Returns (Y, dX, [dF_k]) with the gradients summed over all ranks."""
     from . import ops
     Y = ops.dense_cp(X, *F)
