@@ -16,8 +16,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``bits=8`` keeps the moments as 8-bit codes with a float32 scale per 256 values: 2.03 bytes a value instead of 8.  16-bit
     parameters get a float32 copy that is what is updated (``master=False``: the parameter itself, rounded at each step).
-    ``capturable=True`` keeps a count of the steps on the device, one for all parameters of a group, so that a captured ``step()``
-    counts its replays; make one step before the capture.  ``lr`` may be one float32 in a CUDA tensor.
+    ``capturable=True`` keeps the counts of steps on the device, one for all parameters that have taken the same steps, so that a captured
+    ``step()`` counts its replays; make one step with the same gradients before the capture.  ``lr`` may be one float32 in a CUDA tensor.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, master=True, capturable=False):
@@ -27,16 +27,19 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("lr, eps and weight_decay may not be negative, betas are in [0, 1)")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits, master=master, capturable=capturable))
 
-        self._counts = {}
-
-    def _state_of(self, p, at, group):
+    def _state_of(self, p, group, first):
         s = self.state[p]
         if not s:
             if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
                 raise TypeError(f"parameters are float32, bfloat16 or float16, not {p.dtype}")
             if not p.is_contiguous():
                 raise ValueError("parameters are updated in place and have to be contiguous")
-            s["step"] = self._count(at, p.device) if group["capturable"] else 0
+            if not group["capturable"]:
+                s["step"] = 0
+            else:   # parameters whose first step is the same share a count
+                if p.device not in first:
+                    first[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
+                s["step"] = first[p.device]
             if group["bits"] == 8:
                 blocks = (p.numel() + BLOCK - 1) // BLOCK
                 s["exp_avg"] = torch.zeros(p.shape, dtype=torch.int8, device=p.device)
@@ -48,11 +51,23 @@ class AdamW(torch.optim.Optimizer):
                 s["master"] = p.detach().float()
         return s
 
-    def _count(self, at, device):
-        """The steps of a group's parameters on a device, on that device."""
-        if (at, device) not in self._counts:
-            self._counts[at, device] = torch.zeros((), dtype=torch.int64, device=device)
-        return self._counts[at, device]
+    def _advance(self, group, members):
+        """One step more for the counts of these states of a capturable group.  Parameters that share a count with others that have no gradient
+        this time get one of their own."""
+        counts, sharers = {}, {}
+        for p in group["params"]:
+            s = self.state.get(p)
+            if s:
+                sharers[id(s["step"])] = sharers.get(id(s["step"]), 0) + 1
+        for s in members:
+            counts.setdefault(id(s["step"]), []).append(s)
+        for at, ss in counts.items():
+            count = ss[0]["step"]
+            if len(ss) < sharers[at]:
+                count = count.clone()
+                for s in ss:
+                    s["step"] = count
+            count.add_(1)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -63,56 +78,54 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for at, group in enumerate(self.param_groups):
-            calls, counted = {}, set()
+        for group in self.param_groups:
+            calls, stepped, first = {}, [], {}
             for p in group["params"]:
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
                     raise TypeError("gradients have to be dense")
-                s = self._state_of(p, at, group)
+                s = self._state_of(p, group, first)
                 if group["capturable"]:
-                    counted.add(p.device)
-                    count = None
+                    stepped.append((p, s))
                 else:
                     s["step"] += 1
-                    count = s["step"]
-                calls.setdefault((p.device, p.dtype, p.grad.dtype, "master" in s, count), []).append((p, s))
-            for device in counted:
-                self._count(at, device).add_(1)
-            for (device, _, _, copies, count), members in calls.items():
+                    calls.setdefault((p.device, p.dtype, p.grad.dtype, "master" in s, s["step"]), []).append((p, s))
+            if stepped:
+                self._advance(group, [s for _, s in stepped])
+            for p, s in stepped:
+                calls.setdefault((p.device, p.dtype, p.grad.dtype, "master" in s, id(s["step"])), []).append((p, s))
+            for (_, _, _, copies, _), members in calls.items():
                 ps, ss = zip(*members)
                 ops.adamw_step([p.detach() for p in ps], [p.grad for p in ps], [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss],
-                               self._count(at, device) if count is None else count, group["lr"], group["betas"], group["eps"],
+                               ss[0]["step"], group["lr"], group["betas"], group["eps"],
                                group["weight_decay"], [s["master"] for s in ss] if copies else None,
                                ([s["scale_avg"] for s in ss], [s["scale_sq"] for s in ss]) if group["bits"] == 8 else None)
         return loss
 
-    def __setstate__(self, state):
-        """A copied or unpickled optimiser: the parameters of a group share its count again."""
-        super().__setstate__(state)
-        self._counts = {}
-        for at, group in enumerate(self.param_groups):
+    def _share_counts(self):
+        """Parameters of a capturable group that have taken as many steps share a count (where they took different ones, it divides later)."""
+        for group in self.param_groups:
+            counts = {}
             for p in group["params"]:
                 s = self.state.get(p)
                 if group["capturable"] and s and torch.is_tensor(s.get("step")):
-                    s["step"] = self._counts.setdefault((at, p.device), s["step"])
+                    s["step"] = counts.setdefault((p.device, int(s["step"])), s["step"])
+
+    def __setstate__(self, state):
+        """A copied or unpickled optimiser: parameters share their counts again."""
+        super().__setstate__(state)
+        self._share_counts()
 
     def load_state_dict(self, state_dict):
         """As the base class, but the state keeps its own types (codes, float32 moments of 16-bit parameters)."""
         super().load_state_dict(state_dict)
         names = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
-        self._counts = {}
-        of = {id(p): at for at, g in enumerate(self.param_groups) for p in g["params"]}
-        for name, p in zip(names, chain.from_iterable(g["params"] for g in self.param_groups)):
+        for name, (group, p) in zip(names, ((g, p) for g in self.param_groups for p in g["params"])):
             if name not in state_dict["state"]:
                 continue
             s = {k: v.detach().to(p.device, copy=True) if torch.is_tensor(v) else v for k, v in state_dict["state"][name].items()}
-            at = of[id(p)]
-            if self.param_groups[at]["capturable"]:
-                count = self._count(at, p.device)
-                count.copy_(torch.as_tensor(s["step"]))
-                s["step"] = count
-            elif torch.is_tensor(s["step"]):
-                s["step"] = int(s["step"])
+            steps = int(s["step"])
+            s["step"] = torch.full((), steps, dtype=torch.int64, device=p.device) if group["capturable"] else steps
             self.state[p] = s
+        self._share_counts()
