@@ -17,7 +17,8 @@ class AdamW(torch.optim.Optimizer):
     ``bits=8`` keeps the moments as 8-bit codes with a float32 scale per 256 values: 2.03 bytes a value instead of 8.  16-bit
     parameters get a float32 copy that is what is updated (``master=False``: the parameter itself, rounded at each step).
     ``capturable=True`` keeps the counts of steps on the device, one for all parameters that have taken the same steps, so that a captured
-    ``step()`` counts its replays; make one step with the same gradients before the capture.  ``lr`` may be one float32 in a CUDA tensor.
+    ``step()`` counts its replays; make one step with the same gradients before the capture.  (A step that would begin a state or a count
+    inside a capture is refused: each replay would begin it again.)  ``lr`` may be one float32 in a CUDA tensor.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, master=True, capturable=False):
@@ -27,9 +28,11 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("lr, eps and weight_decay may not be negative, betas are in [0, 1)")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits, master=master, capturable=capturable))
 
-    def _state_of(self, p, group, first):
+    def _state_of(self, p, group, first, capturing):
         s = self.state[p]
         if not s:
+            if capturing:
+                raise RuntimeError("a captured step() begins no state: make a step with the same gradients before the capture")
             if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
                 raise TypeError(f"parameters are float32, bfloat16 or float16, not {p.dtype}")
             if not p.is_contiguous():
@@ -51,7 +54,7 @@ class AdamW(torch.optim.Optimizer):
                 s["master"] = p.detach().float()
         return s
 
-    def _advance(self, group, members):
+    def _advance(self, group, members, capturing):
         """One step more for the counts of these states of a capturable group.  Parameters that share a count with others that have no gradient
         this time get one of their own."""
         counts, sharers = {}, {}
@@ -64,6 +67,8 @@ class AdamW(torch.optim.Optimizer):
         for at, ss in counts.items():
             count = ss[0]["step"]
             if len(ss) < sharers[at]:
+                if capturing:
+                    raise RuntimeError("a captured step() divides no count: make a step with the same gradients before the capture")
                 count = count.clone()
                 for s in ss:
                     s["step"] = count
@@ -78,21 +83,24 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         for group in self.param_groups:
+            if capturing and not group["capturable"] and any(p.grad is not None for p in group["params"]):
+                raise RuntimeError("a captured step() counts its replays with capturable=True alone")
             calls, stepped, first = {}, [], {}
             for p in group["params"]:
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
                     raise TypeError("gradients have to be dense")
-                s = self._state_of(p, group, first)
+                s = self._state_of(p, group, first, capturing)
                 if group["capturable"]:
                     stepped.append((p, s))
                 else:
                     s["step"] += 1
                     calls.setdefault((p.device, p.dtype, p.grad.dtype, "master" in s, s["step"]), []).append((p, s))
             if stepped:
-                self._advance(group, [s for _, s in stepped])
+                self._advance(group, [s for _, s in stepped], capturing)
             for p, s in stepped:
                 calls.setdefault((p.device, p.dtype, p.grad.dtype, "master" in s, id(s["step"])), []).append((p, s))
             for (_, _, _, copies, _), members in calls.items():

@@ -97,3 +97,32 @@ def test_late_parameters_are_updated_as_by_an_eager_optimiser():
             opt.step()
         for a, b in ((a.detach(), b.detach()) for a, b in zip(*twins)):   # a rate that is rounded the other way moves a sum by one place at most, in each of five steps
             assert float((a - b).abs().max()) <= 6 * 2.0 ** -23 * float(a.abs().max())
+
+
+@pytest.mark.gpu
+def test_a_capture_begins_and_divides_nothing():
+    """Refused while a stream is captured; the capture itself ends in order and the optimiser goes on."""
+    from paralleltnnlayers_b200.optim import AdamW
+    p = [torch.nn.Parameter(torch.ones(5, device="cuda")) for _ in range(2)]
+    for q in p:
+        q.grad = torch.ones_like(q)
+
+    def refused(opt, match):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match=match):
+                opt.step()
+            torch.zeros(1, device="cuda")   # something to capture
+
+    opt = AdamW(p, capturable=True)
+    refused(opt, "begins no state")
+    refused(AdamW(p), "capturable=True alone")
+    opt.step()
+    p[1].grad = None
+    refused(opt, "divides no count")
+    p[1].grad = torch.ones_like(p[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    assert [int(opt.state[q]["step"]) for q in p] == [2, 2]
