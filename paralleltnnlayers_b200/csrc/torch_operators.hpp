@@ -334,9 +334,16 @@ PYFN(py_adapters_apply) {
   count_args(n, 7);
   const Tensor &y = any_tensor(a[0], "Y"), &x = any_tensor(a[1], "X"), &A = any_tensor(a[2], "A"), &B = any_tensor(a[3], "B"),
                &which = any_tensor(a[4], "adapters");
-  const int64_t planned = int_arg(a[5]);
+  int64_t planned = int_arg(a[5]);
   const Tensor scale = optional_tensor(a[6], "scale");
+  const bool grad = at::GradMode::is_enabled() && (y.requires_grad() || x.requires_grad() || A.requires_grad() || B.requires_grad());
   return wrap(unlocked([&] {
+    if (!grad) {   // nothing is kept, and a small batch needs no plan
+      const Adapters op(x, A, B, scale);
+      op.fits(y, "Y");
+      const Tensor by = op.numbers(which, &planned);
+      return dense_adapters(op, y, by, planned, Tensor(), nullptr);
+    }
     Tensor plan;
     {
       at::NoGradGuard none;
