@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "b200cp.h"
+#include "spans.hpp"
 
 namespace {
 

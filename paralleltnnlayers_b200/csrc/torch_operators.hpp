@@ -482,8 +482,12 @@ PYFN(py_adamw_step) {
   }
   std::vector<b200cp_adamw_tensor> ts(count);
   std::vector<Tensor> held;   // contiguous copies of gradients
-  std::vector<uintptr_t> seen;
-  seen.reserve(2 * count);
+  // what the launch reads and writes: a list for each kind of tensor
+  enum { kParam, kGrad, kAvg, kSq, kScaleAvg, kScaleSq, kMaster, kKinds };
+  std::vector<b200cp::Span> spans(kKinds * count);
+  const auto span = [&](int kind, size_t i, const void* p, size_t bytes) {
+    spans[kind * count + i] = {reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes};
+  };
   const c10::cuda::OptionalCUDAGuard guard(device);
   const auto at_of = [](const Tensor& t) { return t.mutable_data_ptr(); };
   for (size_t i = 0; i < count; ++i) {
@@ -498,12 +502,22 @@ PYFN(py_adamw_step) {
     }
     ts[i] = {at_of(p[i]), grad, at_of(m[i]), at_of(v[i]), small ? mp(ms[i]) : nullptr, small ? mp(vs[i]) : nullptr, copies ? mp(w[i]) : nullptr,
              (unsigned long long)numel};
-    seen.push_back((uintptr_t)ts[i].param);
-    seen.push_back((uintptr_t)ts[i].exp_avg);
-    seen.push_back((uintptr_t)ts[i].exp_avg_sq);
+    const b200cp_adamw_tensor& e = ts[i];
+    span(kParam, i, e.param, p[i].nbytes());
+    span(kGrad, i, e.grad, g[i].nbytes());
+    span(kAvg, i, e.exp_avg, m[i].nbytes());
+    span(kSq, i, e.exp_avg_sq, v[i].nbytes());
+    if (small) {
+      span(kScaleAvg, i, e.scale_avg, ms[i].nbytes());
+      span(kScaleSq, i, e.scale_sq, vs[i].nbytes());
+    }
+    if (copies) span(kMaster, i, e.master, w[i].nbytes());
   }
-  if (!std::is_sorted(seen.begin(), seen.end())) std::sort(seen.begin(), seen.end());
-  TORCH_CHECK_VALUE(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "adamw_step: a tensor occurs twice in what is updated");
+  b200cp::SpanList kinds[kKinds];
+  size_t used = 0;
+  for (int k = 0; k < kKinds; ++k)
+    if ((small || (k != kScaleAvg && k != kScaleSq)) && (copies || k != kMaster)) kinds[used++] = {&spans[k * count], count, k != kGrad};
+  TORCH_CHECK_VALUE(!b200cp::spans_meet(kinds, used), "adamw_step: a tensor occurs twice in what is updated, or shares memory with another one");
   if (step) h.device_step = reinterpret_cast<const long long*>(step->const_data_ptr());
   if (lr) h.device_lr = static_cast<const float*>(lr->const_data_ptr());
   void* st = stream(p[0]);
