@@ -991,12 +991,13 @@ int launch_tiles(const Args& g, const Plan& p, cudaStream_t st) {
   static std::atomic<int> set[64];
   B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, S::smem));
   // CTAs of a tile: as many as the machine is likely to hold at once, with a chunk of the longer product for each
-  static std::atomic<int> cache[9];
-  int c = 1;
+  static ClusterCounts counts;
+  int c = 1, dev = 0;
+  B200CP_CUDA_OK(cudaGetDevice(&dev));
   const int chunks = std::max(ceil_div(g.K, S::KC), ceil_div(g.N, S::KC));
   for (int q = 2; q <= 8 && q <= chunks; q *= 2) {
     int n = 0;
-    B200CP_CUDA_OK(resident_clusters(kern, kThreads, S::smem, q, cache, &n));
+    B200CP_CUDA_OK(resident_clusters(kern, kThreads, S::smem, dev, q, counts, &n));
     if (p.likely <= n) c = q;
   }
   B200CP_CUDA_OK(launch_clusters(kern, p.tiles, c, kThreads, S::smem, st, g));

@@ -111,13 +111,14 @@ inline int pick_cluster(long tiles, int units, int least, int sm_count) {
 }
 
 // ---- launch of clusters along x ------------------------------------------------------------------------------------------
-// How many clusters of c CTAs of a kernel the device holds at once, asked once per kernel and size (`cache`: nine zeros): those of seven, say,
-// are fewer than a seventh of the CTAs, since a cluster lies within one group of SMs.
+// How many clusters of c CTAs (at most 8) of a kernel the current device, `dev`, holds at once: asked once per kernel, device and size.  Those of seven, say,
+// are fewer than a seventh of the CTAs, since a cluster lies within one group of SMs.  0: a cluster of this size does not run there.
+struct ClusterCounts {   // function-local static of a kernel, all zeros
+  std::atomic<int> of[64][9];
+};
 template <typename Kern>
-cudaError_t resident_clusters(Kern kern, int threads, size_t smem, int c, std::atomic<int>* cache, int* out) {
-  int n = cache[c].load(std::memory_order_relaxed);
-  cudaError_t e = cudaSuccess;
-  if (!n) {
+cudaError_t resident_clusters(Kern kern, int threads, size_t smem, int dev, int c, ClusterCounts& counts, int* out) {
+  const auto ask = [&](int* n) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)c);
     cfg.blockDim = dim3((unsigned)threads);
@@ -128,11 +129,9 @@ cudaError_t resident_clusters(Kern kern, int threads, size_t smem, int c, std::a
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
-    if (e == cudaSuccess) cache[c].store(n > 0 ? n : (n = 1), std::memory_order_relaxed);
-  }
-  *out = n;
-  return e;
+    return cudaOccupancyMaxActiveClusters(n, kern, &cfg);
+  };
+  return dev < 0 || dev >= 64 ? ask(out) : remembered_count(counts.of[dev][c], out, ask);
 }
 // A programmatic dependent launch of `clusters` clusters of c CTAs.
 template <typename... KArgs, typename... Args>

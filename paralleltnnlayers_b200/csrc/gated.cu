@@ -686,13 +686,16 @@ template <int NT, int W, typename T>
 int few_ctas(const FewArgs& g, int* cluster, int* ctas) {
   using F = Few<NT, W>;
   const auto kern = gated_few_kernel<NT, W, T>;
-  static std::atomic<int> set[64], cache[9];
+  static std::atomic<int> set[64];
+  static ClusterCounts counts;
+  int dev = 0;
+  B200CP_CUDA_OK(cudaGetDevice(&dev));
   B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, (int)F::smem));
   const int tiles = ceil_div(g.N, F::cols);
   *cluster = 1;
   for (int q = 2; q <= 8 && g.steps >= 2 * q; ++q) {
     int n = 0;
-    B200CP_CUDA_OK(resident_clusters(kern, kFewThreads, F::smem, q, cache, &n));
+    B200CP_CUDA_OK(resident_clusters(kern, kFewThreads, F::smem, dev, q, counts, &n));
     if (tiles <= n) *cluster = q;
   }
   *ctas = tiles * *cluster;

@@ -1,4 +1,4 @@
-// A limit that host threads raise (dynamic shared memory of a kernel).
+// A limit that host threads raise (dynamic shared memory of a kernel), and a count that they ask for once.
 #pragma once
 
 #include <atomic>
@@ -20,6 +20,20 @@ auto raise_limit(std::atomic<int>& record, int value, Set set) -> decltype(set(v
   if (record.load(std::memory_order_relaxed) >= value) return Error{};
   const Error e = set(value);
   if (e == Error{}) record.store(value, std::memory_order_release);
+  return e;
+}
+
+// A count that `ask` gives, asked once: `slot` holds it plus one (0: not asked yet; no count of zero is taken for that, or for another count).
+template <typename Ask>
+auto remembered_count(std::atomic<int>& slot, int* out, Ask ask) -> decltype(ask(out)) {
+  using Error = decltype(ask(out));
+  const int held = slot.load(std::memory_order_relaxed);
+  if (held > 0) {
+    *out = held - 1;
+    return Error{};
+  }
+  const Error e = ask(out);
+  if (e == Error{}) slot.store(*out + 1, std::memory_order_relaxed);
   return e;
 }
 
