@@ -133,7 +133,7 @@ cudaError_t resident_clusters(Kern kern, int threads, size_t smem, int dev, int 
   };
   return dev < 0 || dev >= 64 ? ask(out) : remembered_count(counts.of[dev][c], out, ask);
 }
-// A programmatic dependent launch of `clusters` clusters of c CTAs.
+// A programmatic dependent launch (unless B200CP_PDL=0) of `clusters` clusters of c CTAs.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_clusters(void (*kern)(KArgs...), int clusters, int c, int threads, size_t smem, cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg{};
@@ -148,7 +148,11 @@ cudaError_t launch_clusters(void (*kern)(KArgs...), int clusters, int c, int thr
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 2;
+  static const bool off = [] {
+    const char* e = getenv("B200CP_PDL");
+    return e && e[0] == '0';
+  }();
+  cfg.numAttrs = off ? 1 : 2;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
