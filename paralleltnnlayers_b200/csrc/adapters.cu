@@ -650,14 +650,17 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, TM, RP>::ctas)) adapters_k
       }
     }
     const int r = i / RP, j = i - r * RP;
+    // (Ranks that are not there are zero whatever the row holds: an infinity times their zeros would be NaN, and so would the whole row of out.)
+    v.x = j < R ? v.x * c : 0.f;
+    v.y = j + 1 < R ? v.y * c : 0.f;
     T* to = reinterpret_cast<T*>(vs + r * S::ls) + j;
-    to[0] = (T)(v.x * c);
-    to[1] = (T)(v.y * c);
+    to[0] = (T)v.x;
+    to[1] = (T)v.y;
     if constexpr (sizeof(T) == 2) {   // what the rounding left (of an infinity nothing)
       T* rest = reinterpret_cast<T*>(vs + (TM + r) * S::ls) + j;
       const float a0 = (float)to[0], a1 = (float)to[1];
-      rest[0] = fabsf(a0) < __int_as_float(0x7f800000) ? (T)(v.x * c - a0) : (T)0.f;
-      rest[1] = fabsf(a1) < __int_as_float(0x7f800000) ? (T)(v.y * c - a1) : (T)0.f;
+      rest[0] = fabsf(a0) < __int_as_float(0x7f800000) ? (T)(v.x - a0) : (T)0.f;
+      rest[1] = fabsf(a1) < __int_as_float(0x7f800000) ? (T)(v.y - a1) : (T)0.f;
     }
     if (g.V && crank == 0 && r < len) {
       T* w = static_cast<T*>(g.V) + (size_t)rowat[r] * R + j;
