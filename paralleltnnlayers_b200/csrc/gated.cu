@@ -83,7 +83,8 @@ __device__ __forceinline__ float gate_share(int act, float g, float* slope) {
     return s;
   }
   const float q = kRootPi * fmaf(0.044715f * g, g * g, g), s = sigmoid(2.f * q);   // (1 + tanh q) / 2
-  if (SLOPE) *slope = s * fmaf(2.f * (1.f - s) * g, kRootPi * fmaf(3.f * 0.044715f * g, g, 1.f), 1.f);
+  // (s (1 - s) first: it is zero from some |g| on, where the other factors' product would be infinite)
+  if (SLOPE) *slope = fmaf(g * (2.f * s * (1.f - s)), fminf(kRootPi * fmaf(3.f * 0.044715f * g, g, 1.f), 3.4028235e38f), s);
   return s;
 }
 
