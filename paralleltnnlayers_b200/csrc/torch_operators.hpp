@@ -114,7 +114,7 @@ struct Adapters {   // operands, checked and contiguous
                           (size_t)which.numel() == std::max<size_t>(16, b200cp_adapter_plan_bytes(rows, count)),
                       "the plan is not one of ", rows, " rows and ", count, " adapters");
   }
-  void takes(const Tensor& out, const Tensor& y) const {   // as the place of the result
+  void takes(const Tensor& out, const Tensor& y, const Tensor& which) const {   // as the place of the result
     fits(out, "out");
     TORCH_CHECK_VALUE(out.is_contiguous(), "out has to be contiguous");
     const auto meets = [&](const Tensor& t) {   // (from the first to behind the last value that a tensor holds)
@@ -124,7 +124,8 @@ struct Adapters {   // operands, checked and contiguous
       const auto a = reinterpret_cast<uintptr_t>(t.const_data_ptr()), b = reinterpret_cast<uintptr_t>(out.const_data_ptr());
       return a < b + out.nbytes() && b < a + (size_t)(last + 1) * t.element_size();
     };
-    for (const Tensor* t : {&x, &A, &B}) TORCH_CHECK_VALUE(!meets(*t), "out may share memory with Y alone");
+    for (const Tensor* t : {&x, &A, &B, &which}) TORCH_CHECK_VALUE(!meets(*t), "out may share memory with Y alone");
+    TORCH_CHECK_VALUE(!scale.defined() || !meets(scale), "out may share memory with Y alone");
     TORCH_CHECK_VALUE(!meets(y) || (y.is_contiguous() && y.const_data_ptr() == out.const_data_ptr()),
                       "out may be Y, but not another part or order of its memory");
   }
@@ -303,7 +304,7 @@ PYFN(py_dense_adapters) {
   Tensor out = unlocked([&] {
     const Adapters op(x, A, B, scale);
     op.fits(y, "Y");
-    if (to.defined()) op.takes(to, y);
+    if (to.defined()) op.takes(to, y, which);
     const Tensor by = op.numbers(which, &planned);
     return dense_adapters(op, y, by, planned, to, nullptr);
   });

@@ -74,3 +74,27 @@ def test_the_library_computes_nothing_from_a_plan_of_another_count(rows, planned
     outs = run(P.adapter_plan(which, count).data)
     P.device_status()
     assert all(not bool((t == 7).any()) for t in outs)
+
+
+@pytest.mark.gpu
+def test_an_output_over_the_numbers_the_plan_or_the_scales_is_refused():
+    """CTAs that are done would write what others still read."""
+    import paralleltnnlayers_b200 as P
+    rows, I, O, R, count = 32, 16, 8, 4, 8
+    n = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    y, x, A, B, scale = n(rows, O), n(rows, I), n(count, I, R), n(count, R, O), torch.ones(count, device="cuda")
+    which = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    buf = torch.zeros(rows * O, device="cuda")
+    over = lambda t: buf[100:100 + t.numel()].view(t.dtype).copy_(t)  # noqa: E731
+    plan = P.adapter_plan(which, count)
+    size = plan.data.numel() // 4
+    room = torch.zeros(rows * O + size, device="cuda")
+    plan.data = room[16:16 + size].view(torch.uint8).copy_(plan.data)
+    with pytest.raises(ValueError, match="share memory"):
+        P.dense_adapters(y, x, A, B, over(which), scale, out=buf.view(rows, O))
+    with pytest.raises(ValueError, match="share memory"):
+        P.dense_adapters(y, x, A, B, which, over(scale), out=buf.view(rows, O))
+    with pytest.raises(ValueError, match="share memory"):
+        P.dense_adapters(y, x, A, B, plan, scale, out=room[:rows * O].view(rows, O))
+    out = P.dense_adapters(y, x, A, B, which, scale, out=buf.view(rows, O))
+    assert torch.equal(out, P.dense_adapters(y, x, A, B, which, scale))
