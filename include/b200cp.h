@@ -416,7 +416,8 @@ int b200cp_adapter_plan(int rows, int count, const int* adapters, void* plan, si
  * X [rows, I], Y, out [rows, O], A [count, I, R], B [count, R, O] of one type (B200CP_FLOAT32, _BFLOAT16, _FLOAT16), R at most 128;
  * scale [count] floats, or NULL for ones.  out may be Y.  The rows' adapters come as a plan, or, with plan NULL, as adapters[rows] for batches of
  * up to B200CP_ADAPTERS_WITHOUT_PLAN rows (a token of each request): then one launch does it all.  V (or NULL): [rows, R] of the same
- * type, receives scale X A for the backward (rows without an adapter are left as they are).  Stands beside b200cp_dense_fwd, whose Y it
+ * type, receives scale X A for the backward (rows without an adapter are left as they are).  scale X A, and in the gradients scale dY B^T, have to
+ * be in the type's range (float16: 65504): both go into products as values of that type.  Stands beside b200cp_dense_fwd, whose Y it
  * takes (a serving batch of test/test_dense_cp.py:41 with one correction per request); the reference has no adapters. */
 enum { B200CP_ADAPTERS_WITHOUT_PLAN = 256 };
 int b200cp_dense_adapters(int rows, int I, int O, int R, int count, int type, const void* Y, const void* X, const void* A, const void* B,

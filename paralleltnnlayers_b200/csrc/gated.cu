@@ -127,9 +127,9 @@ __device__ __forceinline__ void put_block(uint8_t* patch, T* out, int vec, int m
   __syncwarp();
 }
 // The warp's 32 kept rows of 32 floats as the box of a tensor store (128-byte rows, swizzled: neighbouring lanes on other banks).  G and U are 8
-// of the 10 bytes that a value of the forward writes, and what a tile of few inputs waits for: 8192 x 1024 -> 2816 takes 132 us, 2048 x 2048 ->
-// 5120 95, and 167 and 110 where the lanes store them, 64 bytes of a row at a time through the patch.  One block for both, not two: two leave room
-// for five steps of the ring, which saves nothing there (125 and 100 us).
+// of the 10 bytes that a value of the forward writes, and what a tile of few inputs waits for.  4096 x 4096 -> 10240, 8192 x 1024 -> 2816 and 2048 x
+// 2048 -> 5120, cold and alone: 449, 102 and 78 us; 440, 131 and 84 where the lanes store them, 64 bytes of a row at a time through the patch; 412,
+// 92 and 70 where nothing is kept.  One block for both, not two, which leave room for five steps of the ring: 460, 100 and 80 us.
 __device__ __forceinline__ void keep_block(uint8_t* block, const float (&v)[32]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll

@@ -422,9 +422,9 @@ def dense_adapters(Y, X, A, B, adapters, scale=None, out=None):
     """``out[s] = Y[s] + scale[a] (X[s] A[a]) B[a]``, ``a`` the adapter of row ``s``: what a shared projection gave for a batch of many requests,
     corrected for each by its own low-rank adapter (``b200cp_dense_adapters``).  Rows without an adapter come out as ``Y``.
 
-    ``X [..., I]``, ``Y [..., O]``, ``A [count, I, R]``, ``B [count, R, O]`` of one type: float32, bfloat16 or float16 (sums in float32; ``scale (X A)``
-    has to be in the type's range); ``R`` at most 128.  ``adapters``: an int32 or int64 tensor of ``X``'s leading shape, or
-    the ``AdapterPlan`` of one.  ``scale``: float32 per adapter.  ``out`` may be ``Y``."""
+    ``X [..., I]``, ``Y [..., O]``, ``A [count, I, R]``, ``B [count, R, O]`` of one type: float32, bfloat16 or float16 (sums in float32; ``scale (X A)``,
+    and in the gradients ``scale (dY B^T)``, have to be in the type's range); ``R`` at most 128.  ``adapters``: an int32 or int64 tensor of ``X``'s leading shape, or
+    the ``AdapterPlan`` of one, for as many adapters as ``A`` has.  ``scale``: float32 per adapter.  ``out`` may be ``Y``."""
     which, planned = _which(adapters, X)
     return _C.dense_adapters(Y, X, A, B, which, planned, scale, out)
 
@@ -466,13 +466,13 @@ def dense_gated_backward(dH, X, Wg, Wu, G, U, activation="silu", need_dx=True, n
 
 # ---- AdamW step -----------------------------------------------------------------
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, master=None, scales=None):
-    """One AdamW step over all tensors of the lists, in place and in one launch (``b200cp_adamw_step``):
+    """One AdamW step over all tensors of the lists, in place and in one launch per 448 (``b200cp_adamw_step``):
     ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g**2``, ``p -= lr wd p + lr (m / (1 - b1**t)) / (sqrt(v / (1 - b2**t)) + eps)``.
 
     ``params``: contiguous tensors of one type on one device; ``grads`` of that type or float32.  Moments: float32 of the parameters'
     sizes, or, with ``scales = (list, list)``, int8 and uint8 codes with a float32 scale per 256 values (all zero before the first step).
     ``master``: the float32 copies of 16-bit parameters; then they are what is updated, and the parameters are their roundings.
-    ``step`` counts from one; it may be one int64 in a CUDA tensor, and ``lr`` one float32 in one, which a captured step reads at each replay."""
+    What is updated may not share memory with anything else of the call.  ``step`` counts from one; it may be one int64 in a CUDA tensor, and ``lr`` one float32 in one, which a captured step reads at each replay."""
     ms, vs = scales if scales is not None else (None, None)
     _C.adamw_step(params, grads, exp_avg, exp_avg_sq, ms, vs, master, step, lr, betas[0], betas[1], eps, weight_decay)
 

@@ -15,7 +15,8 @@ class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) with ``torch.optim.AdamW``'s arguments, its update in fp32.
 
     ``bits=8`` keeps the moments as 8-bit codes with a float32 scale per 256 values: 2.03 bytes a value instead of 8.  16-bit
-    parameters get a float32 copy that is what is updated (``master=False``: the parameter itself, rounded at each step).
+    parameters get a float32 copy that is what is updated (``master=False``: the parameter itself, rounded at each step); it is taken at a
+    parameter's first step, so values that are put into the parameter later do not reach it.
     ``capturable=True`` keeps the counts of steps on the device, one for all parameters that have taken the same steps, so that a captured
     ``step()`` counts its replays; make one step with the same gradients before the capture.  (A step that would begin a state or a count
     inside a capture is refused: each replay would begin it again.)  ``lr`` may be one float32 in a CUDA tensor.
