@@ -59,15 +59,16 @@ class AdamW(torch.optim.Optimizer):
         """One step more for the counts of these states of a capturable group.  Parameters that share a count with others that have no gradient
         this time get one of their own."""
         counts, sharers = {}, {}
-        for p in group["params"]:
-            s = self.state.get(p)
-            if s:
-                sharers[id(s["step"])] = sharers.get(id(s["step"]), 0) + 1
         for s in members:
             counts.setdefault(id(s["step"]), []).append(s)
+        if len(members) < len(group["params"]):   # (else all that share a count are here)
+            for p in group["params"]:
+                s = self.state.get(p)
+                if s:
+                    sharers[id(s["step"])] = sharers.get(id(s["step"]), 0) + 1
         for at, ss in counts.items():
             count = ss[0]["step"]
-            if len(ss) < sharers[at]:
+            if len(ss) < sharers.get(at, 0):
                 if capturing:
                     raise RuntimeError("a captured step() divides no count: make a step with the same gradients before the capture")
                 count = count.clone()
