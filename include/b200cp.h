@@ -450,6 +450,71 @@ int b200cp_dense_gated_bwd(int rows, int I, int F, int type, int activation, con
                            const float* U, const void* dH, void* dX, void* dWg, void* dWu, void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/* ---- embedding --------------------------------------------------------------------------------------------------- */
+
+/* out[s] = scale W[t] with t = tokens[s]; zeros where t is outside 0 .. V-1 (padding).  tokens [rows]: int (number_type 0) or long long (1);
+ * W [V, D], out [rows, D] of one type.  rows and D are at most 2^30.  No counterpart in the reference: what feeds the dense layers of a language model. */
+int b200cp_embedding(int rows, int V, int D, int type, int number_type, const void* tokens, const void* W, float scale, void* out,
+                     void* stream);
+
+/* dW[v] = scale times the sum of dY[s] over the s with tokens[s] = v; all V rows are written.  Sums are fp32, in the order of s within
+ * parts of fixed length: the same bits each time.  The workspace is 16-byte aligned. */
+size_t b200cp_embedding_bwd_workspace_bytes(int rows, int D);
+int b200cp_embedding_bwd(int rows, int V, int D, int type, int number_type, const void* tokens, const void* dY, float scale, void* dW,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- layer norm ---------------------------------------------------------------------------------------------------- */
+
+/* H = X + R rounded to the type (R and H may both be NULL: H is X), Y = (H - mean) rstd w + b per row, with the mean of the row's D features and
+ * rstd = 1 / sqrt(their variance + eps).  X, R, Y, H [rows, D] of one type; w, b [D] of that type or float (weight_type), each may be NULL.
+ * mean, rstd (both or neither): [rows] floats, kept for the backward.  Statistics are fp32.  No counterpart in the reference. */
+int b200cp_layer_norm(int rows, int D, int type, int weight_type, const void* X, const void* R, const void* w, const void* b, float eps,
+                      void* Y, void* H, float* mean, float* rstd, void* stream);
+
+/* dX = rstd (g - mean(g) - n mean(g n)) + dH with g = dY w and n = (H - mean) rstd (the gradient of X, and of R), dw = sum over rows of dY n, db = sum of
+ * dY, both of weight_type.  dH (the gradient that came to H itself), w, dX, dw and db may each be NULL.  The sums have a fixed order.  The workspace is
+ * 16-byte aligned; it is needed for dw and db. */
+size_t b200cp_layer_norm_bwd_workspace_bytes(int rows, int D);
+int b200cp_layer_norm_bwd(int rows, int D, int type, int weight_type, const void* dY, const void* dH, const void* H, const void* w,
+                          const float* mean, const float* rstd, void* dX, void* dw, void* db, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* ---- Muon step ------------------------------------------------------------------------------------------------------- */
+
+/* A stack of matrices [stack, rows, cols], each orthogonalised by itself (a size of 0: skipped).  momentum: floats of the same shape, zero before the
+ * first step.  master: the fp32 copy of a 16-bit parameter, or NULL. */
+typedef struct b200cp_muon_matrix {
+  void* param;
+  const void* grad;
+  float *momentum, *master;
+  int stack, rows, cols;
+} b200cp_muon_matrix;
+
+/* Factor of the rate: 1; sqrt(max(1, rows / cols)); 0.2 sqrt(max(rows, cols)). */
+enum { B200CP_MUON_PLAIN = 0, B200CP_MUON_ORIGINAL = 1, B200CP_MUON_MATCH_RMS_ADAMW = 2 };
+
+/* coefficients: triples (a, b, c), one for all steps or one for each (host memory).  device_lr (or NULL): lr as a float in device memory, read by the
+ * launch instead of `lr`. */
+typedef struct b200cp_muon {
+  double lr, momentum, weight_decay, eps;
+  int nesterov, steps, adjust, coefficient_count;
+  const double* coefficients;
+  const float* device_lr;
+} b200cp_muon;
+
+/* m = m + (1 - momentum)(g - m); u = g + momentum (m - g) with nesterov, else m; X = u / max(|u|_F, eps); `steps` times, on the smaller side of the matrix,
+ * A = X X^T, X = a X + (b A + c A^2) X; p = p - lr wd p - lr factor X.  In place.  param_type, grad_type: as in b200cp_adamw_step.  Results are fp32-grade (see
+ * csrc/muon.cu); coefficients that may raise a singular value above 100 are refused.  No two entries may overlap.  The workspace is
+ * 256-byte aligned.  Beside b200cp_adamw_step; no counterpart in the reference. */
+size_t b200cp_muon_step_workspace_bytes(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type);
+int b200cp_muon_step(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type, const b200cp_muon* hyper, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* out = X after the steps above, for a stack of matrices.  out and X have one type; out may not share memory with X.  The workspace is that of a
+ * step of one matrix of these sizes and types. */
+int b200cp_orthogonalise(int stack, int rows, int cols, int type, const void* X, void* out, const double* coefficients, int coefficient_count,
+                         int steps, double eps, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- misc --------------------------------------------------------------- */
 
 /* Synchronises the device and reports whether any tensor-path kernel gave up a bounded wait since

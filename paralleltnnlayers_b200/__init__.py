@@ -21,7 +21,9 @@ _OPS_NAMES = ("allclose", "CP3Conv2dFunction", "conv2d_cp_fused_nchw", "cp3_conv
               "cp4_conv2d_forward_save", "cp4_conv2d_backward_data_save", "cp4_conv2d_rebuild_forward", "rcp_recompose", "conv2d_rcp_rebuild_nchw",
               "dense_cp_recompose", "dense_matmul", "dense_cp_rebuild", "adamw_step", "adamw_moments",
               "AdapterPlan", "adapter_plan", "dense_adapters", "dense_adapters_backward", "DenseAdaptersFunction",
-              "dense_gated", "dense_gated_save", "dense_gated_backward", "DenseGatedFunction")
+              "dense_gated", "dense_gated_save", "dense_gated_backward", "DenseGatedFunction",
+              "embedding", "embedding_backward", "EmbeddingFunction", "layer_norm", "layer_norm_save", "layer_norm_backward", "LayerNormFunction",
+              "muon_step", "orthogonalise")
 __all__ = list(_LIB_NAMES + _OPS_NAMES)
 
 

@@ -112,6 +112,15 @@ def _load():
         "b200cp_dense_gated_bwd": (i, [i, i, i, i, i, vp, vp, vp, fp, fp, vp, vp, vp, vp, vp, sz, vp]),
         "b200cp_adamw_step": (i, [vp, i, i, i, i, vp, vp]),
         "b200cp_adamw_moments": (i, [C.c_ulonglong, vp, vp, fp, fp, i, vp, vp, vp]),
+        "b200cp_embedding": (i, [i, i, i, i, i, vp, vp, C.c_float, vp, vp]),
+        "b200cp_embedding_bwd_workspace_bytes": (sz, [i, i]),
+        "b200cp_embedding_bwd": (i, [i, i, i, i, i, vp, vp, C.c_float, vp, vp, sz, vp]),
+        "b200cp_layer_norm": (i, [i, i, i, i, vp, vp, vp, vp, C.c_float, vp, vp, fp, fp, vp]),
+        "b200cp_layer_norm_bwd_workspace_bytes": (sz, [i, i]),
+        "b200cp_layer_norm_bwd": (i, [i, i, i, i, vp, vp, vp, vp, fp, fp, vp, vp, vp, vp, sz, vp]),
+        "b200cp_muon_step_workspace_bytes": (sz, [vp, i, i, i]),
+        "b200cp_muon_step": (i, [vp, i, i, i, vp, vp, sz, vp]),
+        "b200cp_orthogonalise": (i, [i, i, i, i, vp, vp, C.POINTER(C.c_double), i, i, C.c_double, vp, sz, vp]),
         "b200cp_device_status": (i, []),
         "b200cp_last_error_string": (C.c_char_p, []),
         "b200cp_status_string": (C.c_char_p, [i]),

@@ -1,0 +1,1162 @@
+// The Muon step: the update of a matrix is its momentum, orthogonalised by Newton-Schulz products; and the orthogonalisation alone.
+//
+//   m <- m + (1 - b)(g - m),  u = g + b (m - g) (Nesterov) or m,  X = u / max(|u|_F, eps)
+//   per step, on the smaller side:  A = X X^T,  X <- a X + (b A + c A^2) X          (the polynomial a s + b s^3 + c s^5 of each singular value s)
+//   p <- p (1 - lr wd) - lr r X
+//
+// Two forms, by the smaller side n of a matrix.
+//
+// n <= 64 (factors, adapters): with P = a I + b A + c A^2, X goes to P X and A to P A P, and all of these are polynomials of the first A.  So the steps
+// are taken on n x n matrices, and X is touched twice: for A, and for the product of all P with it.  A has the squares of the singular values, and
+// noise in its small ones grows by a^2 a step, so this half is in 64 bits (half the rate of 32 on this GPU, and next to nothing beside the memory).  Three
+// launches for all such matrices of a call together.
+//
+// n > 64: X, A and B = b A + c A^2 are products on the tcgen05 tensor cores.  What is rounded: a value is held as two fp16 numbers (hi + rest, 22 bits)
+// times a power of two that the bound on the singular values gives, so that none overflows and the sums of a product are of hi hi + hi lo + lo hi; its
+// sums are fp32, at most 64 terms in an accumulator (the tensor core cuts sums off: over 4096 terms it loses 3e-5, where fp32 rounding loses 3e-7) and the
+// rest in registers.  One fp16 number would be three times as fast, but directions with small singular values are raised by 3.4445 a step: its 2^-12 comes
+// out as 7 % of a gradient of rank one.  a X is added in fp32.
+// A and B are symmetric: blocks below the diagonal are not computed, the others stored twice.  Either operand is taken in either order, so nothing is
+// transposed; where the rows are the longer side A = X^T X and X <- a X + X B.  Matrices of one shape share their launches.
+// Every wait is bounded: one that runs out sets a status word and the CTA leaves through its normal exit.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "common.cuh"
+#include "tc_common.cuh"
+#include "tc_pair.cuh"
+#include "vec_io.cuh"
+
+namespace b200cp {
+
+__device__ int g_muon_status = 0;   // 0 ok; otherwise (code << 16) | (linear block index & 0xffff)
+
+namespace {
+
+using namespace tc;
+
+struct Pointers {   // of one matrix
+  void* p;          // what is updated, or receives X
+  const void* g;
+  float *m, *w;     // momentum (null: u = g), float32 copy (or null)
+};
+struct Rates {
+  float keep, blend;        // b, 1 - b
+  int nesterov, update;     // update 0: p receives X itself
+  float lr, decay;          // lr, wd
+  const float* device_lr;   // or null
+  double eps;
+};
+template <typename G>
+__device__ __forceinline__ float momentum_of(const Rates& r, float g, float m) { return fmaf(r.blend, g - m, m); }
+__device__ __forceinline__ float direction_of(const Rates& r, float g, float m) { return r.nesterov ? fmaf(r.keep, m - g, g) : m; }
+__device__ __forceinline__ float rate_of(const Rates& r) { return r.device_lr ? *r.device_lr : r.lr; }
+// (what X stands for is far fewer bits than an fp32 value: the sum is rounded once)
+__device__ __forceinline__ float updated(float w, float x, float shrink, float rate) { return fmaf(-rate, x, w * shrink); }
+
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// ======== matrices with a side of at most 64 =====================================================================================
+constexpr int kSmall = 64, kTableSmall = 224, kSub = 128, kGramThreads = 288;
+struct SmallEntry {
+  Pointers at;
+  int rows, cols;
+  int stack;
+  int chunks, length;        // of a matrix: parts of its longer side, and how much of it each has (a multiple of kSub)
+  int first;                 // CTA of the launch over parts
+  int matrix;                // matrices before
+  float scale;               // of the rate
+  size_t gram, q;            // in doubles, in floats: of its first matrix
+};
+struct SmallTable {
+  Rates r;
+  int count, steps, coefficients;
+  double *gram, *inverse;
+  float* q;
+  SmallEntry e[kTableSmall];
+};
+struct Coefficients {
+  double v[3 * 100];
+};
+__device__ __forceinline__ int side_of(const SmallEntry& e) { return min(e.rows, e.cols); }
+template <typename F>
+__device__ __forceinline__ int entry_of(const SmallTable& t, int block, F first) {
+  int a = 0, b = t.count;
+  while (b - a > 1) {
+    const int c = (a + b) / 2;
+    if (first(t.e[c]) <= block) a = c; else b = c;
+  }
+  return a;
+}
+// Register tiles of TS x TS of the upper triangle of 16 x 16 of them
+__device__ __forceinline__ void tile_of(int t, int& ti, int& tj) {
+  ti = 0;
+  for (int left = 16; t >= left; --left, ++ti) t -= left;
+  tj = ti + t;
+}
+constexpr int kTiles = 136;
+
+// A part of A, in 64 bits, from a part of the longer side; the momentum is brought up to date on the way.
+template <typename G, int TS>
+__device__ __forceinline__ void gram_part(const SmallTable& t, const SmallEntry& e, int matrix, int chunk, double* u) {
+  constexpr int N = 16 * TS, LD = N + 2;
+  const int n = side_of(e), len = max(e.rows, e.cols), tid = threadIdx.x;
+  const bool wide = e.rows <= e.cols;
+  const size_t base = (size_t)matrix * e.rows * e.cols;
+  const G* g = static_cast<const G*>(e.at.g) + base;
+  float* m = e.at.m ? e.at.m + base : nullptr;
+  const int half = tid / 144, slot = tid - half * 144;
+  int ti = 0, tj = 0;
+  if (slot < kTiles) tile_of(slot, ti, tj);
+  double acc[TS][TS] = {};
+  const int l0 = chunk * e.length, l1 = min(len, l0 + e.length);
+  for (int i = tid; i < kSub * LD; i += kGramThreads) u[i] = 0.0;   // (rows past n stay zero)
+  for (int k0 = l0; k0 < l1; k0 += kSub) {
+    const int ks = min(kSub, l1 - k0);
+    __syncthreads();
+    for (int i = tid; i < n * kSub; i += kGramThreads) {
+      const int row = wide ? i / kSub : i % n, k = wide ? i % kSub : i / n;
+      double d = 0.0;
+      if (k < ks) {
+        const size_t at = wide ? (size_t)row * e.cols + k0 + k : (size_t)(k0 + k) * n + row;
+        float x = to_float(g[at]);
+        if (m) {
+          const float b = momentum_of<G>(t.r, x, m[at]);
+          m[at] = b;
+          x = direction_of(t.r, x, b);
+        }
+        d = (double)x;
+      }
+      u[k * LD + row] = d;
+    }
+    __syncthreads();
+    if (slot < kTiles) {
+#pragma unroll 2
+      for (int k = half; k < kSub; k += 2) {
+        double a[TS], b[TS];
+#pragma unroll
+        for (int i = 0; i < TS; ++i) {
+          a[i] = u[k * LD + ti * TS + i];
+          b[i] = u[k * LD + tj * TS + i];
+        }
+#pragma unroll
+        for (int i = 0; i < TS; ++i)
+#pragma unroll
+          for (int j = 0; j < TS; ++j) acc[i][j] = fma(a[i], b[j], acc[i][j]);
+      }
+    }
+  }
+  __syncthreads();
+  if (half == 1 && slot < kTiles) {
+#pragma unroll
+    for (int i = 0; i < TS; ++i)
+#pragma unroll
+      for (int j = 0; j < TS; ++j) u[slot * TS * TS + i * TS + j] = acc[i][j];
+  }
+  __syncthreads();
+  if (half == 0 && slot < kTiles) {   // [tile][TS][TS]
+    double* to = t.gram + e.gram + ((size_t)matrix * e.chunks + chunk) * (kTiles * TS * TS) + slot * TS * TS;
+#pragma unroll
+    for (int i = 0; i < TS * TS; ++i) to[i] = acc[i / TS][i % TS] + u[slot * TS * TS + i];
+  }
+}
+template <typename G>
+__global__ void __launch_bounds__(kGramThreads) muon_gram_kernel(const __grid_constant__ SmallTable t) {
+  extern __shared__ double work[];
+  grid_dependency_wait();
+  const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.first; })];
+  const int at = (int)blockIdx.x - e.first, matrix = at / e.chunks, chunk = at - matrix * e.chunks, n = side_of(e);
+  if (n <= 16) gram_part<G, 1>(t, e, matrix, chunk, work);
+  else if (n <= 32) gram_part<G, 2>(t, e, matrix, chunk, work);
+  else gram_part<G, 4>(t, e, matrix, chunk, work);
+}
+
+// out = x y, all symmetric and commuting: only tiles on and above the diagonal are formed.  Rows of N doubles.
+template <int TS>
+__device__ __forceinline__ void symmetric_product(const double* x, const double* y, double* out) {
+  constexpr int N = 16 * TS;
+  const int t = threadIdx.x;
+  if (t < kTiles) {
+    int ti, tj;
+    tile_of(t, ti, tj);
+    double acc[TS][TS] = {};
+#pragma unroll 4
+    for (int k = 0; k < N; ++k) {
+      double a[TS], b[TS];
+#pragma unroll
+      for (int i = 0; i < TS; ++i) {
+        a[i] = x[k * N + ti * TS + i];
+        b[i] = y[k * N + tj * TS + i];
+      }
+#pragma unroll
+      for (int i = 0; i < TS; ++i)
+#pragma unroll
+        for (int j = 0; j < TS; ++j) acc[i][j] = fma(a[i], b[j], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < TS; ++i)
+#pragma unroll
+      for (int j = 0; j < TS; ++j) {
+        out[(ti * TS + i) * N + tj * TS + j] = acc[i][j];
+        out[(tj * TS + j) * N + ti * TS + i] = acc[i][j];
+      }
+  }
+  __syncthreads();
+}
+template <int TS>
+__device__ __forceinline__ void iterate(const SmallTable& t, const Coefficients& co, const SmallEntry& e, int matrix, double* work) {
+  constexpr int N = 16 * TS, NN = N * N, T2 = TS * TS;
+  const int tid = threadIdx.x, n = side_of(e);
+  double *A = work, *P = A + NN, *Q = P + NN, *S = Q + NN;
+  __shared__ double trace_sum;
+  // the parts of A, in their order
+  const double* from = t.gram + e.gram + (size_t)matrix * e.chunks * (kTiles * T2);
+  for (int i = tid; i < kTiles * T2; i += 256) {
+    double s = 0.0;
+#pragma unroll 4
+    for (int c = 0; c < e.chunks; ++c) s += from[(size_t)c * (kTiles * T2) + i];
+    int ti, tj;
+    tile_of(i / T2, ti, tj);
+    const int r = ti * TS + (i % T2) / TS, c = tj * TS + i % TS;
+    A[r * N + c] = s;
+    A[c * N + r] = s;
+  }
+  __syncthreads();
+  if (tid < 32) {
+    double s = 0.0;
+    for (int i = tid; i < n; i += 32) s += A[i * N + i];
+    s = warp_sum(s);
+    if (tid == 0) trace_sum = s;
+  }
+  __syncthreads();
+  const double root = sqrt(trace_sum), inverse = 1.0 / (root > t.r.eps || root != root ? root : t.r.eps);
+  for (int i = tid; i < NN; i += 256) {
+    A[i] *= inverse * inverse;
+    Q[i] = i / N == i % N ? 1.0 : 0.0;
+  }
+  __syncthreads();
+  for (int step = 0; step < t.steps; ++step) {
+    const double* v = co.v + (t.coefficients > 1 ? 3 * step : 0);
+    symmetric_product<TS>(A, A, P);
+    for (int i = tid; i < NN; i += 256) P[i] = fma(v[2], P[i], fma(v[1], A[i], i / N == i % N ? v[0] : 0.0));
+    __syncthreads();
+    if (step == 0) {
+      for (int i = tid; i < NN; i += 256) Q[i] = P[i];
+      __syncthreads();
+    } else {
+      symmetric_product<TS>(Q, P, S);
+      double* q = Q;
+      Q = S;
+      S = q;
+    }
+    if (step + 1 == t.steps) break;
+    symmetric_product<TS>(A, P, S);
+    symmetric_product<TS>(S, P, A);
+  }
+  float* to = t.q + e.q + (size_t)matrix * (n * n);
+  for (int i = tid; i < n * n; i += 256) to[i] = (float)Q[i / n * N + i % n];
+  if (tid == 0) t.inverse[e.matrix + matrix] = inverse;
+}
+__global__ void __launch_bounds__(256) muon_iterate_kernel(const __grid_constant__ SmallTable t, const __grid_constant__ Coefficients co) {
+  extern __shared__ double work[];
+  grid_dependency_wait();
+  const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.matrix; })];
+  const int matrix = (int)blockIdx.x - e.matrix, n = side_of(e);
+  if (n <= 16) iterate<1>(t, co, e, matrix, work);
+  else if (n <= 32) iterate<2>(t, co, e, matrix, work);
+  else iterate<4>(t, co, e, matrix, work);
+}
+
+// X = Q u / |u| for a part of the longer side, and the update.
+template <typename P, typename G>
+__global__ void __launch_bounds__(256) muon_small_apply_kernel(const __grid_constant__ SmallTable t) {
+  extern __shared__ float low[];
+  constexpr int LD = kSub + 1;
+  float *q = low, *x = q + kSmall * kSmall, *o = x + kSmall * LD;   // [j][i], [j][k], [i][k]
+  grid_dependency_wait();
+  const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.first; })];
+  const int at0 = (int)blockIdx.x - e.first, matrix = at0 / e.chunks, chunk = at0 - matrix * e.chunks, n = side_of(e), len = max(e.rows, e.cols);
+  const int tid = threadIdx.x, ld = (n + 7) / 8 * 8;
+  const bool wide = e.rows <= e.cols;
+  const size_t base = (size_t)matrix * e.rows * e.cols;
+  const G* g = static_cast<const G*>(e.at.g) + base;
+  const float* m = e.at.m ? e.at.m + base : nullptr;
+  float* w = e.at.w ? e.at.w + base : nullptr;
+  P* p = static_cast<P*>(e.at.p) + base;
+  const float* from = t.q + e.q + (size_t)matrix * (n * n);
+  const double inverse = t.inverse[e.matrix + matrix];
+  const float lr = rate_of(t.r), rate = lr * e.scale, shrink = 1.f - lr * t.r.decay;
+  for (int i = tid; i < n * ld; i += 256) q[i] = i % ld < n ? from[i / ld * n + i % ld] : 0.f;
+  const int l0 = chunk * e.length, l1 = min(len, l0 + e.length);
+  for (int k0 = l0; k0 < l1; k0 += kSub) {
+    const int ks = min(kSub, l1 - k0);
+    __syncthreads();
+    for (int i = tid; i < n * kSub; i += 256) {
+      const int row = wide ? i / kSub : i % n, k = wide ? i % kSub : i / n;
+      float v = 0.f;
+      if (k < ks) {
+        const size_t at = wide ? (size_t)row * e.cols + k0 + k : (size_t)(k0 + k) * n + row;
+        v = to_float(g[at]);
+        if (m) v = direction_of(t.r, v, m[at]);
+        v = (float)((double)v * inverse);
+      }
+      x[row * LD + k] = v;
+    }
+    __syncthreads();
+    const int k = tid & (kSub - 1);
+    for (int i0 = tid / kSub * 8; i0 < n; i0 += 16) {
+      float acc[8] = {};
+      for (int j = 0; j < n; ++j) {
+        const float v = x[j * LD + k];
+        const float4 a = *reinterpret_cast<const float4*>(q + j * ld + i0), b = *reinterpret_cast<const float4*>(q + j * ld + i0 + 4);
+        acc[0] = fmaf(a.x, v, acc[0]); acc[1] = fmaf(a.y, v, acc[1]); acc[2] = fmaf(a.z, v, acc[2]); acc[3] = fmaf(a.w, v, acc[3]);
+        acc[4] = fmaf(b.x, v, acc[4]); acc[5] = fmaf(b.y, v, acc[5]); acc[6] = fmaf(b.z, v, acc[6]); acc[7] = fmaf(b.w, v, acc[7]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < n) o[(i0 + i) * LD + k] = acc[i];
+    }
+    __syncthreads();
+    for (int i = tid; i < n * kSub; i += 256) {
+      const int row = wide ? i / kSub : i % n, c = wide ? i % kSub : i / n;
+      if (c >= ks) continue;
+      const size_t at = wide ? (size_t)row * e.cols + k0 + c : (size_t)(k0 + c) * n + row;
+      float v = o[row * LD + c];
+      if (t.r.update) {
+        v = updated(w ? w[at] : to_float(p[at]), v, shrink, rate);
+        if (w) w[at] = v;
+      }
+      p[at] = from_float<P>(v);
+    }
+  }
+}
+
+// ======== larger matrices ===========================================================================================================
+constexpr int kBatch = 96, kNormParts = 128;   // matrices of one shape that share launches; parts of a norm
+struct Batch {
+  Rates r;
+  int count, rows, cols, ld;      // ld: of the planes, a multiple of eight
+  size_t plane, matrix;           // halves from one plane, one matrix to the next
+  float scale, rate;              // planes hold scale X; of the rate
+  __half* x;
+  double* norms;                  // [matrix][part]
+  int parts, vec;                 // vec: eight values of every array lie on its boundary, and rows are multiples of eight
+  Pointers at[kBatch];
+};
+
+// Momentum, and a part of |u|^2 in 64 bits.  grid (parts, matrices)
+template <typename G>
+__global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constant__ Batch b) {
+  grid_dependency_wait();
+  const Pointers& at = b.at[blockIdx.y];
+  const G* g = static_cast<const G*>(at.g);
+  const long long n = (long long)b.rows * b.cols;
+  double s = 0.0;
+  if (b.vec) {
+#pragma unroll 2
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long long)b.parts * 256 * 8) {
+      float x[8], m[8];
+#pragma unroll
+      for (int h = 0; h < 8; h += kPerLoad<G>) {
+        float y[kPerLoad<G>];
+        unpack(load_group<G, kPerLoad<G>>(g + i + h), y);
+#pragma unroll
+        for (int k = 0; k < kPerLoad<G>; ++k) x[h + k] = y[k];
+      }
+      if (at.m) {
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(m + h) = *reinterpret_cast<const float4*>(at.m + i + h);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          m[k] = momentum_of<G>(b.r, x[k], m[k]);
+          x[k] = direction_of(b.r, x[k], m[k]);
+        }
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(at.m + i + h) = *reinterpret_cast<const float4*>(m + h);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s = fma((double)x[k], (double)x[k], s);
+    }
+  } else {
+#pragma unroll 4
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)b.parts * 256) {
+      float x = to_float(g[i]);
+      if (at.m) {
+        const float m = momentum_of<G>(b.r, x, at.m[i]);
+        at.m[i] = m;
+        x = direction_of(b.r, x, m);
+      }
+      s = fma((double)x, (double)x, s);
+    }
+  }
+  __shared__ double red[8];
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[i];
+    b.norms[blockIdx.y * kNormParts + blockIdx.x] = s;
+  }
+}
+__device__ __forceinline__ void split8(const float (&v)[8], Group<__half, 8>& hi, Group<__half, 8>& lo) {
+  float r[8];
+  hi = pack<__half>(v);
+  unpack(hi, r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = v[i] - r[i];
+  lo = pack<__half>(r);
+}
+// The planes of X.  Eight columns per thread and turn.
+template <typename G>
+__global__ void __launch_bounds__(256) muon_planes_kernel(const __grid_constant__ Batch b) {
+  __shared__ double inverse;
+  grid_dependency_wait();
+  if (threadIdx.x < 32) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < b.parts; i += 32) s += b.norms[blockIdx.y * kNormParts + i];
+    s = sqrt(warp_sum(s));
+    if (threadIdx.x == 0) inverse = (double)b.scale / (s > b.r.eps || s != s ? s : b.r.eps);
+  }
+  __syncthreads();
+  const double inv = inverse;
+  const Pointers& at = b.at[blockIdx.y];
+  const G* g = static_cast<const G*>(at.g);
+  __half* to = b.x + blockIdx.y * b.matrix;
+  const int per = b.ld / 8;
+  const long long n = (long long)b.rows * per;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long row = i / per;
+    const int c = (int)(i - row * per) * 8;
+    const size_t src = (size_t)row * b.cols + c;
+    float x[8], m[8];
+    if (b.vec) {
+#pragma unroll
+      for (int h = 0; h < 8; h += kPerLoad<G>) {
+        float y[kPerLoad<G>];
+        unpack(load_group<G, kPerLoad<G>>(g + src + h), y);
+#pragma unroll
+        for (int k = 0; k < kPerLoad<G>; ++k) x[h + k] = y[k];
+      }
+      if (at.m)
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(m + h) = *reinterpret_cast<const float4*>(at.m + src + h);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[k] = c + k < b.cols ? to_float(g[src + k]) : 0.f;
+        m[k] = at.m && c + k < b.cols ? at.m[src + k] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (at.m) x[k] = direction_of(b.r, x[k], m[k]);
+      x[k] = (float)((double)x[k] * inv);
+    }
+    Group<__half, 8> hi, lo;
+    split8(x, hi, lo);
+    store_group(to + row * b.ld + c, hi);
+    store_group(to + b.plane + row * b.ld + c, lo);
+  }
+}
+// The update from the planes of the last X.
+template <typename P>
+__global__ void __launch_bounds__(256) muon_apply_kernel(const __grid_constant__ Batch b) {
+  grid_dependency_wait();
+  const Pointers& at = b.at[blockIdx.y];
+  P* p = static_cast<P*>(at.p);
+  const __half* from = b.x + blockIdx.y * b.matrix;
+  const float lr = rate_of(b.r), rate = lr * b.rate, shrink = 1.f - lr * b.r.decay, unit = 1.f / b.scale;
+  const int per = b.ld / 8;
+  const long long n = (long long)b.rows * per;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long row = i / per;
+    const int c = (int)(i - row * per) * 8;
+    const size_t dst = (size_t)row * b.cols + c;
+    float x[8], l[8], w[8];
+    unpack(load_group<__half, 8>(from + row * b.ld + c), x);
+    unpack(load_group<__half, 8>(from + b.plane + row * b.ld + c), l);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = (x[k] + l[k]) * unit;
+    if (b.r.update) {
+      if (b.vec) {
+        if (at.w) {
+#pragma unroll
+          for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(w + h) = *reinterpret_cast<const float4*>(at.w + dst + h);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 8; h += kPerLoad<P>) {
+            float y[kPerLoad<P>];
+            unpack(load_group<P, kPerLoad<P>>(p + dst + h), y);
+#pragma unroll
+            for (int k = 0; k < kPerLoad<P>; ++k) w[h + k] = y[k];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = c + k < b.cols ? (at.w ? at.w[dst + k] : to_float(p[dst + k])) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = updated(w[k], x[k], shrink, rate);
+    }
+    if (b.vec) {
+      if (at.w && b.r.update) {
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(at.w + dst + h) = *reinterpret_cast<const float4*>(x + h);
+      }
+#pragma unroll
+      for (int h = 0; h < 8; h += kPerLoad<P>) {
+        float y[kPerLoad<P>];
+#pragma unroll
+        for (int k = 0; k < kPerLoad<P>; ++k) y[k] = x[h + k];
+        store_group(p + dst + h, pack<P>(y));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (c + k >= b.cols) break;
+        if (at.w && b.r.update) at.w[dst + k] = x[k];
+        p[dst + k] = from_float<P>(x[k]);
+      }
+    }
+  }
+}
+
+// ---- the products ------------------------------------------------------------------------------------------------------------------
+// out = alpha sum_k L[m][k] R[n][k] + beta add, of planes, for a batch of matrices.  A pair of CTAs has a tile of 256 x BN; the shape is that of the
+// split products of gemm_tc.cu: 64 k of both planes in a stage, one thread issues, accumulators in turn, totals in registers.
+constexpr int kStep = 64, kGroup = 16;
+template <int BN>
+struct Tile {
+  static constexpr int aplane = 128 * kStep * 2, bplane = BN / 2 * kStep * 2;
+  static constexpr int abytes = 2 * aplane, stage = abytes + 2 * bplane;      // 64 or 48 KB
+  static constexpr int stages = BN == 256 ? 3 : 4, depth = BN == 256 ? 2 : 4; // of the ring; accumulators
+  static constexpr int readers = 4 * BN / 64, threads = 64 + 32 * readers;
+  static constexpr size_t smem = (size_t)stages * stage + 1024 + 256;
+  static_assert(smem <= 227 * 1024 && depth * BN == 512, "");
+};
+struct Newton {
+  int M, N, K, steps;            // of a result, of a sum
+  int tiles_m, tiles_n, per, units;
+  int symmetric;
+  float alpha, beta;
+  const __half* add;             // planes as out's, or null
+  __half* out;
+  int ld;
+  size_t plane, matrix;
+};
+struct UnitAt {
+  int matrix, m0, n0;
+  bool mirror;
+};
+template <int BN>
+__device__ __forceinline__ UnitAt unit_at(const Newton& g, int unit) {
+  const int i = unit / g.per;
+  int t = unit - i * g.per;
+  if (g.symmetric) {             // rows of blocks, each from its diagonal on
+    constexpr int q = 256 / BN;
+    int row = 0, left = g.tiles_n;
+    while (t >= left) {
+      t -= left;
+      left -= q;
+      ++row;
+    }
+    const int n0 = (row * q + t) * BN;
+    return UnitAt{i, row * 256, n0, n0 >= (row + 1) * 256};
+  }
+  const int band = t / (kGroup * g.tiles_n), m1 = band * kGroup, height = min(kGroup, g.tiles_m - m1), q = t - m1 * g.tiles_n;
+  return UnitAt{i, (m1 + q % height) * 256, (q / height) * BN, false};
+}
+__device__ __forceinline__ void tma_load_planes(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int matrix) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(0), "r"(matrix)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"f"(v[0]),
+      "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+      "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "r"(taddr)
+      : "memory");
+}
+
+// L_MN, R_MN: the operand lies as [k][row] (boxes of 64 rows x 64 k), else as [row][k].
+template <int BN, bool L_MN, bool R_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN>::threads, 1)
+newton_kernel(const __grid_constant__ Newton g, const __grid_constant__ CUtensorMap mapL, const __grid_constant__ CUtensorMap mapR) {
+  using T = Tile<BN>;
+  constexpr int kStages = T::stages, kBox = 2 * kStep * 128;   // bytes of an MN-major box, both planes
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kStages * T::stage);
+  uint64_t* full = bars;                 // [kStages] the leader's: the stage of both CTAs has landed  (tx bytes)
+  uint64_t* empty = full + kStages;      // [kStages] the products that read the stage are done         (commit, both CTAs)
+  uint64_t* accfull = empty + kStages;   // [depth] the accumulator is complete                         (commit, both CTAs)
+  uint64_t* accfree = accfull + 4;       // [depth] the leader's: read out by the warps of both CTAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accfree + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < T::depth; ++i) {
+      mbar_init(&accfull[i], 1);
+      mbar_init(&accfree[i], 2 * T::readers);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&mapL);
+    tma_prefetch_desc(&mapR);
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t fullb = smem_u32(full), emptyb = smem_u32(empty), accfullb = smem_u32(accfull), accfreeb = smem_u32(accfree),
+                 abortb = smem_u32(const_cast<int*>(abort_flag));
+  grid_dependency_wait();
+
+  if (warp == 0) {
+    // ================= TMA: this CTA's rows of L and its half of the rows of R ==============================================
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int unit = pair; unit < g.units && ok; unit += npairs) {
+        const UnitAt t = unit_at<BN>(g, unit);
+        for (int s = 0; s < g.steps; ++s, ++it) {
+          const int slot = it % kStages;
+          if (it >= kStages && !(ok = wait_or_abort(emptyb + slot * 8, ((it / kStages) - 1) & 1, abortb))) break;
+          if (rank == 0) mbar_expect_tx(&full[slot], 2 * T::stage);
+          const uint32_t bar = leader_addr(fullb + slot * 8), a = smem_u32(sm) + slot * T::stage, b = a + T::abytes;
+          const int m = t.m0 + rank * 128, n = t.n0 + rank * (BN / 2), k = s * kStep;
+          if (L_MN) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) tma_load_planes(a + q * kBox, &mapL, bar, m + q * 64, k, t.matrix);
+          } else {
+            tma_load_planes(a, &mapL, bar, k, m, t.matrix);
+          }
+          if (R_MN) {
+#pragma unroll
+            for (int q = 0; q < BN / 128; ++q) tma_load_planes(b + q * kBox, &mapR, bar, n + q * 64, k, t.matrix);
+          } else {
+            tma_load_planes(b, &mapR, bar, k, n, t.matrix);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ================= products: one thread of the pair ======================================================================
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = (1u << 4) | ((L_MN ? 1u : 0u) << 15) | ((R_MN ? 1u : 0u) << 16) | (((uint32_t)BN >> 3) << 17) | ((256u >> 4) << 24);
+      // K-major: rows of 128 bytes, eight rows per swizzle atom (1024 bytes); 16 k = 32 bytes on; the second plane all rows on.
+      // MN-major: 64 rows (128 bytes) per k, eight k per atom, the next 64 rows a box on; 16 k = 2048 bytes on; the second plane 64 k on.
+      const uint64_t dl = make_smem_desc(0, L_MN ? kBox : 16, 1024, kSwizzle128B), dr = make_smem_desc(0, R_MN ? kBox : 16, 1024, kSwizzle128B);
+      constexpr uint64_t sl = (L_MN ? 2048 : 32) >> 4, sr = (R_MN ? 2048 : 32) >> 4;
+      constexpr uint64_t pl = (L_MN ? kStep * 128 : T::aplane) >> 4, pr = (R_MN ? kStep * 128 : T::bplane) >> 4;
+      int it = 0;
+      bool ok = true;
+      for (int unit = pair; unit < g.units && ok; unit += npairs) {
+        for (int s = 0; s < g.steps; ++s, ++it) {
+          const int slot = it % kStages, buf = it % T::depth;
+          if (!(ok = wait_or_abort(fullb + slot * 8, (it / kStages) & 1, abortb))) break;
+          if (it >= T::depth && !(ok = wait_or_abort(accfreeb + buf * 8, (it / T::depth - 1) & 1, abortb))) break;
+          tc_fence_after_sync();
+          const uint32_t a = smem_u32(sm) + slot * T::stage, d = tmem_base + buf * BN;
+          const uint64_t l = dl + (a >> 4), r = dr + ((a + T::abytes) >> 4);
+#pragma unroll
+          for (int i = 0; i < kStep / 16; ++i) {   // the small products first
+            mma_f16_pair(d, l + pl + i * sl, r + i * sr, idesc, i > 0);
+            mma_f16_pair(d, l + i * sl, r + pr + i * sr, idesc, true);
+          }
+#pragma unroll
+          for (int i = 0; i < kStep / 16; ++i) mma_f16_pair(d, l + i * sl, r + i * sr, idesc, true);
+          commit_pair(accfullb + buf * 8);
+          commit_pair(emptyb + slot * 8);
+        }
+      }
+    }
+  } else {
+    // ================= read-out: accumulators -> totals -> planes =============================================================
+    const int qd = warp & 3, c0 = ((warp - 2) >> 2) * 64;   // the lane quarter that this warp may read, and its columns
+    const uint32_t taddr = tmem_base + ((uint32_t)(qd * 32) << 16) + c0;
+    int it = 0;
+    bool ok = true;
+    for (int unit = pair; unit < g.units && ok; unit += npairs) {
+      float tot[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) tot[j] = 0.f;
+      int buf = 0;
+      for (int s = 0; s < g.steps; ++s, ++it) {
+        buf = it % T::depth;
+        if (!(ok = __all_sync(0xffffffffu, wait_or_abort(accfullb + buf * 8, (it / T::depth) & 1, abortb)))) break;
+        tc_fence_after_sync();
+#pragma unroll
+        for (int j0 = 0; j0 < 64; j0 += 16) {
+          float v[16];
+          tmem_ld16(taddr + buf * BN + j0, v);
+          if (j0 == 48 && s + 1 < g.steps) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) tot[j0 + j] += v[j];
+        }
+      }
+      if (!ok) break;
+      // through the accumulator just read, so that a short loop stores them (unrolled over registers it is code that every tile fetches anew)
+#pragma unroll
+      for (int j0 = 0; j0 < 64; j0 += 16) tmem_st16(taddr + buf * BN + j0, tot + j0);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      const UnitAt t = unit_at<BN>(g, unit);
+      const int m = t.m0 + rank * 128 + qd * 32 + lane;
+      const size_t base = t.matrix * g.matrix, row = base + (size_t)m * g.ld;
+#pragma unroll 1
+      for (int j0 = 0; j0 < 64; j0 += 8) {
+        const int n = t.n0 + c0 + j0;
+        float v[8];
+        tmem_ld8(taddr + buf * BN + j0, v);
+        if (n >= g.N || m >= g.M) continue;
+        if (g.add) {
+          float x[8], y[8];
+          unpack(load_group<__half, 8>(g.add + row + n), x);
+          unpack(load_group<__half, 8>(g.add + row + n + g.plane), y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = fmaf(g.alpha, v[j], g.beta * (x[j] + y[j]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] *= g.alpha;
+        }
+        Group<__half, 8> hi, lo;
+        split8(v, hi, lo);
+        store_group(g.out + row + n, hi);   // (the row's padding too)
+        store_group(g.out + row + n + g.plane, lo);
+        if (t.mirror) {   // neighbouring lanes have neighbouring columns of these
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (n + j < g.N) {
+              __half* to = g.out + base + (size_t)(n + j) * g.ld + m;
+              to[0] = hi.v[j];
+              to[g.plane] = lo.v[j];
+            }
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) {
+    atomicCAS(&g_muon_status, 0, (1 << 16) | (blockIdx.x & 0xffff));
+    const long long t0 = clock64();   // copies in flight land before the shared memory is given back
+    while (clock64() - t0 < 40000000ll) {
+    }
+  }
+  cluster_sync();   // the peer's products read this CTA's shared memory, and its commits arrive on its barriers
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ======== host ======================================================================================================================
+struct Planes {   // of a batch of matrices
+  __half* p;
+  int rows, cols, ld, count;
+  size_t plane() const { return (size_t)rows * ld; }
+  size_t matrix() const { return 2 * plane(); }
+};
+int ld8(int n) { return (n + 7) / 8 * 8; }
+int encode(CUtensorMap* map, const Planes& m, int box_rows) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (!enc) return fail(B200CP_ERR_NO_DEVICE, "cuTensorMapEncodeTiled entry point not available");
+  const cuuint64_t dim[4] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, 2, (cuuint64_t)m.count},
+                   stride[3] = {(cuuint64_t)m.ld * 2, (cuuint64_t)m.plane() * 2, (cuuint64_t)m.matrix() * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 2, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult cr = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, m.p, dim, stride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (cr != CUDA_SUCCESS) return fail(B200CP_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)cr);
+  return B200CP_OK;
+}
+int units_of(int M, int N, int BN, bool symmetric) {   // of one matrix
+  const int tm = ceil_div(M, 256), tn = ceil_div(N, BN), q = 256 / BN;
+  return symmetric ? tm * tn - q * tm * (tm - 1) / 2 : tm * tn;
+}
+template <int BN, bool L_MN, bool R_MN>
+int product_of(Newton g, const Planes& L, const Planes& R, const Planes& out, bool symmetric, int pairs, cudaStream_t st) {
+  using T = Tile<BN>;
+  CUtensorMap ml, mr;
+  if (int rc = encode(&ml, L, L_MN ? kStep : 128)) return rc;
+  if (int rc = encode(&mr, R, R_MN ? kStep : BN / 2)) return rc;
+  g.symmetric = symmetric;
+  g.tiles_m = ceil_div(g.M, 256);
+  g.tiles_n = ceil_div(g.N, BN);
+  g.per = units_of(g.M, g.N, BN, symmetric);
+  g.units = g.per * out.count;
+  g.steps = ceil_div(g.K, kStep);
+  const auto kern = newton_kernel<BN, L_MN, R_MN>;
+  static std::atomic<int> set[64];
+  B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, (int)T::smem));
+  B200CP_CUDA_OK(launch_kernel(kern, dim3(2 * std::min(g.units, pairs)), dim3(T::threads), T::smem, st, true, g, ml, mr));
+  B200CP_LAUNCH_OK("newton_kernel");
+  return B200CP_OK;
+}
+// out = alpha L R^T + beta add.  Tiles of 256 columns, or of 128 where there are not two of the wider ones for every pair of CTAs.
+template <bool L_MN, bool R_MN>
+int product(const Planes& L, const Planes& R, int K, float alpha, float beta, const Planes* add, const Planes& out, bool symmetric, cudaStream_t st) {
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  const int pairs = di.sm_count / 2;
+  Newton g{};
+  g.M = out.rows; g.N = out.cols; g.K = K;
+  g.alpha = alpha; g.beta = beta;
+  g.add = add ? add->p : nullptr;
+  g.out = out.p; g.ld = out.ld; g.plane = out.plane(); g.matrix = out.matrix();
+  if ((long long)units_of(g.M, g.N, 256, symmetric) * out.count >= 2LL * pairs) return product_of<256, L_MN, R_MN>(g, L, R, out, symmetric, pairs, st);
+  return product_of<128, L_MN, R_MN>(g, L, R, out, symmetric, pairs, st);
+}
+
+// ---- bounds on the singular values, and the scales of the planes that follow ----------------------------------------------------------
+double grown(double bound, const double* v) {   // the largest |a s + b s^3 + c s^5| for s up to bound
+  const auto at = [&](double y) { return std::fabs(std::sqrt(y) * (v[0] + y * (v[1] + y * v[2]))); };
+  double most = at(bound * bound);
+  const double A = 5 * v[2], B = 3 * v[1], C = v[0], D = B * B - 4 * A * C;   // of the derivative in y = s^2
+  const auto look = [&](double y) {
+    if (y > 0 && y < bound * bound) most = std::max(most, at(y));
+  };
+  if (A == 0) {
+    if (B != 0) look(-C / B);
+  } else if (D >= 0) {
+    look((-B + std::sqrt(D)) / (2 * A));
+    look((-B - std::sqrt(D)) / (2 * A));
+  }
+  return most;
+}
+double room_for(double bound) { return std::ldexp(1.0, 15 - (int)std::ceil(std::log2(bound))); }   // bound times it is at most 2^15
+struct Plan {
+  int steps, coefficients;
+  const double* v;
+  double bound[101];
+};
+int plan_of(const char* who, const b200cp_muon* h, Plan* p) {
+  if (h->steps < 0 || h->steps > 100 || (h->steps && !h->coefficients) || (h->coefficient_count != 1 && h->coefficient_count != h->steps))
+    return fail(B200CP_ERR_INVALID_ARG, "%s: %d steps (0 to 100) with %d triples of coefficients (1, or one for each step)", who, h->steps, h->coefficient_count);
+  if (!(h->momentum >= 0 && h->momentum <= 1 && h->eps > 0)) return fail(B200CP_ERR_INVALID_ARG, "%s: momentum %g or eps %g out of range", who, h->momentum, h->eps);
+  p->steps = h->steps;
+  p->coefficients = h->coefficient_count;
+  p->v = h->coefficients;
+  p->bound[0] = 1.01;   // (a hundredth for what is rounded)
+  for (int s = 0; s < p->steps; ++s) {
+    const double b = grown(p->bound[s], p->v + (p->coefficients > 1 ? 3 * s : 0)) * 1.01;
+    if (!(b <= 100.0)) return fail(B200CP_ERR_UNSUPPORTED, "%s: these coefficients may raise a singular value above 100 in step %d", who, s + 1);
+    p->bound[s + 1] = std::max(b, 1e-3);
+  }
+  return B200CP_OK;
+}
+
+// ---- which matrices go together --------------------------------------------------------------------------------------------------------
+bool small(const b200cp_muon_matrix& a) { return std::min(a.rows, a.cols) <= kSmall; }
+int tile_side(int n) { return n <= 16 ? 1 : n <= 32 ? 2 : 4; }
+struct SmallSizes {
+  size_t doubles = 0, floats = 0;
+  int matrices = 0, ctas = 0;
+};
+// Parts of a matrix: as long as leaves the GPU four CTAs for each SM over all of the call's matrices, so that there are few parts to be added.
+void cut_small(const b200cp_muon_matrix& a, long long all, int sm_count, SmallEntry* e, SmallSizes* s) {
+  const int n = std::min(a.rows, a.cols), len = std::max(a.rows, a.cols), subs = ceil_div(len, kSub), ts = tile_side(n);
+  const int parts = (int)std::min<long long>(subs, std::max<long long>(1, 4LL * sm_count / std::max<long long>(1, all)));
+  e->rows = a.rows; e->cols = a.cols; e->stack = a.stack;
+  e->length = ceil_div(subs, parts) * kSub;
+  e->chunks = ceil_div(len, e->length);
+  e->first = s->ctas;
+  e->matrix = s->matrices;
+  e->gram = s->doubles;
+  e->q = s->floats;
+  s->ctas += e->chunks * a.stack;
+  s->matrices += a.stack;
+  s->doubles += (size_t)a.stack * e->chunks * (kTiles * ts * ts);
+  s->floats += (size_t)a.stack * n * n;
+}
+size_t small_bytes(const SmallSizes& s) {
+  return align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256) + align_up(s.floats * 4, 256);
+}
+// Small matrices of a launch: tensors from `at` on, up to a table's size and 2^20 CTAs.
+int next_small(const std::vector<b200cp_muon_matrix>& ms, size_t at, long long all, int sm_count, SmallTable* t, SmallSizes* s) {
+  int count = 0;
+  while (at + count < ms.size() && count < kTableSmall && s->ctas < (1 << 20)) {
+    SmallEntry e{};
+    cut_small(ms[at + count], all, sm_count, &e, s);
+    const b200cp_muon_matrix& a = ms[at + count];
+    e.at = Pointers{a.param, a.grad, a.momentum, a.master};
+    if (t) t->e[count] = e;
+    ++count;
+  }
+  return count;
+}
+struct Shape {
+  int rows, cols;
+  std::vector<Pointers> at;
+};
+size_t type_size(int type) { return type == B200CP_FLOAT32 ? 4 : 2; }
+struct Work {
+  std::vector<b200cp_muon_matrix> little;
+  long long matrices = 0;   // small ones
+  std::vector<Shape> large;
+  Work(const b200cp_muon_matrix* ms, int count, int ptype, int gtype) {
+    for (int i = 0; i < count; ++i) {
+      const b200cp_muon_matrix& a = ms[i];
+      if (a.stack < 1 || a.rows < 1 || a.cols < 1) continue;
+      if (small(a)) {
+        little.push_back(a);
+        matrices += a.stack;
+        continue;
+      }
+      auto s = std::find_if(large.begin(), large.end(), [&](const Shape& q) { return q.rows == a.rows && q.cols == a.cols; });
+      if (s == large.end()) {
+        large.push_back(Shape{a.rows, a.cols, {}});
+        s = large.end() - 1;
+      }
+      const size_t n = (size_t)a.rows * a.cols;
+      for (int k = 0; k < a.stack; ++k) {
+        const auto on = [&](auto* p, size_t size) { return p ? (decltype(p))((char*)p + k * n * size) : p; };
+        s->at.push_back(Pointers{on(a.param, type_size(ptype)), on(a.grad, type_size(gtype)), on(a.momentum, 4), on(a.master, 4)});
+      }
+    }
+  }
+};
+// Matrices of a shape that share launches: as many as give each pair of CTAs eight tiles of X, within a gigabyte of planes.
+int batch_of(const Shape& s) {
+  const int tiles = ceil_div(s.rows, 256) * ceil_div(s.cols, 256);
+  const size_t each = 8 * ((size_t)s.rows * ld8(s.cols) + (size_t)std::min(s.rows, s.cols) * ld8(std::min(s.rows, s.cols)));
+  const size_t room = std::max<size_t>(1, ((size_t)1 << 30) / each);
+  return (int)std::min<size_t>(std::min<size_t>(s.at.size(), kBatch), std::min<size_t>(room, (size_t)std::max(1, ceil_div(600, tiles))));
+}
+struct LargeSizes {
+  size_t x, a, norms, all;
+};
+LargeSizes large_sizes(const Shape& s, int count) {
+  const size_t n = std::min(s.rows, s.cols);
+  LargeSizes z;
+  z.x = align_up((size_t)count * 2 * s.rows * ld8(s.cols) * 2, 256);
+  z.a = align_up((size_t)count * 2 * n * ld8((int)n) * 2, 256);
+  z.norms = align_up((size_t)count * kNormParts * 8, 256);
+  z.all = 2 * z.x + 2 * z.a + z.norms;
+  return z;
+}
+size_t workspace_of(const Work& w, int sm_count) {
+  size_t most = 0;
+  for (size_t at = 0; at < w.little.size();) {
+    SmallSizes s;
+    at += next_small(w.little, at, w.matrices, sm_count, nullptr, &s);
+    most = std::max(most, small_bytes(s));
+  }
+  for (const Shape& s : w.large) most = std::max(most, large_sizes(s, batch_of(s)).all);
+  return most;
+}
+float factor_of(int adjust, int rows, int cols) {
+  if (adjust == B200CP_MUON_ORIGINAL) return (float)std::sqrt(std::max(1.0, (double)rows / cols));
+  if (adjust == B200CP_MUON_MATCH_RMS_ADAMW) return (float)(0.2 * std::sqrt((double)std::max(rows, cols)));
+  return 1.f;
+}
+
+template <typename P, typename G>
+int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char* ws, const DeviceInfo& di, cudaStream_t st) {
+  Coefficients co{};
+  if (plan.steps) std::copy(plan.v, plan.v + 3 * plan.coefficients, co.v);
+  for (size_t at = 0; at < w.little.size();) {
+    SmallTable t;
+    SmallSizes s;
+    t.count = next_small(w.little, at, w.matrices, di.sm_count, &t, &s);
+    at += t.count;
+    t.r = r;
+    t.steps = plan.steps;
+    t.coefficients = plan.coefficients;
+    t.gram = reinterpret_cast<double*>(ws);
+    t.inverse = reinterpret_cast<double*>(ws + align_up(s.doubles * 8, 256));
+    t.q = reinterpret_cast<float*>(ws + align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256));
+    int widest = 1;
+    for (int i = 0; i < t.count; ++i) {
+      t.e[i].scale = factor_of(adjust, t.e[i].rows, t.e[i].cols);
+      widest = std::max(widest, tile_side(std::min(t.e[i].rows, t.e[i].cols)));
+    }
+    const int N = 16 * widest, gram = kSub * (N + 2) * 8, four = 4 * N * N * 8, low = (kSmall * kSmall + 2 * kSmall * (kSub + 1)) * 4;
+    static std::atomic<int> set1[64], set2[64], set3[64];
+    B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(muon_gram_kernel<G>), set1, gram));
+    B200CP_CUDA_OK(launch_kernel(muon_gram_kernel<G>, dim3(s.ctas), dim3(kGramThreads), gram, st, true, t));
+    B200CP_LAUNCH_OK("muon_gram_kernel");
+    B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(muon_iterate_kernel), set2, four));
+    B200CP_CUDA_OK(launch_kernel(muon_iterate_kernel, dim3(s.matrices), dim3(256), four, st, true, t, co));
+    B200CP_LAUNCH_OK("muon_iterate_kernel");
+    B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(muon_small_apply_kernel<P, G>), set3, low));
+    B200CP_CUDA_OK(launch_kernel(muon_small_apply_kernel<P, G>, dim3(s.ctas), dim3(256), low, st, true, t));
+    B200CP_LAUNCH_OK("muon_small_apply_kernel");
+  }
+  return B200CP_OK;
+}
+
+template <typename P, typename G>
+int run_large(const Shape& s, int first, int count, const Rates& r, const Plan& plan, int adjust, char* ws, const DeviceInfo& di, cudaStream_t st) {
+  const LargeSizes z = large_sizes(s, count);
+  const int n = std::min(s.rows, s.cols), len = std::max(s.rows, s.cols);
+  const bool wide = s.rows <= s.cols;
+  Planes X{reinterpret_cast<__half*>(ws), s.rows, s.cols, ld8(s.cols), count}, Y = X, A{reinterpret_cast<__half*>(ws + 2 * z.x), n, n, ld8(n), count}, B = A;
+  Y.p = reinterpret_cast<__half*>(ws + z.x);
+  B.p = reinterpret_cast<__half*>(ws + 2 * z.x + z.a);
+  Batch b{};
+  b.r = r;
+  b.count = count; b.rows = s.rows; b.cols = s.cols; b.ld = X.ld;
+  b.plane = X.plane(); b.matrix = X.matrix();
+  double sx = room_for(plan.bound[0]);
+  b.scale = (float)sx;
+  b.rate = factor_of(adjust, s.rows, s.cols);
+  b.x = X.p;
+  b.norms = reinterpret_cast<double*>(ws + 2 * z.x + 2 * z.a);
+  uintptr_t off = s.cols % 8;
+  for (int i = 0; i < count; ++i) {
+    b.at[i] = s.at[first + i];
+    off |= (reinterpret_cast<uintptr_t>(b.at[i].p) | reinterpret_cast<uintptr_t>(b.at[i].g) | reinterpret_cast<uintptr_t>(b.at[i].m) |
+            reinterpret_cast<uintptr_t>(b.at[i].w)) & 15;
+  }
+  b.vec = off == 0;
+  const long long values = (long long)s.rows * s.cols;
+  b.parts = (int)std::min<long long>(kNormParts, std::max<long long>(1, values / 4096));
+  B200CP_CUDA_OK(launch_kernel(muon_momentum_kernel<G>, dim3(b.parts, count), dim3(256), 0, st, true, b));
+  B200CP_LAUNCH_OK("muon_momentum_kernel");
+  const int rows8 = (int)std::min<long long>(16LL * di.sm_count, ((long long)s.rows * (X.ld / 8) + 255) / 256);
+  B200CP_CUDA_OK(launch_kernel(muon_planes_kernel<G>, dim3(rows8, count), dim3(256), 0, st, true, b));
+  B200CP_LAUNCH_OK("muon_planes_kernel");
+  for (int step = 0; step < plan.steps; ++step) {
+    const double* v = plan.v + (plan.coefficients > 1 ? 3 * step : 0);
+    const double y = plan.bound[step] * plan.bound[step], sa = room_for(y),
+                 sb = room_for(std::max(1e-3, std::fabs(v[1]) * y + std::fabs(v[2]) * y * y)), sn = room_for(plan.bound[step + 1]);
+    if (int rc = wide ? product<false, false>(X, X, len, (float)(sa / (sx * sx)), 0.f, nullptr, A, true, st)
+                      : product<true, true>(X, X, len, (float)(sa / (sx * sx)), 0.f, nullptr, A, true, st))
+      return rc;
+    if (int rc = product<false, false>(A, A, n, (float)(v[2] * sb / (sa * sa)), (float)(v[1] * sb / sa), &A, B, true, st)) return rc;
+    if (int rc = wide ? product<false, true>(B, X, n, (float)(sn / (sb * sx)), (float)(v[0] * sn / sx), &X, Y, false, st)
+                      : product<false, false>(X, B, n, (float)(sn / (sb * sx)), (float)(v[0] * sn / sx), &X, Y, false, st))
+      return rc;
+    std::swap(X, Y);
+    sx = sn;
+  }
+  b.x = X.p;
+  b.scale = (float)sx;
+  B200CP_CUDA_OK(launch_kernel(muon_apply_kernel<P>, dim3(rows8, count), dim3(256), 0, st, true, b));
+  B200CP_LAUNCH_OK("muon_apply_kernel");
+  return B200CP_OK;
+}
+
+template <typename P, typename G>
+int run(const Work& w, const Rates& r, const Plan& plan, int adjust, char* ws, cudaStream_t st) {
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  if (int rc = run_small<P, G>(w, r, plan, adjust, ws, di, st)) return rc;
+  for (const Shape& s : w.large) {
+    const int most = batch_of(s), all = (int)s.at.size();
+    for (int first = 0; first < all; first += most)
+      if (int rc = run_large<P, G>(s, first, std::min(most, all - first), r, plan, adjust, ws, di, st)) return rc;
+  }
+  return B200CP_OK;
+}
+
+int check_muon(const char* who, const b200cp_muon_matrix* ms, int count, int ptype, int gtype) {
+  if (count < 0 || (count && !ms)) return fail(B200CP_ERR_INVALID_ARG, "%s: null argument or negative count", who);
+  if (ptype < B200CP_FLOAT32 || ptype > B200CP_FLOAT16 || (gtype != ptype && gtype != B200CP_FLOAT32))
+    return fail(B200CP_ERR_UNSUPPORTED, "%s: parameters of type %d with gradients of type %d", who, ptype, gtype);
+  for (int i = 0; i < count; ++i) {
+    const b200cp_muon_matrix& a = ms[i];
+    if (a.stack < 0 || a.rows < 0 || a.cols < 0) return fail(B200CP_ERR_INVALID_ARG, "%s: matrix %d is %d x %d x %d", who, i, a.stack, a.rows, a.cols);
+    if (a.rows > (1 << 24) || a.cols > (1 << 24) || (long long)std::min(a.rows, a.cols) > (1 << 17))
+      return fail(B200CP_ERR_UNSUPPORTED, "%s: matrix %d is %d x %d (sides up to 2^24, the smaller one up to 2^17)", who, i, a.rows, a.cols);
+  }
+  return B200CP_OK;
+}
+int muon(const char* who, const b200cp_muon_matrix* ms, int count, int ptype, int gtype, const b200cp_muon* h, bool update, void* workspace, size_t bytes,
+         void* stream) {
+  if (!h) return fail(B200CP_ERR_INVALID_ARG, "%s: null argument", who);
+  if (int rc = check_muon(who, ms, count, ptype, gtype)) return rc;
+  Plan plan;
+  if (int rc = plan_of(who, h, &plan)) return rc;
+  for (int i = 0; i < count; ++i) {
+    const b200cp_muon_matrix& a = ms[i];
+    if (a.stack && a.rows && a.cols && (!a.param || !a.grad || (update && !a.momentum))) return fail(B200CP_ERR_INVALID_ARG, "%s: null pointer in matrix %d", who, i);
+    if (a.master && ptype == B200CP_FLOAT32) return fail(B200CP_ERR_INVALID_ARG, "%s: a float32 parameter has no float32 copy (matrix %d)", who, i);
+  }
+  const Work w(ms, count, ptype, gtype);
+  if (w.little.empty() && w.large.empty()) return B200CP_OK;
+  const size_t need = b200cp_muon_step_workspace_bytes(ms, count, ptype, gtype);
+  if (need && (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return fail(B200CP_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, %zu given", who, need, bytes);
+  Rates r{};
+  r.keep = (float)h->momentum; r.blend = (float)(1 - h->momentum);
+  r.nesterov = h->nesterov != 0; r.update = update;
+  r.lr = (float)h->lr; r.decay = (float)h->weight_decay;
+  r.device_lr = h->device_lr;
+  r.eps = h->eps;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+#define TYPES(P, G) return run<P, G>(w, r, plan, h->adjust, ws, st)
+  if (ptype == B200CP_FLOAT32) TYPES(float, float);
+  if (ptype == B200CP_BFLOAT16 && gtype == B200CP_BFLOAT16) TYPES(__nv_bfloat16, __nv_bfloat16);
+  if (ptype == B200CP_FLOAT16 && gtype == B200CP_FLOAT16) TYPES(__half, __half);
+  if (ptype == B200CP_BFLOAT16) TYPES(__nv_bfloat16, float);
+  TYPES(__half, float);
+#undef TYPES
+}
+
+}  // namespace
+
+int muon_device_status(int* out) {
+  int v = 0, zero = 0;
+  B200CP_CUDA_OK(cudaMemcpyFromSymbol(&v, g_muon_status, sizeof(int)));
+  if (v) B200CP_CUDA_OK(cudaMemcpyToSymbol(g_muon_status, &zero, sizeof(int)));
+  *out = v;
+  return B200CP_OK;
+}
+
+}  // namespace b200cp
+
+using namespace b200cp;
+
+extern "C" {
+
+size_t b200cp_muon_step_workspace_bytes(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type) {
+  if (check_muon("b200cp_muon_step_workspace_bytes", matrices, count, param_type, grad_type)) return 0;
+  DeviceInfo di;
+  if (device_info(&di)) return 0;
+  return workspace_of(Work(matrices, count, param_type, grad_type), di.sm_count);
+}
+
+int b200cp_muon_step(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type, const b200cp_muon* hyper, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  const char* who = "b200cp_muon_step";
+  if (hyper && (hyper->adjust < B200CP_MUON_PLAIN || hyper->adjust > B200CP_MUON_MATCH_RMS_ADAMW))
+    return fail(B200CP_ERR_INVALID_ARG, "%s: adjust %d", who, hyper->adjust);
+  return muon(who, matrices, count, param_type, grad_type, hyper, true, workspace, workspace_bytes, stream);
+}
+
+int b200cp_orthogonalise(int stack, int rows, int cols, int type, const void* X, void* out, const double* coefficients, int coefficient_count, int steps,
+                         double eps, void* workspace, size_t workspace_bytes, void* stream) {
+  const b200cp_muon_matrix m{out, X, nullptr, nullptr, stack, rows, cols};
+  b200cp_muon h{};
+  h.eps = eps;
+  h.steps = steps;
+  h.coefficients = coefficients;
+  h.coefficient_count = coefficient_count;
+  return muon("b200cp_orthogonalise", &m, 1, type, type, &h, false, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -843,6 +843,9 @@ PyMethodDef g_methods[] = {FAST(cp4_forward), FAST(cp4_forward_save), FAST(cp4_b
                            FAST(adapter_plan), FAST(dense_adapters), FAST(dense_adapters_backward), FAST(adapters_apply),
                            FAST(dense_gated), FAST(dense_gated_save), FAST(dense_gated_backward), FAST(gated_apply),
                            FAST(adamw_step), FAST(adamw_moments),
+                           FAST(embedding), FAST(embedding_backward), FAST(embedding_apply),
+                           FAST(layer_norm), FAST(layer_norm_backward), FAST(layer_norm_apply),
+                           FAST(muon_step), FAST(orthogonalise),
                            {"set_error_class", py_set_error_class, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_C", "native operator bindings", -1, g_methods, nullptr, nullptr, nullptr,

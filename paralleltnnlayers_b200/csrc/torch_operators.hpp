@@ -1,4 +1,5 @@
-// Bindings of the operators that stand beside the factored layers: low-rank adapters, the gated feed-forward block and the AdamW step.
+// Bindings of the operators that stand beside the factored layers: low-rank adapters, the gated feed-forward block, the AdamW step, the embedding, layer
+// norm and the Muon step.
 // Part of torch_binding.cpp's namespace, whose helpers it uses.
 
 // ---- types ------------------------------------------------------------------------------------------------------------
@@ -279,6 +280,12 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   }
 };
 
+PyObject* wrap_tuple(const std::vector<Tensor>& ts) {
+  PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
+  if (!r) throw python_error();
+  for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(r, (Py_ssize_t)i, wrap(ts[i]));
+  return r;
+}
 Tensor optional_tensor(PyObject* o, const char* name) { return o == Py_None ? Tensor() : any_tensor(o, name); }
 bool truth(PyObject* o) {
   const int v = PyObject_IsTrue(o);
@@ -556,5 +563,368 @@ PYFN(py_adamw_moments) {
     ok(b200cp_adamw_moments((unsigned long long)count, m.const_data_ptr(), v.const_data_ptr(), cp(ms), cp(vs), type, om.data_ptr(), ov.data_ptr(), st));
   });
   Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- embedding ------------------------------------------------------------------------------------------------------------
+struct Tokens {   // checked and contiguous
+  Tensor t;
+  int rows, wide;
+  Tokens(const Tensor& t_, const Tensor& like) {
+    TORCH_CHECK_TYPE(t_.is_cuda() && (t_.scalar_type() == at::kInt || t_.scalar_type() == at::kLong), "tokens must be an int32 or int64 CUDA tensor");
+    TORCH_CHECK_VALUE(t_.device() == like.device(), "tokens are on ", t_.device(), ", the rows on ", like.device());
+    rows = size_arg(t_.numel(), "the number of tokens");
+    wide = t_.scalar_type() == at::kLong;
+    t = contiguous(t_);
+  }
+  std::vector<int64_t> size(int64_t last) const {
+    std::vector<int64_t> s = t.sizes().vec();
+    s.push_back(last);
+    return s;
+  }
+};
+Tensor embedding(const Tensor& tokens_, const Tensor& W_, double scale) {
+  const int type = type_of(W_, "W");
+  TORCH_CHECK_VALUE(W_.dim() == 2 && W_.size(0) > 0 && W_.size(1) > 0, "expected W [count, features], it is ", W_.sizes());
+  const Tokens t(tokens_, W_);
+  const Tensor W = contiguous(W_);
+  const int V = size_arg(W.size(0), "the number of rows of W"), D = size_arg(W.size(1), "the number of features");
+  const c10::cuda::OptionalCUDAGuard guard(W.device());
+  Tensor out = empty_as(t.size(D), W);
+  ok(b200cp_embedding(t.rows, V, D, type, t.wide, t.t.const_data_ptr(), W.const_data_ptr(), (float)scale, out.data_ptr(), stream(W)));
+  return out;
+}
+Tensor embedding_backward(const Tensor& dy_, const Tensor& tokens_, int64_t count, double scale) {
+  const int type = type_of(dy_, "dY");
+  const Tokens t(tokens_, dy_);
+  TORCH_CHECK_VALUE(dy_.dim() >= 1 && dy_.size(-1) > 0 && dy_.sizes() == at::IntArrayRef(t.size(dy_.size(-1))), "dY is ", dy_.sizes(), " where there are tokens ",
+                    t.t.sizes());
+  TORCH_CHECK_VALUE(count > 0, "the table has ", count, " rows");
+  const Tensor dy = contiguous(dy_);
+  const int V = size_arg(count, "the number of rows of the table"), D = size_arg(dy.size(-1), "the number of features");
+  const c10::cuda::OptionalCUDAGuard guard(dy.device());
+  Tensor dW = empty_as({V, D}, dy);
+  const Scratch ws(b200cp_embedding_bwd_workspace_bytes(t.rows, D), dy);
+  ok(b200cp_embedding_bwd(t.rows, V, D, type, t.wide, t.t.const_data_ptr(), dy.const_data_ptr(), (float)scale, dW.data_ptr(), ws.ptr, ws.bytes, stream(dy)));
+  return dW;
+}
+struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& W, double scale) {
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["count"] = W.size(0);
+    ctx->save_for_backward({tokens});
+    return embedding(tokens, W, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return {Tensor(), embedding_backward(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["count"].toInt(), ctx->saved_data["scale"].toDouble()), Tensor()};
+  }
+};
+// (tokens, W, scale)
+PYFN(py_embedding) {
+  HANDLE_TH_ERRORS
+  count_args(n, 3);
+  const Tensor &t = any_tensor(a[0], "tokens"), &W = any_tensor(a[1], "W");
+  const double scale = float_arg(a[2]);
+  return wrap(unlocked([&] { return embedding(t, W, scale); }));
+  END_HANDLE_TH_ERRORS
+}
+// (dY, tokens, count, scale)
+PYFN(py_embedding_backward) {
+  HANDLE_TH_ERRORS
+  count_args(n, 4);
+  const Tensor &dy = any_tensor(a[0], "dY"), &t = any_tensor(a[1], "tokens");
+  const int64_t count = int_arg(a[2]);
+  const double scale = float_arg(a[3]);
+  return wrap(unlocked([&] { return embedding_backward(dy, t, count, scale); }));
+  END_HANDLE_TH_ERRORS
+}
+PYFN(py_embedding_apply) {
+  HANDLE_TH_ERRORS
+  count_args(n, 3);
+  const Tensor &t = any_tensor(a[0], "tokens"), &W = any_tensor(a[1], "W");
+  const double scale = float_arg(a[2]);
+  const bool grad = at::GradMode::is_enabled() && W.requires_grad();
+  return wrap(unlocked([&] { return grad ? EmbeddingNode::apply(t, W, scale) : embedding(t, W, scale); }));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- layer norm ------------------------------------------------------------------------------------------------------------
+struct Norm {   // operands, checked and contiguous
+  Tensor x, w, b;
+  int rows, D, type, weight_type;
+  Norm(const Tensor& x_, const Tensor& w_, const Tensor& b_, const char* name) {
+    type = weight_type = type_of(x_, name);
+    TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) > 0, name, " is ", x_.sizes(), ", [..., features] is expected");
+    D = size_arg(x_.size(-1), "the number of features");
+    rows = size_arg(x_.numel() / D, "the number of rows");
+    for (const Tensor* t : {&w_, &b_}) {
+      if (!t->defined()) continue;
+      const char* what = t == &w_ ? "weight" : "bias";
+      weight_type = type_of(*t, what);
+      TORCH_CHECK_TYPE(t->scalar_type() == x_.scalar_type() || t->scalar_type() == at::kFloat, what, " must have the type of ", name, ", ", x_.scalar_type(),
+                       ", or float32");
+      TORCH_CHECK_VALUE(t->device() == x_.device(), what, " is on ", t->device(), ", ", name, " on ", x_.device());
+      TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == D, what, " is ", t->sizes(), " where there are ", D, " features");
+    }
+    TORCH_CHECK_TYPE(!w_.defined() || !b_.defined() || w_.scalar_type() == b_.scalar_type(), "weight and bias must have one type");
+    x = contiguous(x_);
+    if (w_.defined()) w = contiguous(w_);
+    if (b_.defined()) b = contiguous(b_);
+  }
+  void like(const Tensor& t, const char* name) const {
+    TORCH_CHECK_TYPE(t.is_cuda() && t.scalar_type() == x.scalar_type(), name, " must be a CUDA tensor of type ", x.scalar_type());
+    TORCH_CHECK_VALUE(t.device() == x.device(), name, " is on ", t.device(), ", the rows on ", x.device());
+    TORCH_CHECK_VALUE(t.sizes() == x.sizes(), name, " is ", t.sizes(), " where the rows are ", x.sizes());
+  }
+  void statistic(const Tensor& t, const char* name) const {
+    TORCH_CHECK_TYPE(t.is_cuda() && t.scalar_type() == at::kFloat, name, " must be a float32 CUDA tensor");
+    TORCH_CHECK_VALUE(t.device() == x.device(), name, " is on ", t.device(), ", the rows on ", x.device());
+    TORCH_CHECK_VALUE(t.numel() == rows, name, " has ", t.numel(), " values for ", rows, " rows");
+  }
+  static const void* at(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+};
+struct Normed {
+  Tensor y, h, mean, rstd;
+};
+Normed layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps, const Tensor& r_, bool keep) {
+  const Norm g(x, w, b, "X");
+  TORCH_CHECK_VALUE(eps >= 0, "eps is ", eps);
+  if (r_.defined()) g.like(r_, "residual");
+  const Tensor r = r_.defined() ? contiguous(r_) : r_;
+  const c10::cuda::OptionalCUDAGuard guard(g.x.device());
+  Normed o;
+  o.h = r.defined() ? empty_as(g.x.sizes(), g.x) : g.x;
+  o.y = empty_as(g.x.sizes(), g.x);
+  if (keep) {
+    o.mean = empty({g.rows}, g.x);
+    o.rstd = empty({g.rows}, g.x);
+  }
+  ok(b200cp_layer_norm(g.rows, g.D, g.type, g.weight_type, g.x.const_data_ptr(), Norm::at(r), Norm::at(g.w), Norm::at(g.b), (float)eps, o.y.data_ptr(),
+                       r.defined() ? o.h.data_ptr() : nullptr, keep ? mp(o.mean) : nullptr, keep ? mp(o.rstd) : nullptr, stream(g.x)));
+  return o;
+}
+// (b: undefined, or anything of the bias's type and size)
+std::array<Tensor, 3> layer_norm_backward(const Tensor& dy_, const Tensor& h, const Tensor& w, const Tensor& b, const Tensor& mean_, const Tensor& rstd_,
+                                          const Tensor& dh_, bool need_x, bool need_w, bool need_b) {
+  const Norm g(h, w, b, "H");
+  g.like(dy_, "dY");
+  if (dh_.defined()) g.like(dh_, "dH");
+  g.statistic(mean_, "mean");
+  g.statistic(rstd_, "rstd");
+  const Tensor dy = contiguous(dy_), dh = dh_.defined() ? contiguous(dh_) : dh_, mean = contiguous(mean_), rstd = contiguous(rstd_);
+  const Tensor& weights = w.defined() ? g.w : b.defined() ? g.b : g.x;
+  const c10::cuda::OptionalCUDAGuard guard(g.x.device());
+  std::array<Tensor, 3> d;
+  if (need_x) d[0] = empty_as(g.x.sizes(), g.x);
+  if (need_w) d[1] = empty_as({g.D}, weights);
+  if (need_b) d[2] = empty_as({g.D}, weights);
+  const auto to = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  const Scratch ws(need_w || need_b ? b200cp_layer_norm_bwd_workspace_bytes(g.rows, g.D) : 0, g.x);
+  ok(b200cp_layer_norm_bwd(g.rows, g.D, g.type, g.weight_type, dy.const_data_ptr(), Norm::at(dh), g.x.const_data_ptr(), Norm::at(g.w), cp(mean), cp(rstd), to(d[0]),
+                           to(d[1]), to(d[2]), ws.ptr, ws.bytes, stream(g.x)));
+  return d;
+}
+// Results: Y, or Y and H where there is a residual.
+struct NormNode : torch::autograd::Function<NormNode> {
+  using Maybe = std::optional<Tensor>;
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& w_, const Maybe& b_, const Maybe& r_, double eps) {
+    const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor()), r = r_.value_or(Tensor());
+    const Normed o = layer_norm(x, w, b, eps, r, true);
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["residual"] = r.defined();
+    ctx->save_for_backward({o.h, w, b, o.mean, o.rstd});
+    if (r.defined()) return {o.y, o.h};
+    return {o.y};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list v = ctx->get_saved_variables();
+    const bool residual = ctx->saved_data["residual"].toBool();
+    // (only inputs that are there have a place in the node)
+    size_t place = 1;
+    const bool need_w = v[1].defined() && ctx->needs_input_grad(place++), need_b = v[2].defined() && ctx->needs_input_grad(place++);
+    const bool need_x = ctx->needs_input_grad(0) || (residual && ctx->needs_input_grad(place));
+    const Tensor dh = residual ? grads[1] : Tensor();
+    std::array<Tensor, 3> d;
+    if (grads[0].defined()) d = layer_norm_backward(grads[0], v[0], v[1], v[2], v[3], v[4], dh, need_x, need_w, need_b);
+    else d[0] = dh;
+    return {d[0], d[1], d[2], residual ? d[0] : Tensor(), Tensor()};
+  }
+};
+// (X, weight or None, bias or None, eps, residual or None, keep): Y, H where there is a residual, mean and rstd where they are kept
+PYFN(py_layer_norm) {
+  HANDLE_TH_ERRORS
+  count_args(n, 6);
+  const Tensor& x = any_tensor(a[0], "X");
+  const Tensor w = optional_tensor(a[1], "weight"), b = optional_tensor(a[2], "bias"), r = optional_tensor(a[4], "residual");
+  const double eps = float_arg(a[3]);
+  const bool keep = truth(a[5]);
+  const Normed o = unlocked([&] { return layer_norm(x, w, b, eps, r, keep); });
+  if (!keep && !r.defined()) return wrap(o.y);
+  std::vector<Tensor> out{o.y};
+  if (r.defined()) out.push_back(o.h);
+  if (keep) {
+    out.push_back(o.mean);
+    out.push_back(o.rstd);
+  }
+  return wrap_tuple(out);
+  END_HANDLE_TH_ERRORS
+}
+// (dY, H, weight or None, bias or None, mean, rstd, dH or None, need_dx, need_dw, need_db)
+PYFN(py_layer_norm_backward) {
+  HANDLE_TH_ERRORS
+  count_args(n, 10);
+  const Tensor &dy = any_tensor(a[0], "dY"), &h = any_tensor(a[1], "H"), &mean = any_tensor(a[4], "mean"), &rstd = any_tensor(a[5], "rstd");
+  const Tensor w = optional_tensor(a[2], "weight"), b = optional_tensor(a[3], "bias"), dh = optional_tensor(a[6], "dH");
+  const bool nx = truth(a[7]), nw = truth(a[8]), nb = truth(a[9]);
+  return wrap_tuple(unlocked([&] { return layer_norm_backward(dy, h, w, b, mean, rstd, dh, nx, nw, nb); }));
+  END_HANDLE_TH_ERRORS
+}
+// (x, weight or None, bias or None, eps, residual or None)
+PYFN(py_layer_norm_apply) {
+  HANDLE_TH_ERRORS
+  count_args(n, 5);
+  const Tensor& x = any_tensor(a[0], "X");
+  const Tensor w = optional_tensor(a[1], "weight"), b = optional_tensor(a[2], "bias"), r = optional_tensor(a[4], "residual");
+  const double eps = float_arg(a[3]);
+  bool grad = x.requires_grad();
+  for (const Tensor* t : {&w, &b, &r}) grad = grad || (t->defined() && t->requires_grad());
+  grad = grad && at::GradMode::is_enabled();
+  variable_list out;
+  unlocked([&] {
+    if (grad) {
+      const auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+      out = NormNode::apply(x, maybe(w), maybe(b), maybe(r), eps);
+      return;
+    }
+    const Normed o = layer_norm(x, w, b, eps, r, false);
+    out = {o.y};
+    if (r.defined()) out.push_back(o.h);
+  });
+  return r.defined() ? wrap_tuple(out) : wrap(out[0]);
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- Muon step --------------------------------------------------------------------------------------------------------------
+struct Coefficients {
+  std::vector<double> v;
+  int count;
+  explicit Coefficients(PyObject* o) {
+    TORCH_CHECK_TYPE(PyTuple_Check(o), "coefficients must be a tuple of numbers");
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(o); ++i) v.push_back(float_arg(PyTuple_GET_ITEM(o, i)));
+    TORCH_CHECK_VALUE(!v.empty() && v.size() % 3 == 0, "coefficients come in threes");
+    count = (int)(v.size() / 3);
+  }
+};
+// (params, grads, momentum, master or None, lr, momentum, nesterov, weight_decay, coefficients, eps, steps, adjust)
+PYFN(py_muon_step) {
+  HANDLE_TH_ERRORS
+  count_args(n, 12);
+  const TensorList p(a[0], "params"), g(a[1], "grads"), m(a[2], "momentum");
+  const bool copies = a[3] != Py_None;
+  TensorList w;
+  if (copies) w = TensorList(a[3], "master");
+  const size_t count = p.size();
+  TORCH_CHECK_VALUE(g.size() == count && m.size() == count && (!copies || w.size() == count), "muon_step: ", count,
+                    " params need as many grads, momentum buffers and master copies");
+  b200cp_muon h{};
+  const Tensor* lr = nullptr;
+  if (THPVariable_Check(a[4])) {
+    lr = &any_tensor(a[4], "lr");
+    TORCH_CHECK_TYPE(lr->scalar_type() == at::kFloat && lr->numel() == 1, "lr must be a number or one float32 in a CUDA tensor");
+  } else {
+    h.lr = float_arg(a[4]);
+  }
+  h.momentum = float_arg(a[5]);
+  h.nesterov = truth(a[6]);
+  h.weight_decay = float_arg(a[7]);
+  const Coefficients co(a[8]);
+  h.coefficients = co.v.data();
+  h.coefficient_count = co.count;
+  h.eps = float_arg(a[9]);
+  h.steps = (int)std::min<int64_t>(int_arg(a[10]), 1 << 20);
+  h.adjust = (int)int_arg(a[11]);
+  if (!count) Py_RETURN_NONE;
+  const int type = type_of(p[0], "params"), gtype = type_of(g[0], "grads");
+  TORCH_CHECK_TYPE(gtype == type || gtype == B200CP_FLOAT32, "grads must have the params' type or float32");
+  TORCH_CHECK_VALUE(!copies || type != B200CP_FLOAT32, "master copies are of 16-bit parameters");
+  const c10::Device device = p[0].device();
+  const auto fits = [&](const Tensor& t, const char* name, at::ScalarType want, at::IntArrayRef size, bool in_place) {
+    TORCH_CHECK_TYPE(t.scalar_type() == want, name, " must be ", want, ", it is ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.device() == device, name, " is on ", t.device(), ", the first parameter on ", device);
+    TORCH_CHECK_VALUE(t.sizes() == size, name, " is ", t.sizes(), " where the parameter is ", size);
+    TORCH_CHECK_VALUE(!in_place || t.is_contiguous(), name, " is updated in place and has to be contiguous");
+  };
+  TORCH_CHECK_VALUE(!lr || lr->device() == device, "lr has to be on the parameters' device");
+  std::vector<b200cp_muon_matrix> ms(count);
+  std::vector<Tensor> held;   // contiguous copies of gradients
+  enum { kParam, kGrad, kMomentum, kMaster, kKinds };
+  std::vector<b200cp::Span> spans(kKinds * count);
+  const auto span = [&](int kind, size_t i, const void* at, size_t bytes) {
+    spans[kind * count + i] = {reinterpret_cast<uintptr_t>(at), reinterpret_cast<uintptr_t>(at) + bytes};
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const at::IntArrayRef size = p[i].sizes();
+    TORCH_CHECK_VALUE(size.size() >= 2, "params have to be matrices or stacks of them, [..., rows, columns], one is ", size);
+    fits(p[i], "params", p[0].scalar_type(), size, true);
+    fits(g[i], "grads", g[0].scalar_type(), size, false);
+    fits(m[i], "momentum", at::kFloat, size, true);
+    if (copies) fits(w[i], "master", at::kFloat, size, true);
+  }
+  const c10::cuda::OptionalCUDAGuard guard(device);
+  for (size_t i = 0; i < count; ++i) {
+    const at::IntArrayRef size = p[i].sizes();
+    const int rows = size_arg(size[size.size() - 2], "the number of rows"), cols = size_arg(size[size.size() - 1], "the number of columns");
+    if (!p[i].numel()) continue;
+    const void* grad;
+    if (g[i].is_contiguous()) {
+      grad = g[i].const_data_ptr();
+    } else {
+      held.push_back(g[i].contiguous());
+      grad = held.back().const_data_ptr();
+    }
+    ms[i] = {p[i].mutable_data_ptr(), grad, mp(m[i]), copies ? mp(w[i]) : nullptr, size_arg(p[i].numel() / ((int64_t)rows * cols), "the number of matrices"), rows, cols};
+    span(kParam, i, ms[i].param, p[i].nbytes());
+    span(kGrad, i, grad, g[i].nbytes());
+    span(kMomentum, i, ms[i].momentum, m[i].nbytes());
+    if (copies) span(kMaster, i, ms[i].master, w[i].nbytes());
+  }
+  b200cp::SpanList kinds[kKinds];
+  size_t used = 0;
+  for (int k = 0; k < kKinds; ++k)
+    if (copies || k != kMaster) kinds[used++] = {&spans[k * count], count, k != kGrad};
+  TORCH_CHECK_VALUE(!b200cp::spans_meet(kinds, used), "muon_step: a tensor occurs twice in what is updated, or shares memory with another one");
+  if (lr) h.device_lr = static_cast<const float*>(lr->const_data_ptr());
+  void* st = stream(p[0]);
+  const Scratch ws(b200cp_muon_step_workspace_bytes(ms.data(), (int)count, type, gtype), p[0]);
+  unlocked([&] { ok(b200cp_muon_step(ms.data(), (int)count, type, gtype, &h, ws.ptr, ws.bytes, st)); });
+  for (size_t i = 0; i < count; ++i) {
+    written(p[i]);
+    written(m[i]);
+    if (copies) written(w[i]);
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+// (X, coefficients, eps, steps)
+PYFN(py_orthogonalise) {
+  HANDLE_TH_ERRORS
+  count_args(n, 4);
+  const Tensor& x_ = any_tensor(a[0], "X");
+  const Coefficients co(a[1]);
+  const double eps = float_arg(a[2]);
+  const int steps = (int)std::min<int64_t>(int_arg(a[3]), 1 << 20);
+  return wrap(unlocked([&] {
+    const int type = type_of(x_, "X");
+    TORCH_CHECK_VALUE(x_.dim() >= 2, "X has to be a matrix or a stack of them, [..., rows, columns], it is ", x_.sizes());
+    const c10::cuda::OptionalCUDAGuard guard(x_.device());
+    const Tensor x = contiguous(x_);
+    Tensor out = empty_as(x.sizes(), x);
+    const int rows = size_arg(x.size(-2), "the number of rows"), cols = size_arg(x.size(-1), "the number of columns");
+    const int stack = x.numel() ? size_arg(x.numel() / ((int64_t)rows * cols), "the number of matrices") : 0;
+    const b200cp_muon_matrix m{nullptr, nullptr, nullptr, nullptr, stack, rows, cols};
+    const Scratch ws(b200cp_muon_step_workspace_bytes(&m, 1, type, type), x);
+    ok(b200cp_orthogonalise(stack, rows, cols, type, x.const_data_ptr(), out.data_ptr(), co.v.data(), co.count, steps, eps, ws.ptr, ws.bytes, stream(x)));
+    return out;
+  }));
   END_HANDLE_TH_ERRORS
 }

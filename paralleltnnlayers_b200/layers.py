@@ -5,7 +5,8 @@ compression ``rate`` is turned into a CP rank by ``generate_params_*`` (pure int
 factor variables are created, and the layer is the sequential or the fused op.  These modules keep that
 interface for the three CP layer families of the hot path; weights live in the layout the C ABI takes
 (``[dim, R]`` factors for CP4, ``[c_k, t_k, R]`` for rCP, ``[i_k, o_k, R]`` for the dense layer).  Beside them stand
-``AdaptedDense`` (a shared projection with low-rank adapters per request) and ``GatedDense`` (the gated half of a feed-forward block).
+``AdaptedDense`` (a shared projection with low-rank adapters per request), ``GatedDense`` (the gated half of a feed-forward block), ``Embedding`` and
+``LayerNorm`` (what is before and between such blocks).
 """
 from __future__ import annotations
 
@@ -248,3 +249,36 @@ class GatedDense(nn.Module):
 
     def forward(self, x):
         return _ops().DenseGatedFunction.apply(x, self.Wg, self.Wu, self.activation)
+
+
+class Embedding(nn.Module):
+    """Rows of a table by token, times ``scale``; a token outside ``0 .. count - 1`` is none (padding): zeros, and no gradient.  The table's gradient is dense and
+    its sums are in a fixed order.  float32, bfloat16 or float16."""
+
+    def __init__(self, count, features, scale=1.0, dtype=torch.float32):
+        super().__init__()
+        if count < 1 or features < 1:
+            raise ValueError("at least one token and one feature")
+        if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise ValueError("dtype is float32, bfloat16 or float16")
+        self.scale = float(scale)
+        self.W = nn.Parameter((torch.randn(count, features) / abs(self.scale or 1.0)).to(dtype))
+
+    def forward(self, tokens):
+        return _ops().EmbeddingFunction.apply(tokens, self.W, self.scale)
+
+
+class LayerNorm(nn.Module):
+    """Layer norm over the last dimension.  ``forward(x)`` gives ``norm(x)``; ``forward(x, residual)`` gives ``(norm(h), h)`` with ``h = x + residual`` in the same pass:
+    a block's output joins the stream, and the next block gets its input.  ``weight`` and ``bias`` (``affine=False``: neither, ``bias=False``: no bias) are float32 or of the rows' type."""
+
+    def __init__(self, features, eps=1e-5, affine=True, bias=True, dtype=torch.float32):
+        super().__init__()
+        if features < 1 or not eps >= 0:
+            raise ValueError("at least one feature, and eps may not be negative")
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(features, dtype=dtype)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(features, dtype=dtype)) if affine and bias else None
+
+    def forward(self, x, residual=None):
+        return _ops().LayerNormFunction.apply(x, self.weight, self.bias, self.eps, residual)

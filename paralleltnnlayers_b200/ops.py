@@ -484,6 +484,76 @@ def adamw_moments(exp_avg, exp_avg_sq, scales, dtype=torch.bfloat16):
     return m, v
 
 
+# ---- embedding ---------------------------------------------------------------------
+def embedding(tokens, W, scale=1.0):
+    """``out[s] = scale W[tokens[s]]`` (``b200cp_embedding``): ``tokens`` int32 or int64 of any shape, ``W [count, features]`` in float32, bfloat16 or
+    float16.  A token outside ``0 .. count - 1`` is none (padding): zeros."""
+    return _C.embedding(tokens, W, scale)
+
+
+def embedding_backward(dY, tokens, count, scale=1.0):
+    """The gradient of ``W``, ``[count, features]`` in ``dY``'s type: ``scale`` times the sum of ``dY`` over the places of each token, zeros for tokens that do not occur.
+    Sums are float32 and in a fixed order."""
+    return _C.embedding_backward(dY, tokens, count, scale)
+
+
+# ---- layer norm ----------------------------------------------------------------------
+def layer_norm(X, weight=None, bias=None, eps=1e-5, residual=None):
+    """``(H - mean) / sqrt(variance + eps) * weight + bias`` over the last dimension (``b200cp_layer_norm``), ``H = X``; with ``residual``
+    ``H = X + residual``, rounded to the type, and the result is ``(Y, H)``.
+
+    ``X`` and ``residual`` of one type: float32, bfloat16 or float16; ``weight`` and ``bias`` (either may be None) of that type or float32.  Statistics are float32."""
+    return _C.layer_norm(X, weight, bias, eps, residual, False)
+
+
+def layer_norm_save(X, weight=None, bias=None, eps=1e-5, residual=None):
+    """The same, with what ``layer_norm_backward`` needs: (Y, mean, rstd) or (Y, H, mean, rstd)."""
+    return _C.layer_norm(X, weight, bias, eps, residual, True)
+
+
+def layer_norm_backward(dY, H, weight, bias, mean, rstd, dH=None, need_dx=True, need_dw=True, need_db=True):
+    """Gradients of ``layer_norm``: (dX, dweight, dbias), None where not needed.  ``dH``: the gradient that came to ``H`` itself, which dX (the gradient of the
+    residual too) includes.  Those of weight and bias have their type (None: the other's, or that of ``H``); ``bias`` is asked for its type alone."""
+    return _C.layer_norm_backward(dY, H, weight, bias, mean, rstd, dH, need_dx, need_dw, need_db)
+
+
+# ---- Muon step -------------------------------------------------------------------------
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+ADJUSTMENTS = {None: 0, "original": 1, "match_rms_adamw": 2}
+
+
+def _triples(coefficients):
+    """One triple, or one for each step, as a flat tuple."""
+    out = tuple(coefficients)
+    if out and not isinstance(out[0], (int, float)):
+        if any(len(c) != 3 for c in out):
+            raise ValueError("coefficients are a triple, or a triple for each step")
+        out = tuple(v for c in out for v in c)
+    elif len(out) != 3:
+        raise ValueError("coefficients are a triple, or a triple for each step")
+    return out
+
+
+def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True, weight_decay=0.1, coefficients=NEWTON_SCHULZ, eps=1e-7, steps=5,
+              adjust="original", master=None):
+    """One Muon step over all matrices of the lists, in place (``b200cp_muon_step``): ``m += (1 - momentum)(g - m)``, ``u = g + momentum (m - g)`` (``nesterov``) or ``m``,
+    ``X = orthogonalise(u)``, ``p -= lr weight_decay p + lr factor X``.
+
+    ``params``: contiguous ``[..., rows, columns]`` of one type on one device, leading dimensions are stacks of matrices; ``grads`` of that type or float32;
+    ``momentum_buffers`` float32 (zero before the first step).  ``adjust``: the factor is sqrt(max(1, rows / columns)) for "original",
+    0.2 sqrt(max(rows, columns)) for "match_rms_adamw", 1 for None.  ``master``: the float32 copies of 16-bit parameters; then they are what is
+    updated, and the parameters are their roundings.  ``lr`` may be one float32 in a CUDA tensor.  What is updated may not share memory with anything else of the call."""
+    if adjust not in ADJUSTMENTS:
+        raise ValueError(f"adjust {adjust!r}: original, match_rms_adamw or None is possible")
+    _C.muon_step(params, grads, momentum_buffers, master, lr, momentum, nesterov, weight_decay, _triples(coefficients), eps, steps, ADJUSTMENTS[adjust])
+
+
+def orthogonalise(X, coefficients=NEWTON_SCHULZ, eps=1e-7, steps=5):
+    """``X / max(|X|, eps)`` after ``steps`` Newton-Schulz products ``X = a X + (b A + c A^2) X``, ``A = X X^T`` (``b200cp_orthogonalise``): singular values near one,
+    the singular vectors those of ``X [..., rows, columns]``.  ``coefficients``: (a, b, c), or one such triple for each step."""
+    return _C.orthogonalise(X, _triples(coefficients), eps, steps)
+
+
 # ---- autograd wrappers ----------------------------------------------------------
 # The nodes are native (csrc/torch_binding.cpp); each class keeps the ``apply`` its layer calls.
 class CP4Conv2dFunction:
@@ -521,3 +591,19 @@ class DenseGatedFunction:
     @staticmethod
     def apply(x, Wg, Wu, activation="silu"):
         return _C.gated_apply(x, Wg, Wu, _activation(activation))
+
+
+class EmbeddingFunction:
+    """``embedding`` with the gradient of its table: ``apply(tokens, W, scale=1.0)``."""
+
+    @staticmethod
+    def apply(tokens, W, scale=1.0):
+        return _C.embedding_apply(tokens, W, scale)
+
+
+class LayerNormFunction:
+    """``layer_norm`` with its gradients: ``apply(x, weight=None, bias=None, eps=1e-5, residual=None)``, with a residual ``(y, h)``."""
+
+    @staticmethod
+    def apply(x, weight=None, bias=None, eps=1e-5, residual=None):
+        return _C.layer_norm_apply(x, weight, bias, eps, residual)

@@ -1,6 +1,6 @@
-"""Optimiser over the fused AdamW step: what applies the gradients of the layers and of the data-parallel steps.
+"""Optimisers over the fused AdamW and Muon steps: what applies the gradients of the layers and of the data-parallel steps.
 
-A network of factored layers has many small parameters (four factors per convolution); all of them are updated by one launch.
+A network of factored layers has many small parameters (four factors per convolution); all of them are updated by one launch (three for Muon).
 """
 from __future__ import annotations
 
@@ -139,3 +139,76 @@ class AdamW(torch.optim.Optimizer):
             s["step"] = torch.full((), steps, dtype=torch.int64, device=p.device) if group["capturable"] else steps
             self.state[p] = s
         self._share_counts()
+
+
+class Muon(torch.optim.Optimizer):
+    """Muon for matrices: the momentum of each is orthogonalised by Newton-Schulz products before it is subtracted, with ``torch.optim.Muon``'s arguments.
+
+    Parameters have two dimensions or more; leading ones are stacks of matrices (``AdaptedDense.A`` and ``.B``), each orthogonalised by itself.  Vectors (biases,
+    norms) and embeddings belong to an ``AdamW`` beside it.  Momentum is float32.  16-bit parameters get a float32 copy that is what is updated
+    (``master=False``: the parameter itself, rounded at each step); it is taken at a parameter's first step.  ``lr`` may be one float32 in a CUDA tensor.
+    A captured ``step()`` begins no state: make one step with the same gradients before the capture."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, ns_steps=5,
+                 adjust_lr_fn=None, master=True):
+        if not torch.is_tensor(lr) and lr < 0 or weight_decay < 0 or not 0 <= momentum <= 1 or not eps > 0:
+            raise ValueError("lr and weight_decay may not be negative, momentum is in [0, 1], eps above 0")
+        if not 0 <= ns_steps <= 100:
+            raise ValueError("ns_steps is 0 to 100")
+        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+            raise ValueError("adjust_lr_fn is original (also None) or match_rms_adamw")
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov, ns_coefficients=ns_coefficients, eps=eps,
+                                      ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn, master=master))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                raise ValueError(f"Muon is for matrices, a parameter is {tuple(p.shape)}")
+
+    def _state_of(self, p, group, capturing):
+        s = self.state[p]
+        if not s:
+            if capturing:
+                raise RuntimeError("a captured step() begins no state: make a step with the same gradients before the capture")
+            if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                raise TypeError(f"parameters are float32, bfloat16 or float16, not {p.dtype}")
+            if not p.is_contiguous():
+                raise ValueError("parameters are updated in place and have to be contiguous")
+            s["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            if group["master"] and p.dtype != torch.float32:
+                s["master"] = p.detach().float()
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One update of every parameter that has a gradient, a call per type and device."""
+        from . import ops
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        for group in self.param_groups:
+            calls = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise TypeError("gradients have to be dense")
+                s = self._state_of(p, group, capturing)
+                calls.setdefault((p.device, p.dtype, p.grad.dtype, "master" in s), []).append((p, s))
+            for (_, _, _, copies), members in calls.items():
+                ps, ss = zip(*members)
+                ops.muon_step([p.detach() for p in ps], [p.grad for p in ps], [s["momentum_buffer"] for s in ss], group["lr"], group["momentum"],
+                              group["nesterov"], group["weight_decay"], group["ns_coefficients"], group["eps"], group["ns_steps"],
+                              group["adjust_lr_fn"] or "original", [s["master"] for s in ss] if copies else None)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As the base class, but the state keeps its own types (float32 buffers of 16-bit parameters)."""
+        super().load_state_dict(state_dict)
+        names = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        for name, p in zip(names, (p for g in self.param_groups for p in g["params"])):
+            if name in state_dict["state"]:
+                self.state[p] = {k: v.detach().to(p.device, copy=True) if torch.is_tensor(v) else v for k, v in state_dict["state"][name].items()}
