@@ -1294,6 +1294,8 @@ int b200cp_device_status(void) {
   if (v) return fail(B200CP_ERR_TIMEOUT, "gated feed-forward block: a bounded wait ran out in block %d", v & 0xffff);
   if (int rc = muon_device_status(&v)) return rc;
   if (v) return fail(B200CP_ERR_TIMEOUT, "Muon step: a bounded wait ran out in block %d", v & 0xffff);
+  if (int rc = layer_norm_device_status(&v)) return rc;
+  if (v) return fail(B200CP_ERR_TIMEOUT, "layer norm gradients: a bounded wait ran out in block %d", v & 0xffff);
   if (int rc = adapters_device_status(&v)) return rc;
   if (v) return fail(B200CP_ERR_INVALID_ARG, "low-rank adapters: a plan of other rows or of another number of adapters (nothing was computed)");
   return B200CP_OK;

@@ -277,6 +277,7 @@ int kron_device_status(int* out);
 int gated_device_status(int* out);
 int adapters_device_status(int* out);
 int muon_device_status(int* out);
+int layer_norm_device_status(int* out);
 // conv form of the same kernel: G[tap][T][C] from NCHW operands (padded, transposed planes in the scratch)
 bool conv_gemm_tc_supported(int N, int T, int C, int H, int W, int FH, int FW);
 size_t conv_gemm_tc_scratch_floats(int N, int T, int C, int H, int W, int FH, int FW);

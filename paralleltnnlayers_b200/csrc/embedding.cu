@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const __grid_constant__ 
 }
 
 // ---- gradient, 1: places by token, and zeros ------------------------------------------------------------------------------------
-constexpr int kSorters = 8, kSortThreads = 1024, kBins = 1024, kWarps = kSortThreads / 32;
+constexpr int kSorters = 8, kSortThreads = 1024, kFill = 4, kBins = 1024, kWarps = kSortThreads / 32;
 struct Sort {
   int rows, wide, passes, bits;   // bits of a digit
   uint32_t V;
@@ -90,8 +90,11 @@ __global__ void __cluster_dims__(kSorters, 1, 1) __launch_bounds__(kSortThreads)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dependency_wait();
   if (blockIdx.x >= kSorters) {   // zeros
-    const size_t n = (size_t)(gridDim.x - kSorters) * kSortThreads;
-    for (size_t i = (size_t)(blockIdx.x - kSorters) * kSortThreads + tid; i < g.groups; i += n) g.zeros[i] = make_uint4(0, 0, 0, 0);
+    // (a CTA has 64 KB and leaves: a table of 410 MB in 58 us, where CTAs that stay take 66)
+    const size_t first = (size_t)(blockIdx.x - kSorters) * (kSortThreads * kFill) + tid;
+#pragma unroll
+    for (int i = 0; i < kFill; ++i)
+      if (first + i * kSortThreads < g.groups) g.zeros[first + i * kSortThreads] = make_uint4(0, 0, 0, 0);
     if (blockIdx.x == kSorters) {
       if (tid < g.before) g.head[tid] = 0;
       if (tid < g.after) g.tail[tid] = 0;
@@ -172,7 +175,7 @@ struct Sums {
   float* parts;                   // [chunk][the token that began before, the one that goes on][D]
 };
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) embedding_sums_kernel(const __grid_constant__ Sums g) {
+__global__ void __launch_bounds__(256, 4) embedding_sums_kernel(const __grid_constant__ Sums g) {
   grid_dependency_wait();
   const int per = 256 / g.lanes, c = blockIdx.x * per + (int)threadIdx.x / g.lanes;
   const int col = ((int)blockIdx.y * g.lanes + ((int)threadIdx.x & (g.lanes - 1))) * VEC;
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(256) embedding_sums_kernel(const __grid_consta
     for (int i = 0; i < VEC; ++i) x[i] = acc[i] * g.scale;
     store_group(dW + (size_t)now * g.D, pack<T>(x));
   };
-  constexpr int U = 8;
+  constexpr int U = 4;   // rows on their way together (64 registers: four CTAs an SM)
   for (int e = e0; e < e1 && now < g.V; e += U) {
     uint32_t key[U];
     Group<T, VEC> v[U];
@@ -228,17 +231,16 @@ __global__ void __launch_bounds__(256) embedding_sums_kernel(const __grid_consta
 }
 
 // ---- gradient, 3: tokens of several chunks --------------------------------------------------------------------------------------------
-// grid (chunks, columns / 512): the token that goes on behind a chunk and did not begin before it.  Two threads of a CTA share four columns, each with
-// every other part.
-constexpr int kJoinCols = 512;
+// grid (chunks, columns / 4096): the token that goes on behind a chunk and did not begin before it.  A thread has four columns.
+constexpr int kJoinCols = 4096;
 template <typename T>
-__global__ void __launch_bounds__(256) embedding_join_kernel(const __grid_constant__ Sums g) {
+__global__ void __launch_bounds__(1024) embedding_join_kernel(const __grid_constant__ Sums g) {
   grid_dependency_wait();
   const int c = blockIdx.x, e0 = c * g.chunk;
   if ((long long)e0 + g.chunk >= g.rows) return;
   const int e1 = e0 + g.chunk;
-  const uint32_t now = g.key[e1];
-  if (now >= g.V || g.key[e1 - 1] != now || (e0 > 0 && g.key[e0 - 1] == now)) return;
+  const uint32_t now = g.key[e1], last = g.key[e1 - 1], before = e0 > 0 ? g.key[e0 - 1] : g.V;
+  if (now >= g.V || last != now || before == now) return;
   // how many chunks behind this one begin with the token
   int parts = 0;
   for (const int lane = threadIdx.x & 31;;) {
@@ -247,25 +249,24 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const __grid_consta
     parts += not_it ? __ffs(not_it) - 1 : 32;
     if (not_it) break;
   }
-  __shared__ float4 other[128];
-  const int half = threadIdx.x >> 7, q = threadIdx.x & 127, col = blockIdx.y * kJoinCols + q * 4, left = g.D - col;
+  const int col = blockIdx.y * kJoinCols + threadIdx.x * 4, left = g.D - col;
+  if (left <= 0) return;
+  const bool whole = (g.D & 3) == 0;
   float s[4] = {};
-  if (left > 0) {
-    // (the first part is this chunk's second, the others are the first ones of their chunks)
-    const auto part = [&](int p) { return g.parts + ((size_t)(c + p) * 2 + (p == 0)) * g.D + col; };
 #pragma unroll 4
-    for (int p = half; p <= parts; p += 2) {
-      const float* from = part(p);
+  for (int p = 0; p <= parts; ++p) {   // (the first part is this chunk's second, the others are the first ones of their chunks)
+    const float* from = g.parts + ((size_t)(c + p) * 2 + (p == 0)) * g.D + col;
+    float v[4] = {};
+    if (whole) {
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (i < left) s[i] += from[i];
+        if (i < left) v[i] = from[i];
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] += v[i];
   }
-  if (half) other[q] = make_float4(s[0], s[1], s[2], s[3]);
-  __syncthreads();
-  if (half || left <= 0) return;
-  const float4 o = other[q];
-  s[0] += o.x; s[1] += o.y; s[2] += o.z; s[3] += o.w;
   T* to = static_cast<T*>(g.dW) + (size_t)now * g.D + col;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -315,7 +316,8 @@ int sums(Sums g, const Cut& c, cudaStream_t st) {
   B200CP_CUDA_OK(launch_kernel(embedding_sums_kernel<T, VEC>, dim3((unsigned)ceil_div(c.chunks, per), (unsigned)c.slabs), dim3(256), 0, st, true, g));
   B200CP_LAUNCH_OK("embedding_sums_kernel");
   if (c.chunks < 2) return B200CP_OK;
-  B200CP_CUDA_OK(launch_kernel(embedding_join_kernel<T>, dim3((unsigned)c.chunks, (unsigned)ceil_div(g.D, kJoinCols)), dim3(256), 0, st, true, g));
+  B200CP_CUDA_OK(launch_kernel(embedding_join_kernel<T>, dim3((unsigned)c.chunks, (unsigned)ceil_div(g.D, kJoinCols)),
+                               dim3(std::min(1024, (ceil_div(g.D, 4) + 31) / 32 * 32)), 0, st, true, g));
   B200CP_LAUNCH_OK("embedding_join_kernel");
   return B200CP_OK;
 }
@@ -390,9 +392,10 @@ int b200cp_embedding_bwd(int rows, int V, int D, int type, int number_type, cons
   s.before = (int)(from - begin);
   s.tail = reinterpret_cast<unsigned char*>(to);
   s.after = (int)(end - to);
-  const size_t wanted = (s.groups + kSortThreads * 4 - 1) / (kSortThreads * 4);   // four groups a thread, or two CTAs an SM
-  const int fillers = (int)std::min<size_t>(std::max<size_t>(wanted, 1), 2 * (size_t)di.sm_count);
-  B200CP_CUDA_OK(launch_kernel(embedding_sort_kernel, dim3((unsigned)(kSorters * (1 + ceil_div(fillers, kSorters)))), dim3(kSortThreads), 0, st, true, s));
+  const size_t fillers = std::max<size_t>(1, (s.groups + kSortThreads * kFill - 1) / (kSortThreads * kFill));
+  const size_t ctas = kSorters * (1 + (fillers + kSorters - 1) / kSorters);
+  if (ctas > 0x7fffffffull) return fail(B200CP_ERR_UNSUPPORTED, "%s: a table of %zu bytes", who, bytes);
+  B200CP_CUDA_OK(launch_kernel(embedding_sort_kernel, dim3((unsigned)ctas), dim3(kSortThreads), 0, st, true, s));
   B200CP_LAUNCH_OK("embedding_sort_kernel");
   return by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;

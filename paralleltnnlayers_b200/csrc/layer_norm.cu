@@ -8,34 +8,53 @@
 // 8 to 32 features a thread.
 //
 // The gradients are one kernel too: a CTA walks over its rows with the sums of dw and db of its threads' features in registers (8 features a
-// thread, rows of up to 8192), the next row on its way while this one's two sums are joined; the CTAs' sums are added by a second launch in
-// their order, so that a result has the same bits each time.  Longer rows are read twice: for dh and for the sums over rows.
+// thread, rows of up to 8192); the next rows come by bulk copies into a ring in shared memory meanwhile (rows that do not lie on 16-byte boundaries, and short
+// ones, into registers, one ahead).  The CTAs' sums are added by a second launch in their order, so that a result has the same bits each
+// time.  Longer rows are read twice: for dh and for the sums over rows.  Every wait is bounded: one that runs out sets a status word.
 #include <algorithm>
 
 #include "common.cuh"
+#include "tc_common.cuh"
 #include "vec_io.cuh"
 
 namespace b200cp {
+
+__device__ int g_layer_norm_status = 0;   // 0 ok; otherwise (code << 16) | (block index & 0xffff)
+
 namespace {
 
 constexpr int kWarpRow = 256;        // features of a row that a warp takes
 constexpr int kRows = 8;             // rows, and warps, of a CTA then
 constexpr int kGradRow = 8192;       // of a row whose gradients are one pass
+constexpr int kGradEach = 16;        // of them to a thread (8 where they do not lie on 16-byte boundaries, and in short rows: those keep a row ahead in registers)
+constexpr int kGradThreads = kGradRow / kGradEach;   // of a CTA at most, and of an SM at 128 registers each
 
-// Sums over the CTA of two values: `red` holds 2 x 32 pairs, used in turn (`turn` changes between calls), so that one barrier is enough.
-__device__ __forceinline__ float2 block_sum(float a, float b, float2* red, int turn) {
-  a = warp_sum(a);
-  b = warp_sum(b);
-  float2* r = red + turn * 32;
-  if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = make_float2(a, b);
+// Sums of two values over a warp: of the first one in lanes 0 to 15, of the second in the others.
+__device__ __forceinline__ float half_sums(float a, float b) {
+  const bool up = threadIdx.x & 16;
+  float s = (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, 16);
+#pragma unroll
+  for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+__device__ __forceinline__ float2 both(float s) { return make_float2(__shfl_sync(0xffffffffu, s, 0), __shfl_sync(0xffffffffu, s, 16)); }
+// Sums over the CTA of two values: `red` holds 2 x 2 x 32 of the warps', used in turn (`turn` changes between calls), so that one barrier is enough.
+constexpr int kRed = 128;
+__device__ __forceinline__ float2 block_sum(float a, float b, float* red, int turn) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, i = lane & 15;
+  float* r = red + turn * 64 + (lane & 16) * 2;   // (this half's)
+  const float s = half_sums(a, b);
+  if (i == 0) r[threadIdx.x >> 5] = s;
   __syncthreads();
-  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-  const float2 s = lane < warps ? r[lane] : make_float2(0.f, 0.f);
-  return make_float2(warp_sum(s.x), warp_sum(s.y));
+  float v = i < warps ? r[i] : 0.f;
+  if (warps > 16 && i + 16 < warps) v += r[i + 16];
+#pragma unroll
+  for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return both(v);
 }
 template <bool WARP>
-__device__ __forceinline__ float2 row_sum(float a, float b, float2* red, int turn) {
-  if constexpr (WARP) return make_float2(warp_sum(a), warp_sum(b));
+__device__ __forceinline__ float2 row_sum(float a, float b, float* red, int turn) {
+  if constexpr (WARP) return both(half_sums(a, b));
   return block_sum(a, b, red, turn);
 }
 
@@ -48,7 +67,7 @@ struct Forward {
 };
 template <typename T, typename W, int VEC, int K, bool WARP>
 __global__ void __launch_bounds__(WARP ? 32 * kRows : 1024) norm_kernel(const __grid_constant__ Forward g) {
-  __shared__ float2 red[64];
+  __shared__ float red[kRed];
   const int row = WARP ? blockIdx.x * kRows + (threadIdx.x >> 5) : blockIdx.x, t = WARP ? threadIdx.x & 31 : threadIdx.x, n = WARP ? 32 : blockDim.x;
   grid_dependency_wait();
   if (WARP && row >= g.rows) return;
@@ -127,7 +146,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRows : 1024) norm_kernel(const __
     if (w) unpack(load_group<W, VEC>(w + c), m);
     if (b) unpack(load_group<W, VEC>(b + c), a);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) a[i] = fmaf((v[k][i] - off) * rstd, m[i], a[i]);
+    for (int i = 0; i < VEC; ++i) a[i] = fmaf(fmaf(v[k][i], rstd, -off * rstd), m[i], a[i]);
     store_group(y + c, pack<T>(a));
   }
 }
@@ -135,7 +154,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRows : 1024) norm_kernel(const __
 // Rows that a CTA does not hold: three passes, the second and third from the caches.
 template <typename T, typename W, int VEC>
 __global__ void __launch_bounds__(1024) norm_wide_kernel(const __grid_constant__ Forward g) {
-  __shared__ float2 red[64];
+  __shared__ float red[kRed];
   grid_dependency_wait();
   const size_t at = (size_t)blockIdx.x * g.D;
   const T *x = static_cast<const T*>(g.x) + at, *src = x;
@@ -208,6 +227,33 @@ struct Backward {
   void* dx;          // or null
   float* partial;    // [CTA][dw, db][D], or null
 };
+// What a row adds to a thread's sums, and its dh.  n = h rstd - mean rstd in one operation, dh = rstd g - rstd mean(g) - n rstd mean(g n) in two.  Instructions count
+// here: 8192 x 4096 in bfloat16 with dH (HBM: 41 us) took 69 us with eight features a thread and 350 instructions a row and warp, 63 with these forms and
+// sums of two values at once, and takes 53 with 16 features a thread, which halves what a row costs beside its values (115 with a row ahead in registers).
+template <typename T, int VEC>
+__device__ __forceinline__ void add_group(const Group<T, VEC>& h, const Group<T, VEC>& dy, const float (&w)[VEC], float rstd, float shift, float (&n)[VEC],
+                                          float (&e)[VEC], float& s1, float& s2, float (&dw)[VEC], float (&db)[VEC]) {
+  float x[VEC], d[VEC];
+  unpack(h, x);
+  unpack(dy, d);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    n[i] = fmaf(x[i], rstd, shift);
+    e[i] = d[i] * w[i];
+    s1 += e[i];
+    s2 = fmaf(e[i], n[i], s2);
+    dw[i] = fmaf(d[i], n[i], dw[i]);
+    db[i] += d[i];
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ Group<T, VEC> dx_group(const float (&n)[VEC], const float (&e)[VEC], const Group<T, VEC>* dh, float rstd, float c1, float c2) {
+  float a[VEC] = {};
+  if (dh) unpack(*dh, a);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) a[i] = fmaf(-n[i], c2, fmaf(e[i], rstd, a[i] - c1));
+  return pack<T>(a);
+}
 template <typename T, int VEC, int K>
 struct RowOf {   // what a thread has of a row, as it lies in memory
   Group<T, VEC> h[K], dy[K], dh[K];
@@ -228,8 +274,8 @@ __device__ __forceinline__ void load_row(const Backward& g, int row, int t, int 
   }
 }
 template <typename T, typename W, int VEC, int K, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * kRows : 1024) norm_grads_kernel(const __grid_constant__ Backward g) {
-  __shared__ float2 red[64];
+__global__ void __launch_bounds__(WARP ? 32 * kRows : kGradThreads, 1) norm_grads_kernel(const __grid_constant__ Backward g) {
+  __shared__ float red[kRed];
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x, n = WARP ? 32 : blockDim.x;
   const int first = WARP ? blockIdx.x * kRows + (threadIdx.x >> 5) : blockIdx.x, step = WARP ? gridDim.x * kRows : gridDim.x;
   grid_dependency_wait();
@@ -251,35 +297,18 @@ __global__ void __launch_bounds__(WARP ? 32 * kRows : 1024) norm_grads_kernel(co
   for (int row = first; row < g.rows; row += step, turn ^= 1) {
     const RowOf<T, VEC, K> now = next;
     if (row < g.rows - step) load_row(g, row + step, t, n, next);
-    float s1 = 0.f, s2 = 0.f;
+    float s1 = 0.f, s2 = 0.f, x[K][VEC], e[K][VEC];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if ((k * n + t) * VEC >= g.D) continue;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = to_float(now.dy[k].v[i]), x = (to_float(now.h[k].v[i]) - now.mean) * now.rstd, e = d * w[k][i];
-        s1 += e;
-        s2 = fmaf(e, x, s2);
-        dw[k][i] = fmaf(d, x, dw[k][i]);
-        db[k][i] += d;
-      }
-    }
+    for (int k = 0; k < K; ++k)
+      if ((k * n + t) * VEC < g.D) add_group(now.h[k], now.dy[k], w[k], now.rstd, -now.mean * now.rstd, x[k], e[k], s1, s2, dw[k], db[k]);
     if (!g.dx) continue;
     const float2 q = row_sum<WARP>(s1, s2, red, turn);
-    const float c1 = q.x * inv, c2 = q.y * inv;
+    const float c1 = q.x * inv * now.rstd, c2 = q.y * inv * now.rstd;
     T* dx = static_cast<T*>(g.dx) + (size_t)row * g.D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * n + t) * VEC;
-      if (c >= g.D) continue;
-      float a[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float x = (to_float(now.h[k].v[i]) - now.mean) * now.rstd, e = to_float(now.dy[k].v[i]) * w[k][i];
-        a[i] = now.rstd * (e - c1 - x * c2);
-        if (g.dh) a[i] += to_float(now.dh[k].v[i]);
-      }
-      store_group(dx + c, pack<T>(a));
+      if (c < g.D) store_group(dx + c, dx_group(x[k], e[k], g.dh ? &now.dh[k] : nullptr, now.rstd, c1, c2));
     }
   }
   if (!g.partial) return;
@@ -317,10 +346,117 @@ __global__ void __launch_bounds__(WARP ? 32 * kRows : 1024) norm_grads_kernel(co
   }
 }
 
+// The same for rows of whole 16-byte groups that a CTA shares: the rows to come are on their way into `slots` places of shared memory.
+struct Ring {
+  int slots, row;    // places; bytes of a row
+};
+__device__ __forceinline__ void bulk_load(void* to, const void* from, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(to)), "l"(from), "r"(bytes),
+               "r"(tc::smem_u32(bar))
+               : "memory");
+}
+constexpr int kMostSlots = 8;
+template <typename T, typename W, int VEC, int K>
+__global__ void __launch_bounds__(kGradThreads, 1) norm_grads_ring_kernel(const __grid_constant__ Backward g, const __grid_constant__ Ring ring) {
+  extern __shared__ __align__(16) uint8_t places[];   // [slot][h, dy, dh][row]
+  __shared__ float red[kRed];
+  __shared__ uint64_t full[kMostSlots];
+  __shared__ volatile int given_up[2];   // used in turn, so that all threads see the same after a barrier
+  const int t = threadIdx.x, n = blockDim.x, step = gridDim.x;
+  const bool added = g.dh && g.dx;
+  const int arrays = added ? 3 : 2;
+  if (t == 0) {
+    for (int i = 0; i < ring.slots; ++i) tc::mbar_init(&full[i], 1);
+    given_up[0] = given_up[1] = 0;
+    tc::fence_barrier_init();
+  }
+  __syncthreads();
+  grid_dependency_wait();
+  const auto fetch = [&](int row, int slot) {
+    uint8_t* to = places + (size_t)slot * arrays * ring.row;
+    tc::mbar_expect_tx(&full[slot], arrays * ring.row);
+    bulk_load(to, static_cast<const T*>(g.h) + (size_t)row * g.D, ring.row, &full[slot]);
+    bulk_load(to + ring.row, static_cast<const T*>(g.dy) + (size_t)row * g.D, ring.row, &full[slot]);
+    if (added) bulk_load(to + 2 * ring.row, static_cast<const T*>(g.dh) + (size_t)row * g.D, ring.row, &full[slot]);
+  };
+  if (t == 0)
+    for (int i = 0; i < ring.slots && (long long)blockIdx.x + (long long)i * step < g.rows; ++i) fetch(blockIdx.x + i * step, i);
+  float w[K][VEC], dw[K][VEC], db[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * n + t) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      w[k][i] = 1.f;
+      dw[k][i] = db[k][i] = 0.f;
+    }
+    if (g.w && c < g.D) unpack(load_group<W, VEC>(static_cast<const W*>(g.w) + c), w[k]);
+  }
+  const float inv = 1.f / (float)g.D;
+  float mean = g.mean[blockIdx.x], rstd = g.rstd[blockIdx.x];
+  int turn = 0, slot = 0, phase = 0;
+  for (int row = blockIdx.x; row < g.rows; row += step, turn ^= 1) {
+    const float mu = mean, rs = rstd;
+    const bool more = row < g.rows - step;
+    if (more) {
+      mean = g.mean[row + step];
+      rstd = g.rstd[row + step];
+    }
+    if (!tc::mbar_wait(&full[slot], phase)) given_up[turn] = 1;
+    const T* place = reinterpret_cast<const T*>(places + (size_t)slot * arrays * ring.row);
+    Group<T, VEC> dh[K];
+    float s1 = 0.f, s2 = 0.f, x[K][VEC], e[K][VEC];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * n + t) * VEC;
+      if (c >= g.D) continue;
+      if (added) dh[k] = load_group<T, VEC>(place + 2 * g.D + c);
+      add_group(load_group<T, VEC>(place + c), load_group<T, VEC>(place + g.D + c), w[k], rs, -mu * rs, x[k], e[k], s1, s2, dw[k], db[k]);
+    }
+    float2 q = make_float2(0.f, 0.f);
+    if (g.dx) q = block_sum(s1, s2, red, turn);
+    else __syncthreads();
+    if (given_up[turn]) break;
+    // (all threads have taken what they need of the place)
+    if (t == 0 && (long long)row + (long long)ring.slots * step < g.rows) fetch(row + ring.slots * step, slot);
+    if (++slot == ring.slots) {
+      slot = 0;
+      phase ^= 1;
+    }
+    if (!g.dx) continue;
+    const float c1 = q.x * inv * rs, c2 = q.y * inv * rs;
+    T* dx = static_cast<T*>(g.dx) + (size_t)row * g.D;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * n + t) * VEC;
+      if (c < g.D) store_group(dx + c, dx_group(x[k], e[k], added ? &dh[k] : nullptr, rs, c1, c2));
+    }
+  }
+  if (given_up[0] | given_up[1]) {   // copies in flight land before the shared memory is given back
+    if (t == 0) atomicCAS(&g_layer_norm_status, 0, (1 << 16) | (blockIdx.x & 0xffff));
+    const long long t0 = clock64();
+    while (clock64() - t0 < 40000000ll) {
+    }
+    return;
+  }
+  if (!g.partial) return;
+  float* to = g.partial + (size_t)blockIdx.x * 2 * g.D;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * n + t) * VEC;
+    if (c >= g.D) continue;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      to[c + i] = dw[k][i];
+      to[g.D + c + i] = db[k][i];
+    }
+  }
+}
+
 // Long rows: dh, a CTA per row.
 template <typename T, typename W, int VEC>
 __global__ void __launch_bounds__(1024) norm_wide_dx_kernel(const __grid_constant__ Backward g) {
-  __shared__ float2 red[64];
+  __shared__ float red[kRed];
   grid_dependency_wait();
   const size_t at = (size_t)blockIdx.x * g.D;
   const T *h = static_cast<const T*>(g.h) + at, *dy = static_cast<const T*>(g.dy) + at, *dh = g.dh ? static_cast<const T*>(g.dh) + at : nullptr;
@@ -389,10 +525,10 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(const __grid_constant
   }
 }
 
-// dw and db from the CTAs' sums: 32 columns of one of them per CTA, eight threads to a column.
+// dw and db from the CTAs' sums: 32 columns of one of them per CTA, a warp for every 32nd part.
 template <typename W>
-__global__ void __launch_bounds__(256) norm_join_kernel(int parts, int D, const float* partial, W* dw, W* db) {
-  __shared__ float all[8][33];
+__global__ void __launch_bounds__(1024) norm_join_kernel(int parts, int D, const float* partial, W* dw, W* db) {
+  __shared__ float all[32][33];
   const int x = threadIdx.x & 31, q = threadIdx.x >> 5, groups = (D + 31) / 32, second = (int)blockIdx.x >= groups;
   const int c = ((int)blockIdx.x - second * groups) * 32 + x;
   grid_dependency_wait();
@@ -400,17 +536,14 @@ __global__ void __launch_bounds__(256) norm_join_kernel(int parts, int D, const 
   float s = 0.f;
   if (c < D) {
 #pragma unroll 8
-    for (int b = q; b < parts; b += 8) s += from[(size_t)b * 2 * D];
+    for (int b = q; b < parts; b += 32) s += from[(size_t)b * 2 * D];
   }
   all[q][x] = s;
   __syncthreads();
-  if (q == 0 && c < D) {
-    s = all[0][x];
-#pragma unroll
-    for (int k = 1; k < 8; ++k) s += all[k][x];
-    W* to = second ? db : dw;
-    if (to) to[c] = from_float<W>(s);
-  }
+  s = warp_sum(all[x][q]);   // column q
+  const int column = c - x + q;
+  W* to = second ? db : dw;
+  if (x == 0 && column < D && to) to[column] = from_float<W>(s);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
@@ -443,34 +576,48 @@ int forward(const Forward& g, cudaStream_t st) {
   return vec ? forward_by_size<T, W, kPerLoad<T>>(g, st) : forward_by_size<T, W, 1>(g, st);
 }
 
-// CTAs that share the rows of a gradient: as many as an SM holds (by threads, at 64 registers each), with eight rows each where there are that
-// many: a CTA's sums are 8 bytes a feature, as its row's reads and writes are.
+// CTAs that share the rows of a gradient: as many as an SM holds, with eight rows each where there are that many (a CTA's sums are 8 bytes a feature, as what
+// a row of 16-bit values reads and writes).
 int grad_ctas(int rows, int D, int sm_count) {
-  const bool warp = D <= kWarpRow, wide = D > kGradRow;
+  const bool warp = D <= kWarpRow;
   const int units = warp ? ceil_div(rows, kRows) : rows;
-  const int threads = warp ? 32 * kRows : wide ? 256 : threads_of(D, 8);
-  const int most = sm_count * std::max(1, 1024 / threads);
-  return std::max(1, std::min(units, std::max(std::min(sm_count, most), std::min(most, ceil_div(units, 8)))));
+  const int threads = warp ? 32 * kRows : D > kGradRow ? 256 : threads_of(D, kGradEach);
+  const int most = sm_count * std::max(1, kGradThreads / threads);
+  return std::max(1, std::min(units, std::max(sm_count, std::min(most, ceil_div(units, 8)))));
 }
 template <typename T, typename W, int VEC>
 int grads(const Backward& g, int ctas, cudaStream_t st) {
-  constexpr int K = 8 / VEC;
   if (g.D <= kWarpRow) {
-    B200CP_CUDA_OK(launch_kernel(norm_grads_kernel<T, W, VEC, K, true>, dim3(ctas), dim3(32 * kRows), 0, st, true, g));
+    B200CP_CUDA_OK(launch_kernel(norm_grads_kernel<T, W, VEC, 8 / VEC, true>, dim3(ctas), dim3(32 * kRows), 0, st, true, g));
     B200CP_LAUNCH_OK("norm_grads_kernel");
-  } else if (g.D <= kGradRow) {
-    B200CP_CUDA_OK(launch_kernel(norm_grads_kernel<T, W, VEC, K, false>, dim3(ctas), dim3(threads_of(g.D, 8)), 0, st, true, g));
+    return B200CP_OK;
+  }
+  if constexpr (VEC > 1) {
+    if (g.D <= kGradRow) {
+      // (what an SM has of shared memory is shared by as many CTAs as its threads make; two places for rows of 8192 floats are 192 KB)
+      const int threads = threads_of(g.D, kGradEach), row = g.D * (int)sizeof(T), slot = (g.dh && g.dx ? 3 : 2) * row,
+                room = 216 * 1024 / std::max(1, kGradThreads / threads) - 2048;
+      const Ring ring{std::max(2, std::min(kMostSlots, room / slot)), row};
+      const auto kern = norm_grads_ring_kernel<T, W, VEC, kGradEach / VEC>;
+      static std::atomic<int> set[64];
+      B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, ring.slots * slot));
+      B200CP_CUDA_OK(launch_kernel(kern, dim3(ctas), dim3(threads), (size_t)ring.slots * slot, st, true, g, ring));
+      B200CP_LAUNCH_OK("norm_grads_ring_kernel");
+      return B200CP_OK;
+    }
+  } else if (g.D <= kGradThreads * 8) {
+    B200CP_CUDA_OK(launch_kernel(norm_grads_kernel<T, W, 1, 8, false>, dim3(ctas), dim3(threads_of(g.D, 8)), 0, st, true, g));
     B200CP_LAUNCH_OK("norm_grads_kernel");
-  } else {
-    if (g.dx) {
-      B200CP_CUDA_OK(launch_kernel(norm_wide_dx_kernel<T, W, VEC>, dim3(g.rows), dim3(1024), 0, st, true, g));
-      B200CP_LAUNCH_OK("norm_wide_dx_kernel");
-    }
-    if (g.partial) {
-      const unsigned x = (unsigned)((g.D + 256LL * VEC - 1) / (256LL * VEC));
-      B200CP_CUDA_OK(launch_kernel(norm_columns_kernel<T, VEC>, dim3(x, (unsigned)std::min(ctas, 65535)), dim3(256), 0, st, true, g));
-      B200CP_LAUNCH_OK("norm_columns_kernel");
-    }
+    return B200CP_OK;
+  }
+  if (g.dx) {
+    B200CP_CUDA_OK(launch_kernel(norm_wide_dx_kernel<T, W, VEC>, dim3(g.rows), dim3(1024), 0, st, true, g));
+    B200CP_LAUNCH_OK("norm_wide_dx_kernel");
+  }
+  if (g.partial) {
+    const unsigned x = (unsigned)((g.D + 256LL * VEC - 1) / (256LL * VEC));
+    B200CP_CUDA_OK(launch_kernel(norm_columns_kernel<T, VEC>, dim3(x, (unsigned)ctas), dim3(256), 0, st, true, g));
+    B200CP_LAUNCH_OK("norm_columns_kernel");
   }
   return B200CP_OK;
 }
@@ -481,8 +628,7 @@ int backward(Backward g, int ctas, void* dw, void* db, cudaStream_t st) {
   vec = vec && !(reinterpret_cast<uintptr_t>(g.w) & (kPerLoad<T> * sizeof(W) - 1));
   if (int rc = vec ? grads<T, W, kPerLoad<T>>(g, ctas, st) : grads<T, W, 1>(g, ctas, st)) return rc;
   if (!g.partial) return B200CP_OK;
-  const int parts = g.D > kGradRow ? std::min(ctas, 65535) : ctas;
-  B200CP_CUDA_OK(launch_kernel(norm_join_kernel<W>, dim3(2 * ceil_div(g.D, 32)), dim3(256), 0, st, true, parts, g.D, g.partial, static_cast<W*>(dw),
+  B200CP_CUDA_OK(launch_kernel(norm_join_kernel<W>, dim3(2 * ceil_div(g.D, 32)), dim3(1024), 0, st, true, ctas, g.D, g.partial, static_cast<W*>(dw),
                                static_cast<W*>(db)));
   B200CP_LAUNCH_OK("norm_join_kernel");
   return B200CP_OK;
@@ -504,6 +650,15 @@ int by_types(int type, int weight_type, F f) {
 }
 
 }  // namespace
+
+int layer_norm_device_status(int* out) {
+  int v = 0, zero = 0;
+  B200CP_CUDA_OK(cudaMemcpyFromSymbol(&v, g_layer_norm_status, sizeof(int)));
+  if (v) B200CP_CUDA_OK(cudaMemcpyToSymbol(g_layer_norm_status, &zero, sizeof(int)));
+  *out = v;
+  return B200CP_OK;
+}
+
 }  // namespace b200cp
 
 using namespace b200cp;

@@ -62,7 +62,7 @@ __device__ __forceinline__ double warp_sum(double x) {
 }
 
 // ======== matrices with a side of at most 64 =====================================================================================
-constexpr int kSmall = 64, kTableSmall = 224, kSub = 128, kGramThreads = 288;
+constexpr int kSmall = 64, kTableSmall = 224, kSub = 128;
 struct SmallEntry {
   Pointers at;
   int rows, cols;
@@ -70,6 +70,7 @@ struct SmallEntry {
   int chunks, length;        // of a matrix: parts of its longer side, and how much of it each has (a multiple of kSub)
   int first;                 // CTA of the launch over parts
   int matrix;                // matrices before
+  int vec;                   // four values of every array lie on its boundary, and rows are multiples of four
   float scale;               // of the rate
   size_t gram, q;            // in doubles, in floats: of its first matrix
 };
@@ -93,177 +94,260 @@ __device__ __forceinline__ int entry_of(const SmallTable& t, int block, F first)
   }
   return a;
 }
-// Register tiles of TS x TS of the upper triangle of 16 x 16 of them
-__device__ __forceinline__ void tile_of(int t, int& ti, int& tj) {
-  ti = 0;
-  for (int left = 16; t >= left; --left, ++ti) t -= left;
-  tj = ti + t;
+// Sides are padded to N = 16 TS with TS = 1, 2, 4.  A symmetric result has 2 TS x 2 TS tiles of 8 x 8; those on and above the diagonal are taken in TS groups
+// of 2 TS + 1: rows g and 2 TS - 1 - g of tiles.
+template <int TS>
+struct Side {
+  static constexpr int N = 16 * TS, LD = N + 4, rows = 2 * TS, slots = 2 * TS + 1, tiles = TS * slots;   // (LD: fragments without bank conflicts)
+  static constexpr int sub = 2048 / N;                  // of the longer side that a CTA holds: 2048 values
+  static constexpr int slices = 8 / TS;                 // warps that share a group, each with 16 of sub
+  static constexpr int part = tiles * 64;               // doubles of a part of A, [group][slot][lane][2]
+  __device__ static __forceinline__ void tile(int group, int slot, int& ti, int& tj) {
+    const int first = rows - group;
+    ti = slot < first ? group : rows - 1 - group;
+    tj = slot < first ? group + slot : ti + slot - first;
+  }
+};
+constexpr int kPart[5] = {0, Side<1>::part, Side<2>::part, 0, Side<4>::part};
+// c += a b of 8 x 4 by 4 x 8 in 64 bits: a is of row lane / 4 and k lane % 4, b of column lane / 4, c of row lane / 4 and columns 2 (lane % 4) and one on.
+// (The same rate as fma, a fourth of the loads from shared memory: 64 x 64 x 64 in 1.3 us, with tiles of 4 x 2 in fma 4.8.)
+__device__ __forceinline__ void mma_f64(double (&c)[2], double a, double b) {
+  asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
-constexpr int kTiles = 136;
+
+// The 2048 values of a matrix that a CTA of 256 threads takes at a time: eight per thread, VEC neighbours in memory together, all on their way at once.
+template <int TS, int VEC>
+struct Values {
+  static constexpr int each = 8 / VEC, SUB = Side<TS>::sub;
+  int n, ks;                 // sizes of what is there: of the smaller side, of the longer one
+  bool wide;
+  unsigned inverse;          // 2^32 / (n / VEC), rounded up: exact quotients for numbers below 2^16
+  size_t pitch;
+  __device__ Values(const SmallEntry& e) : n(side_of(e)), ks(0), wide(e.rows <= e.cols), inverse(0xffffffffu / (unsigned)max(1, n / VEC) + 1), pitch(e.cols) {}
+  // group j of this thread: its place, and whether it is there
+  __device__ __forceinline__ bool place(int j, int& row, int& k) const {
+    const int i = threadIdx.x + j * 256;
+    if (wide) {
+      row = i / (SUB / VEC);
+      k = i % (SUB / VEC) * VEC;
+      return row < n && k < ks;
+    }
+    const int per = n / VEC;
+    k = per == 1 ? i : (int)__umulhi((unsigned)i, inverse);
+    row = (i - k * per) * VEC;
+    return k < ks;
+  }
+  __device__ __forceinline__ size_t at(int row, int k) const { return wide ? (size_t)row * pitch + k : (size_t)k * n + row; }
+  template <typename T>
+  __device__ __forceinline__ void load(const T* from, int k0, float (&x)[8]) const {
+    Group<T, VEC> v[each];
+#pragma unroll
+    for (int j = 0; j < each; ++j) {
+      int row, k;
+      if (place(j, row, k)) v[j] = load_group<T, VEC>(from + at(row, k0 + k));
+      else
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[j].v[i] = from_float<T>(0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < each; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[j * VEC + i] = to_float(v[j].v[i]);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* to, int k0, const float (&x)[8]) const {
+#pragma unroll
+    for (int j = 0; j < each; ++j) {
+      int row, k;
+      if (!place(j, row, k)) continue;
+      float v[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = x[j * VEC + i];
+      store_group(to + at(row, k0 + k), pack<T>(v));
+    }
+  }
+  // f(row, k, value) of what has a place in N x SUB (zeros where nothing is)
+  template <typename F>
+  __device__ __forceinline__ void each_of(float (&x)[8], F f) const {
+#pragma unroll
+    for (int j = 0; j < each; ++j) {
+      int row, k;
+      const bool in = place(j, row, k);
+      if (!in && (wide ? row >= Side<TS>::N : k >= SUB)) continue;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f(wide ? row : row + i, wide ? k + i : k, x[j * VEC + i]);
+    }
+  }
+};
 
 // A part of A, in 64 bits, from a part of the longer side; the momentum is brought up to date on the way.
-template <typename G, int TS>
+template <typename G, int TS, int VEC>
 __device__ __forceinline__ void gram_part(const SmallTable& t, const SmallEntry& e, int matrix, int chunk, double* u) {
-  constexpr int N = 16 * TS, LD = N + 2;
-  const int n = side_of(e), len = max(e.rows, e.cols), tid = threadIdx.x;
-  const bool wide = e.rows <= e.cols;
+  using S = Side<TS>;
+  constexpr int LD = S::LD;
+  Values<TS, VEC> values(e);
+  const int n = values.n, len = max(e.rows, e.cols), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t base = (size_t)matrix * e.rows * e.cols;
   const G* g = static_cast<const G*>(e.at.g) + base;
   float* m = e.at.m ? e.at.m + base : nullptr;
-  const int half = tid / 144, slot = tid - half * 144;
-  int ti = 0, tj = 0;
-  if (slot < kTiles) tile_of(slot, ti, tj);
-  double acc[TS][TS] = {};
+  const int group = warp % TS, slice = warp / TS;
+  double acc[S::slots][2] = {};
   const int l0 = chunk * e.length, l1 = min(len, l0 + e.length);
-  for (int i = tid; i < kSub * LD; i += kGramThreads) u[i] = 0.0;   // (rows past n stay zero)
-  for (int k0 = l0; k0 < l1; k0 += kSub) {
-    const int ks = min(kSub, l1 - k0);
-    __syncthreads();
-    for (int i = tid; i < n * kSub; i += kGramThreads) {
-      const int row = wide ? i / kSub : i % n, k = wide ? i % kSub : i / n;
-      double d = 0.0;
-      if (k < ks) {
-        const size_t at = wide ? (size_t)row * e.cols + k0 + k : (size_t)(k0 + k) * n + row;
-        float x = to_float(g[at]);
-        if (m) {
-          const float b = momentum_of<G>(t.r, x, m[at]);
-          m[at] = b;
-          x = direction_of(t.r, x, b);
-        }
-        d = (double)x;
-      }
-      u[k * LD + row] = d;
+  if (n < S::N)
+    for (int i = tid; i < S::sub * LD; i += 256) u[i] = 0.0;   // (rows past n stay zero)
+  for (int k0 = l0; k0 < l1; k0 += S::sub) {
+    values.ks = min(S::sub, l1 - k0);
+    float x[8], b[8];
+    values.load(g, k0, x);
+    if (m) {
+      values.load(m, k0, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[i] = momentum_of<G>(t.r, x[i], b[i]);
+      values.store(m, k0, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = direction_of(t.r, x[i], b[i]);
     }
     __syncthreads();
-    if (slot < kTiles) {
-#pragma unroll 2
-      for (int k = half; k < kSub; k += 2) {
-        double a[TS], b[TS];
+    values.each_of(x, [&](int row, int k, float v) {
+      if (row < n) u[k * LD + row] = (double)v;
+    });
+    __syncthreads();
+    const double* from = u + (slice * 16 + (lane & 3)) * LD + (lane >> 2);
 #pragma unroll
-        for (int i = 0; i < TS; ++i) {
-          a[i] = u[k * LD + ti * TS + i];
-          b[i] = u[k * LD + tj * TS + i];
-        }
+    for (int k = 0; k < 16; k += 4) {
+      const double a0 = from[k * LD + group * 8], a1 = from[k * LD + (S::rows - 1 - group) * 8];
 #pragma unroll
-        for (int i = 0; i < TS; ++i)
-#pragma unroll
-          for (int j = 0; j < TS; ++j) acc[i][j] = fma(a[i], b[j], acc[i][j]);
+      for (int s = 0; s < S::slots; ++s) {
+        int ti, tj;
+        S::tile(group, s, ti, tj);
+        mma_f64(acc[s], s < S::rows - group ? a0 : a1, from[k * LD + tj * 8]);
       }
     }
   }
+  // the slices' sums, in their order
   __syncthreads();
-  if (half == 1 && slot < kTiles) {
 #pragma unroll
-    for (int i = 0; i < TS; ++i)
-#pragma unroll
-      for (int j = 0; j < TS; ++j) u[slot * TS * TS + i * TS + j] = acc[i][j];
+  for (int s = 0; s < S::slots; ++s) {
+    double* to = u + ((slice * TS + group) * S::slots + s) * 64 + lane * 2;
+    to[0] = acc[s][0];
+    to[1] = acc[s][1];
   }
   __syncthreads();
-  if (half == 0 && slot < kTiles) {   // [tile][TS][TS]
-    double* to = t.gram + e.gram + ((size_t)matrix * e.chunks + chunk) * (kTiles * TS * TS) + slot * TS * TS;
+  double* to = t.gram + e.gram + ((size_t)matrix * e.chunks + chunk) * S::part;
+  for (int i = tid; i < S::part; i += 256) {
+    double s = u[i];
 #pragma unroll
-    for (int i = 0; i < TS * TS; ++i) to[i] = acc[i / TS][i % TS] + u[slot * TS * TS + i];
+    for (int q = 1; q < S::slices; ++q) s += u[q * S::part + i];
+    to[i] = s;
   }
 }
+constexpr int gram_doubles(int ts) {   // of shared memory: the values, or the slices' sums
+  return ts == 1 ? std::max(Side<1>::sub * Side<1>::LD, 8 * Side<1>::part) : ts == 2 ? std::max(Side<2>::sub * Side<2>::LD, 4 * Side<2>::part)
+                                                                               : std::max(Side<4>::sub * Side<4>::LD, 2 * Side<4>::part);
+}
 template <typename G>
-__global__ void __launch_bounds__(kGramThreads) muon_gram_kernel(const __grid_constant__ SmallTable t) {
-  extern __shared__ double work[];
+__global__ void __launch_bounds__(256, 3) muon_gram_kernel(const __grid_constant__ SmallTable t) {
+  extern __shared__ __align__(16) double work[];
   grid_dependency_wait();
   const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.first; })];
   const int at = (int)blockIdx.x - e.first, matrix = at / e.chunks, chunk = at - matrix * e.chunks, n = side_of(e);
-  if (n <= 16) gram_part<G, 1>(t, e, matrix, chunk, work);
-  else if (n <= 32) gram_part<G, 2>(t, e, matrix, chunk, work);
-  else gram_part<G, 4>(t, e, matrix, chunk, work);
+#define B200CP_GRAM(TS) (e.vec ? gram_part<G, TS, 4>(t, e, matrix, chunk, work) : gram_part<G, TS, 1>(t, e, matrix, chunk, work))
+  if (n <= 16) B200CP_GRAM(1);
+  else if (n <= 32) B200CP_GRAM(2);
+  else B200CP_GRAM(4);
+#undef B200CP_GRAM
 }
 
-// out = x y, all symmetric and commuting: only tiles on and above the diagonal are formed.  Rows of N doubles.
-template <int TS>
-__device__ __forceinline__ void symmetric_product(const double* x, const double* y, double* out) {
-  constexpr int N = 16 * TS;
-  const int t = threadIdx.x;
-  if (t < kTiles) {
-    int ti, tj;
-    tile_of(t, ti, tj);
-    double acc[TS][TS] = {};
+// out = put(x y), all symmetric and commuting, rows of LD doubles: only tiles on and above the diagonal are formed, three by each of twelve warps.
+constexpr int kIterateThreads = 384;
+template <int TS, typename Put>
+__device__ __forceinline__ void symmetric_product(const double* x, const double* y, double* out, Put put) {
+  using S = Side<TS>;
+  constexpr int LD = S::LD, C = (S::tiles + 11) / 12;
+  const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5) * C;
+  if (first < S::tiles) {
+    double acc[C][2] = {};
+    int ti[C], tj[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) S::tile((first + c) / S::slots, (first + c) % S::slots, ti[c], tj[c]);
+    const double *a = x + (lane & 3) * LD + (lane >> 2), *b = y + (lane & 3) * LD + (lane >> 2);
 #pragma unroll 4
-    for (int k = 0; k < N; ++k) {
-      double a[TS], b[TS];
+    for (int k = 0; k < S::N; k += 4)
 #pragma unroll
-      for (int i = 0; i < TS; ++i) {
-        a[i] = x[k * N + ti * TS + i];
-        b[i] = y[k * N + tj * TS + i];
+      for (int c = 0; c < C; ++c) mma_f64(acc[c], a[k * LD + ti[c] * 8], b[k * LD + tj[c] * 8]);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int row = ti[c] * 8 + (lane >> 2), col = tj[c] * 8 + (lane & 3) * 2;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const double v = put(acc[c][i], row, col + i);
+        out[row * LD + col + i] = v;
+        if (ti[c] != tj[c]) out[(col + i) * LD + row] = v;
       }
-#pragma unroll
-      for (int i = 0; i < TS; ++i)
-#pragma unroll
-        for (int j = 0; j < TS; ++j) acc[i][j] = fma(a[i], b[j], acc[i][j]);
     }
-#pragma unroll
-    for (int i = 0; i < TS; ++i)
-#pragma unroll
-      for (int j = 0; j < TS; ++j) {
-        out[(ti * TS + i) * N + tj * TS + j] = acc[i][j];
-        out[(tj * TS + j) * N + ti * TS + i] = acc[i][j];
-      }
   }
   __syncthreads();
 }
 template <int TS>
 __device__ __forceinline__ void iterate(const SmallTable& t, const Coefficients& co, const SmallEntry& e, int matrix, double* work) {
-  constexpr int N = 16 * TS, NN = N * N, T2 = TS * TS;
+  using S = Side<TS>;
+  constexpr int N = S::N, LD = S::LD, NN = N * LD, kOwn = S::part / kIterateThreads + (S::part % kIterateThreads != 0);
   const int tid = threadIdx.x, n = side_of(e);
-  double *A = work, *P = A + NN, *Q = P + NN, *S = Q + NN;
+  double *A = work, *Q = A + NN, *F = Q + NN, *P = F + NN;
   __shared__ double trace_sum;
   // the parts of A, in their order
-  const double* from = t.gram + e.gram + (size_t)matrix * e.chunks * (kTiles * T2);
-  for (int i = tid; i < kTiles * T2; i += 256) {
-    double s = 0.0;
-#pragma unroll 4
-    for (int c = 0; c < e.chunks; ++c) s += from[(size_t)c * (kTiles * T2) + i];
+  const double* from = t.gram + e.gram + (size_t)matrix * e.chunks * S::part;
+  double own[kOwn] = {};
+#pragma unroll 2
+  for (int c = 0; c < e.chunks; ++c)
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j)
+      if (tid + j * kIterateThreads < S::part) own[j] += from[(size_t)c * S::part + tid + j * kIterateThreads];
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) {
+    const int i = tid + j * kIterateThreads;
+    if (i >= S::part) break;
     int ti, tj;
-    tile_of(i / T2, ti, tj);
-    const int r = ti * TS + (i % T2) / TS, c = tj * TS + i % TS;
-    A[r * N + c] = s;
-    A[c * N + r] = s;
+    S::tile(i / 64 / S::slots, i / 64 % S::slots, ti, tj);
+    const int r = ti * 8 + i % 64 / 8, c = tj * 8 + i % 8;
+    A[r * LD + c] = own[j];
+    if (ti != tj) A[c * LD + r] = own[j];
   }
   __syncthreads();
   if (tid < 32) {
     double s = 0.0;
-    for (int i = tid; i < n; i += 32) s += A[i * N + i];
+    for (int i = tid; i < n; i += 32) s += A[i * LD + i];
     s = warp_sum(s);
     if (tid == 0) trace_sum = s;
   }
   __syncthreads();
   const double root = sqrt(trace_sum), inverse = 1.0 / (root > t.r.eps || root != root ? root : t.r.eps);
-  for (int i = tid; i < NN; i += 256) {
+  for (int i = tid; i < NN; i += kIterateThreads) {
     A[i] *= inverse * inverse;
-    Q[i] = i / N == i % N ? 1.0 : 0.0;
+    if (t.steps == 0) Q[i] = i / LD == i % LD ? 1.0 : 0.0;
   }
   __syncthreads();
+  const auto as_is = [](double v, int, int) { return v; };
   for (int step = 0; step < t.steps; ++step) {
-    const double* v = co.v + (t.coefficients > 1 ? 3 * step : 0);
-    symmetric_product<TS>(A, A, P);
-    for (int i = tid; i < NN; i += 256) P[i] = fma(v[2], P[i], fma(v[1], A[i], i / N == i % N ? v[0] : 0.0));
-    __syncthreads();
-    if (step == 0) {
-      for (int i = tid; i < NN; i += 256) Q[i] = P[i];
-      __syncthreads();
-    } else {
-      symmetric_product<TS>(Q, P, S);
+    const double *v = co.v + (t.coefficients > 1 ? 3 * step : 0), v0 = v[0], v1 = v[1], v2 = v[2];
+    double* p = step == 0 ? Q : P;
+    symmetric_product<TS>(A, A, p, [&](double s, int r, int c) { return fma(v2, s, fma(v1, A[r * LD + c], r == c ? v0 : 0.0)); });
+    if (step > 0) {
+      symmetric_product<TS>(Q, p, F, as_is);
       double* q = Q;
-      Q = S;
-      S = q;
+      Q = F;
+      F = q;
     }
     if (step + 1 == t.steps) break;
-    symmetric_product<TS>(A, P, S);
-    symmetric_product<TS>(S, P, A);
+    symmetric_product<TS>(A, p, F, as_is);
+    symmetric_product<TS>(F, p, A, as_is);
   }
   float* to = t.q + e.q + (size_t)matrix * (n * n);
-  for (int i = tid; i < n * n; i += 256) to[i] = (float)Q[i / n * N + i % n];
+  for (int i = tid; i < n * n; i += kIterateThreads) to[i] = (float)Q[i / n * LD + i % n];
   if (tid == 0) t.inverse[e.matrix + matrix] = inverse;
 }
-__global__ void __launch_bounds__(256) muon_iterate_kernel(const __grid_constant__ SmallTable t, const __grid_constant__ Coefficients co) {
-  extern __shared__ double work[];
+__global__ void __launch_bounds__(kIterateThreads) muon_iterate_kernel(const __grid_constant__ SmallTable t, const __grid_constant__ Coefficients co) {
+  extern __shared__ __align__(16) double work[];
   grid_dependency_wait();
   const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.matrix; })];
   const int matrix = (int)blockIdx.x - e.matrix, n = side_of(e);
@@ -273,16 +357,17 @@ __global__ void __launch_bounds__(256) muon_iterate_kernel(const __grid_constant
 }
 
 // X = Q u / |u| for a part of the longer side, and the update.
-template <typename P, typename G>
-__global__ void __launch_bounds__(256) muon_small_apply_kernel(const __grid_constant__ SmallTable t) {
-  extern __shared__ float low[];
-  constexpr int LD = kSub + 1;
-  float *q = low, *x = q + kSmall * kSmall, *o = x + kSmall * LD;   // [j][i], [j][k], [i][k]
-  grid_dependency_wait();
-  const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.first; })];
-  const int at0 = (int)blockIdx.x - e.first, matrix = at0 / e.chunks, chunk = at0 - matrix * e.chunks, n = side_of(e), len = max(e.rows, e.cols);
-  const int tid = threadIdx.x, ld = (n + 7) / 8 * 8;
-  const bool wide = e.rows <= e.cols;
+constexpr int small_apply_floats(int ts) {   // Q [j][i], X [j][k] and what becomes of it
+  const int N = 16 * ts;
+  return N * N + 2 * N * (2048 / N + 1);
+}
+template <typename P, typename G, int TS, int VEC>
+__device__ __forceinline__ void apply_part(const SmallTable& t, const SmallEntry& e, int matrix, int chunk, float* low) {
+  using S = Side<TS>;
+  constexpr int LD = S::sub + 1, N = S::N;
+  Values<TS, VEC> values(e);
+  const int n = values.n, len = max(e.rows, e.cols), tid = threadIdx.x;
+  float *q = low, *x = q + N * N, *o = x + N * LD;
   const size_t base = (size_t)matrix * e.rows * e.cols;
   const G* g = static_cast<const G*>(e.at.g) + base;
   const float* m = e.at.m ? e.at.m + base : nullptr;
@@ -291,53 +376,70 @@ __global__ void __launch_bounds__(256) muon_small_apply_kernel(const __grid_cons
   const float* from = t.q + e.q + (size_t)matrix * (n * n);
   const double inverse = t.inverse[e.matrix + matrix];
   const float lr = rate_of(t.r), rate = lr * e.scale, shrink = 1.f - lr * t.r.decay;
-  for (int i = tid; i < n * ld; i += 256) q[i] = i % ld < n ? from[i / ld * n + i % ld] : 0.f;
+#pragma unroll 4
+  for (int i = tid; i < N * N; i += 256) q[i] = i / N < n && i % N < n ? from[i / N * n + i % N] : 0.f;
   const int l0 = chunk * e.length, l1 = min(len, l0 + e.length);
-  for (int k0 = l0; k0 < l1; k0 += kSub) {
-    const int ks = min(kSub, l1 - k0);
-    __syncthreads();
-    for (int i = tid; i < n * kSub; i += 256) {
-      const int row = wide ? i / kSub : i % n, k = wide ? i % kSub : i / n;
-      float v = 0.f;
-      if (k < ks) {
-        const size_t at = wide ? (size_t)row * e.cols + k0 + k : (size_t)(k0 + k) * n + row;
-        v = to_float(g[at]);
-        if (m) v = direction_of(t.r, v, m[at]);
-        v = (float)((double)v * inverse);
-      }
-      x[row * LD + k] = v;
+  for (int k0 = l0; k0 < l1; k0 += S::sub) {
+    values.ks = min(S::sub, l1 - k0);
+    float v[8], b[8], old[8];
+    values.load(g, k0, v);
+    if (m) values.load(m, k0, b);
+    if (t.r.update) {
+      if (w) values.load(w, k0, old);
+      else values.load(p, k0, old);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)((double)(m ? direction_of(t.r, v[i], b[i]) : v[i]) * inverse);
     __syncthreads();
-    const int k = tid & (kSub - 1);
-    for (int i0 = tid / kSub * 8; i0 < n; i0 += 16) {
+    values.each_of(v, [&](int row, int k, float a) {
+      if (row < n) x[row * LD + k] = a;
+    });
+    __syncthreads();
+    // eight rows of a k per thread
+    const int k = tid % S::sub, i0 = tid / S::sub * 8;
+    if (i0 < n) {
       float acc[8] = {};
+#pragma unroll 4
       for (int j = 0; j < n; ++j) {
-        const float v = x[j * LD + k];
-        const float4 a = *reinterpret_cast<const float4*>(q + j * ld + i0), b = *reinterpret_cast<const float4*>(q + j * ld + i0 + 4);
-        acc[0] = fmaf(a.x, v, acc[0]); acc[1] = fmaf(a.y, v, acc[1]); acc[2] = fmaf(a.z, v, acc[2]); acc[3] = fmaf(a.w, v, acc[3]);
-        acc[4] = fmaf(b.x, v, acc[4]); acc[5] = fmaf(b.y, v, acc[5]); acc[6] = fmaf(b.z, v, acc[6]); acc[7] = fmaf(b.w, v, acc[7]);
+        const float a = x[j * LD + k];
+        const float4 c = *reinterpret_cast<const float4*>(q + j * N + i0), d = *reinterpret_cast<const float4*>(q + j * N + i0 + 4);
+        acc[0] = fmaf(c.x, a, acc[0]); acc[1] = fmaf(c.y, a, acc[1]); acc[2] = fmaf(c.z, a, acc[2]); acc[3] = fmaf(c.w, a, acc[3]);
+        acc[4] = fmaf(d.x, a, acc[4]); acc[5] = fmaf(d.y, a, acc[5]); acc[6] = fmaf(d.z, a, acc[6]); acc[7] = fmaf(d.w, a, acc[7]);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i0 + i < n) o[(i0 + i) * LD + k] = acc[i];
+      for (int i = 0; i < 8; ++i) o[(i0 + i) * LD + k] = acc[i];
     }
     __syncthreads();
-    for (int i = tid; i < n * kSub; i += 256) {
-      const int row = wide ? i / kSub : i % n, c = wide ? i % kSub : i / n;
-      if (c >= ks) continue;
-      const size_t at = wide ? (size_t)row * e.cols + k0 + c : (size_t)(k0 + c) * n + row;
-      float v = o[row * LD + c];
-      if (t.r.update) {
-        v = updated(w ? w[at] : to_float(p[at]), v, shrink, rate);
-        if (w) w[at] = v;
+#pragma unroll
+    for (int j = 0; j < 8 / VEC; ++j) {
+      int row, c;
+      if (!values.place(j, row, c)) continue;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float a = o[(values.wide ? row : row + i) * LD + (values.wide ? c + i : c)];
+        v[j * VEC + i] = t.r.update ? updated(old[j * VEC + i], a, shrink, rate) : a;
       }
-      p[at] = from_float<P>(v);
     }
+    if (w && t.r.update) values.store(w, k0, v);
+    values.store(p, k0, v);
   }
+}
+template <typename P, typename G>
+__global__ void __launch_bounds__(256, 3) muon_small_apply_kernel(const __grid_constant__ SmallTable t) {
+  extern __shared__ __align__(16) float low[];
+  grid_dependency_wait();
+  const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.first; })];
+  const int at = (int)blockIdx.x - e.first, matrix = at / e.chunks, chunk = at - matrix * e.chunks, n = side_of(e);
+#define B200CP_APPLY(TS) (e.vec ? apply_part<P, G, TS, 4>(t, e, matrix, chunk, low) : apply_part<P, G, TS, 1>(t, e, matrix, chunk, low))
+  if (n <= 16) B200CP_APPLY(1);
+  else if (n <= 32) B200CP_APPLY(2);
+  else B200CP_APPLY(4);
+#undef B200CP_APPLY
 }
 
 // ======== larger matrices ===========================================================================================================
-constexpr int kBatch = 96, kNormParts = 128;   // matrices of one shape that share launches; parts of a norm
+constexpr int kFlight = 8;                      // loads of a thread that are on their way together
+constexpr int kBatch = 96, kNormParts = 1024;   // matrices of one shape that share launches; parts of a norm
 struct Batch {
   Rates r;
   int count, rows, cols, ld;      // ld: of the planes, a multiple of eight
@@ -383,15 +485,26 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constan
       for (int k = 0; k < 8; ++k) s = fma((double)x[k], (double)x[k], s);
     }
   } else {
-#pragma unroll 4
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)b.parts * 256) {
-      float x = to_float(g[i]);
-      if (at.m) {
-        const float m = momentum_of<G>(b.r, x, at.m[i]);
-        at.m[i] = m;
-        x = direction_of(b.r, x, m);
+    const long long step = (long long)b.parts * 256;
+    for (long long i0 = (long long)blockIdx.x * 256 + threadIdx.x; i0 < n; i0 += step * kFlight) {
+      float x[kFlight], m[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const long long i = i0 + j * step;
+        x[j] = i < n ? to_float(g[i]) : 0.f;
+        m[j] = at.m && i < n ? at.m[i] : 0.f;
       }
-      s = fma((double)x, (double)x, s);
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const long long i = i0 + j * step;
+        if (i >= n) break;
+        if (at.m) {
+          m[j] = momentum_of<G>(b.r, x[j], m[j]);
+          at.m[i] = m[j];
+          x[j] = direction_of(b.r, x[j], m[j]);
+        }
+        s = fma((double)x[j], (double)x[j], s);
+      }
     }
   }
   __shared__ double red[8];
@@ -415,16 +528,18 @@ __device__ __forceinline__ void split8(const float (&v)[8], Group<__half, 8>& hi
 // The planes of X.  Eight columns per thread and turn.
 template <typename G>
 __global__ void __launch_bounds__(256) muon_planes_kernel(const __grid_constant__ Batch b) {
-  __shared__ double inverse;
+  __shared__ double red[8];
   grid_dependency_wait();
-  if (threadIdx.x < 32) {
-    double s = 0.0;
-    for (int i = threadIdx.x; i < b.parts; i += 32) s += b.norms[blockIdx.y * kNormParts + i];
-    s = sqrt(warp_sum(s));
-    if (threadIdx.x == 0) inverse = (double)b.scale / (s > b.r.eps || s != s ? s : b.r.eps);
-  }
+  double s = 0.0;
+  for (int i = threadIdx.x; i < b.parts; i += 256) s += b.norms[blockIdx.y * kNormParts + i];
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
-  const double inv = inverse;
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += red[i];
+  s = sqrt(s);
+  const double inv = (double)b.scale / (s > b.r.eps || s != s ? s : b.r.eps);
   const Pointers& at = b.at[blockIdx.y];
   const G* g = static_cast<const G*>(at.g);
   __half* to = b.x + blockIdx.y * b.matrix;
@@ -887,7 +1002,7 @@ void cut_small(const b200cp_muon_matrix& a, long long all, int sm_count, SmallEn
   e->q = s->floats;
   s->ctas += e->chunks * a.stack;
   s->matrices += a.stack;
-  s->doubles += (size_t)a.stack * e->chunks * (kTiles * ts * ts);
+  s->doubles += (size_t)a.stack * e->chunks * kPart[ts];
   s->floats += (size_t)a.stack * n * n;
 }
 size_t small_bytes(const SmallSizes& s) {
@@ -901,6 +1016,8 @@ int next_small(const std::vector<b200cp_muon_matrix>& ms, size_t at, long long a
     cut_small(ms[at + count], all, sm_count, &e, s);
     const b200cp_muon_matrix& a = ms[at + count];
     e.at = Pointers{a.param, a.grad, a.momentum, a.master};
+    const auto off = [](const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; };
+    e.vec = a.cols % 4 == 0 && !(off(a.param) | off(a.grad) | off(a.momentum) | off(a.master));
     if (t) t->e[count] = e;
     ++count;
   }
@@ -972,6 +1089,12 @@ float factor_of(int adjust, int rows, int cols) {
   return 1.f;
 }
 
+// (A slot per kernel, not per caller: callers of several types share some, and each would set its own, smaller size.)
+template <auto KERNEL>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<int> set[64];
+  return ensure_dynamic_smem(reinterpret_cast<const void*>(KERNEL), set, bytes);
+}
 template <typename P, typename G>
 int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char* ws, const DeviceInfo& di, cudaStream_t st) {
   Coefficients co{};
@@ -987,20 +1110,21 @@ int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char*
     t.gram = reinterpret_cast<double*>(ws);
     t.inverse = reinterpret_cast<double*>(ws + align_up(s.doubles * 8, 256));
     t.q = reinterpret_cast<float*>(ws + align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256));
-    int widest = 1;
+    int ts = 1;
     for (int i = 0; i < t.count; ++i) {
       t.e[i].scale = factor_of(adjust, t.e[i].rows, t.e[i].cols);
-      widest = std::max(widest, tile_side(std::min(t.e[i].rows, t.e[i].cols)));
+      ts = std::max(ts, tile_side(std::min(t.e[i].rows, t.e[i].cols)));
     }
-    const int N = 16 * widest, gram = kSub * (N + 2) * 8, four = 4 * N * N * 8, low = (kSmall * kSmall + 2 * kSmall * (kSub + 1)) * 4;
-    static std::atomic<int> set1[64], set2[64], set3[64];
-    B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(muon_gram_kernel<G>), set1, gram));
-    B200CP_CUDA_OK(launch_kernel(muon_gram_kernel<G>, dim3(s.ctas), dim3(kGramThreads), gram, st, true, t));
+    // (each as much as the widest matrix of the launch needs; the others need less)
+    const int gram = std::max({gram_doubles(1), ts > 1 ? gram_doubles(2) : 0, ts > 2 ? gram_doubles(4) : 0}) * 8, four = 4 * 16 * ts * (16 * ts + 4) * 8,
+              low = std::max({small_apply_floats(1), ts > 1 ? small_apply_floats(2) : 0, ts > 2 ? small_apply_floats(4) : 0}) * 4;
+    B200CP_CUDA_OK(allow_smem<muon_gram_kernel<G>>(gram));
+    B200CP_CUDA_OK(launch_kernel(muon_gram_kernel<G>, dim3(s.ctas), dim3(256), gram, st, true, t));
     B200CP_LAUNCH_OK("muon_gram_kernel");
-    B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(muon_iterate_kernel), set2, four));
-    B200CP_CUDA_OK(launch_kernel(muon_iterate_kernel, dim3(s.matrices), dim3(256), four, st, true, t, co));
+    B200CP_CUDA_OK(allow_smem<muon_iterate_kernel>(four));
+    B200CP_CUDA_OK(launch_kernel(muon_iterate_kernel, dim3(s.matrices), dim3(kIterateThreads), four, st, true, t, co));
     B200CP_LAUNCH_OK("muon_iterate_kernel");
-    B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(muon_small_apply_kernel<P, G>), set3, low));
+    B200CP_CUDA_OK((allow_smem<muon_small_apply_kernel<P, G>>(low)));
     B200CP_CUDA_OK(launch_kernel(muon_small_apply_kernel<P, G>, dim3(s.ctas), dim3(256), low, st, true, t));
     B200CP_LAUNCH_OK("muon_small_apply_kernel");
   }
@@ -1032,7 +1156,7 @@ int run_large(const Shape& s, int first, int count, const Rates& r, const Plan& 
   }
   b.vec = off == 0;
   const long long values = (long long)s.rows * s.cols;
-  b.parts = (int)std::min<long long>(kNormParts, std::max<long long>(1, values / 4096));
+  b.parts = (int)std::min<long long>(kNormParts, (values + 2047) / 2048);
   B200CP_CUDA_OK(launch_kernel(muon_momentum_kernel<G>, dim3(b.parts, count), dim3(256), 0, st, true, b));
   B200CP_LAUNCH_OK("muon_momentum_kernel");
   const int rows8 = (int)std::min<long long>(16LL * di.sm_count, ((long long)s.rows * (X.ld / 8) + 255) / 256);

@@ -42,10 +42,20 @@ __device__ __forceinline__ Group<T, N> pack(const float (&x)[N]) {
   }
   return g;
 }
+// (bfloat16 by words: one operation a value, where a value by itself takes two)
 template <typename T, int N>
 __device__ __forceinline__ void unpack(const Group<T, N>& g, float (&x)[N]) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value && N % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(g.v);
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = to_float(g.v[i]);
+    for (int i = 0; i < N / 2; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_float(g.v[i]);
+  }
 }
 template <typename T, int N>
 __device__ __forceinline__ Group<T, N> load_group(const T* p) { return *reinterpret_cast<const Group<T, N>*>(p); }

@@ -175,6 +175,18 @@ def test_views_lists_and_rates_on_the_device():
     assert P.orthogonalise(torch.zeros(3, 0, 4, device="cuda")).shape == (3, 0, 4)
 
 
+def test_types_and_sizes_in_turn():
+    """What a kernel is allowed for the largest matrix stays allowed when other types come with smaller ones."""
+    import paralleltnnlayers_b200 as P
+    for side in (60, 10, 60, 30, 60):
+        for dtype, gtype in ((torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.bfloat16, torch.float32)):
+            for n in (side, 7):
+                g = matrices(n, 80, seed=n).to(gtype)
+                p, m = torch.zeros(n, 80, device="cuda", dtype=dtype), torch.zeros(n, 80, device="cuda")
+                P.muon_step([p], [g], [m], 1.0, momentum=0.0, weight_decay=0.0, adjust=None)
+                check(-p, *defined(g))
+
+
 def test_many_matrices():
     """More tensors than a launch's table has, and more matrices of a shape than share launches."""
     import paralleltnnlayers_b200 as P
