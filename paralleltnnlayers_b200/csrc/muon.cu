@@ -13,9 +13,10 @@
 //
 // n > 64: X, A and B = b A + c A^2 are products on the tcgen05 tensor cores.  What is rounded: a value is held as two fp16 numbers (hi + rest, 22 bits)
 // times a power of two that the bound on the singular values gives, so that none overflows and the sums of a product are of hi hi + hi lo + lo hi; its
-// sums are fp32, at most 64 terms in an accumulator (the tensor core cuts sums off: over 4096 terms it loses 3e-5, where fp32 rounding loses 3e-7) and the
-// rest in registers.  One fp16 number would be three times as fast, but directions with small singular values are raised by 3.4445 a step: its 2^-12 comes
-// out as 7 % of a gradient of rank one.  a X is added in fp32.
+// sums are fp32, at most 128 terms in an accumulator (the tensor core cuts sums off: over 4096 terms it loses 3e-5, where fp32 rounding loses 3e-7) and the
+// rest in registers (4096 x 4096 against 64 bits: 5.5e-7 with 64 terms, 6.1e-7 with 128, 1.0e-6 with 256; 4.20, 4.14 and 3.99 ms).  One fp16 number would be three times as fast, but directions with small singular values are raised by 3.4445 a step: its 2^-12 comes
+// out as 7 % of a gradient of rank one.  a X is added in fp32 (as part of
+// the product, with a I in B, 4 % faster and two to three times as far off).
 // A and B are symmetric: blocks below the diagonal are not computed, the others stored twice.  Either operand is taken in either order, so nothing is
 // transposed; where the rows are the longer side A = X^T X and X <- a X + X B.  Matrices of one shape share their launches.
 // Every wait is bounded: one that runs out sets a status word and the CTA leaves through its normal exit.
@@ -62,7 +63,9 @@ __device__ __forceinline__ double warp_sum(double x) {
 }
 
 // ======== matrices with a side of at most 64 =====================================================================================
-constexpr int kSmall = 64, kTableSmall = 224, kSub = 128;
+constexpr int kSmall = 64, kSub = 128;
+// Tensors of a launch: a table's bytes are written for each launch, so there are two sizes of it.
+constexpr int kFewSmall = 24, kTableSmall = 224;
 struct SmallEntry {
   Pointers at;
   int rows, cols;
@@ -74,19 +77,22 @@ struct SmallEntry {
   float scale;               // of the rate
   size_t gram, q;            // in doubles, in floats: of its first matrix
 };
-struct SmallTable {
+struct SmallHead {
   Rates r;
   int count, steps, coefficients;
   double *gram, *inverse;
   float* q;
-  SmallEntry e[kTableSmall];
+};
+template <int CAP>
+struct SmallTable : SmallHead {
+  SmallEntry e[CAP];
 };
 struct Coefficients {
   double v[3 * 100];
 };
 __device__ __forceinline__ int side_of(const SmallEntry& e) { return min(e.rows, e.cols); }
-template <typename F>
-__device__ __forceinline__ int entry_of(const SmallTable& t, int block, F first) {
+template <int CAP, typename F>
+__device__ __forceinline__ int entry_of(const SmallTable<CAP>& t, int block, F first) {
   int a = 0, b = t.count;
   while (b - a > 1) {
     const int c = (a + b) / 2;
@@ -119,13 +125,13 @@ __device__ __forceinline__ void mma_f64(double (&c)[2], double a, double b) {
 template <int TS, int VEC>
 struct Values {
   static constexpr int each = 8 / VEC, SUB = Side<TS>::sub;
-  int n, ks;                 // sizes of what is there: of the smaller side, of the longer one
+  int n, len;                // sizes of the smaller side and of the longer one
   bool wide;
   unsigned inverse;          // 2^32 / (n / VEC), rounded up: exact quotients for numbers below 2^16
   size_t pitch;
-  __device__ Values(const SmallEntry& e) : n(side_of(e)), ks(0), wide(e.rows <= e.cols), inverse(0xffffffffu / (unsigned)max(1, n / VEC) + 1), pitch(e.cols) {}
-  // group j of this thread: its place, and whether it is there
-  __device__ __forceinline__ bool place(int j, int& row, int& k) const {
+  __device__ Values(const SmallEntry& e) : n(side_of(e)), len(max(e.rows, e.cols)), wide(e.rows <= e.cols), inverse(0xffffffffu / (unsigned)max(1, n / VEC) + 1), pitch(e.cols) {}
+  // group j of this thread: its place, and whether it is among the first ks of the longer side
+  __device__ __forceinline__ bool place(int j, int ks, int& row, int& k) const {
     const int i = threadIdx.x + j * 256;
     if (wide) {
       row = i / (SUB / VEC);
@@ -140,11 +146,12 @@ struct Values {
   __device__ __forceinline__ size_t at(int row, int k) const { return wide ? (size_t)row * pitch + k : (size_t)k * n + row; }
   template <typename T>
   __device__ __forceinline__ void load(const T* from, int k0, float (&x)[8]) const {
+    const int ks = min(SUB, len - k0);
     Group<T, VEC> v[each];
 #pragma unroll
     for (int j = 0; j < each; ++j) {
       int row, k;
-      if (place(j, row, k)) v[j] = load_group<T, VEC>(from + at(row, k0 + k));
+      if (place(j, ks, row, k)) v[j] = load_group<T, VEC>(from + at(row, k0 + k));
       else
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[j].v[i] = from_float<T>(0.f);
@@ -156,10 +163,11 @@ struct Values {
   }
   template <typename T>
   __device__ __forceinline__ void store(T* to, int k0, const float (&x)[8]) const {
+    const int ks = min(SUB, len - k0);
 #pragma unroll
     for (int j = 0; j < each; ++j) {
       int row, k;
-      if (!place(j, row, k)) continue;
+      if (!place(j, ks, row, k)) continue;
       float v[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[i] = x[j * VEC + i];
@@ -168,11 +176,12 @@ struct Values {
   }
   // f(row, k, value) of what has a place in N x SUB (zeros where nothing is)
   template <typename F>
-  __device__ __forceinline__ void each_of(float (&x)[8], F f) const {
+  __device__ __forceinline__ void each_of(int k0, float (&x)[8], F f) const {
+    const int ks = min(SUB, len - k0);
 #pragma unroll
     for (int j = 0; j < each; ++j) {
       int row, k;
-      const bool in = place(j, row, k);
+      const bool in = place(j, ks, row, k);
       if (!in && (wide ? row >= Side<TS>::N : k >= SUB)) continue;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) f(wide ? row : row + i, wide ? k + i : k, x[j * VEC + i]);
@@ -182,25 +191,24 @@ struct Values {
 
 // A part of A, in 64 bits, from a part of the longer side; the momentum is brought up to date on the way.
 template <typename G, int TS, int VEC>
-__device__ __forceinline__ void gram_part(const SmallTable& t, const SmallEntry& e, int matrix, int chunk, double* u) {
+__device__ __forceinline__ void gram_part(const SmallHead& t, const SmallEntry& e, int matrix, int chunk, double* u) {
   using S = Side<TS>;
   constexpr int LD = S::LD;
   Values<TS, VEC> values(e);
-  const int n = values.n, len = max(e.rows, e.cols), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = values.n, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t base = (size_t)matrix * e.rows * e.cols;
   const G* g = static_cast<const G*>(e.at.g) + base;
   float* m = e.at.m ? e.at.m + base : nullptr;
   const int group = warp % TS, slice = warp / TS;
   double acc[S::slots][2] = {};
-  const int l0 = chunk * e.length, l1 = min(len, l0 + e.length);
+  const int l0 = chunk * e.length, l1 = min(values.len, l0 + e.length);
   if (n < S::N)
     for (int i = tid; i < S::sub * LD; i += 256) u[i] = 0.0;   // (rows past n stay zero)
+  float x[8], b[8];   // (the next values are on their way while these are multiplied)
+  values.load(g, l0, x);
+  if (m) values.load(m, l0, b);
   for (int k0 = l0; k0 < l1; k0 += S::sub) {
-    values.ks = min(S::sub, l1 - k0);
-    float x[8], b[8];
-    values.load(g, k0, x);
     if (m) {
-      values.load(m, k0, b);
 #pragma unroll
       for (int i = 0; i < 8; ++i) b[i] = momentum_of<G>(t.r, x[i], b[i]);
       values.store(m, k0, b);
@@ -208,10 +216,14 @@ __device__ __forceinline__ void gram_part(const SmallTable& t, const SmallEntry&
       for (int i = 0; i < 8; ++i) x[i] = direction_of(t.r, x[i], b[i]);
     }
     __syncthreads();
-    values.each_of(x, [&](int row, int k, float v) {
+    values.each_of(k0, x, [&](int row, int k, float v) {
       if (row < n) u[k * LD + row] = (double)v;
     });
     __syncthreads();
+    if (k0 + S::sub < l1) {
+      values.load(g, k0 + S::sub, x);
+      if (m) values.load(m, k0 + S::sub, b);
+    }
     const double* from = u + (slice * 16 + (lane & 3)) * LD + (lane >> 2);
 #pragma unroll
     for (int k = 0; k < 16; k += 4) {
@@ -245,8 +257,8 @@ constexpr int gram_doubles(int ts) {   // of shared memory: the values, or the s
   return ts == 1 ? std::max(Side<1>::sub * Side<1>::LD, 8 * Side<1>::part) : ts == 2 ? std::max(Side<2>::sub * Side<2>::LD, 4 * Side<2>::part)
                                                                                : std::max(Side<4>::sub * Side<4>::LD, 2 * Side<4>::part);
 }
-template <typename G>
-__global__ void __launch_bounds__(256, 3) muon_gram_kernel(const __grid_constant__ SmallTable t) {
+template <typename G, int CAP>
+__global__ void __launch_bounds__(256, 3) muon_gram_kernel(const __grid_constant__ SmallTable<CAP> t) {
   extern __shared__ __align__(16) double work[];
   grid_dependency_wait();
   const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.first; })];
@@ -289,7 +301,7 @@ __device__ __forceinline__ void symmetric_product(const double* x, const double*
   __syncthreads();
 }
 template <int TS>
-__device__ __forceinline__ void iterate(const SmallTable& t, const Coefficients& co, const SmallEntry& e, int matrix, double* work) {
+__device__ __forceinline__ void iterate(const SmallHead& t, const Coefficients& co, const SmallEntry& e, int matrix, double* work) {
   using S = Side<TS>;
   constexpr int N = S::N, LD = S::LD, NN = N * LD, kOwn = S::part / kIterateThreads + (S::part % kIterateThreads != 0);
   const int tid = threadIdx.x, n = side_of(e);
@@ -346,7 +358,8 @@ __device__ __forceinline__ void iterate(const SmallTable& t, const Coefficients&
   for (int i = tid; i < n * n; i += kIterateThreads) to[i] = (float)Q[i / n * LD + i % n];
   if (tid == 0) t.inverse[e.matrix + matrix] = inverse;
 }
-__global__ void __launch_bounds__(kIterateThreads) muon_iterate_kernel(const __grid_constant__ SmallTable t, const __grid_constant__ Coefficients co) {
+template <int CAP>
+__global__ void __launch_bounds__(kIterateThreads) muon_iterate_kernel(const __grid_constant__ SmallTable<CAP> t, const __grid_constant__ Coefficients co) {
   extern __shared__ __align__(16) double work[];
   grid_dependency_wait();
   const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.matrix; })];
@@ -362,11 +375,11 @@ constexpr int small_apply_floats(int ts) {   // Q [j][i], X [j][k] and what beco
   return N * N + 2 * N * (2048 / N + 1);
 }
 template <typename P, typename G, int TS, int VEC>
-__device__ __forceinline__ void apply_part(const SmallTable& t, const SmallEntry& e, int matrix, int chunk, float* low) {
+__device__ __forceinline__ void apply_part(const SmallHead& t, const SmallEntry& e, int matrix, int chunk, float* low) {
   using S = Side<TS>;
   constexpr int LD = S::sub + 1, N = S::N;
   Values<TS, VEC> values(e);
-  const int n = values.n, len = max(e.rows, e.cols), tid = threadIdx.x;
+  const int n = values.n, tid = threadIdx.x;
   float *q = low, *x = q + N * N, *o = x + N * LD;
   const size_t base = (size_t)matrix * e.rows * e.cols;
   const G* g = static_cast<const G*>(e.at.g) + base;
@@ -378,23 +391,31 @@ __device__ __forceinline__ void apply_part(const SmallTable& t, const SmallEntry
   const float lr = rate_of(t.r), rate = lr * e.scale, shrink = 1.f - lr * t.r.decay;
 #pragma unroll 4
   for (int i = tid; i < N * N; i += 256) q[i] = i / N < n && i % N < n ? from[i / N * n + i % N] : 0.f;
-  const int l0 = chunk * e.length, l1 = min(len, l0 + e.length);
-  for (int k0 = l0; k0 < l1; k0 += S::sub) {
-    values.ks = min(S::sub, l1 - k0);
-    float v[8], b[8], old[8];
+  const int l0 = chunk * e.length, l1 = min(values.len, l0 + e.length);
+  float v[8], b[8], next[8];   // (the next values are on their way while these are multiplied)
+  const auto fetch = [&](int k0) {
     values.load(g, k0, v);
     if (m) values.load(m, k0, b);
     if (t.r.update) {
-      if (w) values.load(w, k0, old);
-      else values.load(p, k0, old);
+      if (w) values.load(w, k0, next);
+      else values.load(p, k0, next);
     }
+  };
+  fetch(l0);
+  for (int k0 = l0; k0 < l1; k0 += S::sub) {
+    const int ks = min(S::sub, values.len - k0);
+    float old[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)((double)(m ? direction_of(t.r, v[i], b[i]) : v[i]) * inverse);
+    for (int i = 0; i < 8; ++i) {
+      old[i] = next[i];
+      v[i] = (float)((double)(m ? direction_of(t.r, v[i], b[i]) : v[i]) * inverse);
+    }
     __syncthreads();
-    values.each_of(v, [&](int row, int k, float a) {
+    values.each_of(k0, v, [&](int row, int k, float a) {
       if (row < n) x[row * LD + k] = a;
     });
     __syncthreads();
+    if (k0 + S::sub < l1) fetch(k0 + S::sub);
     // eight rows of a k per thread
     const int k = tid % S::sub, i0 = tid / S::sub * 8;
     if (i0 < n) {
@@ -413,19 +434,19 @@ __device__ __forceinline__ void apply_part(const SmallTable& t, const SmallEntry
 #pragma unroll
     for (int j = 0; j < 8 / VEC; ++j) {
       int row, c;
-      if (!values.place(j, row, c)) continue;
+      if (!values.place(j, ks, row, c)) continue;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float a = o[(values.wide ? row : row + i) * LD + (values.wide ? c + i : c)];
-        v[j * VEC + i] = t.r.update ? updated(old[j * VEC + i], a, shrink, rate) : a;
+        old[j * VEC + i] = t.r.update ? updated(old[j * VEC + i], a, shrink, rate) : a;
       }
     }
-    if (w && t.r.update) values.store(w, k0, v);
-    values.store(p, k0, v);
+    if (w && t.r.update) values.store(w, k0, old);
+    values.store(p, k0, old);
   }
 }
-template <typename P, typename G>
-__global__ void __launch_bounds__(256, 3) muon_small_apply_kernel(const __grid_constant__ SmallTable t) {
+template <typename P, typename G, int CAP>
+__global__ void __launch_bounds__(256, 3) muon_small_apply_kernel(const __grid_constant__ SmallTable<CAP> t) {
   extern __shared__ __align__(16) float low[];
   grid_dependency_wait();
   const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.first; })];
@@ -438,70 +459,104 @@ __global__ void __launch_bounds__(256, 3) muon_small_apply_kernel(const __grid_c
 }
 
 // ======== larger matrices ===========================================================================================================
-constexpr int kFlight = 8;                      // loads of a thread that are on their way together
-constexpr int kBatch = 96, kNormParts = 1024;   // matrices of one shape that share launches; parts of a norm
-struct Batch {
-  Rates r;
-  int count, rows, cols, ld;      // ld: of the planes, a multiple of eight
-  size_t plane, matrix;           // halves from one plane, one matrix to the next
-  float scale, rate;              // planes hold scale X; of the rate
+// All of them go together, up to kItems matrices of kProblems shapes and a gigabyte or two of planes: a launch takes all their tiles.
+constexpr int kFlight = 8;                                     // loads of a thread that are on their way together
+constexpr int kFewItems = 16, kItems = 256, kFewProblems = 4, kProblems = 48, kNormParts = 1024;   // (tables of two sizes, as above; kNormParts: parts of a norm)
+constexpr int kTurn = 256 * 8 * 4;                             // values of a CTA
+struct Item {
+  Pointers at;
+  int rows, cols, ld;             // ld: of the planes
+  int vec;                        // eight values of every array lie on its boundary, and rows are multiples of eight
+  size_t plane;                   // halves from one plane to the next
   __half* x;
-  double* norms;                  // [matrix][part]
-  int parts, vec;                 // vec: eight values of every array lie on its boundary, and rows are multiples of eight
-  Pointers at[kBatch];
+  int first, chunk, parts, norm;  // of the launch over the values: its first CTA, values of a CTA, CTAs; its first part of a norm
+  int first8;                     // of the launches over the planes
+  float rate;                     // factor of the rate
 };
+struct ItemsHead {
+  Rates r;
+  int count;
+  float scale;                    // planes hold scale X
+  double* norms;
+};
+template <int CAP>
+struct Items : ItemsHead {
+  Item e[CAP];
+};
+template <int CAP, typename F>
+__device__ __forceinline__ const Item& item_of(const Items<CAP>& t, int block, F first) {
+  int a = 0, b = t.count;
+  while (b - a > 1) {
+    const int c = (a + b) / 2;
+    if (first(t.e[c]) <= block) a = c; else b = c;
+  }
+  return t.e[a];
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* from, float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 8; h += kPerLoad<T>) {
+    float y[kPerLoad<T>];
+    unpack(load_group<T, kPerLoad<T>>(from + h), y);
+#pragma unroll
+    for (int k = 0; k < kPerLoad<T>; ++k) x[h + k] = y[k];
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 8; h += kPerLoad<T>) {
+    float y[kPerLoad<T>];
+#pragma unroll
+    for (int k = 0; k < kPerLoad<T>; ++k) y[k] = x[h + k];
+    store_group(to + h, pack<T>(y));
+  }
+}
 
-// Momentum, and a part of |u|^2 in 64 bits.  grid (parts, matrices)
-template <typename G>
-__global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constant__ Batch b) {
+// Momentum, and a part of |u|^2 in 64 bits.
+template <typename G, int CAP>
+__global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constant__ Items<CAP> t) {
   grid_dependency_wait();
-  const Pointers& at = b.at[blockIdx.y];
-  const G* g = static_cast<const G*>(at.g);
-  const long long n = (long long)b.rows * b.cols;
+  const Item& e = item_of(t, blockIdx.x, [](const Item& i) { return i.first; });
+  const int part = (int)blockIdx.x - e.first;
+  const G* g = static_cast<const G*>(e.at.g);
+  float* m = e.at.m;
+  const long long i0 = (long long)part * e.chunk, n = min((long long)e.rows * e.cols, i0 + e.chunk);
   double s = 0.0;
-  if (b.vec) {
+  if (e.vec) {
 #pragma unroll 2
-    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long long)b.parts * 256 * 8) {
-      float x[8], m[8];
-#pragma unroll
-      for (int h = 0; h < 8; h += kPerLoad<G>) {
-        float y[kPerLoad<G>];
-        unpack(load_group<G, kPerLoad<G>>(g + i + h), y);
-#pragma unroll
-        for (int k = 0; k < kPerLoad<G>; ++k) x[h + k] = y[k];
-      }
-      if (at.m) {
-#pragma unroll
-        for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(m + h) = *reinterpret_cast<const float4*>(at.m + i + h);
+    for (long long i = i0 + threadIdx.x * 8; i < n; i += 256 * 8) {
+      float x[8], b[8];
+      load8(g + i, x);
+      if (m) {
+        load8(m + i, b);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          m[k] = momentum_of<G>(b.r, x[k], m[k]);
-          x[k] = direction_of(b.r, x[k], m[k]);
+          b[k] = momentum_of<G>(t.r, x[k], b[k]);
+          x[k] = direction_of(t.r, x[k], b[k]);
         }
-#pragma unroll
-        for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(at.m + i + h) = *reinterpret_cast<const float4*>(m + h);
+        store8(m + i, b);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) s = fma((double)x[k], (double)x[k], s);
     }
   } else {
-    const long long step = (long long)b.parts * 256;
-    for (long long i0 = (long long)blockIdx.x * 256 + threadIdx.x; i0 < n; i0 += step * kFlight) {
-      float x[kFlight], m[kFlight];
+    for (long long i = i0 + threadIdx.x; i < n; i += 256 * kFlight) {
+      float x[kFlight], b[kFlight];
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        const long long i = i0 + j * step;
-        x[j] = i < n ? to_float(g[i]) : 0.f;
-        m[j] = at.m && i < n ? at.m[i] : 0.f;
+        const long long at = i + j * 256;
+        x[j] = at < n ? to_float(g[at]) : 0.f;
+        b[j] = m && at < n ? m[at] : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        const long long i = i0 + j * step;
-        if (i >= n) break;
-        if (at.m) {
-          m[j] = momentum_of<G>(b.r, x[j], m[j]);
-          at.m[i] = m[j];
-          x[j] = direction_of(b.r, x[j], m[j]);
+        const long long at = i + j * 256;
+        if (at >= n) break;
+        if (m) {
+          b[j] = momentum_of<G>(t.r, x[j], b[j]);
+          m[at] = b[j];
+          x[j] = direction_of(t.r, x[j], b[j]);
         }
         s = fma((double)x[j], (double)x[j], s);
       }
@@ -514,7 +569,7 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constan
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) s += red[i];
-    b.norms[blockIdx.y * kNormParts + blockIdx.x] = s;
+    t.norms[e.norm + part] = s;
   }
 }
 __device__ __forceinline__ void split8(const float (&v)[8], Group<__half, 8>& hi, Group<__half, 8>& lo) {
@@ -525,13 +580,14 @@ __device__ __forceinline__ void split8(const float (&v)[8], Group<__half, 8>& hi
   for (int i = 0; i < 8; ++i) r[i] = v[i] - r[i];
   lo = pack<__half>(r);
 }
-// The planes of X.  Eight columns per thread and turn.
-template <typename G>
-__global__ void __launch_bounds__(256) muon_planes_kernel(const __grid_constant__ Batch b) {
+// The planes of X.  Eight columns per thread and turn, four turns.
+template <typename G, int CAP>
+__global__ void __launch_bounds__(256) muon_planes_kernel(const __grid_constant__ Items<CAP> t) {
   __shared__ double red[8];
   grid_dependency_wait();
+  const Item& e = item_of(t, blockIdx.x, [](const Item& i) { return i.first8; });
   double s = 0.0;
-  for (int i = threadIdx.x; i < b.parts; i += 256) s += b.norms[blockIdx.y * kNormParts + i];
+  for (int i = threadIdx.x; i < e.parts; i += 256) s += t.norms[e.norm + i];
   s = warp_sum(s);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
@@ -539,103 +595,82 @@ __global__ void __launch_bounds__(256) muon_planes_kernel(const __grid_constant_
 #pragma unroll
   for (int i = 0; i < 8; ++i) s += red[i];
   s = sqrt(s);
-  const double inv = (double)b.scale / (s > b.r.eps || s != s ? s : b.r.eps);
-  const Pointers& at = b.at[blockIdx.y];
-  const G* g = static_cast<const G*>(at.g);
-  __half* to = b.x + blockIdx.y * b.matrix;
-  const int per = b.ld / 8;
-  const long long n = (long long)b.rows * per;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const long long row = i / per;
+  const double inv = (double)t.scale / (s > t.r.eps || s != s ? s : t.r.eps);
+  const G* g = static_cast<const G*>(e.at.g);
+  const float* m = e.at.m;
+  const unsigned per = (unsigned)(e.cols + 7) / 8;
+  const unsigned long long n = (unsigned long long)e.rows * per, first = (unsigned long long)((int)blockIdx.x - e.first8) * 1024 + threadIdx.x;
+#pragma unroll 2
+  for (int j = 0; j < 4; ++j) {
+    const unsigned long long i = first + j * 256;
+    if (i >= n) break;
+    const size_t row = n <= 0xffffffffu ? (size_t)((unsigned)i / per) : (size_t)(i / per);
     const int c = (int)(i - row * per) * 8;
-    const size_t src = (size_t)row * b.cols + c;
-    float x[8], m[8];
-    if (b.vec) {
-#pragma unroll
-      for (int h = 0; h < 8; h += kPerLoad<G>) {
-        float y[kPerLoad<G>];
-        unpack(load_group<G, kPerLoad<G>>(g + src + h), y);
-#pragma unroll
-        for (int k = 0; k < kPerLoad<G>; ++k) x[h + k] = y[k];
-      }
-      if (at.m)
-#pragma unroll
-        for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(m + h) = *reinterpret_cast<const float4*>(at.m + src + h);
+    const size_t src = row * e.cols + c;
+    float x[8], b[8];
+    if (e.vec) {
+      load8(g + src, x);
+      if (m) load8(m + src, b);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        x[k] = c + k < b.cols ? to_float(g[src + k]) : 0.f;
-        m[k] = at.m && c + k < b.cols ? at.m[src + k] : 0.f;
+        x[k] = c + k < e.cols ? to_float(g[src + k]) : 0.f;
+        b[k] = m && c + k < e.cols ? m[src + k] : 0.f;
       }
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (at.m) x[k] = direction_of(b.r, x[k], m[k]);
+      if (m) x[k] = direction_of(t.r, x[k], b[k]);
       x[k] = (float)((double)x[k] * inv);
     }
     Group<__half, 8> hi, lo;
     split8(x, hi, lo);
-    store_group(to + row * b.ld + c, hi);
-    store_group(to + b.plane + row * b.ld + c, lo);
+    store_group(e.x + row * e.ld + c, hi);
+    store_group(e.x + e.plane + row * e.ld + c, lo);
   }
 }
 // The update from the planes of the last X.
-template <typename P>
-__global__ void __launch_bounds__(256) muon_apply_kernel(const __grid_constant__ Batch b) {
+template <typename P, int CAP>
+__global__ void __launch_bounds__(256) muon_apply_kernel(const __grid_constant__ Items<CAP> t) {
   grid_dependency_wait();
-  const Pointers& at = b.at[blockIdx.y];
-  P* p = static_cast<P*>(at.p);
-  const __half* from = b.x + blockIdx.y * b.matrix;
-  const float lr = rate_of(b.r), rate = lr * b.rate, shrink = 1.f - lr * b.r.decay, unit = 1.f / b.scale;
-  const int per = b.ld / 8;
-  const long long n = (long long)b.rows * per;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const long long row = i / per;
+  const Item& e = item_of(t, blockIdx.x, [](const Item& i) { return i.first8; });
+  P* p = static_cast<P*>(e.at.p);
+  float* master = e.at.w;
+  const float lr = rate_of(t.r), rate = lr * e.rate, shrink = 1.f - lr * t.r.decay, unit = 1.f / t.scale;
+  const unsigned per = (unsigned)(e.cols + 7) / 8;
+  const unsigned long long n = (unsigned long long)e.rows * per, first = (unsigned long long)((int)blockIdx.x - e.first8) * 1024 + threadIdx.x;
+#pragma unroll 2
+  for (int j = 0; j < 4; ++j) {
+    const unsigned long long i = first + j * 256;
+    if (i >= n) break;
+    const size_t row = n <= 0xffffffffu ? (size_t)((unsigned)i / per) : (size_t)(i / per);
     const int c = (int)(i - row * per) * 8;
-    const size_t dst = (size_t)row * b.cols + c;
+    const size_t dst = row * e.cols + c;
     float x[8], l[8], w[8];
-    unpack(load_group<__half, 8>(from + row * b.ld + c), x);
-    unpack(load_group<__half, 8>(from + b.plane + row * b.ld + c), l);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = (x[k] + l[k]) * unit;
-    if (b.r.update) {
-      if (b.vec) {
-        if (at.w) {
-#pragma unroll
-          for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(w + h) = *reinterpret_cast<const float4*>(at.w + dst + h);
-        } else {
-#pragma unroll
-          for (int h = 0; h < 8; h += kPerLoad<P>) {
-            float y[kPerLoad<P>];
-            unpack(load_group<P, kPerLoad<P>>(p + dst + h), y);
-#pragma unroll
-            for (int k = 0; k < kPerLoad<P>; ++k) w[h + k] = y[k];
-          }
-        }
+    unpack(load_group<__half, 8>(e.x + row * e.ld + c), x);
+    unpack(load_group<__half, 8>(e.x + e.plane + row * e.ld + c), l);
+    if (t.r.update) {
+      if (e.vec) {
+        if (master) load8(master + dst, w);
+        else load8(p + dst, w);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = c + k < b.cols ? (at.w ? at.w[dst + k] : to_float(p[dst + k])) : 0.f;
+        for (int k = 0; k < 8; ++k) w[k] = c + k < e.cols ? (master ? master[dst + k] : to_float(p[dst + k])) : 0.f;
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = updated(w[k], x[k], shrink, rate);
     }
-    if (b.vec) {
-      if (at.w && b.r.update) {
 #pragma unroll
-        for (int h = 0; h < 8; h += 4) *reinterpret_cast<float4*>(at.w + dst + h) = *reinterpret_cast<const float4*>(x + h);
-      }
-#pragma unroll
-      for (int h = 0; h < 8; h += kPerLoad<P>) {
-        float y[kPerLoad<P>];
-#pragma unroll
-        for (int k = 0; k < kPerLoad<P>; ++k) y[k] = x[h + k];
-        store_group(p + dst + h, pack<P>(y));
-      }
+    for (int k = 0; k < 8; ++k) {
+      x[k] = (x[k] + l[k]) * unit;
+      if (t.r.update) x[k] = updated(w[k], x[k], shrink, rate);
+    }
+    if (e.vec) {
+      if (master && t.r.update) store8(master + dst, x);
+      store8(p + dst, x);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (c + k >= b.cols) break;
-        if (at.w && b.r.update) at.w[dst + k] = x[k];
+        if (c + k >= e.cols) break;
+        if (master && t.r.update) master[dst + k] = x[k];
         p[dst + k] = from_float<P>(x[k]);
       }
     }
@@ -643,36 +678,50 @@ __global__ void __launch_bounds__(256) muon_apply_kernel(const __grid_constant__
 }
 
 // ---- the products ------------------------------------------------------------------------------------------------------------------
-// out = alpha sum_k L[m][k] R[n][k] + beta add, of planes, for a batch of matrices.  A pair of CTAs has a tile of 256 x BN; the shape is that of the
-// split products of gemm_tc.cu: 64 k of both planes in a stage, one thread issues, accumulators in turn, totals in registers.
-constexpr int kStep = 64, kGroup = 16;
-template <int BN>
+// out = alpha sum_k L[m][k] R[n][k] + beta add, of planes, for batches of matrices of several shapes (problems).  A pair of CTAs has a tile of
+// 256 x BN; one thread issues, accumulators in turn.
+// TERMS 3 (results of fp32 grade): both planes of 64 k in a stage, products hi hi + hi lo + lo hi; an accumulator holds kGroupSteps stages and is then added to
+// totals in registers.  TERMS 1 (results of 16 bits): hi planes alone, 128 k in a stage, and an accumulator holds the whole sum.
+constexpr int kStep = 64, kBand = 16, kGroupSteps = 2;
+constexpr int kPatch = 32 * 64;   // bytes of a warp's block of 32 x 32 halves on its way in or out
+template <int BN, int TERMS>
 struct Tile {
+  static constexpr int planes = 2;                      // blocks of 64 k in a stage: both planes' (TERMS 3), or two of the one plane
+  static constexpr int k = TERMS == 3 ? kStep : 2 * kStep;   // of a stage
   static constexpr int aplane = 128 * kStep * 2, bplane = BN / 2 * kStep * 2;
-  static constexpr int abytes = 2 * aplane, stage = abytes + 2 * bplane;      // 64 or 48 KB
-  static constexpr int stages = BN == 256 ? 3 : 4, depth = BN == 256 ? 2 : 4; // of the ring; accumulators
+  static constexpr int abytes = planes * aplane, stage = abytes + planes * bplane;                   // 64, 48, 32, 24 KB
+  static constexpr int stages = 192 * 1024 / stage, depth = BN == 256 ? 2 : 4;                       // of the ring; accumulators
   static constexpr int readers = 4 * BN / 64, threads = 64 + 32 * readers;
-  static constexpr size_t smem = (size_t)stages * stage + 1024 + 256;
-  static_assert(smem <= 227 * 1024 && depth * BN == 512, "");
+  static constexpr size_t smem = (size_t)stages * stage + readers * kPatch + 1024 + 256;
+  static_assert(smem <= 227 * 1024 && depth * BN == 512 && (2 * stages + 2 * depth) * 8 + 8 <= 256, "");
 };
-struct Newton {
-  int M, N, K, steps;            // of a result, of a sum
-  int tiles_m, tiles_n, per, units;
-  int symmetric;
+struct alignas(64) Problem {
+  CUtensorMap L, R;
+  int M, N, steps;               // of a result; of a sum, in stages
+  int tiles_m, tiles_n, per, first;   // tiles of a matrix; the problem's first one in the launch
+  int symmetric, l_mn, r_mn;     // an operand lies as [k][row] (boxes of 64 rows x 64 k), else as [row][k]
   float alpha, beta;
-  const __half* add;             // planes as out's, or null
+  const __half* add;             // as out, or null
   __half* out;
   int ld;
-  size_t plane, matrix;
+  size_t plane, add_plane, matrix;   // (planes: 0 where there is one only)
+};
+template <int CAP>
+struct Problems {
+  int count, units;
+  Problem p[CAP];
 };
 struct UnitAt {
-  int matrix, m0, n0;
+  int problem, matrix, m0, n0;
   bool mirror;
 };
-template <int BN>
-__device__ __forceinline__ UnitAt unit_at(const Newton& g, int unit) {
-  const int i = unit / g.per;
-  int t = unit - i * g.per;
+template <int BN, int CAP>
+__device__ __forceinline__ UnitAt unit_at(const Problems<CAP>& all, int unit) {
+  int k = 0;
+  while (k + 1 < all.count && all.p[k + 1].first <= unit) ++k;
+  const Problem& g = all.p[k];
+  const int i = (unit - g.first) / g.per;
+  int t = unit - g.first - i * g.per;
   if (g.symmetric) {             // rows of blocks, each from its diagonal on
     constexpr int q = 256 / BN;
     int row = 0, left = g.tiles_n;
@@ -682,10 +731,10 @@ __device__ __forceinline__ UnitAt unit_at(const Newton& g, int unit) {
       ++row;
     }
     const int n0 = (row * q + t) * BN;
-    return UnitAt{i, row * 256, n0, n0 >= (row + 1) * 256};
+    return UnitAt{k, i, row * 256, n0, n0 >= (row + 1) * 256};
   }
-  const int band = t / (kGroup * g.tiles_n), m1 = band * kGroup, height = min(kGroup, g.tiles_m - m1), q = t - m1 * g.tiles_n;
-  return UnitAt{i, (m1 + q % height) * 256, (q / height) * BN, false};
+  const int band = t / (kBand * g.tiles_n), m1 = band * kBand, height = min(kBand, g.tiles_m - m1), q = t - m1 * g.tiles_n;
+  return UnitAt{k, i, (m1 + q % height) * 256, (q / height) * BN, false};
 }
 __device__ __forceinline__ void tma_load_planes(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int matrix) {
   asm volatile(
@@ -701,20 +750,70 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
       : "memory");
 }
 
-// L_MN, R_MN: the operand lies as [k][row] (boxes of 64 rows x 64 k), else as [row][k].
-template <int BN, bool L_MN, bool R_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN>::threads, 1)
-newton_kernel(const __grid_constant__ Newton g, const __grid_constant__ CUtensorMap mapL, const __grid_constant__ CUtensorMap mapR) {
-  using T = Tile<BN>;
-  constexpr int kStages = T::stages, kBox = 2 * kStep * 128;   // bytes of an MN-major box, both planes
+// A warp's block of 32 rows of 32 halves, a row to a lane in registers, but 64 bytes of each of eight rows at a time in memory: through shared memory (rows of 64 bytes,
+// their 16-byte pieces swizzled).  Straight from the registers every access is of 32 rows and 16 bytes of each; the read-out of a tile then took 16 000 cycles, more than
+// the accumulators that wait meanwhile last.
+struct Block {
+  int M, N, ld, m0, n;
+  // (rows are longer than N where that is no multiple of eight: nobody reads what is behind)
+  __device__ __forceinline__ bool in(int i, int& row, int& col) const {
+    const int lane = threadIdx.x & 31;
+    row = m0 + i * 8 + (lane >> 2);
+    col = n + (lane & 3) * 8;
+    return row < M && col < N;
+  }
+  __device__ __forceinline__ static uint4* place(uint8_t* patch, int row, int piece) {
+    return reinterpret_cast<uint4*>(patch + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+  }
+  __device__ __forceinline__ void load(const __half* from, uint4 (&q)[4]) const {   // as it lies in memory
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int row, col;
+      q[i] = in(i, row, col) ? *reinterpret_cast<const uint4*>(from + (size_t)row * ld + col) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void turn(uint8_t* patch, uint4 (&q)[4]) const {       // to a row per lane
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *place(patch, i * 8 + (lane >> 2), lane & 3) = q[i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = *place(patch, lane, i);
+  }
+  __device__ __forceinline__ void store(uint8_t* patch, __half* to, const uint4 (&q)[4]) const {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *place(patch, lane, i) = q[i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int row, col;
+      if (in(i, row, col)) *reinterpret_cast<uint4*>(to + (size_t)row * ld + col) = *place(patch, i * 8 + (lane >> 2), lane & 3);
+    }
+  }
+};
+__device__ __forceinline__ void unpack_times(const uint4& q, float by, float* v, bool more) {
+  float x[8];
+  unpack(*reinterpret_cast<const Group<__half, 8>*>(&q), x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = more ? fmaf(by, x[i], v[i]) : by * x[i];
+}
+
+template <int BN, int TERMS, int CAP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN, TERMS>::threads, 1) newton_kernel(const __grid_constant__ Problems<CAP> all) {
+  using T = Tile<BN, TERMS>;
+  constexpr int kStages = T::stages, kBox = T::planes * kStep * 128;   // kBox: bytes of 64 rows, MN-major
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kStages * T::stage);
+  uint8_t* patches = sm + kStages * T::stage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(patches + T::readers * kPatch);
   uint64_t* full = bars;                 // [kStages] the leader's: the stage of both CTAs has landed  (tx bytes)
   uint64_t* empty = full + kStages;      // [kStages] the products that read the stage are done         (commit, both CTAs)
   uint64_t* accfull = empty + kStages;   // [depth] the accumulator is complete                         (commit, both CTAs)
-  uint64_t* accfree = accfull + 4;       // [depth] the leader's: read out by the warps of both CTAs
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accfree + 4);
+  uint64_t* accfree = accfull + T::depth;   // [depth] the leader's: read out by the warps of both CTAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accfree + T::depth);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
@@ -729,8 +828,6 @@ newton_kernel(const __grid_constant__ Newton g, const __grid_constant__ CUtensor
     }
     *abort_flag = 0;
     fence_barrier_init();
-    tma_prefetch_desc(&mapL);
-    tma_prefetch_desc(&mapR);
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before_sync();
@@ -747,25 +844,32 @@ newton_kernel(const __grid_constant__ Newton g, const __grid_constant__ CUtensor
     if (lane == 0) {
       int it = 0;
       bool ok = true;
-      for (int unit = pair; unit < g.units && ok; unit += npairs) {
-        const UnitAt t = unit_at<BN>(g, unit);
+      for (int unit = pair; unit < all.units && ok; unit += npairs) {
+        const UnitAt t = unit_at<BN>(all, unit);
+        const Problem& g = all.p[t.problem];
+        const int m = t.m0 + rank * 128, n = t.n0 + rank * (BN / 2);
         for (int s = 0; s < g.steps; ++s, ++it) {
           const int slot = it % kStages;
           if (it >= kStages && !(ok = wait_or_abort(emptyb + slot * 8, ((it / kStages) - 1) & 1, abortb))) break;
           if (rank == 0) mbar_expect_tx(&full[slot], 2 * T::stage);
           const uint32_t bar = leader_addr(fullb + slot * 8), a = smem_u32(sm) + slot * T::stage, b = a + T::abytes;
-          const int m = t.m0 + rank * 128, n = t.n0 + rank * (BN / 2), k = s * kStep;
-          if (L_MN) {
+          const int k = s * T::k;
+          // (TERMS 1: a box holds one block of 64 k; those of k past the end are zeros)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) tma_load_planes(a + q * kBox, &mapL, bar, m + q * 64, k, t.matrix);
-          } else {
-            tma_load_planes(a, &mapL, bar, k, m, t.matrix);
-          }
-          if (R_MN) {
+          for (int h = 0; h < (TERMS == 3 ? 1 : 2); ++h) {
+            const int kh = k + h * kStep;
+            if (g.l_mn) {
 #pragma unroll
-            for (int q = 0; q < BN / 128; ++q) tma_load_planes(b + q * kBox, &mapR, bar, n + q * 64, k, t.matrix);
-          } else {
-            tma_load_planes(b, &mapR, bar, k, n, t.matrix);
+              for (int q = 0; q < 2; ++q) tma_load_planes(a + q * kBox + h * (kStep * 128), &g.L, bar, m + q * 64, kh, t.matrix);
+            } else {
+              tma_load_planes(a + h * T::aplane, &g.L, bar, kh, m, t.matrix);
+            }
+            if (g.r_mn) {
+#pragma unroll
+              for (int q = 0; q < BN / 128; ++q) tma_load_planes(b + q * kBox + h * (kStep * 128), &g.R, bar, n + q * 64, kh, t.matrix);
+            } else {
+              tma_load_planes(b + h * T::bplane, &g.R, bar, kh, n, t.matrix);
+            }
           }
         }
       }
@@ -773,98 +877,147 @@ newton_kernel(const __grid_constant__ Newton g, const __grid_constant__ CUtensor
   } else if (warp == 1) {
     // ================= products: one thread of the pair ======================================================================
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = (1u << 4) | ((L_MN ? 1u : 0u) << 15) | ((R_MN ? 1u : 0u) << 16) | (((uint32_t)BN >> 3) << 17) | ((256u >> 4) << 24);
-      // K-major: rows of 128 bytes, eight rows per swizzle atom (1024 bytes); 16 k = 32 bytes on; the second plane all rows on.
-      // MN-major: 64 rows (128 bytes) per k, eight k per atom, the next 64 rows a box on; 16 k = 2048 bytes on; the second plane 64 k on.
-      const uint64_t dl = make_smem_desc(0, L_MN ? kBox : 16, 1024, kSwizzle128B), dr = make_smem_desc(0, R_MN ? kBox : 16, 1024, kSwizzle128B);
-      constexpr uint64_t sl = (L_MN ? 2048 : 32) >> 4, sr = (R_MN ? 2048 : 32) >> 4;
-      constexpr uint64_t pl = (L_MN ? kStep * 128 : T::aplane) >> 4, pr = (R_MN ? kStep * 128 : T::bplane) >> 4;
-      int it = 0;
+      int it = 0, gi = 0;   // stages, accumulators
       bool ok = true;
-      for (int unit = pair; unit < g.units && ok; unit += npairs) {
-        for (int s = 0; s < g.steps; ++s, ++it) {
-          const int slot = it % kStages, buf = it % T::depth;
+      for (int unit = pair; unit < all.units && ok; unit += npairs) {
+        const Problem& g = all.p[unit_at<BN>(all, unit).problem];
+        const uint32_t idesc = (1u << 4) | ((uint32_t)g.l_mn << 15) | ((uint32_t)g.r_mn << 16) | (((uint32_t)BN >> 3) << 17) | ((256u >> 4) << 24);
+        // K-major: rows of 128 bytes, eight rows per swizzle atom (1024 bytes); 16 k = 32 bytes on; the second plane all rows on.
+        // MN-major: 64 rows (128 bytes) per k, eight k per atom, the next 64 rows a box on; 16 k = 2048 bytes on; the second plane 64 k on.
+        const uint64_t dl = make_smem_desc(0, g.l_mn ? kBox : 16, 1024, kSwizzle128B), dr = make_smem_desc(0, g.r_mn ? kBox : 16, 1024, kSwizzle128B);
+        const uint64_t sl = (g.l_mn ? 2048 : 32) >> 4, sr = (g.r_mn ? 2048 : 32) >> 4;
+        const uint64_t pl = (g.l_mn ? kStep * 128 : T::aplane) >> 4, pr = (g.r_mn ? kStep * 128 : T::bplane) >> 4;
+        const int steps = g.steps;
+        for (int s = 0; s < steps; ++s, ++it) {
+          const int slot = it % kStages, buf = gi % T::depth;
+          const bool first = TERMS == 3 ? s % kGroupSteps == 0 : s == 0, last = s + 1 == steps || (TERMS == 3 && s % kGroupSteps == kGroupSteps - 1);
           if (!(ok = wait_or_abort(fullb + slot * 8, (it / kStages) & 1, abortb))) break;
-          if (it >= T::depth && !(ok = wait_or_abort(accfreeb + buf * 8, (it / T::depth - 1) & 1, abortb))) break;
+          if (first && gi >= T::depth && !(ok = wait_or_abort(accfreeb + buf * 8, (gi / T::depth - 1) & 1, abortb))) break;
           tc_fence_after_sync();
           const uint32_t a = smem_u32(sm) + slot * T::stage, d = tmem_base + buf * BN;
           const uint64_t l = dl + (a >> 4), r = dr + ((a + T::abytes) >> 4);
+          if (TERMS == 3) {
 #pragma unroll
-          for (int i = 0; i < kStep / 16; ++i) {   // the small products first
-            mma_f16_pair(d, l + pl + i * sl, r + i * sr, idesc, i > 0);
-            mma_f16_pair(d, l + i * sl, r + pr + i * sr, idesc, true);
+            for (int i = 0; i < kStep / 16; ++i) {   // the small products first
+              mma_f16_pair(d, l + pl + i * sl, r + i * sr, idesc, !first || i > 0);
+              mma_f16_pair(d, l + i * sl, r + pr + i * sr, idesc, true);
+            }
           }
 #pragma unroll
-          for (int i = 0; i < kStep / 16; ++i) mma_f16_pair(d, l + i * sl, r + i * sr, idesc, true);
-          commit_pair(accfullb + buf * 8);
+          for (int i = 0; i < kStep / 16; ++i) mma_f16_pair(d, l + i * sl, r + i * sr, idesc, TERMS == 3 || !first || i > 0);
+          if (TERMS == 1) {
+#pragma unroll
+            for (int i = 0; i < kStep / 16; ++i) mma_f16_pair(d, l + pl + i * sl, r + pr + i * sr, idesc, true);
+          }
+          if (last) {
+            commit_pair(accfullb + buf * 8);
+            ++gi;
+          }
           commit_pair(emptyb + slot * 8);
         }
       }
     }
   } else {
-    // ================= read-out: accumulators -> totals -> planes =============================================================
+    // ================= read-out: accumulators -> (totals ->) planes ===========================================================
     const int qd = warp & 3, c0 = ((warp - 2) >> 2) * 64;   // the lane quarter that this warp may read, and its columns
     const uint32_t taddr = tmem_base + ((uint32_t)(qd * 32) << 16) + c0;
-    int it = 0;
+    int gi = 0;
     bool ok = true;
-    for (int unit = pair; unit < g.units && ok; unit += npairs) {
-      float tot[64];
-#pragma unroll
-      for (int j = 0; j < 64; ++j) tot[j] = 0.f;
+    for (int unit = pair; unit < all.units && ok; unit += npairs) {
       int buf = 0;
-      for (int s = 0; s < g.steps; ++s, ++it) {
-        buf = it % T::depth;
-        if (!(ok = __all_sync(0xffffffffu, wait_or_abort(accfullb + buf * 8, (it / T::depth) & 1, abortb)))) break;
-        tc_fence_after_sync();
+      if constexpr (TERMS == 3) {
+        float tot[64];
 #pragma unroll
-        for (int j0 = 0; j0 < 64; j0 += 16) {
-          float v[16];
-          tmem_ld16(taddr + buf * BN + j0, v);
-          if (j0 == 48 && s + 1 < g.steps) {
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
+        for (int j = 0; j < 64; ++j) tot[j] = 0.f;
+        const int groups = (all.p[unit_at<BN>(all, unit).problem].steps + kGroupSteps - 1) / kGroupSteps;
+        for (int s = 0; s < groups; ++s, ++gi) {
+          buf = gi % T::depth;
+          if (!(ok = __all_sync(0xffffffffu, wait_or_abort(accfullb + buf * 8, (gi / T::depth) & 1, abortb)))) break;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int j0 = 0; j0 < 64; j0 += 16) {
+            float v[16];
+            tmem_ld16(taddr + buf * BN + j0, v);
+            if (j0 == 48 && s + 1 < groups) {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) tot[j0 + j] += v[j];
           }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) tot[j0 + j] += v[j];
         }
+        if (!ok) break;
+        // through the accumulator just read, so that a short loop stores them (unrolled over registers it is code that every tile fetches anew)
+#pragma unroll
+        for (int j0 = 0; j0 < 64; j0 += 16) tmem_st16(taddr + buf * BN + j0, tot + j0);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      } else {
+        buf = gi % T::depth;
+        if (!(ok = __all_sync(0xffffffffu, wait_or_abort(accfullb + buf * 8, (gi / T::depth) & 1, abortb)))) break;
+        tc_fence_after_sync();
+        ++gi;
       }
-      if (!ok) break;
-      // through the accumulator just read, so that a short loop stores them (unrolled over registers it is code that every tile fetches anew)
-#pragma unroll
-      for (int j0 = 0; j0 < 64; j0 += 16) tmem_st16(taddr + buf * BN + j0, tot + j0);
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      const UnitAt t = unit_at<BN>(g, unit);
-      const int m = t.m0 + rank * 128 + qd * 32 + lane;
-      const size_t base = t.matrix * g.matrix, row = base + (size_t)m * g.ld;
+      const UnitAt t = unit_at<BN>(all, unit);
+      const Problem& g = all.p[t.problem];
+      const int m0 = t.m0 + rank * 128 + qd * 32, m = m0 + lane;
+      uint8_t* patch = patches + (warp - 2) * kPatch;
+      const size_t base = t.matrix * g.matrix;
 #pragma unroll 1
-      for (int j0 = 0; j0 < 64; j0 += 8) {
+      for (int j0 = 0; j0 < 64; j0 += 32) {
         const int n = t.n0 + c0 + j0;
-        float v[8];
-        tmem_ld8(taddr + buf * BN + j0, v);
-        if (n >= g.N || m >= g.M) continue;
+        if (m0 >= g.M || n >= g.N) continue;   // (all lanes)
+        __syncwarp();
+        const Block at{g.M, g.N, g.ld, m0, n};
+        float v[32];
         if (g.add) {
-          float x[8], y[8];
-          unpack(load_group<__half, 8>(g.add + row + n), x);
-          unpack(load_group<__half, 8>(g.add + row + n + g.plane), y);
+          uint4 in[4], more[4];
+          at.load(g.add + base, in);
+          if (g.add_plane) at.load(g.add + base + g.add_plane, more);
+          at.turn(patch, in);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = fmaf(g.alpha, v[j], g.beta * (x[j] + y[j]));
+          for (int j = 0; j < 32; j += 8) unpack_times(in[j / 8], g.beta, v + j, false);
+          if (g.add_plane) {
+            at.turn(patch, more);
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) unpack_times(more[j / 8], g.beta, v + j, true);
+          }
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] *= g.alpha;
+          for (int j = 0; j < 32; ++j) v[j] = 0.f;
         }
-        Group<__half, 8> hi, lo;
-        split8(v, hi, lo);
-        store_group(g.out + row + n, hi);   // (the row's padding too)
-        store_group(g.out + row + n + g.plane, lo);
-        if (t.mirror) {   // neighbouring lanes have neighbouring columns of these
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (n + j < g.N) {
-              __half* to = g.out + base + (size_t)(n + j) * g.ld + m;
-              to[0] = hi.v[j];
-              to[g.plane] = lo.v[j];
-            }
+        for (int j = 0; j < 32; j += 8) {
+          float x[8];
+          tmem_ld8(taddr + buf * BN + j0 + j, x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[j + i] = fmaf(g.alpha, x[i], v[j + i]);
+        }
+        __half* out = g.out + base;
+#pragma unroll
+        for (int plane = 0; plane < 2; ++plane) {   // hi, then what is left
+          if (plane && !g.plane) break;
+          uint4 q[4];
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            Group<__half, 8> h;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = v[j + i];
+            h = pack<__half>(x);
+            unpack(h, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j + i] -= x[i];
+            q[j / 8] = *reinterpret_cast<const uint4*>(&h);
+          }
+          __half* to = out + plane * g.plane;
+          if (t.mirror && m < g.M) {   // neighbouring lanes have neighbouring columns of these
+            const __half* h = reinterpret_cast<const __half*>(q);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (n + j < g.N) to[(size_t)(n + j) * g.ld + m] = h[j];
+          }
+          at.store(patch, to, q);
         }
       }
       tc_fence_before_sync();
@@ -888,60 +1041,98 @@ newton_kernel(const __grid_constant__ Newton g, const __grid_constant__ CUtensor
 }
 
 // ======== host ======================================================================================================================
-struct Planes {   // of a batch of matrices
+// (A slot per kernel, not per caller: callers of several types share some, and each would set its own, smaller size.)
+template <auto KERNEL>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<int> set[64];
+  return ensure_dynamic_smem(reinterpret_cast<const void*>(KERNEL), set, bytes);
+}
+struct Planes {   // of a batch of matrices; one plane or two
   __half* p;
-  int rows, cols, ld, count;
+  int rows, cols, ld, count, planes;
   size_t plane() const { return (size_t)rows * ld; }
-  size_t matrix() const { return 2 * plane(); }
+  size_t matrix() const { return planes * plane(); }
 };
-int ld8(int n) { return (n + 7) / 8 * 8; }
-int encode(CUtensorMap* map, const Planes& m, int box_rows) {
+// Rows of planes start on 128-byte lines, so that what a tile takes of one is one line (1030 x 2051 in rows of 2056: 32.8 us for X X^T, now 28.7).
+int pitch_of(int n) { return (n + 63) / 64 * 64; }
+int encode(CUtensorMap* map, const Planes& m, int box_rows, int terms) {
   PFN_encodeTiled enc = get_encode_tiled();
   if (!enc) return fail(B200CP_ERR_NO_DEVICE, "cuTensorMapEncodeTiled entry point not available");
-  const cuuint64_t dim[4] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, 2, (cuuint64_t)m.count},
+  const cuuint64_t dim[4] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.planes, (cuuint64_t)m.count},
                    stride[3] = {(cuuint64_t)m.ld * 2, (cuuint64_t)m.plane() * 2, (cuuint64_t)m.matrix() * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 2, 1}, estr[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, terms == 3 ? 2u : 1u, 1}, estr[4] = {1, 1, 1, 1};
   const CUresult cr = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, m.p, dim, stride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (cr != CUDA_SUCCESS) return fail(B200CP_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)cr);
   return B200CP_OK;
 }
-int units_of(int M, int N, int BN, bool symmetric) {   // of one matrix
-  const int tm = ceil_div(M, 256), tn = ceil_div(N, BN), q = 256 / BN;
+long long tiles_of(int M, int N, int BN, bool symmetric) {   // of one matrix
+  const long long tm = ceil_div(M, 256), tn = ceil_div(N, BN), q = 256 / BN;
   return symmetric ? tm * tn - q * tm * (tm - 1) / 2 : tm * tn;
 }
-template <int BN, bool L_MN, bool R_MN>
-int product_of(Newton g, const Planes& L, const Planes& R, const Planes& out, bool symmetric, int pairs, cudaStream_t st) {
-  using T = Tile<BN>;
-  CUtensorMap ml, mr;
-  if (int rc = encode(&ml, L, L_MN ? kStep : 128)) return rc;
-  if (int rc = encode(&mr, R, R_MN ? kStep : BN / 2)) return rc;
-  g.symmetric = symmetric;
-  g.tiles_m = ceil_div(g.M, 256);
-  g.tiles_n = ceil_div(g.N, BN);
-  g.per = units_of(g.M, g.N, BN, symmetric);
-  g.units = g.per * out.count;
-  g.steps = ceil_div(g.K, kStep);
-  const auto kern = newton_kernel<BN, L_MN, R_MN>;
-  static std::atomic<int> set[64];
-  B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, (int)T::smem));
-  B200CP_CUDA_OK(launch_kernel(kern, dim3(2 * std::min(g.units, pairs)), dim3(T::threads), T::smem, st, true, g, ml, mr));
+// out = alpha L R^T + beta add
+struct Product {
+  Planes L, R, out;
+  bool l_mn, r_mn, symmetric;
+  int K;
+  double alpha, beta;
+  const Planes* add;
+};
+template <int BN, int TERMS, int CAP>
+int launch_table(const std::vector<Product>& ps, int pairs, cudaStream_t st) {
+  using T = Tile<BN, TERMS>;
+  Problems<CAP> all;
+  all.count = 0;
+  long long units = 0;
+  for (const Product& q : ps) {
+    Problem& p = all.p[all.count++];
+    if (int rc = encode(&p.L, q.L, q.l_mn ? kStep : 128, TERMS)) return rc;
+    if (int rc = encode(&p.R, q.R, q.r_mn ? kStep : BN / 2, TERMS)) return rc;
+    p.M = q.out.rows;
+    p.N = q.out.cols;
+    p.steps = ceil_div(q.K, T::k);
+    p.tiles_m = ceil_div(p.M, 256);
+    p.tiles_n = ceil_div(p.N, BN);
+    p.per = (int)tiles_of(p.M, p.N, BN, q.symmetric);
+    p.first = (int)units;
+    p.symmetric = q.symmetric;
+    p.l_mn = q.l_mn;
+    p.r_mn = q.r_mn;
+    p.alpha = (float)q.alpha;
+    p.beta = (float)q.beta;
+    p.add = q.add ? q.add->p : nullptr;
+    p.add_plane = q.add && q.add->planes == 2 ? q.add->plane() : 0;
+    p.out = q.out.p;
+    p.ld = q.out.ld;
+    p.plane = q.out.planes == 2 ? q.out.plane() : 0;
+    p.matrix = q.out.matrix();
+    units += (long long)p.per * q.out.count;
+  }
+  if (units > 0x3fffffff) return fail(B200CP_ERR_UNSUPPORTED, "b200cp_muon_step: the matrices are too large");
+  all.units = (int)units;
+  const auto kern = newton_kernel<BN, TERMS, CAP>;
+  B200CP_CUDA_OK((allow_smem<newton_kernel<BN, TERMS, CAP>>((int)T::smem)));
+  B200CP_CUDA_OK(launch_kernel(kern, dim3((unsigned)(2 * std::min<long long>(units, pairs))), dim3(T::threads), T::smem, st, true, all));
   B200CP_LAUNCH_OK("newton_kernel");
   return B200CP_OK;
 }
-// out = alpha L R^T + beta add.  Tiles of 256 columns, or of 128 where there are not two of the wider ones for every pair of CTAs.
-template <bool L_MN, bool R_MN>
-int product(const Planes& L, const Planes& R, int K, float alpha, float beta, const Planes* add, const Planes& out, bool symmetric, cudaStream_t st) {
-  DeviceInfo di;
-  if (int rc = device_info(&di)) return rc;
+template <int BN, int TERMS>
+int launch_products(const std::vector<Product>& ps, int pairs, cudaStream_t st) {
+  return ps.size() <= kFewProblems ? launch_table<BN, TERMS, kFewProblems>(ps, pairs, st) : launch_table<BN, TERMS, kProblems>(ps, pairs, st);
+}
+// One launch for all, the longest sums first.  Tiles of 256 columns, or of 128 where those fill the pairs of CTAs better: a narrow tile takes 0.55 of a wide one (0.65 with one
+// plane, where the loads count), so 4096 x 4096 goes in seven rounds of narrow ones, not in four of wide ones (279 us a product, and 350); 4096 x 10240 in nine of wide
+// ones, not in 18.
+int products(std::vector<Product> ps, int terms, const DeviceInfo& di, cudaStream_t st) {
   const int pairs = di.sm_count / 2;
-  Newton g{};
-  g.M = out.rows; g.N = out.cols; g.K = K;
-  g.alpha = alpha; g.beta = beta;
-  g.add = add ? add->p : nullptr;
-  g.out = out.p; g.ld = out.ld; g.plane = out.plane(); g.matrix = out.matrix();
-  if ((long long)units_of(g.M, g.N, 256, symmetric) * out.count >= 2LL * pairs) return product_of<256, L_MN, R_MN>(g, L, R, out, symmetric, pairs, st);
-  return product_of<128, L_MN, R_MN>(g, L, R, out, symmetric, pairs, st);
+  std::stable_sort(ps.begin(), ps.end(), [](const Product& a, const Product& b) { return a.K > b.K; });
+  long long tiles[2] = {};
+  for (const Product& p : ps)
+    for (int i = 0; i < 2; ++i) tiles[i] += tiles_of(p.out.rows, p.out.cols, 128 << i, p.symmetric) * p.out.count;
+  const auto rounds = [&](long long n) { return (double)((n + pairs - 1) / pairs); };
+  const bool wide = rounds(tiles[1]) <= (terms == 3 ? 0.55 : 0.65) * rounds(tiles[0]);
+  if (terms == 3) return wide ? launch_products<256, 3>(ps, pairs, st) : launch_products<128, 3>(ps, pairs, st);
+  return wide ? launch_products<256, 1>(ps, pairs, st) : launch_products<128, 1>(ps, pairs, st);
 }
 
 // ---- bounds on the singular values, and the scales of the planes that follow ----------------------------------------------------------
@@ -989,10 +1180,10 @@ struct SmallSizes {
   size_t doubles = 0, floats = 0;
   int matrices = 0, ctas = 0;
 };
-// Parts of a matrix: as long as leaves the GPU four CTAs for each SM over all of the call's matrices, so that there are few parts to be added.
+// Parts of a matrix: as long as gives every SM the three CTAs that it holds over all of the call's matrices: one round of them, and few parts to be added.
 void cut_small(const b200cp_muon_matrix& a, long long all, int sm_count, SmallEntry* e, SmallSizes* s) {
   const int n = std::min(a.rows, a.cols), len = std::max(a.rows, a.cols), subs = ceil_div(len, kSub), ts = tile_side(n);
-  const int parts = (int)std::min<long long>(subs, std::max<long long>(1, 4LL * sm_count / std::max<long long>(1, all)));
+  const int parts = (int)std::min<long long>(subs, std::max<long long>(1, 3LL * sm_count / std::max<long long>(1, all)));
   e->rows = a.rows; e->cols = a.cols; e->stack = a.stack;
   e->length = ceil_div(subs, parts) * kSub;
   e->chunks = ceil_div(len, e->length);
@@ -1009,7 +1200,7 @@ size_t small_bytes(const SmallSizes& s) {
   return align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256) + align_up(s.floats * 4, 256);
 }
 // Small matrices of a launch: tensors from `at` on, up to a table's size and 2^20 CTAs.
-int next_small(const std::vector<b200cp_muon_matrix>& ms, size_t at, long long all, int sm_count, SmallTable* t, SmallSizes* s) {
+int next_small(const std::vector<b200cp_muon_matrix>& ms, size_t at, long long all, int sm_count, SmallTable<kTableSmall>* t, SmallSizes* s) {
   int count = 0;
   while (at + count < ms.size() && count < kTableSmall && s->ctas < (1 << 20)) {
     SmallEntry e{};
@@ -1054,24 +1245,50 @@ struct Work {
     }
   }
 };
-// Matrices of a shape that share launches: as many as give each pair of CTAs eight tiles of X, within a gigabyte of planes.
-int batch_of(const Shape& s) {
-  const int tiles = ceil_div(s.rows, 256) * ceil_div(s.cols, 256);
-  const size_t each = 8 * ((size_t)s.rows * ld8(s.cols) + (size_t)std::min(s.rows, s.cols) * ld8(std::min(s.rows, s.cols)));
-  const size_t room = std::max<size_t>(1, ((size_t)1 << 30) / each);
-  return (int)std::min<size_t>(std::min<size_t>(s.at.size(), kBatch), std::min<size_t>(room, (size_t)std::max(1, ceil_div(600, tiles))));
-}
-struct LargeSizes {
-  size_t x, a, norms, all;
+// Larger matrices that share launches: parts of shapes, as the tables and some memory hold them.
+struct Share {
+  const Shape* s;
+  int first, count;
 };
-LargeSizes large_sizes(const Shape& s, int count) {
+struct ShareSizes {
+  size_t x, a;   // bytes of the planes of X, of a square matrix
+};
+ShareSizes share_sizes(const Shape& s, int count) {
   const size_t n = std::min(s.rows, s.cols);
-  LargeSizes z;
-  z.x = align_up((size_t)count * 2 * s.rows * ld8(s.cols) * 2, 256);
-  z.a = align_up((size_t)count * 2 * n * ld8((int)n) * 2, 256);
-  z.norms = align_up((size_t)count * kNormParts * 8, 256);
-  z.all = 2 * z.x + 2 * z.a + z.norms;
-  return z;
+  return ShareSizes{align_up((size_t)count * 4 * s.rows * pitch_of(s.cols), 256), align_up((size_t)count * 4 * n * pitch_of((int)n), 256)};
+}
+size_t share_bytes(const Share& s) {
+  const ShareSizes z = share_sizes(*s.s, s.count);
+  return 2 * z.x + 2 * z.a;
+}
+std::vector<std::vector<Share>> rounds_of(const Work& w) {
+  constexpr size_t kRoom = (size_t)3 << 29;   // 1.5 GB, or one matrix
+  std::vector<std::vector<Share>> out(1);
+  size_t used = 0;
+  int items = 0;
+  for (const Shape& s : w.large) {
+    const size_t each = share_bytes(Share{&s, 0, 1});
+    for (int first = 0; first < (int)s.at.size();) {
+      if (items == kItems || (int)out.back().size() == kProblems || (items && used + each > kRoom)) {
+        out.emplace_back();
+        used = 0;
+        items = 0;
+      }
+      const size_t room = used < kRoom ? (kRoom - used) / each : 0;
+      const int count = (int)std::min<size_t>({s.at.size() - first, (size_t)(kItems - items), std::max<size_t>(1, room)});
+      out.back().push_back(Share{&s, first, count});
+      used += each * count;
+      items += count;
+      first += count;
+    }
+  }
+  if (out.back().empty()) out.pop_back();
+  return out;
+}
+size_t round_bytes(const std::vector<Share>& round) {
+  size_t n = align_up((size_t)kItems * kNormParts * 8, 256);
+  for (const Share& s : round) n += share_bytes(s);
+  return n;
 }
 size_t workspace_of(const Work& w, int sm_count) {
   size_t most = 0;
@@ -1080,7 +1297,7 @@ size_t workspace_of(const Work& w, int sm_count) {
     at += next_small(w.little, at, w.matrices, sm_count, nullptr, &s);
     most = std::max(most, small_bytes(s));
   }
-  for (const Shape& s : w.large) most = std::max(most, large_sizes(s, batch_of(s)).all);
+  for (const std::vector<Share>& r : rounds_of(w)) most = std::max(most, round_bytes(r));
   return most;
 }
 float factor_of(int adjust, int rows, int cols) {
@@ -1089,18 +1306,33 @@ float factor_of(int adjust, int rows, int cols) {
   return 1.f;
 }
 
-// (A slot per kernel, not per caller: callers of several types share some, and each would set its own, smaller size.)
-template <auto KERNEL>
-cudaError_t allow_smem(int bytes) {
-  static std::atomic<int> set[64];
-  return ensure_dynamic_smem(reinterpret_cast<const void*>(KERNEL), set, bytes);
+template <typename P, typename G, int CAP>
+int launch_small(const SmallHead& head, const SmallEntry* e, const Coefficients& co, const SmallSizes& s, cudaStream_t st) {
+  SmallTable<CAP> t;
+  static_cast<SmallHead&>(t) = head;
+  std::copy(e, e + head.count, t.e);
+  int ts = 1;
+  for (int i = 0; i < t.count; ++i) ts = std::max(ts, tile_side(std::min(t.e[i].rows, t.e[i].cols)));
+  // (each as much as the widest matrix of the launch needs; the others need less)
+  const int gram = std::max({gram_doubles(1), ts > 1 ? gram_doubles(2) : 0, ts > 2 ? gram_doubles(4) : 0}) * 8, four = 4 * 16 * ts * (16 * ts + 4) * 8,
+            low = std::max({small_apply_floats(1), ts > 1 ? small_apply_floats(2) : 0, ts > 2 ? small_apply_floats(4) : 0}) * 4;
+  B200CP_CUDA_OK((allow_smem<muon_gram_kernel<G, CAP>>(gram)));
+  B200CP_CUDA_OK(launch_kernel(muon_gram_kernel<G, CAP>, dim3(s.ctas), dim3(256), gram, st, true, t));
+  B200CP_LAUNCH_OK("muon_gram_kernel");
+  B200CP_CUDA_OK(allow_smem<muon_iterate_kernel<CAP>>(four));
+  B200CP_CUDA_OK(launch_kernel(muon_iterate_kernel<CAP>, dim3(s.matrices), dim3(kIterateThreads), four, st, true, t, co));
+  B200CP_LAUNCH_OK("muon_iterate_kernel");
+  B200CP_CUDA_OK((allow_smem<muon_small_apply_kernel<P, G, CAP>>(low)));
+  B200CP_CUDA_OK(launch_kernel(muon_small_apply_kernel<P, G, CAP>, dim3(s.ctas), dim3(256), low, st, true, t));
+  B200CP_LAUNCH_OK("muon_small_apply_kernel");
+  return B200CP_OK;
 }
 template <typename P, typename G>
 int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char* ws, const DeviceInfo& di, cudaStream_t st) {
-  Coefficients co{};
+  Coefficients co;
   if (plan.steps) std::copy(plan.v, plan.v + 3 * plan.coefficients, co.v);
+  SmallTable<kTableSmall> t;
   for (size_t at = 0; at < w.little.size();) {
-    SmallTable t;
     SmallSizes s;
     t.count = next_small(w.little, at, w.matrices, di.sm_count, &t, &s);
     at += t.count;
@@ -1110,88 +1342,117 @@ int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char*
     t.gram = reinterpret_cast<double*>(ws);
     t.inverse = reinterpret_cast<double*>(ws + align_up(s.doubles * 8, 256));
     t.q = reinterpret_cast<float*>(ws + align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256));
-    int ts = 1;
-    for (int i = 0; i < t.count; ++i) {
-      t.e[i].scale = factor_of(adjust, t.e[i].rows, t.e[i].cols);
-      ts = std::max(ts, tile_side(std::min(t.e[i].rows, t.e[i].cols)));
-    }
-    // (each as much as the widest matrix of the launch needs; the others need less)
-    const int gram = std::max({gram_doubles(1), ts > 1 ? gram_doubles(2) : 0, ts > 2 ? gram_doubles(4) : 0}) * 8, four = 4 * 16 * ts * (16 * ts + 4) * 8,
-              low = std::max({small_apply_floats(1), ts > 1 ? small_apply_floats(2) : 0, ts > 2 ? small_apply_floats(4) : 0}) * 4;
-    B200CP_CUDA_OK(allow_smem<muon_gram_kernel<G>>(gram));
-    B200CP_CUDA_OK(launch_kernel(muon_gram_kernel<G>, dim3(s.ctas), dim3(256), gram, st, true, t));
-    B200CP_LAUNCH_OK("muon_gram_kernel");
-    B200CP_CUDA_OK(allow_smem<muon_iterate_kernel>(four));
-    B200CP_CUDA_OK(launch_kernel(muon_iterate_kernel, dim3(s.matrices), dim3(kIterateThreads), four, st, true, t, co));
-    B200CP_LAUNCH_OK("muon_iterate_kernel");
-    B200CP_CUDA_OK((allow_smem<muon_small_apply_kernel<P, G>>(low)));
-    B200CP_CUDA_OK(launch_kernel(muon_small_apply_kernel<P, G>, dim3(s.ctas), dim3(256), low, st, true, t));
-    B200CP_LAUNCH_OK("muon_small_apply_kernel");
+    for (int i = 0; i < t.count; ++i) t.e[i].scale = factor_of(adjust, t.e[i].rows, t.e[i].cols);
+    if (int rc = t.count <= kFewSmall ? launch_small<P, G, kFewSmall>(t, t.e, co, s, st) : launch_small<P, G, kTableSmall>(t, t.e, co, s, st)) return rc;
   }
   return B200CP_OK;
 }
 
-template <typename P, typename G>
-int run_large(const Shape& s, int first, int count, const Rates& r, const Plan& plan, int adjust, char* ws, const DeviceInfo& di, cudaStream_t st) {
-  const LargeSizes z = large_sizes(s, count);
-  const int n = std::min(s.rows, s.cols), len = std::max(s.rows, s.cols);
-  const bool wide = s.rows <= s.cols;
-  Planes X{reinterpret_cast<__half*>(ws), s.rows, s.cols, ld8(s.cols), count}, Y = X, A{reinterpret_cast<__half*>(ws + 2 * z.x), n, n, ld8(n), count}, B = A;
-  Y.p = reinterpret_cast<__half*>(ws + z.x);
-  B.p = reinterpret_cast<__half*>(ws + 2 * z.x + z.a);
-  Batch b{};
-  b.r = r;
-  b.count = count; b.rows = s.rows; b.cols = s.cols; b.ld = X.ld;
-  b.plane = X.plane(); b.matrix = X.matrix();
+// (Taking the last steps on A, as the small matrices do, is 20 % less work for sides of 1 to 2.5, but Q then raises what X lacks by 41 while it leaves what X has:
+// sums that cancel, where the tensor core's cut sums show.  A gradient of rank one came out 1e-3 off, of these forms 3e-5.)
+struct Large {
+  Planes X, Y, A, B;
+  bool wide;
+  int n, len;
+};
+template <typename P, typename G, int CAP>
+int run_large(const std::vector<Share>& round, const Rates& r, const Plan& plan, int adjust, int terms, char* ws, const DeviceInfo& di, cudaStream_t st) {
+  Items<CAP> t;
+  t.r = r;
+  t.count = 0;
+  t.norms = reinterpret_cast<double*>(ws);
+  ws += align_up((size_t)kItems * kNormParts * 8, 256);
   double sx = room_for(plan.bound[0]);
-  b.scale = (float)sx;
-  b.rate = factor_of(adjust, s.rows, s.cols);
-  b.x = X.p;
-  b.norms = reinterpret_cast<double*>(ws + 2 * z.x + 2 * z.a);
-  uintptr_t off = s.cols % 8;
-  for (int i = 0; i < count; ++i) {
-    b.at[i] = s.at[first + i];
-    off |= (reinterpret_cast<uintptr_t>(b.at[i].p) | reinterpret_cast<uintptr_t>(b.at[i].g) | reinterpret_cast<uintptr_t>(b.at[i].m) |
-            reinterpret_cast<uintptr_t>(b.at[i].w)) & 15;
+  t.scale = (float)sx;
+  std::vector<Large> ms;
+  long long ctas = 0, ctas8 = 0;
+  int norm = 0;
+  const int planes = terms == 3 ? 2 : 1;
+  for (const Share& q : round) {
+    const Shape& s = *q.s;
+    const ShareSizes z = share_sizes(s, q.count);
+    Large m;
+    m.n = std::min(s.rows, s.cols);
+    m.len = std::max(s.rows, s.cols);
+    m.wide = s.rows <= s.cols;
+    const auto half = [&](size_t at) { return reinterpret_cast<__half*>(ws + at); };
+    m.X = Planes{half(0), s.rows, s.cols, pitch_of(s.cols), q.count, 2};
+    m.Y = m.X;
+    m.Y.p = half(z.x);
+    m.A = Planes{half(2 * z.x), m.n, m.n, pitch_of(m.n), q.count, planes};
+    m.B = m.A;
+    m.B.p = half(2 * z.x + z.a);
+    ws += share_bytes(q);
+    const long long values = (long long)s.rows * s.cols, groups = (long long)s.rows * ((s.cols + 7) / 8);
+    const long long chunk = std::max<long long>(kTurn, (values + kNormParts * 2048LL - 1) / (kNormParts * 2048LL) * 2048);
+    if (chunk > 0x7fffffff) return fail(B200CP_ERR_UNSUPPORTED, "b200cp_muon_step: a matrix of %d x %d", s.rows, s.cols);
+    for (int i = 0; i < q.count; ++i) {
+      Item& e = t.e[t.count++];
+      e.at = s.at[q.first + i];
+      e.rows = s.rows;
+      e.cols = s.cols;
+      e.ld = m.X.ld;
+      e.plane = m.X.plane();
+      e.x = m.X.p + i * m.X.matrix();
+      e.vec = s.cols % 8 == 0 && !((reinterpret_cast<uintptr_t>(e.at.p) | reinterpret_cast<uintptr_t>(e.at.g) | reinterpret_cast<uintptr_t>(e.at.m) |
+                                    reinterpret_cast<uintptr_t>(e.at.w)) & 15);
+      e.first = (int)ctas;
+      e.chunk = (int)chunk;
+      e.parts = (int)((values + chunk - 1) / chunk);
+      e.norm = norm;
+      e.first8 = (int)ctas8;
+      e.rate = factor_of(adjust, s.rows, s.cols);
+      ctas += e.parts;
+      ctas8 += (groups + 1023) / 1024;
+      norm += e.parts;
+    }
+    ms.push_back(m);
   }
-  b.vec = off == 0;
-  const long long values = (long long)s.rows * s.cols;
-  b.parts = (int)std::min<long long>(kNormParts, (values + 2047) / 2048);
-  B200CP_CUDA_OK(launch_kernel(muon_momentum_kernel<G>, dim3(b.parts, count), dim3(256), 0, st, true, b));
+  if (ctas8 > 0x7fffffff) return fail(B200CP_ERR_UNSUPPORTED, "b200cp_muon_step: the matrices are too large");
+  B200CP_CUDA_OK(launch_kernel(muon_momentum_kernel<G, CAP>, dim3((unsigned)ctas), dim3(256), 0, st, true, t));
   B200CP_LAUNCH_OK("muon_momentum_kernel");
-  const int rows8 = (int)std::min<long long>(16LL * di.sm_count, ((long long)s.rows * (X.ld / 8) + 255) / 256);
-  B200CP_CUDA_OK(launch_kernel(muon_planes_kernel<G>, dim3(rows8, count), dim3(256), 0, st, true, b));
+  B200CP_CUDA_OK(launch_kernel(muon_planes_kernel<G, CAP>, dim3((unsigned)ctas8), dim3(256), 0, st, true, t));
   B200CP_LAUNCH_OK("muon_planes_kernel");
   for (int step = 0; step < plan.steps; ++step) {
     const double* v = plan.v + (plan.coefficients > 1 ? 3 * step : 0);
     const double y = plan.bound[step] * plan.bound[step], sa = room_for(y),
                  sb = room_for(std::max(1e-3, std::fabs(v[1]) * y + std::fabs(v[2]) * y * y)), sn = room_for(plan.bound[step + 1]);
-    if (int rc = wide ? product<false, false>(X, X, len, (float)(sa / (sx * sx)), 0.f, nullptr, A, true, st)
-                      : product<true, true>(X, X, len, (float)(sa / (sx * sx)), 0.f, nullptr, A, true, st))
-      return rc;
-    if (int rc = product<false, false>(A, A, n, (float)(v[2] * sb / (sa * sa)), (float)(v[1] * sb / sa), &A, B, true, st)) return rc;
-    if (int rc = wide ? product<false, true>(B, X, n, (float)(sn / (sb * sx)), (float)(v[0] * sn / sx), &X, Y, false, st)
-                      : product<false, false>(X, B, n, (float)(sn / (sb * sx)), (float)(v[0] * sn / sx), &X, Y, false, st))
-      return rc;
-    std::swap(X, Y);
+    std::vector<Product> ps;
+    for (Large& m : ms) ps.push_back(Product{m.X, m.X, m.A, !m.wide, !m.wide, true, m.len, sa / (sx * sx), 0, nullptr});
+    if (int rc = products(ps, terms, di, st)) return rc;
+    ps.clear();
+    for (Large& m : ms) ps.push_back(Product{m.A, m.A, m.B, false, false, true, m.n, v[2] * sb / (sa * sa), v[1] * sb / sa, &m.A});
+    if (int rc = products(ps, terms, di, st)) return rc;
+    ps.clear();
+    for (Large& m : ms)
+      ps.push_back(m.wide ? Product{m.B, m.X, m.Y, false, true, false, m.n, sn / (sb * sx), v[0] * sn / sx, &m.X}
+                          : Product{m.X, m.B, m.Y, false, false, false, m.n, sn / (sb * sx), v[0] * sn / sx, &m.X});
+    if (int rc = products(ps, terms, di, st)) return rc;
+    for (Large& m : ms) std::swap(m.X, m.Y);
     sx = sn;
   }
-  b.x = X.p;
-  b.scale = (float)sx;
-  B200CP_CUDA_OK(launch_kernel(muon_apply_kernel<P>, dim3(rows8, count), dim3(256), 0, st, true, b));
+  t.scale = (float)sx;
+  int at = 0;
+  for (const Large& m : ms)
+    for (int i = 0; i < m.X.count; ++i) t.e[at++].x = m.X.p + i * m.X.matrix();
+  B200CP_CUDA_OK(launch_kernel(muon_apply_kernel<P, CAP>, dim3((unsigned)ctas8), dim3(256), 0, st, true, t));
   B200CP_LAUNCH_OK("muon_apply_kernel");
   return B200CP_OK;
 }
 
 template <typename P, typename G>
-int run(const Work& w, const Rates& r, const Plan& plan, int adjust, char* ws, cudaStream_t st) {
+int run(const Work& w, const Rates& r, const Plan& plan, int adjust, bool copies, char* ws, cudaStream_t st) {
   DeviceInfo di;
   if (int rc = device_info(&di)) return rc;
   if (int rc = run_small<P, G>(w, r, plan, adjust, ws, di, st)) return rc;
-  for (const Shape& s : w.large) {
-    const int most = batch_of(s), all = (int)s.at.size();
-    for (int first = 0; first < all; first += most)
-      if (int rc = run_large<P, G>(s, first, std::min(most, all - first), r, plan, adjust, ws, di, st)) return rc;
+  // fp32 grade where a result has it: not in a 16-bit parameter, nor in X itself as bfloat16 (whose rounding is eight times what one fp16 operand's is)
+  const bool coarse = !copies && (r.update ? sizeof(P) == 2 : std::is_same<P, __nv_bfloat16>::value);
+  const int terms = coarse ? 1 : 3;
+  for (const std::vector<Share>& round : rounds_of(w)) {
+    int items = 0;
+    for (const Share& s : round) items += s.count;
+    if (int rc = items <= kFewItems ? run_large<P, G, kFewItems>(round, r, plan, adjust, terms, ws, di, st) : run_large<P, G, kItems>(round, r, plan, adjust, terms, ws, di, st))
+      return rc;
   }
   return B200CP_OK;
 }
@@ -1214,8 +1475,10 @@ int muon(const char* who, const b200cp_muon_matrix* ms, int count, int ptype, in
   if (int rc = check_muon(who, ms, count, ptype, gtype)) return rc;
   Plan plan;
   if (int rc = plan_of(who, h, &plan)) return rc;
+  bool copies = false;
   for (int i = 0; i < count; ++i) {
     const b200cp_muon_matrix& a = ms[i];
+    copies = copies || a.master;
     if (a.stack && a.rows && a.cols && (!a.param || !a.grad || (update && !a.momentum))) return fail(B200CP_ERR_INVALID_ARG, "%s: null pointer in matrix %d", who, i);
     if (a.master && ptype == B200CP_FLOAT32) return fail(B200CP_ERR_INVALID_ARG, "%s: a float32 parameter has no float32 copy (matrix %d)", who, i);
   }
@@ -1232,7 +1495,7 @@ int muon(const char* who, const b200cp_muon_matrix* ms, int count, int ptype, in
   r.eps = h->eps;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-#define TYPES(P, G) return run<P, G>(w, r, plan, h->adjust, ws, st)
+#define TYPES(P, G) return run<P, G>(w, r, plan, h->adjust, copies, ws, st)
   if (ptype == B200CP_FLOAT32) TYPES(float, float);
   if (ptype == B200CP_BFLOAT16 && gtype == B200CP_BFLOAT16) TYPES(__nv_bfloat16, __nv_bfloat16);
   if (ptype == B200CP_FLOAT16 && gtype == B200CP_FLOAT16) TYPES(__half, __half);

@@ -2,7 +2,11 @@
 
 Bound, in the Frobenius norm.  A step's products carry operands of 22 bits or more and sums of fp32: what step k adds is at most 2**-21 of |X_k|.  A later step
 raises it by the slope of a s + b s^3 + c s^5, at most 4 where singular values are up to 1.21.  So X is off by at most 2**-21 sum_k 4**(steps - k) |X_k|, and by
-the half step of its type.  The update is one product and one sum in fp32 more (2**-23 of their sizes)."""
+the half step of its type.  The update is one product and one sum in fp32 more (2**-23 of their sizes).
+
+Where the result has 16 bits (bfloat16 X, 16-bit parameters without a copy), the products of matrices with sides above 64 take operands of 11 bits.  Their
+roundings stay in the row or column space of what is multiplied, where later steps do not raise them; they are independent, 2**-12 / 3**0.5 of an operand in
+the norm, five operands a step whose products are at most 2.8 times X: 2.8 (5 / 3)**0.5 2**-12 a step, and 8 * 2**-12 of |X| after five."""
 import math
 
 import pytest
@@ -42,8 +46,10 @@ def defined(X, coefficients=ABC, eps=1e-7, steps=5):
     return X, bound * 2.0 ** -21
 
 
-def check(got, want, bound):
+def check(got, want, bound, coarse=False):
     t = half(got.dtype)
+    if coarse:
+        bound = bound + 2.0 ** -9 * want.square().sum((-2, -1)).sqrt()
     off = (got.double() - want).square().sum((-2, -1)).sqrt()
     bound = bound + t * (want.square().sum((-2, -1)).sqrt() + bound) + least(got.dtype) * math.sqrt(want.shape[-1] * want.shape[-2])
     assert got.shape == want.shape and bool((off <= bound).all()), f"{float((off / bound).max()):.2f} of the bound"
@@ -60,7 +66,7 @@ def test_orthogonalise(shape, dtype):
     X = matrices(*shape, seed=sum(shape)).to(dtype)
     kept = X.clone()
     out = P.orthogonalise(X)
-    check(out, *defined(X))
+    check(out, *defined(X), coarse=dtype == torch.bfloat16 and min(shape[-2:]) > 64)
     assert torch.equal(X, kept) and torch.equal(out, P.orthogonalise(X))
     P.device_status()
 
@@ -73,16 +79,17 @@ def test_steps_and_coefficients(shape, steps, coefficients):
     check(P.orthogonalise(X, coefficients, steps=steps), *defined(X, coefficients, steps=steps))
 
 
-@pytest.mark.parametrize("shape", [(48, 90), (150, 260), (260, 150), (400, 400)], ids=str)
+@pytest.mark.parametrize("shape", [(48, 90), (150, 260), (260, 150), (400, 400), (130, 900)], ids=str)
 @pytest.mark.parametrize("rank", [1, 3])
-def test_few_directions(shape, rank):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_few_directions(shape, rank, dtype):
     """What rounding adds in the directions that a matrix has not is raised by every step, and has to stay small beside those that it has."""
     import paralleltnnlayers_b200 as P
     gen = torch.Generator(device="cuda").manual_seed(rank)
     U, V = (torch.linalg.qr(torch.randn(n, rank, generator=gen, device="cuda", dtype=torch.float64))[0] for n in shape)
-    X = ((U * torch.tensor([1.0, 0.5, 0.25], device="cuda")[:rank]) @ V.mT).float()
+    X = ((U * torch.tensor([1.0, 0.5, 0.25], device="cuda")[:rank]) @ V.mT).to(dtype)
     out = P.orthogonalise(X)
-    check(out, *defined(X))
+    check(out, *defined(X), coarse=dtype == torch.bfloat16 and min(shape) > 64)
     s = torch.linalg.svdvals(out.double())
     assert 0.6 < float(s[rank - 1]) and float(s[0]) < 1.3
 
@@ -135,10 +142,12 @@ def test_step(shapes, dtype, gtype, copies, nesterov, adjust):
     for step in range(2):
         g = [(0.01 * matrices(*s, seed=10 * step + k)).to(gtype) for k, s in enumerate(shapes)]
         want = [expected(a, b, c, 0.02, 0.9, nesterov, 0.1, adjust) for a, b, c in zip(w if copies else p, g, m)]
+        before = [t.clone() for t in p]
         P.muon_step(p, g, m, 0.02, 0.9, nesterov, 0.1, adjust=adjust, master=w if copies else None)
         for k, (v, mom, bound) in enumerate(want):
             assert bool(((m[k].double() - mom).abs() <= 2.0 ** -22 * (mom.abs() + g[k].double().abs())).all())
-            check(w[k] if copies else p[k], v, bound)
+            coarse = 2.0 ** -9 * (v - 0.998 * before[k].double()).square().sum((-2, -1)).sqrt()   # of the update
+            check(w[k] if copies else p[k], v, bound + (coarse if dtype != torch.float32 and not copies and min(v.shape[-2:]) > 64 else 0))
             if copies:
                 assert torch.equal(p[k], w[k].to(dtype))
     P.device_status()
