@@ -13,15 +13,17 @@
 //
 // n > 64: X, A and B = b A + c A^2 are products on the tcgen05 tensor cores.  What is rounded: a value is held as two fp16 numbers (hi + rest, 22 bits)
 // times a power of two that the bound on the singular values gives, so that none overflows and the sums of a product are of hi hi + hi lo + lo hi; its
-// sums are fp32, at most 128 terms in an accumulator (the tensor core cuts sums off: over 4096 terms it loses 3e-5, where fp32 rounding loses 3e-7) and the
-// rest in registers (4096 x 4096 against 64 bits: 5.5e-7 with 64 terms, 6.1e-7 with 128, 1.0e-6 with 256; 4.20, 4.14 and 3.99 ms).  One fp16 number would be three times as fast, but directions with small singular values are raised by 3.4445 a step: its 2^-12 comes
-// out as 7 % of a gradient of rank one.  a X is added in fp32 (as part of
-// the product, with a I in B, 4 % faster and two to three times as far off).
+// sums are fp32, at most 256 terms in an accumulator (the tensor core cuts sums off: over 4096 terms it loses 3e-5, where fp32 rounding loses 3e-7) and the
+// rest in registers (4096 x 4096 against 64 bits: 5.5e-7 with 64 terms, 6.3e-7 with 128, 1.1e-6 with 256, in 3.85 ms with 128 and 3.66 with 256; fp32 products by
+// a library: 3.6e-6 in 34 ms).  One fp16 number would be three times as fast, but directions with small singular values are raised by 3.4445 a step: its 2^-12 comes
+// out as 7 % of a gradient of rank one where X itself is held in it.  a X is added
+// in fp32 (as part of the product, with a I in B, 5 % faster and two to three times as far off).
 // A and B are symmetric: blocks below the diagonal are not computed, the others stored twice.  Either operand is taken in either order, so nothing is
 // transposed; where the rows are the longer side A = X^T X and X <- a X + X B.  Matrices of one shape share their launches.
 // Every wait is bounded: one that runs out sets a status word and the CTA leaves through its normal exit.
 #include <algorithm>
 #include <cmath>
+#include <exception>
 #include <vector>
 
 #include "common.cuh"
@@ -335,7 +337,7 @@ __device__ __forceinline__ void iterate(const SmallHead& t, const Coefficients& 
   __syncthreads();
   const double root = sqrt(trace_sum), inverse = 1.0 / (root > t.r.eps || root != root ? root : t.r.eps);
   for (int i = tid; i < NN; i += kIterateThreads) {
-    A[i] *= inverse * inverse;
+    A[i] = A[i] * inverse * inverse;   // (one after the other: the square of 1 / eps may be infinite, and A zero)
     if (t.steps == 0) Q[i] = i / LD == i % LD ? 1.0 : 0.0;
   }
   __syncthreads();
@@ -682,7 +684,7 @@ __global__ void __launch_bounds__(256) muon_apply_kernel(const __grid_constant__
 // 256 x BN; one thread issues, accumulators in turn.
 // TERMS 3 (results of fp32 grade): both planes of 64 k in a stage, products hi hi + hi lo + lo hi; an accumulator holds kGroupSteps stages and is then added to
 // totals in registers.  TERMS 1 (results of 16 bits): hi planes alone, 128 k in a stage, and an accumulator holds the whole sum.
-constexpr int kStep = 64, kBand = 16, kGroupSteps = 2;
+constexpr int kStep = 64, kBand = 16, kGroupSteps = 4;
 constexpr int kPatch = 32 * 64;   // bytes of a warp's block of 32 x 32 halves on its way in or out
 template <int BN, int TERMS>
 struct Tile {
@@ -1199,10 +1201,10 @@ void cut_small(const b200cp_muon_matrix& a, long long all, int sm_count, SmallEn
 size_t small_bytes(const SmallSizes& s) {
   return align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256) + align_up(s.floats * 4, 256);
 }
-// Small matrices of a launch: tensors from `at` on, up to a table's size and 2^20 CTAs.
+// Small matrices of a launch: tensors (of stacks, at most kMostStack matrices) from `at` on, up to a table's size, 2^20 CTAs and 256 MB of parts.
 int next_small(const std::vector<b200cp_muon_matrix>& ms, size_t at, long long all, int sm_count, SmallTable<kTableSmall>* t, SmallSizes* s) {
   int count = 0;
-  while (at + count < ms.size() && count < kTableSmall && s->ctas < (1 << 20)) {
+  while (at + count < ms.size() && count < kTableSmall && s->ctas < (1 << 20) && s->doubles < (size_t)1 << 25) {
     SmallEntry e{};
     cut_small(ms[at + count], all, sm_count, &e, s);
     const b200cp_muon_matrix& a = ms[at + count];
@@ -1219,6 +1221,7 @@ struct Shape {
   std::vector<Pointers> at;
 };
 size_t type_size(int type) { return type == B200CP_FLOAT32 ? 4 : 2; }
+constexpr int kMostStack = 4096;
 struct Work {
   std::vector<b200cp_muon_matrix> little;
   long long matrices = 0;   // small ones
@@ -1227,8 +1230,13 @@ struct Work {
     for (int i = 0; i < count; ++i) {
       const b200cp_muon_matrix& a = ms[i];
       if (a.stack < 1 || a.rows < 1 || a.cols < 1) continue;
+      const size_t n = (size_t)a.rows * a.cols;
+      const auto part = [&](int k, int stack) {   // of a stack, from matrix k on
+        const auto on = [&](auto* p, size_t size) { return p ? (decltype(p))((char*)p + k * n * size) : p; };
+        return b200cp_muon_matrix{on(a.param, type_size(ptype)), on(a.grad, type_size(gtype)), on(a.momentum, 4), on(a.master, 4), stack, a.rows, a.cols};
+      };
       if (small(a)) {
-        little.push_back(a);
+        for (int k = 0; k < a.stack; k += kMostStack) little.push_back(part(k, std::min(kMostStack, a.stack - k)));
         matrices += a.stack;
         continue;
       }
@@ -1237,10 +1245,9 @@ struct Work {
         large.push_back(Shape{a.rows, a.cols, {}});
         s = large.end() - 1;
       }
-      const size_t n = (size_t)a.rows * a.cols;
       for (int k = 0; k < a.stack; ++k) {
-        const auto on = [&](auto* p, size_t size) { return p ? (decltype(p))((char*)p + k * n * size) : p; };
-        s->at.push_back(Pointers{on(a.param, type_size(ptype)), on(a.grad, type_size(gtype)), on(a.momentum, 4), on(a.master, 4)});
+        const b200cp_muon_matrix q = part(k, 1);
+        s->at.push_back(Pointers{q.param, q.grad, q.momentum, q.master});
       }
     }
   }
@@ -1520,23 +1527,29 @@ using namespace b200cp;
 
 extern "C" {
 
-size_t b200cp_muon_step_workspace_bytes(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type) {
+// (A list of matrices takes host memory: what that throws does not leave the library.)
+size_t b200cp_muon_step_workspace_bytes(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type) try {
   if (check_muon("b200cp_muon_step_workspace_bytes", matrices, count, param_type, grad_type)) return 0;
   DeviceInfo di;
   if (device_info(&di)) return 0;
   return workspace_of(Work(matrices, count, param_type, grad_type), di.sm_count);
+} catch (const std::exception& e) {
+  fail(B200CP_ERR_UNSUPPORTED, "b200cp_muon_step_workspace_bytes: %s", e.what());
+  return 0;
 }
 
 int b200cp_muon_step(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type, const b200cp_muon* hyper, void* workspace,
-                     size_t workspace_bytes, void* stream) {
+                     size_t workspace_bytes, void* stream) try {
   const char* who = "b200cp_muon_step";
   if (hyper && (hyper->adjust < B200CP_MUON_PLAIN || hyper->adjust > B200CP_MUON_MATCH_RMS_ADAMW))
     return fail(B200CP_ERR_INVALID_ARG, "%s: adjust %d", who, hyper->adjust);
   return muon(who, matrices, count, param_type, grad_type, hyper, true, workspace, workspace_bytes, stream);
+} catch (const std::exception& e) {
+  return fail(B200CP_ERR_UNSUPPORTED, "b200cp_muon_step: %s", e.what());
 }
 
 int b200cp_orthogonalise(int stack, int rows, int cols, int type, const void* X, void* out, const double* coefficients, int coefficient_count, int steps,
-                         double eps, void* workspace, size_t workspace_bytes, void* stream) {
+                         double eps, void* workspace, size_t workspace_bytes, void* stream) try {
   const b200cp_muon_matrix m{out, X, nullptr, nullptr, stack, rows, cols};
   b200cp_muon h{};
   h.eps = eps;
@@ -1544,6 +1557,8 @@ int b200cp_orthogonalise(int stack, int rows, int cols, int type, const void* X,
   h.coefficients = coefficients;
   h.coefficient_count = coefficient_count;
   return muon("b200cp_orthogonalise", &m, 1, type, type, &h, false, workspace, workspace_bytes, stream);
+} catch (const std::exception& e) {
+  return fail(B200CP_ERR_UNSUPPORTED, "b200cp_orthogonalise: %s", e.what());
 }
 
 }  // extern "C"

@@ -207,6 +207,29 @@ def test_many_matrices():
     check(P.orthogonalise(Y), *defined(Y))
 
 
+def test_long_stacks():
+    """Stacks that are taken in several parts, small and large matrices of one call, and one matrix of a long side."""
+    import paralleltnnlayers_b200 as P
+    X = matrices(9001, 3, 5, seed=5)
+    check(P.orthogonalise(X), *defined(X))
+    p = [torch.zeros(4100, 2, 2, device="cuda"), torch.zeros(66, 200, device="cuda"), torch.zeros(17, 70001, device="cuda"), torch.zeros(50003, 40, device="cuda")]
+    g = [matrices(*t.shape, seed=k) for k, t in enumerate(p)]
+    P.muon_step(p, g, [torch.zeros_like(t) for t in p], 1.0, momentum=0.0, weight_decay=0.0, adjust=None)
+    for a, b in zip(p, g):
+        check(-a, *defined(b))
+
+
+def test_nothing_to_orthogonalise():
+    """A gradient of zeros moves nothing, however small eps is; the weight decays all the same."""
+    import paralleltnnlayers_b200 as P
+    for shape in ((5, 9), (40, 60), (100, 80)):
+        for eps in (1e-7, 1e-30, 1e-200):
+            p, z = torch.randn(*shape, device="cuda"), torch.zeros(*shape, device="cuda")
+            kept, m = p.clone(), z.clone()
+            P.muon_step([p], [z], [m], 0.5, weight_decay=0.5, eps=eps)
+            assert torch.equal(p, kept * 0.75) and not m.any()
+
+
 def test_streams_and_graphs():
     import paralleltnnlayers_b200 as P
     for shapes in ([(16, 40), (100, 120)], [(130, 66), (5, 9)]):
