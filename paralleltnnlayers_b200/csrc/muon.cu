@@ -259,16 +259,23 @@ constexpr int gram_doubles(int ts) {   // of shared memory: the values, or the s
   return ts == 1 ? std::max(Side<1>::sub * Side<1>::LD, 8 * Side<1>::part) : ts == 2 ? std::max(Side<2>::sub * Side<2>::LD, 4 * Side<2>::part)
                                                                                : std::max(Side<4>::sub * Side<4>::LD, 2 * Side<4>::part);
 }
-template <typename G, int CAP>
-__global__ void __launch_bounds__(256, 3) muon_gram_kernel(const __grid_constant__ SmallTable<CAP> t) {
+// W: what the widest matrix of the launch takes.  Sides of at most 16 alone (factors of adapters) leave registers for more CTAs an SM, and those are bound by what is
+// on its way: 32 matrices of 4096 x 16 and 32 of 16 x 4096, in bfloat16 with copies, 57 us with three of them.
+constexpr int per_sm(int w) { return w == 1 ? 5 : 3; }
+template <typename G, int W, int CAP>
+__global__ void __launch_bounds__(256, per_sm(W)) muon_gram_kernel(const __grid_constant__ SmallTable<CAP> t) {
   extern __shared__ __align__(16) double work[];
   grid_dependency_wait();
   const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.first; })];
   const int at = (int)blockIdx.x - e.first, matrix = at / e.chunks, chunk = at - matrix * e.chunks, n = side_of(e);
 #define B200CP_GRAM(TS) (e.vec ? gram_part<G, TS, 4>(t, e, matrix, chunk, work) : gram_part<G, TS, 1>(t, e, matrix, chunk, work))
-  if (n <= 16) B200CP_GRAM(1);
-  else if (n <= 32) B200CP_GRAM(2);
-  else B200CP_GRAM(4);
+  if constexpr (W == 1) {
+    B200CP_GRAM(1);
+  } else {
+    if (n <= 16) B200CP_GRAM(1);
+    else if (n <= 32) B200CP_GRAM(2);
+    else B200CP_GRAM(4);
+  }
 #undef B200CP_GRAM
 }
 
@@ -447,16 +454,20 @@ __device__ __forceinline__ void apply_part(const SmallHead& t, const SmallEntry&
     values.store(p, k0, old);
   }
 }
-template <typename P, typename G, int CAP>
-__global__ void __launch_bounds__(256, 3) muon_small_apply_kernel(const __grid_constant__ SmallTable<CAP> t) {
+template <typename P, typename G, int W, int CAP>
+__global__ void __launch_bounds__(256, per_sm(W)) muon_small_apply_kernel(const __grid_constant__ SmallTable<CAP> t) {
   extern __shared__ __align__(16) float low[];
   grid_dependency_wait();
   const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.first; })];
   const int at = (int)blockIdx.x - e.first, matrix = at / e.chunks, chunk = at - matrix * e.chunks, n = side_of(e);
 #define B200CP_APPLY(TS) (e.vec ? apply_part<P, G, TS, 4>(t, e, matrix, chunk, low) : apply_part<P, G, TS, 1>(t, e, matrix, chunk, low))
-  if (n <= 16) B200CP_APPLY(1);
-  else if (n <= 32) B200CP_APPLY(2);
-  else B200CP_APPLY(4);
+  if constexpr (W == 1) {
+    B200CP_APPLY(1);
+  } else {
+    if (n <= 16) B200CP_APPLY(1);
+    else if (n <= 32) B200CP_APPLY(2);
+    else B200CP_APPLY(4);
+  }
 #undef B200CP_APPLY
 }
 
@@ -1182,10 +1193,10 @@ struct SmallSizes {
   size_t doubles = 0, floats = 0;
   int matrices = 0, ctas = 0;
 };
-// Parts of a matrix: as long as gives every SM the three CTAs that it holds over all of the call's matrices: one round of them, and few parts to be added.
-void cut_small(const b200cp_muon_matrix& a, long long all, int sm_count, SmallEntry* e, SmallSizes* s) {
+// Parts of a matrix: as long as gives every SM the CTAs that it holds (per_sm) over all of the call's matrices: one round of them, and few parts to be added.
+void cut_small(const b200cp_muon_matrix& a, long long all, int slots, SmallEntry* e, SmallSizes* s) {
   const int n = std::min(a.rows, a.cols), len = std::max(a.rows, a.cols), subs = ceil_div(len, kSub), ts = tile_side(n);
-  const int parts = (int)std::min<long long>(subs, std::max<long long>(1, 3LL * sm_count / std::max<long long>(1, all)));
+  const int parts = (int)std::min<long long>(subs, std::max<long long>(1, slots / std::max<long long>(1, all)));
   e->rows = a.rows; e->cols = a.cols; e->stack = a.stack;
   e->length = ceil_div(subs, parts) * kSub;
   e->chunks = ceil_div(len, e->length);
@@ -1202,11 +1213,11 @@ size_t small_bytes(const SmallSizes& s) {
   return align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256) + align_up(s.floats * 4, 256);
 }
 // Small matrices of a launch: tensors (of stacks, at most kMostStack matrices) from `at` on, up to a table's size, 2^20 CTAs and 256 MB of parts.
-int next_small(const std::vector<b200cp_muon_matrix>& ms, size_t at, long long all, int sm_count, SmallTable<kTableSmall>* t, SmallSizes* s) {
+int next_small(const std::vector<b200cp_muon_matrix>& ms, size_t at, long long all, int slots, SmallTable<kTableSmall>* t, SmallSizes* s) {
   int count = 0;
   while (at + count < ms.size() && count < kTableSmall && s->ctas < (1 << 20) && s->doubles < (size_t)1 << 25) {
     SmallEntry e{};
-    cut_small(ms[at + count], all, sm_count, &e, s);
+    cut_small(ms[at + count], all, slots, &e, s);
     const b200cp_muon_matrix& a = ms[at + count];
     e.at = Pointers{a.param, a.grad, a.momentum, a.master};
     const auto off = [](const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; };
@@ -1225,6 +1236,7 @@ constexpr int kMostStack = 4096;
 struct Work {
   std::vector<b200cp_muon_matrix> little;
   long long matrices = 0;   // small ones
+  int widest = 1;           // 1: all of them have a side of at most 16; or 4
   std::vector<Shape> large;
   Work(const b200cp_muon_matrix* ms, int count, int ptype, int gtype) {
     for (int i = 0; i < count; ++i) {
@@ -1238,6 +1250,7 @@ struct Work {
       if (small(a)) {
         for (int k = 0; k < a.stack; k += kMostStack) little.push_back(part(k, std::min(kMostStack, a.stack - k)));
         matrices += a.stack;
+        if (tile_side(std::min(a.rows, a.cols)) > 1) widest = 4;
         continue;
       }
       auto s = std::find_if(large.begin(), large.end(), [&](const Shape& q) { return q.rows == a.rows && q.cols == a.cols; });
@@ -1301,7 +1314,7 @@ size_t workspace_of(const Work& w, int sm_count) {
   size_t most = 0;
   for (size_t at = 0; at < w.little.size();) {
     SmallSizes s;
-    at += next_small(w.little, at, w.matrices, sm_count, nullptr, &s);
+    at += next_small(w.little, at, w.matrices, per_sm(w.widest) * sm_count, nullptr, &s);
     most = std::max(most, small_bytes(s));
   }
   for (const std::vector<Share>& r : rounds_of(w)) most = std::max(most, round_bytes(r));
@@ -1313,7 +1326,7 @@ float factor_of(int adjust, int rows, int cols) {
   return 1.f;
 }
 
-template <typename P, typename G, int CAP>
+template <typename P, typename G, int W, int CAP>
 int launch_small(const SmallHead& head, const SmallEntry* e, const Coefficients& co, const SmallSizes& s, cudaStream_t st) {
   SmallTable<CAP> t;
   static_cast<SmallHead&>(t) = head;
@@ -1323,14 +1336,14 @@ int launch_small(const SmallHead& head, const SmallEntry* e, const Coefficients&
   // (each as much as the widest matrix of the launch needs; the others need less)
   const int gram = std::max({gram_doubles(1), ts > 1 ? gram_doubles(2) : 0, ts > 2 ? gram_doubles(4) : 0}) * 8, four = 4 * 16 * ts * (16 * ts + 4) * 8,
             low = std::max({small_apply_floats(1), ts > 1 ? small_apply_floats(2) : 0, ts > 2 ? small_apply_floats(4) : 0}) * 4;
-  B200CP_CUDA_OK((allow_smem<muon_gram_kernel<G, CAP>>(gram)));
-  B200CP_CUDA_OK(launch_kernel(muon_gram_kernel<G, CAP>, dim3(s.ctas), dim3(256), gram, st, true, t));
+  B200CP_CUDA_OK((allow_smem<muon_gram_kernel<G, W, CAP>>(gram)));
+  B200CP_CUDA_OK(launch_kernel(muon_gram_kernel<G, W, CAP>, dim3(s.ctas), dim3(256), gram, st, true, t));
   B200CP_LAUNCH_OK("muon_gram_kernel");
   B200CP_CUDA_OK(allow_smem<muon_iterate_kernel<CAP>>(four));
   B200CP_CUDA_OK(launch_kernel(muon_iterate_kernel<CAP>, dim3(s.matrices), dim3(kIterateThreads), four, st, true, t, co));
   B200CP_LAUNCH_OK("muon_iterate_kernel");
-  B200CP_CUDA_OK((allow_smem<muon_small_apply_kernel<P, G, CAP>>(low)));
-  B200CP_CUDA_OK(launch_kernel(muon_small_apply_kernel<P, G, CAP>, dim3(s.ctas), dim3(256), low, st, true, t));
+  B200CP_CUDA_OK((allow_smem<muon_small_apply_kernel<P, G, W, CAP>>(low)));
+  B200CP_CUDA_OK(launch_kernel(muon_small_apply_kernel<P, G, W, CAP>, dim3(s.ctas), dim3(256), low, st, true, t));
   B200CP_LAUNCH_OK("muon_small_apply_kernel");
   return B200CP_OK;
 }
@@ -1341,7 +1354,7 @@ int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char*
   SmallTable<kTableSmall> t;
   for (size_t at = 0; at < w.little.size();) {
     SmallSizes s;
-    t.count = next_small(w.little, at, w.matrices, di.sm_count, &t, &s);
+    t.count = next_small(w.little, at, w.matrices, per_sm(w.widest) * di.sm_count, &t, &s);
     at += t.count;
     t.r = r;
     t.steps = plan.steps;
@@ -1350,7 +1363,10 @@ int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char*
     t.inverse = reinterpret_cast<double*>(ws + align_up(s.doubles * 8, 256));
     t.q = reinterpret_cast<float*>(ws + align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256));
     for (int i = 0; i < t.count; ++i) t.e[i].scale = factor_of(adjust, t.e[i].rows, t.e[i].cols);
-    if (int rc = t.count <= kFewSmall ? launch_small<P, G, kFewSmall>(t, t.e, co, s, st) : launch_small<P, G, kTableSmall>(t, t.e, co, s, st)) return rc;
+    const bool few = t.count <= kFewSmall;
+    const int rc = w.widest == 1 ? (few ? launch_small<P, G, 1, kFewSmall>(t, t.e, co, s, st) : launch_small<P, G, 1, kTableSmall>(t, t.e, co, s, st))
+                                 : (few ? launch_small<P, G, 4, kFewSmall>(t, t.e, co, s, st) : launch_small<P, G, 4, kTableSmall>(t, t.e, co, s, st));
+    if (rc) return rc;
   }
   return B200CP_OK;
 }

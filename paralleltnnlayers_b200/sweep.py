@@ -1,6 +1,6 @@
 """Kernel timings of every layer family at the sizes of the benchmark configurations.
 
-    python -m paralleltnnlayers_b200.sweep [cp4] [rcp] [dense] [adapters] [gated] [adamw] [--reps 12] [--json]
+    python -m paralleltnnlayers_b200.sweep [cp4] [rcp] [dense] [adapters] [gated] [adamw] [embedding] [norm] [muon] [--reps 12] [--json]
     python -m paralleltnnlayers_b200.sweep --shapes FILE [--ranks 1,2,4,8,16] [--reps 47] [--out results.csv] [--mem]
 
 The second form reads a shape list in the reference's format (``N C H W pad T Y X`` per line, ``#`` comments;
@@ -134,6 +134,9 @@ def sweep_dense(P, reps, rows):
 
 ADAPTERS = [(64, 32, 16), (4096, 8, 16), (4096, 8, 64)]   # rows, adapters, rank; 4096 -> 4096
 GATED = [1, 64, 4096]                                     # rows; 4096 -> 10240
+EMBEDDING = [(64, 50000), (8192, 50000)]                  # tokens, rows of the table; 4096 features
+NORM = [(64, 4096), (8192, 1024), (8192, 4096)]           # rows, features
+MUON = [(64, 64, 16), (1, 1024, 1024), (1, 4096, 4096), (1, 4096, 10240)]   # matrices, rows, columns
 
 
 def sweep_adapters(P, reps, rows):
@@ -184,6 +187,47 @@ def sweep_adamw(P, reps, rows):
             rows.append({"layer": "adamw", "tensors": name, "values": sum(sizes), "bits": bits,
                          "step": timeit(lambda i: P.adamw_step(p, g, m, v, 10, 1e-3, scales=scales), reps),
                          "hbm_floor_us": sum(sizes) * (28 if bits == 32 else 16.0625) / 6.45e12 * 1e6})
+
+
+def sweep_embedding(P, reps, rows):
+    for S, V in EMBEDDING:
+        W = torch.randn(V, 4096, device="cuda").bfloat16()
+        k = 2 if S > 1024 else 8
+        t = [torch.randint(V, (S,), device="cuda") for _ in range(k)]
+        dy = [torch.randn(S, 4096, device="cuda").bfloat16() for _ in range(k)]
+        rows.append({"layer": "embedding", "tokens": S, "count": V, "fwd": timeit(lambda i: P.embedding(t[i % k], W, 8.0), reps),
+                     "bwd": timeit(lambda i: P.embedding_backward(dy[i % k], t[i % k], V, 8.0), reps),
+                     "hbm_floor_us": 2 * 4096 * 2 * S / 6.45e12 * 1e6, "hbm_floor_bwd_us": 2 * 4096 * (S + V) / 6.45e12 * 1e6})
+        del W, dy
+        torch.cuda.empty_cache()
+
+
+def sweep_norm(P, reps, rows):
+    for S, D in NORM:
+        k = 2 if S * D > 1 << 24 else 16
+        mk = lambda: [torch.randn(S, D, device="cuda").bfloat16() for _ in range(k)]  # noqa: E731,B023
+        x, r, dy, dh = mk(), mk(), mk(), mk()
+        w, b = torch.ones(D, device="cuda").bfloat16(), torch.zeros(D, device="cuda").bfloat16()
+        _, h, mean, rstd = P.layer_norm_save(x[0], w, b, 1e-5, r[0])
+        rows.append({"layer": "norm", "rows": S, "features": D, "fwd": timeit(lambda i: P.layer_norm(x[i % k], w, b), reps),
+                     "fwd_residual": timeit(lambda i: P.layer_norm(x[i % k], w, b, 1e-5, r[i % k]), reps),
+                     "bwd": timeit(lambda i: P.layer_norm_backward(dy[i % k], x[i % k], w, b, mean, rstd, dh[i % k]), reps),
+                     "hbm_floor_us": 2 * S * D * 2 / 6.45e12 * 1e6, "hbm_floor_bwd_us": 2 * S * D * 4 / 6.45e12 * 1e6})
+        del x, r, dy, dh, h
+        torch.cuda.empty_cache()
+
+
+def sweep_muon(P, reps, rows):
+    for n, r, c in MUON:
+        for dtype in (torch.float32, torch.bfloat16):
+            x = torch.randn(n, r, c, device="cuda").to(dtype)
+            a, b = min(r, c), max(r, c)
+            flops = 5 * n * (a * a * (a + b) + 2 * a * a * b) * (3 if dtype == torch.float32 else 1)   # of fp16 products: three for a result in fp32
+            rows.append({"layer": "muon", "matrices": n, "rows": r, "columns": c, "dtype": str(dtype)[6:],
+                         "orthogonalise": timeit(lambda i: P.orthogonalise(x), max(2, reps // 3)), "tc_floor_us": flops / 1.38e15 * 1e6})
+            del x
+            torch.cuda.empty_cache()
+    P.device_status()
 
 
 def read_shapes(path):
@@ -245,12 +289,13 @@ def bench_shapes(P, path, ranks, reps, out):
         sys.stdout.write(text)
 
 
-SWEEPS = {"cp4": sweep_cp4, "rcp": sweep_rcp, "dense": sweep_dense, "adapters": sweep_adapters, "gated": sweep_gated, "adamw": sweep_adamw}
+SWEEPS = {"cp4": sweep_cp4, "rcp": sweep_rcp, "dense": sweep_dense, "adapters": sweep_adapters, "gated": sweep_gated, "adamw": sweep_adamw,
+          "embedding": sweep_embedding, "norm": sweep_norm, "muon": sweep_muon}
 
 
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
-    ap.add_argument("which", nargs="*", help="any of cp4, rcp, dense (default: these three), adapters, gated, adamw")
+    ap.add_argument("which", nargs="*", help="any of cp4, rcp, dense (default: these three), adapters, gated, adamw, embedding, norm, muon")
     ap.add_argument("--reps", type=int, default=12)
     ap.add_argument("--json", action="store_true", help="one JSON object per line instead of text")
     ap.add_argument("--shapes", help="shape list in the reference's format: time the CP4 forward per shape and rank")
