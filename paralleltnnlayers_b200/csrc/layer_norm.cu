@@ -58,16 +58,6 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float* red, int turn
   return block_sum(a, b, red, turn);
 }
 
-// Rows to come, on their way into `slots` places of shared memory.
-struct Ring {
-  int slots, row;    // places; bytes of a row
-};
-__device__ __forceinline__ void bulk_load(void* to, const void* from, int bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(to)), "l"(from), "r"(bytes),
-               "r"(tc::smem_u32(bar))
-               : "memory");
-}
-constexpr int kMostSlots = 8;
 struct Forward {
   int rows, D;
   float eps;
@@ -158,105 +148,6 @@ __global__ void __launch_bounds__(WARP ? 32 * kRows : 1024) norm_kernel(const __
 #pragma unroll
     for (int i = 0; i < VEC; ++i) a[i] = fmaf(fmaf(v[k][i], rstd, -off * rstd), m[i], a[i]);
     store_group(y + c, pack<T>(a));
-  }
-}
-
-// Many rows of whole 16-byte groups: CTAs that stay, the rows to come on their way meanwhile (8192 x 4096 in bfloat16: 34.5 us with a CTA per row, of which an SM
-// holds six).
-template <typename T, typename W, int VEC, int K>
-__global__ void __launch_bounds__(kGradThreads, 2) norm_ring_kernel(const __grid_constant__ Forward g, const __grid_constant__ Ring ring) {
-  extern __shared__ __align__(16) uint8_t places[];   // [slot][x, r][row]
-  __shared__ float red[kRed];
-  __shared__ uint64_t full[kMostSlots];
-  __shared__ volatile int given_up[2];   // used in turn, so that all threads see the same after a barrier
-  const int t = threadIdx.x, n = blockDim.x, step = gridDim.x, arrays = g.r ? 2 : 1;
-  if (t == 0) {
-    for (int i = 0; i < ring.slots; ++i) tc::mbar_init(&full[i], 1);
-    given_up[0] = given_up[1] = 0;
-    tc::fence_barrier_init();
-  }
-  __syncthreads();
-  grid_dependency_wait();
-  const auto fetch = [&](int row, int slot) {
-    uint8_t* to = places + (size_t)slot * arrays * ring.row;
-    tc::mbar_expect_tx(&full[slot], arrays * ring.row);
-    bulk_load(to, static_cast<const T*>(g.x) + (size_t)row * g.D, ring.row, &full[slot]);
-    if (g.r) bulk_load(to + ring.row, static_cast<const T*>(g.r) + (size_t)row * g.D, ring.row, &full[slot]);
-  };
-  if (t == 0)
-    for (int i = 0; i < ring.slots && (long long)blockIdx.x + (long long)i * step < g.rows; ++i) fetch(blockIdx.x + i * step, i);
-  const float inv = 1.f / (float)g.D;
-  const W *w = static_cast<const W*>(g.w), *b = static_cast<const W*>(g.b);
-  int slot = 0, phase = 0, turn = 0;
-  for (int row = blockIdx.x; row < g.rows; row += step, turn ^= 1) {
-    if (!tc::mbar_wait(&full[slot], phase)) given_up[turn] = 1;
-    const T* place = reinterpret_cast<const T*>(places + (size_t)slot * arrays * ring.row);
-    const size_t at = (size_t)row * g.D;
-    float v[K][VEC], s = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * n + t) * VEC;
-      if (c >= g.D) continue;
-      unpack(load_group<T, VEC>(place + c), v[k]);
-      if (g.r) {
-        float a[VEC];
-        unpack(load_group<T, VEC>(place + g.D + c), a);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) a[i] += v[k][i];
-        const Group<T, VEC> p = pack<T>(a);
-        store_group(static_cast<T*>(g.h) + at + c, p);
-        unpack(p, v[k]);
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) s += v[k][i];
-    }
-    const float mean = block_sum(s, 0.f, red, 0).x * inv;
-    if (given_up[turn]) break;
-    // (all threads have taken what they need of the place)
-    if (t == 0 && (long long)row + (long long)ring.slots * step < g.rows) fetch(row + ring.slots * step, slot);
-    if (++slot == ring.slots) {
-      slot = 0;
-      phase ^= 1;
-    }
-    float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if ((k * n + t) * VEC >= g.D) continue;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        v[k][i] -= mean;
-        s1 += v[k][i];
-        s2 = fmaf(v[k][i], v[k][i], s2);
-      }
-    }
-    const float2 q = block_sum(s1, s2, red, 1);
-    const float off = q.x * inv, rstd = 1.f / sqrtf(fmaxf(fmaf(-off, off, q.y * inv), 0.f) + g.eps);
-    if (g.mean && t == 0) {
-      g.mean[row] = mean + off;
-      g.rstd[row] = rstd;
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * n + t) * VEC;
-      if (c >= g.D) continue;
-      float m[VEC], a[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        m[i] = 1.f;
-        a[i] = 0.f;
-      }
-      if (w) unpack(load_group<W, VEC>(w + c), m);
-      if (b) unpack(load_group<W, VEC>(b + c), a);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) a[i] = fmaf(fmaf(v[k][i], rstd, -off * rstd), m[i], a[i]);
-      store_group(static_cast<T*>(g.y) + at + c, pack<T>(a));
-    }
-  }
-  if (given_up[0] | given_up[1]) {   // copies in flight land before the shared memory is given back
-    if (t == 0) atomicCAS(&g_layer_norm_status, 0, (2 << 16) | (blockIdx.x & 0xffff));
-    const long long t0 = clock64();
-    while (clock64() - t0 < 40000000ll) {
-    }
   }
 }
 
@@ -455,7 +346,16 @@ __global__ void __launch_bounds__(WARP ? 32 * kRows : kGradThreads, 1) norm_grad
   }
 }
 
-// The same for rows of whole 16-byte groups that a CTA shares: the rows to come are on their way into the ring.
+// The same for rows of whole 16-byte groups that a CTA shares: the rows to come are on their way into `slots` places of shared memory.
+struct Ring {
+  int slots, row;    // places; bytes of a row
+};
+__device__ __forceinline__ void bulk_load(void* to, const void* from, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(to)), "l"(from), "r"(bytes),
+               "r"(tc::smem_u32(bar))
+               : "memory");
+}
+constexpr int kMostSlots = 8;
 template <typename T, typename W, int VEC, int K>
 __global__ void __launch_bounds__(kGradThreads, 1) norm_grads_ring_kernel(const __grid_constant__ Backward g, const __grid_constant__ Ring ring) {
   extern __shared__ __align__(16) uint8_t places[];   // [slot][h, dy, dh][row]
@@ -658,30 +558,21 @@ int forward_of(const Forward& g, cudaStream_t st) {
   B200CP_LAUNCH_OK("norm_kernel");
   return B200CP_OK;
 }
+// Features of a thread.  Few rows (less than four an SM): 8, the shortest way through a row (64 x 4096 2.4 us, with 32 3.0).  Many rows: 32 of 16-bit types, which halves and
+// quarters what a row costs beside its values (8192 x 4096 in bfloat16 28.0 us, with 16 34.5, with 8 39.6; with the residual 43.2, 44.2, 47.9; HBM 20.6 and 41.3), 8 in
+// rows up to 512 (6.5 us, 7.1).  float32 is bound by HBM sooner: 8 up to 2048, then 32, with the residual 16 (4096: 45.5 of 48.2, 81.9 of 95).
 template <typename T, typename W, int VEC>
 int forward_by_size(const Forward& g, cudaStream_t st) {
-  if constexpr (VEC > 1) {
-    if (g.D > kWarpRow && g.D <= kGradRow) {
-      DeviceInfo di;
-      if (int rc = device_info(&di)) return rc;
-      // 16 features a thread, 1024 threads an SM; at least two places to each CTA
-      const int threads = threads_of(g.D, kGradEach), row = g.D * (int)sizeof(T), slot = (g.r ? 2 : 1) * row, room = 216 * 1024;
-      const int each = std::max(1, std::min(2 * kGradThreads / threads, room / (2 * slot + 2048)));
-      const Ring ring{std::max(2, std::min(kMostSlots, (room / each - 2048) / slot)), row};
-      if (g.rows >= 2 * each * di.sm_count) {   // (two rows to a CTA at least)
-        const auto kern = norm_ring_kernel<T, W, VEC, kGradEach / VEC>;
-        static std::atomic<int> set[64];
-        B200CP_CUDA_OK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), set, ring.slots * slot));
-        B200CP_CUDA_OK(launch_kernel(kern, dim3(each * di.sm_count), dim3(threads), (size_t)ring.slots * slot, st, true, g, ring));
-        B200CP_LAUNCH_OK("norm_ring_kernel");
-        return B200CP_OK;
-      }
-    }
-  }
-  if (g.D <= 2048) return forward_of<T, W, VEC, 8 / VEC>(g, st);
-  if (g.D <= 8192) return forward_of<T, W, VEC, 16 / VEC>(g, st);
-  if (g.D <= 32768 && VEC > 1) return forward_of<T, W, VEC, 32 / VEC>(g, st);
-  if (g.D <= 16384) return forward_of<T, W, VEC, 16 / VEC>(g, st);
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  const bool half = sizeof(T) == 2;
+  int each = g.rows < 4 * di.sm_count || g.D <= (half ? 512 : 2048) ? 8 : half || !g.r ? 32 : 16;
+  if (VEC == 1) each = g.D <= 2048 ? 8 : 16;   // (odd rows)
+  if (g.D > 1024 * each) each = g.D <= 16384 ? 16 : 32;
+  if (each == 8) return forward_of<T, W, VEC, 8 / VEC>(g, st);
+  if (each == 16 && g.D <= 16384) return forward_of<T, W, VEC, 16 / VEC>(g, st);
+  if constexpr (VEC > 1)
+    if (g.D <= 32768) return forward_of<T, W, VEC, 32 / VEC>(g, st);
   B200CP_CUDA_OK(launch_kernel(norm_wide_kernel<T, W, VEC>, dim3(g.rows), dim3(1024), 0, st, true, g));
   B200CP_LAUNCH_OK("norm_wide_kernel");
   return B200CP_OK;
