@@ -65,14 +65,14 @@ __device__ __forceinline__ double warp_sum(double x) {
 }
 
 // ======== matrices with a side of at most 64 =====================================================================================
-constexpr int kSmall = 64, kSub = 128;
+constexpr int kSmall = 64;
 // Tensors of a launch: a table's bytes are written for each launch, so there are two sizes of it.
 constexpr int kFewSmall = 24, kTableSmall = 224;
 struct SmallEntry {
   Pointers at;
   int rows, cols;
   int stack;
-  int chunks, length;        // of a matrix: parts of its longer side, and how much of it each has (a multiple of kSub)
+  int chunks, length;        // of a matrix: parts of its longer side, and how much of it each has (a multiple of Side::sub)
   int first;                 // CTA of the launch over parts
   int matrix;                // matrices before
   int vec;                   // four values of every array lie on its boundary, and rows are multiples of four
@@ -1195,10 +1195,10 @@ struct SmallSizes {
 };
 // Parts of a matrix: as long as gives every SM the CTAs that it holds (per_sm) over all of the call's matrices: one round of them, and few parts to be added.
 void cut_small(const b200cp_muon_matrix& a, long long all, int slots, SmallEntry* e, SmallSizes* s) {
-  const int n = std::min(a.rows, a.cols), len = std::max(a.rows, a.cols), subs = ceil_div(len, kSub), ts = tile_side(n);
+  const int n = std::min(a.rows, a.cols), len = std::max(a.rows, a.cols), ts = tile_side(n), sub = 2048 / (16 * ts), subs = ceil_div(len, sub);
   const int parts = (int)std::min<long long>(subs, std::max<long long>(1, slots / std::max<long long>(1, all)));
   e->rows = a.rows; e->cols = a.cols; e->stack = a.stack;
-  e->length = ceil_div(subs, parts) * kSub;
+  e->length = ceil_div(subs, parts) * sub;
   e->chunks = ceil_div(len, e->length);
   e->first = s->ctas;
   e->matrix = s->matrices;
