@@ -12,14 +12,15 @@
 // launches for all such matrices of a call together.
 //
 // n > 64: X, A and B = b A + c A^2 are products on the tcgen05 tensor cores.  What is rounded: a value is held as two fp16 numbers (hi + rest, 22 bits)
-// times a power of two that the bound on the singular values gives, so that none overflows and the sums of a product are of hi hi + hi lo + lo hi; its
-// sums are fp32, at most 256 terms in an accumulator (the tensor core cuts sums off: over 4096 terms it loses 3e-5, where fp32 rounding loses 3e-7) and the
-// rest in registers (4096 x 4096 against 64 bits: 5.5e-7 with 64 terms, 6.3e-7 with 128, 1.1e-6 with 256, in 3.85 ms with 128 and 3.66 with 256; fp32 products by
-// a library: 3.6e-6 in 34 ms).  One fp16 number would be three times as fast, but directions with small singular values are raised by 3.4445 a step: its 2^-12 comes
-// out as 7 % of a gradient of rank one where X itself is held in it.  a X is added
-// in fp32 (as part of the product, with a I in B, 5 % faster and two to three times as far off).
+// times a power of two that the bound on the singular values gives, so that none overflows, and a product is hi hi + hi lo + lo hi; its sums are fp32, at
+// most 256 terms in an accumulator (the tensor core cuts sums off: over 4096 terms it loses 3e-5, where fp32 rounding loses 3e-7) and the rest in registers
+// (4096 x 4096 against 64 bits: 5.5e-7 with 64 terms, 6.3e-7 with 128, 1.1e-6 with 256, in 3.85 ms with 128 and 3.66 with 256; fp32 products of a library: 3.6e-6
+// in 34 ms).  a X is added in fp32 (as part of the product, with a I in B, 5 % faster and two to three times as far off).
+// Where the result has 16 bits (bfloat16 X, 16-bit parameters without a copy) operands are the hi parts alone, a third of the work: 4096 x 10240 in bfloat16 3.1 ms, in
+// float32 6.8.  X keeps both parts: directions with small singular values are raised by 3.4445 a step, and what one part lacks of X would come out as 7 % of a gradient of
+// rank one; what it lacks as an operand stays in the row or column space of what it is multiplied with.
 // A and B are symmetric: blocks below the diagonal are not computed, the others stored twice.  Either operand is taken in either order, so nothing is
-// transposed; where the rows are the longer side A = X^T X and X <- a X + X B.  Matrices of one shape share their launches.
+// transposed; where the rows are the longer side A = X^T X and X <- a X + X B.  Matrices of all shapes share their launches.
 // Every wait is bounded: one that runs out sets a status word and the CTA leaves through its normal exit.
 #include <algorithm>
 #include <cmath>
@@ -55,7 +56,6 @@ template <typename G>
 __device__ __forceinline__ float momentum_of(const Rates& r, float g, float m) { return fmaf(r.blend, g - m, m); }
 __device__ __forceinline__ float direction_of(const Rates& r, float g, float m) { return r.nesterov ? fmaf(r.keep, m - g, g) : m; }
 __device__ __forceinline__ float rate_of(const Rates& r) { return r.device_lr ? *r.device_lr : r.lr; }
-// (what X stands for is far fewer bits than an fp32 value: the sum is rounded once)
 __device__ __forceinline__ float updated(float w, float x, float shrink, float rate) { return fmaf(-rate, x, w * shrink); }
 
 __device__ __forceinline__ double warp_sum(double x) {

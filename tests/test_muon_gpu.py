@@ -207,6 +207,19 @@ def test_many_matrices():
     check(P.orthogonalise(Y), *defined(Y))
 
 
+def test_many_shapes():
+    """More shapes than a launch's table has, and more large matrices than go together."""
+    import paralleltnnlayers_b200 as P
+    shapes = [(65 + k, 70 + 3 * (k % 7)) if k % 2 else (90, 65 + k) for k in range(60)]
+    p, g = [torch.zeros(*s, device="cuda") for s in shapes], [matrices(*s, seed=k) for k, s in enumerate(shapes)]
+    P.muon_step(p, g, [torch.zeros_like(t) for t in p], 1.0, momentum=0.0, weight_decay=0.0, adjust=None)
+    for a, b in zip(p, g):
+        check(-a, *defined(b))
+    X = matrices(300, 66, 68, seed=9)
+    check(P.orthogonalise(X), *defined(X))
+    P.device_status()
+
+
 def test_long_stacks():
     """Stacks that are taken in several parts, small and large matrices of one call, and one matrix of a long side."""
     import paralleltnnlayers_b200 as P

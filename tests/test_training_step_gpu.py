@@ -1,4 +1,8 @@
 """The embedding, layer norm and the Muon step as they are used together: a small language model trained, served, and stepped by a captured graph."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -188,3 +192,44 @@ def test_a_data_parallel_step_takes_the_optimiser():
     dist.dense_data_parallel_step(X, dY, F, allreduce=lambda t: t, optimizer=Muon(F, lr=0.05))
     for f, w in zip(F, want):
         assert torch.equal(f.detach(), w)
+
+
+SCRIPT = """
+import torch, paralleltnnlayers_b200 as P
+gen = torch.Generator(device="cuda").manual_seed(0)
+n = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+t, W, x, r, w = torch.randint(50, (400,), generator=gen, device="cuda"), n(50, 64), n(3000, 512), n(3000, 512), n(512)
+out = [P.embedding(t, W, 2.0), P.embedding_backward(n(400, 64), t, 50)]
+y, h, mean, rstd = P.layer_norm_save(x, w, None, 1e-5, r)
+out += [y, h, *P.layer_norm_backward(r, h, w, None, mean, rstd, x)]
+out += [P.orthogonalise(n(3, 20, 40)), P.orthogonalise(n(150, 300))]
+P.device_status()
+print("sums", *[repr(float(o.double().abs().sum())) for o in out])
+"""
+
+
+def test_plain_launches_give_the_same():
+    """B200CP_PDL=0: every launch waits for the one before it to end."""
+    root, lines = os.path.dirname(os.path.dirname(os.path.abspath(__file__))), []
+    for value in ("0", "1"):
+        run = subprocess.run([sys.executable, "-c", SCRIPT], cwd=root, env={**os.environ, "B200CP_PDL": value}, capture_output=True, text=True, timeout=120)
+        assert run.returncode == 0, run.stderr[-2000:]
+        lines.append(run.stdout.split("sums")[1])
+    assert lines[0] == lines[1]
+
+
+def test_a_trained_model_uses_every_type():
+    """A step of each type of parameter: the layers in bfloat16 and float16 under norms of float32, and all of it in float32."""
+    from paralleltnnlayers_b200 import layers as L
+    from paralleltnnlayers_b200.optim import Muon
+    for dtype in (torch.float32, BF16, torch.float16):
+        torch.manual_seed(1)
+        embed, norm, dense = L.Embedding(30, 48, dtype=dtype).cuda(), L.LayerNorm(48).cuda(), torch.nn.Linear(48, 80, bias=False).cuda().to(dtype)
+        opt = Muon(dense.parameters(), lr=0.01, master=dtype != torch.float32)
+        kept = dense.weight.detach().clone()
+        tokens = torch.randint(30, (64,), device="cuda")
+        dense(norm(embed(tokens))).float().square().mean().backward()
+        assert embed.W.grad.dtype == dtype and norm.weight.grad.dtype == torch.float32
+        opt.step()
+        step = (dense.weight.detach() - kept).float()
+        assert step.isfinite().all() and bool(step.any())
