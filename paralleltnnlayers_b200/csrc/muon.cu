@@ -25,6 +25,8 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <map>
+#include <utility>
 #include <vector>
 
 #include "common.cuh"
@@ -722,6 +724,7 @@ struct alignas(64) Problem {
 template <int CAP>
 struct Problems {
   int count, units;
+  int early;                     // few tiles: the next launch takes its place on the other SMs meanwhile (66 x 70 in a graph: 131 us a step, 119 so)
   Problem p[CAP];
 };
 struct UnitAt {
@@ -851,6 +854,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN, TERMS>::thr
   const uint32_t fullb = smem_u32(full), emptyb = smem_u32(empty), accfullb = smem_u32(accfull), accfreeb = smem_u32(accfree),
                  abortb = smem_u32(const_cast<int*>(abort_flag));
   grid_dependency_wait();
+  if (all.early) grid_launch_dependents();
 
   if (warp == 0) {
     // ================= TMA: this CTA's rows of L and its half of the rows of R ==============================================
@@ -1083,6 +1087,17 @@ long long tiles_of(int M, int N, int BN, bool symmetric) {   // of one matrix
   const long long tm = ceil_div(M, 256), tn = ceil_div(N, BN), q = 256 / BN;
   return symmetric ? tm * tn - q * tm * (tm - 1) / 2 : tm * tn;
 }
+// The tensor maps of a call, each encoded once: by the planes' address and the rows of a box.
+struct Maps {
+  std::map<std::pair<const void*, int>, CUtensorMap> all;
+  int get(CUtensorMap* to, const Planes& m, int box_rows, int terms) {
+    const auto [at, is_new] = all.try_emplace({m.p, box_rows});
+    if (is_new)
+      if (int rc = encode(&at->second, m, box_rows, terms)) return rc;
+    *to = at->second;
+    return B200CP_OK;
+  }
+};
 // out = alpha L R^T + beta add
 struct Product {
   Planes L, R, out;
@@ -1092,15 +1107,15 @@ struct Product {
   const Planes* add;
 };
 template <int BN, int TERMS, int CAP>
-int launch_table(const std::vector<Product>& ps, int pairs, cudaStream_t st) {
+int launch_table(const std::vector<Product>& ps, Maps& maps, int pairs, cudaStream_t st) {
   using T = Tile<BN, TERMS>;
   Problems<CAP> all;
   all.count = 0;
   long long units = 0;
   for (const Product& q : ps) {
     Problem& p = all.p[all.count++];
-    if (int rc = encode(&p.L, q.L, q.l_mn ? kStep : 128, TERMS)) return rc;
-    if (int rc = encode(&p.R, q.R, q.r_mn ? kStep : BN / 2, TERMS)) return rc;
+    if (int rc = maps.get(&p.L, q.L, q.l_mn ? kStep : 128, TERMS)) return rc;
+    if (int rc = maps.get(&p.R, q.R, q.r_mn ? kStep : BN / 2, TERMS)) return rc;
     p.M = q.out.rows;
     p.N = q.out.cols;
     p.steps = ceil_div(q.K, T::k);
@@ -1123,6 +1138,7 @@ int launch_table(const std::vector<Product>& ps, int pairs, cudaStream_t st) {
   }
   if (units > 0x3fffffff) return fail(B200CP_ERR_UNSUPPORTED, "b200cp_muon_step: the matrices are too large");
   all.units = (int)units;
+  all.early = 2 * units <= pairs;
   const auto kern = newton_kernel<BN, TERMS, CAP>;
   B200CP_CUDA_OK((allow_smem<newton_kernel<BN, TERMS, CAP>>((int)T::smem)));
   B200CP_CUDA_OK(launch_kernel(kern, dim3((unsigned)(2 * std::min<long long>(units, pairs))), dim3(T::threads), T::smem, st, true, all));
@@ -1130,13 +1146,13 @@ int launch_table(const std::vector<Product>& ps, int pairs, cudaStream_t st) {
   return B200CP_OK;
 }
 template <int BN, int TERMS>
-int launch_products(const std::vector<Product>& ps, int pairs, cudaStream_t st) {
-  return ps.size() <= kFewProblems ? launch_table<BN, TERMS, kFewProblems>(ps, pairs, st) : launch_table<BN, TERMS, kProblems>(ps, pairs, st);
+int launch_products(const std::vector<Product>& ps, Maps& maps, int pairs, cudaStream_t st) {
+  return ps.size() <= kFewProblems ? launch_table<BN, TERMS, kFewProblems>(ps, maps, pairs, st) : launch_table<BN, TERMS, kProblems>(ps, maps, pairs, st);
 }
 // One launch for all, the longest sums first.  Tiles of 256 columns, or of 128 where those fill the pairs of CTAs better: a narrow tile takes 0.55 of a wide one (0.65 with one
 // plane, where the loads count), so 4096 x 4096 goes in seven rounds of narrow ones, not in four of wide ones (279 us a product, and 350); 4096 x 10240 in nine of wide
 // ones, not in 18.
-int products(std::vector<Product> ps, int terms, const DeviceInfo& di, cudaStream_t st) {
+int products(std::vector<Product> ps, Maps& maps, int terms, const DeviceInfo& di, cudaStream_t st) {
   const int pairs = di.sm_count / 2;
   std::stable_sort(ps.begin(), ps.end(), [](const Product& a, const Product& b) { return a.K > b.K; });
   long long tiles[2] = {};
@@ -1144,8 +1160,8 @@ int products(std::vector<Product> ps, int terms, const DeviceInfo& di, cudaStrea
     for (int i = 0; i < 2; ++i) tiles[i] += tiles_of(p.out.rows, p.out.cols, 128 << i, p.symmetric) * p.out.count;
   const auto rounds = [&](long long n) { return (double)((n + pairs - 1) / pairs); };
   const bool wide = rounds(tiles[1]) <= (terms == 3 ? 0.55 : 0.65) * rounds(tiles[0]);
-  if (terms == 3) return wide ? launch_products<256, 3>(ps, pairs, st) : launch_products<128, 3>(ps, pairs, st);
-  return wide ? launch_products<256, 1>(ps, pairs, st) : launch_products<128, 1>(ps, pairs, st);
+  if (terms == 3) return wide ? launch_products<256, 3>(ps, maps, pairs, st) : launch_products<128, 3>(ps, maps, pairs, st);
+  return wide ? launch_products<256, 1>(ps, maps, pairs, st) : launch_products<128, 1>(ps, maps, pairs, st);
 }
 
 // ---- bounds on the singular values, and the scales of the planes that follow ----------------------------------------------------------
@@ -1193,10 +1209,12 @@ struct SmallSizes {
   size_t doubles = 0, floats = 0;
   int matrices = 0, ctas = 0;
 };
-// Parts of a matrix: as long as gives every SM the CTAs that it holds (per_sm) over all of the call's matrices: one round of them, and few parts to be added.
+// Parts of a matrix: as long as gives every SM the CTAs that it holds (per_sm) over all of the call's matrices, one round of them; and no more than are added (one after another,
+// by the one CTA that takes the matrix's steps) in the time that they save: 64 x 8192 takes 65 us in 64 parts, 86 in 256.
 void cut_small(const b200cp_muon_matrix& a, long long all, int slots, SmallEntry* e, SmallSizes* s) {
   const int n = std::min(a.rows, a.cols), len = std::max(a.rows, a.cols), ts = tile_side(n), sub = 2048 / (16 * ts), subs = ceil_div(len, sub);
-  const int parts = (int)std::min<long long>(subs, std::max<long long>(1, slots / std::max<long long>(1, all)));
+  const int most = (int)std::ceil(4 * std::sqrt((double)subs));
+  const int parts = (int)std::min<long long>({subs, most, std::max<long long>(1, slots / std::max<long long>(1, all))});
   e->rows = a.rows; e->cols = a.cols; e->stack = a.stack;
   e->length = ceil_div(subs, parts) * sub;
   e->chunks = ceil_div(len, e->length);
@@ -1436,21 +1454,22 @@ int run_large(const std::vector<Share>& round, const Rates& r, const Plan& plan,
   B200CP_LAUNCH_OK("muon_momentum_kernel");
   B200CP_CUDA_OK(launch_kernel(muon_planes_kernel<G, CAP>, dim3((unsigned)ctas8), dim3(256), 0, st, true, t));
   B200CP_LAUNCH_OK("muon_planes_kernel");
+  Maps maps;
   for (int step = 0; step < plan.steps; ++step) {
     const double* v = plan.v + (plan.coefficients > 1 ? 3 * step : 0);
     const double y = plan.bound[step] * plan.bound[step], sa = room_for(y),
                  sb = room_for(std::max(1e-3, std::fabs(v[1]) * y + std::fabs(v[2]) * y * y)), sn = room_for(plan.bound[step + 1]);
     std::vector<Product> ps;
     for (Large& m : ms) ps.push_back(Product{m.X, m.X, m.A, !m.wide, !m.wide, true, m.len, sa / (sx * sx), 0, nullptr});
-    if (int rc = products(ps, terms, di, st)) return rc;
+    if (int rc = products(ps, maps, terms, di, st)) return rc;
     ps.clear();
     for (Large& m : ms) ps.push_back(Product{m.A, m.A, m.B, false, false, true, m.n, v[2] * sb / (sa * sa), v[1] * sb / sa, &m.A});
-    if (int rc = products(ps, terms, di, st)) return rc;
+    if (int rc = products(ps, maps, terms, di, st)) return rc;
     ps.clear();
     for (Large& m : ms)
       ps.push_back(m.wide ? Product{m.B, m.X, m.Y, false, true, false, m.n, sn / (sb * sx), v[0] * sn / sx, &m.X}
                           : Product{m.X, m.B, m.Y, false, false, false, m.n, sn / (sb * sx), v[0] * sn / sx, &m.X});
-    if (int rc = products(ps, terms, di, st)) return rc;
+    if (int rc = products(ps, maps, terms, di, st)) return rc;
     for (Large& m : ms) std::swap(m.X, m.Y);
     sx = sn;
   }
