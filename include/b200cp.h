@@ -467,7 +467,7 @@ int b200cp_embedding_bwd(int rows, int V, int D, int type, int number_type, cons
 
 /* H = X + R rounded to the type (R and H may both be NULL: H is X), Y = (H - mean) rstd w + b per row, with the mean of the row's D features and
  * rstd = 1 / sqrt(their variance + eps).  X, R, Y, H [rows, D] of one type; w, b [D] of that type or float (weight_type), each may be NULL.
- * mean, rstd (both or neither): [rows] floats, kept for the backward.  Statistics are fp32.  No counterpart in the reference. */
+ * mean, rstd (both or neither): [rows] floats, kept for the backward.  Statistics are fp32.  rows and D are at most 2^30.  No counterpart in the reference. */
 int b200cp_layer_norm(int rows, int D, int type, int weight_type, const void* X, const void* R, const void* w, const void* b, float eps,
                       void* Y, void* H, float* mean, float* rstd, void* stream);
 

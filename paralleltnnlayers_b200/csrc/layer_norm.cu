@@ -647,7 +647,7 @@ int check_norm(const char* who, int rows, int D, int type, int weight_type) {
   if (type < B200CP_FLOAT32 || type > B200CP_FLOAT16) return fail(B200CP_ERR_INVALID_ARG, "%s: type %d", who, type);
   if (weight_type != type && weight_type != B200CP_FLOAT32)
     return fail(B200CP_ERR_UNSUPPORTED, "%s: weights of type %d for rows of type %d (that type, or float)", who, weight_type, type);
-  if (D > (1 << 30)) return fail(B200CP_ERR_UNSUPPORTED, "%s: rows of %d features (at most 2^30)", who, D);
+  if (D > (1 << 30) || rows > (1 << 30)) return fail(B200CP_ERR_UNSUPPORTED, "%s: %d rows of %d features (at most 2^30 of both)", who, rows, D);
   return B200CP_OK;
 }
 template <typename F>

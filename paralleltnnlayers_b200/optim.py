@@ -147,7 +147,7 @@ class Muon(torch.optim.Optimizer):
     Parameters have two dimensions or more; leading ones are stacks of matrices (``AdaptedDense.A`` and ``.B``), each orthogonalised by itself.  Vectors (biases,
     norms) and embeddings belong to an ``AdamW`` beside it.  Momentum is float32.  16-bit parameters get a float32 copy that is what is updated
     (``master=False``: the parameter itself, rounded at each step); it is taken at a parameter's first step.  ``lr`` may be one float32 in a CUDA tensor.
-    A captured ``step()`` begins no state: make one step with the same gradients before the capture."""
+    A captured ``step()`` begins no state: make one step with the same gradients before the capture.  A ``torch.optim.Muon``'s state can be loaded."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, ns_steps=5,
                  adjust_lr_fn=None, master=True):
@@ -166,17 +166,24 @@ class Muon(torch.optim.Optimizer):
             if p.dim() < 2:
                 raise ValueError(f"Muon is for matrices, a parameter is {tuple(p.shape)}")
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("master", True)
+
     def _state_of(self, p, group, capturing):
         s = self.state[p]
-        if not s:
+        copied = group["master"] and p.dtype != torch.float32
+        if "momentum_buffer" not in s or copied and "master" not in s:
             if capturing:
                 raise RuntimeError("a captured step() begins no state: make a step with the same gradients before the capture")
             if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
                 raise TypeError(f"parameters are float32, bfloat16 or float16, not {p.dtype}")
             if not p.is_contiguous():
                 raise ValueError("parameters are updated in place and have to be contiguous")
-            s["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-            if group["master"] and p.dtype != torch.float32:
+            if "momentum_buffer" not in s:
+                s["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            if copied:
                 s["master"] = p.detach().float()
         return s
 
@@ -206,9 +213,9 @@ class Muon(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As the base class, but the state keeps its own types (float32 buffers of 16-bit parameters)."""
+        """As the base class, but buffers are float32, those of 16-bit parameters too."""
         super().load_state_dict(state_dict)
         names = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         for name, p in zip(names, (p for g in self.param_groups for p in g["params"])):
             if name in state_dict["state"]:
-                self.state[p] = {k: v.detach().to(p.device, copy=True) if torch.is_tensor(v) else v for k, v in state_dict["state"][name].items()}
+                self.state[p] = {k: v.detach().to(p.device, torch.float32, copy=True).contiguous() if torch.is_tensor(v) else v for k, v in state_dict["state"][name].items()}

@@ -155,3 +155,32 @@ def test_the_optimiser_calls_the_step(monkeypatch, lib_built):
     assert calls[0][3:11] == (0.5, 0.8, True, 0.1, (3.4445, -4.7750, 2.0315), 1e-7, 5, "match_rms_adamw") and calls[0][11] is None
     assert calls[1][11][0].dtype == torch.float32 and calls[1][2][0].dtype == torch.float32
     assert calls[1][11][0] is calls[3][11][0] and p[2] not in opt.state
+
+
+def test_the_state_of_torchs_muon_is_loaded(monkeypatch, lib_built):
+    """Buffers of the parameter's type become float32, float32 copies are taken at the first step, and groups without ``master`` have them."""
+    from paralleltnnlayers_b200 import ops
+    from paralleltnnlayers_b200.optim import Muon
+    p = [torch.nn.Parameter(torch.full((3, 2), 0.5, dtype=BF16)), torch.nn.Parameter(torch.full((2, 4), 0.25))]
+    theirs = torch.optim.Muon(p, lr=0.3, momentum=0.8, ns_steps=4)
+    theirs.state[p[0]] = {"momentum_buffer": torch.full((3, 2), 1.5, dtype=BF16)}
+    theirs.state[p[1]] = {"momentum_buffer": torch.full((2, 4), 2.5)}
+    opt = Muon(p)
+    opt.load_state_dict(theirs.state_dict())
+    calls = []
+    monkeypatch.setattr(ops, "muon_step", lambda *a: calls.append(a))
+    for t in p:
+        t.grad = torch.ones_like(t)
+    opt.step()
+    assert len(calls) == 2 and all(c[3:5] == (0.3, 0.8) and c[9] == 4 for c in calls)
+    assert torch.equal(calls[0][2][0], torch.full((3, 2), 1.5)) and torch.equal(calls[1][2][0], torch.full((2, 4), 2.5))
+    assert torch.equal(calls[0][11][0], torch.full((3, 2), 0.5)) and calls[1][11] is None
+
+
+def test_too_many_rows_are_refused(lib_built):
+    from paralleltnnlayers_b200 import _lib
+    lib, at, rows = _lib.lib, 4096, (1 << 31) - 1
+    assert lib.b200cp_layer_norm(rows, 4, 0, 0, at, None, at, None, 1e-5, at, None, None, None, None) == -2
+    assert lib.b200cp_layer_norm_bwd(rows, 4, 0, 0, at, None, at, at, at, at, at, None, None, None, 0, None) == -2
+    assert lib.b200cp_embedding(rows, 5, 4, 0, 0, at, at, 1.0, at, None) == -2
+    assert lib.b200cp_embedding_bwd(rows, 5, 4, 0, 0, at, at, 1.0, at, None, 0, None) == -2
