@@ -29,6 +29,8 @@
 #include <utility>
 #include <vector>
 
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "tc_common.cuh"
 #include "tc_pair.cuh"
@@ -40,6 +42,7 @@ __device__ int g_muon_status = 0;   // 0 ok; otherwise (code << 16) | (linear bl
 
 namespace {
 
+namespace cg = cooperative_groups;
 using namespace tc;
 
 struct Pointers {   // of one matrix
@@ -281,62 +284,80 @@ __global__ void __launch_bounds__(256, per_sm(W)) muon_gram_kernel(const __grid_
 #undef B200CP_GRAM
 }
 
-// out = put(x y), all symmetric and commuting, rows of LD doubles: only tiles on and above the diagonal are formed, three by each of twelve warps.
-constexpr int kIterateThreads = 384;
-template <int TS, typename Put>
+// out = put(x y), all symmetric and commuting, rows of LD doubles: only tiles on and above the diagonal are there, up to three are formed by each of twelve warps (those below are read
+// from above, transposed).  CL CTAs of a cluster share the tiles, and each writes its own into the memory of all.
+constexpr int kIterateThreads = 384, kShare = 4;
+template <int CL>
+__device__ __forceinline__ int rank_in_cluster() {
+  if constexpr (CL == 1) return 0;
+  else return (int)cg::this_cluster().block_rank();
+}
+template <int CL>
+__device__ __forceinline__ void sync_all() {
+  if constexpr (CL == 1) __syncthreads();
+  else cg::this_cluster().sync();
+}
+// f(what lies at p in each of the CTAs)
+template <int CL, typename F>
+__device__ __forceinline__ void for_all(double* p, F f) {
+  if constexpr (CL == 1) {
+    f(p);
+  } else {
+#pragma unroll
+    for (int q = 0; q < CL; ++q) f(cg::this_cluster().map_shared_rank(p, q));
+  }
+}
+template <int TS, int CL, typename Put>
 __device__ __forceinline__ void symmetric_product(const double* x, const double* y, double* out, Put put) {
   using S = Side<TS>;
-  constexpr int LD = S::LD, C = (S::tiles + 11) / 12;
-  const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5) * C;
-  if (first < S::tiles) {
+  constexpr int LD = S::LD, share = (S::tiles + CL - 1) / CL, C = (share + 11) / 12;
+  static_assert(share % C == 0 && (CL == 1 || S::tiles % CL == 0));
+  const int lane = threadIdx.x & 31, mine = (threadIdx.x >> 5) * C, first = rank_in_cluster<CL>() * share + mine;
+  if (mine < share) {
     double acc[C][2] = {};
     int ti[C], tj[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) S::tile((first + c) / S::slots, (first + c) % S::slots, ti[c], tj[c]);
-    const double *a = x + (lane & 3) * LD + (lane >> 2), *b = y + (lane & 3) * LD + (lane >> 2);
-#pragma unroll 4
+    const int direct = (lane & 3) * LD + (lane >> 2), crossed = (lane >> 2) * LD + (lane & 3);
+    const auto fragment = [&](const double* z, int k, int tile) { return z[k / 8 <= tile ? direct + k * LD + tile * 8 : crossed + tile * 8 * LD + k]; };
+#pragma unroll
     for (int k = 0; k < S::N; k += 4)
 #pragma unroll
-      for (int c = 0; c < C; ++c) mma_f64(acc[c], a[k * LD + ti[c] * 8], b[k * LD + tj[c] * 8]);
+      for (int c = 0; c < C; ++c) mma_f64(acc[c], fragment(x, k, ti[c]), fragment(y, k, tj[c]));
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int row = ti[c] * 8 + (lane >> 2), col = tj[c] * 8 + (lane & 3) * 2;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const double v = put(acc[c][i], row, col + i);
-        out[row * LD + col + i] = v;
-        if (ti[c] != tj[c]) out[(col + i) * LD + row] = v;
-      }
+      const double2 v = make_double2(put(acc[c][0], row, col), put(acc[c][1], row, col + 1));
+      for_all<CL>(out, [&](double* to) { *reinterpret_cast<double2*>(to + row * LD + col) = v; });
     }
   }
-  __syncthreads();
+  sync_all<CL>();
 }
-template <int TS>
+template <int TS, int CL>
 __device__ __forceinline__ void iterate(const SmallHead& t, const Coefficients& co, const SmallEntry& e, int matrix, double* work) {
   using S = Side<TS>;
-  constexpr int N = S::N, LD = S::LD, NN = N * LD, kOwn = S::part / kIterateThreads + (S::part % kIterateThreads != 0);
-  const int tid = threadIdx.x, n = side_of(e);
+  constexpr int N = S::N, LD = S::LD, NN = N * LD, share = S::part / CL, kOwn = (share + kIterateThreads - 1) / kIterateThreads;
+  const int tid = threadIdx.x, rank = rank_in_cluster<CL>(), n = side_of(e);
   double *A = work, *Q = A + NN, *F = Q + NN, *P = F + NN;
   __shared__ double trace_sum;
   // the parts of A, in their order
-  const double* from = t.gram + e.gram + (size_t)matrix * e.chunks * S::part;
+  const double* from = t.gram + e.gram + (size_t)matrix * e.chunks * S::part + rank * share;
   double own[kOwn] = {};
-#pragma unroll 2
+#pragma unroll (CL == 1 ? 2 : 8)
   for (int c = 0; c < e.chunks; ++c)
 #pragma unroll
     for (int j = 0; j < kOwn; ++j)
-      if (tid + j * kIterateThreads < S::part) own[j] += from[(size_t)c * S::part + tid + j * kIterateThreads];
+      if (tid + j * kIterateThreads < share) own[j] += from[(size_t)c * S::part + tid + j * kIterateThreads];
 #pragma unroll
   for (int j = 0; j < kOwn; ++j) {
-    const int i = tid + j * kIterateThreads;
-    if (i >= S::part) break;
+    if (tid + j * kIterateThreads >= share) break;
+    const int i = rank * share + tid + j * kIterateThreads;
     int ti, tj;
     S::tile(i / 64 / S::slots, i / 64 % S::slots, ti, tj);
     const int r = ti * 8 + i % 64 / 8, c = tj * 8 + i % 8;
-    A[r * LD + c] = own[j];
-    if (ti != tj) A[c * LD + r] = own[j];
+    for_all<CL>(A, [&](double* to) { to[r * LD + c] = own[j]; });
   }
-  __syncthreads();
+  sync_all<CL>();
   if (tid < 32) {
     double s = 0.0;
     for (int i = tid; i < n; i += 32) s += A[i * LD + i];
@@ -354,30 +375,55 @@ __device__ __forceinline__ void iterate(const SmallHead& t, const Coefficients& 
   for (int step = 0; step < t.steps; ++step) {
     const double *v = co.v + (t.coefficients > 1 ? 3 * step : 0), v0 = v[0], v1 = v[1], v2 = v[2];
     double* p = step == 0 ? Q : P;
-    symmetric_product<TS>(A, A, p, [&](double s, int r, int c) { return fma(v2, s, fma(v1, A[r * LD + c], r == c ? v0 : 0.0)); });
+    symmetric_product<TS, CL>(A, A, p, [&](double s, int r, int c) { return fma(v2, s, fma(v1, A[r * LD + c], r == c ? v0 : 0.0)); });
     if (step > 0) {
-      symmetric_product<TS>(Q, p, F, as_is);
+      symmetric_product<TS, CL>(Q, p, F, as_is);
       double* q = Q;
       Q = F;
       F = q;
     }
     if (step + 1 == t.steps) break;
-    symmetric_product<TS>(A, p, F, as_is);
-    symmetric_product<TS>(F, p, A, as_is);
+    symmetric_product<TS, CL>(A, p, F, as_is);
+    symmetric_product<TS, CL>(F, p, A, as_is);
   }
   float* to = t.q + e.q + (size_t)matrix * (n * n);
-  for (int i = tid; i < n * n; i += kIterateThreads) to[i] = (float)Q[i / n * LD + i % n];
-  if (tid == 0) t.inverse[e.matrix + matrix] = inverse;
+  for (int i = rank * kIterateThreads + tid; i < n * n; i += CL * kIterateThreads) {
+    const int r = i / n, c = i % n;
+    to[i] = (float)Q[r / 8 <= c / 8 ? r * LD + c : c * LD + r];
+  }
+  if (tid == 0 && rank == 0) t.inverse[e.matrix + matrix] = inverse;
+}
+template <int CAP>
+__device__ __forceinline__ const SmallEntry& entry_with(const SmallTable<CAP>& t, int matrix) {
+  return t.e[entry_of(t, matrix, [](const SmallEntry& s) { return s.matrix; })];
 }
 template <int CAP>
 __global__ void __launch_bounds__(kIterateThreads) muon_iterate_kernel(const __grid_constant__ SmallTable<CAP> t, const __grid_constant__ Coefficients co) {
   extern __shared__ __align__(16) double work[];
   grid_dependency_wait();
-  const SmallEntry& e = t.e[entry_of(t, blockIdx.x, [](const SmallEntry& s) { return s.matrix; })];
+  const SmallEntry& e = entry_with(t, blockIdx.x);
   const int matrix = (int)blockIdx.x - e.matrix, n = side_of(e);
-  if (n <= 16) iterate<1>(t, co, e, matrix, work);
-  else if (n <= 32) iterate<2>(t, co, e, matrix, work);
-  else iterate<4>(t, co, e, matrix, work);
+  if (n <= 16) iterate<1, 1>(t, co, e, matrix, work);
+  else if (n <= 32) iterate<2, 1>(t, co, e, matrix, work);
+  else iterate<4, 1>(t, co, e, matrix, work);
+}
+// The same with a cluster for each of the first `wide` matrices, whose sides are above 32, and a CTA for each of the others: where all of them have an SM.  A product of
+// 64 x 64 takes 3100 cycles of one SM (2300 of its 64-bit tensor instructions), 2250 of four: 1150 for the tiles, 800 until they are in all memories, 300 for the barrier.  (One
+// matrix of 64 x 64 42 us in all when one CTA took its steps, 33 so.)  Where they do not all have an SM, clusters would wait for the SMs of other ones.
+template <int CAP>
+__global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kIterateThreads)
+    muon_iterate_shared_kernel(const __grid_constant__ SmallTable<CAP> t, const __grid_constant__ Coefficients co, int wide, int matrices) {
+  extern __shared__ __align__(16) double work[];
+  const bool shared = (int)blockIdx.x < kShare * wide;
+  const int at = shared ? (int)blockIdx.x / kShare : (int)blockIdx.x - (kShare - 1) * wide;
+  if (shared) sync_all<kShare>();   // (all CTAs of the cluster are there before one writes into another)
+  grid_dependency_wait();
+  if (at >= matrices) return;
+  const SmallEntry& e = entry_with(t, at);
+  const int matrix = at - e.matrix, n = side_of(e);
+  if (shared) iterate<4, kShare>(t, co, e, matrix, work);
+  else if (n <= 16) iterate<1, 1>(t, co, e, matrix, work);
+  else iterate<2, 1>(t, co, e, matrix, work);
 }
 
 // X = Q u / |u| for a part of the longer side, and the update.
@@ -1210,10 +1256,10 @@ struct SmallSizes {
   int matrices = 0, ctas = 0;
 };
 // Parts of a matrix: as long as gives every SM the CTAs that it holds (per_sm) over all of the call's matrices, one round of them; and no more than are added (one after another,
-// by the one CTA that takes the matrix's steps) in the time that they save: 64 x 8192 takes 65 us in 64 parts, 86 in 256.
+// by the CTAs that take the matrix's steps) in the time that they save: 64 x 8192 takes 50 us in 64 parts, 45 in 128, 49 in 256.
 void cut_small(const b200cp_muon_matrix& a, long long all, int slots, SmallEntry* e, SmallSizes* s) {
   const int n = std::min(a.rows, a.cols), len = std::max(a.rows, a.cols), ts = tile_side(n), sub = 2048 / (16 * ts), subs = ceil_div(len, sub);
-  const int most = (int)std::ceil(4 * std::sqrt((double)subs));
+  const int most = (int)std::ceil(8 * std::sqrt((double)subs));
   const int parts = (int)std::min<long long>({subs, most, std::max<long long>(1, slots / std::max<long long>(1, all))});
   e->rows = a.rows; e->cols = a.cols; e->stack = a.stack;
   e->length = ceil_div(subs, parts) * sub;
@@ -1252,7 +1298,7 @@ struct Shape {
 size_t type_size(int type) { return type == B200CP_FLOAT32 ? 4 : 2; }
 constexpr int kMostStack = 4096;
 struct Work {
-  std::vector<b200cp_muon_matrix> little;
+  std::vector<b200cp_muon_matrix> little;   // those with sides above 32 first
   long long matrices = 0;   // small ones
   int widest = 1;           // 1: all of them have a side of at most 16; or 4
   std::vector<Shape> large;
@@ -1281,6 +1327,7 @@ struct Work {
         s->at.push_back(Pointers{q.param, q.grad, q.momentum, q.master});
       }
     }
+    std::stable_partition(little.begin(), little.end(), [](const b200cp_muon_matrix& a) { return tile_side(std::min(a.rows, a.cols)) == 4; });
   }
 };
 // Larger matrices that share launches: parts of shapes, as the tables and some memory hold them.
@@ -1345,7 +1392,7 @@ float factor_of(int adjust, int rows, int cols) {
 }
 
 template <typename P, typename G, int W, int CAP>
-int launch_small(const SmallHead& head, const SmallEntry* e, const Coefficients& co, const SmallSizes& s, cudaStream_t st) {
+int launch_small(const SmallHead& head, const SmallEntry* e, const Coefficients& co, const SmallSizes& s, int sm_count, cudaStream_t st) {
   SmallTable<CAP> t;
   static_cast<SmallHead&>(t) = head;
   std::copy(e, e + head.count, t.e);
@@ -1357,8 +1404,16 @@ int launch_small(const SmallHead& head, const SmallEntry* e, const Coefficients&
   B200CP_CUDA_OK((allow_smem<muon_gram_kernel<G, W, CAP>>(gram)));
   B200CP_CUDA_OK(launch_kernel(muon_gram_kernel<G, W, CAP>, dim3(s.ctas), dim3(256), gram, st, true, t));
   B200CP_LAUNCH_OK("muon_gram_kernel");
-  B200CP_CUDA_OK(allow_smem<muon_iterate_kernel<CAP>>(four));
-  B200CP_CUDA_OK(launch_kernel(muon_iterate_kernel<CAP>, dim3(s.matrices), dim3(kIterateThreads), four, st, true, t, co));
+  int wide = 0;   // (they are the first ones)
+  for (int i = 0; i < t.count; ++i) wide += tile_side(std::min(t.e[i].rows, t.e[i].cols)) == 4 ? t.e[i].stack : 0;
+  const int shared = ceil_div(s.matrices + (kShare - 1) * wide, kShare) * kShare;
+  if (wide && shared <= sm_count) {
+    B200CP_CUDA_OK(allow_smem<muon_iterate_shared_kernel<CAP>>(four));
+    B200CP_CUDA_OK(launch_kernel(muon_iterate_shared_kernel<CAP>, dim3(shared), dim3(kIterateThreads), four, st, true, t, co, wide, s.matrices));
+  } else {
+    B200CP_CUDA_OK(allow_smem<muon_iterate_kernel<CAP>>(four));
+    B200CP_CUDA_OK(launch_kernel(muon_iterate_kernel<CAP>, dim3(s.matrices), dim3(kIterateThreads), four, st, true, t, co));
+  }
   B200CP_LAUNCH_OK("muon_iterate_kernel");
   B200CP_CUDA_OK((allow_smem<muon_small_apply_kernel<P, G, W, CAP>>(low)));
   B200CP_CUDA_OK(launch_kernel(muon_small_apply_kernel<P, G, W, CAP>, dim3(s.ctas), dim3(256), low, st, true, t));
@@ -1382,8 +1437,8 @@ int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char*
     t.q = reinterpret_cast<float*>(ws + align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256));
     for (int i = 0; i < t.count; ++i) t.e[i].scale = factor_of(adjust, t.e[i].rows, t.e[i].cols);
     const bool few = t.count <= kFewSmall;
-    const int rc = w.widest == 1 ? (few ? launch_small<P, G, 1, kFewSmall>(t, t.e, co, s, st) : launch_small<P, G, 1, kTableSmall>(t, t.e, co, s, st))
-                                 : (few ? launch_small<P, G, 4, kFewSmall>(t, t.e, co, s, st) : launch_small<P, G, 4, kTableSmall>(t, t.e, co, s, st));
+    const int rc = w.widest == 1 ? (few ? launch_small<P, G, 1, kFewSmall>(t, t.e, co, s, di.sm_count, st) : launch_small<P, G, 1, kTableSmall>(t, t.e, co, s, di.sm_count, st))
+                                 : (few ? launch_small<P, G, 4, kFewSmall>(t, t.e, co, s, di.sm_count, st) : launch_small<P, G, 4, kTableSmall>(t, t.e, co, s, di.sm_count, st));
     if (rc) return rc;
   }
   return B200CP_OK;

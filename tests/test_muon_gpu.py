@@ -263,3 +263,26 @@ def test_streams_and_graphs():
         for k in (0, 1, 0):
             graphs[k][0].replay()
             assert torch.equal(graphs[k][1], want[k])
+
+
+@pytest.mark.parametrize("wide,others", [(1, 0), (1, 1), (3, 7), (8, 66), (37, 0), (37, 1), (38, 3), (150, 20)])
+def test_small_sides_together(wide, others):
+    """Sides above and below 32 in turn, up to and beyond four CTAs an SM's worth for each of the wide ones; one of them zero, one not a number."""
+    import paralleltnnlayers_b200 as P
+    shapes = [None] * (wide + others)
+    for k in range(wide + others):
+        turn = k * wide // (wide + others) != (k + 1) * wide // (wide + others)
+        shapes[k] = (33 + k % 32, 64 + 5 * (k % 9)) if turn else (1 + k % 32, 40 - k % 11)
+    assert sum(min(s) > 32 for s in shapes) == wide
+    for bad in (False, True):
+        p, g = [torch.zeros(*s, device="cuda") for s in shapes], [matrices(*s, seed=k) for k, s in enumerate(shapes)]
+        if bad:
+            g[0].zero_()
+            g[-1][0, 0] = float("nan")
+        P.muon_step(p, g, [torch.zeros_like(t) for t in p], 1.0, momentum=0.0, weight_decay=0.0, adjust=None)
+        for k, (a, b) in enumerate(zip(p, g)):
+            if bad and k == len(p) - 1:
+                assert bool(a.isnan().all())
+            else:
+                check(-a, *defined(b))
+    P.device_status()
