@@ -1255,14 +1255,17 @@ struct SmallSizes {
   size_t doubles = 0, floats = 0;
   int matrices = 0, ctas = 0;
 };
-// Parts of a matrix: as long as gives every SM the CTAs that it holds (per_sm) over all of the call's matrices, one round of them; and no more than are added (one after another,
-// by the CTAs that take the matrix's steps) in the time that they save: 64 x 8192 takes 50 us in 64 parts, 45 in 128, 49 in 256.
+// What a CTA takes at a time of a matrix's longer side, and how many such turns there are.
+int turn_of(const b200cp_muon_matrix& a) { return 2048 / (16 * tile_side(std::min(a.rows, a.cols))); }
+int turns_of(const b200cp_muon_matrix& a) { return ceil_div(std::max(a.rows, a.cols), turn_of(a)); }
+// Parts of a matrix: its share, by its turns, of the CTAs that the SMs hold (slots), so that the call is one round of CTAs that all have about as many turns; and no more than are
+// added (one after another, by the CTAs that take the matrix's steps) in the time that they save: 64 x 8192 takes 50 us in 64 parts, 45 in 128, 49 in 256.
 void cut_small(const b200cp_muon_matrix& a, long long all, int slots, SmallEntry* e, SmallSizes* s) {
-  const int n = std::min(a.rows, a.cols), len = std::max(a.rows, a.cols), ts = tile_side(n), sub = 2048 / (16 * ts), subs = ceil_div(len, sub);
-  const int most = (int)std::ceil(8 * std::sqrt((double)subs));
-  const int parts = (int)std::min<long long>({subs, most, std::max<long long>(1, slots / std::max<long long>(1, all))});
+  const int n = std::min(a.rows, a.cols), len = std::max(a.rows, a.cols), ts = tile_side(n), sub = turn_of(a), turns = turns_of(a);
+  const int most = (int)std::ceil(8 * std::sqrt((double)turns));
+  const int parts = (int)std::min<long long>({turns, most, std::max<long long>(1, (long long)slots * turns / all)});
   e->rows = a.rows; e->cols = a.cols; e->stack = a.stack;
-  e->length = ceil_div(subs, parts) * sub;
+  e->length = ceil_div(turns, parts) * sub;
   e->chunks = ceil_div(len, e->length);
   e->first = s->ctas;
   e->matrix = s->matrices;
@@ -1299,7 +1302,7 @@ size_t type_size(int type) { return type == B200CP_FLOAT32 ? 4 : 2; }
 constexpr int kMostStack = 4096;
 struct Work {
   std::vector<b200cp_muon_matrix> little;   // those with sides above 32 first
-  long long matrices = 0;   // small ones
+  long long turns = 0;      // of small ones
   int widest = 1;           // 1: all of them have a side of at most 16; or 4
   std::vector<Shape> large;
   Work(const b200cp_muon_matrix* ms, int count, int ptype, int gtype) {
@@ -1313,7 +1316,7 @@ struct Work {
       };
       if (small(a)) {
         for (int k = 0; k < a.stack; k += kMostStack) little.push_back(part(k, std::min(kMostStack, a.stack - k)));
-        matrices += a.stack;
+        turns += (long long)a.stack * turns_of(a);
         if (tile_side(std::min(a.rows, a.cols)) > 1) widest = 4;
         continue;
       }
@@ -1379,7 +1382,7 @@ size_t workspace_of(const Work& w, int sm_count) {
   size_t most = 0;
   for (size_t at = 0; at < w.little.size();) {
     SmallSizes s;
-    at += next_small(w.little, at, w.matrices, per_sm(w.widest) * sm_count, nullptr, &s);
+    at += next_small(w.little, at, w.turns, per_sm(w.widest) * sm_count, nullptr, &s);
     most = std::max(most, small_bytes(s));
   }
   for (const std::vector<Share>& r : rounds_of(w)) most = std::max(most, round_bytes(r));
@@ -1427,7 +1430,7 @@ int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char*
   SmallTable<kTableSmall> t;
   for (size_t at = 0; at < w.little.size();) {
     SmallSizes s;
-    t.count = next_small(w.little, at, w.matrices, per_sm(w.widest) * di.sm_count, &t, &s);
+    t.count = next_small(w.little, at, w.turns, per_sm(w.widest) * di.sm_count, &t, &s);
     at += t.count;
     t.r = r;
     t.steps = plan.steps;
