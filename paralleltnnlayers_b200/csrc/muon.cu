@@ -123,7 +123,7 @@ struct Side {
 };
 constexpr int kPart[5] = {0, Side<1>::part, Side<2>::part, 0, Side<4>::part};
 // c += a b of 8 x 4 by 4 x 8 in 64 bits: a is of row lane / 4 and k lane % 4, b of column lane / 4, c of row lane / 4 and columns 2 (lane % 4) and one on.
-// (The same rate as fma, a fourth of the loads from shared memory: 64 x 64 x 64 in 1.3 us, with tiles of 4 x 2 in fma 4.8.)
+// (The same rate as fma, a fourth of the loads from shared memory: a symmetric product of 64 x 64 x 64 in 1.3 us, with tiles of 4 x 2 in fma 4.8.)
 __device__ __forceinline__ void mma_f64(double (&c)[2], double a, double b) {
   asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
@@ -399,15 +399,19 @@ template <int CAP>
 __device__ __forceinline__ const SmallEntry& entry_with(const SmallTable<CAP>& t, int matrix) {
   return t.e[entry_of(t, matrix, [](const SmallEntry& s) { return s.matrix; })];
 }
-template <int CAP>
-__global__ void __launch_bounds__(kIterateThreads) muon_iterate_kernel(const __grid_constant__ SmallTable<CAP> t, const __grid_constant__ Coefficients co) {
+// WIDEST: of the launch's matrices, as Side's TS.  Sides up to 32 leave room for three CTAs an SM (3000 of 16 x 64 86 us, with
+// one 122), 64 takes 174 KB of shared memory.
+template <int WIDEST, int CAP>
+__global__ void __launch_bounds__(kIterateThreads, WIDEST == 4 ? 1 : 3) muon_iterate_kernel(const __grid_constant__ SmallTable<CAP> t, const __grid_constant__ Coefficients co) {
   extern __shared__ __align__(16) double work[];
   grid_dependency_wait();
   const SmallEntry& e = entry_with(t, blockIdx.x);
   const int matrix = (int)blockIdx.x - e.matrix, n = side_of(e);
-  if (n <= 16) iterate<1, 1>(t, co, e, matrix, work);
-  else if (n <= 32) iterate<2, 1>(t, co, e, matrix, work);
-  else iterate<4, 1>(t, co, e, matrix, work);
+  if constexpr (WIDEST == 4)
+    if (n > 32) return iterate<4, 1>(t, co, e, matrix, work);
+  if constexpr (WIDEST >= 2)
+    if (n > 16) return iterate<2, 1>(t, co, e, matrix, work);
+  iterate<1, 1>(t, co, e, matrix, work);
 }
 // The same with a cluster for each of the first `wide` matrices, whose sides are above 32, and a CTA for each of the others: where all of them have an SM.  A product of
 // 64 x 64 takes 3100 cycles of one SM (2300 of its 64-bit tensor instructions), 2250 of four: 1150 for the tiles, 800 until they are in all memories, 300 for the barrier.  (One
@@ -1416,8 +1420,15 @@ int launch_small(const SmallHead& head, const SmallEntry* e, const Coefficients&
     B200CP_CUDA_OK(allow_smem<muon_iterate_shared_kernel<CAP>>(five));
     B200CP_CUDA_OK(launch_kernel(muon_iterate_shared_kernel<CAP>, dim3(shared), dim3(kIterateThreads), five, st, true, t, co, wide, s.matrices));
   } else {
-    B200CP_CUDA_OK(allow_smem<muon_iterate_kernel<CAP>>(five));
-    B200CP_CUDA_OK(launch_kernel(muon_iterate_kernel<CAP>, dim3(s.matrices), dim3(kIterateThreads), five, st, true, t, co));
+    const auto steps = [&](auto kernel, auto allow) {
+      B200CP_CUDA_OK(allow(five));
+      B200CP_CUDA_OK(launch_kernel(kernel, dim3(s.matrices), dim3(kIterateThreads), five, st, true, t, co));
+      return (int)B200CP_OK;
+    };
+    const int rc = ts == 1   ? steps(muon_iterate_kernel<1, CAP>, allow_smem<muon_iterate_kernel<1, CAP>>)
+                   : ts == 2 ? steps(muon_iterate_kernel<2, CAP>, allow_smem<muon_iterate_kernel<2, CAP>>)
+                             : steps(muon_iterate_kernel<4, CAP>, allow_smem<muon_iterate_kernel<4, CAP>>);
+    if (rc) return rc;
   }
   B200CP_LAUNCH_OK("muon_iterate_kernel");
   B200CP_CUDA_OK((allow_smem<muon_small_apply_kernel<P, G, W, CAP>>(low)));
