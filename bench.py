@@ -225,7 +225,7 @@ def extra_configs(P, world, rank, reduce_fn, max_over_ranks):
 def reference_gpu_forward_us():
     """The reference's own forward kernel (compiled unmodified for this GPU by oracle/build_ref.py) timed by its own
     PROFCOUNT loop (47 launches, Cuda_kernels/cp4Conv2dForward.cu:245-327; bench/BenchBothTime.cu:90) at config 1 and
-    config 2.  Forward only; part of the CPU-baseline leg: it is the checker's code, not the product's."""
+    config 2.  Forward only; part of the CPU-baseline leg: it is the oracle's code, not the product's."""
     try:
         from oracle import cp_oracle as O
         from oracle import reference_cuda as RC
