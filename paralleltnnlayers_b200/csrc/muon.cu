@@ -16,9 +16,8 @@
 // most 256 terms in an accumulator (the tensor core cuts sums off: over 4096 terms it loses 3e-5, where fp32 rounding loses 3e-7) and the rest in registers
 // (4096 x 4096 against 64 bits: 5.5e-7 with 64 terms, 6.3e-7 with 128, 1.1e-6 with 256, in 3.85 ms with 128 and 3.66 with 256; fp32 products of a library: 3.6e-6
 // in 34 ms).  a X is added in fp32 (as part of the product, with a I in B, 5 % faster and two to three times as far off).
-// Where the result has 16 bits (bfloat16 X, 16-bit parameters without a copy) operands are the hi parts alone, a third of the work: 4096 x 10240 in bfloat16 3.1 ms, in
-// float32 6.8.  X keeps both parts: directions with small singular values are raised by 3.4445 a step, and what one part lacks of X would come out as 7 % of a gradient of
-// rank one; what it lacks as an operand stays in the row or column space of what it is multiplied with.
+// Results of 16 bits are computed the same way and rounded once.  (Products of the hi parts alone are a third of the work, 4096 x 10240 in bfloat16 2.7 ms where these take
+// 7.6, but leave X 1e-3 off: a rounding that no caller has asked for, and more than that of fp16 itself.)
 // A and B are symmetric: blocks below the diagonal are not computed, the others stored twice.  Either operand is taken in either order, so nothing is
 // transposed; where the rows are the longer side A = X^T X and X <- a X + X B.  Matrices of all shapes share their launches.
 // Every wait is bounded: one that runs out sets a status word and the CTA leaves through its normal exit.
@@ -746,17 +745,15 @@ __global__ void __launch_bounds__(256) muon_apply_kernel(const __grid_constant__
 
 // ---- the products ------------------------------------------------------------------------------------------------------------------
 // out = alpha sum_k L[m][k] R[n][k] + beta add, of planes, for batches of matrices of several shapes (problems).  A pair of CTAs has a tile of
-// 256 x BN; one thread issues, accumulators in turn.
-// TERMS 3 (results of fp32 grade): both planes of 64 k in a stage, products hi hi + hi lo + lo hi; an accumulator holds kGroupSteps stages and is then added to
-// totals in registers.  TERMS 1 (results of 16 bits): hi planes alone, 128 k in a stage, and an accumulator holds the whole sum.
+// 256 x BN; one thread issues, accumulators in turn.  A stage has both planes of 64 k, products are hi hi + hi lo + lo hi; an accumulator holds kGroupSteps stages and is then
+// added to totals in registers.
 constexpr int kStep = 64, kBand = 16, kGroupSteps = 4;
 constexpr int kPatch = 32 * 64;   // bytes of a warp's block of 32 x 32 halves on its way in or out
-template <int BN, int TERMS>
+template <int BN>
 struct Tile {
-  static constexpr int planes = 2;                      // blocks of 64 k in a stage: both planes' (TERMS 3), or two of the one plane
-  static constexpr int k = TERMS == 3 ? kStep : 2 * kStep;   // of a stage
+  static constexpr int planes = 2;
   static constexpr int aplane = 128 * kStep * 2, bplane = BN / 2 * kStep * 2;
-  static constexpr int abytes = planes * aplane, stage = abytes + planes * bplane;                   // 64, 48, 32, 24 KB
+  static constexpr int abytes = planes * aplane, stage = abytes + planes * bplane;                   // 64 or 48 KB
   static constexpr int stages = 192 * 1024 / stage, depth = BN == 256 ? 2 : 4;                       // of the ring; accumulators
   static constexpr int readers = 4 * BN / 64, threads = 64 + 32 * readers;
   static constexpr size_t smem = (size_t)stages * stage + readers * kPatch + 1024 + 256;
@@ -771,7 +768,7 @@ struct alignas(64) Problem {
   const __half* add;             // as out, or null
   __half* out;
   int ld;
-  size_t plane, add_plane, matrix;   // (planes: 0 where there is one only)
+  size_t plane, matrix;          // halves from one plane to the next, and from one matrix
 };
 template <int CAP>
 struct Problems {
@@ -869,9 +866,9 @@ __device__ __forceinline__ void unpack_times(const uint4& q, float by, float* v,
   for (int i = 0; i < 8; ++i) v[i] = more ? fmaf(by, x[i], v[i]) : by * x[i];
 }
 
-template <int BN, int TERMS, int CAP>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN, TERMS>::threads, 1) newton_kernel(const __grid_constant__ Problems<CAP> all) {
-  using T = Tile<BN, TERMS>;
+template <int BN, int CAP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN>::threads, 1) newton_kernel(const __grid_constant__ Problems<CAP> all) {
+  using T = Tile<BN>;
   constexpr int kStages = T::stages, kBox = T::planes * kStep * 128;   // kBox: bytes of 64 rows, MN-major
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -922,23 +919,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN, TERMS>::thr
           if (it >= kStages && !(ok = wait_or_abort(emptyb + slot * 8, ((it / kStages) - 1) & 1, abortb))) break;
           if (rank == 0) mbar_expect_tx(&full[slot], 2 * T::stage);
           const uint32_t bar = leader_addr(fullb + slot * 8), a = smem_u32(sm) + slot * T::stage, b = a + T::abytes;
-          const int k = s * T::k;
-          // (TERMS 1: a box holds one block of 64 k; those of k past the end are zeros)
+          const int k = s * kStep;
+          if (g.l_mn) {
 #pragma unroll
-          for (int h = 0; h < (TERMS == 3 ? 1 : 2); ++h) {
-            const int kh = k + h * kStep;
-            if (g.l_mn) {
+            for (int q = 0; q < 2; ++q) tma_load_planes(a + q * kBox, &g.L, bar, m + q * 64, k, t.matrix);
+          } else {
+            tma_load_planes(a, &g.L, bar, k, m, t.matrix);
+          }
+          if (g.r_mn) {
 #pragma unroll
-              for (int q = 0; q < 2; ++q) tma_load_planes(a + q * kBox + h * (kStep * 128), &g.L, bar, m + q * 64, kh, t.matrix);
-            } else {
-              tma_load_planes(a + h * T::aplane, &g.L, bar, kh, m, t.matrix);
-            }
-            if (g.r_mn) {
-#pragma unroll
-              for (int q = 0; q < BN / 128; ++q) tma_load_planes(b + q * kBox + h * (kStep * 128), &g.R, bar, n + q * 64, kh, t.matrix);
-            } else {
-              tma_load_planes(b + h * T::bplane, &g.R, bar, kh, n, t.matrix);
-            }
+            for (int q = 0; q < BN / 128; ++q) tma_load_planes(b + q * kBox, &g.R, bar, n + q * 64, k, t.matrix);
+          } else {
+            tma_load_planes(b, &g.R, bar, k, n, t.matrix);
           }
         }
       }
@@ -959,25 +951,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN, TERMS>::thr
         const int steps = g.steps;
         for (int s = 0; s < steps; ++s, ++it) {
           const int slot = it % kStages, buf = gi % T::depth;
-          const bool first = TERMS == 3 ? s % kGroupSteps == 0 : s == 0, last = s + 1 == steps || (TERMS == 3 && s % kGroupSteps == kGroupSteps - 1);
+          const bool first = s % kGroupSteps == 0, last = s + 1 == steps || s % kGroupSteps == kGroupSteps - 1;
           if (!(ok = wait_or_abort(fullb + slot * 8, (it / kStages) & 1, abortb))) break;
           if (first && gi >= T::depth && !(ok = wait_or_abort(accfreeb + buf * 8, (gi / T::depth - 1) & 1, abortb))) break;
           tc_fence_after_sync();
           const uint32_t a = smem_u32(sm) + slot * T::stage, d = tmem_base + buf * BN;
           const uint64_t l = dl + (a >> 4), r = dr + ((a + T::abytes) >> 4);
-          if (TERMS == 3) {
 #pragma unroll
-            for (int i = 0; i < kStep / 16; ++i) {   // the small products first
-              mma_f16_pair(d, l + pl + i * sl, r + i * sr, idesc, !first || i > 0);
-              mma_f16_pair(d, l + i * sl, r + pr + i * sr, idesc, true);
-            }
+          for (int i = 0; i < kStep / 16; ++i) {   // the small products first
+            mma_f16_pair(d, l + pl + i * sl, r + i * sr, idesc, !first || i > 0);
+            mma_f16_pair(d, l + i * sl, r + pr + i * sr, idesc, true);
           }
 #pragma unroll
-          for (int i = 0; i < kStep / 16; ++i) mma_f16_pair(d, l + i * sl, r + i * sr, idesc, TERMS == 3 || !first || i > 0);
-          if (TERMS == 1) {
-#pragma unroll
-            for (int i = 0; i < kStep / 16; ++i) mma_f16_pair(d, l + pl + i * sl, r + pr + i * sr, idesc, true);
-          }
+          for (int i = 0; i < kStep / 16; ++i) mma_f16_pair(d, l + i * sl, r + i * sr, idesc, true);
           if (last) {
             commit_pair(accfullb + buf * 8);
             ++gi;
@@ -987,46 +973,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN, TERMS>::thr
       }
     }
   } else {
-    // ================= read-out: accumulators -> (totals ->) planes ===========================================================
+    // ================= read-out: accumulators -> totals -> planes =============================================================
     const int qd = warp & 3, c0 = ((warp - 2) >> 2) * 64;   // the lane quarter that this warp may read, and its columns
     const uint32_t taddr = tmem_base + ((uint32_t)(qd * 32) << 16) + c0;
     int gi = 0;
     bool ok = true;
     for (int unit = pair; unit < all.units && ok; unit += npairs) {
       int buf = 0;
-      if constexpr (TERMS == 3) {
-        float tot[64];
+      float tot[64];
 #pragma unroll
-        for (int j = 0; j < 64; ++j) tot[j] = 0.f;
-        const int groups = (all.p[unit_at<BN>(all, unit).problem].steps + kGroupSteps - 1) / kGroupSteps;
-        for (int s = 0; s < groups; ++s, ++gi) {
-          buf = gi % T::depth;
-          if (!(ok = __all_sync(0xffffffffu, wait_or_abort(accfullb + buf * 8, (gi / T::depth) & 1, abortb)))) break;
-          tc_fence_after_sync();
-#pragma unroll
-          for (int j0 = 0; j0 < 64; j0 += 16) {
-            float v[16];
-            tmem_ld16(taddr + buf * BN + j0, v);
-            if (j0 == 48 && s + 1 < groups) {
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) tot[j0 + j] += v[j];
-          }
-        }
-        if (!ok) break;
-        // through the accumulator just read, so that a short loop stores them (unrolled over registers it is code that every tile fetches anew)
-#pragma unroll
-        for (int j0 = 0; j0 < 64; j0 += 16) tmem_st16(taddr + buf * BN + j0, tot + j0);
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      } else {
+      for (int j = 0; j < 64; ++j) tot[j] = 0.f;
+      const int groups = (all.p[unit_at<BN>(all, unit).problem].steps + kGroupSteps - 1) / kGroupSteps;
+      for (int s = 0; s < groups; ++s, ++gi) {
         buf = gi % T::depth;
         if (!(ok = __all_sync(0xffffffffu, wait_or_abort(accfullb + buf * 8, (gi / T::depth) & 1, abortb)))) break;
         tc_fence_after_sync();
-        ++gi;
+#pragma unroll
+        for (int j0 = 0; j0 < 64; j0 += 16) {
+          float v[16];
+          tmem_ld16(taddr + buf * BN + j0, v);
+          if (j0 == 48 && s + 1 < groups) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(leader_addr(accfreeb + buf * 8));
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) tot[j0 + j] += v[j];
+        }
       }
+      if (!ok) break;
+      // through the accumulator just read, so that a short loop stores them (unrolled over registers it is code that every tile fetches anew)
+#pragma unroll
+      for (int j0 = 0; j0 < 64; j0 += 16) tmem_st16(taddr + buf * BN + j0, tot + j0);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       const UnitAt t = unit_at<BN>(all, unit);
       const Problem& g = all.p[t.problem];
       const int m0 = t.m0 + rank * 128 + qd * 32, m = m0 + lane;
@@ -1042,15 +1021,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN, TERMS>::thr
         if (g.add) {
           uint4 in[4], more[4];
           at.load(g.add + base, in);
-          if (g.add_plane) at.load(g.add + base + g.add_plane, more);
+          at.load(g.add + base + g.plane, more);
           at.turn(patch, in);
 #pragma unroll
           for (int j = 0; j < 32; j += 8) unpack_times(in[j / 8], g.beta, v + j, false);
-          if (g.add_plane) {
-            at.turn(patch, more);
+          at.turn(patch, more);
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) unpack_times(more[j / 8], g.beta, v + j, true);
-          }
+          for (int j = 0; j < 32; j += 8) unpack_times(more[j / 8], g.beta, v + j, true);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = 0.f;
@@ -1065,7 +1042,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<BN, TERMS>::thr
         __half* out = g.out + base;
 #pragma unroll
         for (int plane = 0; plane < 2; ++plane) {   // hi, then what is left
-          if (plane && !g.plane) break;
           uint4 q[4];
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
@@ -1116,20 +1092,20 @@ cudaError_t allow_smem(int bytes) {
   static std::atomic<int> set[64];
   return ensure_dynamic_smem(reinterpret_cast<const void*>(KERNEL), set, bytes);
 }
-struct Planes {   // of a batch of matrices; one plane or two
+struct Planes {   // of a batch of matrices
   __half* p;
-  int rows, cols, ld, count, planes;
+  int rows, cols, ld, count;
   size_t plane() const { return (size_t)rows * ld; }
-  size_t matrix() const { return planes * plane(); }
+  size_t matrix() const { return 2 * plane(); }
 };
 // Rows of planes start on 128-byte lines, so that what a tile takes of one is one line (1030 x 2051 in rows of 2056: 32.8 us for X X^T, now 28.7).
 int pitch_of(int n) { return (n + 63) / 64 * 64; }
-int encode(CUtensorMap* map, const Planes& m, int box_rows, int terms) {
+int encode(CUtensorMap* map, const Planes& m, int box_rows) {
   PFN_encodeTiled enc = get_encode_tiled();
   if (!enc) return fail(B200CP_ERR_NO_DEVICE, "cuTensorMapEncodeTiled entry point not available");
-  const cuuint64_t dim[4] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.planes, (cuuint64_t)m.count},
+  const cuuint64_t dim[4] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, 2, (cuuint64_t)m.count},
                    stride[3] = {(cuuint64_t)m.ld * 2, (cuuint64_t)m.plane() * 2, (cuuint64_t)m.matrix() * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, terms == 3 ? 2u : 1u, 1}, estr[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 2, 1}, estr[4] = {1, 1, 1, 1};
   const CUresult cr = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, m.p, dim, stride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (cr != CUDA_SUCCESS) return fail(B200CP_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)cr);
@@ -1142,10 +1118,10 @@ long long tiles_of(int M, int N, int BN, bool symmetric) {   // of one matrix
 // The tensor maps of a call, each encoded once: by the planes' address and the rows of a box.
 struct Maps {
   std::map<std::pair<const void*, int>, CUtensorMap> all;
-  int get(CUtensorMap* to, const Planes& m, int box_rows, int terms) {
+  int get(CUtensorMap* to, const Planes& m, int box_rows) {
     const auto [at, is_new] = all.try_emplace({m.p, box_rows});
     if (is_new)
-      if (int rc = encode(&at->second, m, box_rows, terms)) return rc;
+      if (int rc = encode(&at->second, m, box_rows)) return rc;
     *to = at->second;
     return B200CP_OK;
   }
@@ -1158,19 +1134,19 @@ struct Product {
   double alpha, beta;
   const Planes* add;
 };
-template <int BN, int TERMS, int CAP>
+template <int BN, int CAP>
 int launch_table(const std::vector<Product>& ps, Maps& maps, int pairs, cudaStream_t st) {
-  using T = Tile<BN, TERMS>;
+  using T = Tile<BN>;
   Problems<CAP> all;
   all.count = 0;
   long long units = 0;
   for (const Product& q : ps) {
     Problem& p = all.p[all.count++];
-    if (int rc = maps.get(&p.L, q.L, q.l_mn ? kStep : 128, TERMS)) return rc;
-    if (int rc = maps.get(&p.R, q.R, q.r_mn ? kStep : BN / 2, TERMS)) return rc;
+    if (int rc = maps.get(&p.L, q.L, q.l_mn ? kStep : 128)) return rc;
+    if (int rc = maps.get(&p.R, q.R, q.r_mn ? kStep : BN / 2)) return rc;
     p.M = q.out.rows;
     p.N = q.out.cols;
-    p.steps = ceil_div(q.K, T::k);
+    p.steps = ceil_div(q.K, kStep);
     p.tiles_m = ceil_div(p.M, 256);
     p.tiles_n = ceil_div(p.N, BN);
     p.per = (int)tiles_of(p.M, p.N, BN, q.symmetric);
@@ -1181,39 +1157,36 @@ int launch_table(const std::vector<Product>& ps, Maps& maps, int pairs, cudaStre
     p.alpha = (float)q.alpha;
     p.beta = (float)q.beta;
     p.add = q.add ? q.add->p : nullptr;
-    p.add_plane = q.add && q.add->planes == 2 ? q.add->plane() : 0;
     p.out = q.out.p;
     p.ld = q.out.ld;
-    p.plane = q.out.planes == 2 ? q.out.plane() : 0;
+    p.plane = q.out.plane();
     p.matrix = q.out.matrix();
     units += (long long)p.per * q.out.count;
   }
   if (units > 0x3fffffff) return fail(B200CP_ERR_UNSUPPORTED, "b200cp_muon_step: the matrices are too large");
   all.units = (int)units;
   all.early = 2 * units <= pairs;
-  const auto kern = newton_kernel<BN, TERMS, CAP>;
-  B200CP_CUDA_OK((allow_smem<newton_kernel<BN, TERMS, CAP>>((int)T::smem)));
+  const auto kern = newton_kernel<BN, CAP>;
+  B200CP_CUDA_OK((allow_smem<newton_kernel<BN, CAP>>((int)T::smem)));
   B200CP_CUDA_OK(launch_kernel(kern, dim3((unsigned)(2 * std::min<long long>(units, pairs))), dim3(T::threads), T::smem, st, true, all));
   B200CP_LAUNCH_OK("newton_kernel");
   return B200CP_OK;
 }
-template <int BN, int TERMS>
+template <int BN>
 int launch_products(const std::vector<Product>& ps, Maps& maps, int pairs, cudaStream_t st) {
-  return ps.size() <= kFewProblems ? launch_table<BN, TERMS, kFewProblems>(ps, maps, pairs, st) : launch_table<BN, TERMS, kProblems>(ps, maps, pairs, st);
+  return ps.size() <= kFewProblems ? launch_table<BN, kFewProblems>(ps, maps, pairs, st) : launch_table<BN, kProblems>(ps, maps, pairs, st);
 }
-// One launch for all, the longest sums first.  Tiles of 256 columns, or of 128 where those fill the pairs of CTAs better: a narrow tile takes 0.55 of a wide one (0.65 with one
-// plane, where the loads count), so 4096 x 4096 goes in seven rounds of narrow ones, not in four of wide ones (279 us a product, and 350); 4096 x 10240 in nine of wide
+// One launch for all, the longest sums first.  Tiles of 256 columns, or of 128 where those fill the pairs of CTAs better: a narrow tile takes 0.55 of a wide
+// one, so 4096 x 4096 goes in seven rounds of narrow ones, not in four of wide ones (279 us a product, and 350); 4096 x 10240 in nine of wide
 // ones, not in 18.
-int products(std::vector<Product> ps, Maps& maps, int terms, const DeviceInfo& di, cudaStream_t st) {
+int products(std::vector<Product> ps, Maps& maps, const DeviceInfo& di, cudaStream_t st) {
   const int pairs = di.sm_count / 2;
   std::stable_sort(ps.begin(), ps.end(), [](const Product& a, const Product& b) { return a.K > b.K; });
   long long tiles[2] = {};
   for (const Product& p : ps)
     for (int i = 0; i < 2; ++i) tiles[i] += tiles_of(p.out.rows, p.out.cols, 128 << i, p.symmetric) * p.out.count;
   const auto rounds = [&](long long n) { return (double)((n + pairs - 1) / pairs); };
-  const bool wide = rounds(tiles[1]) <= (terms == 3 ? 0.55 : 0.65) * rounds(tiles[0]);
-  if (terms == 3) return wide ? launch_products<256, 3>(ps, maps, pairs, st) : launch_products<128, 3>(ps, maps, pairs, st);
-  return wide ? launch_products<256, 1>(ps, maps, pairs, st) : launch_products<128, 1>(ps, maps, pairs, st);
+  return rounds(tiles[1]) <= 0.55 * rounds(tiles[0]) ? launch_products<256>(ps, maps, pairs, st) : launch_products<128>(ps, maps, pairs, st);
 }
 
 // ---- bounds on the singular values, and the scales of the planes that follow ----------------------------------------------------------
@@ -1468,7 +1441,7 @@ struct Large {
   int n, len;
 };
 template <typename P, typename G, int CAP>
-int run_large(const std::vector<Share>& round, const Rates& r, const Plan& plan, int adjust, int terms, char* ws, const DeviceInfo& di, cudaStream_t st) {
+int run_large(const std::vector<Share>& round, const Rates& r, const Plan& plan, int adjust, char* ws, const DeviceInfo& di, cudaStream_t st) {
   Items<CAP> t;
   t.r = r;
   t.count = 0;
@@ -1479,7 +1452,6 @@ int run_large(const std::vector<Share>& round, const Rates& r, const Plan& plan,
   std::vector<Large> ms;
   long long ctas = 0, ctas8 = 0;
   int norm = 0;
-  const int planes = terms == 3 ? 2 : 1;
   for (const Share& q : round) {
     const Shape& s = *q.s;
     const ShareSizes z = share_sizes(s, q.count);
@@ -1488,10 +1460,10 @@ int run_large(const std::vector<Share>& round, const Rates& r, const Plan& plan,
     m.len = std::max(s.rows, s.cols);
     m.wide = s.rows <= s.cols;
     const auto half = [&](size_t at) { return reinterpret_cast<__half*>(ws + at); };
-    m.X = Planes{half(0), s.rows, s.cols, pitch_of(s.cols), q.count, 2};
+    m.X = Planes{half(0), s.rows, s.cols, pitch_of(s.cols), q.count};
     m.Y = m.X;
     m.Y.p = half(z.x);
-    m.A = Planes{half(2 * z.x), m.n, m.n, pitch_of(m.n), q.count, planes};
+    m.A = Planes{half(2 * z.x), m.n, m.n, pitch_of(m.n), q.count};
     m.B = m.A;
     m.B.p = half(2 * z.x + z.a);
     ws += share_bytes(q);
@@ -1532,15 +1504,15 @@ int run_large(const std::vector<Share>& round, const Rates& r, const Plan& plan,
                  sb = room_for(std::max(1e-3, std::fabs(v[1]) * y + std::fabs(v[2]) * y * y)), sn = room_for(plan.bound[step + 1]);
     std::vector<Product> ps;
     for (Large& m : ms) ps.push_back(Product{m.X, m.X, m.A, !m.wide, !m.wide, true, m.len, sa / (sx * sx), 0, nullptr});
-    if (int rc = products(ps, maps, terms, di, st)) return rc;
+    if (int rc = products(ps, maps, di, st)) return rc;
     ps.clear();
     for (Large& m : ms) ps.push_back(Product{m.A, m.A, m.B, false, false, true, m.n, v[2] * sb / (sa * sa), v[1] * sb / sa, &m.A});
-    if (int rc = products(ps, maps, terms, di, st)) return rc;
+    if (int rc = products(ps, maps, di, st)) return rc;
     ps.clear();
     for (Large& m : ms)
       ps.push_back(m.wide ? Product{m.B, m.X, m.Y, false, true, false, m.n, sn / (sb * sx), v[0] * sn / sx, &m.X}
                           : Product{m.X, m.B, m.Y, false, false, false, m.n, sn / (sb * sx), v[0] * sn / sx, &m.X});
-    if (int rc = products(ps, maps, terms, di, st)) return rc;
+    if (int rc = products(ps, maps, di, st)) return rc;
     for (Large& m : ms) std::swap(m.X, m.Y);
     sx = sn;
   }
@@ -1554,17 +1526,14 @@ int run_large(const std::vector<Share>& round, const Rates& r, const Plan& plan,
 }
 
 template <typename P, typename G>
-int run(const Work& w, const Rates& r, const Plan& plan, int adjust, bool copies, char* ws, cudaStream_t st) {
+int run(const Work& w, const Rates& r, const Plan& plan, int adjust, char* ws, cudaStream_t st) {
   DeviceInfo di;
   if (int rc = device_info(&di)) return rc;
   if (int rc = run_small<P, G>(w, r, plan, adjust, ws, di, st)) return rc;
-  // fp32 grade where a result has it: not in a 16-bit parameter, nor in X itself as bfloat16 (whose rounding is eight times what one fp16 operand's is)
-  const bool coarse = !copies && (r.update ? sizeof(P) == 2 : std::is_same<P, __nv_bfloat16>::value);
-  const int terms = coarse ? 1 : 3;
   for (const std::vector<Share>& round : rounds_of(w)) {
     int items = 0;
     for (const Share& s : round) items += s.count;
-    if (int rc = items <= kFewItems ? run_large<P, G, kFewItems>(round, r, plan, adjust, terms, ws, di, st) : run_large<P, G, kItems>(round, r, plan, adjust, terms, ws, di, st))
+    if (int rc = items <= kFewItems ? run_large<P, G, kFewItems>(round, r, plan, adjust, ws, di, st) : run_large<P, G, kItems>(round, r, plan, adjust, ws, di, st))
       return rc;
   }
   return B200CP_OK;
@@ -1588,10 +1557,8 @@ int muon(const char* who, const b200cp_muon_matrix* ms, int count, int ptype, in
   if (int rc = check_muon(who, ms, count, ptype, gtype)) return rc;
   Plan plan;
   if (int rc = plan_of(who, h, &plan)) return rc;
-  bool copies = false;
   for (int i = 0; i < count; ++i) {
     const b200cp_muon_matrix& a = ms[i];
-    copies = copies || a.master;
     if (a.stack && a.rows && a.cols && (!a.param || !a.grad || (update && !a.momentum))) return fail(B200CP_ERR_INVALID_ARG, "%s: null pointer in matrix %d", who, i);
     if (a.master && ptype == B200CP_FLOAT32) return fail(B200CP_ERR_INVALID_ARG, "%s: a float32 parameter has no float32 copy (matrix %d)", who, i);
   }
@@ -1608,7 +1575,7 @@ int muon(const char* who, const b200cp_muon_matrix* ms, int count, int ptype, in
   r.eps = h->eps;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-#define TYPES(P, G) return run<P, G>(w, r, plan, h->adjust, copies, ws, st)
+#define TYPES(P, G) return run<P, G>(w, r, plan, h->adjust, ws, st)
   if (ptype == B200CP_FLOAT32) TYPES(float, float);
   if (ptype == B200CP_BFLOAT16 && gtype == B200CP_BFLOAT16) TYPES(__nv_bfloat16, __nv_bfloat16);
   if (ptype == B200CP_FLOAT16 && gtype == B200CP_FLOAT16) TYPES(__half, __half);

@@ -1,0 +1,32 @@
+"""What the Muon step's products are worth: results of 16 bits are those of float32, rounded once; sums of any length.  Bounds are those
+of test_muon_gpu.py."""
+import pytest
+import torch
+
+from test_muon_gpu import check, defined, matrices
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(40, 100), (64, 64), (65, 65), (300, 66), (257, 513), (640, 129), (3, 70, 90), (104, 6777)], ids=str)
+def test_results_of_16_bits(shape, dtype):
+    """The same values in float32 go through the same operations: the bits are those of its result, rounded."""
+    import paralleltnnlayers_b200 as P
+    X = matrices(*shape, seed=sum(shape)).to(dtype)
+    assert torch.equal(P.orthogonalise(X), P.orthogonalise(X.float()).to(dtype))
+    p, q = torch.zeros_like(X), torch.zeros(shape, device="cuda")
+    P.muon_step([p], [X], [torch.zeros_like(q)], 1.0)
+    P.muon_step([q], [X.float()], [torch.zeros_like(q)], 1.0)
+    assert torch.equal(p, q.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(80, 300001), (200003, 72)], ids=str)
+def test_long_sums(shape, dtype):
+    """An accumulator of the tensor cores holds 256 terms, however many a sum has: what they cut off does not grow with it."""
+    import paralleltnnlayers_b200 as P
+    X = matrices(*shape, seed=4).to(dtype)
+    out = P.orthogonalise(X)
+    check(out, *defined(X))
+    assert torch.equal(out, P.orthogonalise(X.float()).to(dtype))
