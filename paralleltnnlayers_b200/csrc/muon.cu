@@ -9,7 +9,10 @@
 // n <= 64 (factors, adapters): with P = a I + b A + c A^2, X goes to P X and A to P A P, and all of these are polynomials of the first A.  So the steps
 // are taken on n x n matrices, and X is touched twice: for A, and for the product of all P with it.  A has the squares of the singular values, and
 // noise in its small ones grows by a^2 a step, so this half is in 64 bits (half the rate of 32 on this GPU, and next to nothing beside the memory).  Three
-// launches for all such matrices of a call together.
+// launches for all such matrices of a call together.  Not for any number of steps: what is noise in A (1e-16, of either sign) must stay small, since a negative square of
+// a singular value grows without end, and Q, the product of the P, is applied in fp32.  So X is formed anew, and A from it, before Q could pass 2^10 (kMostGrowth): after
+// five steps of a = 3.4445.  (64 x 64 at random, 8 steps: 3e-5 off in one run of steps, 3e-6 in two, fp32 products 4e-6; 16 x 64 of rank one, 20 steps: not a number in one
+// run.)  Runs take three launches each.
 //
 // n > 64: X, A and B = b A + c A^2 are products on the tcgen05 tensor cores.  What is rounded: a value is held as two fp16 numbers (hi + rest, 22 bits)
 // times a power of two that the bound on the singular values gives, so that none overflows, and a product is hi hi + hi lo + lo hi; its sums are fp32, at
@@ -85,7 +88,8 @@ struct SmallEntry {
 };
 struct SmallHead {
   Rates r;
-  int count, steps, coefficients;
+  int count, first_step, steps, coefficients;   // steps of this run, from first_step on
+  int normed;                // X is an earlier run's, not to be divided by its norm
   double *gram, *inverse;
   float* q;
 };
@@ -365,7 +369,7 @@ __device__ __forceinline__ void iterate(const SmallHead& t, const Coefficients& 
     if (tid == 0) trace_sum = s;
   }
   __syncthreads();
-  const double root = sqrt(trace_sum), inverse = 1.0 / (root > t.r.eps || root != root ? root : t.r.eps);
+  const double root = sqrt(trace_sum), inverse = t.normed ? 1.0 : 1.0 / (root > t.r.eps || root != root ? root : t.r.eps);
   for (int i = tid; i < NN; i += kIterateThreads) {
     A[i] = A[i] * inverse * inverse;   // (one after the other: the square of 1 / eps may be infinite, and A zero)
     if (t.steps == 0) Q[i] = i / LD == i % LD ? 1.0 : 0.0;
@@ -373,7 +377,7 @@ __device__ __forceinline__ void iterate(const SmallHead& t, const Coefficients& 
   __syncthreads();
   const auto as_is = [](double v, int, int) { return v; };
   for (int step = 0; step < t.steps; ++step) {
-    const double *v = co.v + (t.coefficients > 1 ? 3 * step : 0), v0 = v[0], v1 = v[1], v2 = v[2];
+    const double *v = co.v + (t.coefficients > 1 ? 3 * (t.first_step + step) : 0), v0 = v[0], v1 = v[1], v2 = v[2];
     double* p = step == 0 ? Q : P;
     symmetric_product<TS, CL, true>(A, A, p, [&](double s, int r, int c) { return fma(v2, s, fma(v1, A[r * LD + c], r == c ? v0 : 0.0)); });
     const bool last = step + 1 == t.steps;
@@ -1206,10 +1210,12 @@ double grown(double bound, const double* v) {   // the largest |a s + b s^3 + c 
   return most;
 }
 double room_for(double bound) { return std::ldexp(1.0, 15 - (int)std::ceil(std::log2(bound))); }   // bound times it is at most 2^15
+constexpr double kMostGrowth = 1024;   // of a direction with a small singular value, in a run of steps on A
 struct Plan {
   int steps, coefficients;
   const double* v;
   double bound[101];
+  int runs, run[101];        // of the small matrices: where each begins, and the end
 };
 int plan_of(const char* who, const b200cp_muon* h, Plan* p) {
   if (h->steps < 0 || h->steps > 100 || (h->steps && !h->coefficients) || (h->coefficient_count != 1 && h->coefficient_count != h->steps))
@@ -1224,6 +1230,18 @@ int plan_of(const char* who, const b200cp_muon* h, Plan* p) {
     if (!(b <= 100.0)) return fail(B200CP_ERR_UNSUPPORTED, "%s: these coefficients may raise a singular value above 100 in step %d", who, s + 1);
     p->bound[s + 1] = std::max(b, 1e-3);
   }
+  p->runs = 0;
+  p->run[0] = 0;
+  double growth = 1;
+  for (int s = 0; s < p->steps; ++s) {
+    const double a = std::max(1.0, std::fabs(p->v[p->coefficients > 1 ? 3 * s : 0]));
+    if (s > p->run[p->runs] && growth * a > kMostGrowth) {
+      p->run[++p->runs] = s;
+      growth = 1;
+    }
+    growth *= a;
+  }
+  p->run[++p->runs] = p->steps;
   return B200CP_OK;
 }
 
@@ -1231,7 +1249,7 @@ int plan_of(const char* who, const b200cp_muon* h, Plan* p) {
 bool small(const b200cp_muon_matrix& a) { return std::min(a.rows, a.cols) <= kSmall; }
 int tile_side(int n) { return n <= 16 ? 1 : n <= 32 ? 2 : 4; }
 struct SmallSizes {
-  size_t doubles = 0, floats = 0;
+  size_t doubles = 0, floats = 0, values = 0;   // of parts of A; of Q; of X between two runs of steps
   int matrices = 0, ctas = 0;
 };
 // What a CTA takes at a time of a matrix's longer side, and how many such turns there are.
@@ -1254,9 +1272,10 @@ void cut_small(const b200cp_muon_matrix& a, long long all, int slots, SmallEntry
   s->matrices += a.stack;
   s->doubles += (size_t)a.stack * e->chunks * kPart[ts];
   s->floats += (size_t)a.stack * n * n;
+  s->values += align_up((size_t)a.stack * a.rows * a.cols, 64);
 }
 size_t small_bytes(const SmallSizes& s) {
-  return align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256) + align_up(s.floats * 4, 256);
+  return align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256) + align_up(s.floats * 4, 256) + s.values * 4;
 }
 // Small matrices of a launch: tensors (of stacks, at most kMostStack matrices) from `at` on, up to a table's size, 2^20 CTAs and 256 MB of parts.
 int next_small(const std::vector<b200cp_muon_matrix>& ms, size_t at, long long all, int slots, SmallTable<kTableSmall>* t, SmallSizes* s) {
@@ -1373,19 +1392,18 @@ float factor_of(int adjust, int rows, int cols) {
   return 1.f;
 }
 
-template <typename P, typename G, int W, int CAP>
-int launch_small(const SmallHead& head, const SmallEntry* e, const Coefficients& co, const SmallSizes& s, int sm_count, cudaStream_t st) {
-  SmallTable<CAP> t;
-  static_cast<SmallHead&>(t) = head;
-  std::copy(e, e + head.count, t.e);
-  int ts = 1;
-  for (int i = 0; i < t.count; ++i) ts = std::max(ts, tile_side(std::min(t.e[i].rows, t.e[i].cols)));
+template <typename G, int W, int CAP>
+int launch_gram(const SmallTable<CAP>& t, const SmallSizes& s, int ts, cudaStream_t st) {
   // (each as much as the widest matrix of the launch needs; the others need less)
-  const int gram = std::max({gram_doubles(1), ts > 1 ? gram_doubles(2) : 0, ts > 2 ? gram_doubles(4) : 0}) * 8, five = 5 * 16 * ts * (16 * ts + 4) * 8,
-            low = std::max({small_apply_floats(1), ts > 1 ? small_apply_floats(2) : 0, ts > 2 ? small_apply_floats(4) : 0}) * 4;
+  const int gram = std::max({gram_doubles(1), ts > 1 ? gram_doubles(2) : 0, ts > 2 ? gram_doubles(4) : 0}) * 8;
   B200CP_CUDA_OK((allow_smem<muon_gram_kernel<G, W, CAP>>(gram)));
   B200CP_CUDA_OK(launch_kernel(muon_gram_kernel<G, W, CAP>, dim3(s.ctas), dim3(256), gram, st, true, t));
   B200CP_LAUNCH_OK("muon_gram_kernel");
+  return B200CP_OK;
+}
+template <int CAP>
+int launch_iterate(const SmallTable<CAP>& t, const Coefficients& co, const SmallSizes& s, int ts, int sm_count, cudaStream_t st) {
+  const int five = 5 * 16 * ts * (16 * ts + 4) * 8;
   int wide = 0;   // (they are the first ones)
   for (int i = 0; i < t.count; ++i) wide += tile_side(std::min(t.e[i].rows, t.e[i].cols)) == 4 ? t.e[i].stack : 0;
   const int shared = ceil_div(s.matrices + (kShare - 1) * wide, kShare) * kShare;
@@ -1404,9 +1422,47 @@ int launch_small(const SmallHead& head, const SmallEntry* e, const Coefficients&
     if (rc) return rc;
   }
   B200CP_LAUNCH_OK("muon_iterate_kernel");
+  return B200CP_OK;
+}
+template <typename P, typename G, int W, int CAP>
+int launch_apply(const SmallTable<CAP>& t, const SmallSizes& s, int ts, cudaStream_t st) {
+  const int low = std::max({small_apply_floats(1), ts > 1 ? small_apply_floats(2) : 0, ts > 2 ? small_apply_floats(4) : 0}) * 4;
   B200CP_CUDA_OK((allow_smem<muon_small_apply_kernel<P, G, W, CAP>>(low)));
   B200CP_CUDA_OK(launch_kernel(muon_small_apply_kernel<P, G, W, CAP>, dim3(s.ctas), dim3(256), low, st, true, t));
   B200CP_LAUNCH_OK("muon_small_apply_kernel");
+  return B200CP_OK;
+}
+// x: where X lies between two runs of steps.
+template <typename P, typename G, int W, int CAP>
+int launch_small(const SmallHead& head, const SmallEntry* e, const Plan& plan, const Coefficients& co, const SmallSizes& s, float* x, int sm_count, cudaStream_t st) {
+  SmallTable<CAP> t;
+  static_cast<SmallHead&>(t) = head;
+  std::copy(e, e + head.count, t.e);
+  int ts = 1;
+  for (int i = 0; i < t.count; ++i) ts = std::max(ts, tile_side(std::min(t.e[i].rows, t.e[i].cols)));
+  for (int run = 0; run < plan.runs; ++run) {
+    const bool first = run == 0, last = run + 1 == plan.runs;
+    t.first_step = plan.run[run];
+    t.steps = plan.run[run + 1] - t.first_step;
+    t.normed = !first;
+    t.r.update = last && head.r.update;
+    float* at = x;
+    for (int i = 0; i < t.count; ++i) {   // (X is replaced in place: a CTA stores the values that it has read)
+      Pointers& to = t.e[i].at;
+      to = e[i].at;
+      if (!first) {
+        to.g = at;
+        to.m = nullptr;
+      }
+      if (!last) to.p = at;
+      at += align_up((size_t)e[i].stack * e[i].rows * e[i].cols, 64);
+    }
+    if (int rc = first ? launch_gram<G, W, CAP>(t, s, ts, st) : launch_gram<float, W, CAP>(t, s, ts, st)) return rc;
+    if (int rc = launch_iterate<CAP>(t, co, s, ts, sm_count, st)) return rc;
+    if (int rc = first ? (last ? launch_apply<P, G, W, CAP>(t, s, ts, st) : launch_apply<float, G, W, CAP>(t, s, ts, st))
+                       : (last ? launch_apply<P, float, W, CAP>(t, s, ts, st) : launch_apply<float, float, W, CAP>(t, s, ts, st)))
+      return rc;
+  }
   return B200CP_OK;
 }
 template <typename P, typename G>
@@ -1419,15 +1475,16 @@ int run_small(const Work& w, const Rates& r, const Plan& plan, int adjust, char*
     t.count = next_small(w.little, at, w.turns, per_sm(w.widest) * di.sm_count, &t, &s);
     at += t.count;
     t.r = r;
-    t.steps = plan.steps;
     t.coefficients = plan.coefficients;
-    t.gram = reinterpret_cast<double*>(ws);
-    t.inverse = reinterpret_cast<double*>(ws + align_up(s.doubles * 8, 256));
-    t.q = reinterpret_cast<float*>(ws + align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256));
+    char* to = ws;
+    t.gram = reinterpret_cast<double*>(to);
+    t.inverse = reinterpret_cast<double*>(to += align_up(s.doubles * 8, 256));
+    t.q = reinterpret_cast<float*>(to += align_up((size_t)s.matrices * 8, 256));
+    float* x = reinterpret_cast<float*>(to += align_up(s.floats * 4, 256));
     for (int i = 0; i < t.count; ++i) t.e[i].scale = factor_of(adjust, t.e[i].rows, t.e[i].cols);
     const bool few = t.count <= kFewSmall;
-    const int rc = w.widest == 1 ? (few ? launch_small<P, G, 1, kFewSmall>(t, t.e, co, s, di.sm_count, st) : launch_small<P, G, 1, kTableSmall>(t, t.e, co, s, di.sm_count, st))
-                                 : (few ? launch_small<P, G, 4, kFewSmall>(t, t.e, co, s, di.sm_count, st) : launch_small<P, G, 4, kTableSmall>(t, t.e, co, s, di.sm_count, st));
+    const int rc = w.widest == 1 ? (few ? launch_small<P, G, 1, kFewSmall>(t, t.e, plan, co, s, x, di.sm_count, st) : launch_small<P, G, 1, kTableSmall>(t, t.e, plan, co, s, x, di.sm_count, st))
+                                 : (few ? launch_small<P, G, 4, kFewSmall>(t, t.e, plan, co, s, x, di.sm_count, st) : launch_small<P, G, 4, kTableSmall>(t, t.e, plan, co, s, x, di.sm_count, st));
     if (rc) return rc;
   }
   return B200CP_OK;
