@@ -8,8 +8,8 @@
 //      longer where the table is large;
 //   2. the sorted places are cut into chunks of equal length, whatever tokens they belong to: a thread adds its columns of a chunk's rows
 //      in fp32 and stores a token's sum when the next one begins.  A token whose places reach over the end of a chunk leaves parts;
-//   3. which are joined in their order.
-// So a token that makes up a tenth of the batch costs what any others do, and no work depends on which tokens there are.
+//   3. which are joined in their order, up to 64 by a CTA, and the sums of 64 by another launch: a token that makes up the whole batch has as many CTAs for its parts
+//      as there are groups of 64 of them.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -231,46 +231,85 @@ __global__ void __launch_bounds__(256, 4) embedding_sums_kernel(const __grid_con
 }
 
 // ---- gradient, 3: tokens of several chunks --------------------------------------------------------------------------------------------
-// grid (chunks, columns / 4096): the token that goes on behind a chunk and did not begin before it.  A thread has four columns.
-constexpr int kJoinCols = 4096;
+// A token that goes on behind its first chunk has parts: that chunk's second one, and the first ones of the chunks that begin with it.  Chunks are taken in groups of 64.
+//   grid (chunks, columns / 4096): what a token has within a group is added up by the CTA of its first chunk there, and kept in that chunk's place; or written, if that is all.
+//   grid (groups, columns / 4096), where there are several: what a token has in the group where it begins and in those behind it.
+// A thread has four columns.  (One CTA for all of a token's parts: 65536 times one token, rows of 64: 1140 us, so 68; of different tokens 74.)
+constexpr int kJoinCols = 4096, kGroup = 64;
+// The places from `first` on, `step` apart and before `end`, at which chunks begin with the token: they are the first ones.  All lanes have the answer.
+__device__ __forceinline__ int begin_with(const Sums& g, uint32_t token, long long first, int step, long long end) {
+  for (int n = 0;; n += 32) {
+    const long long c = first + (long long)(n + (int)(threadIdx.x & 31)) * step;
+    const unsigned not_it = ~__ballot_sync(0xffffffffu, c < end && g.key[c * g.chunk] == token);
+    if (not_it) return n + __ffs(not_it) - 1;
+  }
+}
+// s += a part's four columns, as many as there are.
+__device__ __forceinline__ void add_part(const Sums& g, const float* from, int left, float (&s)[4]) {
+  float v[4] = {};
+  if ((g.D & 3) == 0) {
+    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) v[i] = from[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] += v[i];
+}
 template <typename T>
-__global__ void __launch_bounds__(1024) embedding_join_kernel(const __grid_constant__ Sums g) {
-  grid_dependency_wait();
-  const int c = blockIdx.x, e0 = c * g.chunk;
-  if ((long long)e0 + g.chunk >= g.rows) return;
-  const int e1 = e0 + g.chunk;
-  const uint32_t now = g.key[e1], last = g.key[e1 - 1], before = e0 > 0 ? g.key[e0 - 1] : g.V;
-  if (now >= g.V || last != now || before == now) return;
-  // how many chunks behind this one begin with the token
-  int parts = 0;
-  for (const int lane = threadIdx.x & 31;;) {
-    const long long e = (long long)(c + 1 + parts + lane) * g.chunk;
-    const unsigned not_it = ~__ballot_sync(0xffffffffu, e < g.rows && g.key[e] == now);
-    parts += not_it ? __ffs(not_it) - 1 : 32;
-    if (not_it) break;
-  }
-  const int col = blockIdx.y * kJoinCols + threadIdx.x * 4, left = g.D - col;
-  if (left <= 0) return;
-  const bool whole = (g.D & 3) == 0;
-  float s[4] = {};
-#pragma unroll 4
-  for (int p = 0; p <= parts; ++p) {   // (the first part is this chunk's second, the others are the first ones of their chunks)
-    const float* from = g.parts + ((size_t)(c + p) * 2 + (p == 0)) * g.D + col;
-    float v[4] = {};
-    if (whole) {
-      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < left) v[i] = from[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] += v[i];
-  }
-  T* to = static_cast<T*>(g.dW) + (size_t)now * g.D + col;
+__device__ __forceinline__ void store_row(const Sums& g, uint32_t token, int col, int left, const float (&s)[4]) {
+  T* to = static_cast<T*>(g.dW) + (size_t)token * g.D + col;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (i < left) to[i] = from_float<T>(s[i] * g.scale);
+}
+template <typename T>
+__global__ void __launch_bounds__(1024) embedding_join_kernel(const __grid_constant__ Sums g) {
+  grid_dependency_wait();
+  const int c = blockIdx.x;
+  const long long e0 = (long long)c * g.chunk, e1 = e0 + g.chunk;
+  if (e1 >= g.rows) return;
+  const uint32_t now = g.key[e1];
+  if (now >= g.V || g.key[e1 - 1] != now) return;
+  const bool begun = e0 > 0 && g.key[e0 - 1] == now;   // in an earlier chunk
+  if (begun && c % kGroup) return;
+  const long long next = ((long long)c / kGroup + 1) * kGroup;   // group
+  const int more = begin_with(g, now, c + 1, 1, min(next, (long long)g.chunks));
+  const bool all = !begun && !(next < g.chunks && g.key[next * g.chunk] == now);
+  const int col = blockIdx.y * kJoinCols + threadIdx.x * 4, left = g.D - col;
+  if (left <= 0) return;
+  float s[4] = {};
+  float* place = g.parts + ((size_t)c * 2 + !begun) * g.D + col;
+  add_part(g, place, left, s);
+#pragma unroll 8
+  for (int p = 1; p <= more; ++p) add_part(g, g.parts + (size_t)(c + p) * 2 * g.D + col, left, s);
+  if (all) {
+    store_row<T>(g, now, col, left, s);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < left) place[i] = s[i];
+}
+template <typename T>
+__global__ void __launch_bounds__(1024) embedding_join_groups_kernel(const __grid_constant__ Sums g) {
+  grid_dependency_wait();
+  const long long first = (long long)blockIdx.x * kGroup, next = first + kGroup;
+  if (next >= g.chunks) return;
+  const uint32_t now = g.key[next * g.chunk];
+  if (now >= g.V || g.key[next * g.chunk - 1] != now || (first > 0 && g.key[first * g.chunk - 1] == now)) return;   // (does not reach over the end, or began before)
+  int before = 0;   // chunks of the group that end with other tokens
+#pragma unroll
+  for (int n = 0; n < kGroup; n += 32) before += __popc(__ballot_sync(0xffffffffu, g.key[(first + n + (threadIdx.x & 31) + 1) * g.chunk - 1] != now));
+  const int more = begin_with(g, now, next, kGroup, g.chunks);
+  const int col = blockIdx.y * kJoinCols + threadIdx.x * 4, left = g.D - col;
+  if (left <= 0) return;
+  float s[4] = {};
+  add_part(g, g.parts + ((size_t)(first + before) * 2 + 1) * g.D + col, left, s);
+#pragma unroll 8
+  for (int p = 0; p < more; ++p) add_part(g, g.parts + (size_t)(next + (long long)p * kGroup) * 2 * g.D + col, left, s);
+  store_row<T>(g, now, col, left, s);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
@@ -316,9 +355,13 @@ int sums(Sums g, const Cut& c, cudaStream_t st) {
   B200CP_CUDA_OK(launch_kernel(embedding_sums_kernel<T, VEC>, dim3((unsigned)ceil_div(c.chunks, per), (unsigned)c.slabs), dim3(256), 0, st, true, g));
   B200CP_LAUNCH_OK("embedding_sums_kernel");
   if (c.chunks < 2) return B200CP_OK;
-  B200CP_CUDA_OK(launch_kernel(embedding_join_kernel<T>, dim3((unsigned)c.chunks, (unsigned)ceil_div(g.D, kJoinCols)),
-                               dim3(std::min(1024, (ceil_div(g.D, 4) + 31) / 32 * 32)), 0, st, true, g));
+  const unsigned slabs = (unsigned)ceil_div(g.D, kJoinCols);
+  const dim3 threads(std::min(1024, (ceil_div(g.D, 4) + 31) / 32 * 32));
+  B200CP_CUDA_OK(launch_kernel(embedding_join_kernel<T>, dim3((unsigned)c.chunks, slabs), threads, 0, st, true, g));
   B200CP_LAUNCH_OK("embedding_join_kernel");
+  if (c.chunks <= kGroup) return B200CP_OK;
+  B200CP_CUDA_OK(launch_kernel(embedding_join_groups_kernel<T>, dim3((unsigned)ceil_div(c.chunks, kGroup), slabs), threads, 0, st, true, g));
+  B200CP_LAUNCH_OK("embedding_join_groups_kernel");
   return B200CP_OK;
 }
 
