@@ -458,7 +458,7 @@ int b200cp_embedding(int rows, int V, int D, int type, int number_type, const vo
                      void* stream);
 
 /* dW[v] = scale times the sum of dY[s] over the s with tokens[s] = v; all V rows are written.  Sums are fp32, in the order of s within
- * parts of fixed length: the same bits each time.  The workspace is 16-byte aligned. */
+ * parts whose length goes by rows, D, type and the number of SMs: the same bits each time on GPUs of a model.  The workspace is 16-byte aligned. */
 size_t b200cp_embedding_bwd_workspace_bytes(int rows, int D);
 int b200cp_embedding_bwd(int rows, int V, int D, int type, int number_type, const void* tokens, const void* dY, float scale, void* dW,
                          void* workspace, size_t workspace_bytes, void* stream);
@@ -472,8 +472,9 @@ int b200cp_layer_norm(int rows, int D, int type, int weight_type, const void* X,
                       void* Y, void* H, float* mean, float* rstd, void* stream);
 
 /* dX = rstd (g - mean(g) - n mean(g n)) + dH with g = dY w and n = (H - mean) rstd (the gradient of X, and of R), dw = sum over rows of dY n, db = sum of
- * dY, both of weight_type.  dH (the gradient that came to H itself), w, dX, dw and db may each be NULL.  The sums have a fixed order.  The workspace is
- * 16-byte aligned; it is needed for dw and db. */
+ * dY, both of weight_type.  dH (the gradient that came to H itself), w, dX, dw and db may each be NULL.  The sums have a fixed order, which goes by
+ * rows, D, type, the number of SMs, and whether all arrays lie on 16-byte boundaries (w of floats beside 16-bit rows: 32): the same bits each time for arrays that lie alike.
+ * The workspace is 16-byte aligned; it is needed for dw and db. */
 size_t b200cp_layer_norm_bwd_workspace_bytes(int rows, int D);
 int b200cp_layer_norm_bwd(int rows, int D, int type, int weight_type, const void* dY, const void* dH, const void* H, const void* w,
                           const float* mean, const float* rstd, void* dX, void* dw, void* db, void* workspace, size_t workspace_bytes,

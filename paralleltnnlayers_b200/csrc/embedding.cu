@@ -336,14 +336,19 @@ int lookup(const Lookup& g, cudaStream_t st) {
 }
 // Where the parts of a row's columns, a chunk's length and its parts are
 struct Cut {
-  int vec, lanes, slabs, chunk, chunks;
+  int lanes, slabs, chunk, chunks;
 };
-// (vec: values of a load.)  Chunks are as long as 64 where that leaves four CTAs for each SM, and eight at least: their parts are 8 / chunk of dY's size.
-Cut cut_of(int rows, int D, int vec, int sm_count) {
-  Cut c{vec, 1, 1, 64, 1};
-  while (c.lanes < 256 && c.lanes * vec < D) c.lanes *= 2;
-  c.slabs = (int)((D + (long long)c.lanes * vec - 1) / ((long long)c.lanes * vec));
-  while (c.chunk > 8 && (long long)ceil_div(rows, c.chunk) * c.slabs * c.lanes < 4LL * 256 * sm_count) c.chunk /= 2;
+// Chunks are as long as 64 where that leaves four CTAs for each SM, and eight at least: their parts are 8 / chunk of dY's size.  Their length goes by the loads that
+// the type and the rows' length allow (each), so that sums have one order wherever the arrays lie; vec: the values of a load that their addresses allow too.
+Cut cut_of(int rows, int D, int each, int vec, int sm_count) {
+  const auto lanes = [&](int n) {
+    int l = 1;
+    while (l < 256 && l * n < D) l *= 2;
+    return l;
+  };
+  const auto slabs = [&](int n) { return (int)((D + (long long)lanes(n) * n - 1) / ((long long)lanes(n) * n)); };
+  Cut c{lanes(vec), slabs(vec), 64, 1};
+  while (c.chunk > 8 && (long long)ceil_div(rows, c.chunk) * slabs(each) * lanes(each) < 4LL * 256 * sm_count) c.chunk /= 2;
   c.chunks = ceil_div(rows, c.chunk);
   return c;
 }
@@ -389,8 +394,8 @@ size_t b200cp_embedding_bwd_workspace_bytes(int rows, int D) {
   if (rows < 1 || D < 1) return 0;
   DeviceInfo di;
   if (device_info(&di)) return 0;
-  int chunks = 0;   // (those of the shortest chunk that any alignment gives)
-  for (int vec : {1, 4, 8}) chunks = std::max(chunks, cut_of(rows, D, vec, di.sm_count).chunks);
+  int chunks = 0;   // (those of the shortest chunk that any type gives)
+  for (int each : {1, 4, 8}) chunks = std::max(chunks, cut_of(rows, D, each, 1, di.sm_count).chunks);
   return 4 * keys_bytes(rows) + (size_t)chunks * 2 * (size_t)D * sizeof(float);
 }
 
@@ -443,7 +448,7 @@ int b200cp_embedding_bwd(int rows, int V, int D, int type, int number_type, cons
   return by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const bool vec = rows_of_16<T>(dY, D) && rows_of_16<T>(dW, D);
-    const Cut c = cut_of(rows, D, vec ? kPerLoad<T> : 1, di.sm_count);
+    const Cut c = cut_of(rows, D, D % kPerLoad<T> ? 1 : kPerLoad<T>, vec ? kPerLoad<T> : 1, di.sm_count);
     const int last = (s.passes - 1) & 1;
     Sums g{rows, D, c.chunk, c.chunks, c.lanes, (uint32_t)V, scale, s.key[last], s.place[last], dY, dW, reinterpret_cast<float*>(ws + 4 * kb)};
     return vec ? sums<T, kPerLoad<T>>(g, c, st) : sums<T, 1>(g, c, st);

@@ -58,3 +58,14 @@ def test_time_of_one_token(S, D):
             took.append(a.elapsed_time(b))
         best.append(min(took))
     assert best[1] < 4 * best[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("S,D", [(300, 64), (3000, 8), (3000, 1024), (20000, 264), (1500, 4096), (2000, 513)])
+def test_bits_wherever_the_rows_lie(S, D, dtype):
+    import paralleltnnlayers_b200 as P
+    dY = rows(S, D, dtype)
+    off = torch.cat([dY.reshape(-1)[:1], dY.reshape(-1)])[1:].view(S, D)   # (off the boundary of a load)
+    assert off.data_ptr() % 16 and torch.equal(off, dY)
+    t = torch.randint(7, (S,), generator=torch.Generator().manual_seed(2)).cuda()
+    assert torch.equal(P.embedding_backward(dY, t, 9), P.embedding_backward(off, t, 9))
