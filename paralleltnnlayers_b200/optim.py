@@ -164,6 +164,7 @@ class Muon(torch.optim.Optimizer):
         super().add_param_group(param_group)
         for p in self.param_groups[-1]["params"]:
             if p.dim() < 2:
+                self.param_groups.pop()   # (what is refused is not stepped either)
                 raise ValueError(f"Muon is for matrices, a parameter is {tuple(p.shape)}")
 
     def __setstate__(self, state):
