@@ -280,6 +280,11 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   }
 };
 
+// Where nothing requires a gradient no node is made, and a tangent (forward-mode differentiation) would be lost without a word.
+void no_tangents(const char* who, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), who, ": forward-mode differentiation is not there");
+}
 PyObject* wrap_tuple(const std::vector<Tensor>& ts) {
   PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
   if (!r) throw python_error();
@@ -344,6 +349,7 @@ PYFN(py_adapters_apply) {
                &which = any_tensor(a[4], "adapters");
   int64_t planned = int_arg(a[5]);
   const Tensor scale = optional_tensor(a[6], "scale");
+  no_tangents("DenseAdaptersFunction", {&y, &x, &A, &B, &scale});
   const bool grad = at::GradMode::is_enabled() && (y.requires_grad() || x.requires_grad() || A.requires_grad() || B.requires_grad());
   return wrap(unlocked([&] {
     if (!grad) {   // nothing is kept, and a small batch needs no plan
@@ -643,6 +649,7 @@ PYFN(py_embedding_apply) {
   count_args(n, 3);
   const Tensor &t = any_tensor(a[0], "tokens"), &W = any_tensor(a[1], "W");
   const double scale = float_arg(a[2]);
+  no_tangents("EmbeddingFunction", {&W});
   const bool grad = at::GradMode::is_enabled() && W.requires_grad();
   return wrap(unlocked([&] { return grad ? EmbeddingNode::apply(t, W, scale) : embedding(t, W, scale); }));
   END_HANDLE_TH_ERRORS
@@ -786,6 +793,7 @@ PYFN(py_layer_norm_apply) {
   const Tensor& x = any_tensor(a[0], "X");
   const Tensor w = optional_tensor(a[1], "weight"), b = optional_tensor(a[2], "bias"), r = optional_tensor(a[4], "residual");
   const double eps = float_arg(a[3]);
+  no_tangents("LayerNormFunction", {&x, &w, &b, &r});
   bool grad = x.requires_grad();
   for (const Tensor* t : {&w, &b, &r}) grad = grad || (t->defined() && t->requires_grad());
   grad = grad && at::GradMode::is_enabled();
