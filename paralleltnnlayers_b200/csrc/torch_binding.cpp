@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -417,9 +418,34 @@ FactorGrads dense_backward(const Tensor& U_, const Tensor& dV_, at::TensorList F
 }
 
 // ---- autograd nodes -------------------------------------------------------------------------------------------------------
+// A node's gradients (N::gradients) are computed by kernels, outside of what autograd records: with create_graph they would be constants to whatever is
+// differentiated behind them.  They get an error for a function instead, on every way to what they depend on: the gradients that came, and what the node has
+// saved.  What is handed on as it came stays as it is.
+template <typename N>
+struct OnceNode : torch::autograd::Function<N> {
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const bool again = at::GradMode::is_enabled();
+    variable_list out;
+    {
+      at::AutoGradMode off(false);
+      out = N::gradients(ctx, grads);
+    }
+    if (!again) return out;
+    variable_list from = ctx->get_saved_variables();
+    from.insert(from.end(), grads.begin(), grads.end());
+    if (std::none_of(from.begin(), from.end(), [](const Tensor& t) { return t.defined() && t.requires_grad(); })) return out;
+    const auto error = std::make_shared<torch::autograd::Error>("the gradients of this operator cannot be differentiated again", torch::autograd::collect_next_edges(from));
+    for (Tensor& t : out) {
+      if (!t.defined() || std::any_of(grads.begin(), grads.end(), [&](const Tensor& g) { return t.is_same(g); })) continue;
+      t = t.detach();
+      torch::autograd::create_gradient_edge(t, error);
+    }
+    return out;
+  }
+};
 // `grad`: gradients are recorded where the node is applied (inside a forward the mode is always off; the factors of a
 // module require a gradient under no_grad too, where a rank plane would be written and dropped)
-struct CP4Node : torch::autograd::Function<CP4Node> {
+struct CP4Node : OnceNode<CP4Node> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& FT, const Tensor& FC, const Tensor& FY,
                         const Tensor& FX, int64_t pad, int64_t flags, bool grad) {
     ctx->saved_data["pad"] = pad;
@@ -439,7 +465,7 @@ struct CP4Node : torch::autograd::Function<CP4Node> {
     ctx->save_for_backward({x, FT, FC, FY, FX});
     return cp4_forward(x, FT, FC, FY, FX, pad, (int)flags);
   }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
     const int64_t pad = ctx->saved_data["pad"].toInt();
     const int flags = (int)ctx->saved_data["flags"].toInt();
@@ -464,7 +490,7 @@ struct CP4Node : torch::autograd::Function<CP4Node> {
   }
 };
 
-struct CP3Node : torch::autograd::Function<CP3Node> {
+struct CP3Node : OnceNode<CP3Node> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& KT, const Tensor& KCin, const Tensor& KC,
                         int64_t pad, bool grad) {
     ctx->saved_data["pad"] = pad;
@@ -483,7 +509,7 @@ struct CP3Node : torch::autograd::Function<CP3Node> {
     ctx->save_for_backward({x, KT, KCin, KC});
     return cp3_forward(x, KT, KCin, KC, pad, 0);
   }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
     const int64_t pad = ctx->saved_data["pad"].toInt();
     const Tensor dy = grads[0].contiguous();
@@ -504,14 +530,14 @@ struct CP3Node : torch::autograd::Function<CP3Node> {
   }
 };
 
-struct RCPNode : torch::autograd::Function<RCPNode> {
+struct RCPNode : OnceNode<RCPNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& KC, at::TensorList A) {
     variable_list save{x, KC};
     save.insert(save.end(), A.begin(), A.end());
     ctx->save_for_backward(std::move(save));
     return rcp_forward(x, A, KC, 0);
   }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
     const Tensor& x = v[0];
     const int64_t nd = x.dim();
@@ -523,14 +549,14 @@ struct RCPNode : torch::autograd::Function<RCPNode> {
   }
 };
 
-struct DenseNode : torch::autograd::Function<DenseNode> {
+struct DenseNode : OnceNode<DenseNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, at::TensorList F) {
     variable_list save{x};
     save.insert(save.end(), F.begin(), F.end());
     ctx->save_for_backward(std::move(save));
     return dense_forward(x, F, 0);
   }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
     const Tensor& x = v[0];
     const Tensor dy = grads[0].contiguous().reshape({x.size(0), -1});

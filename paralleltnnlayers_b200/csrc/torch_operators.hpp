@@ -160,7 +160,7 @@ std::array<Tensor, 3> dense_adapters_backward(const Adapters& a, const Tensor& d
                                ws.data_ptr(), (size_t)ws.numel(), stream(a.x)));
   return g;
 }
-struct AdaptersNode : torch::autograd::Function<AdaptersNode> {
+struct AdaptersNode : OnceNode<AdaptersNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& x, const Tensor& A, const Tensor& B, const Tensor& plan,
                         const std::optional<Tensor>& scale_) {
     const Tensor scale = scale_.value_or(Tensor());
@@ -170,7 +170,7 @@ struct AdaptersNode : torch::autograd::Function<AdaptersNode> {
     ctx->save_for_backward({x, A, B, plan, scale, V});
     return out;
   }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
     variable_list out(6);
     if (ctx->needs_input_grad(0)) out[0] = grads[0];
@@ -261,7 +261,7 @@ std::array<Tensor, 3> dense_gated_backward(const Gated& g, const Tensor& G_, con
                             dH.const_data_ptr(), at(d[0]), at(d[1]), at(d[2]), ws.ptr, ws.bytes, stream(g.x)));
   return d;
 }
-struct GatedNode : torch::autograd::Function<GatedNode> {
+struct GatedNode : OnceNode<GatedNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& Wg, const Tensor& Wu, int64_t act, bool grad) {
     const Gated g(x, Wg, Wu, act);
     ctx->saved_data["act"] = act;
@@ -271,7 +271,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     ctx->save_for_backward({x, Wg, Wu, G, U});
     return H;
   }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
     const Gated g(v[0], v[1], v[2], ctx->saved_data["act"].toInt());
     const std::array<Tensor, 3> d =
@@ -614,14 +614,14 @@ Tensor embedding_backward(const Tensor& dy_, const Tensor& tokens_, int64_t coun
   ok(b200cp_embedding_bwd(t.rows, V, D, type, t.wide, t.t.const_data_ptr(), dy.const_data_ptr(), (float)scale, dW.data_ptr(), ws.ptr, ws.bytes, stream(dy)));
   return dW;
 }
-struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
+struct EmbeddingNode : OnceNode<EmbeddingNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& W, double scale) {
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["count"] = W.size(0);
     ctx->save_for_backward({tokens});
     return embedding(tokens, W, scale);
   }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     return {Tensor(), embedding_backward(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["count"].toInt(), ctx->saved_data["scale"].toDouble()), Tensor()};
   }
 };
@@ -732,7 +732,7 @@ std::array<Tensor, 3> layer_norm_backward(const Tensor& dy_, const Tensor& h, co
   return d;
 }
 // Results: Y, or Y and H where there is a residual.
-struct NormNode : torch::autograd::Function<NormNode> {
+struct NormNode : OnceNode<NormNode> {
   using Maybe = std::optional<Tensor>;
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& w_, const Maybe& b_, const Maybe& r_, double eps) {
     const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor()), r = r_.value_or(Tensor());
@@ -743,7 +743,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     if (r.defined()) return {o.y, o.h};
     return {o.y};
   }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
     const bool residual = ctx->saved_data["residual"].toBool();
     // (only inputs that are there have a place in the node)
