@@ -227,18 +227,19 @@ struct Backward {
   void* dx;          // or null
   float* partial;    // [CTA][dw, db][D], or null
 };
-// What a row adds to a thread's sums, and its dh.  n = h rstd - mean rstd in one operation, dh = rstd g - rstd mean(g) - n rstd mean(g n) in two.  Instructions count
+// What a row adds to a thread's sums, and its dh.  n = (h - mean) rstd in two operations (h rstd - mean rstd, in one, rounds mean rstd: rows of one value, whose n is 0, gave
+// what that rounding is, 2 at a value of 12345), dh = rstd g - rstd mean(g) - n rstd mean(g n) in two.  Instructions count
 // here: 8192 x 4096 in bfloat16 with dH (HBM: 41 us) took 69 us with eight features a thread and 350 instructions a row and warp, 63 with these forms and
 // sums of two values at once, and takes 53 with 16 features a thread, which halves what a row costs beside its values (115 with a row ahead in registers).
 template <typename T, int VEC>
-__device__ __forceinline__ void add_group(const Group<T, VEC>& h, const Group<T, VEC>& dy, const float (&w)[VEC], float rstd, float shift, float (&n)[VEC],
+__device__ __forceinline__ void add_group(const Group<T, VEC>& h, const Group<T, VEC>& dy, const float (&w)[VEC], float mean, float rstd, float (&n)[VEC],
                                           float (&e)[VEC], float& s1, float& s2, float (&dw)[VEC], float (&db)[VEC]) {
   float x[VEC], d[VEC];
   unpack(h, x);
   unpack(dy, d);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    n[i] = fmaf(x[i], rstd, shift);
+    n[i] = (x[i] - mean) * rstd;
     e[i] = d[i] * w[i];
     s1 += e[i];
     s2 = fmaf(e[i], n[i], s2);
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRows : kGradThreads, 1) norm_grad
     float s1 = 0.f, s2 = 0.f, x[K][VEC], e[K][VEC];
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if ((k * n + t) * VEC < g.D) add_group(now.h[k], now.dy[k], w[k], now.rstd, -now.mean * now.rstd, x[k], e[k], s1, s2, dw[k], db[k]);
+      if ((k * n + t) * VEC < g.D) add_group(now.h[k], now.dy[k], w[k], now.mean, now.rstd, x[k], e[k], s1, s2, dw[k], db[k]);
     if (!g.dx) continue;
     const float2 q = row_sum<WARP>(s1, s2, red, turn);
     const float c1 = q.x * inv * now.rstd, c2 = q.y * inv * now.rstd;
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) norm_grads_ring_kernel(const 
       const int c = (k * n + t) * VEC;
       if (c >= g.D) continue;
       if (added) dh[k] = load_group<T, VEC>(place + 2 * g.D + c);
-      add_group(load_group<T, VEC>(place + c), load_group<T, VEC>(place + g.D + c), w[k], rs, -mu * rs, x[k], e[k], s1, s2, dw[k], db[k]);
+      add_group(load_group<T, VEC>(place + c), load_group<T, VEC>(place + g.D + c), w[k], mu, rs, x[k], e[k], s1, s2, dw[k], db[k]);
     }
     float2 q = make_float2(0.f, 0.f);
     if (g.dx) q = block_sum(s1, s2, red, turn);
