@@ -58,6 +58,9 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float* red, int turn
   return block_sum(a, b, red, turn);
 }
 
+// (rounding may leave a variance below 0; one that is not a number stays that)
+__device__ __forceinline__ float rstd_of(float variance, float eps) { return 1.f / sqrtf((variance < 0.f ? 0.f : variance) + eps); }
+
 struct Forward {
   int rows, D;
   float eps;
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRows : 1024) norm_kernel(const __
     }
   }
   const float2 q = row_sum<WARP>(s1, s2, red, 1);
-  const float off = q.x * inv, rstd = 1.f / sqrtf(fmaxf(fmaf(-off, off, q.y * inv), 0.f) + g.eps);
+  const float off = q.x * inv, rstd = rstd_of(fmaf(-off, off, q.y * inv), g.eps);
   if (g.mean && t == 0) {
     g.mean[row] = mean + off;
     g.rstd[row] = rstd;
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(1024) norm_wide_kernel(const __grid_constant__
     }
   }
   const float2 q = block_sum(s1, s2, red, 1);
-  const float off = q.x * inv, rstd = 1.f / sqrtf(fmaxf(fmaf(-off, off, q.y * inv), 0.f) + g.eps);
+  const float off = q.x * inv, rstd = rstd_of(fmaf(-off, off, q.y * inv), g.eps);
   if (g.mean && threadIdx.x == 0) {
     g.mean[blockIdx.x] = mean + off;
     g.rstd[blockIdx.x] = rstd;

@@ -1,4 +1,4 @@
-"""Rows whose statistics are at an edge: gradients of rows of one value."""
+"""Rows whose statistics are at an edge: gradients of rows of one value, statistics of rows that are not finite."""
 import pytest
 import torch
 
@@ -23,3 +23,18 @@ def test_gradients_of_rows_of_one_value(D, dtype):
     (_, want, _, sums), (_, bound, _, slack) = defined(x, w, None, 1e-5, dy, None)
     check(dx, want, bound, "dx")
     check(db, sums, slack, "db")
+
+
+@pytest.mark.parametrize("D", [*SIZES, 40000])
+def test_statistics_of_rows_that_are_not_finite(D):
+    import paralleltnnlayers_b200 as P
+    x = torch.randn(5, D, device="cuda")
+    _, m, r = P.layer_norm_save(x)
+    z = x.clone()
+    z[1, D // 2], z[2, 1], z[3] = float("nan"), float("inf"), float("-inf")
+    y, mean, rstd = P.layer_norm_save(z)
+    assert y[1:4].isnan().all() and rstd[1:4].isnan().all() and not mean[1:4].isfinite().any()
+    for k in (0, 4):
+        assert torch.equal(mean[k], m[k]) and torch.equal(rstd[k], r[k])
+    dx, dw, db = P.layer_norm_backward(torch.ones_like(z), z, torch.ones(D, device="cuda"), None, mean, rstd)
+    assert dx[1:4].isnan().all() and dw.isnan().all() and bool((db == 5).all()) and dx[[0, 4]].isfinite().all()
