@@ -453,7 +453,7 @@ int b200cp_dense_gated_bwd(int rows, int I, int F, int type, int activation, con
 /* ---- embedding --------------------------------------------------------------------------------------------------- */
 
 /* out[s] = scale W[t] with t = tokens[s]; zeros where t is outside 0 .. V-1 (padding).  tokens [rows]: int (number_type 0) or long long (1);
- * W [V, D], out [rows, D] of one type.  rows and D are at most 2^30.  No counterpart in the reference: what feeds the dense layers of a language model. */
+ * W [V, D], out [rows, D] of one type.  rows and D are at most 2^30 (D in the gradient: 2^24 - 256).  No counterpart in the reference: what feeds the dense layers of a language model. */
 int b200cp_embedding(int rows, int V, int D, int type, int number_type, const void* tokens, const void* W, float scale, void* out,
                      void* stream);
 
@@ -505,7 +505,7 @@ typedef struct b200cp_muon {
 
 /* m = m + (1 - momentum)(g - m); u = g + momentum (m - g) with nesterov, else m; X = u / max(|u|_F, eps); `steps` times, on the smaller side of the matrix,
  * A = X X^T, X = a X + (b A + c A^2) X; p = p - lr wd p - lr factor X.  In place.  param_type, grad_type: as in b200cp_adamw_step.  Results are fp32-grade (see
- * csrc/muon.cu); coefficients that may raise a singular value above 100 are refused.  No two entries may overlap.  The workspace is
+ * csrc/muon.cu), those of 16 bits rounded once, for up to 100 steps; coefficients that may raise a singular value above 100 are refused.  No two entries may overlap.  The workspace is
  * 256-byte aligned.  Beside b200cp_adamw_step; no counterpart in the reference. */
 size_t b200cp_muon_step_workspace_bytes(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type);
 int b200cp_muon_step(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type, const b200cp_muon* hyper, void* workspace,

@@ -7,10 +7,10 @@
 // the mean's own rounding: no second pass over memory and no difference of large sums.  Rows of up to 256 features belong to a warp, others to a CTA,
 // 8 to 32 features a thread.
 //
-// The gradients are one kernel too: a CTA walks over its rows with the sums of dw and db of its threads' features in registers (8 features a
-// thread, rows of up to 8192); the next rows come by bulk copies into a ring in shared memory meanwhile (rows that do not lie on 16-byte boundaries, and short
-// ones, into registers, one ahead).  The CTAs' sums are added by a second launch in their order, so that a result has the same bits each
-// time.  Longer rows are read twice: for dh and for the sums over rows.  Every wait is bounded: one that runs out sets a status word.
+// The gradients are one kernel too: a CTA walks over its rows with the sums of dw and db of its threads' features in registers (16 features a
+// thread, rows of up to 8192); the next rows come by bulk copies into a ring in shared memory meanwhile (rows that do not lie on 16-byte boundaries, up to 4096, and those of
+// up to 256 features, into registers, one ahead, 8 features a thread).  The CTAs' sums are added by a second launch in their order, so that a result has the same bits each
+// time.  Longer rows are read twice: for dh and for the sums over rows.  Every wait is bounded: one that runs out sets a status word, and leaves what comes behind it unwritten.
 #include <algorithm>
 
 #include "common.cuh"
@@ -233,7 +233,7 @@ struct Backward {
 // What a row adds to a thread's sums, and its dh.  n = (h - mean) rstd in two operations (h rstd - mean rstd, in one, rounds mean rstd: rows of one value, whose n is 0, gave
 // what that rounding is, 2 at a value of 12345), dh = rstd g - rstd mean(g) - n rstd mean(g n) in two.  Instructions count
 // here: 8192 x 4096 in bfloat16 with dH (HBM: 41 us) took 69 us with eight features a thread and 350 instructions a row and warp, 63 with these forms and
-// sums of two values at once, and takes 53 with 16 features a thread, which halves what a row costs beside its values (115 with a row ahead in registers).
+// sums of two values at once, and takes 53 to 55 with 16 features a thread, which halves what a row costs beside its values (115 with a row ahead in registers).
 template <typename T, int VEC>
 __device__ __forceinline__ void add_group(const Group<T, VEC>& h, const Group<T, VEC>& dy, const float (&w)[VEC], float mean, float rstd, float (&n)[VEC],
                                           float (&e)[VEC], float& s1, float& s2, float (&dw)[VEC], float (&db)[VEC]) {

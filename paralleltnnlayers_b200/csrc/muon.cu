@@ -17,8 +17,8 @@
 // n > 64: X, A and B = b A + c A^2 are products on the tcgen05 tensor cores.  What is rounded: a value is held as two fp16 numbers (hi + rest, 22 bits)
 // times a power of two that the bound on the singular values gives, so that none overflows, and a product is hi hi + hi lo + lo hi; its sums are fp32, at
 // most 256 terms in an accumulator (the tensor core cuts sums off: over 4096 terms it loses 3e-5, where fp32 rounding loses 3e-7) and the rest in registers
-// (4096 x 4096 against 64 bits: 5.5e-7 with 64 terms, 6.3e-7 with 128, 1.1e-6 with 256, in 3.85 ms with 128 and 3.66 with 256; fp32 products of a library: 3.6e-6
-// in 34 ms).  a X is added in fp32 (as part of the product, with a I in B, 5 % faster and two to three times as far off).
+// (4096 x 4096 against 64 bits: 5.5e-7 with 64 terms, 6.3e-7 with 128, 1.1e-6 with 256, in 3.85 ms with 128 and 3.66 with 256 in turn, 3.7 to 4.0 in others under
+// the power cap; fp32 products of a library: 3.6e-6 in 34 ms).  a X is added in fp32 (as part of the product, with a I in B, 5 % faster and two to three times as far off).
 // Results of 16 bits are computed the same way and rounded once.  (Products of the hi parts alone are a third of the work, 4096 x 10240 in bfloat16 2.7 ms where these take
 // 7.6, but leave X 1e-3 off: a rounding that no caller has asked for, and more than that of fp16 itself.)
 // A and B are symmetric: blocks below the diagonal are not computed, the others stored twice.  Either operand is taken in either order, so nothing is

@@ -555,7 +555,8 @@ def orthogonalise(X, coefficients=NEWTON_SCHULZ, eps=1e-7, steps=5):
 
 
 # ---- autograd wrappers ----------------------------------------------------------
-# The nodes are native (csrc/torch_binding.cpp); each class keeps the ``apply`` its layer calls.
+# The nodes are native (csrc/torch_binding.cpp); each class keeps the ``apply`` its layer calls.  Gradients are of the first order: differentiating them again
+# (``create_graph=True``) and forward-mode differentiation are errors.
 class CP4Conv2dFunction:
     """y = CP4 conv2d(x; FT, FC, FY, FX) with the fused backward kernels: ``apply(x, FT, FC, FY, FX, pad=1, flags=0)``."""
     apply = staticmethod(_C.cp4_apply)

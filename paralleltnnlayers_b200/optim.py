@@ -1,6 +1,7 @@
 """Optimisers over the fused AdamW and Muon steps: what applies the gradients of the layers and of the data-parallel steps.
 
-A network of factored layers has many small parameters (four factors per convolution); all of them are updated by one launch (three for Muon).
+A network of factored layers has many small parameters (four factors per convolution); all of them are updated by one launch (three for
+Muon, and 18 more where a matrix has both sides above 64).
 """
 from __future__ import annotations
 
