@@ -506,8 +506,10 @@ typedef struct b200cp_muon {
 /* m = m + (1 - momentum)(g - m); u = g + momentum (m - g) with nesterov, else m; X = u / max(|u|_F, eps); `steps` times, on the smaller side of the matrix,
  * A = X X^T, X = a X + (b A + c A^2) X; p = p - lr wd p - lr factor X.  In place.  param_type, grad_type: as in b200cp_adamw_step.  Results are fp32-grade (see
  * csrc/muon.cu), those of 16 bits rounded once, for up to 100 steps; coefficients that may raise a singular value above 100 are refused.  No two entries may overlap.  The workspace is
- * 256-byte aligned.  Beside b200cp_adamw_step; no counterpart in the reference. */
+ * 256-byte aligned; the first size below is enough for any hyper, the second one for this one (matrices with a side of at most 64 take four bytes a value less where the first coefficients |a| of
+ * all steps multiply to at most 1024, as those of five usual ones do).  Beside b200cp_adamw_step; no counterpart in the reference. */
 size_t b200cp_muon_step_workspace_bytes(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type);
+size_t b200cp_muon_workspace_bytes(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type, const b200cp_muon* hyper);
 int b200cp_muon_step(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type, const b200cp_muon* hyper, void* workspace,
                      size_t workspace_bytes, void* stream);
 

@@ -119,6 +119,7 @@ def _load():
         "b200cp_layer_norm_bwd_workspace_bytes": (sz, [i, i]),
         "b200cp_layer_norm_bwd": (i, [i, i, i, i, vp, vp, vp, vp, fp, fp, vp, vp, vp, vp, sz, vp]),
         "b200cp_muon_step_workspace_bytes": (sz, [vp, i, i, i]),
+        "b200cp_muon_workspace_bytes": (sz, [vp, i, i, i, vp]),
         "b200cp_muon_step": (i, [vp, i, i, i, vp, vp, sz, vp]),
         "b200cp_orthogonalise": (i, [i, i, i, i, vp, vp, C.POINTER(C.c_double), i, i, C.c_double, vp, sz, vp]),
         "b200cp_device_status": (i, []),

@@ -1279,8 +1279,8 @@ void cut_small(const b200cp_muon_matrix& a, long long all, int slots, SmallEntry
   s->floats += (size_t)a.stack * n * n;
   s->values += align_up((size_t)a.stack * a.rows * a.cols, 64);
 }
-size_t small_bytes(const SmallSizes& s) {
-  return align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256) + align_up(s.floats * 4, 256) + s.values * 4;
+size_t small_bytes(const SmallSizes& s, bool several_runs) {
+  return align_up(s.doubles * 8, 256) + align_up((size_t)s.matrices * 8, 256) + align_up(s.floats * 4, 256) + (several_runs ? s.values * 4 : 0);
 }
 // Small matrices of a launch: tensors (of stacks, at most kMostStack matrices) from `at` on, up to a table's size, 2^20 CTAs and 256 MB of parts.
 int next_small(const std::vector<b200cp_muon_matrix>& ms, size_t at, long long all, int slots, SmallTable<kTableSmall>* t, SmallSizes* s) {
@@ -1381,12 +1381,12 @@ size_t round_bytes(const std::vector<Share>& round) {
   for (const Share& s : round) n += share_bytes(s);
   return n;
 }
-size_t workspace_of(const Work& w, int sm_count) {
+size_t workspace_of(const Work& w, int sm_count, bool several_runs) {
   size_t most = 0;
   for (size_t at = 0; at < w.little.size();) {
     SmallSizes s;
     at += next_small(w.little, at, w.turns, per_sm(w.widest) * sm_count, nullptr, &s);
-    most = std::max(most, small_bytes(s));
+    most = std::max(most, small_bytes(s, several_runs));
   }
   for (const std::vector<Share>& r : rounds_of(w)) most = std::max(most, round_bytes(r));
   return most;
@@ -1626,7 +1626,9 @@ int muon(const char* who, const b200cp_muon_matrix* ms, int count, int ptype, in
   }
   const Work w(ms, count, ptype, gtype);
   if (w.little.empty() && w.large.empty()) return B200CP_OK;
-  const size_t need = b200cp_muon_step_workspace_bytes(ms, count, ptype, gtype);
+  DeviceInfo di;
+  if (int rc = device_info(&di)) return rc;
+  const size_t need = workspace_of(w, di.sm_count, plan.runs > 1);
   if (need && (!workspace || bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return fail(B200CP_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, %zu given", who, need, bytes);
   Rates r{};
@@ -1667,9 +1669,20 @@ size_t b200cp_muon_step_workspace_bytes(const b200cp_muon_matrix* matrices, int 
   if (check_muon("b200cp_muon_step_workspace_bytes", matrices, count, param_type, grad_type)) return 0;
   DeviceInfo di;
   if (device_info(&di)) return 0;
-  return workspace_of(Work(matrices, count, param_type, grad_type), di.sm_count);
+  return workspace_of(Work(matrices, count, param_type, grad_type), di.sm_count, true);
 } catch (const std::exception& e) {
   fail(B200CP_ERR_UNSUPPORTED, "b200cp_muon_step_workspace_bytes: %s", e.what());
+  return 0;
+}
+
+size_t b200cp_muon_workspace_bytes(const b200cp_muon_matrix* matrices, int count, int param_type, int grad_type, const b200cp_muon* hyper) try {
+  const char* who = "b200cp_muon_workspace_bytes";
+  Plan plan;
+  DeviceInfo di;
+  if (!hyper || check_muon(who, matrices, count, param_type, grad_type) || plan_of(who, hyper, &plan) || device_info(&di)) return 0;
+  return workspace_of(Work(matrices, count, param_type, grad_type), di.sm_count, plan.runs > 1);
+} catch (const std::exception& e) {
+  fail(B200CP_ERR_UNSUPPORTED, "b200cp_muon_workspace_bytes: %s", e.what());
   return 0;
 }
 

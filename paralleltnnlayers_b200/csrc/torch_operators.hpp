@@ -903,7 +903,7 @@ PYFN(py_muon_step) {
   TORCH_CHECK_VALUE(!b200cp::spans_meet(kinds, used), "muon_step: a tensor occurs twice in what is updated, or shares memory with another one");
   if (lr) h.device_lr = static_cast<const float*>(lr->const_data_ptr());
   void* st = stream(p[0]);
-  const Scratch ws(b200cp_muon_step_workspace_bytes(ms.data(), (int)count, type, gtype), p[0]);
+  const Scratch ws(b200cp_muon_workspace_bytes(ms.data(), (int)count, type, gtype, &h), p[0]);
   unlocked([&] { ok(b200cp_muon_step(ms.data(), (int)count, type, gtype, &h, ws.ptr, ws.bytes, st)); });
   for (size_t i = 0; i < count; ++i) {
     written(p[i]);
@@ -930,7 +930,12 @@ PYFN(py_orthogonalise) {
     const int rows = size_arg(x.size(-2), "the number of rows"), cols = size_arg(x.size(-1), "the number of columns");
     const int stack = x.numel() ? size_arg(x.numel() / ((int64_t)rows * cols), "the number of matrices") : 0;
     const b200cp_muon_matrix m{nullptr, nullptr, nullptr, nullptr, stack, rows, cols};
-    const Scratch ws(b200cp_muon_step_workspace_bytes(&m, 1, type, type), x);
+    b200cp_muon h{};   // (what the size goes by)
+    h.eps = eps;
+    h.steps = steps;
+    h.coefficients = co.v.data();
+    h.coefficient_count = co.count;
+    const Scratch ws(b200cp_muon_workspace_bytes(&m, 1, type, type, &h), x);
     ok(b200cp_orthogonalise(stack, rows, cols, type, x.const_data_ptr(), out.data_ptr(), co.v.data(), co.count, steps, eps, ws.ptr, ws.bytes, stream(x)));
     return out;
   }));

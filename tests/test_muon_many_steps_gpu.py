@@ -82,3 +82,33 @@ def test_a_step_of_several_runs(dtype, master):
         assert bool(((got.double() - want).abs() <= e + torch.finfo(got.dtype).eps / 2 * (want.abs() + e) + 2.0 ** -25).all())
         if master:
             assert torch.equal(a, copy.to(dtype))
+
+
+def test_workspaces():
+    """The size for any step is enough for every one; that of a step is what it needs, and X between two runs of steps is in it only where there are two."""
+    import ctypes as C
+
+    import paralleltnnlayers_b200 as P
+
+    from paralleltnnlayers_b200 import _lib
+    from test_training_operators_refusals import Hyper, Matrix
+    lib = _lib.lib
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    shapes = [(40, 16, 300), (1, 64, 2000), (1, 700, 9)]
+    g = [torch.randn(*s, generator=gen, device="cuda") for s in shapes]
+    abc = (C.c_double * 3)(3.4445, -4.7750, 2.0315)
+    values = sum(t.numel() for t in g)
+    for steps in (5, 6, 20):
+        h = Hyper(lr=1.0, momentum=0.0, wd=0.0, eps=1e-7, nesterov=0, steps=steps, adjust=0, count=1, coefficients=abc)
+        p, m = [torch.zeros_like(t) for t in g], [torch.zeros_like(t) for t in g]
+        ms = (Matrix * 3)(*[Matrix(a.data_ptr(), b.data_ptr(), c.data_ptr(), None, *s) for a, b, c, s in zip(p, g, m, shapes)])
+        any_step, this = lib.b200cp_muon_step_workspace_bytes(ms, 3, 0, 0), lib.b200cp_muon_workspace_bytes(ms, 3, 0, 0, C.byref(h))
+        assert any_step >= this and (any_step - this >= 4 * values) == (steps == 5)
+        ws = torch.empty(this + 256, dtype=torch.uint8, device="cuda")
+        at = (ws.data_ptr() + 255) // 256 * 256
+        stream = torch.cuda.current_stream().cuda_stream
+        assert lib.b200cp_muon_step(ms, 3, 0, 0, C.byref(h), at, this - 1, stream) != 0 and not any(t.any() for t in m)
+        assert lib.b200cp_muon_step(ms, 3, 0, 0, C.byref(h), at, this, stream) == 0
+        for a, b in zip(p, g):
+            assert torch.equal(-a, P.orthogonalise(b, steps=steps))
+    assert lib.b200cp_muon_workspace_bytes(ms, 3, 0, 0, None) == 0
